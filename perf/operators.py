@@ -117,7 +117,7 @@ def _cache_bytes(nkv, cap):
     nblk = -(-cap // BLK)
     up = lambda n: (n + 255) // 256 * 256  # noqa: E731
     codes, scales = nkv * nblk * 2 * BLK * HD, up(nkv * nblk * 8)
-    tail, state = nkv * 2 * BLK * HD * 4, up(nkv * 16)
+    tail, state = nkv * 2 * BLK * HD * 4, up(nkv * 8)
     return nblk, (codes, codes + scales, codes + scales + tail, codes + scales + tail + state)
 
 
@@ -136,8 +136,7 @@ def _arranged(kc, vc, ks, vs, tail, n, cap):
     sc = buf[o_s:o_s + nkv * nblk * 8].view(torch.float32).view(nkv, nblk, 2)
     sc[:, :nb, 0], sc[:, :nb, 1] = ks, vs
     buf[o_t:o_l].view(torch.float32).view(nkv, 2, BLK, HD).copy_(tail)
-    state = buf[o_l:o_l + nkv * 16].view(torch.int32).view(nkv, 2, 2)
-    state[..., 0], state[..., 1] = n, max(n - 1, 0) // BLK
+    buf[o_l:o_l + nkv * 8].view(torch.int32).fill_(n)
     return buf
 
 
@@ -175,9 +174,6 @@ def prepare(case, seed):
         none = torch.zeros(nkv, 0, BLK, HD, dtype=torch.int8, device="cuda")
         flat = torch.zeros(nkv, 0, device="cuda")
         s["kv"] = _arranged(none, none, flat, flat, tail, pos0, s["cap"])
-        _, (_, _, o_l, _) = _cache_bytes(nkv, s["cap"])
-        state = s["kv"][o_l:o_l + nkv * 16].view(torch.int32).view(nkv, 2, 2)
-        state[..., 1] = first // BLK
         s["pos"] = torch.tensor([pos0], dtype=torch.int32, device="cuda")
         s["out"] = [torch.zeros(pos0 - first + ntok, nkv, HD, device="cuda") for _ in range(2)]
         return s
