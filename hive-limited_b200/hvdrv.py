@@ -90,6 +90,16 @@ _SIGS = {
     "hv_attn_decode": [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP],
     "hv_kv_append_f16": [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _VP],
     "hv_attn_decode_f16": [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP],
+    "hv_kv_q8_size": [_I, _I, _I, C.POINTER(_SZ)],
+    "hv_kv_append_q8": [_VP, _VP, _VP, _VP, _I, _I, _I, _VP],
+    "hv_kv_rows_q8": [_VP, _VP, _I, _VP, _I, _I, _I, _I, _I, _VP],
+    "hv_qk_rows_q8": [_VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _I, _I, _I, _I, _F, _I, _VP],
+    "hv_kv_read_q8": [_VP, _VP, _VP, _I, _I, _I, _I, _I, _VP],
+    "hv_attn_q8_scratch": [_I, _I, _I, _I, C.POINTER(_SZ)],
+    "hv_attn_decode_q8": [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _VP],
+    "hv_attn_rows_q8": [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP, _VP],
+    "hv_logprob_scratch": [_I, _I, _I, C.POINTER(_SZ)],
+    "hv_logprob_rows": [_VP, C.c_longlong, _I, _I, _VP, _I, _VP, _VP, _VP, _VP, _VP, _VP],
     "hv_attn_reserve": [_I, _I, _I],
     "hv_attn_decode_noalloc": [_VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP],
     "hv_silu_mul": [_VP, _VP, _VP, _I, _VP],
@@ -601,6 +611,70 @@ def attn_rows(q, kc, vc, ctx, scale, pos0, nq, hd, group, kvstride, ntok, part, 
     _call("hv_attn_rows_f16" if f16 else "hv_attn_rows", _p(q), _p(kc), _p(vc), _p(ctx),
           _p(scale), int(pos0), nq, hd, group, kvstride, ntok, _p(part), _p(ticket),
           _p(stream))
+
+
+def kv_q8_size(nkv, hd, cap) -> int:
+    """Bytes of one layer's 8-bit K and V cache (hv_kv_q8_size); zeroed, it is empty."""
+    n = C.c_size_t()
+    _call("hv_kv_q8_size", nkv, hd, cap, C.byref(n))
+    return n.value
+
+
+def kv_append_q8(k, v, kv, pos, nkv, hd, cap, stream=0):
+    """One row per kv head at the device position *pos of an 8-bit cache."""
+    _call("hv_kv_append_q8", _p(k), _p(v), _p(kv), _p(pos), nkv, hd, cap, _p(stream))
+
+
+def kv_rows_q8(k, v, ld, kv, pos0, nkv, hd, cap, ntok, stream=0):
+    """ntok rows at pos0 of an 8-bit cache; row t of k and v at t * ld floats."""
+    _call("hv_kv_rows_q8", _p(k), _p(v), int(ld), _p(kv), int(pos0), nkv, hd, cap, ntok,
+          _p(stream))
+
+
+def qk_rows_q8(qkv, qn, kn, cos_t, sin_t, pos0, q_out, kv, nq, nkv, hd, cap, eps, ntok,
+               stream=0):
+    """qk_rows (head norms, RoPE, append) over an 8-bit cache."""
+    _call("hv_qk_rows_q8", _p(qkv), _p(qn), _p(kn), _p(cos_t), _p(sin_t), int(pos0), _p(q_out),
+          _p(kv), nq, nkv, hd, cap, C.c_float(eps), ntok, _p(stream))
+
+
+def kv_read_q8(kv, k_out, v_out, pos0, nkv, hd, cap, ntok, stream=0):
+    """Positions pos0 .. pos0 + ntok - 1 of an 8-bit cache as f32 rows [ntok][nkv][hd]."""
+    _call("hv_kv_read_q8", _p(kv), _p(k_out), _p(v_out), int(pos0), nkv, hd, cap, ntok,
+          _p(stream))
+
+
+def attn_q8_scratch(nq, group, cap, ntok=1) -> int:
+    """Bytes of the scratch of attn_decode_q8 (ntok = 1) and attn_rows_q8; zero it once."""
+    n = C.c_size_t()
+    _call("hv_attn_q8_scratch", nq, group, cap, ntok, C.byref(n))
+    return n.value
+
+
+def attn_decode_q8(q, kv, ctx, scale, pos, nq, hd, group, cap, scratch, stream=0):
+    """Decode attention over positions 0 .. *pos of an 8-bit cache."""
+    _call("hv_attn_decode_q8", _p(q), _p(kv), _p(ctx), _p(scale), _p(pos), nq, hd, group, cap,
+          _p(scratch), _p(stream))
+
+
+def attn_rows_q8(q, kv, ctx, scale, pos0, nq, hd, group, cap, ntok, scratch, stream=0):
+    """Attention of ntok query rows over an 8-bit cache, row t over positions 0 .. pos0 + t."""
+    _call("hv_attn_rows_q8", _p(q), _p(kv), _p(ctx), _p(scale), int(pos0), nq, hd, group, cap,
+          ntok, _p(scratch), _p(stream))
+
+
+def logprob_scratch(rows, n, top=0) -> int:
+    """Bytes of logprob_rows's scratch; zero it once."""
+    b = C.c_size_t()
+    _call("hv_logprob_scratch", rows, n, top, C.byref(b))
+    return b.value
+
+
+def logprob_rows(logits, ld, rows, n, tok, top, lp, ent, top_id, top_lp, scratch, stream=0):
+    """Log probabilities of given tokens, entropies and the `top` most likely tokens of rows
+    of logits (hv_logprob_rows)."""
+    _call("hv_logprob_rows", _p(logits), int(ld), rows, n, _p(tok), top, _p(lp), _p(ent),
+          _p(top_id), _p(top_lp), _p(scratch), _p(stream))
 
 
 def silu_rows(gu, act, ffn, ntok, stream=0):

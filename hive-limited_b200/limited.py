@@ -147,8 +147,18 @@ class Engine:
                            per step). Each k/v row is rounded to nearest-even binary16 when
                            appended and attention reads the widened values; the results
                            then follow the oracle run with that rounding, not the
-                           reference's fp32 cache.
+                           reference's fp32 cache; "q8": int8 codes with an f32 scale per
+                           kv head and block of 32 positions (about a quarter of the KV
+                           bytes; hv_kv_q8_size), attention in f32 precision in its own
+                           order. The q8 lane runs the eager sequence (fused=False), with
+                           either prefill, and has no limit on max_context from the
+                           reference-order attention. Its batched prefill reads the rows of
+                           a block that the same run completed quantised, where the
+                           token-by-token prefill still read them in f32.
     """
+
+    kv_q8 = False
+    _sc = None
 
     def __init__(self, model_dir=None, kernels_dir=None, verify_kernels=True, quiet=False, *,
                  config=None, tensors=None, max_context=None, device=0, fused=True,
@@ -170,10 +180,13 @@ class Engine:
         if prefill == "batched" and self.world > 1:
             raise ValueError("the batched prefill runs on one GPU (world = 1)")
         self.prefill_mode = prefill
-        if kv_dtype not in ("f32", "f16"):
-            raise ValueError(f"kv_dtype={kv_dtype!r}: 'f32' or 'f16'")
+        if kv_dtype not in ("f32", "f16", "q8"):
+            raise ValueError(f"kv_dtype={kv_dtype!r}: 'f32', 'f16' or 'q8'")
+        if kv_dtype == "q8" and self.fused:
+            raise ValueError("kv_dtype='q8' runs the eager sequence: pass fused=False")
         self.kv_dtype = kv_dtype
         self.kv_f16 = kv_dtype == "f16"
+        self.kv_q8 = kv_dtype == "q8"
         if gemv_layout not in ("pp", "dq"):
             raise ValueError(f"gemv_layout={gemv_layout!r}: 'pp' or 'dq'")
         self.gemv_layout = gemv_layout
@@ -414,13 +427,20 @@ class Engine:
         self.d_logits = self._alloc(self.n_head_rows * 4)
         self.d_a8 = self._alloc(wide)
         self.d_sa = self._alloc(2 * (wide // BLOCK) * 4)
-        # KV cache: f32 (or binary16), one allocation, [layer][k|v][n_kv][cap][hd]
-        esz = 2 if self.kv_f16 else 4
-        self.kv_bytes = 2 * c.n_layer * nkv * cap * qd * esz
-        self.d_kv = self._alloc(self.kv_bytes)
-        per = nkv * cap * qd * esz
-        self.KC = [self.d_kv + (2 * l) * per for l in range(c.n_layer)]
-        self.VC = [self.d_kv + (2 * l + 1) * per for l in range(c.n_layer)]
+        if self.kv_q8:
+            # one buffer per layer with K and V (hv_kv_q8_size); zeroed = empty
+            per = hvdrv.kv_q8_size(nkv, qd, cap)
+            self.kv_bytes = c.n_layer * per
+            self.d_kv = self._alloc(self.kv_bytes)
+            self.KC = self.VC = [self.d_kv + l * per for l in range(c.n_layer)]
+        else:
+            # KV cache: f32 (or binary16), one allocation, [layer][k|v][n_kv][cap][hd]
+            esz = 2 if self.kv_f16 else 4
+            self.kv_bytes = 2 * c.n_layer * nkv * cap * qd * esz
+            self.d_kv = self._alloc(self.kv_bytes)
+            per = nkv * cap * qd * esz
+            self.KC = [self.d_kv + (2 * l) * per for l in range(c.n_layer)]
+            self.VC = [self.d_kv + (2 * l + 1) * per for l in range(c.n_layer)]
         hvdrv.memset8(self.d_kv, 0, self.kv_bytes)
         half = qd // 2
         pos = np.arange(cap, dtype=np.float64)[:, None]
@@ -436,6 +456,11 @@ class Engine:
         self.d_pv = self._alloc(ARGMAX_PARTS * 4)
         self.d_pi = self._alloc(ARGMAX_PARTS * 4)
         self.d_gen = self._alloc((cap + 1) * 4)
+        if self.kv_q8:
+            n = hvdrv.attn_q8_scratch(nq, c.group, cap)
+            self.d_q8scr = self._alloc(n)
+            hvdrv.memset8(self.d_q8scr, 0, n)
+            return                         # no fused step over this cache
         hvdrv.attn_reserve(nkv, c.group, cap)
         self._build_desc()
 
@@ -548,10 +573,15 @@ class Engine:
             hvdrv.rmsnorm(dk, dk, w["kn"], nkv, qd, RMS_EPS, s)
             hvdrv.rope(dq, self.d_cos, self.d_sin, self.d_pos, nq, qd // 2, s)
             hvdrv.rope(dk, self.d_cos, self.d_sin, self.d_pos, nkv, qd // 2, s)
-            hvdrv.kv_append(dk, dv, self.KC[l], self.VC[l], self.d_pos, nkv, qd, cap, s,
-                            f16=self.kv_f16)
-            hvdrv.attn_decode(dq, self.KC[l], self.VC[l], self.d_ctx, self.d_scale,
-                              self.d_pos, nq, qd, c.group, cap * qd, s, f16=self.kv_f16)
+            if self.kv_q8:
+                hvdrv.kv_append_q8(dk, dv, self.KC[l], self.d_pos, nkv, qd, cap, s)
+                hvdrv.attn_decode_q8(dq, self.KC[l], self.d_ctx, self.d_scale, self.d_pos, nq,
+                                     qd, c.group, cap, self.d_q8scr, s)
+            else:
+                hvdrv.kv_append(dk, dv, self.KC[l], self.VC[l], self.d_pos, nkv, qd, cap, s,
+                                f16=self.kv_f16)
+                hvdrv.attn_decode(dq, self.KC[l], self.VC[l], self.d_ctx, self.d_scale,
+                                  self.d_pos, nq, qd, c.group, cap * qd, s, f16=self.kv_f16)
             self._gemv(self.d_ctx, w["o"], self.d_o)
             hvdrv.vadd(self.d_h, self.d_o, self.d_h, hid, s)
             hvdrv.rmsnorm(self.d_h, self.d_hn, w["fn"], 1, hid, RMS_EPS, s)
@@ -734,7 +764,10 @@ class Engine:
         b, hid, ffn, qd, nq, nkv = (self.PREFILL_BATCH, c.hidden, c.ffn, c.head_dim, c.n_head,
                                     c.n_kv)
         wide = max(hid, ffn, nq * qd)
-        part_b, ticket_b = hvdrv.attn_rows_scratch(nq, c.group, c.max_context, b)
+        if self.kv_q8:
+            part_b, ticket_b = hvdrv.attn_q8_scratch(nq, c.group, c.max_context, b), 4
+        else:
+            part_b, ticket_b = hvdrv.attn_rows_scratch(nq, c.group, c.max_context, b)
         pf = {"n": b, "tok": self._alloc(b * 4), "h": self._alloc(b * hid * 4),
               "hn": self._alloc(b * hid * 4), "a8": self._alloc(b * wide),
               "sa": self._alloc(b * 2 * (wide // BLOCK) * 4),
@@ -743,6 +776,8 @@ class Engine:
               "gu": self._alloc(b * 2 * ffn * 4), "act": self._alloc(b * ffn * 4),
               "part": self._alloc(part_b), "ticket": self._alloc(ticket_b)}
         hvdrv.memset8(pf["ticket"], 0, ticket_b)
+        if self.kv_q8:
+            hvdrv.memset8(pf["part"], 0, part_b)
         self._pf = pf
         return pf
 
@@ -754,6 +789,41 @@ class Engine:
         gemm = hvdrv.a4gemm_dq if self.gemv_layout == "dq" else hvdrv.a4gemm_pp
         gemm(pf["a8"], pf["sa"], pb4, psw, dst, k // 8, n, pair, m, s)
 
+    def _prefill_run(self, toks: np.ndarray, b0: int):
+        """toks (at most PREFILL_BATCH) at positions b0 .. through every layer: their K and V
+        rows into the cache, their final hidden rows (before the last norm) into the
+        buffers' "h"."""
+        c = self.cfg
+        hid, ffn, qd, nq, nkv, cap = (c.hidden, c.ffn, c.head_dim, c.n_head, c.n_kv,
+                                      c.max_context)
+        pf, m = self._pf, toks.size
+        s = self._stream_cur
+        hvdrv.synchronize()                 # the host copy below reuses pf["tok"]
+        hvdrv.upload(pf["tok"], toks.ctypes.data, 4 * m)
+        hvdrv.gather_rows(self.d_emb16, pf["tok"], pf["h"], hid, m, s)
+        for l, w in enumerate(self.layers):
+            hvdrv.rmsnorm(pf["h"], pf["hn"], w["an"], m, hid, RMS_EPS, s)
+            self._gemm(pf["hn"], w["qkv"], pf["qkv"], m)
+            if self.kv_q8:
+                hvdrv.qk_rows_q8(pf["qkv"], w["qn"], w["kn"], self.d_cos, self.d_sin, b0,
+                                 pf["q"], self.KC[l], nq, nkv, qd, cap, RMS_EPS, m, s)
+                hvdrv.attn_rows_q8(pf["q"], self.KC[l], pf["ctx"], self.d_scale, b0, nq, qd,
+                                   c.group, cap, m, pf["part"], s)
+            else:
+                hvdrv.qk_rows(pf["qkv"], w["qn"], w["kn"], self.d_cos, self.d_sin, b0, pf["q"],
+                              self.KC[l], self.VC[l], nq, nkv, qd, cap, RMS_EPS, m, s,
+                              f16=self.kv_f16)
+                hvdrv.attn_rows(pf["q"], self.KC[l], self.VC[l], pf["ctx"], self.d_scale, b0,
+                                nq, qd, c.group, cap * qd, m, pf["part"], pf["ticket"], s,
+                                f16=self.kv_f16)
+            self._gemm(pf["ctx"], w["o"], pf["o"], m)
+            hvdrv.vadd(pf["h"], pf["o"], pf["h"], m * hid, s)
+            hvdrv.rmsnorm(pf["h"], pf["hn"], w["fn"], m, hid, RMS_EPS, s)
+            self._gemm(pf["hn"], w["gu"], pf["gu"], m)
+            hvdrv.silu_rows(pf["gu"], pf["act"], ffn, m, s)
+            self._gemm(pf["act"], w["down"], pf["o"], m)
+            hvdrv.vadd(pf["h"], pf["o"], pf["h"], m * hid, s)
+
     def _prefill_batched(self, prompt_ids, argmax: bool):
         """The prompt through every layer PREFILL_BATCH tokens at a time: per token the
         arithmetic of the eager step (engine/limited.py:374-419), so the KV cache and the
@@ -762,8 +832,7 @@ class Engine:
         pos at it, step 0 -- then, with `argmax`, the first greedy token taken as the
         fused step's last prompt launch does (gen[0], step 1, pos = prompt length)."""
         c = self.cfg
-        hid, ffn, qd, nq, nkv, cap = (c.hidden, c.ffn, c.head_dim, c.n_head, c.n_kv,
-                                      c.max_context)
+        hid, cap = c.hidden, c.max_context
         toks = np.ascontiguousarray(prompt_ids, np.int32)
         n = toks.size
         if n == 0 or n > cap:
@@ -775,25 +844,7 @@ class Engine:
         m = 0
         for b0 in range(0, n, pf["n"]):
             m = min(pf["n"], n - b0)
-            hvdrv.synchronize()                 # the host copy below reuses pf["tok"]
-            hvdrv.upload(pf["tok"], toks[b0:b0 + m].ctypes.data, 4 * m)
-            hvdrv.gather_rows(self.d_emb16, pf["tok"], pf["h"], hid, m, s)
-            for l, w in enumerate(self.layers):
-                hvdrv.rmsnorm(pf["h"], pf["hn"], w["an"], m, hid, RMS_EPS, s)
-                self._gemm(pf["hn"], w["qkv"], pf["qkv"], m)
-                hvdrv.qk_rows(pf["qkv"], w["qn"], w["kn"], self.d_cos, self.d_sin, b0, pf["q"],
-                              self.KC[l], self.VC[l], nq, nkv, qd, cap, RMS_EPS, m, s,
-                              f16=self.kv_f16)
-                hvdrv.attn_rows(pf["q"], self.KC[l], self.VC[l], pf["ctx"], self.d_scale, b0,
-                                nq, qd, c.group, cap * qd, m, pf["part"], pf["ticket"], s,
-                                f16=self.kv_f16)
-                self._gemm(pf["ctx"], w["o"], pf["o"], m)
-                hvdrv.vadd(pf["h"], pf["o"], pf["h"], m * hid, s)
-                hvdrv.rmsnorm(pf["h"], pf["hn"], w["fn"], m, hid, RMS_EPS, s)
-                self._gemm(pf["hn"], w["gu"], pf["gu"], m)
-                hvdrv.silu_rows(pf["gu"], pf["act"], ffn, m, s)
-                self._gemm(pf["act"], w["down"], pf["o"], m)
-                hvdrv.vadd(pf["h"], pf["o"], pf["h"], m * hid, s)
+            self._prefill_run(toks[b0:b0 + m], b0)
         # the last prompt token: final norm and LM head, as the eager step ends
         hvdrv.copy_async(self.d_h, pf["h"] + (m - 1) * hid * 4, hid * 4, s)
         hvdrv.rmsnorm(self.d_h, self.d_hn, self.d_onorm, 1, hid, RMS_EPS, s)
@@ -963,6 +1014,63 @@ class Engine:
     def download_logits(self) -> np.ndarray:
         out = np.zeros(self.n_head_rows, F32)
         hvdrv.download(out.ctypes.data, self.d_logits, out.nbytes)
+        return out
+
+    # ---- scoring ------------------------------------------------------------------------
+
+    def _score_buffers(self, rows: int, top: int) -> dict:
+        """Device buffers of one scored run (allocated on first use; the alternatives' part
+        grows when a later call wants more of them)."""
+        sc = self._sc
+        if sc is None:
+            sc = self._sc = {"top": -1, "logits": self._alloc(rows * self.n_head_rows * 4),
+                             "lp": self._alloc(rows * 4), "ent": self._alloc(rows * 4),
+                             "tok": self._alloc(rows * 4)}
+        if top > sc["top"]:
+            nb = hvdrv.logprob_scratch(rows, self.n_head_rows, top)
+            sc.update(top=top, id=self._alloc(rows * top * 4), alt=self._alloc(rows * top * 4),
+                      scratch=self._alloc(nb))
+            hvdrv.memset8(sc["scratch"], 0, nb)
+        return sc
+
+    def score(self, ids, top: int = 0) -> dict:
+        """How likely the model finds the text `ids`: for every position i from 1 on, the log
+        probability of ids[i] given ids[:i] ("logprob", f32 [n - 1]), the entropy of that
+        distribution ("entropy") and its `top` most likely tokens with their log
+        probabilities ("top_ids" i32, "top_logprobs" f32, [n - 1][top], best first). The text
+        goes through the layers and the LM head PREFILL_BATCH tokens at a time, whatever
+        `prefill` is; one GPU. Leaves the KV cache holding ids[:-1]."""
+        c = self.cfg
+        toks = np.ascontiguousarray(ids, np.int32)
+        n = toks.size
+        if self.world > 1:
+            raise ValueError("score() runs on one GPU (world = 1)")
+        if toks.ndim != 1 or n < 2 or n - 1 > c.max_context:
+            raise ValueError(f"{n} tokens to score: 2 to {c.max_context + 1}")
+        if toks.min() < 0 or toks.max() >= c.vocab:
+            raise ValueError("a token id outside the vocabulary")
+        if not 0 <= top <= min(32, c.vocab):
+            raise ValueError(f"top={top}: 0 to {min(32, c.vocab)} alternatives")
+        pf = self._prefill_buffers()
+        sc = self._score_buffers(pf["n"], top)
+        s, v = self._stream_cur, self.n_head_rows
+        out = {"logprob": np.empty(n - 1, F32), "entropy": np.empty(n - 1, F32),
+               "top_ids": np.empty((n - 1, top), np.int32),
+               "top_logprobs": np.empty((n - 1, top), F32)}
+        for b0 in range(0, n - 1, pf["n"]):
+            m = min(pf["n"], n - 1 - b0)
+            self._prefill_run(toks[b0:b0 + m], b0)
+            hvdrv.upload(sc["tok"], toks[b0 + 1:b0 + 1 + m].ctypes.data, 4 * m)
+            hvdrv.rmsnorm(pf["h"], pf["hn"], self.d_onorm, m, c.hidden, RMS_EPS, s)
+            self._gemm(pf["hn"], self.head, sc["logits"], m)
+            hvdrv.logprob_rows(sc["logits"], v, m, v, sc["tok"], top, sc["lp"], sc["ent"],
+                               sc["id"], sc["alt"], sc["scratch"], s)
+            hvdrv.synchronize()
+            for key, ptr in (("logprob", "lp"), ("entropy", "ent"), ("top_ids", "id"),
+                             ("top_logprobs", "alt")):
+                part = out[key][b0:b0 + m]
+                if part.size:
+                    hvdrv.download(part.ctypes.data, sc[ptr], part.nbytes)
         return out
 
     def _weight_bits(self) -> tuple[int, int]:

@@ -258,6 +258,59 @@ int hv_attn_decode_f16(const float* q, const uint16_t* kc, const uint16_t* vc, f
                        const float* scale, const int32_t* pos, int nq, int hd, int group,
                        int kvstride, void* stream);
 
+/* The 8-bit KV lane (no counterpart in the reference): one opaque buffer per layer holds K
+ * and V as int8 codes with one f32 scale per (kv head, block of 32 positions), K and V
+ * apart. With x a block's 32 x 128 values: s = f32(max|x| / 127), 1 where that is 0;
+ * c = trunc(f32(x / s) + (x < 0 ? -0.5 : 0.5)), clipped to +-127 (quant_a8s's rule,
+ * engine/reference.py:44-59); a value reads back as f32(c s). A block that holds a NaN or an
+ * infinity reads NaN throughout. The block that is still open (fewer than 32 rows) stays in
+ * f32 and is quantised once, when its last row arrives, so no value is rounded twice and the
+ * cache does not depend on how the rows were divided into calls.
+ *   The buffer: hv_kv_q8_size bytes, 16-byte aligned, zeroed = empty. It knows how many
+ * positions it holds (on the device: the calls may be captured). Rows are written in order:
+ * a write at pos0 makes the length pos0 + ntok, positions from there on are no longer held,
+ * and a write past the length (a gap) writes nothing. Going back into a complete block
+ * reopens it from its codes, except the block of the last row written, whose f32 rows are
+ * still there. Positions that are not held read NaN and attend to NaN. hd must be 128.
+ *   Arrangement (nblk = ceil(cap / 32); every part padded to 256 bytes): codes u8
+ * [nkv][nblk][K, V][4096], each code + 128; scales f32 [nkv][nblk][K, V]; the open rows f32
+ * [nkv][K, V][32][128]; the length i32 [nkv][K, V]. In a block K's code of position
+ * 8 j + g, dim 64 h + 16 s + 4 t + e stands at byte 512 (2 j + h) + 16 (4 g + t) + 4 s + e,
+ * V's of position 16 k + 8 j + 2 t + e, dim 16 u + 8 h + g at
+ * 512 u + 16 (4 g + t) + 8 h + 4 k + 2 j + e (the tensor pipe's fragments, lane by lane).
+ *   hv_kv_append_q8  one row per head, k, v [nkv][128], at the device position *pos (nothing
+ *                    outside [0, cap))                                      (kvapp_pos)
+ *   hv_kv_rows_q8    ntok rows at pos0; row t of k and of v at t * ld floats, head after
+ *                    head (ld >= nkv * 128, a multiple of 4)
+ *   hv_qk_rows_q8    hv_qk_rows over this cache: head norms, RoPE and the write in one pass
+ *   hv_kv_read_q8    positions pos0 .. pos0 + ntok - 1 as f32 rows [ntok][nkv][128] */
+int hv_kv_q8_size(int nkv, int hd, int cap, size_t* bytes);
+int hv_kv_append_q8(const float* k, const float* v, void* kv, const int32_t* pos, int nkv,
+                    int hd, int cap, void* stream);
+int hv_kv_rows_q8(const float* k, const float* v, int ld, void* kv, int pos0, int nkv, int hd,
+                  int cap, int ntok, void* stream);
+int hv_qk_rows_q8(const float* qkv, const float* qn, const float* kn, const float* cos_t,
+                  const float* sin_t, int pos0, float* q_out, void* kv, int nq, int nkv, int hd,
+                  int cap, float eps, int ntok, void* stream);
+int hv_kv_read_q8(const void* kv, float* k_out, float* v_out, int pos0, int nkv, int hd,
+                  int cap, int ntok, void* stream);
+/* Attention over that cache, softmax(scale q k^T) v in f32 precision (not the reference's
+ * order of operations: the lane has its own results). Query head h reads kv head h / group,
+ * group 1 to 8; q and ctx [ntok][nq][128], 16-byte aligned.
+ *   hv_attn_decode_q8  one query row over positions 0 .. *pos. A *pos that is not held
+ *                      leaves NaN in ctx and reads no cache row.            (fda_warp_pos)
+ *   hv_attn_rows_q8    row t over positions 0 .. pos0 + t of the cache as it stands: rows of
+ *                      a block that this run completed are read quantised.
+ * scratch: hv_attn_q8_scratch bytes, 16-byte aligned, zeroed once by the caller; every call
+ * leaves it ready for the next. Calls that may overlap on the GPU (streams, captured graphs)
+ * need a scratch each. Nothing is allocated. */
+int hv_attn_q8_scratch(int nq, int group, int cap, int ntok, size_t* bytes);
+int hv_attn_decode_q8(const float* q, const void* kv, float* ctx, const float* scale,
+                      const int32_t* pos, int nq, int hd, int group, int cap, void* scratch,
+                      void* stream);
+int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const float* scale, int pos0,
+                    int nq, int hd, int group, int cap, int ntok, void* scratch, void* stream);
+
 /* Makes sure the attention scratch can serve nkv heads at a cache of `cap` positions. */
 int hv_attn_reserve(int nkv, int group, int cap);
 
@@ -304,6 +357,21 @@ int hv_argmax_key(const float* logits, int n, int base, uint64_t* key, void* str
  * argmax_f: *tok, gen[*step] = tok, ++*step, ++*pos; every keys[i] is reset to 0. */
 int hv_argmax_key_final(uint64_t* keys, int nkeys, int32_t* tok, int32_t* gen,
                         int32_t* step, int32_t* pos, void* stream);
+
+/* Scoring (no counterpart in the reference, which returns greedy tokens only): for every row
+ * of logits [rows][n] (row r at r * ld floats), with p its softmax:
+ *   lp[r]      log p of token tok[r]; NaN if tok[r] is outside [0, n)
+ *   ent[r]     the entropy, -sum p log p (natural logarithm)
+ *   top_id, top_lp [rows][top]   the `top` most likely tokens, best first, and their log p
+ *              (top 0 to 32, at most n; ties to the lower id, as np.argmax takes them)
+ * -infinity is a token that cannot occur. A row with a NaN, a +infinity or only -infinity
+ * has no distribution: lp, ent and top_lp are NaN, top_id still in np.argmax's order.
+ * scratch: hv_logprob_scratch bytes, 16-byte aligned, zeroed once by the caller; every call
+ * leaves it ready for the next; calls that may overlap need one each. */
+int hv_logprob_scratch(int rows, int n, int top, size_t* bytes);
+int hv_logprob_rows(const float* logits, long long ld, int rows, int n, const int32_t* tok,
+                    int top, float* lp, float* ent, int32_t* top_id, float* top_lp,
+                    void* scratch, void* stream);
 
 /* The bounded device-side wait that every cross-CTA and cross-rank wait of the fused
  * step is built on (no counterpart in the reference, whose kernels never wait on each

@@ -1,0 +1,468 @@
+"""The 8-bit KV cache on a B200: writing (one row, runs, with the head norms and rotation in
+the same pass), reading back, attention of one token and of runs, and the engine over it,
+against the numpy model of kv_q8_ref.py."""
+import numpy as np
+import pytest
+
+import hv_oracle as O
+import kv_q8_ref as R
+import synth
+import w4format
+from gpu_util import Dev, bits
+
+pytestmark = pytest.mark.gpu
+F32 = np.float32
+HD = 128
+
+
+def rows(g, n, nkv, spread=1.0):
+    k = (g.standard_normal((n, nkv, HD)) * np.exp(spread * g.standard_normal((1, nkv, HD))))
+    return k.astype(F32), g.standard_normal((n, nkv, HD)).astype(F32)
+
+
+def i32(x):
+    return Dev(np.array([x], np.int32))
+
+
+def new_cache(hv, nkv, cap, fill=0):
+    n = hv.kv_q8_size(nkv, HD, cap)
+    (_, _, held, _), _ = R.parts(nkv, cap)
+    b = np.full(n, fill, np.uint8)
+    b[held:] = 0
+    return Dev(b)
+
+
+def write(hv, kv, k, v, pos0, cap):
+    nkv = k.shape[1]
+    hv.kv_rows_q8(Dev(k), Dev(v), nkv * HD, kv, pos0, nkv, HD, cap, len(k))
+
+
+def read(hv, kv, nkv, cap, pos0=0, n=None):
+    n = cap - pos0 if n is None else n
+    ko, vo = (Dev(nbytes=n * nkv * HD * 4) for _ in range(2))
+    hv.kv_read_q8(kv, ko, vo, pos0, nkv, HD, cap, n)
+    out = np.stack([x.get(F32, (n, nkv, HD)) for x in (ko, vo)])
+    return out.swapaxes(1, 2)                                  # [2, nkv, n, 128]
+
+
+def same(a, b):
+    """Equal bit for bit, any NaN counting as any other."""
+    return np.array_equal(np.where(np.isnan(a), 0, bits(a)), np.where(np.isnan(b), 0, bits(b)))
+
+
+def check_buffer(kv, ref):
+    """Codes, scales, open rows and length of the device buffer against the model's."""
+    (a, b, c, end), nblk = R.parts(ref.nkv, ref.cap)
+    got, want = kv.get(np.uint8), ref.buffer()
+    closed = ref.held // R.BLK
+    cut = lambda x: x[:a].reshape(ref.nkv, nblk, 2, 4096)[:, :closed]  # noqa: E731
+    assert np.array_equal(cut(got), cut(want))
+    sc = lambda x: x[a:a + ref.nkv * nblk * 8].view(F32).reshape(ref.nkv, nblk, 2)[:, :closed]  # noqa: E731
+    assert same(sc(got), sc(want))
+    if ref.held:
+        n = (ref.held - 1) % R.BLK + 1
+        tl = lambda x: x[b:c].view(F32).reshape(ref.nkv, 2, 32, HD)[:, :, :n]  # noqa: E731
+        assert same(tl(got), tl(want))
+    assert np.array_equal(got[c:c + 8 * ref.nkv], want[c:c + 8 * ref.nkv])
+
+
+@pytest.mark.parametrize("nkv,cap,cuts", [
+    (1, 1, [1]), (2, 40, [1, 1, 30, 1]), (8, 64, [64]), (3, 200, [5, 27, 32, 65, 1, 31, 39]),
+    (8, 97, [33, 63, 1]), (2, 4352, [4096, 128, 1, 100])])
+def test_rows_are_quantised_as_written(hv, nkv, cap, cuts):
+    g = np.random.default_rng(cap)
+    k, v = rows(g, sum(cuts), nkv)
+    ref, kv, at = R.Cache(nkv, cap), new_cache(hv, nkv, cap, 0xFF), 0
+    for n in cuts:
+        ref.write(k[at:at + n], v[at:at + n], at)
+        if n == 1:
+            hv.kv_append_q8(Dev(k[at]), Dev(v[at]), kv, i32(at), nkv, HD, cap)
+        else:
+            write(hv, kv, k[at:at + n], v[at:at + n], at, cap)
+        at += n
+        check_buffer(kv, ref)
+    assert same(read(hv, kv, nkv, cap), ref.val)
+    if at > 3:
+        assert same(read(hv, kv, nkv, cap, 3, at - 3), ref.val[:, :, 3:at])
+
+
+def test_one_row_at_a_time_equals_one_run(hv):
+    nkv, cap, n = 2, 100, 97
+    k, v = rows(np.random.default_rng(4), n, nkv)
+    a, b = new_cache(hv, nkv, cap), new_cache(hv, nkv, cap, 0x55)
+    write(hv, a, k, v, 0, cap)
+    for t in range(n):
+        hv.kv_append_q8(Dev(k[t]), Dev(v[t]), b, i32(t), nkv, HD, cap)
+    assert same(read(hv, a, nkv, cap), read(hv, b, nkv, cap))
+
+
+def test_going_back_and_gaps(hv):
+    nkv, cap = 2, 256
+    g = np.random.default_rng(5)
+    ref, kv = R.Cache(nkv, cap), new_cache(hv, nkv, cap)
+    for pos0, n in ((0, 100), (90, 3),       # back inside the open block
+                    (96, 1), (95, 4),        # over the edge of the last block and back
+                    (40, 1),                 # into a complete block: reopened from its codes
+                    (41, 60), (0, 32), (31, 1), (5, 2), (0, 200), (64, 64),
+                    (130, 5),                # a gap: 128 are held
+                    (128, 128), (10, 1), (200, 1)):
+        k, v = rows(g, n, nkv)
+        ref.write(k, v, pos0)
+        if n == 1:
+            hv.kv_append_q8(Dev(k[0]), Dev(v[0]), kv, i32(pos0), nkv, HD, cap)
+        else:
+            write(hv, kv, k, v, pos0, cap)
+        check_buffer(kv, ref)
+        assert same(read(hv, kv, nkv, cap), ref.val), (pos0, n)
+
+
+def test_append_outside_the_cache_writes_nothing(hv):
+    nkv, cap = 2, 64
+    k, v = rows(np.random.default_rng(6), 10, nkv)
+    kv = new_cache(hv, nkv, cap)
+    write(hv, kv, k, v, 0, cap)
+    before = kv.get(np.uint8)
+    for p in (-1, 64, 1 << 30, -(1 << 31), 11):
+        hv.kv_append_q8(Dev(k[0]), Dev(v[0]), kv, i32(p), nkv, HD, cap)
+        assert np.array_equal(kv.get(np.uint8), before)
+
+
+def test_blocks_of_hard_values(hv):
+    """Zeros, one non-finite value, the largest and the smallest floats, halves of a step."""
+    nkv, cap = 1, 256
+    k, v = rows(np.random.default_rng(7), cap, nkv)
+    k[0:32] = 0
+    k[40, 0, 7] = np.nan
+    k[70, 0, 127] = np.inf
+    v[100, 0, 0] = -np.inf
+    k[128:160] = np.ldexp(k[128:160], -140).astype(F32)              # subnormals
+    k[160:192] *= F32(3e38) / np.abs(k[160:192]).max()
+    k[192] = (np.arange(128) - 63.5).astype(F32)                      # ties at scale 1
+    k[192, 0, 0], k[193:224] = 127, 0
+    v[224:256] = F32(1e-45)
+    ref, kv = R.Cache(nkv, cap), new_cache(hv, nkv, cap)
+    ref.write(k, v, 0)
+    write(hv, kv, k, v, 0, cap)
+    check_buffer(kv, ref)
+    got = read(hv, kv, nkv, cap)
+    assert same(got, ref.val)
+    assert np.isnan(got[0, 0, 32:96]).all() and np.isnan(got[1, 0, 96:128]).all()
+
+
+def test_strided_rows(hv):
+    nkv, cap, n, ld = 3, 80, 50, 7 * HD
+    g = np.random.default_rng(8)
+    src = g.standard_normal((n, ld)).astype(F32)
+    k, v = src[:, HD:4 * HD].reshape(n, 3, HD), src[:, 4 * HD:].reshape(n, 3, HD)
+    d, kv, ref = Dev(src), new_cache(hv, nkv, cap), R.Cache(nkv, cap)
+    hv.kv_rows_q8(int(d) + 4 * HD, int(d) + 16 * HD, ld, kv, 0, nkv, HD, cap, n)
+    ref.write(k, v, 0)
+    assert same(read(hv, kv, nkv, cap), ref.val)
+
+
+@pytest.mark.parametrize("nq,nkv,pos0,ntok", [(8, 2, 0, 40), (4, 4, 37, 91), (5, 1, 31, 1),
+                                              (16, 8, 64, 32)])
+def test_qk_rows_is_qk_rows_then_the_write(hv, nq, nkv, pos0, ntok):
+    cap, eps = 160, 1e-5
+    g = np.random.default_rng(pos0 + ntok)
+    qkv = g.standard_normal((ntok, (nq + 2 * nkv) * HD)).astype(F32)
+    qn, kn = ((1 + 0.01 * g.standard_normal(HD)).astype(F32) for _ in range(2))
+    cos_t, sin_t = (x.astype(F32) for x in O.rope_tables(cap, HD, 1e6))
+    dev = [Dev(x) for x in (qkv, qn, kn, cos_t, sin_t)]
+    hk, hvv = rows(g, pos0, nkv) if pos0 else (None, None)
+    kv, ref = new_cache(hv, nkv, cap), R.Cache(nkv, cap)
+    if pos0:
+        write(hv, kv, hk, hvv, 0, cap)
+        ref.write(hk, hvv, 0)
+    qo, qf = Dev(nbytes=ntok * nq * HD * 4), Dev(nbytes=ntok * nq * HD * 4)
+    kf, vf = Dev(nbytes=nkv * cap * HD * 4), Dev(nbytes=nkv * cap * HD * 4)
+    hv.qk_rows_q8(*dev, pos0, qo, kv, nq, nkv, HD, cap, eps, ntok)
+    hv.qk_rows(*dev, pos0, qf, kf, vf, nq, nkv, HD, cap, eps, ntok)
+    assert np.array_equal(bits(qo.get(F32)), bits(qf.get(F32)))
+    k32, v32 = (x.get(F32, (nkv, cap, HD))[:, pos0:pos0 + ntok].swapaxes(0, 1)
+                for x in (kf, vf))
+    ref.write(np.ascontiguousarray(k32), np.ascontiguousarray(v32), pos0)
+    check_buffer(kv, ref)
+
+
+# ---- attention -----------------------------------------------------------------------
+
+SCALE = F32(1.0 / np.sqrt(HD))
+
+
+def filled(hv, seed, nkv, n, cap, look=3.0):
+    """A cache of n positions whose other bytes are 0xFF (NaN scales, NaN rows)."""
+    g = np.random.default_rng(seed)
+    k, v = rows(g, n, nkv, 0.3)
+    ref = R.Cache(nkv, cap)
+    ref.write(k, v, 0)
+    return g, ref, Dev(ref.buffer(0xFF))
+
+
+def queries(g, ref, ntok, nq):
+    q = g.standard_normal((ntok, nq, HD))
+    n, group = ref.held, nq // ref.nkv
+    for h in range(nq):                         # weights that are not flat
+        q[:, h] += 1.5 * np.nan_to_num(ref.val[0, h // group, g.integers(0, n)])
+    return q.astype(F32)
+
+
+def scratch(hv, nq, group, cap, ntok=1):
+    return Dev(nbytes=hv.attn_q8_scratch(nq, group, cap, ntok))
+
+
+def near(got, want, tol):
+    off = np.abs(got.astype(np.float64) - want)
+    assert np.isfinite(got).all()
+    assert (off <= tol).all(), float((off / tol).max())
+
+
+@pytest.mark.parametrize("nkv,group,n", [
+    (1, 1, 1), (2, 4, 2), (8, 2, 31), (8, 4, 32), (8, 8, 33), (2, 5, 63), (1, 3, 64), (4, 6, 65),
+    (2, 7, 97), (8, 2, 300), (1, 8, 1000), (8, 4, 4225), (3, 4, 2048), (1, 4, 9000)])
+def test_decode_attention(hv, nkv, group, n):
+    nq, cap = nkv * group, n + 37
+    g, ref, kv = filled(hv, n + group, nkv, n, cap)
+    q, ctx = queries(g, ref, 1, nq), Dev(np.full((nq, HD), 7, F32))
+    s = scratch(hv, nq, group, cap)
+    for pos in sorted({n - 1, n // 2, 0, max(0, n - 33)}):     # whole and part of the cache
+        hv.attn_decode_q8(Dev(q), kv, ctx, Dev(np.array([SCALE])), i32(pos), nq, HD, group, cap,
+                          s)
+        near(ctx.get(F32, (nq, HD)), *R.attention(q[0], ref.val, pos, group, float(SCALE)))
+
+
+@pytest.mark.parametrize("nkv,group,pos0,ntok", [
+    (1, 1, 0, 1), (2, 4, 0, 33), (8, 2, 256, 44), (2, 5, 31, 70), (4, 8, 100, 129), (1, 3, 5, 200),
+    (8, 4, 992, 64), (2, 1, 0, 256), (1, 8, 3000, 17), (2, 4, 4000, 3), (2, 7, 511, 1)])
+def test_rows_attention(hv, nkv, group, pos0, ntok):
+    nq, n = nkv * group, pos0 + ntok
+    cap = n + 50
+    g, ref, kv = filled(hv, n + group, nkv, n, cap)
+    q, ctx = queries(g, ref, ntok, nq), Dev(np.full((ntok + 1, nq, HD), 7, F32))
+    hv.attn_rows_q8(Dev(q), kv, ctx, Dev(np.array([SCALE])), pos0, nq, HD, group, cap, ntok,
+                    scratch(hv, nq, group, cap, ntok))
+    got = ctx.get(F32, (ntok + 1, nq, HD))
+    assert (got[ntok] == 7).all()                              # rows behind the last stay
+    for t in {0, 1, ntok // 2, ntok - 2, ntok - 1} & set(range(ntok)):
+        near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
+    # the same rows over the cache when it holds more positions: still causal
+    if ntok > 4:
+        m = ntok - 4
+        part = Dev(np.full((m, nq, HD), 7, F32))
+        hv.attn_rows_q8(Dev(q), kv, part, Dev(np.array([SCALE])), pos0, nq, HD, group, cap, m,
+                        scratch(hv, nq, group, cap, m))
+        near(part.get(F32, (m, nq, HD))[m - 1],
+             *R.attention(q[m - 1], ref.val, pos0 + m - 1, group, float(SCALE)))
+
+
+def test_positions_not_held_give_nan(hv):
+    nkv, group, n, cap = 2, 4, 40, 64
+    nq = nkv * group
+    g, ref, kv = filled(hv, 1, nkv, n, cap)
+    q, sc = queries(g, ref, 4, nq), Dev(np.array([SCALE]))
+    for pos in (-1, 40, 63, 64, 1 << 30, -(1 << 31)):
+        ctx = Dev(np.zeros((nq, HD), F32))
+        hv.attn_decode_q8(Dev(q[0]), kv, ctx, sc, i32(pos), nq, HD, group, cap,
+                          scratch(hv, nq, group, cap))
+        assert np.isnan(ctx.get(F32)).all(), pos
+    ctx = Dev(np.zeros((4, nq, HD), F32))
+    hv.attn_rows_q8(Dev(q), kv, ctx, sc, 38, nq, HD, group, cap, 4,
+                    scratch(hv, nq, group, cap, 4))
+    got = ctx.get(F32, (4, nq, HD))
+    assert np.isnan(got[2:]).all()
+    for t in (0, 1):
+        near(got[t], *R.attention(q[t], ref.val, 38 + t, group, float(SCALE)))
+    empty = new_cache(hv, nkv, cap, 0xFF)
+    hv.attn_decode_q8(Dev(q[0]), empty, ctx, sc, i32(0), nq, HD, group, cap,
+                      scratch(hv, nq, group, cap))
+    assert np.isnan(ctx.get(F32, (4, nq, HD))[0]).all()
+
+
+@pytest.mark.parametrize("size", [1e-20, 1.0, 1e4, 1e18])
+def test_sizes_of_q_and_k(hv, size):
+    """q k^T is what counts: q as large as k is small, and the other way round."""
+    nkv, group, n, cap = 2, 4, 150, 160
+    g = np.random.default_rng(11)
+    k, v = rows(g, n, nkv, 0.3)
+    ref = R.Cache(nkv, cap)
+    ref.write((k / F32(size)).astype(F32), (v * F32(size)).astype(F32), 0)
+    kv, q = Dev(ref.buffer(0xFF)), (g.standard_normal((1, 8, HD)) * size).astype(F32)
+    ctx = Dev(np.zeros((8, HD), F32))
+    hv.attn_decode_q8(Dev(q), kv, ctx, Dev(np.array([SCALE])), i32(n - 1), 8, HD, group, cap,
+                      scratch(hv, 8, group, cap))
+    near(ctx.get(F32, (8, HD)), *R.attention(q[0], ref.val, n - 1, group, float(SCALE)))
+    q3 = np.repeat(q, 3, 0)
+    ctx = Dev(np.zeros((3, 8, HD), F32))
+    hv.attn_rows_q8(Dev(q3), kv, ctx, Dev(np.array([SCALE])), n - 3, 8, HD, group, cap, 3,
+                    scratch(hv, 8, group, cap, 3))
+    near(ctx.get(F32, (3, 8, HD))[2], *R.attention(q[0], ref.val, n - 1, group, float(SCALE)))
+
+
+def test_steep_weights_and_bad_queries(hv):
+    """Scores far apart (one weight takes all), a zero query (all weights equal), a NaN and an
+    infinity in one head's query: only that head's context is lost."""
+    nkv, group, n, cap = 1, 4, 333, 352
+    g, ref, kv = filled(hv, 12, nkv, n, cap)
+    q = queries(g, ref, 1, 4)
+    q[0, 0] = ref.val[0, 0, 200] * 30
+    q[0, 1] = 0
+    sc = Dev(np.array([SCALE]))
+    for bad in (None, np.nan, np.inf):
+        if bad is not None:
+            q[0, 2, 5] = bad
+        for ntok in (0, 2):                       # 0: the decode call
+            qq = np.repeat(q, max(1, ntok), 0)
+            ctx = Dev(np.zeros((max(1, ntok), 4, HD), F32))
+            if ntok:
+                hv.attn_rows_q8(Dev(qq), kv, ctx, sc, n - ntok, 4, HD, group, cap, ntok,
+                                scratch(hv, 4, group, cap, ntok))
+            else:
+                hv.attn_decode_q8(Dev(qq), kv, ctx, sc, i32(n - 1), 4, HD, group, cap,
+                                  scratch(hv, 4, group, cap))
+            got = ctx.get(F32, (max(1, ntok), 4, HD))[-1]
+            live = [0, 1, 3] if bad is not None else [0, 1, 2, 3]
+            want, tol = R.attention(np.nan_to_num(q[0], posinf=0), ref.val, n - 1, group,
+                                    float(SCALE))
+            near(got[live], want[live], tol[live])
+            if bad is not None:
+                assert np.isnan(got[2]).all()
+
+
+def test_a_poisoned_block_poisons_what_reads_it(hv):
+    nkv, group, cap = 1, 2, 128
+    g = np.random.default_rng(13)
+    k, v = rows(g, 100, nkv, 0.3)
+    v[70, 0, 3] = np.inf
+    ref, sc = R.Cache(nkv, cap), Dev(np.array([SCALE]))
+    ref.write(k, v, 0)
+    kv, q, ctx = Dev(ref.buffer()), g.standard_normal((2, HD)).astype(F32), Dev(nbytes=1024)
+    for pos, lost in ((63, False), (64, True), (99, True)):
+        hv.attn_decode_q8(Dev(q), kv, ctx, sc, i32(pos), 2, HD, group, cap,
+                          scratch(hv, 2, group, cap))
+        got = ctx.get(F32, (2, HD))
+        assert np.isnan(got).all() if lost else np.isfinite(got).all(), pos
+    out = Dev(np.zeros((4, 2, HD), F32))
+    hv.attn_rows_q8(Dev(np.stack([q] * 4)), kv, out, sc, 62, 2, HD, group, cap, 4,
+                    scratch(hv, 2, group, cap, 4))
+    got = out.get(F32, (4, 2, HD))
+    assert np.isfinite(got[:2]).all() and np.isnan(got[2:]).all()
+
+
+def test_captured_decode_follows_the_device_position(hv):
+    """Append and attention captured once, replayed while *pos moves over block edges, equal
+    to direct calls; two graphs with a scratch each, on two streams."""
+    nkv, group, cap, n0 = 2, 4, 200, 30
+    nq = nkv * group
+    g = np.random.default_rng(14)
+    k, v = rows(g, n0 + 40, nkv)
+    q = g.standard_normal((nq, HD)).astype(F32)
+    dq, sc = Dev(q), Dev(np.array([SCALE]))
+    want = []
+    kv = new_cache(hv, nkv, cap)
+    write(hv, kv, k[:n0], v[:n0], 0, cap)
+    s = scratch(hv, nq, group, cap)
+    for t in range(n0, n0 + 40):
+        ctx = Dev(nbytes=nq * HD * 4)
+        hv.kv_append_q8(Dev(k[t]), Dev(v[t]), kv, i32(t), nkv, HD, cap)
+        hv.attn_decode_q8(dq, kv, ctx, sc, i32(t), nq, HD, group, cap, s)
+        want.append(ctx.get(F32))
+    lanes = []
+    for _ in range(2):
+        L = dict(kv=new_cache(hv, nkv, cap), s=scratch(hv, nq, group, cap), pos=i32(n0),
+                 k=Dev(k[0]), v=Dev(v[0]), ctx=Dev(nbytes=nq * HD * 4), st=hv.stream_create())
+        write(hv, L["kv"], k[:n0], v[:n0], 0, cap)
+        hv.synchronize()
+        hv.capture_begin(L["st"])
+        hv.kv_append_q8(L["k"], L["v"], L["kv"], L["pos"], nkv, HD, cap, L["st"])
+        hv.attn_decode_q8(dq, L["kv"], L["ctx"], sc, L["pos"], nq, HD, group, cap, L["s"],
+                          L["st"])
+        L["graph"] = hv.capture_end(L["st"])
+        L["exec"] = hv.graph_instantiate(L["graph"])
+        lanes.append(L)
+    for i, t in enumerate(range(n0, n0 + 40)):
+        for L in lanes:
+            L["k"].put(k[t])
+            L["v"].put(v[t])
+            L["pos"].put(np.array([t], np.int32))
+        hv.synchronize()
+        for L in lanes:
+            hv.graph_launch(L["exec"], L["st"])
+        for L in lanes:
+            assert np.array_equal(bits(L["ctx"].get(F32)), bits(want[i])), t
+    for L in lanes:
+        hv.graph_destroy(L["graph"], L["exec"])
+        hv.stream_destroy(L["st"])
+
+
+def test_same_call_same_bits(hv):
+    nkv, group, n = 8, 4, 3000
+    g, ref, kv = filled(hv, 15, nkv, n, n)
+    q, sc = queries(g, ref, 20, 32), Dev(np.array([SCALE]))
+    s, s2, out = scratch(hv, 32, group, n), scratch(hv, 32, group, n, 20), []
+    for _ in range(3):
+        a, b = Dev(nbytes=32 * HD * 4), Dev(nbytes=20 * 32 * HD * 4)
+        hv.attn_decode_q8(Dev(q[0]), kv, a, sc, i32(n - 1), 32, HD, group, n, s)
+        hv.attn_rows_q8(Dev(q), kv, b, sc, n - 20, 32, HD, group, n, 20, s2)
+        out.append((bits(a.get(F32)), bits(b.get(F32))))
+    for a, b in out[1:]:
+        assert np.array_equal(a, out[0][0]) and np.array_equal(b, out[0][1])
+
+
+# ---- the engine ----------------------------------------------------------------------
+
+def engine(arch, seed, cap, **kw):
+    import limited
+    cfg = w4format.Config(arch)
+    return limited.Engine(config=cfg, tensors=synth.iter_tensors(cfg, seed), quiet=True,
+                          max_context=cap, **kw)
+
+
+@pytest.mark.parametrize("prefill", ["steps", "batched"])
+def test_engine_over_the_8bit_cache(hv, prefill):
+    """The first layer's cache is the f32 engine's rows quantised (they do not depend on
+    attention); the last layer's context is attention over what its cache reads back; the
+    graph-replayed decode gives the direct one's tokens."""
+    arch = synth.tiny_arch(hidden=512, n_head=8, n_kv=2)
+    ids = synth.prompt_ids(w4format.Config(arch), 3, 300)
+    cap = 352
+    a = engine(arch, 3, cap, kv_dtype="q8", fused=False, prefill=prefill)
+    f = engine(arch, 3, cap, fused=False, prefill=prefill)
+    try:
+        c = a.cfg
+        assert a.kv_bytes == c.n_layer * hv.kv_q8_size(c.n_kv, HD, cap)
+        lf, la = f.logits(ids), a.logits(ids)
+        assert np.isfinite(la).all() and la.shape == lf.shape
+        n = len(ids)
+        k32, v32 = (f._download(p, (c.n_kv, cap, HD), F32)[:, :n].swapaxes(0, 1)
+                    for p in (f.KC[0], f.VC[0]))
+        ref = R.Cache(c.n_kv, cap)
+        ref.write(k32, v32, 0)
+        assert same(read(hv, a.KC[0], c.n_kv, cap, 0, n), ref.val[:, :, :n])
+        if prefill == "steps":
+            q = a._download(a.d_qkv, (c.n_head, HD), F32)
+            ctx = a._download(a.d_ctx, (c.n_head, HD), F32)
+        else:
+            m = (n - 1) % a.PREFILL_BATCH
+            at = m * c.n_head * HD * 4
+            q = a._download(a._pf["q"] + at, (c.n_head, HD), F32)
+            ctx = a._download(a._pf["ctx"] + at, (c.n_head, HD), F32)
+        val = read(hv, a.KC[-1], c.n_kv, cap, 0, n)
+        near(ctx, *R.attention(q, val, n - 1, c.group, float(a.attn_scale)))
+        toks, _, _ = a.generate(ids, 40, stop_on_eos=False)
+        assert a.generate(ids, 40, stop_on_eos=False, use_graph=True)[0] == toks
+        assert a.generate(ids, 40)[0] == toks                  # a shorter cache written over
+    finally:
+        a.free()
+        f.free()
+
+
+def test_engine_q8_with_odd_group_and_long_context(hv):
+    """A group of 5 query heads and a capacity over the reference-order attention's 16384."""
+    arch = synth.tiny_arch(hidden=256, n_head=10, n_kv=2)
+    a = engine(arch, 4, 20000, kv_dtype="q8", fused=False, prefill="batched")
+    try:
+        ids = synth.prompt_ids(a.cfg, 4, 600)
+        toks, _, _ = a.generate(ids, 8, stop_on_eos=False)
+        assert len(toks) == 8
+    finally:
+        a.free()
