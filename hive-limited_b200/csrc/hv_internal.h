@@ -14,6 +14,8 @@ namespace hv {
 void set_error(const char* fmt, ...);
 int cuda_fail(const char* what, cudaError_t e);
 int sm_count(int* out);
+// Raises a kernel's dynamic shared-memory limit once per device.
+int smem_attr(const void* fn, size_t bytes);
 
 // The reference-order decode attention (attn_exact.cuh, kernels in k_ops.cu), shared by
 // hv_attn_decode, the batched prefill rows and the allocation-free entry point.

@@ -105,7 +105,9 @@ def attention(q, val, pos, group, scale):
     at most 16 partial sums of an accumulator that may cut instead of round (2u each), then
     the scale and log2 e (2u each), so |dx| <= 44 u B, B = scale * max_t sum_i |q_i k_ti|;
     subtracting the maximum and 2^x add 4u |x| <= 4 u B; weights are off by that on both sides
-    of the quotient: 96 u B. The weighted sum adds each of the n positions once in tiles
+    of the quotient: 96 u B. A weight enters the second product as two binary16 terms of 2^15
+    times itself over the largest: what is left is at most half of binary16's smallest step,
+    2^-25, so 2^-40 of the largest weight, whatever the weight. The weighted sum adds each of the n positions once in tiles
     of 16 and 32: (n / 8 + 64) u of sum w |v| covers it with the sum of the weights."""
     q = q.astype(np.float64)
     out, tol = np.empty(q.shape), np.empty(q.shape)
@@ -117,5 +119,6 @@ def attention(q, val, pos, group, scale):
         w = np.exp(x - x.max())
         w /= w.sum()
         out[h] = w @ v
-        tol[h] = (96 * U * big + (n / 8 + 64) * U) * (w @ np.abs(v)) + 1e-37
+        tol[h] = (96 * U * big + (n / 8 + 64) * U) * (w @ np.abs(v))
+        tol[h] += 2.0 ** -40 * w.max() * np.abs(v).sum(0) + 1e-37
     return out, tol
