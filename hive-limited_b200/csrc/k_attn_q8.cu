@@ -96,6 +96,7 @@ constexpr int kDecWarps = 8;
 constexpr int kDecStages = 3;
 constexpr int kDecBlocksMin = 8;       // blocks a chunk holds before a head gets another CTA
 constexpr int kDecStride = 132;        // floats between the columns of a warp's sums
+constexpr int kDecTickets = 1024;      // kv heads with chunks to join: first in the scratch
 constexpr int kDecPart = 8 * (kHd + 2);    // scratch floats of a chunk: sums, then (max, sum)
 constexpr int kDecSmem = kDecWarps * kDecStages * 2 * kQ8Codes;
 
@@ -422,15 +423,13 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   }
 }
 
-size_t dec_tickets(int nkv) { return kv_q8_up((size_t)nkv * sizeof(unsigned)); }
-
 // CTAs per kv head: every SM has one, unless the cache cannot fill them.
 int dec_chunks(int nkv, int cap, int* out) {
   int sms = 0;
   const int rc = sm_count(&sms);
   if (rc) return rc;
   const int most = (cap / kQ8Blk + kDecBlocksMin - 1) / kDecBlocksMin;
-  *out = std::max(1, std::min(sms / nkv, most));
+  *out = nkv > kDecTickets ? 1 : std::max(1, std::min(sms / nkv, most));
   return HV_OK;
 }
 
@@ -461,7 +460,7 @@ extern "C" int hv_attn_q8_scratch(int nq, int group, int cap, int ntok, size_t* 
   int nch = 0;
   const int rc = dec_chunks(nq / group, cap, &nch);
   if (rc) return rc;
-  *bytes = dec_tickets(nq / group) + (size_t)(nq / group) * nch * kDecPart * sizeof(float);
+  *bytes = kDecTickets * sizeof(unsigned) + (size_t)(nq / group) * nch * kDecPart * sizeof(float);
   return HV_OK;
 }
 
@@ -479,7 +478,7 @@ extern "C" int hv_attn_decode_q8(const float* q, const void* kv, float* ctx, con
   const int rc2 = dec_chunks(nkv, cap, &nch);
   if (rc2) return rc2;
   unsigned* ticket = static_cast<unsigned*>(scratch);
-  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + dec_tickets(nkv));
+  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + kDecTickets * sizeof(unsigned));
   const void* fn = group > 4 ? (const void*)k_attn_dec_q8<true> : (const void*)k_attn_dec_q8<false>;
   const int rc3 = smem_attr(fn, kDecSmem);
   if (rc3) return rc3;

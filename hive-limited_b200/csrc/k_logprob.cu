@@ -19,86 +19,327 @@ namespace hv {
 namespace {
 
 constexpr int kMaxTop = 32;
+constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32;
+constexpr int kLpEach = 8;                        // logits a thread holds of a tile
+constexpr int kLpTile = kLpThreads * kLpEach;
+constexpr int kLpBuf = 2048;                      // candidates a CTA keeps in shared memory
+constexpr int kLpPieces = 64;                     // CTAs that may share a row
+constexpr int kLpTickets = 1024;                  // rows that may be shared; their tickets stand
+                                                  // first in the scratch whatever the call
+static_assert(kLpPieces * kMaxTop <= kLpBuf && kMaxTop * kLpEach <= kLpBuf, "candidates fit");
 
-// 64-bit key in np.argmax's order: the f32 bits mapped to an unsigned order, then ~id.
-HV_DEV unsigned long long lp_key(float v, int id) {
+using u64 = unsigned long long;
+
+// 64-bit key in np.argmax's order: the f32 bits mapped to an unsigned order, then ~id. A key
+// is never 0.
+HV_DEV u64 lp_key(float v, int id) {
   unsigned u = __float_as_uint(v);
   if (v != v) u = 0x7FC00000u;
   else if (v == 0.f) u = 0u;
   const unsigned ord = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return ((unsigned long long)ord << 32) | (unsigned long long)(~(unsigned)id);
+  return ((u64)ord << 32) | (u64)(~(unsigned)id);
+}
+HV_DEV float lp_key_value(u64 k) {
+  const unsigned ord = (unsigned)(k >> 32);
+  return __uint_as_float((ord & 0x80000000u) ? (ord & 0x7FFFFFFFu) : ~ord);
+}
+HV_DEV u64 max64(u64 a, u64 b) { return a > b ? a : b; }
+HV_DEV u64 min64(u64 a, u64 b) { return a < b ? a : b; }
+
+HV_DEV float max_nan(float a, float b) {          // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+HV_DEV float ex2f(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-HV_DEV unsigned long long block_max64(unsigned long long v, unsigned long long* s) {
+// A warp's 32 keys in falling order over the lanes.
+HV_DEV u64 warp_sort(u64 v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1) {
+#pragma unroll
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const u64 w = __shfl_xor_sync(0xFFFFFFFFu, v, j);
+      const bool high = ((lane & j) == 0) == ((lane & k) == 0 || k == 32);
+      v = high ? max64(v, w) : min64(v, w);
+    }
+  }
+  return v;
+}
+// The 32 largest of two falling lists, falling.
+HV_DEV u64 warp_merge(u64 a, u64 b) {
+  const int lane = threadIdx.x & 31;
+  a = max64(a, __shfl_sync(0xFFFFFFFFu, b, 31 - lane));
+#pragma unroll
+  for (int j = 16; j > 0; j >>= 1) {
+    const u64 w = __shfl_xor_sync(0xFFFFFFFFu, a, j);
+    a = (lane & j) == 0 ? max64(a, w) : min64(a, w);
+  }
+  return a;
+}
+
+// What a set of logits adds to a row: its maximum m, and over all its elements but one at the
+// maximum S = sum exp(x - m), T = sum (m - x) exp(x - m). m = -inf: nothing (yet).
+struct LpSum {
+  float m, s, t;
+};
+HV_DEV LpSum lp_join(LpSum a, LpSum b) {
+  if (b.m == -INFINITY) return a;
+  if (a.m == -INFINITY) return b;
+  if (a.m < b.m) { const LpSum c = a; a = b; b = c; }
+  const float d = fmaxf(b.m - a.m, -200.0f), f = ex2f(d * 1.4426950408889634f);
+  a.t += f * (b.t - d * (1.0f + b.s));
+  a.s += f * (1.0f + b.s);
+  if (!(b.m <= a.m)) a.m = b.m - b.m + a.m;         // a NaN on either side stays one
+  return a;
+}
+
+struct LpShared {
+  u64 buf[kLpBuf];
+  u64 lists[kLpWarps][32];
+  LpSum sums[kLpWarps];
+  int count;                 // candidates in buf
+  int more;                  // candidates of the current tile
+  unsigned last;
+};
+
+// The 32 largest of every warp's falling list `v`, falling, in warp 0 (all warps call).
+HV_DEV u64 block_merge(u64 v, LpShared& sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int half = kLpWarps / 2; half > 0; half >>= 1) {
+    if (warp >= half && warp < 2 * half) sh.lists[warp][lane] = v;
+    __syncthreads();
+    if (warp < half) v = warp_merge(v, sh.lists[warp + half][lane]);
+  }
+  return v;
+}
+
+// The 32 largest of the first n candidates, falling, in warp 0.
+HV_DEV u64 block_select(int n, LpShared& sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  u64 v = 0;
+  for (int i = warp * 32; i < n; i += kLpThreads) {
+    const u64 w = warp_sort(i + lane < n ? sh.buf[i + lane] : 0);
+    v = i == warp * 32 ? w : warp_merge(v, w);
+  }
+  return block_merge(v, sh);
+}
+
+// One CTA per (row, piece of the row). Four logits of a row stand on 16 bytes: `off` floats
+// before the row's first one make it so, and units at the edges are read one by one.
+// kTop: alternatives are wanted.
+template <bool kTop>
+__global__ void __launch_bounds__(kLpThreads)
+    k_logprob(const float* __restrict__ logits, size_t ld, int n, const int32_t* __restrict__ tok,
+              int top, float* __restrict__ lp, float* __restrict__ ent,
+              int32_t* __restrict__ top_id, float* __restrict__ top_lp, int pieces,
+              LpSum* __restrict__ psum, u64* __restrict__ plist, unsigned* __restrict__ ticket) {
+  __shared__ LpShared sh;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.x / pieces, piece = blockIdx.x % pieces;
+  const float* x = logits + (size_t)r * ld;
+  const int off = (int)(((uintptr_t)x >> 2) & 3);
+  const int units = (int)(((long long)off + n + 3) / 4), tiles = (units + kLpTile / 4 - 1) / (kLpTile / 4);
+  const int t0 = (int)((long long)tiles * piece / pieces);
+  const int t1 = (int)((long long)tiles * (piece + 1) / pieces);
+
+  // unit u holds logits 4 u - off ..; a thread has units base + i 512 of a tile
+  auto load = [&](int tile, float (&v)[kLpEach]) {
+#pragma unroll
+    for (int i = 0; i < kLpEach / 4; ++i) {
+      const int u = tile * (kLpTile / 4) + i * kLpThreads + threadIdx.x;
+      const int e = 4 * u - off;
+      if (e >= 0 && e + 4 <= n) {
+        const float4 f = __ldcs(reinterpret_cast<const float4*>(x + e));
+        v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * i + j] = e + j >= 0 && e + j < n ? x[e + j] : -INFINITY;
+      }
+    }
+  };
+  auto id_of = [&](int tile, int k) {
+    return 4 * (tile * (kLpTile / 4) + (k >> 2) * kLpThreads + (int)threadIdx.x) + (k & 3) - off;
+  };
+
+  float m = -INFINITY, s = 0.0f, t = 0.0f, ties = 0.0f;   // m is the warp's
+  u64 least = 0;                                         // a candidate is above it
+  float least_v = -INFINITY;
+  int have = 0;                                          // sh.count, between tiles
+  if (threadIdx.x == 0) sh.count = sh.more = 0;
+  __syncthreads();
+
+  float v[kLpEach], next[kLpEach];
+  if (t0 < t1) load(t0, next);
+  for (int tile = t0; tile < t1; ++tile) {
+#pragma unroll
+    for (int k = 0; k < kLpEach; ++k) v[k] = next[k];
+    if (tile + 1 < t1) load(tile + 1, next);
+    float mine = v[0];
+#pragma unroll
+    for (int k = 1; k < kLpEach; ++k) mine = max_nan(mine, v[k]);
+    float lm = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) lm = max_nan(lm, __shfl_xor_sync(0xFFFFFFFFu, lm, o));
+    if (lm < m) {                                        // the usual tile: nothing at the top
+#pragma unroll
+      for (int k = 0; k < kLpEach; ++k) {
+        const float z = fmaxf(v[k] - m, -200.0f), e = ex2f(z * 1.4426950408889634f);
+        s += e;
+        t = fmaf(-z, e, t);
+      }
+    } else if (lm != -INFINITY) {
+      if (!(lm == m)) {
+        const float d = fmaxf(m - lm, -200.0f);
+        const float f = m == -INFINITY ? 0.0f : ex2f(d * 1.4426950408889634f);
+        t = f * (t - d * (s + ties));
+        s = f * (s + ties);
+        ties = 0.0f;
+        m = max_nan(m, lm);
+      }
+#pragma unroll
+      for (int k = 0; k < kLpEach; ++k) {
+        if (v[k] == m) {
+          ties += 1.0f;
+        } else {
+          const float z = fmaxf(v[k] - m, -200.0f), e = ex2f(z * 1.4426950408889634f);
+          s += e;
+          t = fmaf(-z, e, t);
+        }
+      }
+    }
+    if constexpr (kTop) {
+      auto above = [&](int k) {                          // is logit k a candidate?
+        const int id = id_of(tile, k);
+        return !(v[k] < least_v) && id >= 0 && id < n && lp_key(v[k], id) > least;
+      };
+      int c = 0;
+      if (!(mine < least_v)) {
+#pragma unroll
+        for (int k = 0; k < kLpEach; ++k) c += above(k);
+      }
+      if (__syncthreads_or(c)) {
+        if (c) atomicAdd(&sh.more, c);
+        __syncthreads();
+        if (have + sh.more > kLpBuf) {
+          // too many: the 32nd largest of what is kept and of the threads' maxima bounds the
+          // row's 32nd largest from below, and at most 32 threads have logits above it
+          u64 w = have ? block_select(have, sh) : 0;
+          __syncthreads();
+          u64 best = 0;
+#pragma unroll
+          for (int k = 0; k < kLpEach; ++k)
+            if (above(k)) best = max64(best, lp_key(v[k], id_of(tile, k)));
+          const u64 b = block_merge(warp_sort(best), sh);
+          if (warp == 0) {
+            sh.buf[lane] = w;
+            w = warp_merge(w, b);
+            if (lane == top - 1) sh.lists[0][0] = w;
+            if (lane == 0) sh.count = have ? 32 : 0;
+          }
+          __syncthreads();
+          least = sh.lists[0][0];
+          least_v = least ? lp_key_value(least) : -INFINITY;
+          // the bound itself is a candidate
+          if (least) least -= 1;
+        }
+#pragma unroll
+        for (int k = 0; k < kLpEach; ++k)
+          if (above(k)) sh.buf[atomicAdd(&sh.count, 1)] = lp_key(v[k], id_of(tile, k));
+        __syncthreads();
+        have = sh.count;
+        if (threadIdx.x == 0) sh.more = 0;
+      }
+    }
+  }
+
+  // the warp's sums, then the CTA's
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long w = __shfl_xor_sync(0xFFFFFFFFu, v, o);
-    v = w > v ? w : v;
+    s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+    t += __shfl_xor_sync(0xFFFFFFFFu, t, o);
+    ties += __shfl_xor_sync(0xFFFFFFFFu, ties, o);
   }
+  if (lane == 0) sh.sums[warp] = LpSum{m, s + (ties - 1.0f), t};
+  u64 list = 0;
+  if constexpr (kTop) list = block_select(have, sh);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  for (int i = 0; i < (int)blockDim.x / 32; ++i) v = s[i] > v ? s[i] : v;
-  return v;
-}
-
-HV_DEV float block_sum(float v, float* s) {
+  if (warp > 0 && pieces == 1) return;
+  LpSum sum = lane < kLpWarps ? sh.sums[lane] : LpSum{-INFINITY, 0.f, 0.f};
+  auto warp_join = [&](LpSum a) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.0f;
-  for (int i = 0; i < (int)blockDim.x / 32; ++i) v += s[i];
-  return v;
+    for (int o = 16; o > 0; o >>= 1) {
+      const LpSum b{__shfl_xor_sync(0xFFFFFFFFu, a.m, o), __shfl_xor_sync(0xFFFFFFFFu, a.s, o),
+                    __shfl_xor_sync(0xFFFFFFFFu, a.t, o)};
+      a = lane & o ? lp_join(b, a) : lp_join(a, b);      // the same bits in every lane
+    }
+    return a;
+  };
+  if (warp == 0) sum = warp_join(sum);
+
+  if (pieces > 1) {
+    if (warp == 0) {
+      if (lane == 0) psum[(size_t)r * pieces + piece] = sum;
+      if (kTop && lane < top) plist[((size_t)r * pieces + piece) * kMaxTop + lane] = list;
+      __threadfence();
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      sh.last = atomicAdd(ticket + r, 1u) == (unsigned)pieces - 1;
+      if (sh.last) ticket[r] = 0;
+    }
+    __syncthreads();
+    if (!sh.last) return;
+    __threadfence();
+    if constexpr (kTop) {
+      for (int i = threadIdx.x; i < pieces * top; i += kLpThreads)
+        sh.buf[i] = __ldcg(plist + ((size_t)r * pieces + i / top) * kMaxTop + i % top);
+      __syncthreads();
+      list = block_select(pieces * top, sh);
+    }
+    if (warp > 0) return;
+    sum = LpSum{-INFINITY, 0.f, 0.f};
+    for (int i = lane; i < pieces; i += 32) {
+      const float* p = reinterpret_cast<const float*>(psum + (size_t)r * pieces + i);
+      sum = lp_join(sum, LpSum{__ldcg(p), __ldcg(p + 1), __ldcg(p + 2)});
+    }
+    sum = warp_join(sum);
+  }
+  const float nan = __int_as_float(0x7fc00000), ls = log1pf(sum.s);
+  const bool fine = fabsf(sum.m) <= FLT_MAX;             // not NaN, +inf, or all -inf
+  if (lane == 0) {
+    const int i = tok[r];
+    lp[r] = fine && i >= 0 && i < n ? (x[i] - sum.m) - ls : nan;
+    ent[r] = fine ? ls + sum.t / (1.0f + sum.s) : nan;
+  }
+  if (kTop && lane < top) {
+    const int id = (int)~(unsigned)list;
+    top_id[(size_t)r * top + lane] = id;
+    top_lp[(size_t)r * top + lane] = fine ? (x[id] - sum.m) - ls : nan;
+  }
 }
 
-__global__ void __launch_bounds__(512) k_logprob(const float* __restrict__ logits, size_t ld,
-                                                 int n, const int32_t* __restrict__ tok, int top,
-                                                 float* __restrict__ lp, float* __restrict__ ent,
-                                                 int32_t* __restrict__ top_id,
-                                                 float* __restrict__ top_lp) {
-  __shared__ unsigned long long s_k[16];
-  __shared__ float s_f[16];
-  const int r = blockIdx.x;
-  const float* x = logits + (size_t)r * ld;
-  unsigned long long best = 0;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const unsigned long long k = lp_key(x[i], i);
-    best = k > best ? k : best;
-  }
-  best = block_max64(best, s_k);
-  const int a = (int)~(unsigned)best;
-  const float m = x[a];
-  const bool fine = fabsf(m) <= FLT_MAX;       // not NaN, +inf, or all -inf
-  float S = 0.0f, T = 0.0f;
-  for (int i = threadIdx.x; i < n; i += blockDim.x) {
-    const float z = x[i] - m, e = expf(z);
-    if (i != a && e > 0.0f) { S += e; T -= z * e; }
-  }
-  S = block_sum(S, s_f);
-  T = block_sum(T, s_f);
-  const float nan = __int_as_float(0x7fc00000), ls = log1pf(S);
-  if (threadIdx.x == 0) {
-    const int t = tok[r];
-    lp[r] = fine && t >= 0 && t < n ? (x[t] - m) - ls : nan;
-    ent[r] = fine ? ls + T / (1.0f + S) : nan;
-  }
-  unsigned long long last = ~0ull;
-  for (int j = 0; j < top; ++j) {
-    unsigned long long b = 0;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-      const unsigned long long k = lp_key(x[i], i);
-      if (k < last && k > b) b = k;
-    }
-    last = block_max64(b, s_k);
-    if (threadIdx.x == 0) {
-      const int id = (int)~(unsigned)last;
-      top_id[(size_t)r * top + j] = id;
-      top_lp[(size_t)r * top + j] = fine ? (x[id] - m) - ls : nan;
-    }
-  }
+// CTAs per row: enough rows fill the SMs with one each; few rows are cut into pieces of whole
+// tiles.
+int lp_pieces(int rows, int n, int* out) {
+  int sms = 0;
+  const int rc = sm_count(&sms);
+  if (rc) return rc;
+  const int tiles = (int)(((long long)n + 3 + kLpTile - 1) / kLpTile);
+  int p = 4 * sms / rows;
+  p = p < tiles ? p : tiles;
+  p = p < kLpPieces ? p : kLpPieces;
+  *out = p < 1 || rows > kLpTickets ? 1 : p;
+  return HV_OK;
 }
+
+size_t lp_up(size_t b) { return (b + 255) & ~(size_t)255; }
 
 }  // namespace
 }  // namespace hv
@@ -110,7 +351,12 @@ extern "C" int hv_logprob_scratch(int rows, int n, int top, size_t* bytes) {
              "hv_logprob_scratch: bad arguments");
   HV_REQUIRE(top <= kMaxTop, HV_E_UNSUPPORTED, "hv_logprob_scratch: %d alternatives (at most %d)",
              top, kMaxTop);
-  *bytes = 256;
+  int pieces = 0;
+  const int rc = lp_pieces(rows, n, &pieces);
+  if (rc) return rc;
+  *bytes = kLpTickets * sizeof(unsigned) +
+           lp_up((size_t)rows * pieces * sizeof(LpSum)) +
+           (size_t)rows * pieces * (top ? kMaxTop : 0) * sizeof(u64);
   return HV_OK;
 }
 
@@ -121,10 +367,28 @@ extern "C" int hv_logprob_rows(const float* logits, long long ld, int rows, int 
                  (top == 0 || (top_id && top_lp)),
              HV_E_INVALID, "hv_logprob_rows: bad arguments");
   HV_REQUIRE(ld >= n, HV_E_INVALID, "hv_logprob_rows: row stride %lld under %d", ld, n);
+  HV_REQUIRE(n <= 1 << 30, HV_E_UNSUPPORTED, "hv_logprob_rows: %d tokens", n);
   HV_REQUIRE(top <= n, HV_E_INVALID, "hv_logprob_rows: %d alternatives of %d tokens", top, n);
   HV_REQUIRE(top <= kMaxTop, HV_E_UNSUPPORTED, "hv_logprob_rows: %d alternatives (at most %d)",
              top, kMaxTop);
-  k_logprob<<<rows, 512, 0, (cudaStream_t)stream>>>(logits, (size_t)ld, n, tok, top, lp, ent,
-                                                    top_id, top_lp);
+  HV_REQUIRE(((uintptr_t)logits & 3) == 0 && ((uintptr_t)scratch & 15) == 0, HV_E_INVALID,
+             "hv_logprob_rows: unaligned pointer");
+  int pieces = 0;
+  const int rc = lp_pieces(rows, n, &pieces);
+  if (rc) return rc;
+  HV_REQUIRE((long long)rows * pieces <= 0x7FFFFFFFll, HV_E_UNSUPPORTED,
+             "hv_logprob_rows: %d rows at once", rows);
+  uint8_t* p = static_cast<uint8_t*>(scratch);
+  unsigned* ticket = reinterpret_cast<unsigned*>(p);
+  p += kLpTickets * sizeof(unsigned);
+  LpSum* psum = reinterpret_cast<LpSum*>(p);
+  p += lp_up((size_t)rows * pieces * sizeof(LpSum));
+  u64* plist = reinterpret_cast<u64*>(p);
+  if (top)
+    k_logprob<true><<<rows * pieces, kLpThreads, 0, (cudaStream_t)stream>>>(
+        logits, (size_t)ld, n, tok, top, lp, ent, top_id, top_lp, pieces, psum, plist, ticket);
+  else
+    k_logprob<false><<<rows * pieces, kLpThreads, 0, (cudaStream_t)stream>>>(
+        logits, (size_t)ld, n, tok, top, lp, ent, top_id, top_lp, pieces, psum, plist, ticket);
   HV_LAUNCHED("k_logprob");
 }

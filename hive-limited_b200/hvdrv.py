@@ -622,26 +622,26 @@ def kv_q8_size(nkv, hd, cap) -> int:
 
 def kv_append_q8(k, v, kv, pos, nkv, hd, cap, stream=0):
     """One row per kv head at the device position *pos of an 8-bit cache."""
-    _call("hv_kv_append_q8", _p(k), _p(v), _p(kv), _p(pos), nkv, hd, cap, _p(stream))
+    _call("hv_kv_append_q8", int(k), int(v), int(kv), int(pos), nkv, hd, cap, int(stream))
 
 
 def kv_rows_q8(k, v, ld, kv, pos0, nkv, hd, cap, ntok, stream=0):
     """ntok rows at pos0 of an 8-bit cache; row t of k and v at t * ld floats."""
-    _call("hv_kv_rows_q8", _p(k), _p(v), int(ld), _p(kv), int(pos0), nkv, hd, cap, ntok,
-          _p(stream))
+    _call("hv_kv_rows_q8", int(k), int(v), int(ld), int(kv), int(pos0), nkv, hd, cap, ntok,
+          int(stream))
 
 
 def qk_rows_q8(qkv, qn, kn, cos_t, sin_t, pos0, q_out, kv, nq, nkv, hd, cap, eps, ntok,
                stream=0):
     """qk_rows (head norms, RoPE, append) over an 8-bit cache."""
-    _call("hv_qk_rows_q8", _p(qkv), _p(qn), _p(kn), _p(cos_t), _p(sin_t), int(pos0), _p(q_out),
-          _p(kv), nq, nkv, hd, cap, C.c_float(eps), ntok, _p(stream))
+    _call("hv_qk_rows_q8", int(qkv), int(qn), int(kn), int(cos_t), int(sin_t), int(pos0), int(q_out),
+          int(kv), nq, nkv, hd, cap, C.c_float(eps), ntok, int(stream))
 
 
 def kv_read_q8(kv, k_out, v_out, pos0, nkv, hd, cap, ntok, stream=0):
     """Positions pos0 .. pos0 + ntok - 1 of an 8-bit cache as f32 rows [ntok][nkv][hd]."""
-    _call("hv_kv_read_q8", _p(kv), _p(k_out), _p(v_out), int(pos0), nkv, hd, cap, ntok,
-          _p(stream))
+    _call("hv_kv_read_q8", int(kv), int(k_out), int(v_out), int(pos0), nkv, hd, cap, ntok,
+          int(stream))
 
 
 def attn_q8_scratch(nq, group, cap, ntok=1) -> int:
@@ -653,14 +653,14 @@ def attn_q8_scratch(nq, group, cap, ntok=1) -> int:
 
 def attn_decode_q8(q, kv, ctx, scale, pos, nq, hd, group, cap, scratch, stream=0):
     """Decode attention over positions 0 .. *pos of an 8-bit cache."""
-    _call("hv_attn_decode_q8", _p(q), _p(kv), _p(ctx), _p(scale), _p(pos), nq, hd, group, cap,
-          _p(scratch), _p(stream))
+    _call("hv_attn_decode_q8", int(q), int(kv), int(ctx), int(scale), int(pos), nq, hd, group, cap,
+          int(scratch), int(stream))
 
 
 def attn_rows_q8(q, kv, ctx, scale, pos0, nq, hd, group, cap, ntok, scratch, stream=0):
     """Attention of ntok query rows over an 8-bit cache, row t over positions 0 .. pos0 + t."""
-    _call("hv_attn_rows_q8", _p(q), _p(kv), _p(ctx), _p(scale), int(pos0), nq, hd, group, cap,
-          ntok, _p(scratch), _p(stream))
+    _call("hv_attn_rows_q8", int(q), int(kv), int(ctx), int(scale), int(pos0), nq, hd, group, cap,
+          ntok, int(scratch), int(stream))
 
 
 def logprob_scratch(rows, n, top=0) -> int:
@@ -673,8 +673,8 @@ def logprob_scratch(rows, n, top=0) -> int:
 def logprob_rows(logits, ld, rows, n, tok, top, lp, ent, top_id, top_lp, scratch, stream=0):
     """Log probabilities of given tokens, entropies and the `top` most likely tokens of rows
     of logits (hv_logprob_rows)."""
-    _call("hv_logprob_rows", _p(logits), int(ld), rows, n, _p(tok), top, _p(lp), _p(ent),
-          _p(top_id), _p(top_lp), _p(scratch), _p(stream))
+    _call("hv_logprob_rows", int(logits), int(ld), rows, n, int(tok), top, int(lp), int(ent),
+          int(top_id), int(top_lp), int(scratch), int(stream))
 
 
 def silu_rows(gu, act, ffn, ntok, stream=0):

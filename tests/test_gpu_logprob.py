@@ -191,3 +191,26 @@ def test_engine_score(hv, kv):
             e.score(ids, top=33)
     finally:
         e.free()
+
+
+def test_one_scratch_for_calls_of_different_sizes(hv):
+    """The scratch of the largest call serves any smaller one in any order."""
+    g = np.random.default_rng(9)
+    s = Dev(nbytes=max(hv.logprob_scratch(r, 30000, 32) for r in (1, 2, 100, 290)))
+    for rows in (100, 2, 290, 1, 100, 290):
+        x = g.standard_normal((rows, 30000)).astype(F32)
+        tok = g.integers(0, 30000, rows)
+        check(call(hv, x, tok, 32, scratch=s), x, tok, 32)
+
+
+@pytest.mark.parametrize("order", ["up", "down", "saw", "late"])
+def test_orders_that_keep_bringing_larger_logits(hv, order):
+    n = 50000
+    x = np.linspace(-30, 30, n).astype(F32)[None].repeat(2, 0)
+    if order == "down":
+        x = x[:, ::-1].copy()
+    if order == "saw":
+        x = x + 20 * (np.arange(n) % 4096 / 4096).astype(F32)
+    if order == "late":
+        x[:, :-40] = 0
+    check(call(hv, x, [5, n - 1], 32), x, np.array([5, n - 1]), 32)
