@@ -13,73 +13,6 @@
 namespace hv {
 namespace {
 
-// One CTA per (query head, query row); its warps take positions in turn, a lane four dims.
-__global__ void __launch_bounds__(128) k_attn_q8(const float* __restrict__ q, KvQ8 c,
-                                                 float* __restrict__ ctx,
-                                                 const float* __restrict__ scale,
-                                                 const int32_t* __restrict__ pos_p, int pos0,
-                                                 int nq, int group) {
-  __shared__ float s_m[4], s_l[4];
-  __shared__ float4 s_acc[4][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.x, g = h / group;
-  const int pos = pos_p ? *pos_p : pos0 + (int)blockIdx.y;
-  const size_t row = ((size_t)blockIdx.y * nq + h) * kHd;
-  const int held = q8_held(c, g);
-  if (pos < 0 || pos >= held) {
-    ctx[row + threadIdx.x] = __int_as_float(0x7fc00000);
-    return;
-  }
-  const float4 qv = __ldg(reinterpret_cast<const float4*>(q + row) + lane);
-  const float sc = __ldg(scale) * kLog2e;
-  float m = -INFINITY, l = 0.0f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p = warp; p <= pos; p += 4) {
-    const int blk = p / kQ8Blk, r = p % kQ8Blk;
-    float4 k, v;
-    if ((blk + 1) * kQ8Blk <= held) {
-      const uint8_t* kc = c.codes + ((size_t)g * c.nblk + blk) * 2 * kQ8Codes;
-      const float2 s = __ldg(reinterpret_cast<const float2*>(c.scales) + (size_t)g * c.nblk + blk);
-      float kk[4], vv[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        kk[e] = q8_value(__ldg(kc + q8_k_at(r, 4 * lane + e)), s.x);
-        vv[e] = q8_value(__ldg(kc + kQ8Codes + q8_v_at(r, 4 * lane + e)), s.y);
-      }
-      k = make_float4(kk[0], kk[1], kk[2], kk[3]);
-      v = make_float4(vv[0], vv[1], vv[2], vv[3]);
-    } else {
-      const float4* t = reinterpret_cast<const float4*>(c.tail + (size_t)g * 2 * kQ8Codes);
-      k = __ldg(t + r * (kHd / 4) + lane);
-      v = __ldg(t + kQ8Codes / 4 + r * (kHd / 4) + lane);
-    }
-    float x = qv.x * k.x + qv.y * k.y + qv.z * k.z + qv.w * k.w;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
-    x *= sc;
-    const float m1 = fmaxf(m, x);
-    const float a = exp2f(m - m1), w = exp2f(x - m1);
-    m = m1;
-    l = l * a + w;
-    acc.x = acc.x * a + w * v.x;
-    acc.y = acc.y * a + w * v.y;
-    acc.z = acc.z * a + w * v.z;
-    acc.w = acc.w * a + w * v.w;
-  }
-  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
-  s_acc[warp][lane] = acc;
-  __syncthreads();
-  const float mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  float num = 0.0f, den = 0.0f;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    const float a = s_l[w] == 0.0f ? 0.0f : exp2f(s_m[w] - mx);
-    den += a * s_l[w];
-    num += a * reinterpret_cast<const float*>(s_acc[w])[threadIdx.x];
-  }
-  ctx[row + threadIdx.x] = num / den;
-}
-
 // ---- one query token ------------------------------------------------------------------
 //
 // Bound by the bytes of the cache for long contexts and by latency for short ones: the
@@ -433,6 +366,444 @@ int dec_chunks(int nkv, int cap, int* out) {
   return HV_OK;
 }
 
+// ---- a run of query tokens ------------------------------------------------------------
+//
+// The rows of a kv head are its (token, head of the group) pairs; a CTA takes 16 kWM of them
+// and a chunk of the positions. Its eight warps stand as kWM groups of 16 rows by 8 / kWM
+// shares of the chunk's blocks: few rows spread over the positions, many share each block.
+// Here the rows are the 16-row operand: S = q K^T and ctx += w V, both terms of q (of w) into
+// the same sums. The open block's f32 rows become two binary16 terms as well, so that it is
+// a block like the others with a third product, hi x lo.
+constexpr int kRowWarps = 8;
+
+template <int kWM>
+struct RowsCfg {
+  static constexpr int kShares = kRowWarps / kWM;
+  static constexpr int kRows = 16 * kWM;
+  static constexpr int kStages = kShares == 8 ? 2 : 3;
+  static constexpr int kRing = kShares * kStages * 2 * kQ8Codes;
+  static constexpr int kMerge = kShares > 1 ? kRowWarps * 16 * (kHd + 4) * 4 : 0;
+  static constexpr int kTail = 4 * kQ8Codes * 2;          // K hi, K lo, V hi, V lo
+  static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kTail;
+};
+
+struct RowsArgs {
+  const float* q;
+  float* ctx;
+  const float* scale;
+  int pos0, ntok, nq, group, chunks;
+  float* part;
+  unsigned* ticket;
+};
+
+// Floats of the scratch per (row tile of n rows, chunk): their sums, then (max, sum).
+HV_HD size_t rows_part(int n) { return (size_t)n * (kHd + 2); }
+
+template <int kWM>
+__global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, KvQ8 c) {
+  using Cfg = RowsCfg<kWM>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float s_m[kRowWarps][16], s_l[kRowWarps][16], s_amax[2];
+  __shared__ int s_bad;
+  __shared__ unsigned s_last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
+  const int wm = warp % kWM, share = warp / kWM;
+  const int kvh = blockIdx.y, tile = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
+  const int nrows = a.ntok * a.group, row0 = tile * Cfg::kRows;
+  const int last_row = min(nrows, row0 + Cfg::kRows) - 1;
+  const int held = q8_held(c, kvh), closed = held / kQ8Blk;
+  const int top = min(a.pos0 + last_row / a.group, held - 1);     // the last position to read
+  const int nb = min(closed, top < 0 ? 0 : top / kQ8Blk + 1);
+  const bool tail = top >= closed * kQ8Blk;
+  const int items = nb + (tail ? 1 : 0);
+  const int nact = max(1, min(a.chunks, items / 2));
+  if (chunk >= nact) return;
+  const int b0 = (int)((long long)items * chunk / nact);
+  const int b1 = (int)((long long)items * (chunk + 1) / nact);
+  const int c1 = min(b1, nb);                       // blocks b0 .. c1 from codes, then the tail
+
+  // this warp's two rows per lane
+  const int r0 = row0 + 16 * wm + gl, r1 = r0 + 8;
+  const int lim0 = r0 < nrows ? min(a.pos0 + r0 / a.group, held - 1) : -1;
+  const int lim1 = r1 < nrows ? min(a.pos0 + r1 / a.group, held - 1) : -1;
+  const int warp_last = min(row0 + 16 * wm + 15, nrows - 1);
+  const int warp_first = row0 + 16 * wm;
+  const int warp_top = warp_first < nrows ? a.pos0 + warp_last / a.group : -1;
+  const int warp_low = warp_first < nrows ? min(a.pos0 + warp_first / a.group, held - 1) : -1;
+
+  uint8_t* ring = smem + (size_t)share * Cfg::kStages * 2 * kQ8Codes;
+  const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring) + 16 * lane;
+  const uint8_t* codes = c.codes + (size_t)kvh * c.nblk * 2 * kQ8Codes + 16 * lane;
+  const float2* scales = reinterpret_cast<const float2*>(c.scales) + (size_t)kvh * c.nblk;
+  auto fetch = [&](int b, int stage) {
+    if (b < c1) {
+      const uint8_t* src = codes + (size_t)b * 2 * kQ8Codes;
+#pragma unroll
+      for (int u = wm; u < 16; u += kWM)
+        cp_async16(ring_s + stage * 2 * kQ8Codes + 512 * u, src + 512 * u);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto share_sync = [&] {
+    if constexpr (kWM == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" :: "r"(1 + share), "n"(32 * kWM) : "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < Cfg::kStages; ++i) fetch(b0 + share + i * Cfg::kShares, i);
+
+  uint32_t qh[8][4], ql[8][4];
+  float qs0, qs1;
+  {
+    const float qscale = __ldg(a.scale) * kLog2e;
+    auto row_ptr = [&](int r) {
+      return a.q + (((size_t)(r / a.group)) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd;
+    };
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = half ? r1 : r0;
+      float4 x[8];
+      float amax = 0.0f;
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        x[s] = r < nrows ? __ldg(reinterpret_cast<const float4*>(row_ptr(r) + 16 * s + 4 * t))
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
+        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[s].x), fabsf(x[s].y))),
+                     fmaxf(fabsf(x[s].z), fabsf(x[s].w)));
+      }
+      amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
+      const float lift = q8_lift(amax);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        split_half2(x[s].x * lift, x[s].y * lift, &qh[s][half], &ql[s][half]);
+        split_half2(x[s].z * lift, x[s].w * lift, &qh[s][2 + half], &ql[s][2 + half]);
+      }
+      (half ? qs1 : qs0) = qscale / lift;
+    }
+  }
+
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+  float acc[16][4];
+#pragma unroll
+  for (int d = 0; d < 16; ++d) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0.0f;
+
+  // scores of block b in s (position 32 b + 8 j + 2 t + e: s[j][e] of row r0, s[j][2 + e] of
+  // r1), already sums of products; f0, f1 make them exponents of 2. Leaves the weights as A
+  // fragments of the second product.
+  uint32_t wh[2][4], wl[2][4];
+  auto weights = [&](int b, float (&s)[4][4], float f0, float f1) {
+    const bool cut = 32 * b + 31 > warp_low;
+    float y0 = -INFINITY, y1 = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        s[j][e] *= f0;
+        s[j][2 + e] *= f1;
+        if (cut) {
+          const int p = 32 * b + 8 * j + 2 * t + e;
+          if (p > lim0) s[j][e] = -INFINITY;
+          if (p > lim1) s[j][2 + e] = -INFINITY;
+        }
+        y0 = fmaxf(y0, s[j][e]);
+        y1 = fmaxf(y1, s[j][2 + e]);
+      }
+    }
+    y0 = fmaxf(y0, __shfl_xor_sync(0xFFFFFFFFu, y0, 1));
+    y1 = fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, 1));
+    y0 = fmaxf(m0, fmaxf(y0, __shfl_xor_sync(0xFFFFFFFFu, y0, 2)));
+    y1 = fmaxf(m1, fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, 2)));
+    if (__any_sync(0xFFFFFFFFu, y0 > m0 || y1 > m1)) {
+      const float a0 = m0 == -INFINITY ? 0.0f : ex2(m0 - y0);
+      const float a1 = m1 == -INFINITY ? 0.0f : ex2(m1 - y1);
+      m0 = y0; m1 = y1;
+      l0 *= a0; l1 *= a1;
+#pragma unroll
+      for (int d = 0; d < 16; ++d) { acc[d][0] *= a0; acc[d][1] *= a0; acc[d][2] *= a1; acc[d][3] *= a1; }
+    }
+    // a row that sees none of the positions so far keeps m = -inf and weights of 0
+    const float n0 = m0 == -INFINITY ? 0.0f : m0, n1 = m1 == -INFINITY ? 0.0f : m1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float p[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        p[e] = ex2(s[j][e] - n0) * 32768.0f;
+        p[2 + e] = ex2(s[j][2 + e] - n1) * 32768.0f;
+        l0 += p[e];
+        l1 += p[2 + e];
+      }
+      // A fragment: (row g, k 2t), (row g + 8, k 2t), (row g, k 2t + 8), (row g + 8, k 2t + 8)
+      split_half2(p[0], p[1], &wh[j >> 1][2 * (j & 1)], &wl[j >> 1][2 * (j & 1)]);
+      split_half2(p[2], p[3], &wh[j >> 1][2 * (j & 1) + 1], &wl[j >> 1][2 * (j & 1) + 1]);
+    }
+  };
+
+  int stage = 0;
+  for (int b = b0 + share; b < c1; b += Cfg::kShares) {
+    asm volatile("cp.async.wait_group %0;" :: "n"(Cfg::kStages - 1) : "memory");
+    share_sync();
+    if (32 * b <= warp_top) {
+      const float2 sc = __ldg(scales + b);
+      const uint8_t* blk = ring + stage * 2 * kQ8Codes + 16 * lane;
+      float s[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 x = *reinterpret_cast<const uint4*>(blk + 512 * (2 * j + h));
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t k0, k1;
+            q8_halves(w[k], &k0, &k1);
+            mma_f16(s[j], qh[4 * h + k], k0, k1);
+            mma_f16(s[j], ql[4 * h + k], k0, k1);
+          }
+        }
+      }
+      weights(b, s, sc.x * qs0, sc.x * qs1);
+      // a row that sees nothing of the block takes nothing from it, whatever its scale
+      const float f0 = 32 * b <= lim0 ? sc.y : 0.0f, f1 = 32 * b <= lim1 ? sc.y : 0.0f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const uint4 x = *reinterpret_cast<const uint4*>(blk + kQ8Codes + 512 * u);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint32_t v0, v1;
+            q8_halves(w[2 * h + k], &v0, &v1);
+            mma_f16(d, wh[k], v0, v1);
+            mma_f16(d, wl[k], v0, v1);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            acc[2 * u + h][i] = fmaf(d[i], i < 2 ? f0 : f1, acc[2 * u + h][i]);
+        }
+      }
+    }
+    share_sync();
+    fetch(b + Cfg::kStages * Cfg::kShares, stage);
+    stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
+  }
+
+  if (tail && b1 == items) {
+    // the open rows as fragments in two terms; rows past the last one held are zero, and so
+    // are values that are not finite, whose weight of 0 for the rows that do not see them
+    // would not be nothing: the rows that see one get a sum of NaN instead
+    __half* frag = reinterpret_cast<__half*>(smem + Cfg::kSmem - Cfg::kTail);
+    const int n = min(held - closed * kQ8Blk, kQ8Blk);
+    const float* src = c.tail + (size_t)kvh * 2 * kQ8Codes;
+    if (threadIdx.x < 2) s_amax[threadIdx.x] = 0.0f;
+    if (threadIdx.x == 0) s_bad = kQ8Blk;
+    __syncthreads();
+    for (int which = 0; which < 2; ++which) {
+      float amax = 0.0f;
+      for (int i = threadIdx.x; i < n * kHd; i += blockDim.x) {
+        const float x = fabsf(__ldg(src + which * kQ8Codes + i));
+        if (x < INFINITY) amax = fmaxf(amax, x);
+        else atomicMin(&s_bad, i / kHd);
+      }
+      atomicMax(reinterpret_cast<int*>(&s_amax[which]), __float_as_int(amax));
+    }
+    __syncthreads();
+    const float lk = q8_lift(s_amax[0]), lv = q8_lift(s_amax[1]);
+    for (int i = threadIdx.x; i < 2 * kQ8Codes; i += blockDim.x) {
+      const int which = i / kQ8Codes, r = i % kQ8Codes / kHd, d = i % kHd;
+      float x = r < n ? __ldg(src + i) * (which ? lv : lk) : 0.0f;
+      if (!(fabsf(x) < INFINITY)) x = 0.0f;
+      const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
+      const int at = which ? q8_v_at(r, d) : q8_k_at(r, d);
+      frag[(2 * which) * kQ8Codes + at] = hi;
+      frag[(2 * which + 1) * kQ8Codes + at] = lo;
+    }
+    __syncthreads();
+    if (share == 0 && 32 * closed <= warp_top) {
+      // 16 halves of a unit: the 16 bytes of a coded one
+      auto word2 = [&](int part, int u, int w) {
+        return *reinterpret_cast<const uint2*>(frag + part * kQ8Codes + 512 * u + 16 * lane + 4 * w);
+      };
+      float s[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint2 kh = word2(0, 2 * j + (k >> 2), k & 3), kl = word2(1, 2 * j + (k >> 2), k & 3);
+          mma_f16(s[j], qh[k], kh.x, kh.y);
+          mma_f16(s[j], ql[k], kh.x, kh.y);
+          mma_f16(s[j], qh[k], kl.x, kl.y);
+        }
+      }
+      weights(closed, s, qs0 / lk, qs1 / lk);
+      const float f = 1.0f / lv;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint2 vh = word2(2, u, 2 * h + k), vl = word2(3, u, 2 * h + k);
+            mma_f16(d, wh[k], vh.x, vh.y);
+            mma_f16(d, wl[k], vh.x, vh.y);
+            mma_f16(d, wh[k], vl.x, vl.y);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[2 * u + h][i] = fmaf(d[i], f, acc[2 * u + h][i]);
+        }
+      }
+      if (lim0 >= closed * kQ8Blk + s_bad) l0 = __int_as_float(0x7fc00000);
+      if (lim1 >= closed * kQ8Blk + s_bad) l1 = __int_as_float(0x7fc00000);
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 4; o <<= 1) {
+    l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, o);
+    l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, o);
+  }
+
+  // the shares meet in share 0
+  if constexpr (Cfg::kShares > 1) {
+    if (t == 0) {
+      s_m[warp][gl] = m0; s_m[warp][gl + 8] = m1;
+      s_l[warp][gl] = l0; s_l[warp][gl + 8] = l1;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    float M0 = -INFINITY, M1 = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < Cfg::kShares; ++w) {
+      M0 = fmaxf(M0, s_m[w * kWM + wm][gl]);
+      M1 = fmaxf(M1, s_m[w * kWM + wm][gl + 8]);
+    }
+    const float a0 = l0 == 0.0f ? 0.0f : ex2(m0 - M0), a1 = l1 == 0.0f ? 0.0f : ex2(m1 - M1);
+    float* red = reinterpret_cast<float*>(smem) + (size_t)warp * 16 * (kHd + 4);
+    if (share > 0) {
+#pragma unroll
+      for (int d = 0; d < 16; ++d) {
+        *reinterpret_cast<float2*>(red + gl * (kHd + 4) + 8 * d + 2 * t) =
+            make_float2(acc[d][0] * a0, acc[d][1] * a0);
+        *reinterpret_cast<float2*>(red + (gl + 8) * (kHd + 4) + 8 * d + 2 * t) =
+            make_float2(acc[d][2] * a1, acc[d][3] * a1);
+      }
+    }
+    __syncthreads();
+    if (share == 0) {
+#pragma unroll
+      for (int d = 0; d < 16; ++d) { acc[d][0] *= a0; acc[d][1] *= a0; acc[d][2] *= a1; acc[d][3] *= a1; }
+      l0 *= a0;
+      l1 *= a1;
+      for (int w = 1; w < Cfg::kShares; ++w) {
+        const float* o = reinterpret_cast<const float*>(smem) + (size_t)(w * kWM + wm) * 16 * (kHd + 4);
+        const float v0 = s_l[w * kWM + wm][gl], v1 = s_l[w * kWM + wm][gl + 8];
+        l0 += v0 == 0.0f ? 0.0f : v0 * ex2(s_m[w * kWM + wm][gl] - M0);
+        l1 += v1 == 0.0f ? 0.0f : v1 * ex2(s_m[w * kWM + wm][gl + 8] - M1);
+#pragma unroll
+        for (int d = 0; d < 16; ++d) {
+          const float2 x = *reinterpret_cast<const float2*>(o + gl * (kHd + 4) + 8 * d + 2 * t);
+          const float2 y = *reinterpret_cast<const float2*>(o + (gl + 8) * (kHd + 4) + 8 * d + 2 * t);
+          acc[d][0] += x.x; acc[d][1] += x.y; acc[d][2] += y.x; acc[d][3] += y.y;
+        }
+      }
+      m0 = M0;
+      m1 = M1;
+    }
+  }
+
+  auto ctx_row = [&](int r) {
+    return a.ctx + (((size_t)(r / a.group)) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd;
+  };
+  auto not_held = [&](int r) { return a.pos0 + r / a.group >= held; };
+  const float nan = __int_as_float(0x7fc00000);
+  if (nact == 1) {
+    if (share == 0) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = half ? r1 : r0;
+        if (r >= nrows) continue;
+        const float inv = not_held(r) ? nan : 1.0f / (half ? l1 : l0);
+        float* o = ctx_row(r) + 2 * t;
+#pragma unroll
+        for (int d = 0; d < 16; ++d)
+          *reinterpret_cast<float2*>(o + 8 * d) =
+              make_float2(acc[d][2 * half] * inv, acc[d][2 * half + 1] * inv);
+      }
+    }
+    return;
+  }
+  // the chunks meet in the scratch; the last CTA to arrive adds them in order
+  const int ntile = gridDim.x / a.chunks;
+  const size_t slot = ((size_t)kvh * ntile + tile) * a.chunks;
+  float* mine = a.part + (slot + chunk) * rows_part(Cfg::kRows);
+  if (share == 0) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = 16 * wm + gl + 8 * half;
+      float* o = mine + (size_t)r * kHd + 2 * t;
+#pragma unroll
+      for (int d = 0; d < 16; ++d)
+        *reinterpret_cast<float2*>(o + 8 * d) = make_float2(acc[d][2 * half], acc[d][2 * half + 1]);
+      if (t == 0)
+        *reinterpret_cast<float2*>(mine + (size_t)Cfg::kRows * kHd + 2 * r) =
+            half ? make_float2(m1, l1) : make_float2(m0, l0);
+    }
+    __threadfence();
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    unsigned* tk = a.ticket + (size_t)kvh * ntile + tile;
+    s_last = atomicAdd(tk, 1u) == (unsigned)nact - 1;
+    if (s_last) *tk = 0;
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  const float* base = a.part + slot * rows_part(Cfg::kRows);
+  for (int i = threadIdx.x; i < Cfg::kRows * (kHd / 4); i += blockDim.x) {
+    const int r = i / (kHd / 4), d4 = i % (kHd / 4);
+    if (row0 + r >= nrows) break;
+    float M = -INFINITY, L = 0.0f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < nact; ++k)
+      M = fmaxf(M, __ldcg(base + k * rows_part(Cfg::kRows) + Cfg::kRows * kHd + 2 * r));
+    for (int k = 0; k < nact; ++k) {
+      const float* p = base + k * rows_part(Cfg::kRows);
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + Cfg::kRows * kHd + 2 * r));
+      if (ml.y == 0.0f) continue;                 // this row sees nothing of the chunk
+      const float w = ex2(ml.x - M);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(p + (size_t)r * kHd) + d4);
+      L += w * ml.y;
+      A.x += w * x.x; A.y += w * x.y; A.z += w * x.z; A.w += w * x.w;
+    }
+    const float inv = not_held(row0 + r) ? nan : 1.0f / L;
+    reinterpret_cast<float4*>(ctx_row(row0 + r))[d4] =
+        make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
+  }
+}
+
+// Rows per CTA and chunks per row tile of a run: 16 rows at a time up to 128, and as many
+// chunks as leave no SM without a CTA, of two blocks or more.
+struct RowsPlan {
+  int rows, tiles, chunks;
+};
+int rows_plan(int nkv, int group, int cap, int ntok, RowsPlan* p) {
+  int sms = 0;
+  const int rc = sm_count(&sms);
+  if (rc) return rc;
+  const long long n = (long long)ntok * group;
+  p->rows = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128;
+  p->tiles = (int)((n + p->rows - 1) / p->rows);
+  const long long ctas = (long long)p->tiles * nkv;
+  const int most = std::max(1, (cap + kQ8Blk - 1) / kQ8Blk / 2);
+  p->chunks = ctas > kDecTickets ? 1 : (int)std::max(1ll, std::min((long long)most, sms / ctas));
+  return HV_OK;
+}
+
 int attn_q8_check(const char* name, const float* q, const void* kv, const float* ctx,
                   const float* scale, int nq, int hd, int group, int cap, const void* scratch) {
   HV_REQUIRE(q && kv && ctx && scale && scratch && nq > 0 && group > 0 && cap > 0, HV_E_INVALID,
@@ -460,7 +831,12 @@ extern "C" int hv_attn_q8_scratch(int nq, int group, int cap, int ntok, size_t* 
   int nch = 0;
   const int rc = dec_chunks(nq / group, cap, &nch);
   if (rc) return rc;
-  *bytes = kDecTickets * sizeof(unsigned) + (size_t)(nq / group) * nch * kDecPart * sizeof(float);
+  RowsPlan p;
+  const int rc2 = rows_plan(nq / group, group, cap, ntok, &p);
+  if (rc2) return rc2;
+  const size_t dec = (size_t)(nq / group) * nch * kDecPart;
+  const size_t rows = p.chunks > 1 ? (size_t)(nq / group) * p.tiles * p.chunks * rows_part(p.rows) : 0;
+  *bytes = kDecTickets * sizeof(unsigned) + std::max(dec, rows) * sizeof(float);
   return HV_OK;
 }
 
@@ -503,7 +879,24 @@ extern "C" int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const
   HV_REQUIRE(ntok <= 65535, HV_E_UNSUPPORTED, "hv_attn_rows_q8: %d rows at once", ntok);
   KvQ8 c;
   kv_q8_view(const_cast<void*>(kv), nq / group, cap, &c);
-  k_attn_q8<<<dim3(nq, ntok), 128, 0, (cudaStream_t)stream>>>(q, c, ctx, scale, nullptr, pos0, nq,
-                                                              group);
-  HV_LAUNCHED("k_attn_q8");
+  RowsPlan p;
+  const int rc2 = rows_plan(nq / group, group, cap, ntok, &p);
+  if (rc2) return rc2;
+  RowsArgs a{q, ctx, scale, pos0, ntok, nq, group, p.chunks,
+             reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) +
+                                      kDecTickets * sizeof(unsigned)),
+             static_cast<unsigned*>(scratch)};
+  const dim3 grid((unsigned)(p.tiles * p.chunks), (unsigned)(nq / group));
+#define HV_ROWS(WM)                                                                        \
+  {                                                                                        \
+    const int rc3 = smem_attr((const void*)k_attn_rows_q8<WM>, RowsCfg<WM>::kSmem);        \
+    if (rc3) return rc3;                                                                   \
+    k_attn_rows_q8<WM><<<grid, 32 * kRowWarps, RowsCfg<WM>::kSmem, (cudaStream_t)stream>>>(a, c); \
+  }
+  if (p.rows == 16) HV_ROWS(1)
+  else if (p.rows == 32) HV_ROWS(2)
+  else if (p.rows == 64) HV_ROWS(4)
+  else HV_ROWS(8)
+#undef HV_ROWS
+  HV_LAUNCHED("k_attn_rows_q8");
 }

@@ -348,6 +348,31 @@ def test_a_poisoned_block_poisons_what_reads_it(hv):
     assert np.isfinite(got[:2]).all() and np.isnan(got[2:]).all()
 
 
+def test_open_rows_that_are_not_finite_reach_only_who_sees_them(hv):
+    """Rows of the open block stay f32: a NaN or infinity in one is seen from its position on."""
+    nkv, group, cap, n = 1, 4, 128, 60
+    g = np.random.default_rng(16)
+    k, v = rows(g, n, nkv, 0.3)
+    v[45, 0, 7], k[50, 0, 9], v[58, 0, 0] = np.inf, np.nan, np.nan
+    ref, sc = R.Cache(nkv, cap), Dev(np.array([SCALE]))
+    ref.write(k, v, 0)
+    kv = Dev(ref.buffer(0xFF))
+    q = g.standard_normal((30, 4, HD)).astype(F32)
+    out, s = Dev(np.zeros((30, 4, HD), F32)), scratch(hv, 4, group, cap, 30)
+    hv.attn_rows_q8(Dev(q), kv, out, sc, 30, 4, HD, group, cap, 30, s)
+    got = out.get(F32, (30, 4, HD))
+    for t in (0, 1, 2, 14):
+        near(got[t], *R.attention(q[t], ref.val, 30 + t, group, float(SCALE)))
+    for t in range(15, 30):
+        assert not np.isfinite(got[t][:, 7]).any()
+        assert t < 20 or np.isnan(got[t]).all()
+    one = Dev(np.zeros((4, HD), F32))
+    for pos, lost in ((44, False), (45, True), (59, True)):
+        hv.attn_decode_q8(Dev(q[0]), kv, one, sc, i32(pos), 4, HD, group, cap, s)
+        x = one.get(F32, (4, HD))
+        assert (not np.isfinite(x[:, 7]).any()) if lost else np.isfinite(x).all(), pos
+
+
 def test_captured_decode_follows_the_device_position(hv):
     """Append and attention captured once, replayed while *pos moves over block edges, equal
     to direct calls; two graphs with a scratch each, on two streams."""
