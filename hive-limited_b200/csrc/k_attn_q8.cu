@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "attn_q8.cuh"
+#include "attn_q8_rows.h"
 #include "hv_internal.h"
 
 namespace hv {
@@ -387,18 +388,6 @@ struct RowsCfg {
   static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kTail;
 };
 
-struct RowsArgs {
-  const float* q;
-  float* ctx;
-  const float* scale;
-  int pos0, ntok, nq, group, chunks;
-  float* part;
-  unsigned* ticket;
-};
-
-// Floats of the scratch per (row tile of n rows, chunk): their sums, then (max, sum).
-HV_HD size_t rows_part(int n) { return (size_t)n * (kHd + 2); }
-
 template <int kWM>
 __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, KvQ8 c) {
   using Cfg = RowsCfg<kWM>;
@@ -763,27 +752,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  const float* base = a.part + slot * rows_part(Cfg::kRows);
-  for (int i = threadIdx.x; i < Cfg::kRows * (kHd / 4); i += blockDim.x) {
-    const int r = i / (kHd / 4), d4 = i % (kHd / 4);
-    if (row0 + r >= nrows) break;
-    float M = -INFINITY, L = 0.0f;
-    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < nact; ++k)
-      M = fmaxf(M, __ldcg(base + k * rows_part(Cfg::kRows) + Cfg::kRows * kHd + 2 * r));
-    for (int k = 0; k < nact; ++k) {
-      const float* p = base + k * rows_part(Cfg::kRows);
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(p + Cfg::kRows * kHd + 2 * r));
-      if (ml.y == 0.0f) continue;                 // this row sees nothing of the chunk
-      const float w = ex2(ml.x - M);
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(p + (size_t)r * kHd) + d4);
-      L += w * ml.y;
-      A.x += w * x.x; A.y += w * x.y; A.z += w * x.z; A.w += w * x.w;
-    }
-    const float inv = not_held(row0 + r) ? nan : 1.0f / L;
-    reinterpret_cast<float4*>(ctx_row(row0 + r))[d4] =
-        make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
-  }
+  rows_join<Cfg::kRows>(a, kvh, slot, nact, row0, nrows, held);
 }
 
 // Rows per CTA and chunks per row tile of a run: 16 rows at a time up to 128, and as many
@@ -799,7 +768,7 @@ int rows_plan(int nkv, int group, int cap, int ntok, RowsPlan* p) {
   p->rows = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128;
   p->tiles = (int)((n + p->rows - 1) / p->rows);
   const long long ctas = (long long)p->tiles * nkv;
-  const int most = std::max(1, (cap + kQ8Blk - 1) / kQ8Blk / 2);
+  const int most = std::max(1, (cap + kQ8Blk - 1) / kQ8Blk / (p->rows == 128 ? 8 : 2));
   p->chunks = ctas > kDecTickets ? 1 : (int)std::max(1ll, std::min((long long)most, sms / ctas));
   return HV_OK;
 }
@@ -896,7 +865,9 @@ extern "C" int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const
   if (p.rows == 16) HV_ROWS(1)
   else if (p.rows == 32) HV_ROWS(2)
   else if (p.rows == 64) HV_ROWS(4)
-  else HV_ROWS(8)
+  else
+    return attn_tile_q8_launch(a, c, (unsigned)p.tiles, (unsigned)(nq / group),
+                               (cudaStream_t)stream);
 #undef HV_ROWS
   HV_LAUNCHED("k_attn_rows_q8");
 }

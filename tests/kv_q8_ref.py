@@ -105,10 +105,17 @@ def attention(q, val, pos, group, scale):
     at most 16 partial sums of an accumulator that may cut instead of round (2u each), then
     the scale and log2 e (2u each), so |dx| <= 44 u B, B = scale * max_t sum_i |q_i k_ti|;
     subtracting the maximum and 2^x add 4u |x| <= 4 u B; weights are off by that on both sides
-    of the quotient: 96 u B. A weight enters the second product as two binary16 terms of 2^15
-    times itself over the largest: what is left is at most half of binary16's smallest step,
-    2^-25, so 2^-40 of the largest weight, whatever the weight. The weighted sum adds each of the n positions once in tiles
-    of 16 and 32: (n / 8 + 64) u of sum w |v| covers it with the sum of the weights."""
+    of the quotient: 96 u B. (Keys of the open block have two terms too, the second exact to
+    2^-38 of the block's largest, which adds 2^-14 sum_i |q_i| times that to B.) The weighted
+    sum adds each of the n positions once in tiles of 16 and 32: (n / 8 + 64) u of sum w |v|
+    covers it with the sum of the weights.
+    A weight enters the second product as two binary16 terms, and what is left is at most half
+    of binary16's smallest step, 2^-25, whatever the weight. At the least it stands as 2^11
+    times w s over the largest w s, s the scale that its block's values have been divided by:
+    codes go to 127, the open block's values to 2^10. So w |v| is off by at most 2^-36 127
+    max(w s) = 2^-36 max(w V) in a coded block, where V is a block's largest |v|, and by 2^-36
+    2^10 max(w s) <= 2^-33 max(w V) in the open one, whose second terms of v add 2^-34 V w. The
+    n positions together: 2^-32 n max(w V)."""
     q = q.astype(np.float64)
     out, tol = np.empty(q.shape), np.empty(q.shape)
     n = pos + 1
@@ -116,9 +123,12 @@ def attention(q, val, pos, group, scale):
         k, v = val[:, h // group, :n].astype(np.float64)
         x = (k @ q[h]) * scale
         big = (np.abs(k) @ np.abs(q[h])).max() * abs(scale)
+        big += 2.0 ** -14 * np.abs(q[h]).sum() * np.abs(k[n // BLK * BLK:]).max(initial=0)
+        peak = np.abs(v).max(1)
+        peak = np.maximum.reduceat(peak, np.arange(0, n, BLK)).repeat(BLK)[:n]
         w = np.exp(x - x.max())
         w /= w.sum()
         out[h] = w @ v
         tol[h] = (96 * U * big + (n / 8 + 64) * U) * (w @ np.abs(v))
-        tol[h] += 2.0 ** -40 * w.max() * np.abs(v).sum(0) + 1e-37
+        tol[h] += 2.0 ** -32 * n * (w * peak).max() + 1e-37
     return out, tol
