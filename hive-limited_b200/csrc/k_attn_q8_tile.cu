@@ -53,21 +53,32 @@ HV_DEV uint64_t smem_desc(uint32_t addr) {      // 128-byte swizzle, 1024 bytes 
   return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) |
          (2ull << 61);
 }
-HV_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, bool add) {
+// One lane of a whole warp issues: the warp stays together, so that the descriptors are uniform
+// registers, which the instruction wants (in a branch of one lane it took 190 cycles to issue
+// a product that runs for 64).
+HV_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, bool add, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      :: "r"(d), "l"(a), "l"(b), "r"(kTlDesc), "r"((uint32_t)add) : "memory");
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      :: "r"(d), "l"(a), "l"(b), "r"(kTlDesc), "r"((uint32_t)add), "r"(leader) : "memory");
 }
-HV_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, bool add) {
+HV_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, bool add, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      :: "r"(d), "r"(a), "l"(b), "r"(kTlDesc), "r"((uint32_t)add) : "memory");
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      :: "r"(d), "r"(a), "l"(b), "r"(kTlDesc), "r"((uint32_t)add), "r"(leader) : "memory");
 }
-HV_DEV void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
-               :: "r"(bar) : "memory");
+HV_DEV void mma_commit(uint32_t bar, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      :: "r"(bar), "r"(leader) : "memory");
+}
+HV_DEV uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
 }
 HV_DEV void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 HV_DEV void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -87,6 +98,12 @@ HV_DEV void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
 HV_DEV void tmem_wait(uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : HV_P4(v, 0), HV_P4(v, 4), HV_P4(v, 8), HV_P4(v, 12) :: "memory");
+}
+// Columns past `see` become -infinity.
+HV_DEV void hide(uint32_t (&v)[16], int see) {
+  asm volatile("" ::: "memory");                // a branch, not 16 selections every time
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v[k] = k <= see ? v[k] : 0xFF800000u;
 }
 HV_DEV void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
   asm volatile(
@@ -169,7 +186,7 @@ static_assert(kTlSmem <= 232448, "shared memory of an SM");
 __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8 c) {
   extern __shared__ __align__(1024) uint8_t smem[];
   TlShared& sh = *reinterpret_cast<TlShared*>(smem + 6 * kTlTile + kTlStage);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kvh = blockIdx.y, tile = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   const int nrows = a.ntok * a.group, row0 = tile * kTlRows;
   const int last_row = min(nrows, row0 + kTlRows) - 1;
@@ -262,63 +279,62 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       uint32_t v[2][16];
       // the largest exponent of the row in this tile
       float up = m, mx = -INFINITY;
+      // (loops over blocks stay rolled: three roles' code has to fit the instruction cache)
       tmem_ld16(s_at, v[0]);
+#pragma unroll 1
+      for (int b = 0; b < 4; ++b) {
+        const int see = see0 - 32 * b;
 #pragma unroll
-      for (int h = 0; h < 8; ++h) {
-        uint32_t (&x)[16] = v[h & 1];
-        tmem_wait(x);
-        if (h < 7) tmem_ld16(s_at + 16 * (h + 1), v[(h + 1) & 1]);
-        if (!all) {
+        for (int h = 0; h < 2; ++h) {
+          uint32_t (&x)[16] = v[h];
+          tmem_wait(x);
+          tmem_ld16(s_at + (32 * b + 16 * (h + 1)) % 128, v[1 - h]);
+          if (!all) hide(x, see - 16 * h);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) x[k] = 16 * h + k <= see0 ? x[k] : 0xFF800000u;
+          for (int k = 0; k < 16; ++k) mx = fmaxf(mx, __uint_as_float(x[k]));
         }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) mx = fmaxf(mx, __uint_as_float(x[k]));
-        if (h & 1) {
-          const float f = sh.sc[i & 3][h >> 1][0] * qs;
-          if (see0 >= 16 * (h - 1)) up = fmaxf(up, fmaf(mx, f, sh.sc[i & 3][h >> 1][1]));
-          mx = -INFINITY;
-        }
+        if (see >= 0) up = fmaxf(up, fmaf(mx, sh.sc[i & 3][b][0] * qs, sh.sc[i & 3][b][1]));
+        mx = -INFINITY;
       }
       const float shrink = m == -INFINITY ? 0.0f : ex2(m - up);
       l *= shrink;
       m = up;
       const float m0 = m == -INFINITY ? 0.0f : m;
-      uint64_t sum = 0;
-      tmem_ld16(s_at, v[0]);
-#pragma unroll
-      for (int h = 0; h < 8; ++h) {
-        uint32_t (&x)[16] = v[h & 1];
-        tmem_wait(x);
-        if (h < 7) tmem_ld16(s_at + 16 * (h + 1), v[(h + 1) & 1]);
-        const float f = sh.sc[i & 3][h >> 1][0] * qs, lv = sh.sc[i & 3][h >> 1][1] - m0;
+      // the first columns are under way again
+#pragma unroll 1
+      for (int b = 0; b < 4; ++b) {
+        const int see = see0 - 32 * b;
+        float f = sh.sc[i & 3][b][0] * qs;
+        f = f == 0.0f ? 1e-38f : f;                         // -inf f has to stay -inf
+        const float lv = sh.sc[i & 3][b][1] - m0;
         const uint64_t f2 = pair(f, f), lv2 = pair(lv, lv);
-        uint32_t hi[8], lo[8];
+        uint64_t sum = 0;
 #pragma unroll
-        for (int k = 0; k < 16; k += 2) {
-          const float2 e = unpair(fma2(pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), f2, lv2));
-          float2 p = make_float2(ex2(e.x), ex2(e.y));
-          if (!all) {
-            p.x = 16 * h + k <= see0 ? p.x : 0.0f;
-            p.y = 16 * h + k + 1 <= see0 ? p.y : 0.0f;
+        for (int h = 0; h < 2; ++h) {
+          uint32_t (&x)[16] = v[h];
+          tmem_wait(x);
+          if (h == 0 || b < 3) tmem_ld16(s_at + 32 * b + 16 * (h + 1), v[1 - h]);
+          if (!all) hide(x, see - 16 * h);
+          uint32_t hi[8], lo[8];
+#pragma unroll
+          for (int k = 0; k < 16; k += 2) {
+            const float2 e = unpair(fma2(pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), f2, lv2));
+            float2 p = make_float2(ex2(e.x), ex2(e.y));
+            const uint64_t p2 = mul2(pair(p.x, p.y), pair(kTlLift, kTlLift));
+            sum = add2(sum, p2);
+            // the first term is cut to binary16's 11 bits, so that the rest is exact
+            p = unpair(p2);
+            const float2 c1 = make_float2(__uint_as_float(__float_as_uint(p.x) & 0xFFFFE000u),
+                                          __uint_as_float(__float_as_uint(p.y) & 0xFFFFE000u));
+            const float2 r = unpair(fma2(pair(c1.x, c1.y), pair(-1.0f, -1.0f), p2));
+            hi[k >> 1] = pack_half2(c1.x, c1.y);
+            lo[k >> 1] = pack_half2(r.x, r.y);
           }
-          const uint64_t p2 = mul2(pair(p.x, p.y), pair(kTlLift, kTlLift));
-          sum = add2(sum, p2);
-          // the first term is cut to binary16's 11 bits, so that the rest is exact
-          p = unpair(p2);
-          const float2 c1 = make_float2(__uint_as_float(__float_as_uint(p.x) & 0xFFFFE000u),
-                                        __uint_as_float(__float_as_uint(p.y) & 0xFFFFE000u));
-          const float2 r = unpair(fma2(pair(c1.x, c1.y), pair(-1.0f, -1.0f), p2));
-          hi[k >> 1] = pack_half2(c1.x, c1.y);
-          lo[k >> 1] = pack_half2(r.x, r.y);
+          tmem_st8(s_at + 32 * b + 16 * h, hi);
+          tmem_st8(s_at + 32 * b + 16 * h + 8, lo);
         }
-        if (h & 1) {
-          const float2 s = unpair(sum);
-          l = fmaf(s.x + s.y, sh.sc[i & 3][h >> 1][2], l);
-          sum = 0;
-        }
-        tmem_st8(s_at + 16 * h, hi);
-        tmem_st8(s_at + 16 * h + 8, lo);
+        const float2 s = unpair(sum);
+        l = fmaf(s.x + s.y, sh.sc[i & 3][b][2], l);
       }
       if (has_tail && i == nt - 1 && lim >= 32 * closed + sh.bad) l = __int_as_float(0x7fc00000);
       tmem_st_wait();
@@ -405,11 +421,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // unit u of K (V); a block past the chunk's last one has codes of 0 and scales of 1
-    auto unit = [&](int i, int which, int u) {
-      return live(i) ? *reinterpret_cast<const uint4*>(stage + which * kQ8Codes + 512 * u)
-                     : make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
-    };
     auto put_k = [&](uint8_t* to, int j, int h, int s, uint32_t x, uint32_t y) {
       // position 32 cw + 8 j + g, dims 64 h + 16 s + 4 t ..
       *reinterpret_cast<uint2*>(to + h * kTlHalf + (32 * cw + 8 * j + g) * 128 +
@@ -451,6 +462,14 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
           put_v(to, uh >> 1, uh & 1, kj >> 1, kj & 1, term(x0, x1, lv, second));
         }
     };
+    auto none_k = [&](uint8_t* to) {
+#pragma unroll 1
+      for (int u = 0; u < 32; ++u) put_k(to, u >> 3, (u >> 2) & 1, u & 3, 0u, 0u);
+    };
+    auto none_v = [&](uint8_t* to) {
+#pragma unroll 1
+      for (int u = 0; u < 64; ++u) put_v(to, u >> 3, (u >> 2) & 1, (u >> 1) & 1, u & 1, 0u);
+    };
     fetch(0, 0);
     fetch(0, 1);
     sc_next = live(0) ? __ldg(scales + b0 + cw) : sc;
@@ -489,10 +508,12 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         lv = q8_lift(mv) * 0.0625f;
         sc = make_float2(1.0f / lk, 1.0f / lv);
         open_k(kt, 0);
+      } else if (!live(i)) {                    // past the chunk's last block
+        none_k(kt);
       } else {
-#pragma unroll
+#pragma unroll 2
         for (int u = 0; u < 8; ++u) {
-          const uint4 y4 = unit(i, 0, u);
+          const uint4 y4 = *reinterpret_cast<const uint4*>(stage + 512 * u);
           const uint32_t x[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -514,12 +535,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       fetch(i + 1, 0);
       if (two) {
         if (!bar_wait_warp(bar(sh.k_free), 0, given_up)) break;
-        if (mine) {
-          open_k(kt, 1);
-        } else {
-#pragma unroll 4
-          for (int u = 0; u < 32; ++u) put_k(kt, u >> 3, (u >> 2) & 1, u & 3, 0u, 0u);
-        }
+        if (mine) open_k(kt, 1);
+        else none_k(kt);
         fence_async();
         bar_arrive(bar(sh.full_k[s]));
       }
@@ -527,10 +544,12 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       if (mine) {
         open_v(vt, 0);
+      } else if (!live(i)) {
+        none_v(vt);
       } else {
-#pragma unroll
+#pragma unroll 2
         for (int u = 0; u < 8; ++u) {
-          const uint4 y4 = unit(i, 1, u);
+          const uint4 y4 = *reinterpret_cast<const uint4*>(stage + kQ8Codes + 512 * u);
           const uint32_t x[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {                     // word 2 h + k
@@ -546,12 +565,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       fetch(i + 1, 1);
       if (two) {
         if (!bar_wait_warp(bar(sh.v_free), 0, given_up)) break;
-        if (mine) {
-          open_v(vt, 1);
-        } else {
-#pragma unroll 4
-          for (int u = 0; u < 64; ++u) put_v(vt, u >> 3, (u >> 2) & 1, (u >> 1) & 1, u & 1, 0u);
-        }
+        if (mine) open_v(vt, 1);
+        else none_v(vt);
         fence_async();
         bar_arrive(bar(sh.full_v[s]));
       }
@@ -560,7 +575,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsIssue));
   }
-  if (warp == 12 && lane == 0) {
+  if (warp == 12) {
+    const uint32_t leader = elect_one();
     const uint64_t qh = smem_desc(sm), ql = smem_desc(sm + kTlTile);
     // step k of 16 along the inner dimension: the half it is in, then 32 bytes each
     auto step = [](int k) { return (uint64_t)(((k >> 2) * kTlHalf + (k & 3) * 32) >> 4); };
@@ -569,48 +585,45 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       const int s = i & 1;
       const uint64_t kd = smem_desc(sm + (2 + s) * kTlTile);
       const uint32_t d = tmem + 128 * s;
-      ok = ok && bar_wait(bar(sh.full_k[s]), (i >> 1) & 1, given_up);
+      ok = ok && bar_wait_warp(bar(sh.full_k[s]), (i >> 1) & 1, given_up);
       if (!ok) return;
       fence_after();
-#pragma unroll 1
-      for (int k = 0; k < 8; ++k) mma_ss(d, ql + step(k), kd + step(k), k > 0);
-#pragma unroll 1
-      for (int k = 0; k < 8; ++k) mma_ss(d, qh + step(k), kd + step(k), true);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mma_ss(d, ql + step(k), kd + step(k), k > 0, leader);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mma_ss(d, qh + step(k), kd + step(k), true, leader);
       if (has_tail && i == nt - 1) {
-        mma_commit(bar(sh.k_free));
-        ok = bar_wait(bar(sh.full_k[s]), ((i >> 1) + 1) & 1, given_up);
+        mma_commit(bar(sh.k_free), leader);
+        ok = bar_wait_warp(bar(sh.full_k[s]), ((i >> 1) + 1) & 1, given_up);
         if (!ok) return;
         fence_after();
-#pragma unroll 1
-      for (int k = 0; k < 8; ++k) mma_ss(d, qh + step(k), kd + step(k), true);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mma_ss(d, qh + step(k), kd + step(k), true, leader);
       }
-      mma_commit(bar(sh.s_ready[s]));
+      mma_commit(bar(sh.s_ready[s]), leader);
     };
     auto product_o = [&](int i) {
       const int s = i & 1;
       const uint64_t vd = smem_desc(sm + (4 + s) * kTlTile);
       const uint32_t p = tmem + 128 * s, d = tmem + 256 + 128 * s;
-      ok = ok && bar_wait(bar(sh.full_v[s]), (i >> 1) & 1, given_up);
-      ok = ok && bar_wait(bar(sh.w_ready[s]), (i >> 1) & 1, given_up);
+      ok = ok && bar_wait_warp(bar(sh.full_v[s]), (i >> 1) & 1, given_up);
+      ok = ok && bar_wait_warp(bar(sh.w_ready[s]), (i >> 1) & 1, given_up);
       if (!ok) return;
       fence_after();
       // the weights of 16 positions are 8 columns of first terms, then 8 of second ones
-#pragma unroll 1
-      for (int k = 0; k < 8; ++k)
-        mma_ts(d, p + 16 * k + 8, vd + step(k), k > 0);
-#pragma unroll 1
-      for (int k = 0; k < 8; ++k)
-        mma_ts(d, p + 16 * k, vd + step(k), true);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k + 8, vd + step(k), k > 0, leader);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k, vd + step(k), true, leader);
       if (has_tail && i == nt - 1) {
-        mma_commit(bar(sh.v_free));
-        ok = bar_wait(bar(sh.full_v[s]), ((i >> 1) + 1) & 1, given_up);
+        mma_commit(bar(sh.v_free), leader);
+        ok = bar_wait_warp(bar(sh.full_v[s]), ((i >> 1) + 1) & 1, given_up);
         if (!ok) return;
         fence_after();
-#pragma unroll 1
-        for (int k = 0; k < 8; ++k)
-          mma_ts(d, p + 16 * k, vd + step(k), true);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k, vd + step(k), true, leader);
       }
-      mma_commit(bar(sh.o_done[s]));
+      mma_commit(bar(sh.o_done[s]), leader);
     };
     if (nt > 0) product_s(0);
     if (nt > 1) product_s(1);
@@ -620,8 +633,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     }
     if (!ok) {                                    // what was issued ends before the memory goes
       int no = 0;
-      mma_commit(bar(sh.drain));
-      bar_wait(bar(sh.drain), 0, &no);
+      mma_commit(bar(sh.drain), leader);
+      bar_wait_warp(bar(sh.drain), 0, &no);
     }
   }
   __syncwarp();
