@@ -3,18 +3,26 @@
 //
 // A CTA has 128 (token, head) rows of a kv head and a chunk of its positions, 128 positions
 // (four blocks) to a tile, tiles in turn to two lanes of work w = tile mod 2:
-//   warps 8-11  turn the codes of a tile into binary16 in shared memory: K [position][dim] and
-//               V transposed [dim][position], 128-byte swizzled rows; the codes of the next
-//               tile come by asynchronous copies meanwhile
-//   warp 12     issues S_w = ql K^T + qh K^T and O_w = wl V + wh V (wh, wl in tensor memory)
-//   warps 0-3   (lane of work 0) and 4-7 (1): a thread has one row of S_w; it writes the row's
-//               weights over S_w, two binary16 terms in place of 32 sums, and adds O_w to the
-//               row's 128 sums in registers
+//   warps 12-15  turn the codes of a tile into binary16 in shared memory: K [position][dim] and
+//                V transposed [dim][position], 128-byte swizzled rows
+//   warps 0-3    (lane of work 0) and 4-7 (1): a thread has one row of S_w; it writes the row's
+//                weights over S_w, two binary16 terms in place of 16 sums; then warp 0 (4),
+//                which has nothing to do until S_w is there again, issues O = wl V + wh V and
+//                the next S_w = ql K^T + qh K^T
+//   warps 8-11   a thread adds its row of O to 128 sums in registers
 // so while one lane of work is at its weights the tensor cores run the other's products. Each
-// lane has its own maximum and sums, and the two meet at the end.
+// lane has its own maximum; the sums go by the larger of the two. The queries and the weights
+// are the operand in tensor memory (S twice, O, and the queries fill its 512 columns), so that
+// shared memory, which would bound the products if it held both operands, is left to K and V.
+//
+// The order of dims in a K row (and of the queries) and that of positions in a tile are free as
+// long as both operands agree. They are such that a lane's codes of one 16-byte unit become 16
+// or 32 adjacent bytes, and that eight lanes' 16-byte stores meet no bank twice: dim
+// 64 h + 16 s + 4 t + e stands at 64 h + 16 t + 4 s + e, position 8 j + 2 t + e of block c of
+// the tile at 64 (c / 2) + 16 t + 8 (c mod 2) + 2 j + e.
 //
 // The tensor cores cut their f32 sums instead of rounding them, once for every 16 positions:
-// kept in tensor memory over 64 tiles, O was 1.8e-5 too small. So O_w is of one tile, and the
+// kept in tensor memory over 64 tiles, O was 1.8e-5 too small. So O is of one tile, and the
 // small terms go first, while the sums are small.
 //
 // The scale of a V block has to multiply its weights here, as a tile's sum stays in tensor
@@ -38,12 +46,11 @@ constexpr int kTlRows = 128;                    // rows of a CTA and positions o
 constexpr int kTlThreads = 512;
 constexpr int kTlHalf = 128 * 128;              // bytes of 128 rows of 64 halves
 constexpr int kTlTile = 2 * kTlHalf;            // bytes of a 128 x 128 binary16 tile
-constexpr int kTlStage = 4 * 2 * kQ8Codes;      // codes of a tile's four blocks
 constexpr float kTlLift = 32768.0f;             // 2^15
-// registers per thread: 128 at launch, given from the converting and issuing warps to the rows
-constexpr int kTlRegsRow = 192, kTlRegsConv = 80, kTlRegsIssue = 48;
-constexpr int kTlRegsSum = 256 * kTlRegsRow + 128 * kTlRegsConv + 128 * kTlRegsIssue;
-static_assert(kTlRegsSum <= 512 * 128, "registers");
+constexpr uint32_t kTlColO = 256, kTlColQ = 384;   // tensor memory: S twice, O, qh, ql
+// registers per thread: 128 at launch, then dealt out anew
+constexpr int kTlRegs = 128, kTlRegsRow = 112, kTlRegsSum = 184, kTlRegsConv = 104;
+static_assert(2 * kTlRegsRow + kTlRegsSum + kTlRegsConv <= 4 * kTlRegs, "registers");
 constexpr unsigned long long kTlWaitNs = 2000000000ull;
 
 // kind::f16 with f32 sums, 128 x 128, both operands with the inner dimension contiguous
@@ -56,12 +63,6 @@ HV_DEV uint64_t smem_desc(uint32_t addr) {      // 128-byte swizzle, 1024 bytes 
 // One lane of a whole warp issues: the warp stays together, so that the descriptors are uniform
 // registers, which the instruction wants (in a branch of one lane it took 190 cycles to issue
 // a product that runs for 64).
-HV_DEV void mma_ss(uint32_t d, uint64_t a, uint64_t b, bool add, uint32_t leader) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-      :: "r"(d), "l"(a), "l"(b), "r"(kTlDesc), "r"((uint32_t)add), "r"(leader) : "memory");
-}
 HV_DEV void mma_ts(uint32_t d, uint32_t a, uint64_t b, bool add, uint32_t leader) {
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
@@ -87,8 +88,22 @@ HV_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "m
 #define HV_R4(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3])
 #define HV_P4(v, i) "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3])
 #define HV_W4(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
-// 16 columns of this thread's row: begun here, in hand after tmem_wait. One load is under way
+// Columns of this thread's row: begun here, in hand after tmem_wait. One load is under way
 // while the columns before it are worked on.
+HV_DEV void tmem_ld32(uint32_t at, uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+      "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : HV_R4(v, 0), HV_R4(v, 4), HV_R4(v, 8), HV_R4(v, 12), HV_R4(v, 16), HV_R4(v, 20),
+        HV_R4(v, 24), HV_R4(v, 28)
+      : "r"(at) : "memory");
+}
+HV_DEV void tmem_wait(uint32_t (&v)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : HV_P4(v, 0), HV_P4(v, 4), HV_P4(v, 8), HV_P4(v, 12), HV_P4(v, 16), HV_P4(v, 20),
+                 HV_P4(v, 24), HV_P4(v, 28) :: "memory");
+}
 HV_DEV void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
@@ -99,16 +114,21 @@ HV_DEV void tmem_wait(uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : HV_P4(v, 0), HV_P4(v, 4), HV_P4(v, 8), HV_P4(v, 12) :: "memory");
 }
-// Columns past `see` become -infinity.
-HV_DEV void hide(uint32_t (&v)[16], int see) {
-  asm volatile("" ::: "memory");                // a branch, not 16 selections every time
+// Of 32 columns, those of positions past `see` become -infinity (see the order of columns at
+// the kernel; see1 is for the second one of the two blocks that share them).
+HV_DEV void hide(uint32_t (&v)[32], int see0, int see1) {
+  asm volatile("" ::: "memory");                // a branch, not 32 selections every time
 #pragma unroll
-  for (int k = 0; k < 16; ++k) v[k] = k <= see ? v[k] : 0xFF800000u;
+  for (int k = 0; k < 32; ++k) {
+    const int r = 8 * ((k & 7) >> 1) + 2 * (k >> 4) + (k & 1);
+    v[k] = r <= ((k & 8) ? see1 : see0) ? v[k] : 0xFF800000u;
+  }
 }
-HV_DEV void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
+HV_DEV void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-      :: "r"(at), HV_W4(v, 0), HV_W4(v, 4) : "memory");
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      :: "r"(at), HV_W4(v, 0), HV_W4(v, 4), HV_W4(v, 8), HV_W4(v, 12) : "memory");
 }
 HV_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -171,21 +191,21 @@ HV_DEV uint64_t add2(uint64_t a, uint64_t b) {
 }
 
 struct TlShared {
-  unsigned long long full_k[2], full_v[2], s_ready[2], w_ready[2], o_done[2], k_free, v_free, drain;
+  unsigned long long full_k[2], full_v[2], s_ready[2], w_ready[2], o_done[2];
+  unsigned long long o_free, k_free, v_free, drain[2];
   float sc[4][4][4];             // of the last four tiles' blocks: s_k, log2 s_v, 1 / s_v
-  float lift[kTlRows];
+  float top[4][kTlRows];         // of the last four tiles: what their weights are relative to
   float m[2][kTlRows], l[2][kTlRows];
   uint32_t tmem;
   int bad;                       // first open row with a value that is not finite
   int given_up;
   unsigned last;
 };
-constexpr int kTlSmem = 6 * kTlTile + kTlStage + (int)sizeof(TlShared);   // qh, ql, K, V twice
-static_assert(kTlSmem <= 232448, "shared memory of an SM");
+constexpr int kTlSmem = 4 * kTlTile + (int)sizeof(TlShared);   // K and V twice
 
 __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8 c) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  TlShared& sh = *reinterpret_cast<TlShared*>(smem + 6 * kTlTile + kTlStage);
+  TlShared& sh = *reinterpret_cast<TlShared*>(smem + 4 * kTlTile);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kvh = blockIdx.y, tile = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   const int nrows = a.ntok * a.group, row0 = tile * kTlRows;
@@ -203,8 +223,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   const bool has_tail = tail && b1 == items;
 
   const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem);
-  uint8_t* k_buf = smem + 2 * kTlTile;            // two tiles, then V's two
-  uint8_t* v_buf = smem + 4 * kTlTile;
+  uint8_t* k_buf = smem;                          // two tiles, then V's two
+  uint8_t* v_buf = smem + 2 * kTlTile;
   auto bar = [](const unsigned long long& b) { return (uint32_t)__cvta_generic_to_shared(&b); };
 
   if (threadIdx.x == 0) {
@@ -215,221 +235,320 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       bar_init(bar(sh.w_ready[i]), 128);
       bar_init(bar(sh.o_done[i]), 1);
     }
+    bar_init(bar(sh.o_free), 128);
     bar_init(bar(sh.k_free), 1);
     bar_init(bar(sh.v_free), 1);
-    bar_init(bar(sh.drain), 1);
+    bar_init(bar(sh.drain[0]), 1);
+    bar_init(bar(sh.drain[1]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.bad = kQ8Blk;
     sh.given_up = 0;
   }
-  if (warp == 12) {
+  if (warp == 15) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
                  :: "r"((uint32_t)__cvta_generic_to_shared(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // the queries in two terms, a row per warp at a time; they take the scale's sign, so that the
-  // largest sum of products is the largest exponent
-  const float qscale = __ldg(a.scale) * kLog2e;
-  for (int r = warp; r < kTlRows; r += kTlThreads / 32) {
-    const int gr = row0 + r;
+  // rows pass through shared memory on their way in and out, whole lines at a time
+  constexpr int kLine = kHd + 4;
+  float* lines = reinterpret_cast<float*>(smem);
+  for (int i = threadIdx.x; i < kTlRows * (kHd / 4); i += kTlThreads) {
+    const int r = row0 + i / (kHd / 4);
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (gr < nrows)
+    if (r < nrows)
       x = __ldg(reinterpret_cast<const float4*>(
-                    a.q + ((size_t)(gr / a.group) * a.nq + (size_t)kvh * a.group + gr % a.group) * kHd) +
-                lane);
-    float amax = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-    const float lift = copysignf(q8_lift(amax), qscale);
-    uint32_t h0, h1, l0, l1;
-    split_half2(x.x * lift, x.y * lift, &h0, &l0);
-    split_half2(x.z * lift, x.w * lift, &h1, &l1);
-    const int at = (lane >> 4) * kTlHalf + r * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) +
-                   (lane & 1) * 8;
-    *reinterpret_cast<uint2*>(smem + at) = make_uint2(h0, h1);
-    *reinterpret_cast<uint2*>(smem + kTlTile + at) = make_uint2(l0, l1);
-    if (lane == 0) sh.lift[r] = lift;
+                    a.q + ((size_t)(r / a.group) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd) +
+                i % (kHd / 4));
+    *reinterpret_cast<float4*>(lines + (size_t)(i / (kHd / 4)) * kLine + 4 * (i % (kHd / 4))) = x;
   }
-  fence_async();
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
   volatile int* given_up = &sh.given_up;
-
+  const int w = warp >> 2, row = threadIdx.x & 127, grow = row0 + row;
+  // the queries in two terms, a row per thread: the first ones from warps 0-3, the second from
+  // 4-7. They take the scale's sign, so that the largest sum of products is the largest exponent
+  const float qscale = __ldg(a.scale) * kLog2e;
+  float qs = 0.0f;
+  if (warp < 8) {
+    const float4* q = reinterpret_cast<const float4*>(lines + (size_t)row * kLine);
+    float amax = 0.0f;
+#pragma unroll 8
+    for (int d = 0; d < kHd / 4; ++d) {
+      const float4 x = q[d];
+      amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+    }
+    const float lift = copysignf(q8_lift(amax), qscale);
+    qs = qscale / lift;
+    const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kTlColQ + 64 * w;
+    // dims in the order of K's tiles: 64 h + 16 s + 4 t + e stands at 64 h + 16 t + 4 s + e
+#pragma unroll 1
+    for (int d = 0; d < kHd / 4; d += 8) {
+      uint32_t v[16];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float4 x = q[(d & 16) + 4 * (k & 3) + ((d >> 2) & 2) + (k >> 2)];
+        uint32_t h0, h1, l0, l1;
+        split_half2(x.x * lift, x.y * lift, &h0, &l0);
+        split_half2(x.z * lift, x.w * lift, &h1, &l1);
+        v[2 * k] = w ? l0 : h0;
+        v[2 * k + 1] = w ? l1 : h1;
+      }
+      tmem_st16(to + 2 * d, v);
+    }
+    tmem_st_wait();
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
   const int ntile = gridDim.x / a.chunks;
   const size_t slot = ((size_t)kvh * ntile + tile) * a.chunks;
   if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsRow));
     float m = -INFINITY, l = 0.0f;                // of this thread's row
-    uint64_t acc[kHd / 2];
-    const int w = warp >> 2, row = threadIdx.x & 127, grow = row0 + row;
-    auto rows_sync = [] { asm volatile("bar.sync 1, 256;" ::: "memory"); };
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kTlRegsRow));
-#pragma unroll
-    for (int d = 0; d < kHd / 2; ++d) acc[d] = 0;
     const uint32_t s_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * w;
-    const uint32_t o_at = s_at + 256;
     const int lim = grow < nrows ? min(min(a.pos0 + grow / a.group, held - 1), 32 * b1 - 1) : -1;
-    const float qs = qscale / sh.lift[row];
+    const uint32_t leader = elect_one();
+    const uint32_t qh = tmem + kTlColQ, ql = qh + 64;
+    // step k of 16 along the inner dimension: the half it is in, then 32 bytes each
+    auto step = [](int k) { return (uint64_t)(((k >> 2) * kTlHalf + (k & 3) * 32) >> 4); };
+    bool ok = true;
+    auto product_s = [&](int i) {
+      const int s = i & 1;
+      const uint64_t kd = smem_desc(sm + s * kTlTile);
+      const uint32_t d = tmem + 128 * s;
+      ok = ok && bar_wait_warp(bar(sh.full_k[s]), (i >> 1) & 1, given_up);
+      if (!ok) return;
+      fence_after();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mma_ts(d, ql + 8 * k, kd + step(k), k > 0, leader);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mma_ts(d, qh + 8 * k, kd + step(k), true, leader);
+      if (has_tail && i == nt - 1) {
+        mma_commit(bar(sh.k_free), leader);
+        ok = bar_wait_warp(bar(sh.full_k[s]), ((i >> 1) + 1) & 1, given_up);
+        if (!ok) return;
+        fence_after();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mma_ts(d, qh + 8 * k, kd + step(k), true, leader);
+      }
+      mma_commit(bar(sh.s_ready[s]), leader);
+    };
+    auto product_o = [&](int i) {
+      const int s = i & 1;
+      const uint64_t vd = smem_desc(sm + (2 + s) * kTlTile);
+      const uint32_t p = tmem + 128 * s, d = tmem + kTlColO;
+      ok = ok && bar_wait_warp(bar(sh.full_v[s]), (i >> 1) & 1, given_up);
+      ok = ok && bar_wait_warp(bar(sh.w_ready[s]), (i >> 1) & 1, given_up);
+      if (i > 0) ok = ok && bar_wait_warp(bar(sh.o_free), (i - 1) & 1, given_up);
+      if (!ok) return;
+      fence_after();
+      // the weights of 16 positions are 8 columns of first terms, then 8 of second ones
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k + 8, vd + step(k), k > 0, leader);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k, vd + step(k), true, leader);
+      if (has_tail && i == nt - 1) {
+        mma_commit(bar(sh.v_free), leader);
+        ok = bar_wait_warp(bar(sh.full_v[s]), ((i >> 1) + 1) & 1, given_up);
+        if (!ok) return;
+        fence_after();
+#pragma unroll
+        for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k, vd + step(k), true, leader);
+      }
+      mma_commit(bar(sh.o_done[s]), leader);
+    };
+    const bool issues = (warp & 3) == 0;
+    if (issues && w < nt) product_s(w);
     for (int i = w; i < nt; i += 2) {
       if (!bar_wait_warp(bar(sh.s_ready[w]), (i >> 1) & 1, given_up)) break;
       fence_after();
-      const int see0 = lim - 32 * (b0 + 4 * i);            // columns 0 .. see0 are seen
+      const int see0 = lim - 32 * (b0 + 4 * i);            // positions 0 .. see0 are seen
       const bool all = __all_sync(0xFFFFFFFFu, see0 >= kTlRows - 1);
-      uint32_t v[2][16];
+      const float (&sc)[4][4] = sh.sc[i & 3];
+      uint32_t v[2][32];
       // the largest exponent of the row in this tile
-      float up = m, mx = -INFINITY;
-      // (loops over blocks stay rolled: three roles' code has to fit the instruction cache)
-      tmem_ld16(s_at, v[0]);
+      // (loops over pairs of blocks stay rolled: the code of all roles has to fit the
+      // instruction cache)
+      float up = m;
+      tmem_ld32(s_at, v[0]);
 #pragma unroll 1
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < 4; b += 2) {
         const int see = see0 - 32 * b;
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t (&x)[16] = v[h];
+          uint32_t (&x)[32] = v[h];
           tmem_wait(x);
-          tmem_ld16(s_at + (32 * b + 16 * (h + 1)) % 128, v[1 - h]);
-          if (!all) hide(x, see - 16 * h);
+          tmem_ld32(s_at + 32 * ((b + h + 1) & 3), v[1 - h]);
+          if (__builtin_expect(!all, 0)) hide(x, see - 4 * h, see - 4 * h - 32);
 #pragma unroll
-          for (int k = 0; k < 16; ++k) mx = fmaxf(mx, __uint_as_float(x[k]));
+          for (int k = 0; k < 32; ++k) {
+            float& y = mx[((k >> 3) & 1) + 2 * (k & 1)];
+            y = fmaxf(y, __uint_as_float(x[k]));
+          }
         }
-        if (see >= 0) up = fmaxf(up, fmaf(mx, sh.sc[i & 3][b][0] * qs, sh.sc[i & 3][b][1]));
-        mx = -INFINITY;
+        if (see >= 0) up = fmaxf(up, fmaf(fmaxf(mx[0], mx[2]), sc[b][0] * qs, sc[b][1]));
+        if (see >= 32) up = fmaxf(up, fmaf(fmaxf(mx[1], mx[3]), sc[b + 1][0] * qs, sc[b + 1][1]));
       }
-      const float shrink = m == -INFINITY ? 0.0f : ex2(m - up);
-      l *= shrink;
+      l *= m == -INFINITY ? 0.0f : ex2(m - up);
       m = up;
+      sh.top[i & 3][row] = m;
       const float m0 = m == -INFINITY ? 0.0f : m;
       // the first columns are under way again
 #pragma unroll 1
-      for (int b = 0; b < 4; ++b) {
+      for (int b = 0; b < 4; b += 2) {
         const int see = see0 - 32 * b;
-        float f = sh.sc[i & 3][b][0] * qs;
-        f = f == 0.0f ? 1e-38f : f;                         // -inf f has to stay -inf
-        const float lv = sh.sc[i & 3][b][1] - m0;
-        const uint64_t f2 = pair(f, f), lv2 = pair(lv, lv);
-        uint64_t sum = 0;
+        uint64_t f2[2], lv2[2], sum[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float f = sc[b + e][0] * qs;
+          f = f == 0.0f ? 1e-38f : f;                       // -inf f has to stay -inf
+          f2[e] = pair(f, f);
+          lv2[e] = pair(sc[b + e][1] - m0, sc[b + e][1] - m0);
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t (&x)[16] = v[h];
+          uint32_t (&x)[32] = v[h];
           tmem_wait(x);
-          if (h == 0 || b < 3) tmem_ld16(s_at + 32 * b + 16 * (h + 1), v[1 - h]);
-          if (!all) hide(x, see - 16 * h);
-          uint32_t hi[8], lo[8];
+          if (h == 0 || b == 0) tmem_ld32(s_at + 32 * (b + h + 1), v[1 - h]);
+          if (__builtin_expect(!all, 0)) hide(x, see - 4 * h, see - 4 * h - 32);
 #pragma unroll
-          for (int k = 0; k < 16; k += 2) {
-            const float2 e = unpair(fma2(pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])), f2, lv2));
-            float2 p = make_float2(ex2(e.x), ex2(e.y));
-            const uint64_t p2 = mul2(pair(p.x, p.y), pair(kTlLift, kTlLift));
-            sum = add2(sum, p2);
-            // the first term is cut to binary16's 11 bits, so that the rest is exact
-            p = unpair(p2);
-            const float2 c1 = make_float2(__uint_as_float(__float_as_uint(p.x) & 0xFFFFE000u),
-                                          __uint_as_float(__float_as_uint(p.y) & 0xFFFFE000u));
-            const float2 r = unpair(fma2(pair(c1.x, c1.y), pair(-1.0f, -1.0f), p2));
-            hi[k >> 1] = pack_half2(c1.x, c1.y);
-            lo[k >> 1] = pack_half2(r.x, r.y);
+          for (int g = 0; g < 2; ++g) {
+            // 16 positions: 8 columns of first terms, 8 of second ones
+            uint32_t wt[16];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint64_t s2 = pair(__uint_as_float(x[16 * g + 2 * k]), __uint_as_float(x[16 * g + 2 * k + 1]));
+              const float2 e = unpair(fma2(s2, f2[k >> 2], lv2[k >> 2]));
+              const uint64_t p2 = mul2(pair(ex2(e.x), ex2(e.y)), pair(kTlLift, kTlLift));
+              sum[k >> 2] = add2(sum[k >> 2], p2);
+              // the first term is cut to binary16's 11 bits, so that the rest is exact
+              const float2 p = unpair(p2);
+              const float2 c1 = make_float2(__uint_as_float(__float_as_uint(p.x) & 0xFFFFE000u),
+                                            __uint_as_float(__float_as_uint(p.y) & 0xFFFFE000u));
+              const float2 r = unpair(fma2(pair(c1.x, c1.y), pair(-1.0f, -1.0f), p2));
+              wt[k] = pack_half2(c1.x, c1.y);
+              wt[8 + k] = pack_half2(r.x, r.y);
+            }
+            tmem_st16(s_at + 32 * (b + h) + 16 * g, wt);
           }
-          tmem_st8(s_at + 32 * b + 16 * h, hi);
-          tmem_st8(s_at + 32 * b + 16 * h + 8, lo);
         }
-        const float2 s = unpair(sum);
-        l = fmaf(s.x + s.y, sh.sc[i & 3][b][2], l);
+        const float2 s0 = unpair(sum[0]), s1 = unpair(sum[1]);
+        l = fmaf(s0.x + s0.y, sc[b][2], l);
+        l = fmaf(s1.x + s1.y, sc[b + 1][2], l);
       }
       if (has_tail && i == nt - 1 && lim >= 32 * closed + sh.bad) l = __int_as_float(0x7fc00000);
       tmem_st_wait();
       fence_before();
       bar_arrive(bar(sh.w_ready[w]));
-      // this tile's O, while the tensor cores go on
-      if (!bar_wait_warp(bar(sh.o_done[w]), (i >> 1) & 1, given_up)) break;
+      if (issues) {
+        product_o(i);
+        if (i + 2 < nt) product_s(i + 2);
+      }
+    }
+    if (issues && !ok) {                          // what was issued ends before the memory goes
+      int no = 0;
+      mma_commit(bar(sh.drain[w]), leader);
+      bar_wait_warp(bar(sh.drain[w]), 0, &no);
+    }
+    sh.m[w][row] = m;
+    sh.l[w][row] = l;
+    asm volatile("bar.sync 1, 384;" ::: "memory");         // with the warps that have the sums
+  } else if (warp < 12) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kTlRegsSum));
+    uint64_t acc[kHd / 2];
+#pragma unroll
+    for (int d = 0; d < kHd / 2; ++d) acc[d] = 0;
+    float M = -INFINITY;                          // what the sums are relative to
+    const uint32_t o_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kTlColO;
+    for (int i = 0; i < nt; ++i) {
+      if (!bar_wait_warp(bar(sh.o_done[i & 1]), (i >> 1) & 1, given_up)) break;
       fence_after();
-      const uint64_t shrink2 = pair(shrink, shrink);
+      const float m = sh.top[i & 3][row], up = fmaxf(M, m);
+      const float fa = M == -INFINITY ? 0.0f : ex2(M - up), fo = m == -INFINITY ? 0.0f : ex2(m - up);
+      const uint64_t fa2 = pair(fa, fa), fo2 = pair(fo, fo);
+      M = up;
+      uint32_t v[2][16];
       tmem_ld16(o_at, v[0]);
 #pragma unroll
       for (int h = 0; h < 8; ++h) {
         uint32_t (&x)[16] = v[h & 1];
         tmem_wait(x);
-        if (h < 7) tmem_ld16(o_at + 16 * (h + 1), v[(h + 1) & 1]);
+        if (h < 7) {
+          tmem_ld16(o_at + 16 * (h + 1), v[(h + 1) & 1]);
+        } else {
+          fence_before();
+          bar_arrive(bar(sh.o_free));
+        }
 #pragma unroll
-        for (int k = 0; k < 16; k += 2)
-          acc[8 * h + (k >> 1)] = fma2(acc[8 * h + (k >> 1)], shrink2,
-                                       pair(__uint_as_float(x[k]), __uint_as_float(x[k + 1])));
+        for (int k = 0; k < 8; ++k)
+          acc[8 * h + k] = fma2(acc[8 * h + k], fa2,
+                                mul2(pair(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), fo2));
       }
     }
-    // the two lanes of work meet in what was K's (and, for the last rows, V's) memory
-    float* red = reinterpret_cast<float*>(k_buf) + (size_t)row * (kHd + 4);
-    sh.m[w][row] = m;
-    sh.l[w][row] = l;
-    rows_sync();
+    asm volatile("bar.sync 1, 384;" ::: "memory");
+    const float nan = __int_as_float(0x7fc00000);
     const float l0 = sh.l[0][row], l1 = sh.l[1][row];
-    const float M = fmaxf(sh.m[0][row], sh.m[1][row]);
-    const float a0 = l0 == 0.0f ? 0.0f : ex2(sh.m[0][row] - M);
-    const float a1 = l1 == 0.0f ? 0.0f : ex2(sh.m[1][row] - M);
-    if (w == 1) {
-#pragma unroll
-      for (int d = 0; d < kHd / 2; d += 2) {
-        const float2 x = unpair(acc[d]), y = unpair(acc[d + 1]);
-        *reinterpret_cast<float4*>(red + 2 * d) = make_float4(x.x * a1, x.y * a1, y.x * a1, y.y * a1);
-      }
+    float L = (l0 == 0.0f ? 0.0f : l0 * ex2(sh.m[0][row] - M)) +
+              (l1 == 0.0f ? 0.0f : l1 * ex2(sh.m[1][row] - M));
+    if (*given_up) L = nan;
+    if (nact == 1) {
+      L = 1.0f / L;
+      if (a.pos0 + grow / a.group >= held) L = nan;
     }
-    rows_sync();
-    if (w == 0) {
-      const float nan = __int_as_float(0x7fc00000);
-      const float L = *given_up ? nan : l0 * a0 + l1 * a1;
-      float* part = a.part + (slot + chunk) * rows_part(kTlRows);
-      float* out = part + (size_t)row * kHd;
-      float f = 1.0f;
-      if (nact == 1) {
-        const int r = min(grow, nrows - 1);
-        out = a.ctx + ((size_t)(r / a.group) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd;
-        f = a.pos0 + grow / a.group >= held ? nan : 1.0f / L;
-      }
+    const float f = nact > 1 ? 1.0f : L;
+    float* line = lines + (size_t)row * kLine;
 #pragma unroll
-      for (int d = 0; d < kHd / 2; d += 2) {
-        const float2 x = unpair(acc[d]), y = unpair(acc[d + 1]);
-        const float4 o = *reinterpret_cast<const float4*>(red + 2 * d);
-        if (nact > 1 || grow < nrows)
-          *reinterpret_cast<float4*>(out + 2 * d) =
-              make_float4((x.x * a0 + o.x) * f, (x.y * a0 + o.y) * f, (y.x * a0 + o.z) * f,
-                          (y.y * a0 + o.w) * f);
-      }
-      if (nact > 1) {
-        *reinterpret_cast<float2*>(part + kTlRows * kHd + 2 * row) = make_float2(M, L);
-        __threadfence();
-      }
+    for (int d = 0; d < kHd / 2; d += 2) {
+      const float2 x = unpair(acc[d]), y = unpair(acc[d + 1]);
+      *reinterpret_cast<float4*>(line + 2 * d) = make_float4(x.x * f, x.y * f, y.x * f, y.y * f);
     }
-  } else if (warp < 12) {
+    float* part = a.part + (slot + chunk) * rows_part(kTlRows);
+    if (nact > 1)
+      *reinterpret_cast<float2*>(part + kTlRows * kHd + 2 * row) = make_float2(M, L);
+    asm volatile("bar.sync 2, 128;" ::: "memory");
+    for (int i = threadIdx.x & 127; i < kTlRows * (kHd / 4); i += 128) {
+      const int n = i / (kHd / 4), d = i % (kHd / 4), r = row0 + n;
+      const float4 x = *reinterpret_cast<const float4*>(lines + (size_t)n * kLine + 4 * d);
+      if (nact > 1)
+        reinterpret_cast<float4*>(part)[i] = x;
+      else if (r < nrows)
+        reinterpret_cast<float4*>(a.ctx + ((size_t)(r / a.group) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd)[d] = x;
+    }
+    if (nact > 1) __threadfence();
+  } else if (warp < 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsConv));
     // a warp per block of the tile
-    const int cw = warp - 8, g = lane >> 2, t = lane & 3;
+    const int cw = warp - 12, g = lane >> 2, t = lane & 3;
     const uint8_t* codes = c.codes + (size_t)kvh * c.nblk * 2 * kQ8Codes + 16 * lane;
     const float2* scales = reinterpret_cast<const float2*>(c.scales) + (size_t)kvh * c.nblk;
     const float* open = c.tail + (size_t)kvh * 2 * kQ8Codes;
     const int nopen = held - closed * kQ8Blk;
-    // a lane's 16-byte units of a block pass through its own bytes of the staging area
-    uint8_t* stage = smem + 6 * kTlTile + cw * 2 * kQ8Codes + 16 * lane;
-    const uint32_t stage_s = (uint32_t)__cvta_generic_to_shared(stage);
+    // the codes of the next tile are loaded while this one's are worked on
+    uint4 kx[8], vx[8];
     float2 sc = make_float2(1.f, 1.f), sc_next;
     auto live = [&](int i) { return i < nt && b0 + 4 * i + cw < min(b1, nb); };
-    auto fetch = [&](int i, int which) {
+    auto fetch = [&](int i, int which, uint4 (&x)[8]) {
       if (live(i)) {
         const uint8_t* src = codes + ((size_t)(b0 + 4 * i + cw) * 2 + which) * kQ8Codes;
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                       :: "r"(stage_s + which * kQ8Codes + 512 * u), "l"(src + 512 * u) : "memory");
+        for (int u = 0; u < 8; ++u) x[u] = __ldg(reinterpret_cast<const uint4*>(src + 512 * u));
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto put_k = [&](uint8_t* to, int j, int h, int s, uint32_t x, uint32_t y) {
-      // position 32 cw + 8 j + g, dims 64 h + 16 s + 4 t ..
-      *reinterpret_cast<uint2*>(to + h * kTlHalf + (32 * cw + 8 * j + g) * 128 +
-                                (((2 * s + (t >> 1)) ^ g) << 4) + (t & 1) * 8) = make_uint2(x, y);
+    auto put_k = [&](uint8_t* to, int j, int h, const uint32_t (&x)[8]) {
+      // position 8 j + g of block cw, dims 64 h + 16 s + 4 t .. for s = 0 .. 3
+      const int n = 64 * (cw >> 1) + 16 * (g >> 1) + 8 * (cw & 1) + 2 * j + (g & 1);
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        *reinterpret_cast<uint4*>(to + h * kTlHalf + n * 128 + (((2 * t + c) ^ (n & 7)) << 4)) =
+            make_uint4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
     };
-    auto put_v = [&](uint8_t* to, int u, int h, int k, int j, uint32_t x) {
-      // dim 16 u + 8 h + g, positions 32 cw + 16 k + 8 j + 2 t ..
-      *reinterpret_cast<uint32_t*>(to + (cw >> 1) * kTlHalf + (16 * u + 8 * h + g) * 128 +
-                                   (((4 * (cw & 1) + 2 * k + j) ^ g) << 4) + 4 * t) = x;
+    auto put_v = [&](uint8_t* to, int u, int h, const uint32_t (&x)[4]) {
+      // dim 16 u + 8 h + g, positions 8 j + 2 t .. of block cw for j = 0 .. 3
+      *reinterpret_cast<uint4*>(to + (cw >> 1) * kTlHalf + (16 * u + 8 * h + g) * 128 +
+                                (((2 * t + (cw & 1)) ^ g) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
     };
     // the open rows' values in one of their two terms (second: 1)
     float lk = 1.0f, lv = 1.0f;
@@ -442,36 +561,46 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     };
     auto open_k = [&](uint8_t* to, int second) {
 #pragma unroll 1
-      for (int j = 0; j < 4; ++j)
-#pragma unroll 1
-        for (int hs = 0; hs < 8; ++hs) {
-          const int r = 8 * j + g;
+      for (int u = 0; u < 8; ++u) {
+        const int r = 8 * (u >> 1) + g;
+        uint32_t y[8];
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
           float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (r < nopen) x = __ldg(reinterpret_cast<const float4*>(open + r * kHd + 16 * hs + 4 * t));
-          put_k(to, j, hs >> 2, hs & 3, term(x.x, x.y, lk, second), term(x.z, x.w, lk, second));
+          if (r < nopen)
+            x = __ldg(reinterpret_cast<const float4*>(open + r * kHd + 64 * (u & 1) + 16 * s + 4 * t));
+          y[2 * s] = term(x.x, x.y, lk, second);
+          y[2 * s + 1] = term(x.z, x.w, lk, second);
         }
+        put_k(to, u >> 1, u & 1, y);
+      }
     };
     auto open_v = [&](uint8_t* to, int second) {
 #pragma unroll 1
-      for (int uh = 0; uh < 16; ++uh)
+      for (int uh = 0; uh < 16; ++uh) {
+        uint32_t y[4];
 #pragma unroll
-        for (int kj = 0; kj < 4; ++kj) {
-          const int r = 8 * kj + 2 * t, d = 8 * uh + g;
+        for (int j = 0; j < 4; ++j) {
+          const int r = 8 * j + 2 * t, d = 8 * uh + g;
           const float x0 = r < nopen ? __ldg(open + kQ8Codes + r * kHd + d) : 0.0f;
           const float x1 = r + 1 < nopen ? __ldg(open + kQ8Codes + (r + 1) * kHd + d) : 0.0f;
-          put_v(to, uh >> 1, uh & 1, kj >> 1, kj & 1, term(x0, x1, lv, second));
+          y[j] = term(x0, x1, lv, second);
         }
+        put_v(to, uh >> 1, uh & 1, y);
+      }
     };
     auto none_k = [&](uint8_t* to) {
+      const uint32_t y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
-      for (int u = 0; u < 32; ++u) put_k(to, u >> 3, (u >> 2) & 1, u & 3, 0u, 0u);
+      for (int u = 0; u < 8; ++u) put_k(to, u >> 1, u & 1, y);
     };
     auto none_v = [&](uint8_t* to) {
+      const uint32_t y[4] = {0, 0, 0, 0};
 #pragma unroll 1
-      for (int u = 0; u < 64; ++u) put_v(to, u >> 3, (u >> 2) & 1, (u >> 1) & 1, u & 1, 0u);
+      for (int uh = 0; uh < 16; ++uh) put_v(to, uh >> 1, uh & 1, y);
     };
-    fetch(0, 0);
-    fetch(0, 1);
+    fetch(0, 0, kx);
+    fetch(0, 1, vx);
     sc_next = live(0) ? __ldg(scales + b0 + cw) : sc;
     for (int i = 0; i < nt; ++i) {
       const int s = i & 1;
@@ -482,7 +611,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       sc = sc_next;
       sc_next = live(i + 1) ? __ldg(scales + b0 + 4 * (i + 1) + cw) : make_float2(1.f, 1.f);
       if (i >= 2 && !bar_wait_warp(bar(sh.s_ready[s]), ((i - 2) >> 1) & 1, given_up)) break;
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
       if (mine) {
         float mk = 0.0f, mv = 0.0f;
         for (int r = 0; r < nopen; ++r) {
@@ -511,16 +639,13 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       } else if (!live(i)) {                    // past the chunk's last block
         none_k(kt);
       } else {
-#pragma unroll 2
-        for (int u = 0; u < 8; ++u) {
-          const uint4 y4 = *reinterpret_cast<const uint4*>(stage + 512 * u);
-          const uint32_t x[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t y0, y1;
-            q8_halves(x[k], &y0, &y1);
-            put_k(kt, u >> 1, u & 1, k, y0, y1);
-          }
+        for (int u = 0; u < 8; ++u) {
+          const uint32_t x[4] = {kx[u].x, kx[u].y, kx[u].z, kx[u].w};
+          uint32_t y[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) q8_halves(x[k], &y[2 * k], &y[2 * k + 1]);
+          put_k(kt, u >> 1, u & 1, y);
         }
       }
       if (lane == 0) {
@@ -532,7 +657,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       }
       fence_async();
       bar_arrive(bar(sh.full_k[s]));
-      fetch(i + 1, 0);
+      fetch(i + 1, 0, kx);
       if (two) {
         if (!bar_wait_warp(bar(sh.k_free), 0, given_up)) break;
         if (mine) open_k(kt, 1);
@@ -541,28 +666,26 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         bar_arrive(bar(sh.full_k[s]));
       }
       if (i >= 2 && !bar_wait_warp(bar(sh.o_done[s]), ((i - 2) >> 1) & 1, given_up)) break;
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
       if (mine) {
         open_v(vt, 0);
       } else if (!live(i)) {
         none_v(vt);
       } else {
-#pragma unroll 2
-        for (int u = 0; u < 8; ++u) {
-          const uint4 y4 = *reinterpret_cast<const uint4*>(stage + kQ8Codes + 512 * u);
-          const uint32_t x[4] = {y4.x, y4.y, y4.z, y4.w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {                     // word 2 h + k
-            uint32_t y0, y1;
-            q8_halves(x[k], &y0, &y1);
-            put_v(vt, u, k >> 1, k & 1, 0, y0);
-            put_v(vt, u, k >> 1, k & 1, 1, y1);
+        for (int u = 0; u < 8; ++u) {
+          const uint32_t x[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t y[4];
+            q8_halves(x[2 * h], &y[0], &y[1]);
+            q8_halves(x[2 * h + 1], &y[2], &y[3]);
+            put_v(vt, u, h, y);
           }
         }
       }
       fence_async();
       bar_arrive(bar(sh.full_v[s]));
-      fetch(i + 1, 1);
+      fetch(i + 1, 1, vx);
       if (two) {
         if (!bar_wait_warp(bar(sh.v_free), 0, given_up)) break;
         if (mine) open_v(vt, 1);
@@ -571,76 +694,11 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         bar_arrive(bar(sh.full_v[s]));
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsIssue));
-  }
-  if (warp == 12) {
-    const uint32_t leader = elect_one();
-    const uint64_t qh = smem_desc(sm), ql = smem_desc(sm + kTlTile);
-    // step k of 16 along the inner dimension: the half it is in, then 32 bytes each
-    auto step = [](int k) { return (uint64_t)(((k >> 2) * kTlHalf + (k & 3) * 32) >> 4); };
-    bool ok = true;
-    auto product_s = [&](int i) {
-      const int s = i & 1;
-      const uint64_t kd = smem_desc(sm + (2 + s) * kTlTile);
-      const uint32_t d = tmem + 128 * s;
-      ok = ok && bar_wait_warp(bar(sh.full_k[s]), (i >> 1) & 1, given_up);
-      if (!ok) return;
-      fence_after();
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mma_ss(d, ql + step(k), kd + step(k), k > 0, leader);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mma_ss(d, qh + step(k), kd + step(k), true, leader);
-      if (has_tail && i == nt - 1) {
-        mma_commit(bar(sh.k_free), leader);
-        ok = bar_wait_warp(bar(sh.full_k[s]), ((i >> 1) + 1) & 1, given_up);
-        if (!ok) return;
-        fence_after();
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mma_ss(d, qh + step(k), kd + step(k), true, leader);
-      }
-      mma_commit(bar(sh.s_ready[s]), leader);
-    };
-    auto product_o = [&](int i) {
-      const int s = i & 1;
-      const uint64_t vd = smem_desc(sm + (4 + s) * kTlTile);
-      const uint32_t p = tmem + 128 * s, d = tmem + 256 + 128 * s;
-      ok = ok && bar_wait_warp(bar(sh.full_v[s]), (i >> 1) & 1, given_up);
-      ok = ok && bar_wait_warp(bar(sh.w_ready[s]), (i >> 1) & 1, given_up);
-      if (!ok) return;
-      fence_after();
-      // the weights of 16 positions are 8 columns of first terms, then 8 of second ones
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k + 8, vd + step(k), k > 0, leader);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k, vd + step(k), true, leader);
-      if (has_tail && i == nt - 1) {
-        mma_commit(bar(sh.v_free), leader);
-        ok = bar_wait_warp(bar(sh.full_v[s]), ((i >> 1) + 1) & 1, given_up);
-        if (!ok) return;
-        fence_after();
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k, vd + step(k), true, leader);
-      }
-      mma_commit(bar(sh.o_done[s]), leader);
-    };
-    if (nt > 0) product_s(0);
-    if (nt > 1) product_s(1);
-    for (int i = 0; i < nt && ok; ++i) {
-      product_o(i);
-      if (i + 2 < nt) product_s(i + 2);
-    }
-    if (!ok) {                                    // what was issued ends before the memory goes
-      int no = 0;
-      mma_commit(bar(sh.drain), leader);
-      bar_wait_warp(bar(sh.drain), 0, &no);
-    }
   }
   __syncwarp();
   fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 15) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem));
   }
@@ -662,13 +720,12 @@ int attn_tile_q8_launch(const RowsArgs& a, const KvQ8& c, unsigned tiles, unsign
                         cudaStream_t st) {
   const int rc = smem_attr((const void*)k_attn_tile_q8, kTlSmem);
   if (rc) return rc;
-  // a split of more registers than the kernel starts with would wait for good
+  // registers are dealt out of what the kernel starts with: a share too large would wait for good
   static const int regs = [] {
     cudaFuncAttributes f{};
     return cudaFuncGetAttributes(&f, k_attn_tile_q8) == cudaSuccess ? f.numRegs : 0;
   }();
-  HV_REQUIRE(regs * kTlThreads >= kTlRegsSum, HV_E_UNSUPPORTED,
-             "k_attn_tile_q8: built with %d registers", regs);
+  HV_REQUIRE(regs == kTlRegs, HV_E_UNSUPPORTED, "k_attn_tile_q8: built with %d registers", regs);
   k_attn_tile_q8<<<dim3(tiles * a.chunks, nkv), kTlThreads, kTlSmem, st>>>(a, c);
   HV_LAUNCHED("k_attn_tile_q8");
 }
