@@ -752,7 +752,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   __syncthreads();
   if (!s_last) return;
   __threadfence();
-  rows_join<Cfg::kRows>(a, kvh, slot, nact, row0, nrows, held);
+  rows_join<Cfg::kRows>(a, kvh, slot, nact, row0, nrows, held, reinterpret_cast<float*>(smem));
 }
 
 // Rows per CTA and chunks per row tile of a run: 16 rows at a time up to 128, and as many

@@ -46,6 +46,7 @@ constexpr int kTlRows = 128;                    // rows of a CTA and positions o
 constexpr int kTlThreads = 512;
 constexpr int kTlHalf = 128 * 128;              // bytes of 128 rows of 64 halves
 constexpr int kTlTile = 2 * kTlHalf;            // bytes of a 128 x 128 binary16 tile
+constexpr int kTlLine = kHd + 4;               // floats from row to row on their way in and out
 constexpr float kTlLift = 32768.0f;             // 2^15
 constexpr uint32_t kTlColO = 256, kTlColQ = 384;   // tensor memory: S twice, O, qh, ql
 // registers per thread: 128 at launch, then dealt out anew
@@ -113,16 +114,6 @@ HV_DEV void tmem_ld16(uint32_t at, uint32_t (&v)[16]) {
 HV_DEV void tmem_wait(uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : HV_P4(v, 0), HV_P4(v, 4), HV_P4(v, 8), HV_P4(v, 12) :: "memory");
-}
-// Of 32 columns, those of positions past `see` become -infinity (see the order of columns at
-// the kernel; see1 is for the second one of the two blocks that share them).
-HV_DEV void hide(uint32_t (&v)[32], int see0, int see1) {
-  asm volatile("" ::: "memory");                // a branch, not 32 selections every time
-#pragma unroll
-  for (int k = 0; k < 32; ++k) {
-    const int r = 8 * ((k & 7) >> 1) + 2 * (k >> 4) + (k & 1);
-    v[k] = r <= ((k & 8) ? see1 : see0) ? v[k] : 0xFF800000u;
-  }
 }
 HV_DEV void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
   asm volatile(
@@ -197,15 +188,16 @@ struct TlShared {
   float top[4][kTlRows];         // of the last four tiles: what their weights are relative to
   float m[2][kTlRows], l[2][kTlRows];
   uint32_t tmem;
+  float open_max[2];             // of the open rows: largest |K|, |V|
   int bad;                       // first open row with a value that is not finite
   int given_up;
   unsigned last;
 };
-constexpr int kTlSmem = 4 * kTlTile + (int)sizeof(TlShared);   // K and V twice
+constexpr int kTlSmem = 4 * kTlTile + kTlRows * kTlLine * 4 + (int)sizeof(TlShared);   // K, V twice
 
 __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8 c) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  TlShared& sh = *reinterpret_cast<TlShared*>(smem + 4 * kTlTile);
+  TlShared& sh = *reinterpret_cast<TlShared*>(smem + 4 * kTlTile + kTlRows * kTlLine * 4);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kvh = blockIdx.y, tile = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   const int nrows = a.ntok * a.group, row0 = tile * kTlRows;
@@ -242,6 +234,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     bar_init(bar(sh.drain[1]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.bad = kQ8Blk;
+    sh.open_max[0] = sh.open_max[1] = 0.0f;
     sh.given_up = 0;
   }
   if (warp == 15) {
@@ -249,63 +242,65 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
                  :: "r"((uint32_t)__cvta_generic_to_shared(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // rows pass through shared memory on their way in and out, whole lines at a time
-  constexpr int kLine = kHd + 4;
-  float* lines = reinterpret_cast<float*>(smem);
-  for (int i = threadIdx.x; i < kTlRows * (kHd / 4); i += kTlThreads) {
-    const int r = row0 + i / (kHd / 4);
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < nrows)
-      x = __ldg(reinterpret_cast<const float4*>(
-                    a.q + ((size_t)(r / a.group) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd) +
-                i % (kHd / 4));
-    *reinterpret_cast<float4*>(lines + (size_t)(i / (kHd / 4)) * kLine + 4 * (i % (kHd / 4))) = x;
-  }
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = sh.tmem;
   volatile int* given_up = &sh.given_up;
   const int w = warp >> 2, row = threadIdx.x & 127, grow = row0 + row;
-  // the queries in two terms, a row per thread: the first ones from warps 0-3, the second from
-  // 4-7. They take the scale's sign, so that the largest sum of products is the largest exponent
-  const float qscale = __ldg(a.scale) * kLog2e;
-  float qs = 0.0f;
-  if (warp < 8) {
-    const float4* q = reinterpret_cast<const float4*>(lines + (size_t)row * kLine);
-    float amax = 0.0f;
-#pragma unroll 8
-    for (int d = 0; d < kHd / 4; ++d) {
-      const float4 x = q[d];
-      amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
-    }
-    const float lift = copysignf(q8_lift(amax), qscale);
-    qs = qscale / lift;
-    const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kTlColQ + 64 * w;
-    // dims in the order of K's tiles: 64 h + 16 s + 4 t + e stands at 64 h + 16 t + 4 s + e
-#pragma unroll 1
-    for (int d = 0; d < kHd / 4; d += 8) {
-      uint32_t v[16];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float4 x = q[(d & 16) + 4 * (k & 3) + ((d >> 2) & 2) + (k >> 2)];
-        uint32_t h0, h1, l0, l1;
-        split_half2(x.x * lift, x.y * lift, &h0, &l0);
-        split_half2(x.z * lift, x.w * lift, &h1, &l1);
-        v[2 * k] = w ? l0 : h0;
-        v[2 * k + 1] = w ? l1 : h1;
-      }
-      tmem_st16(to + 2 * d, v);
-    }
-    tmem_st_wait();
-  }
-  fence_before();
-  __syncthreads();
-  fence_after();
   const int ntile = gridDim.x / a.chunks;
   const size_t slot = ((size_t)kvh * ntile + tile) * a.chunks;
+  float* lines = reinterpret_cast<float*>(smem + 4 * kTlTile);    // [row][kTlLine]
+  auto rows_sync = [] { asm volatile("bar.sync 3, 256;" ::: "memory"); };
   if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsRow));
+    // The queries in two terms, a row per thread (whole lines at a time through shared memory):
+    // the first ones from warps 0-3, the second from 4-7. They take the scale's sign, so that
+    // the largest sum of products is the largest exponent.
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kTlRows * (kHd / 4); i += 256) {
+      const int r = row0 + i / (kHd / 4);
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < nrows)
+        x = __ldg(reinterpret_cast<const float4*>(
+                      a.q + ((size_t)(r / a.group) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd) +
+                  i % (kHd / 4));
+      *reinterpret_cast<float4*>(lines + (size_t)(i / (kHd / 4)) * kTlLine + 4 * (i % (kHd / 4))) = x;
+    }
+    const float qscale = __ldg(a.scale) * kLog2e;
+    rows_sync();
+    float qs;
+    {
+      const float4* q = reinterpret_cast<const float4*>(lines + (size_t)row * kTlLine);
+      float amax = 0.0f;
+#pragma unroll 4
+      for (int d = 0; d < kHd / 4; ++d) {
+        const float4 x = q[d];
+        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
+      }
+      const float lift = copysignf(q8_lift(amax), qscale);
+      qs = qscale / lift;
+      const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kTlColQ + 64 * w;
+      // dims in the order of K's tiles: 64 h + 16 s + 4 t + e stands at 64 h + 16 t + 4 s + e
+#pragma unroll 1
+      for (int d = 0; d < kHd / 4; d += 8) {
+        uint32_t v[16];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float4 x = q[(d & 16) + 4 * (k & 3) + ((d >> 2) & 2) + (k >> 2)];
+          uint32_t h0, h1, l0, l1;
+          split_half2(x.x * lift, x.y * lift, &h0, &l0);
+          split_half2(x.z * lift, x.w * lift, &h1, &l1);
+          v[2 * k] = w ? l0 : h0;
+          v[2 * k + 1] = w ? l1 : h1;
+        }
+        tmem_st16(to + 2 * d, v);
+      }
+      tmem_st_wait();
+    }
+    fence_before();
+    rows_sync();
+    fence_after();
     float m = -INFINITY, l = 0.0f;                // of this thread's row
     const uint32_t s_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * w;
     const int lim = grow < nrows ? min(min(a.pos0 + grow / a.group, held - 1), 32 * b1 - 1) : -1;
@@ -314,63 +309,83 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     // step k of 16 along the inner dimension: the half it is in, then 32 bytes each
     auto step = [](int k) { return (uint64_t)(((k >> 2) * kTlHalf + (k & 3) * 32) >> 4); };
     bool ok = true;
+    // the small terms first; with the open block, its values' second terms last
     auto product_s = [&](int i) {
-      const int s = i & 1;
+      const int s = i & 1, passes = has_tail && i == nt - 1 ? 3 : 2;
       const uint64_t kd = smem_desc(sm + s * kTlTile);
       const uint32_t d = tmem + 128 * s;
       ok = ok && bar_wait_warp(bar(sh.full_k[s]), (i >> 1) & 1, given_up);
-      if (!ok) return;
       fence_after();
+#pragma unroll 1
+      for (int pass = 0; pass < passes && ok; ++pass) {
+        if (pass == 2) {
+          mma_commit(bar(sh.k_free), leader);
+          ok = bar_wait_warp(bar(sh.full_k[s]), ((i >> 1) + 1) & 1, given_up);
+          if (!ok) break;
+          fence_after();
+        }
+        const uint32_t q = pass ? qh : ql;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) mma_ts(d, ql + 8 * k, kd + step(k), k > 0, leader);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mma_ts(d, qh + 8 * k, kd + step(k), true, leader);
-      if (has_tail && i == nt - 1) {
-        mma_commit(bar(sh.k_free), leader);
-        ok = bar_wait_warp(bar(sh.full_k[s]), ((i >> 1) + 1) & 1, given_up);
-        if (!ok) return;
-        fence_after();
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mma_ts(d, qh + 8 * k, kd + step(k), true, leader);
+        for (int k = 0; k < 8; ++k) mma_ts(d, q + 8 * k, kd + step(k), pass > 0 || k > 0, leader);
       }
       mma_commit(bar(sh.s_ready[s]), leader);
     };
     auto product_o = [&](int i) {
-      const int s = i & 1;
+      const int s = i & 1, passes = has_tail && i == nt - 1 ? 3 : 2;
       const uint64_t vd = smem_desc(sm + (2 + s) * kTlTile);
-      const uint32_t p = tmem + 128 * s, d = tmem + kTlColO;
+      const uint32_t d = tmem + kTlColO;
       ok = ok && bar_wait_warp(bar(sh.full_v[s]), (i >> 1) & 1, given_up);
       ok = ok && bar_wait_warp(bar(sh.w_ready[s]), (i >> 1) & 1, given_up);
       if (i > 0) ok = ok && bar_wait_warp(bar(sh.o_free), (i - 1) & 1, given_up);
-      if (!ok) return;
       fence_after();
-      // the weights of 16 positions are 8 columns of first terms, then 8 of second ones
+#pragma unroll 1
+      for (int pass = 0; pass < passes && ok; ++pass) {
+        if (pass == 2) {
+          mma_commit(bar(sh.v_free), leader);
+          ok = bar_wait_warp(bar(sh.full_v[s]), ((i >> 1) + 1) & 1, given_up);
+          if (!ok) break;
+          fence_after();
+        }
+        // the weights of 16 positions are 8 columns of first terms, then 8 of second ones
+        const uint32_t wt = tmem + 128 * s + (pass ? 0 : 8);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k + 8, vd + step(k), k > 0, leader);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k, vd + step(k), true, leader);
-      if (has_tail && i == nt - 1) {
-        mma_commit(bar(sh.v_free), leader);
-        ok = bar_wait_warp(bar(sh.full_v[s]), ((i >> 1) + 1) & 1, given_up);
-        if (!ok) return;
-        fence_after();
-#pragma unroll
-        for (int k = 0; k < 8; ++k) mma_ts(d, p + 16 * k, vd + step(k), true, leader);
+        for (int k = 0; k < 8; ++k) mma_ts(d, wt + 16 * k, vd + step(k), pass > 0 || k > 0, leader);
       }
       mma_commit(bar(sh.o_done[s]), leader);
     };
     const bool issues = (warp & 3) == 0;
-    if (issues && w < nt) product_s(w);
-    for (int i = w; i < nt; i += 2) {
+#pragma unroll 1
+    for (int i = w;; i += 2) {
+      if (issues) {
+        if (i >= 2) product_o(i - 2);
+        if (i < nt) product_s(i);
+      }
+      if (i >= nt) break;
       if (!bar_wait_warp(bar(sh.s_ready[w]), (i >> 1) & 1, given_up)) break;
       fence_after();
       const int see0 = lim - 32 * (b0 + 4 * i);            // positions 0 .. see0 are seen
       const bool all = __all_sync(0xFFFFFFFFu, see0 >= kTlRows - 1);
       const float (&sc)[4][4] = sh.sc[i & 3];
+      if (!all) {
+        // columns of positions that the row does not see become -infinity
+#pragma unroll 1
+        for (int h = 0; h < 8; ++h) {
+          uint32_t x[16];
+          tmem_ld16(s_at + 16 * h, x);
+          tmem_wait(x);
+          const int see = see0 - 64 * (h >> 2) - 2 * (h & 3);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) {
+            const int r = 32 * (k >> 3) + 8 * ((k & 7) >> 1) + (k & 1);
+            x[k] = r <= see ? x[k] : 0xFF800000u;
+          }
+          tmem_st16(s_at + 16 * h, x);
+        }
+        tmem_st_wait();
+      }
+      // The largest exponent of the row in this tile. Here and below loops stay as rolled as
+      // the two buffers allow: the code of all roles has to fit the instruction cache.
       uint32_t v[2][32];
-      // the largest exponent of the row in this tile
-      // (loops over pairs of blocks stay rolled: the code of all roles has to fit the
-      // instruction cache)
       float up = m;
       tmem_ld32(s_at, v[0]);
 #pragma unroll 1
@@ -381,8 +396,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         for (int h = 0; h < 2; ++h) {
           uint32_t (&x)[32] = v[h];
           tmem_wait(x);
-          tmem_ld32(s_at + 32 * ((b + h + 1) & 3), v[1 - h]);
-          if (__builtin_expect(!all, 0)) hide(x, see - 4 * h, see - 4 * h - 32);
+          if (h == 0 || b == 0) tmem_ld32(s_at + 32 * (b + h + 1), v[1 - h]);
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
             float& y = mx[((k >> 3) & 1) + 2 * (k & 1)];
@@ -396,10 +410,10 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       m = up;
       sh.top[i & 3][row] = m;
       const float m0 = m == -INFINITY ? 0.0f : m;
-      // the first columns are under way again
+      uint32_t z[2][16];
+      tmem_ld16(s_at, z[0]);
 #pragma unroll 1
       for (int b = 0; b < 4; b += 2) {
-        const int see = see0 - 32 * b;
         uint64_t f2[2], lv2[2], sum[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -408,19 +422,18 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
           f2[e] = pair(f, f);
           lv2[e] = pair(sc[b + e][1] - m0, sc[b + e][1] - m0);
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t (&x)[32] = v[h];
-          tmem_wait(x);
-          if (h == 0 || b == 0) tmem_ld32(s_at + 32 * (b + h + 1), v[1 - h]);
-          if (__builtin_expect(!all, 0)) hide(x, see - 4 * h, see - 4 * h - 32);
+#pragma unroll 1
+        for (int h = 0; h < 4; h += 2) {
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
+            uint32_t (&x)[16] = z[g];
+            tmem_wait(x);
+            if (g == 0 || b + h < 4) tmem_ld16(s_at + 32 * b + 16 * (h + g) + 16, z[1 - g]);
             // 16 positions: 8 columns of first terms, 8 of second ones
             uint32_t wt[16];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const uint64_t s2 = pair(__uint_as_float(x[16 * g + 2 * k]), __uint_as_float(x[16 * g + 2 * k + 1]));
+              const uint64_t s2 = pair(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1]));
               const float2 e = unpair(fma2(s2, f2[k >> 2], lv2[k >> 2]));
               const uint64_t p2 = mul2(pair(ex2(e.x), ex2(e.y)), pair(kTlLift, kTlLift));
               sum[k >> 2] = add2(sum[k >> 2], p2);
@@ -432,7 +445,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
               wt[k] = pack_half2(c1.x, c1.y);
               wt[8 + k] = pack_half2(r.x, r.y);
             }
-            tmem_st16(s_at + 32 * (b + h) + 16 * g, wt);
+            tmem_st16(s_at + 32 * b + 16 * (h + g), wt);
           }
         }
         const float2 s0 = unpair(sum[0]), s1 = unpair(sum[1]);
@@ -443,10 +456,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       tmem_st_wait();
       fence_before();
       bar_arrive(bar(sh.w_ready[w]));
-      if (issues) {
-        product_o(i);
-        if (i + 2 < nt) product_s(i + 2);
-      }
     }
     if (issues && !ok) {                          // what was issued ends before the memory goes
       int no = 0;
@@ -499,7 +508,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       if (a.pos0 + grow / a.group >= held) L = nan;
     }
     const float f = nact > 1 ? 1.0f : L;
-    float* line = lines + (size_t)row * kLine;
+    float* line = lines + (size_t)row * kTlLine;
 #pragma unroll
     for (int d = 0; d < kHd / 2; d += 2) {
       const float2 x = unpair(acc[d]), y = unpair(acc[d + 1]);
@@ -511,7 +520,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     asm volatile("bar.sync 2, 128;" ::: "memory");
     for (int i = threadIdx.x & 127; i < kTlRows * (kHd / 4); i += 128) {
       const int n = i / (kHd / 4), d = i % (kHd / 4), r = row0 + n;
-      const float4 x = *reinterpret_cast<const float4*>(lines + (size_t)n * kLine + 4 * d);
+      const float4 x = *reinterpret_cast<const float4*>(lines + (size_t)n * kTlLine + 4 * d);
       if (nact > 1)
         reinterpret_cast<float4*>(part)[i] = x;
       else if (r < nrows)
@@ -528,7 +537,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     const int nopen = held - closed * kQ8Blk;
     // the codes of the next tile are loaded while this one's are worked on
     uint4 kx[8], vx[8];
-    float2 sc = make_float2(1.f, 1.f), sc_next;
     auto live = [&](int i) { return i < nt && b0 + 4 * i + cw < min(b1, nb); };
     auto fetch = [&](int i, int which, uint4 (&x)[8]) {
       if (live(i)) {
@@ -537,18 +545,18 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         for (int u = 0; u < 8; ++u) x[u] = __ldg(reinterpret_cast<const uint4*>(src + 512 * u));
       }
     };
-    auto put_k = [&](uint8_t* to, int j, int h, const uint32_t (&x)[8]) {
-      // position 8 j + g of block cw, dims 64 h + 16 s + 4 t .. for s = 0 .. 3
-      const int n = 64 * (cw >> 1) + 16 * (g >> 1) + 8 * (cw & 1) + 2 * j + (g & 1);
+    auto put_k = [&](uint8_t* to, int c, int j, int h, const uint32_t (&x)[8]) {
+      // position 8 j + g of block c, dims 64 h + 16 s + 4 t .. for s = 0 .. 3
+      const int n = 64 * (c >> 1) + 16 * (g >> 1) + 8 * (c & 1) + 2 * j + (g & 1);
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        *reinterpret_cast<uint4*>(to + h * kTlHalf + n * 128 + (((2 * t + c) ^ (n & 7)) << 4)) =
-            make_uint4(x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]);
+      for (int e = 0; e < 2; ++e)
+        *reinterpret_cast<uint4*>(to + h * kTlHalf + n * 128 + (((2 * t + e) ^ (n & 7)) << 4)) =
+            make_uint4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]);
     };
-    auto put_v = [&](uint8_t* to, int u, int h, const uint32_t (&x)[4]) {
-      // dim 16 u + 8 h + g, positions 8 j + 2 t .. of block cw for j = 0 .. 3
-      *reinterpret_cast<uint4*>(to + (cw >> 1) * kTlHalf + (16 * u + 8 * h + g) * 128 +
-                                (((2 * t + (cw & 1)) ^ g) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
+    auto put_v = [&](uint8_t* to, int c, int u, int h, const uint32_t (&x)[4]) {
+      // dim 16 u + 8 h + g, positions 8 j + 2 t .. of block c for j = 0 .. 3
+      *reinterpret_cast<uint4*>(to + (c >> 1) * kTlHalf + (16 * u + 8 * h + g) * 128 +
+                                (((2 * t + (c & 1)) ^ g) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
     };
     // the open rows' values in one of their two terms (second: 1)
     float lk = 1.0f, lv = 1.0f;
@@ -559,137 +567,183 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       split_half2(x0, x1, &hi, &lo);
       return second ? lo : hi;
     };
+    // all four warps share the open block, block `oc` of its tile: two units of K and four of V
+    // each, several loads under way at a time
+    const int oc = (nb - b0) & 3;
     auto open_k = [&](uint8_t* to, int second) {
-#pragma unroll 1
-      for (int u = 0; u < 8; ++u) {
-        const int r = 8 * (u >> 1) + g;
+      float4 x[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const int r = 8 * cw + g;
+          x[i][s] = r < nopen ? __ldg(reinterpret_cast<const float4*>(open + r * kHd + 64 * i + 16 * s + 4 * t))
+                              : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
         uint32_t y[8];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (r < nopen)
-            x = __ldg(reinterpret_cast<const float4*>(open + r * kHd + 64 * (u & 1) + 16 * s + 4 * t));
-          y[2 * s] = term(x.x, x.y, lk, second);
-          y[2 * s + 1] = term(x.z, x.w, lk, second);
+          y[2 * s] = term(x[i][s].x, x[i][s].y, lk, second);
+          y[2 * s + 1] = term(x[i][s].z, x[i][s].w, lk, second);
         }
-        put_k(to, u >> 1, u & 1, y);
+        put_k(to, oc, cw, i, y);
       }
     };
     auto open_v = [&](uint8_t* to, int second) {
 #pragma unroll 1
-      for (int uh = 0; uh < 16; ++uh) {
-        uint32_t y[4];
+      for (int i0 = 0; i0 < 4; i0 += 2) {
+        float x[2][8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = 8 * j + 2 * t, d = 8 * uh + g;
-          const float x0 = r < nopen ? __ldg(open + kQ8Codes + r * kHd + d) : 0.0f;
-          const float x1 = r + 1 < nopen ? __ldg(open + kQ8Codes + (r + 1) * kHd + d) : 0.0f;
-          y[j] = term(x0, x1, lv, second);
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int r = 8 * (j >> 1) + 2 * t + (j & 1), d = 8 * (4 * cw + i0 + i) + g;
+            x[i][j] = r < nopen ? __ldg(open + kQ8Codes + r * kHd + d) : 0.0f;
+          }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = term(x[i][2 * j], x[i][2 * j + 1], lv, second);
+          put_v(to, oc, 2 * cw + (i0 >> 1), i, y);
         }
-        put_v(to, uh >> 1, uh & 1, y);
       }
+    };
+    // the largest of the open rows' values, eight rows a warp
+    auto open_scan = [&] {
+      float mk = 0.0f, mv = 0.0f;
+#pragma unroll 1
+      for (int i0 = 0; i0 < 8; i0 += 4) {
+        float4 x[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = 8 * cw + i0 + i;
+            x[i][e] = r < nopen ? __ldg(reinterpret_cast<const float4*>(open + e * kQ8Codes + r * kHd) + lane)
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& m = e ? mv : mk;
+            const float v[4] = {fabsf(x[i][e].x), fabsf(x[i][e].y), fabsf(x[i][e].z), fabsf(x[i][e].w)};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if (v[k] < INFINITY) m = fmaxf(m, v[k]);
+              else atomicMin(&sh.bad, 8 * cw + i0 + i);
+            }
+          }
+      }
+      atomicMax(reinterpret_cast<int*>(&sh.open_max[0]), __float_as_int(mk));
+      atomicMax(reinterpret_cast<int*>(&sh.open_max[1]), __float_as_int(mv));
+      asm volatile("bar.sync 4, 128;" ::: "memory");
+      lk = q8_lift(sh.open_max[0]);
+      // values up to 2^10: their scale is then near that of coded values, which is what a
+      // weight's precision goes by
+      lv = q8_lift(sh.open_max[1]) * 0.0625f;
     };
     auto none_k = [&](uint8_t* to) {
       const uint32_t y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
-      for (int u = 0; u < 8; ++u) put_k(to, u >> 1, u & 1, y);
+      for (int u = 0; u < 8; ++u) put_k(to, cw, u >> 1, u & 1, y);
     };
     auto none_v = [&](uint8_t* to) {
       const uint32_t y[4] = {0, 0, 0, 0};
 #pragma unroll 1
-      for (int uh = 0; uh < 16; ++uh) put_v(to, uh >> 1, uh & 1, y);
+      for (int uh = 0; uh < 16; ++uh) put_v(to, cw, uh >> 1, uh & 1, y);
     };
-    fetch(0, 0, kx);
-    fetch(0, 1, vx);
-    sc_next = live(0) ? __ldg(scales + b0 + cw) : sc;
-    for (int i = 0; i < nt; ++i) {
-      const int s = i & 1;
-      uint8_t* kt = k_buf + s * kTlTile;
-      uint8_t* vt = v_buf + s * kTlTile;
-      const bool two = has_tail && i == nt - 1;             // this tile ends with the open block
-      const bool mine = two && b0 + 4 * i + cw == closed;   // and this warp has it
-      sc = sc_next;
-      sc_next = live(i + 1) ? __ldg(scales + b0 + 4 * (i + 1) + cw) : make_float2(1.f, 1.f);
-      if (i >= 2 && !bar_wait_warp(bar(sh.s_ready[s]), ((i - 2) >> 1) & 1, given_up)) break;
-      if (mine) {
-        float mk = 0.0f, mv = 0.0f;
-        for (int r = 0; r < nopen; ++r) {
-          const float4 x = __ldg(reinterpret_cast<const float4*>(open + r * kHd) + lane);
-          const float4 y = __ldg(reinterpret_cast<const float4*>(open + kQ8Codes + r * kHd) + lane);
-          const float e[8] = {fabsf(x.x), fabsf(x.y), fabsf(x.z), fabsf(x.w),
-                              fabsf(y.x), fabsf(y.y), fabsf(y.z), fabsf(y.w)};
+    auto coded_k = [&](int i, uint8_t* to) {
+      if (!live(i)) return none_k(to);          // past the chunk's last block
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if (!(e[k] < INFINITY)) atomicMin(&sh.bad, r);
-            else if (k < 4) mk = fmaxf(mk, e[k]);
-            else mv = fmaxf(mv, e[k]);
-          }
-        }
+      for (int u = 0; u < 8; ++u) {
+        const uint32_t x[4] = {kx[u].x, kx[u].y, kx[u].z, kx[u].w};
+        uint32_t y[8];
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          mk = fmaxf(mk, __shfl_xor_sync(0xFFFFFFFFu, mk, o));
-          mv = fmaxf(mv, __shfl_xor_sync(0xFFFFFFFFu, mv, o));
-        }
-        lk = q8_lift(mk);
-        // values up to 2^10: their scale is then near that of coded values, which is what a
-        // weight's precision goes by
-        lv = q8_lift(mv) * 0.0625f;
-        sc = make_float2(1.0f / lk, 1.0f / lv);
-        open_k(kt, 0);
-      } else if (!live(i)) {                    // past the chunk's last block
-        none_k(kt);
-      } else {
+        for (int k = 0; k < 4; ++k) q8_halves(x[k], &y[2 * k], &y[2 * k + 1]);
+        put_k(to, cw, u >> 1, u & 1, y);
+      }
+    };
+    auto coded_v = [&](int i, uint8_t* to) {
+      if (!live(i)) return none_v(to);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const uint32_t x[4] = {kx[u].x, kx[u].y, kx[u].z, kx[u].w};
-          uint32_t y[8];
+      for (int u = 0; u < 8; ++u) {
+        const uint32_t x[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) q8_halves(x[k], &y[2 * k], &y[2 * k + 1]);
-          put_k(kt, u >> 1, u & 1, y);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t y[4];
+          q8_halves(x[2 * h], &y[0], &y[1]);
+          q8_halves(x[2 * h + 1], &y[2], &y[3]);
+          put_v(to, cw, u, h, y);
         }
       }
+    };
+    auto put_scales = [&](int i, float sk, float sv) {
       if (lane == 0) {
         // a scale under 2^-120 counts as that, so that its reciprocal is a number; a NaN stays
-        const float sv = sc.y < 0x1p-120f ? 0x1p-120f : sc.y;
-        sh.sc[i & 3][cw][0] = sc.x;
+        sv = sv < 0x1p-120f ? 0x1p-120f : sv;
+        sh.sc[i & 3][cw][0] = sk;
         sh.sc[i & 3][cw][1] = log2f(sv);
         sh.sc[i & 3][cw][2] = sv == sv ? 1.0f / sv : 0.0f;
       }
+    };
+    auto scales_of = [&](int i) { return live(i) ? __ldg(scales + b0 + 4 * i + cw) : make_float2(1.f, 1.f); };
+    fetch(0, 0, kx);
+    fetch(0, 1, vx);
+    float2 sc = scales_of(0);
+    const int coded = nt - (has_tail ? 1 : 0);  // tiles without the open block
+    bool ok = true;
+#pragma unroll 1
+    for (int i = 0; i < coded && ok; ++i) {
+      const int s = i & 1;
+      ok = i < 2 || bar_wait_warp(bar(sh.s_ready[s]), ((i - 2) >> 1) & 1, given_up);
+      if (!ok) break;
+      coded_k(i, k_buf + s * kTlTile);
+      put_scales(i, sc.x, sc.y);
       fence_async();
       bar_arrive(bar(sh.full_k[s]));
       fetch(i + 1, 0, kx);
-      if (two) {
-        if (!bar_wait_warp(bar(sh.k_free), 0, given_up)) break;
-        if (mine) open_k(kt, 1);
-        else none_k(kt);
-        fence_async();
-        bar_arrive(bar(sh.full_k[s]));
-      }
-      if (i >= 2 && !bar_wait_warp(bar(sh.o_done[s]), ((i - 2) >> 1) & 1, given_up)) break;
-      if (mine) {
-        open_v(vt, 0);
-      } else if (!live(i)) {
-        none_v(vt);
-      } else {
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const uint32_t x[4] = {vx[u].x, vx[u].y, vx[u].z, vx[u].w};
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint32_t y[4];
-            q8_halves(x[2 * h], &y[0], &y[1]);
-            q8_halves(x[2 * h + 1], &y[2], &y[3]);
-            put_v(vt, u, h, y);
-          }
-        }
-      }
+      sc = scales_of(i + 1);
+      ok = i < 2 || bar_wait_warp(bar(sh.o_done[s]), ((i - 2) >> 1) & 1, given_up);
+      if (!ok) break;
+      coded_v(i, v_buf + s * kTlTile);
       fence_async();
       bar_arrive(bar(sh.full_v[s]));
       fetch(i + 1, 1, vx);
-      if (two) {
-        if (!bar_wait_warp(bar(sh.v_free), 0, given_up)) break;
-        if (mine) open_v(vt, 1);
-        else none_v(vt);
+    }
+    if (has_tail && ok) {
+      // the last tile, twice: with the open block's first terms and what comes before it, then
+      // with its second terms alone
+      const int i = nt - 1, s = i & 1;
+      uint8_t* kt = k_buf + s * kTlTile;
+      uint8_t* vt = v_buf + s * kTlTile;
+      const bool mine = b0 + 4 * i + cw == closed;          // the open block is this warp's
+      ok = i < 2 || bar_wait_warp(bar(sh.s_ready[s]), ((i - 2) >> 1) & 1, given_up);
+      if (ok && !mine) coded_k(i, kt);
+      if (ok) open_scan();
+      put_scales(i, mine ? 1.0f / lk : sc.x, mine ? 1.0f / lv : sc.y);
+#pragma unroll 1
+      for (int pass = 0; pass < 2 && ok; ++pass) {
+        if (pass) {
+          ok = bar_wait_warp(bar(sh.k_free), 0, given_up);
+          if (!mine) none_k(kt);
+        }
+        open_k(kt, pass);
+        fence_async();
+        bar_arrive(bar(sh.full_k[s]));
+      }
+      ok = ok && (i < 2 || bar_wait_warp(bar(sh.o_done[s]), ((i - 2) >> 1) & 1, given_up));
+      if (ok && !mine) coded_v(i, vt);
+#pragma unroll 1
+      for (int pass = 0; pass < 2 && ok; ++pass) {
+        if (pass) {
+          ok = bar_wait_warp(bar(sh.v_free), 0, given_up);
+          if (!mine) none_v(vt);
+        }
+        open_v(vt, pass);
         fence_async();
         bar_arrive(bar(sh.full_v[s]));
       }
@@ -711,7 +765,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   __syncthreads();
   if (!sh.last) return;
   __threadfence();
-  rows_join<kTlRows>(a, kvh, slot, nact, row0, nrows, held);
+  rows_join<kTlRows>(a, kvh, slot, nact, row0, nrows, held, reinterpret_cast<float*>(smem));
 }
 
 }  // namespace
