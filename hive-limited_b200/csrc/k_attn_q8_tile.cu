@@ -252,32 +252,53 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   const size_t slot = ((size_t)kvh * ntile + tile) * a.chunks;
   float* lines = reinterpret_cast<float*>(smem + 4 * kTlTile);    // [row][kTlLine]
   auto rows_sync = [] { asm volatile("bar.sync 3, 256;" ::: "memory"); };
+  // the rows' sums, once they stand in `lines`: to ctx, or to this chunk's part of the scratch
+  auto rows_out = [&] {
+    asm volatile("bar.sync 2, 384;" ::: "memory");
+    float4* part = reinterpret_cast<float4*>(a.part + (slot + chunk) * rows_part(kTlRows));
+#pragma unroll 4
+    for (int r = warp; r < kTlRows; r += 12) {
+      const float4 x = *reinterpret_cast<const float4*>(lines + (size_t)r * kTlLine + 4 * lane);
+      const int gr = row0 + r, tok = gr / a.group;
+      if (nact > 1)
+        part[r * (kHd / 4) + lane] = x;
+      else if (gr < nrows)
+        reinterpret_cast<float4*>(a.ctx + ((size_t)tok * a.nq + (size_t)kvh * a.group + gr - tok * a.group) * kHd)[lane] = x;
+    }
+    if (nact > 1) __threadfence();
+  };
   if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsRow));
     // The queries in two terms, a row per thread (whole lines at a time through shared memory):
     // the first ones from warps 0-3, the second from 4-7. They take the scale's sign, so that
     // the largest sum of products is the largest exponent.
+    {
+      // a warp takes rows warp, warp + 8, ..., all of them under way at once
+      const uint32_t to = sm + 4 * kTlTile + 16 * lane;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < kTlRows * (kHd / 4); i += 256) {
-      const int r = row0 + i / (kHd / 4);
-      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < nrows)
-        x = __ldg(reinterpret_cast<const float4*>(
-                      a.q + ((size_t)(r / a.group) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd) +
-                  i % (kHd / 4));
-      *reinterpret_cast<float4*>(lines + (size_t)(i / (kHd / 4)) * kTlLine + 4 * (i % (kHd / 4))) = x;
+      for (int r = warp; r < kTlRows; r += 8) {
+        const int gr = min(row0 + r, nrows - 1), tok = gr / a.group;
+        const float* src = a.q + ((size_t)tok * a.nq + (size_t)kvh * a.group + gr - tok * a.group) * kHd + 4 * lane;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                     :: "r"(to + r * kTlLine * 4), "l"(src) : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
     const float qscale = __ldg(a.scale) * kLog2e;
     rows_sync();
     float qs;
     {
+      // each of a row's two threads looks over half of it
       const float4* q = reinterpret_cast<const float4*>(lines + (size_t)row * kTlLine);
       float amax = 0.0f;
 #pragma unroll 4
-      for (int d = 0; d < kHd / 4; ++d) {
-        const float4 x = q[d];
+      for (int d = 0; d < kHd / 8; ++d) {
+        const float4 x = q[(kHd / 8) * w + d];
         amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
       }
+      sh.m[w][row] = amax;
+      rows_sync();
+      amax = fmaxf(amax, sh.m[1 - w][row]);
       const float lift = copysignf(q8_lift(amax), qscale);
       qs = qscale / lift;
       const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kTlColQ + 64 * w;
@@ -465,6 +486,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     sh.m[w][row] = m;
     sh.l[w][row] = l;
     asm volatile("bar.sync 1, 384;" ::: "memory");         // with the warps that have the sums
+    rows_out();
   } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kTlRegsSum));
     uint64_t acc[kHd / 2];
@@ -517,16 +539,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     float* part = a.part + (slot + chunk) * rows_part(kTlRows);
     if (nact > 1)
       *reinterpret_cast<float2*>(part + kTlRows * kHd + 2 * row) = make_float2(M, L);
-    asm volatile("bar.sync 2, 128;" ::: "memory");
-    for (int i = threadIdx.x & 127; i < kTlRows * (kHd / 4); i += 128) {
-      const int n = i / (kHd / 4), d = i % (kHd / 4), r = row0 + n;
-      const float4 x = *reinterpret_cast<const float4*>(lines + (size_t)n * kTlLine + 4 * d);
-      if (nact > 1)
-        reinterpret_cast<float4*>(part)[i] = x;
-      else if (r < nrows)
-        reinterpret_cast<float4*>(a.ctx + ((size_t)(r / a.group) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd)[d] = x;
-    }
-    if (nact > 1) __threadfence();
+    rows_out();
   } else if (warp < 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsConv));
     // a warp per block of the tile
