@@ -342,18 +342,37 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   if (!s_last) return;
   __threadfence();
   const float* base = part + (size_t)kvh * gridDim.x * kDecPart;
-  for (int i = threadIdx.x; i < vals; i += blockDim.x) {
-    const int h = i / kHd;
-    float M = -INFINITY, L = 0.0f, A = 0.0f;
-    for (int k = 0; k < nact; ++k) M = fmaxf(M, __ldcg(base + (size_t)k * kDecPart + 8 * kHd + 2 * h));
+  float2* ml = reinterpret_cast<float2*>(smem);          // [chunk][head]: (max, sum), then factors
+  for (int i = threadIdx.x; i < nact * 8; i += blockDim.x)
+    if ((i & 7) < group)
+      ml[i] = __ldcg(reinterpret_cast<const float2*>(base + (size_t)(i >> 3) * kDecPart + 8 * kHd) + (i & 7));
+  __syncthreads();
+  if (warp < group) {                                    // a warp per head
+    float M = -INFINITY, L = 0.0f;
+    for (int k = lane; k < nact; k += 32) M = fmaxf(M, ml[8 * k + warp].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+    for (int k = lane; k < nact; k += 32) {
+      const float f = ex2(ml[8 * k + warp].x - M);
+      L += f * ml[8 * k + warp].y;
+      ml[8 * k + warp].x = f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, o);
+    if (lane == 0) s_l[0][warp] = L;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < vals / 4; i += blockDim.x) {
+    const int h = i / (kHd / 4);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int k = 0; k < nact; ++k) {
-      const float* p = base + (size_t)k * kDecPart;
-      const float a = ex2(__ldcg(p + 8 * kHd + 2 * h) - M);
-      L += a * __ldcg(p + 8 * kHd + 2 * h + 1);
-      A += a * __ldcg(p + i);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(base + (size_t)k * kDecPart) + i);
+      const float f = ml[8 * k + h].x;
+      s.x += f * x.x; s.y += f * x.y; s.z += f * x.z; s.w += f * x.w;
     }
-    out[i] = A / L;
+    const float L = s_l[0][h];
+    reinterpret_cast<float4*>(out)[i] = make_float4(s.x / L, s.y / L, s.z / L, s.w / L);
   }
 }
 
