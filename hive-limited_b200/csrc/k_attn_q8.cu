@@ -27,12 +27,14 @@ namespace {
 // between a head's chunks, in the caller's scratch, where the last CTA to arrive adds them
 // in chunk order.
 constexpr int kDecWarps = 8;
-constexpr int kDecStages = 3;
+constexpr int kDecStages = 2;
 constexpr int kDecBlocksMin = 8;       // blocks a chunk holds before a head gets another CTA
 constexpr int kDecStride = 132;        // floats between the columns of a warp's sums
 constexpr int kDecTickets = 1024;      // kv heads with chunks to join: first in the scratch
 constexpr int kDecPart = 8 * (kHd + 2);    // scratch floats of a chunk: sums, then (max, sum)
-constexpr int kDecSmem = kDecWarps * kDecStages * 2 * kQ8Codes;
+constexpr int kDecLine = kHd + 4;      // floats between rows that a warp reads four at a time
+constexpr int kDecRing = kDecWarps * kDecStages * 2 * kQ8Codes;
+constexpr int kDecSmem = kDecRing + kQ8Blk * (kDecLine + kHd) * 4;     // then the open rows
 
 HV_DEV void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
@@ -44,7 +46,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
                   const float* __restrict__ scale, const int32_t* __restrict__ pos_p, int group,
                   float* __restrict__ part, unsigned* __restrict__ ticket) {
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float s_m[kDecWarps][8], s_l[kDecWarps][8], s_q[8][kHd];
+  __shared__ float s_m[kDecWarps][8], s_l[kDecWarps][8], s_x[kQ8Blk][8];
+  __shared__ __align__(16) float s_q[8][kDecLine];
   __shared__ unsigned s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, chunk = blockIdx.x;
@@ -77,6 +80,18 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  // the open block's rows go first, to the CTA with the last chunk
+  const bool open = chunk == nact - 1 && ntail > 0;
+  float* open_k = reinterpret_cast<float*>(smem + kDecRing);           // [row][kDecLine]
+  float* open_v = open_k + kQ8Blk * kDecLine;                          // [row][kHd]
+  if (open) {
+    const float* src = c.tail + (size_t)kvh * 2 * kQ8Codes + 4 * lane;
+    for (int r = warp; r < ntail; r += kDecWarps) {
+      cp_async16((uint32_t)__cvta_generic_to_shared(open_k + r * kDecLine + 4 * lane), src + r * kHd);
+      cp_async16((uint32_t)__cvta_generic_to_shared(open_v + r * kHd + 4 * lane), src + kQ8Codes + r * kHd);
+    }
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < kDecStages; ++i) fetch(b0 + warp + i * kDecWarps, i);
   float2 sc_next = make_float2(0.f, 0.f);
@@ -138,6 +153,53 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       for (int u = 0; u < 8; ++u) { acc[u][0] *= a0; acc[u][1] *= a1; acc[u][2] *= a0; acc[u][3] *= a1; }
     }
   };
+
+  if (open) {                                    // in f32, while the first blocks come in
+    asm volatile("cp.async.wait_group %0;" :: "n"(kDecStages) : "memory");
+    __syncthreads();
+    const int xr = threadIdx.x >> 3, xh = threadIdx.x & 7;     // a thread per row and head
+    if (xr < ntail && xh < group) {
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int d = 0; d < kHd; d += 4) {
+        const float4 k = *reinterpret_cast<const float4*>(open_k + xr * kDecLine + d);
+        const float4 x = *reinterpret_cast<const float4*>(&s_q[xh][d]);
+        v[0] = fmaf(k.x, x.x, v[0]);
+        v[1] = fmaf(k.y, x.y, v[1]);
+        v[2] = fmaf(k.z, x.z, v[2]);
+        v[3] = fmaf(k.w, x.w, v[3]);
+      }
+      s_x[xr][xh] = ((v[0] + v[1]) + (v[2] + v[3])) * qscale;
+    }
+    __syncthreads();
+    float x0[4], x1[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = warp + kDecWarps * i;
+      x0[i] = r < ntail && head0 < group ? s_x[r][head0] : -INFINITY;
+      x1[i] = r < ntail && head0 + 1 < group ? s_x[r][head0 + 1] : -INFINITY;
+    }
+    raise(fmaxf(fmaxf(x0[0], x0[1]), fmaxf(x0[2], x0[3])),
+          fmaxf(fmaxf(x1[0], x1[1]), fmaxf(x1[2], x1[3])));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = warp + kDecWarps * i;
+      if (r >= ntail) continue;
+      const float p0 = head0 < group ? ex2(x0[i] - m0) * 32768.0f : 0.0f;
+      const float p1 = head0 + 1 < group ? ex2(x1[i] - m1) * 32768.0f : 0.0f;
+      if (gl == 0) { l0 += p0; l1 += p1; }
+      if (kTwo || t < 2) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const float va = open_v[r * kHd + 16 * u + gl], vb = open_v[r * kHd + 16 * u + 8 + gl];
+          acc[u][0] = fmaf(p0, va, acc[u][0]);
+          acc[u][1] = fmaf(p1, va, acc[u][1]);
+          acc[u][2] = fmaf(p0, vb, acc[u][2]);
+          acc[u][3] = fmaf(p1, vb, acc[u][3]);
+        }
+      }
+    }
+  }
 
   int stage = 0;
   for (int b = b0 + warp; b < b1; b += kDecWarps) {
@@ -230,49 +292,6 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     stage = stage + 1 == kDecStages ? 0 : stage + 1;
   }
 
-  if (chunk == nact - 1 && ntail > 0) {          // the open block's rows, in f32
-    __syncthreads();                             // s_q
-    const float* tail = c.tail + (size_t)kvh * 2 * kQ8Codes;
-    float x0[4], x1[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = warp + kDecWarps * i;
-      x0[i] = x1[i] = -INFINITY;
-      if (r < ntail) {
-        const float4 k = __ldg(reinterpret_cast<const float4*>(tail + r * kHd) + lane);
-        for (int h = 0; h < group; ++h) {
-          const float4 w = *reinterpret_cast<const float4*>(&s_q[h][4 * lane]);
-          float v = k.x * w.x + k.y * w.y + k.z * w.z + k.w * w.w;
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
-          v *= qscale;
-          if (h == head0) x0[i] = v;
-          if (h == head0 + 1) x1[i] = v;
-        }
-      }
-    }
-    raise(fmaxf(fmaxf(x0[0], x0[1]), fmaxf(x0[2], x0[3])),
-          fmaxf(fmaxf(x1[0], x1[1]), fmaxf(x1[2], x1[3])));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = warp + kDecWarps * i;
-      if (r >= ntail) continue;
-      const float p0 = head0 < group ? ex2(x0[i] - m0) * 32768.0f : 0.0f;
-      const float p1 = head0 + 1 < group ? ex2(x1[i] - m1) * 32768.0f : 0.0f;
-      if (gl == 0) { l0 += p0; l1 += p1; }
-      if (kTwo || t < 2) {
-        const float* v = tail + kQ8Codes + r * kHd;
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float va = __ldg(v + 16 * u + gl), vb = __ldg(v + 16 * u + 8 + gl);
-          acc[u][0] = fmaf(p0, va, acc[u][0]);
-          acc[u][1] = fmaf(p1, va, acc[u][1]);
-          acc[u][2] = fmaf(p0, vb, acc[u][2]);
-          acc[u][3] = fmaf(p1, vb, acc[u][3]);
-        }
-      }
-    }
-  }
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
     l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, o);
