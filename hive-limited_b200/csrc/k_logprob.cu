@@ -19,14 +19,13 @@ namespace hv {
 namespace {
 
 constexpr int kMaxTop = 32;
-constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32;
-constexpr int kLpEach = 8;                        // logits a thread holds of a tile
-constexpr int kLpTile = kLpThreads * kLpEach;
-constexpr int kLpBuf = 2048;                      // candidates a CTA keeps in shared memory
+constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
+constexpr int kLpEach = 8;                        // logits a thread holds at a time
+constexpr int kLpBatch = 32 * kLpEach;            // a warp's
+constexpr int kLpTile = kLpWarps * kLpBatch;      // a CTA's
 constexpr int kLpPieces = 64;                     // CTAs that may share a row
 constexpr int kLpTickets = 1024;                  // rows that may be shared; their tickets stand
                                                   // first in the scratch whatever the call
-static_assert(kLpPieces * kMaxTop <= kLpBuf && kMaxTop * kLpEach <= kLpBuf, "candidates fit");
 
 using u64 = unsigned long long;
 
@@ -100,11 +99,8 @@ HV_DEV LpSum lp_join(LpSum a, LpSum b) {
 }
 
 struct LpShared {
-  u64 buf[kLpBuf];
   u64 lists[kLpWarps][32];
   LpSum sums[kLpWarps];
-  int count;                 // candidates in buf
-  int more;                  // candidates of the current tile
   unsigned last;
 };
 
@@ -120,22 +116,51 @@ HV_DEV u64 block_merge(u64 v, LpShared& sh) {
   return v;
 }
 
-// The 32 largest of the first n candidates, falling, in warp 0.
-HV_DEV u64 block_select(int n, LpShared& sh) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  u64 v = 0;
-  for (int i = warp * 32; i < n; i += kLpThreads) {
-    const u64 w = warp_sort(i + lane < n ? sh.buf[i + lane] : 0);
-    v = i == warp * 32 ? w : warp_merge(v, w);
+HV_DEV u64 shfl64(u64 v, int src) { return __shfl_sync(0xFFFFFFFFu, v, src); }
+
+// Takes a batch's logits (of ids id + (k & 3) + 128 (k >> 2)) into the warp's falling list of 32:
+// lane by lane its largest, then its next, while any is above the list's `top`th. Few of them are
+// put in one by one, many are sorted and merged.
+HV_DEV u64 warp_take(u64 list, const float (&v)[kLpEach], int id, int n, int top) {
+  const int lane = threadIdx.x & 31;
+  unsigned left = 0;
+#pragma unroll
+  for (int k = 0; k < kLpEach; ++k) {
+    const int i = id + (k & 3) + 128 * (k >> 2);
+    if (i >= 0 && i < n) left |= 1u << k;
   }
-  return block_merge(v, sh);
+  while (true) {
+    u64 best = 0;
+    int at = 0;
+#pragma unroll
+    for (int k = 0; k < kLpEach; ++k) {
+      const u64 key = (left >> k) & 1 ? lp_key(v[k], id + (k & 3) + 128 * (k >> 2)) : 0;
+      if (key > best) { best = key; at = k; }
+    }
+    const u64 least = shfl64(list, top - 1);
+    if (best <= least) best = 0;
+    unsigned who = __ballot_sync(0xFFFFFFFFu, best != 0);
+    if (who == 0) return list;
+    if (best) left &= ~(1u << at);
+    if (__popc(who) > 8) {
+      list = warp_merge(list, warp_sort(best));
+      continue;
+    }
+    while (who) {
+      const u64 key = shfl64(best, __ffs(who) - 1);
+      who &= who - 1;
+      const int pos = __popc(__ballot_sync(0xFFFFFFFFu, list > key));
+      const u64 up = __shfl_up_sync(0xFFFFFFFFu, list, 1);
+      list = lane < pos ? list : lane == pos ? key : up;
+    }
+  }
 }
 
-// One CTA per (row, piece of the row). Four logits of a row stand on 16 bytes: `off` floats
-// before the row's first one make it so, and units at the edges are read one by one.
-// kTop: alternatives are wanted.
+// One CTA per (row, piece of the row); a warp takes batches of 256 logits. Four logits of a row
+// stand on 16 bytes: `off` floats before the row's first one make it so, and units at the edges
+// are read one by one. kTop: alternatives are wanted.
 template <bool kTop>
-__global__ void __launch_bounds__(kLpThreads)
+__global__ void __launch_bounds__(kLpThreads, 4)
     k_logprob(const float* __restrict__ logits, size_t ld, int n, const int32_t* __restrict__ tok,
               int top, float* __restrict__ lp, float* __restrict__ ent,
               int32_t* __restrict__ top_id, float* __restrict__ top_lp, int pieces,
@@ -145,16 +170,15 @@ __global__ void __launch_bounds__(kLpThreads)
   const int r = blockIdx.x / pieces, piece = blockIdx.x % pieces;
   const float* x = logits + (size_t)r * ld;
   const int off = (int)(((uintptr_t)x >> 2) & 3);
-  const int units = (int)(((long long)off + n + 3) / 4), tiles = (units + kLpTile / 4 - 1) / (kLpTile / 4);
-  const int t0 = (int)((long long)tiles * piece / pieces);
-  const int t1 = (int)((long long)tiles * (piece + 1) / pieces);
+  const int batches = (int)(((long long)off + n + kLpBatch - 1) / kLpBatch);
+  const int b0 = (int)((long long)batches * piece / pieces);
+  const int b1 = (int)((long long)batches * (piece + 1) / pieces);
 
-  // unit u holds logits 4 u - off ..; a thread has units base + i 512 of a tile
-  auto load = [&](int tile, float (&v)[kLpEach]) {
+  // a lane holds ids 256 b + 4 lane - off .. + 3 of batch b, and the same 128 later
+  auto load = [&](int b, float (&v)[kLpEach]) {
 #pragma unroll
     for (int i = 0; i < kLpEach / 4; ++i) {
-      const int u = tile * (kLpTile / 4) + i * kLpThreads + threadIdx.x;
-      const int e = 4 * u - off;
+      const int e = b * kLpBatch + 128 * i + 4 * lane - off;
       if (e >= 0 && e + 4 <= n) {
         const float4 f = __ldcs(reinterpret_cast<const float4*>(x + e));
         v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
@@ -164,30 +188,23 @@ __global__ void __launch_bounds__(kLpThreads)
       }
     }
   };
-  auto id_of = [&](int tile, int k) {
-    return 4 * (tile * (kLpTile / 4) + (k >> 2) * kLpThreads + (int)threadIdx.x) + (k & 3) - off;
-  };
 
   float m = -INFINITY, s = 0.0f, t = 0.0f, ties = 0.0f;   // m is the warp's
-  u64 least = 0;                                         // a candidate is above it
-  float least_v = -INFINITY;
-  int have = 0;                                          // sh.count, between tiles
-  if (threadIdx.x == 0) sh.count = sh.more = 0;
-  __syncthreads();
-
+  u64 list = 0;                                          // the warp's 32 largest, falling
+  float least = -INFINITY;                               // the value of its `top`th
   float v[kLpEach], next[kLpEach];
-  if (t0 < t1) load(t0, next);
-  for (int tile = t0; tile < t1; ++tile) {
+  if (b0 + warp < b1) load(b0 + warp, next);
+  for (int b = b0 + warp; b < b1; b += kLpWarps) {
 #pragma unroll
     for (int k = 0; k < kLpEach; ++k) v[k] = next[k];
-    if (tile + 1 < t1) load(tile + 1, next);
+    if (b + kLpWarps < b1) load(b + kLpWarps, next);
     float mine = v[0];
 #pragma unroll
     for (int k = 1; k < kLpEach; ++k) mine = max_nan(mine, v[k]);
     float lm = mine;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) lm = max_nan(lm, __shfl_xor_sync(0xFFFFFFFFu, lm, o));
-    if (lm < m) {                                        // the usual tile: nothing at the top
+    if (lm < m) {                                        // the usual batch: nothing at the top
 #pragma unroll
       for (int k = 0; k < kLpEach; ++k) {
         const float z = fmaxf(v[k] - m, -200.0f), e = ex2f(z * 1.4426950408889634f);
@@ -214,48 +231,10 @@ __global__ void __launch_bounds__(kLpThreads)
         }
       }
     }
-    if constexpr (kTop) {
-      auto above = [&](int k) {                          // is logit k a candidate?
-        const int id = id_of(tile, k);
-        return !(v[k] < least_v) && id >= 0 && id < n && lp_key(v[k], id) > least;
-      };
-      int c = 0;
-      if (!(mine < least_v)) {
-#pragma unroll
-        for (int k = 0; k < kLpEach; ++k) c += above(k);
-      }
-      if (__syncthreads_or(c)) {
-        if (c) atomicAdd(&sh.more, c);
-        __syncthreads();
-        if (have + sh.more > kLpBuf) {
-          // too many: the 32nd largest of what is kept and of the threads' maxima bounds the
-          // row's 32nd largest from below, and at most 32 threads have logits above it
-          u64 w = have ? block_select(have, sh) : 0;
-          __syncthreads();
-          u64 best = 0;
-#pragma unroll
-          for (int k = 0; k < kLpEach; ++k)
-            if (above(k)) best = max64(best, lp_key(v[k], id_of(tile, k)));
-          const u64 b = block_merge(warp_sort(best), sh);
-          if (warp == 0) {
-            sh.buf[lane] = w;
-            w = warp_merge(w, b);
-            if (lane == top - 1) sh.lists[0][0] = w;
-            if (lane == 0) sh.count = have ? 32 : 0;
-          }
-          __syncthreads();
-          least = sh.lists[0][0];
-          least_v = least ? lp_key_value(least) : -INFINITY;
-          // the bound itself is a candidate
-          if (least) least -= 1;
-        }
-#pragma unroll
-        for (int k = 0; k < kLpEach; ++k)
-          if (above(k)) sh.buf[atomicAdd(&sh.count, 1)] = lp_key(v[k], id_of(tile, k));
-        __syncthreads();
-        have = sh.count;
-        if (threadIdx.x == 0) sh.more = 0;
-      }
+    if (kTop && !(lm < least)) {
+      list = warp_take(list, v, b * kLpBatch + 4 * lane - off, n, top);
+      const u64 k = shfl64(list, top - 1);
+      least = k ? lp_key_value(k) : -INFINITY;
     }
   }
 
@@ -267,8 +246,7 @@ __global__ void __launch_bounds__(kLpThreads)
     ties += __shfl_xor_sync(0xFFFFFFFFu, ties, o);
   }
   if (lane == 0) sh.sums[warp] = LpSum{m, s + (ties - 1.0f), t};
-  u64 list = 0;
-  if constexpr (kTop) list = block_select(have, sh);
+  if constexpr (kTop) list = block_merge(list, sh);
   __syncthreads();
   if (warp > 0 && pieces == 1) return;
   LpSum sum = lane < kLpWarps ? sh.sums[lane] : LpSum{-INFINITY, 0.f, 0.f};
@@ -297,18 +275,22 @@ __global__ void __launch_bounds__(kLpThreads)
     __syncthreads();
     if (!sh.last) return;
     __threadfence();
+    sum = LpSum{-INFINITY, 0.f, 0.f};
+    if (warp == 0)
+      for (int i = lane; i < pieces; i += 32) {
+        const float* p = reinterpret_cast<const float*>(psum + (size_t)r * pieces + i);
+        sum = lp_join(sum, LpSum{__ldcg(p), __ldcg(p + 1), __ldcg(p + 2)});
+      }
     if constexpr (kTop) {
-      for (int i = threadIdx.x; i < pieces * top; i += kLpThreads)
-        sh.buf[i] = __ldcg(plist + ((size_t)r * pieces + i / top) * kMaxTop + i % top);
-      __syncthreads();
-      list = block_select(pieces * top, sh);
+      list = 0;
+#pragma unroll 4
+      for (int i = warp; i < pieces; i += kLpWarps) {
+        const u64 k = lane < top ? __ldcg(plist + ((size_t)r * pieces + i) * kMaxTop + lane) : 0;
+        list = warp_merge(list, k);
+      }
+      list = block_merge(list, sh);
     }
     if (warp > 0) return;
-    sum = LpSum{-INFINITY, 0.f, 0.f};
-    for (int i = lane; i < pieces; i += 32) {
-      const float* p = reinterpret_cast<const float*>(psum + (size_t)r * pieces + i);
-      sum = lp_join(sum, LpSum{__ldcg(p), __ldcg(p + 1), __ldcg(p + 2)});
-    }
     sum = warp_join(sum);
   }
   const float nan = __int_as_float(0x7fc00000), ls = log1pf(sum.s);
@@ -331,7 +313,7 @@ int lp_pieces(int rows, int n, int* out) {
   int sms = 0;
   const int rc = sm_count(&sms);
   if (rc) return rc;
-  const int tiles = (int)(((long long)n + 3 + kLpTile - 1) / kLpTile);
+  const int tiles = (int)(((long long)n + 3 + 2 * kLpTile - 1) / (2 * kLpTile));   // two each
   int p = 4 * sms / rows;
   p = p < tiles ? p : tiles;
   p = p < kLpPieces ? p : kLpPieces;
