@@ -27,6 +27,8 @@ constexpr int kLpPieces = 64;                     // CTAs that may share a row
 constexpr int kLpTickets = 1024;                  // rows that may be shared; their tickets stand
                                                   // first in the scratch whatever the call
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 using u64 = unsigned long long;
 
 // 64-bit key in np.argmax's order: the f32 bits mapped to an unsigned order, then ~id. A key
@@ -50,9 +52,9 @@ HV_DEV float max_nan(float a, float b) {          // NaN if either is
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-HV_DEV float ex2f(float x) {
+HV_DEV float ex2f(float x) {                       // 0 below 2^-126
   float y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -91,16 +93,43 @@ HV_DEV LpSum lp_join(LpSum a, LpSum b) {
   if (b.m == -INFINITY) return a;
   if (a.m == -INFINITY) return b;
   if (a.m < b.m) { const LpSum c = a; a = b; b = c; }
-  const float d = fmaxf(b.m - a.m, -200.0f), f = ex2f(d * 1.4426950408889634f);
+  const float d = fmaxf(b.m - a.m, -200.0f), f = ex2f(d * kLog2e);
   a.t += f * (b.t - d * (1.0f + b.s));
   a.s += f * (1.0f + b.s);
   if (!(b.m <= a.m)) a.m = b.m - b.m + a.m;         // a NaN on either side stays one
   return a;
 }
 
+HV_DEV uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+HV_DEV float2 unpair(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+HV_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+HV_DEV uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+HV_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 struct LpShared {
   u64 lists[kLpWarps][32];
   LpSum sums[kLpWarps];
+  u64 least;
   unsigned last;
 };
 
@@ -118,42 +147,39 @@ HV_DEV u64 block_merge(u64 v, LpShared& sh) {
 
 HV_DEV u64 shfl64(u64 v, int src) { return __shfl_sync(0xFFFFFFFFu, v, src); }
 
-// Takes a batch's logits (of ids id + (k & 3) + 128 (k >> 2)) into the warp's falling list of 32:
-// lane by lane its largest, then its next, while any is above the list's `top`th. Few of them are
-// put in one by one, many are sorted and merged.
-HV_DEV u64 warp_take(u64 list, const float (&v)[kLpEach], int id, int n, int top) {
+// Takes a batch's logits (of ids id + (k & 3) + 128 (k >> 2)) that are above `least` into the
+// warp's falling list of 32; a list that is still empty starts from the lanes' largest.
+// Returns the list; the `top`th of it raises `least`.
+HV_DEV u64 warp_take(u64 list, const float (&v)[kLpEach], int id, int n, int top, u64* least) {
   const int lane = threadIdx.x & 31;
-  unsigned left = 0;
+  if (shfl64(list, 0) == 0) {
+    u64 best = 0;
+#pragma unroll
+    for (int k = 0; k < kLpEach; ++k) {
+      const int i = id + (k & 3) + 128 * (k >> 2);
+      if (i >= 0 && i < n) best = max64(best, lp_key(v[k], i));
+    }
+    list = warp_sort(best);
+    *least = max64(*least, shfl64(list, top - 1));
+  }
+  float bar = lp_key_value(*least);                       // NaN while there is no bound
 #pragma unroll
   for (int k = 0; k < kLpEach; ++k) {
     const int i = id + (k & 3) + 128 * (k >> 2);
-    if (i >= 0 && i < n) left |= 1u << k;
-  }
-  while (true) {
-    u64 best = 0;
-    int at = 0;
-#pragma unroll
-    for (int k = 0; k < kLpEach; ++k) {
-      const u64 key = (left >> k) & 1 ? lp_key(v[k], id + (k & 3) + 128 * (k >> 2)) : 0;
-      if (key > best) { best = key; at = k; }
-    }
-    const u64 least = shfl64(list, top - 1);
-    if (best <= least) best = 0;
-    unsigned who = __ballot_sync(0xFFFFFFFFu, best != 0);
-    if (who == 0) return list;
-    if (best) left &= ~(1u << at);
-    if (__popc(who) > 8) {
-      list = warp_merge(list, warp_sort(best));
-      continue;
-    }
+    unsigned who = __ballot_sync(0xFFFFFFFFu, i >= 0 && i < n && !(v[k] < bar));
     while (who) {
-      const u64 key = shfl64(best, __ffs(who) - 1);
+      const int src = __ffs(who) - 1;
       who &= who - 1;
+      const u64 key = lp_key(__shfl_sync(0xFFFFFFFFu, v[k], src), __shfl_sync(0xFFFFFFFFu, i, src));
+      if (key <= *least || __any_sync(0xFFFFFFFFu, list == key)) continue;
       const int pos = __popc(__ballot_sync(0xFFFFFFFFu, list > key));
       const u64 up = __shfl_up_sync(0xFFFFFFFFu, list, 1);
       list = lane < pos ? list : lane == pos ? key : up;
+      *least = max64(*least, shfl64(list, top - 1));
+      bar = lp_key_value(*least);
     }
   }
+  return list;
 }
 
 // One CTA per (row, piece of the row); a warp takes batches of 256 logits. Four logits of a row
@@ -189,56 +215,84 @@ __global__ void __launch_bounds__(kLpThreads, 4)
     }
   };
 
-  float m = -INFINITY, s = 0.0f, t = 0.0f, ties = 0.0f;   // m is the warp's
-  u64 list = 0;                                          // the warp's 32 largest, falling
-  float least = -INFINITY;                               // the value of its `top`th
+  float m = -INFINITY, ties = 0.0f;                      // m is the warp's
+  uint64_t s2 = 0, t2 = 0;                               // two sums each of exp(z) and z exp(z)
+  u64 list = 0, least = 0;                               // the warp's 32 largest, falling
+  float bar = -INFINITY;                                 // a lower logit is not among the `top`
   float v[kLpEach], next[kLpEach];
+  auto add = [&](const float (&y)[kLpEach]) {
+#pragma unroll
+    for (int k = 0; k < kLpEach; k += 2) {
+      float2 z = unpair(add2(pair(y[k], y[k + 1]), pair(-m, -m)));
+      z = make_float2(fmaxf(z.x, -200.0f), fmaxf(z.y, -200.0f));
+      const float2 g = unpair(mul2(pair(z.x, z.y), pair(kLog2e, kLog2e)));
+      const uint64_t e = pair(ex2f(g.x), ex2f(g.y));
+      s2 = add2(s2, e);
+      t2 = fma2(pair(z.x, z.y), e, t2);
+    }
+  };
+  const int rounds = (b1 - b0 + kLpWarps - 1) / kLpWarps;
+  int meet = 1;                                          // the round after which lists meet
   if (b0 + warp < b1) load(b0 + warp, next);
-  for (int b = b0 + warp; b < b1; b += kLpWarps) {
+  for (int i = 0; i < rounds; ++i) {
+    const int b = b0 + i * kLpWarps + warp;
+    if (b < b1) {
 #pragma unroll
-    for (int k = 0; k < kLpEach; ++k) v[k] = next[k];
-    if (b + kLpWarps < b1) load(b + kLpWarps, next);
-    float mine = v[0];
+      for (int k = 0; k < kLpEach; ++k) v[k] = next[k];
+      if (b + kLpWarps < b1) load(b + kLpWarps, next);
+      float mine = v[0];
 #pragma unroll
-    for (int k = 1; k < kLpEach; ++k) mine = max_nan(mine, v[k]);
-    float lm = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) lm = max_nan(lm, __shfl_xor_sync(0xFFFFFFFFu, lm, o));
-    if (lm < m) {                                        // the usual batch: nothing at the top
-#pragma unroll
-      for (int k = 0; k < kLpEach; ++k) {
-        const float z = fmaxf(v[k] - m, -200.0f), e = ex2f(z * 1.4426950408889634f);
-        s += e;
-        t = fmaf(-z, e, t);
+      for (int k = 1; k < kLpEach; ++k) mine = max_nan(mine, v[k]);
+      const bool usual = __all_sync(0xFFFFFFFFu, mine < m);
+      if (kTop && __any_sync(0xFFFFFFFFu, !(mine < bar))) {
+        list = warp_take(list, v, b * kLpBatch + 4 * lane - off, n, top, &least);
+        bar = least ? lp_key_value(least) : -INFINITY;
       }
-    } else if (lm != -INFINITY) {
-      if (!(lm == m)) {
-        const float d = fmaxf(m - lm, -200.0f);
-        const float f = m == -INFINITY ? 0.0f : ex2f(d * 1.4426950408889634f);
-        t = f * (t - d * (s + ties));
-        s = f * (s + ties);
-        ties = 0.0f;
-        m = max_nan(m, lm);
-      }
+      if (usual) {                                       // nothing at the warp's maximum
+        add(v);
+      } else {
+        float lm = mine;
 #pragma unroll
-      for (int k = 0; k < kLpEach; ++k) {
-        if (v[k] == m) {
-          ties += 1.0f;
-        } else {
-          const float z = fmaxf(v[k] - m, -200.0f), e = ex2f(z * 1.4426950408889634f);
-          s += e;
-          t = fmaf(-z, e, t);
+        for (int o = 16; o > 0; o >>= 1) lm = max_nan(lm, __shfl_xor_sync(0xFFFFFFFFu, lm, o));
+        if (lm != -INFINITY) {
+          if (!(lm <= m)) {
+            // what was summed counts less: S' = f (S + ties), T' = f (T + (m' - m)(S + ties))
+            const float d = fmaxf(m - lm, -200.0f);
+            const float f = m == -INFINITY ? 0.0f : ex2f(d * kLog2e);
+            float2 s = unpair(s2), u = unpair(t2);
+            s.x += ties;
+            ties = 0.0f;
+            u.x = f * fmaf(d, s.x, u.x);
+            u.y = f * fmaf(d, s.y, u.y);
+            s2 = pair(f * s.x, f * s.y);
+            t2 = pair(u.x, u.y);
+            m = max_nan(m, lm);
+          }
+#pragma unroll
+          for (int k = 0; k < kLpEach; ++k)
+            if (v[k] == m) {
+              ties += 1.0f;
+              v[k] = -INFINITY;                          // adds nothing below
+            }
+          add(v);
         }
       }
     }
-    if (kTop && !(lm < least)) {
-      list = warp_take(list, v, b * kLpBatch + 4 * lane - off, n, top);
-      const u64 k = shfl64(list, top - 1);
-      least = k ? lp_key_value(k) : -INFINITY;
+    if (kTop && i + 1 == meet && meet < rounds) {
+      // The warps' lists become one, warp 0's, whose `top`th bounds all of them from below.
+      // With each doubling of what has been seen, about `top` logits pass the bound.
+      meet *= 2;
+      list = block_merge(list, sh);
+      if (warp == 0 && lane == top - 1) sh.least = list;
+      if (warp > 0) list = 0;
+      __syncthreads();
+      least = max64(least, sh.least);
+      bar = least ? lp_key_value(least) : -INFINITY;
     }
   }
 
   // the warp's sums, then the CTA's
+  float s = unpair(s2).x + unpair(s2).y, t = -(unpair(t2).x + unpair(t2).y);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
