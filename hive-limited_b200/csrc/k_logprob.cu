@@ -19,7 +19,7 @@ namespace hv {
 namespace {
 
 constexpr int kMaxTop = 32;
-constexpr int kLpThreads = 256, kLpWarps = kLpThreads / 32;
+constexpr int kLpThreads = 512, kLpWarps = kLpThreads / 32;
 constexpr int kLpEach = 8;                        // logits a thread holds at a time
 constexpr int kLpBatch = 32 * kLpEach;            // a warp's
 constexpr int kLpTile = kLpWarps * kLpBatch;      // a CTA's
@@ -148,11 +148,11 @@ HV_DEV u64 block_merge(u64 v, LpShared& sh) {
 HV_DEV u64 shfl64(u64 v, int src) { return __shfl_sync(0xFFFFFFFFu, v, src); }
 
 // Takes a batch's logits (of ids id + (k & 3) + 128 (k >> 2)) that are above `least` into the
-// warp's falling list of 32; a list that is still empty starts from the lanes' largest.
+// warp's falling list of 32; without a bound yet it starts from the lanes' largest.
 // Returns the list; the `top`th of it raises `least`.
 HV_DEV u64 warp_take(u64 list, const float (&v)[kLpEach], int id, int n, int top, u64* least) {
   const int lane = threadIdx.x & 31;
-  if (shfl64(list, 0) == 0) {
+  if (*least == 0) {                                      // nothing to go by yet
     u64 best = 0;
 #pragma unroll
     for (int k = 0; k < kLpEach; ++k) {
@@ -186,7 +186,7 @@ HV_DEV u64 warp_take(u64 list, const float (&v)[kLpEach], int id, int n, int top
 // stand on 16 bytes: `off` floats before the row's first one make it so, and units at the edges
 // are read one by one. kTop: alternatives are wanted.
 template <bool kTop>
-__global__ void __launch_bounds__(kLpThreads, 4)
+__global__ void __launch_bounds__(kLpThreads, 2)
     k_logprob(const float* __restrict__ logits, size_t ld, int n, const int32_t* __restrict__ tok,
               int top, float* __restrict__ lp, float* __restrict__ ent,
               int32_t* __restrict__ top_id, float* __restrict__ top_lp, int pieces,
@@ -280,8 +280,8 @@ __global__ void __launch_bounds__(kLpThreads, 4)
     }
     if (kTop && i + 1 == meet && meet < rounds) {
       // The warps' lists become one, warp 0's, whose `top`th bounds all of them from below.
-      // With each doubling of what has been seen, about `top` logits pass the bound.
-      meet *= 2;
+      // While what has been seen grows fourfold, a few times `top` logits pass the bound.
+      meet *= 4;
       list = block_merge(list, sh);
       if (warp == 0 && lane == top - 1) sh.least = list;
       if (warp > 0) list = 0;
@@ -367,8 +367,8 @@ int lp_pieces(int rows, int n, int* out) {
   int sms = 0;
   const int rc = sm_count(&sms);
   if (rc) return rc;
-  const int tiles = (int)(((long long)n + 3 + 2 * kLpTile - 1) / (2 * kLpTile));   // two each
-  int p = 4 * sms / rows;
+  const int tiles = (int)(((long long)n + 3 + kLpTile - 1) / kLpTile);
+  int p = 2 * sms / rows;
   p = p < tiles ? p : tiles;
   p = p < kLpPieces ? p : kLpPieces;
   *out = p < 1 || rows > kLpTickets ? 1 : p;
