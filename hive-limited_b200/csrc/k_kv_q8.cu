@@ -25,6 +25,16 @@ struct Q8Src {
   float eps;
 };
 
+// Bytes between the 512-byte units of a block's codes in shared memory: such that the warps'
+// 4-byte pieces of K and 2-byte pieces of V fall on different banks (two to a bank for V).
+constexpr int kKUnit = 576, kVUnit = 528;
+
+HV_DEV float q8_max(float a, float b) {          // the larger magnitude; NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
 // Row `t` of the call for head g as a float4 per lane (dims 4 lane ..). One warp.
 template <bool kNorm>
 HV_DEV float4 q8_row(const Q8Src& s, int which, int g, int t, int pos, float* tmp) {
@@ -49,7 +59,7 @@ HV_DEV void q8_write_block(const Q8Src& src, const KvQ8& c, int item, int nth, i
                            int ntok) {
   __shared__ float s_max[8];
   __shared__ int s_held;
-  __shared__ __align__(16) uint8_t s_codes[kQ8Codes];
+  __shared__ __align__(16) uint8_t s_codes[8 * kKUnit];
   __shared__ __align__(16) float s_tmp[kNorm ? 8 : 1][kNorm ? 2 * kHd : 4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = item >> 1, which = item & 1;
@@ -69,13 +79,12 @@ HV_DEV void q8_write_block(const Q8Src& src, const KvQ8& c, int item, int nth, i
     in_tail = old == 0 || (s_held - 1) / kQ8Blk == blk;
   }
 
-  // rows 8 i + warp of the block
+  // rows 4 warp .. 4 warp + 3 of the block
   float4 x[4];
-  float mx = 0.0f;
-  bool bad = false;
+  float mx = 0.0f;                     // NaN once a NaN has been seen
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + warp;
+    const int r = 4 * warp + i;
     x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < old) {
       if (in_tail) {
@@ -93,40 +102,66 @@ HV_DEV void q8_write_block(const Q8Src& src, const KvQ8& c, int item, int nth, i
       x[i] = q8_row<kNorm>(src, which, g, blk * kQ8Blk + r - pos0, blk * kQ8Blk + r,
                            s_tmp[kNorm ? warp : 0]);
     }
-    const float a[4] = {fabsf(x[i].x), fabsf(x[i].y), fabsf(x[i].z), fabsf(x[i].w)};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      mx = fmaxf(mx, a[e]);
-      bad |= !(a[e] <= FLT_MAX);
-    }
+    mx = q8_max(q8_max(mx, x[i].x), q8_max(x[i].y, x[i].z));
+    mx = q8_max(mx, x[i].w);
   }
   if (have == kQ8Blk) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+    for (int o = 16; o > 0; o >>= 1) mx = q8_max(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
     if (lane == 0) s_max[warp] = mx;
-    const bool any_bad = __syncthreads_or(bad) != 0;
+    __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; ++w) mx = fmaxf(mx, s_max[w]);
+    for (int w = 0; w < 8; ++w) mx = q8_max(mx, s_max[w]);
+    const bool any_bad = !(mx <= FLT_MAX);
     float s = __fdiv_rn(mx, 127.0f);
     if (s == 0.0f) s = 1.0f;
+    // The code is the nearest integer to x / s. x times 1 / s is off by 2 parts in 2^24 of 127,
+    // and the rule's own roundings are 2^-17 together: where that product is not within 5e-5 of
+    // a half the nearest integer to it is the rule's, and else the rule itself is asked (so too
+    // where s is so small that its rounding counts).
+    const float inv = __frcp_rn(s);
+    const bool slow = any_bad || s < 0x1p-100f;
+    const int unit = which ? kVUnit : kKUnit;
+    uint32_t y[4];                     // a row's four codes each, plus 128
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + warp;
       const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      int q[4];
+      uint32_t q[4];
+      bool near = slow;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) q[e] = any_bad ? 128 : q8_code(v[e], s) + 128;
-      if (which == 0) {
-        *reinterpret_cast<uint32_t*>(s_codes + q8_k_at(r, 4 * lane)) =
-            (uint32_t)q[0] | (uint32_t)q[1] << 8 | (uint32_t)q[2] << 16 | (uint32_t)q[3] << 24;
-      } else {
+      for (int e = 0; e < 4; ++e) {
+        constexpr float kMagic = 12582912.0f + 128.0f;      // 1.5 2^23: the sum's low bits count
+        const float z = __fmul_rn(v[e], inv), n = __fadd_rn(z, kMagic);
+        q[e] = __float_as_uint(n);
+        near |= fabsf(__fsub_rn(z, __fsub_rn(n, kMagic))) > 0.49995f;
+      }
+      if (near) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s_codes[q8_v_at(r, 4 * lane + e)] = (uint8_t)q[e];
+        for (int e = 0; e < 4; ++e) q[e] = any_bad ? 128u : (uint32_t)(q8_code(v[e], s) + 128);
+      }
+      y[i] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+    }
+    if (which == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = q8_k_at(4 * warp + i, 4 * lane);
+        *reinterpret_cast<uint32_t*>(s_codes + (at >> 9) * unit + (at & 511)) = y[i];
+      }
+    } else {
+      // two rows' codes of a dim are neighbours
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = q8_v_at(4 * warp + i, 4 * lane + e);
+          const uint32_t two = __byte_perm(y[i], y[i + 1], e | (4 + e) << 4);
+          *reinterpret_cast<uint16_t*>(s_codes + (at >> 9) * unit + (at & 511)) = (uint16_t)two;
+        }
       }
     }
     __syncthreads();
     reinterpret_cast<uint4*>(codes)[threadIdx.x] =
-        reinterpret_cast<const uint4*>(s_codes)[threadIdx.x];
+        *reinterpret_cast<const uint4*>(s_codes + (threadIdx.x >> 5) * unit + (threadIdx.x & 31) * 16);
     if (threadIdx.x == 0) *scale = any_bad ? __int_as_float(0x7fc00000) : s;
   }
   if (!first) return;
@@ -135,7 +170,7 @@ HV_DEV void q8_write_block(const Q8Src& src, const KvQ8& c, int item, int nth, i
   if (blk_last == blk) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + warp;
+      const int r = 4 * warp + i;
       if (r < have && (r >= old || !in_tail))
         reinterpret_cast<float4*>(tail + (size_t)r * kHd)[lane] = x[i];
     }
@@ -143,7 +178,7 @@ HV_DEV void q8_write_block(const Q8Src& src, const KvQ8& c, int item, int nth, i
     const int n = end - blk_last * kQ8Blk;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + warp;
+      const int r = 4 * warp + i;
       if (r < n)
         reinterpret_cast<float4*>(tail + (size_t)r * kHd)[lane] =
             q8_row<kNorm>(src, which, g, blk_last * kQ8Blk + r - pos0, blk_last * kQ8Blk + r,
@@ -187,42 +222,59 @@ __global__ void __launch_bounds__(256) k_qk_rows_q8(Q8Src src, KvQ8 c,
 }
 
 // Positions pos0 .. pos0 + ntok - 1 as f32 rows [ntok][nkv][128]; NaN where nothing is held.
-// One CTA per (head, K or V) and block; the codes pass through shared memory, whose units
-// are 528 bytes apart so that a row's bytes fall on different banks.
+// One CTA per (head, K or V) and block; the codes pass through shared memory.
 __global__ void __launch_bounds__(256) k_kv_read_q8(KvQ8 c, float* __restrict__ k_out,
                                                     float* __restrict__ v_out, int pos0, int ntok,
                                                     int nkv) {
-  constexpr int kUnit = 528;
-  __shared__ __align__(16) uint8_t s_codes[8 * kUnit];
+  __shared__ __align__(16) uint8_t s_codes[8 * kKUnit];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = blockIdx.x >> 1, which = blockIdx.x & 1;
   const int blk = pos0 / kQ8Blk + blockIdx.y;
   const int held = q8_held(c, g), p0 = blk * kQ8Blk;
   const bool closed = p0 + kQ8Blk <= held;
+  const int unit = which ? kVUnit : kKUnit;
   float s = 0.0f;
   if (closed) {
     const uint8_t* codes = c.codes + (((size_t)g * c.nblk + blk) * 2 + which) * kQ8Codes;
     const uint4 w = __ldg(reinterpret_cast<const uint4*>(codes) + threadIdx.x);
-    *reinterpret_cast<uint4*>(s_codes + (threadIdx.x >> 5) * kUnit + (threadIdx.x & 31) * 16) = w;
+    *reinterpret_cast<uint4*>(s_codes + (threadIdx.x >> 5) * unit + (threadIdx.x & 31) * 16) = w;
     s = __ldg(c.scales + ((size_t)g * c.nblk + blk) * 2 + which);
   }
   __syncthreads();
   const float* tail = c.tail + ((size_t)g * 2 + which) * kQ8Codes;
   float* out = which ? v_out : k_out;
+  uint32_t y[4] = {0, 0, 0, 0};                  // a row's four codes each
+  if (closed) {
+    if (which == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = q8_k_at(4 * warp + i, 4 * lane);
+        y[i] = *reinterpret_cast<const uint32_t*>(s_codes + (at >> 9) * unit + (at & 511));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        uint32_t two[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = q8_v_at(4 * warp + i, 4 * lane + e);
+          two[e] = *reinterpret_cast<const uint16_t*>(s_codes + (at >> 9) * unit + (at & 511));
+        }
+        const uint32_t a = __byte_perm(two[0], two[1], 0x5140), b = __byte_perm(two[2], two[3], 0x5140);
+        y[i] = __byte_perm(a, b, 0x5410);
+        y[i + 1] = __byte_perm(a, b, 0x7632);
+      }
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = 8 * i + warp, p = p0 + r;
+    const int r = 4 * warp + i, p = p0 + r;
     if (p < pos0 || p >= pos0 + ntok) continue;
     float4 x;
     if (closed) {
-      float v[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int d = 4 * lane + e;
-        const int at = which ? q8_v_at(r, d) : q8_k_at(r, d);
-        v[e] = q8_value(s_codes[(at >> 9) * kUnit + (at & 511)], s);
-      }
-      x = make_float4(v[0], v[1], v[2], v[3]);
+      const uint32_t w = y[i];
+      x = make_float4(q8_value(w & 255, s), q8_value((w >> 8) & 255, s), q8_value((w >> 16) & 255, s),
+                      q8_value(w >> 24, s));
     } else if (p < held) {
       x = __ldg(reinterpret_cast<const float4*>(tail + (size_t)r * kHd) + lane);
     } else {

@@ -67,7 +67,9 @@ HV_DEV int q8_code(float x, float s) {
   return q > 127 ? 127 : (q < -127 ? -127 : q);
 }
 
-HV_DEV float q8_value(int biased, float s) { return __fmul_rn((float)(biased - 128), s); }
+HV_DEV float q8_value(uint32_t biased, float s) {   // 2^23 + code + 128 as a float, less that
+  return __fmul_rn(__fsub_rn(__uint_as_float(0x4B000000u | biased), 8388608.0f + 128.0f), s);
+}
 
 // Positions the cache holds for kv head g: those both K and V have.
 HV_DEV int q8_held(const KvQ8& c, int g) {
