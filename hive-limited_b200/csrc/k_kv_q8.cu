@@ -82,26 +82,40 @@ HV_DEV void q8_write_block(const Q8Src& src, const KvQ8& c, int item, int nth, i
   // rows 4 warp .. 4 warp + 3 of the block
   float4 x[4];
   float mx = 0.0f;                     // NaN once a NaN has been seen
+  if (old == 0 && have == kQ8Blk) {     // the usual block: four loads under way at once
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = blk * kQ8Blk + 4 * warp + i;
+      x[i] = q8_row<kNorm>(src, which, g, p - pos0, p, s_tmp[kNorm ? warp : 0]);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {
+      const int r = 4 * warp + i;
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < old) {
+        if (in_tail) {
+          y = reinterpret_cast<const float4*>(tail + (size_t)r * kHd)[lane];
+        } else {                         // the block was complete: reopen it from its codes
+          const float s = *scale;
+          float v[4];
+          for (int e = 0; e < 4; ++e) {
+            const int d = 4 * lane + e;
+            v[e] = q8_value(codes[which ? q8_v_at(r, d) : q8_k_at(r, d)], s);
+          }
+          y = make_float4(v[0], v[1], v[2], v[3]);
+        }
+      } else if (r < have) {
+        y = q8_row<kNorm>(src, which, g, blk * kQ8Blk + r - pos0, blk * kQ8Blk + r,
+                             s_tmp[kNorm ? warp : 0]);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k == i) x[k] = y;
+    }
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = 4 * warp + i;
-    x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < old) {
-      if (in_tail) {
-        x[i] = reinterpret_cast<const float4*>(tail + (size_t)r * kHd)[lane];
-      } else {                         // the block was complete: reopen it from its codes
-        const float s = *scale;
-        float v[4];
-        for (int e = 0; e < 4; ++e) {
-          const int d = 4 * lane + e;
-          v[e] = q8_value(codes[which ? q8_v_at(r, d) : q8_k_at(r, d)], s);
-        }
-        x[i] = make_float4(v[0], v[1], v[2], v[3]);
-      }
-    } else if (r < have) {
-      x[i] = q8_row<kNorm>(src, which, g, blk * kQ8Blk + r - pos0, blk * kQ8Blk + r,
-                           s_tmp[kNorm ? warp : 0]);
-    }
     mx = q8_max(q8_max(mx, x[i].x), q8_max(x[i].y, x[i].z));
     mx = q8_max(mx, x[i].w);
   }
@@ -188,7 +202,7 @@ HV_DEV void q8_write_block(const Q8Src& src, const KvQ8& c, int item, int nth, i
   if (threadIdx.x == 0) c.held[item] = end;
 }
 
-__global__ void __launch_bounds__(256) k_kv_rows_q8(Q8Src src, KvQ8 c, int pos0, int ntok) {
+__global__ void __launch_bounds__(256, 7) k_kv_rows_q8(Q8Src src, KvQ8 c, int pos0, int ntok) {
   q8_write_block<false>(src, c, blockIdx.x, blockIdx.y, pos0, ntok);
 }
 
