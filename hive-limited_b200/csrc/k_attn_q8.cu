@@ -43,7 +43,7 @@ HV_DEV void cp_async16(uint32_t dst, const void* src) {
 template <bool kTwo>
 __global__ void __launch_bounds__(32 * kDecWarps, 1)
     k_attn_dec_q8(const float* __restrict__ q, KvQ8 c, float* __restrict__ ctx,
-                  const float* __restrict__ scale, const int32_t* __restrict__ pos_p, int group,
+                  const float* __restrict__ scale, const int32_t* __restrict__ pos_p, int pos0, int group,
                   float* __restrict__ part, unsigned* __restrict__ ticket) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_m[kDecWarps][8], s_l[kDecWarps][8], s_x[kQ8Blk][8];
@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   __shared__ unsigned s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, chunk = blockIdx.x;
-  const int pos = *pos_p, held = q8_held(c, kvh);
+  const int pos = pos_p ? *pos_p : pos0, held = q8_held(c, kvh);
   float* out = ctx + (size_t)kvh * group * kHd;
   if (pos < 0 || pos >= held) {
     if (chunk == 0)
@@ -421,9 +421,10 @@ struct RowsCfg {
   static constexpr int kRows = 16 * kWM;
   static constexpr int kStages = kShares == 8 ? 2 : 3;
   static constexpr int kRing = kShares * kStages * 2 * kQ8Codes;
-  static constexpr int kMerge = kShares > 1 ? kRowWarps * 16 * (kHd + 4) * 4 : 0;
+  static constexpr int kMerge = kRowWarps * 16 * (kHd + 4) * 4;
   static constexpr int kTail = 4 * kQ8Codes * 2;          // K hi, K lo, V hi, V lo
-  static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kTail;
+  static constexpr int kOpen = 2 * kQ8Codes * 4;          // the open rows in f32
+  static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kTail + kOpen;
 };
 
 template <int kWM>
@@ -475,6 +476,18 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
     if constexpr (kWM == 1) __syncwarp();
     else asm volatile("bar.sync %0, %1;" :: "r"(1 + share), "n"(32 * kWM) : "memory");
   };
+  // the open rows go first, to the CTA with the last chunk
+  const bool has_open = tail && b1 == items;
+  const int nopen = min(held - closed * kQ8Blk, kQ8Blk);
+  float* open = reinterpret_cast<float*>(smem + Cfg::kSmem - Cfg::kOpen);
+  if (has_open) {
+    const float* src = c.tail + (size_t)kvh * 2 * kQ8Codes + 4 * lane;
+    for (int r = warp; r < 2 * nopen; r += kRowWarps) {
+      const int at = r < nopen ? r * kHd : kQ8Codes + (r - nopen) * kHd;
+      cp_async16((uint32_t)__cvta_generic_to_shared(open + at + 4 * lane), src + at);
+    }
+  }
+  asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < Cfg::kStages; ++i) fetch(b0 + share + i * Cfg::kShares, i);
 
@@ -566,6 +579,93 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
     }
   };
 
+  if (has_open) {                                // while the first blocks come in
+    // the open rows as fragments in two terms; rows past the last one held are zero, and so
+    // are values that are not finite, whose weight of 0 for the rows that do not see them
+    // would not be nothing: the rows that see one get a sum of NaN instead
+    __half* frag = reinterpret_cast<__half*>(smem + Cfg::kSmem - Cfg::kOpen - Cfg::kTail);
+    if (threadIdx.x < 2) s_amax[threadIdx.x] = 0.0f;
+    if (threadIdx.x == 0) s_bad = kQ8Blk;
+    asm volatile("cp.async.wait_group %0;" :: "n"(Cfg::kStages) : "memory");
+    __syncthreads();
+    for (int which = 0; which < 2; ++which) {
+      float amax = 0.0f;
+      for (int i = threadIdx.x; i < nopen * (kHd / 4); i += blockDim.x) {
+        const float4 x = reinterpret_cast<const float4*>(open + which * kQ8Codes)[i];
+        const float v[4] = {fabsf(x.x), fabsf(x.y), fabsf(x.z), fabsf(x.w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (v[e] < INFINITY) amax = fmaxf(amax, v[e]);
+          else atomicMin(&s_bad, i / (kHd / 4));
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
+      if (lane == 0) atomicMax(reinterpret_cast<int*>(&s_amax[which]), __float_as_int(amax));
+    }
+    __syncthreads();
+    const float lk = q8_lift(s_amax[0]), lv = q8_lift(s_amax[1]);
+    auto term = [&](float x, float lift) { return fabsf(x) < INFINITY ? x * lift : 0.0f; };
+    // four dims of a K row are neighbours in a fragment, two rows of a V dim
+    for (int i = threadIdx.x; i < kQ8Codes / 4; i += blockDim.x) {
+      const int r = i / (kHd / 4), d = 4 * (i % (kHd / 4));
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < nopen) x = *reinterpret_cast<const float4*>(open + r * kHd + d);
+      uint2 hi, lo;
+      split_half2(term(x.x, lk), term(x.y, lk), &hi.x, &lo.x);
+      split_half2(term(x.z, lk), term(x.w, lk), &hi.y, &lo.y);
+      *reinterpret_cast<uint2*>(frag + q8_k_at(r, d)) = hi;
+      *reinterpret_cast<uint2*>(frag + kQ8Codes + q8_k_at(r, d)) = lo;
+    }
+    for (int i = threadIdx.x; i < kQ8Codes / 2; i += blockDim.x) {
+      const int r = 2 * (i / kHd), d = i % kHd;
+      const float* v = open + kQ8Codes + r * kHd + d;
+      uint32_t hi, lo;
+      split_half2(r < nopen ? term(v[0], lv) : 0.0f, r + 1 < nopen ? term(v[kHd], lv) : 0.0f, &hi, &lo);
+      *reinterpret_cast<uint32_t*>(frag + 2 * kQ8Codes + q8_v_at(r, d)) = hi;
+      *reinterpret_cast<uint32_t*>(frag + 3 * kQ8Codes + q8_v_at(r, d)) = lo;
+    }
+    __syncthreads();
+    if (share == 0 && 32 * closed <= warp_top) {
+      // 16 halves of a unit: the 16 bytes of a coded one
+      auto word2 = [&](int part, int u, int w) {
+        return *reinterpret_cast<const uint2*>(frag + part * kQ8Codes + 512 * u + 16 * lane + 4 * w);
+      };
+      float s[4][4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint2 kh = word2(0, 2 * j + (k >> 2), k & 3), kl = word2(1, 2 * j + (k >> 2), k & 3);
+          mma_f16(s[j], qh[k], kh.x, kh.y);
+          mma_f16(s[j], ql[k], kh.x, kh.y);
+          mma_f16(s[j], qh[k], kl.x, kl.y);
+        }
+      }
+      weights(closed, s, qs0 / lk, qs1 / lk);
+      const float f = 1.0f / lv;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const uint2 vh = word2(2, u, 2 * h + k), vl = word2(3, u, 2 * h + k);
+            mma_f16(d, wh[k], vh.x, vh.y);
+            mma_f16(d, wl[k], vh.x, vh.y);
+            mma_f16(d, wh[k], vl.x, vl.y);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[2 * u + h][i] = fmaf(d[i], f, acc[2 * u + h][i]);
+        }
+      }
+      if (lim0 >= closed * kQ8Blk + s_bad) l0 = __int_as_float(0x7fc00000);
+      if (lim1 >= closed * kQ8Blk + s_bad) l1 = __int_as_float(0x7fc00000);
+    }
+  }
+
   int stage = 0;
   for (int b = b0 + share; b < c1; b += Cfg::kShares) {
     asm volatile("cp.async.wait_group %0;" :: "n"(Cfg::kStages - 1) : "memory");
@@ -618,90 +718,21 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
     stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
   }
 
-  if (tail && b1 == items) {
-    // the open rows as fragments in two terms; rows past the last one held are zero, and so
-    // are values that are not finite, whose weight of 0 for the rows that do not see them
-    // would not be nothing: the rows that see one get a sum of NaN instead
-    __half* frag = reinterpret_cast<__half*>(smem + Cfg::kSmem - Cfg::kTail);
-    const int n = min(held - closed * kQ8Blk, kQ8Blk);
-    const float* src = c.tail + (size_t)kvh * 2 * kQ8Codes;
-    if (threadIdx.x < 2) s_amax[threadIdx.x] = 0.0f;
-    if (threadIdx.x == 0) s_bad = kQ8Blk;
-    __syncthreads();
-    for (int which = 0; which < 2; ++which) {
-      float amax = 0.0f;
-      for (int i = threadIdx.x; i < n * kHd; i += blockDim.x) {
-        const float x = fabsf(__ldg(src + which * kQ8Codes + i));
-        if (x < INFINITY) amax = fmaxf(amax, x);
-        else atomicMin(&s_bad, i / kHd);
-      }
-      atomicMax(reinterpret_cast<int*>(&s_amax[which]), __float_as_int(amax));
-    }
-    __syncthreads();
-    const float lk = q8_lift(s_amax[0]), lv = q8_lift(s_amax[1]);
-    for (int i = threadIdx.x; i < 2 * kQ8Codes; i += blockDim.x) {
-      const int which = i / kQ8Codes, r = i % kQ8Codes / kHd, d = i % kHd;
-      float x = r < n ? __ldg(src + i) * (which ? lv : lk) : 0.0f;
-      if (!(fabsf(x) < INFINITY)) x = 0.0f;
-      const __half hi = __float2half_rn(x), lo = __float2half_rn(x - __half2float(hi));
-      const int at = which ? q8_v_at(r, d) : q8_k_at(r, d);
-      frag[(2 * which) * kQ8Codes + at] = hi;
-      frag[(2 * which + 1) * kQ8Codes + at] = lo;
-    }
-    __syncthreads();
-    if (share == 0 && 32 * closed <= warp_top) {
-      // 16 halves of a unit: the 16 bytes of a coded one
-      auto word2 = [&](int part, int u, int w) {
-        return *reinterpret_cast<const uint2*>(frag + part * kQ8Codes + 512 * u + 16 * lane + 4 * w);
-      };
-      float s[4][4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint2 kh = word2(0, 2 * j + (k >> 2), k & 3), kl = word2(1, 2 * j + (k >> 2), k & 3);
-          mma_f16(s[j], qh[k], kh.x, kh.y);
-          mma_f16(s[j], ql[k], kh.x, kh.y);
-          mma_f16(s[j], qh[k], kl.x, kl.y);
-        }
-      }
-      weights(closed, s, qs0 / lk, qs1 / lk);
-      const float f = 1.0f / lv;
-#pragma unroll
-      for (int u = 0; u < 8; ++u) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint2 vh = word2(2, u, 2 * h + k), vl = word2(3, u, 2 * h + k);
-            mma_f16(d, wh[k], vh.x, vh.y);
-            mma_f16(d, wl[k], vh.x, vh.y);
-            mma_f16(d, wh[k], vl.x, vl.y);
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[2 * u + h][i] = fmaf(d[i], f, acc[2 * u + h][i]);
-        }
-      }
-      if (lim0 >= closed * kQ8Blk + s_bad) l0 = __int_as_float(0x7fc00000);
-      if (lim1 >= closed * kQ8Blk + s_bad) l1 = __int_as_float(0x7fc00000);
-    }
-  }
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
     l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, o);
     l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, o);
   }
 
-  // the shares meet in share 0
-  if constexpr (Cfg::kShares > 1) {
-    if (t == 0) {
-      s_m[warp][gl] = m0; s_m[warp][gl + 8] = m1;
-      s_l[warp][gl] = l0; s_l[warp][gl + 8] = l1;
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncthreads();
+  // the shares meet: all of a row's sums in shared memory, then four outputs a thread
+  static_assert(Cfg::kShares > 1, "more rows are the tile kernel's");
+  if (t == 0) {
+    s_m[warp][gl] = m0; s_m[warp][gl + 8] = m1;
+    s_l[warp][gl] = l0; s_l[warp][gl + 8] = l1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  {
     float M0 = -INFINITY, M1 = -INFINITY;
 #pragma unroll
     for (int w = 0; w < Cfg::kShares; ++w) {
@@ -710,77 +741,46 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
     }
     const float a0 = l0 == 0.0f ? 0.0f : ex2(m0 - M0), a1 = l1 == 0.0f ? 0.0f : ex2(m1 - M1);
     float* red = reinterpret_cast<float*>(smem) + (size_t)warp * 16 * (kHd + 4);
-    if (share > 0) {
 #pragma unroll
-      for (int d = 0; d < 16; ++d) {
-        *reinterpret_cast<float2*>(red + gl * (kHd + 4) + 8 * d + 2 * t) =
-            make_float2(acc[d][0] * a0, acc[d][1] * a0);
-        *reinterpret_cast<float2*>(red + (gl + 8) * (kHd + 4) + 8 * d + 2 * t) =
-            make_float2(acc[d][2] * a1, acc[d][3] * a1);
-      }
-    }
-    __syncthreads();
-    if (share == 0) {
-#pragma unroll
-      for (int d = 0; d < 16; ++d) { acc[d][0] *= a0; acc[d][1] *= a0; acc[d][2] *= a1; acc[d][3] *= a1; }
-      l0 *= a0;
-      l1 *= a1;
-      for (int w = 1; w < Cfg::kShares; ++w) {
-        const float* o = reinterpret_cast<const float*>(smem) + (size_t)(w * kWM + wm) * 16 * (kHd + 4);
-        const float v0 = s_l[w * kWM + wm][gl], v1 = s_l[w * kWM + wm][gl + 8];
-        l0 += v0 == 0.0f ? 0.0f : v0 * ex2(s_m[w * kWM + wm][gl] - M0);
-        l1 += v1 == 0.0f ? 0.0f : v1 * ex2(s_m[w * kWM + wm][gl + 8] - M1);
-#pragma unroll
-        for (int d = 0; d < 16; ++d) {
-          const float2 x = *reinterpret_cast<const float2*>(o + gl * (kHd + 4) + 8 * d + 2 * t);
-          const float2 y = *reinterpret_cast<const float2*>(o + (gl + 8) * (kHd + 4) + 8 * d + 2 * t);
-          acc[d][0] += x.x; acc[d][1] += x.y; acc[d][2] += y.x; acc[d][3] += y.y;
-        }
-      }
-      m0 = M0;
-      m1 = M1;
+    for (int d = 0; d < 16; ++d) {
+      *reinterpret_cast<float2*>(red + gl * (kHd + 4) + 8 * d + 2 * t) =
+          make_float2(acc[d][0] * a0, acc[d][1] * a0);
+      *reinterpret_cast<float2*>(red + (gl + 8) * (kHd + 4) + 8 * d + 2 * t) =
+          make_float2(acc[d][2] * a1, acc[d][3] * a1);
     }
   }
-
-  auto ctx_row = [&](int r) {
-    return a.ctx + (((size_t)(r / a.group)) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd;
-  };
-  auto not_held = [&](int r) { return a.pos0 + r / a.group >= held; };
-  const float nan = __int_as_float(0x7fc00000);
-  if (nact == 1) {
-    if (share == 0) {
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = half ? r1 : r0;
-        if (r >= nrows) continue;
-        const float inv = not_held(r) ? nan : 1.0f / (half ? l1 : l0);
-        float* o = ctx_row(r) + 2 * t;
-#pragma unroll
-        for (int d = 0; d < 16; ++d)
-          *reinterpret_cast<float2*>(o + 8 * d) =
-              make_float2(acc[d][2 * half] * inv, acc[d][2 * half + 1] * inv);
-      }
-    }
-    return;
-  }
-  // the chunks meet in the scratch; the last CTA to arrive adds them in order
   const int ntile = gridDim.x / a.chunks;
   const size_t slot = ((size_t)kvh * ntile + tile) * a.chunks;
   float* mine = a.part + (slot + chunk) * rows_part(Cfg::kRows);
-  if (share == 0) {
+  __syncthreads();
+  for (int i = threadIdx.x; i < Cfg::kRows * (kHd / 4); i += blockDim.x) {
+    const int r = i / (kHd / 4), d4 = i % (kHd / 4), gr = row0 + r;     // a warp's row
+    if (gr >= nrows) break;
+    float M = -INFINITY, L = 0.0f;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = 16 * wm + gl + 8 * half;
-      float* o = mine + (size_t)r * kHd + 2 * t;
+    for (int w = 0; w < Cfg::kShares; ++w) M = fmaxf(M, s_m[w * kWM + (r >> 4)][r & 15]);
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int d = 0; d < 16; ++d)
-        *reinterpret_cast<float2*>(o + 8 * d) = make_float2(acc[d][2 * half], acc[d][2 * half + 1]);
-      if (t == 0)
-        *reinterpret_cast<float2*>(mine + (size_t)Cfg::kRows * kHd + 2 * r) =
-            half ? make_float2(m1, l1) : make_float2(m0, l0);
+    for (int w = 0; w < Cfg::kShares; ++w) {
+      const int at = w * kWM + (r >> 4);
+      const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) +
+                                                        ((size_t)at * 16 + (r & 15)) * (kHd + 4) + 4 * d4);
+      const float lw = s_l[at][r & 15];
+      L += lw == 0.0f ? 0.0f : lw * ex2(s_m[at][r & 15] - M);
+      s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
     }
-    __threadfence();
+    if (nact == 1) {
+      const float inv = a.pos0 + gr / a.group >= held ? __int_as_float(0x7fc00000) : 1.0f / L;
+      float* o = a.ctx + ((size_t)(gr / a.group) * a.nq + (size_t)kvh * a.group + gr % a.group) * kHd;
+      reinterpret_cast<float4*>(o)[d4] = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+    } else {
+      reinterpret_cast<float4*>(mine)[i] = s;
+      if (d4 == 0) *reinterpret_cast<float2*>(mine + (size_t)Cfg::kRows * kHd + 2 * r) = make_float2(M, L);
+    }
   }
+  if (nact == 1) return;
+  // the chunks meet in the scratch; the last CTA to arrive adds them in order
+  __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) {
     unsigned* tk = a.ticket + (size_t)kvh * ntile + tile;
@@ -809,6 +809,27 @@ int rows_plan(int nkv, int group, int cap, int ntok, RowsPlan* p) {
   const int most = std::max(1, (cap + kQ8Blk - 1) / kQ8Blk / (p->rows == 128 ? 8 : 2));
   p->chunks = ctas > kDecTickets ? 1 : (int)std::max(1ll, std::min((long long)most, sms / ctas));
   return HV_OK;
+}
+
+// One query token at *pos (at pos0 without one).
+int dec_launch(const float* q, const KvQ8& c, float* ctx, const float* scale, const int32_t* pos,
+               int pos0, int nkv, int group, int cap, void* scratch, void* stream) {
+  int nch = 0;
+  int rc = dec_chunks(nkv, cap, &nch);
+  if (rc) return rc;
+  const bool two = group > 4;
+  rc = smem_attr(two ? (const void*)k_attn_dec_q8<true> : (const void*)k_attn_dec_q8<false>, kDecSmem);
+  if (rc) return rc;
+  unsigned* ticket = static_cast<unsigned*>(scratch);
+  float* part = reinterpret_cast<float*>(ticket + kDecTickets);
+  const dim3 grid(nch, nkv);
+  if (two)
+    k_attn_dec_q8<true><<<grid, 32 * kDecWarps, kDecSmem, (cudaStream_t)stream>>>(
+        q, c, ctx, scale, pos, pos0, group, part, ticket);
+  else
+    k_attn_dec_q8<false><<<grid, 32 * kDecWarps, kDecSmem, (cudaStream_t)stream>>>(
+        q, c, ctx, scale, pos, pos0, group, part, ticket);
+  HV_LAUNCHED("k_attn_dec_q8");
 }
 
 int attn_q8_check(const char* name, const float* q, const void* kv, const float* ctx,
@@ -856,22 +877,7 @@ extern "C" int hv_attn_decode_q8(const float* q, const void* kv, float* ctx, con
   HV_REQUIRE(pos, HV_E_INVALID, "hv_attn_decode_q8: bad arguments");
   KvQ8 c;
   kv_q8_view(const_cast<void*>(kv), nq / group, cap, &c);
-  const int nkv = nq / group;
-  int nch = 0;
-  const int rc2 = dec_chunks(nkv, cap, &nch);
-  if (rc2) return rc2;
-  unsigned* ticket = static_cast<unsigned*>(scratch);
-  float* part = reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + kDecTickets * sizeof(unsigned));
-  const void* fn = group > 4 ? (const void*)k_attn_dec_q8<true> : (const void*)k_attn_dec_q8<false>;
-  const int rc3 = smem_attr(fn, kDecSmem);
-  if (rc3) return rc3;
-  if (group > 4)
-    k_attn_dec_q8<true><<<dim3(nch, nkv), 32 * kDecWarps, kDecSmem, (cudaStream_t)stream>>>(
-        q, c, ctx, scale, pos, group, part, ticket);
-  else
-    k_attn_dec_q8<false><<<dim3(nch, nkv), 32 * kDecWarps, kDecSmem, (cudaStream_t)stream>>>(
-        q, c, ctx, scale, pos, group, part, ticket);
-  HV_LAUNCHED("k_attn_dec_q8");
+  return dec_launch(q, c, ctx, scale, pos, 0, nq / group, group, cap, scratch, stream);
 }
 
 extern "C" int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const float* scale,
@@ -886,6 +892,8 @@ extern "C" int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const
   HV_REQUIRE(ntok <= 65535, HV_E_UNSUPPORTED, "hv_attn_rows_q8: %d rows at once", ntok);
   KvQ8 c;
   kv_q8_view(const_cast<void*>(kv), nq / group, cap, &c);
+  if (ntok == 1)
+    return dec_launch(q, c, ctx, scale, nullptr, pos0, nq / group, group, cap, scratch, stream);
   RowsPlan p;
   const int rc2 = rows_plan(nq / group, group, cap, ntok, &p);
   if (rc2) return rc2;
