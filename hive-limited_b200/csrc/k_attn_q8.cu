@@ -414,6 +414,7 @@ int dec_chunks(int nkv, int cap, int* out) {
 // the same sums. The open block's f32 rows become two binary16 terms as well, so that it is
 // a block like the others with a third product, hi x lo.
 constexpr int kRowWarps = 8;
+constexpr int kRowLeast = 2;           // blocks of a chunk at the least
 
 template <int kWM>
 struct RowsCfg {
@@ -433,18 +434,12 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float s_m[kRowWarps][16], s_l[kRowWarps][16], s_amax[2];
   __shared__ int s_bad;
-  __shared__ unsigned s_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
   const int wm = warp % kWM, share = warp / kWM;
   const int kvh = blockIdx.y, tile = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   const int nrows = a.ntok * a.group, row0 = tile * Cfg::kRows;
-  const int last_row = min(nrows, row0 + Cfg::kRows) - 1;
-  const int held = q8_held(c, kvh), closed = held / kQ8Blk;
-  const int top = min(a.pos0 + last_row / a.group, held - 1);     // the last position to read
-  const int nb = min(closed, top < 0 ? 0 : top / kQ8Blk + 1);
-  const bool tail = top >= closed * kQ8Blk;
-  const int items = nb + (tail ? 1 : 0);
-  const int nact = max(1, min(a.chunks, items / 2));
+  const RowsSpan sp = rows_span(a, c, kvh, row0, Cfg::kRows, kRowLeast);
+  const int held = sp.held, closed = sp.closed, nb = sp.nb, items = sp.items, nact = sp.nact;
   if (chunk >= nact) return;
   const int b0 = (int)((long long)items * chunk / nact);
   const int b1 = (int)((long long)items * (chunk + 1) / nact);
@@ -477,7 +472,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
     else asm volatile("bar.sync %0, %1;" :: "r"(1 + share), "n"(32 * kWM) : "memory");
   };
   // the open rows go first, to the CTA with the last chunk
-  const bool has_open = tail && b1 == items;
+  const bool has_open = items > nb && b1 == items;
   const int nopen = min(held - closed * kQ8Blk, kQ8Blk);
   float* open = reinterpret_cast<float*>(smem + Cfg::kSmem - Cfg::kOpen);
   if (has_open) {
@@ -498,25 +493,28 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
     auto row_ptr = [&](int r) {
       return a.q + (((size_t)(r / a.group)) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd;
     };
+    float4 x[2][8];                      // both rows' loads under way at once
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int r = half ? r1 : r0;
-      float4 x[8];
+      const float4* src = reinterpret_cast<const float4*>(row_ptr(min(r, nrows - 1)) + 4 * t);
+#pragma unroll
+      for (int s = 0; s < 8; ++s) x[half][s] = __ldg(src + 4 * s);
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
       float amax = 0.0f;
 #pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        x[s] = r < nrows ? __ldg(reinterpret_cast<const float4*>(row_ptr(r) + 16 * s + 4 * t))
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
-        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[s].x), fabsf(x[s].y))),
-                     fmaxf(fabsf(x[s].z), fabsf(x[s].w)));
-      }
+      for (int s = 0; s < 8; ++s)
+        amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[half][s].x), fabsf(x[half][s].y))),
+                     fmaxf(fabsf(x[half][s].z), fabsf(x[half][s].w)));
       amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, 2));
       const float lift = q8_lift(amax);
 #pragma unroll
       for (int s = 0; s < 8; ++s) {
-        split_half2(x[s].x * lift, x[s].y * lift, &qh[s][half], &ql[s][half]);
-        split_half2(x[s].z * lift, x[s].w * lift, &qh[s][2 + half], &ql[s][2 + half]);
+        split_half2(x[half][s].x * lift, x[half][s].y * lift, &qh[s][half], &ql[s][half]);
+        split_half2(x[half][s].z * lift, x[half][s].w * lift, &qh[s][2 + half], &ql[s][2 + half]);
       }
       (half ? qs1 : qs0) = qscale / lift;
     }
@@ -778,19 +776,48 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       if (d4 == 0) *reinterpret_cast<float2*>(mine + (size_t)Cfg::kRows * kHd + 2 * r) = make_float2(M, L);
     }
   }
-  if (nact == 1) return;
-  // the chunks meet in the scratch; the last CTA to arrive adds them in order
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    unsigned* tk = a.ticket + (size_t)kvh * ntile + tile;
-    s_last = atomicAdd(tk, 1u) == (unsigned)nact - 1;
-    if (s_last) *tk = 0;
+}
+
+// Adds the chunks of every row, in order: a warp per row, a lane per four dims. (The last CTA of
+// a row tile did this behind a ticket before: 8 us for 16 rows of 18 chunks.)
+__global__ void __launch_bounds__(256) k_rows_join_q8(RowsArgs a, KvQ8 c, int rows, int least) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y;
+  const int row = blockIdx.x * 8 + warp, nrows = a.ntok * a.group;
+  if (row >= nrows) return;
+  const int tile = row / rows, r = row % rows;
+  const RowsSpan sp = rows_span(a, c, kvh, tile * rows, rows, least);
+  if (sp.nact == 1) return;                    // the rows are in ctx already
+  const int ntile = (nrows + rows - 1) / rows;
+  const size_t step = rows_part(rows);
+  const float* base = a.part + ((size_t)kvh * ntile + tile) * a.chunks * step;
+  const float2* ml = reinterpret_cast<const float2*>(base + (size_t)rows * kHd) + r;
+  float M = -INFINITY, L = 0.0f;
+  for (int k = lane; k < sp.nact; k += 32) M = fmaxf(M, __ldcg(ml + k * (step / 2)).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, o));
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = 0; k0 < sp.nact; k0 += 32) {
+    const int k = k0 + lane;
+    float w = 0.0f;                            // a row that sees nothing of a chunk has no sum there
+    if (k < sp.nact) {
+      const float2 x = __ldcg(ml + k * (step / 2));
+      w = x.y == 0.0f ? 0.0f : ex2(x.x - M);
+      L += w * x.y;
+    }
+    const int n = min(32, sp.nact - k0);
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      const float f = __shfl_sync(0xFFFFFFFFu, w, j);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(base + (k0 + j) * step + (size_t)r * kHd) + lane);
+      s.x += f * x.x; s.y += f * x.y; s.z += f * x.z; s.w += f * x.w;
+    }
   }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  rows_join<Cfg::kRows>(a, kvh, slot, nact, row0, nrows, held, reinterpret_cast<float*>(smem));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, o);
+  const int tok = row / a.group;
+  const float inv = a.pos0 + tok >= sp.held ? __int_as_float(0x7fc00000) : 1.0f / L;
+  float* o = a.ctx + ((size_t)tok * a.nq + (size_t)kvh * a.group + row - tok * a.group) * kHd;
+  reinterpret_cast<float4*>(o)[lane] = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
 }
 
 // Rows per CTA and chunks per row tile of a run: 16 rows at a time up to 128, and as many
@@ -806,7 +833,7 @@ int rows_plan(int nkv, int group, int cap, int ntok, RowsPlan* p) {
   p->rows = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128;
   p->tiles = (int)((n + p->rows - 1) / p->rows);
   const long long ctas = (long long)p->tiles * nkv;
-  const int most = std::max(1, (cap + kQ8Blk - 1) / kQ8Blk / (p->rows == 128 ? 8 : 2));
+  const int most = std::max(1, (cap + kQ8Blk - 1) / kQ8Blk / (p->rows == 128 ? kTileLeast : kRowLeast));
   p->chunks = ctas > kDecTickets ? 1 : (int)std::max(1ll, std::min((long long)most, sms / ctas));
   return HV_OK;
 }
@@ -899,8 +926,7 @@ extern "C" int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const
   if (rc2) return rc2;
   RowsArgs a{q, ctx, scale, pos0, ntok, nq, group, p.chunks,
              reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) +
-                                      kDecTickets * sizeof(unsigned)),
-             static_cast<unsigned*>(scratch)};
+                                      kDecTickets * sizeof(unsigned))};
   const dim3 grid((unsigned)(p.tiles * p.chunks), (unsigned)(nq / group));
 #define HV_ROWS(WM)                                                                        \
   {                                                                                        \
@@ -911,9 +937,16 @@ extern "C" int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const
   if (p.rows == 16) HV_ROWS(1)
   else if (p.rows == 32) HV_ROWS(2)
   else if (p.rows == 64) HV_ROWS(4)
-  else
-    return attn_tile_q8_launch(a, c, (unsigned)p.tiles, (unsigned)(nq / group),
-                               (cudaStream_t)stream);
+  else {
+    const int rc3 = attn_tile_q8_launch(a, c, (unsigned)p.tiles, (unsigned)(nq / group),
+                                        (cudaStream_t)stream);
+    if (rc3) return rc3;
+  }
 #undef HV_ROWS
-  HV_LAUNCHED("k_attn_rows_q8");
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail("k_attn_rows_q8", e);
+  if (p.chunks == 1) return HV_OK;
+  k_rows_join_q8<<<dim3((unsigned)((ntok * group + 7) / 8), (unsigned)(nq / group)), 256, 0,
+                   (cudaStream_t)stream>>>(a, c, p.rows, p.rows == 128 ? kTileLeast : kRowLeast);
+  HV_LAUNCHED("k_rows_join_q8");
 }

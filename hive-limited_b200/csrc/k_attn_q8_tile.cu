@@ -191,7 +191,6 @@ struct TlShared {
   float open_max[2];             // of the open rows: largest |K|, |V|
   int bad;                       // first open row with a value that is not finite
   int given_up;
-  unsigned last;
 };
 constexpr int kTlSmem = 4 * kTlTile + kTlRows * kTlLine * 4 + (int)sizeof(TlShared);   // K, V twice
 
@@ -201,18 +200,13 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int kvh = blockIdx.y, tile = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   const int nrows = a.ntok * a.group, row0 = tile * kTlRows;
-  const int last_row = min(nrows, row0 + kTlRows) - 1;
-  const int held = q8_held(c, kvh), closed = held / kQ8Blk;
-  const int top = min(a.pos0 + last_row / a.group, held - 1);     // the last position to read
-  const int nb = min(closed, top < 0 ? 0 : top / kQ8Blk + 1);
-  const bool tail = top >= closed * kQ8Blk;
-  const int items = nb + (tail ? 1 : 0);                          // blocks, the open one last
-  const int nact = max(1, min(a.chunks, items / 8));
+  const RowsSpan sp = rows_span(a, c, kvh, row0, kTlRows, kTileLeast);
+  const int held = sp.held, closed = sp.closed, nb = sp.nb, items = sp.items, nact = sp.nact;
   if (chunk >= nact) return;
   const int b0 = (int)((long long)items * chunk / nact);
   const int b1 = (int)((long long)items * (chunk + 1) / nact);
   const int nt = (b1 - b0 + 3) / 4;
-  const bool has_tail = tail && b1 == items;
+  const bool has_tail = items > nb && b1 == items;
 
   const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem);
   uint8_t* k_buf = smem;                          // two tiles, then V's two
@@ -235,7 +229,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.bad = kQ8Blk;
     sh.open_max[0] = sh.open_max[1] = 0.0f;
-    sh.given_up = 0;
+    sh.given_up = (sm & 1023) != 0;               // the swizzle goes by addresses
   }
   if (warp == 15) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
@@ -265,7 +259,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       else if (gr < nrows)
         reinterpret_cast<float4*>(a.ctx + ((size_t)tok * a.nq + (size_t)kvh * a.group + gr - tok * a.group) * kHd)[lane] = x;
     }
-    if (nact > 1) __threadfence();
   };
   if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsRow));
@@ -769,16 +762,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" :: "r"(tmem));
   }
-  if (nact == 1) return;
-  if (threadIdx.x == 0) {
-    unsigned* tk = a.ticket + (size_t)kvh * ntile + tile;
-    sh.last = atomicAdd(tk, 1u) == (unsigned)nact - 1;
-    if (sh.last) *tk = 0;
-  }
-  __syncthreads();
-  if (!sh.last) return;
-  __threadfence();
-  rows_join<kTlRows>(a, kvh, slot, nact, row0, nrows, held, reinterpret_cast<float*>(smem));
 }
 
 }  // namespace
