@@ -431,10 +431,14 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         uint64_t f2[2], lv2[2], sum[2] = {0, 0};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float f = sc[b + e][0] * qs;
-          f = f == 0.0f ? 1e-38f : f;                       // -inf f has to stay -inf
+          // -inf f has to stay -inf: not with a scale of 0, nor with the scales (which may be
+          // NaN) of a block that the row sees nothing of
+          const bool seen = see0 >= 32 * (b + e);
+          float f = seen ? sc[b + e][0] * qs : 1.0f;
+          f = f == 0.0f ? 1e-38f : f;
+          const float add = seen ? sc[b + e][1] - m0 : 0.0f;
           f2[e] = pair(f, f);
-          lv2[e] = pair(sc[b + e][1] - m0, sc[b + e][1] - m0);
+          lv2[e] = pair(add, add);
         }
 #pragma unroll 1
         for (int h = 0; h < 4; h += 2) {

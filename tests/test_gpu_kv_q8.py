@@ -433,6 +433,118 @@ def test_same_call_same_bits(hv):
         assert np.array_equal(a, out[0][0]) and np.array_equal(b, out[0][1])
 
 
+# Runs of 2^21 (row, position) pairs and more with over 64 rows a head take a kernel of their own.
+
+@pytest.mark.parametrize("nkv,group,pos0,ntok", [
+    (1, 1, 15001, 200), (2, 5, 4000, 71), (4, 8, 100, 250), (8, 8, 0, 200), (1, 3, 5, 1000),
+    (8, 4, 31, 257), (2, 1, 9300, 129), (1, 8, 9000, 33), (5, 7, 1023, 65), (8, 2, 3840, 256)])
+def test_long_runs_attention(hv, nkv, group, pos0, ntok):
+    nq, n = nkv * group, pos0 + ntok
+    assert ntok * group > 64 and ntok * nq * n >= 1 << 21
+    cap = n + 50
+    g, ref, kv = filled(hv, n + group, nkv, n, cap)
+    q, ctx = queries(g, ref, ntok, nq), Dev(np.full((ntok + 1, nq, HD), 7, F32))
+    s = scratch(hv, nq, group, cap, ntok)
+    for _ in range(2):                                         # the scratch is ready again
+        hv.attn_rows_q8(Dev(q), kv, ctx, Dev(np.array([SCALE])), pos0, nq, HD, group, cap, ntok,
+                        s)
+    got = ctx.get(F32, (ntok + 1, nq, HD))
+    assert (got[ntok] == 7).all()
+    for t in {0, 1, ntok // 2, ntok - 2, ntok - 1}:
+        near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
+
+
+def test_long_run_over_positions_that_are_lost_or_not_held(hv):
+    """A poisoned block, non-finite rows of the open block and rows past the length, seen from
+    their positions on; a NaN query and an infinite one lose their own rows only."""
+    nkv, group, cap, pos0, n = 8, 8, 288, 40, 250
+    nq, ntok = nkv * group, 230                                # positions 250 .. 269: not held
+    assert ntok * nq * (pos0 + ntok) >= 1 << 21
+    g = np.random.default_rng(21)
+    k, v = rows(g, n, nkv, 0.3)
+    v[170, 2, 3] = np.inf                                      # block 160 .. 191 of head 2
+    v[231, 1, 7], k[240, 1, 9] = np.inf, np.nan                # the open block, 224 ..
+    ref = R.Cache(nkv, cap)
+    ref.write(k, v, 0)
+    kv, sc = Dev(ref.buffer(0xFF)), Dev(np.array([SCALE]))
+    q = g.standard_normal((ntok, nq, HD)).astype(F32)
+    q[50, 0, 1], q[50, 1, 1], q[51, 60, 127] = np.nan, np.inf, -np.inf
+    ctx = Dev(np.full((ntok + 1, nq, HD), 7, F32))
+    hv.attn_rows_q8(Dev(q), kv, ctx, sc, pos0, nq, HD, group, cap, ntok,
+                    scratch(hv, nq, group, cap, ntok))
+    got = ctx.get(F32, (ntok + 1, nq, HD))
+    assert (got[ntok] == 7).all()
+    assert np.isnan(got[n - pos0:ntok]).all()
+    assert np.isnan(got[50, :2]).all() and np.isnan(got[51, 60]).all()
+    for t in (0, 49, 50, 51, 119, 120, 183, 190, 191, 199, 200, 209):
+        pos = pos0 + t
+        head = np.arange(nq) // group
+        lost = (head == 2) & (pos >= 160)
+        part = (head == 1) & (pos >= 231)
+        bad = lost | part
+        if t == 50:
+            bad |= np.arange(nq) < 2
+        if t == 51:
+            bad |= np.arange(nq) == 60
+        assert np.isnan(got[t][lost]).all()
+        assert not np.isfinite(got[t][part][:, 7]).any()
+        if pos >= 240:
+            assert np.isnan(got[t][head == 1]).all()
+        clean = np.nan_to_num(q[t], posinf=0, neginf=0)
+        want, tol = R.attention(clean, np.nan_to_num(ref.val, posinf=0), pos, group,
+                                float(SCALE))
+        near(got[t][~bad], want[~bad], tol[~bad])
+
+
+@pytest.mark.parametrize("size", [1e-20, 1.0, 1e4, 1e18])
+def test_long_run_sizes_of_q_and_k(hv, size):
+    nkv, group, pos0, ntok, cap = 8, 8, 30, 220, 256
+    nq, n = nkv * group, pos0 + ntok
+    g = np.random.default_rng(22)
+    k, v = rows(g, n, nkv, 0.3)
+    ref = R.Cache(nkv, cap)
+    ref.write((k / F32(size)).astype(F32), (v * F32(size)).astype(F32), 0)
+    q = (g.standard_normal((ntok, nq, HD)) * size).astype(F32)
+    q[-1, 0], q[-1, 1] = 0, ref.val[0, 0, 100] * F32(30) * F32(size) * F32(size)
+    ctx = Dev(np.zeros((ntok, nq, HD), F32))
+    hv.attn_rows_q8(Dev(q), Dev(ref.buffer(0xFF)), ctx, Dev(np.array([SCALE])), pos0, nq, HD,
+                    group, cap, ntok, scratch(hv, nq, group, cap, ntok))
+    got = ctx.get(F32, (ntok, nq, HD))
+    for t in (0, 100, ntok - 1):
+        near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
+
+
+def test_captured_run_equals_the_direct_one(hv):
+    """A write of a run and its attention captured, on a stream that is not the default one."""
+    nkv, group, cap, pos0, ntok = 4, 4, 1000, 700, 200
+    nq = nkv * group
+    g = np.random.default_rng(24)
+    k, v = rows(g, pos0 + ntok, nkv, 0.3)
+    q, sc = Dev(g.standard_normal((ntok, nq, HD)).astype(F32)), Dev(np.array([SCALE]))
+    out = []
+    for graph in (False, True):
+        kv, s = new_cache(hv, nkv, cap), scratch(hv, nq, group, cap, ntok)
+        write(hv, kv, k[:pos0], v[:pos0], 0, cap)
+        dk, dv, ctx = Dev(k[pos0:]), Dev(v[pos0:]), Dev(np.zeros((ntok, nq, HD), F32))
+        hv.synchronize()
+        st = hv.stream_create()
+        if graph:
+            hv.capture_begin(st)
+        hv.kv_rows_q8(dk, dv, nkv * HD, kv, pos0, nkv, HD, cap, ntok, st)
+        hv.attn_rows_q8(q, kv, ctx, sc, pos0, nq, HD, group, cap, ntok, s, st)
+        if graph:
+            gr = hv.capture_end(st)
+            ex = hv.graph_instantiate(gr)
+            for _ in range(3):                                 # the same run again: a rewind
+                hv.graph_launch(ex, st)
+        hv.stream_synchronize(st)
+        out.append(bits(ctx.get(F32)))
+        if graph:
+            hv.graph_destroy(gr, ex)
+        hv.stream_destroy(st)
+    assert np.array_equal(*out)
+
+
 # ---- the engine ----------------------------------------------------------------------
 
 def engine(arch, seed, cap, **kw):
