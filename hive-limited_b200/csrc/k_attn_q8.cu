@@ -820,21 +820,48 @@ __global__ void __launch_bounds__(256) k_rows_join_q8(RowsArgs a, KvQ8 c, int ro
   reinterpret_cast<float4*>(o)[lane] = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
 }
 
-// Rows per CTA and chunks per row tile of a run: 16 rows at a time up to 128, and as many
-// chunks as leave no SM without a CTA, of two blocks or more.
+// Rows per CTA and chunks per row tile of a run. The tile kernel (k_attn_q8_tile.cu) pays for
+// filling its tensor memory, its shared memory and a pipeline of five roles, so it takes runs of
+// more than 64 rows a head that have 2^21 (row, position) pairs or more. Tiles of 64 rows here
+// against it, in microseconds, on either side of that: 0.5 M pairs (8 heads x 64 rows, 200
+// positions x 4) 16.0 : 19.5, 1.0 M 17.2 : 22.7, 1.9 M 26.7 : 29.0, 1.9 M 22.4 : 21.1,
+// 2.2 M 28.1 : 27.3, 4.2 M 24.7 : 20.9, 8.3 M 44.1 : 22.7, 16 M 71.8 : 32.6.
+// Up to 64 rows fill at most half of the 128 that a product of the tile kernel has.
+// As many chunks as leave no SM without a CTA, of two blocks or more (kRowLeast; eight in the
+// tile kernel, whose step is four blocks).
 struct RowsPlan {
   int rows, tiles, chunks;
 };
-int rows_plan(int nkv, int group, int cap, int ntok, RowsPlan* p) {
+constexpr long long kTilePairs = 1ll << 21;
+int rows_chunks(int nkv, int cap, int rows, int tiles, int sms) {
+  const int most = (cap + kQ8Blk - 1) / kQ8Blk / (rows == 128 ? kTileLeast : kRowLeast);
+  return (int)std::max(1ll, std::min((long long)most, sms / ((long long)tiles * nkv)));
+}
+int rows_plan(int nkv, int group, int cap, int pos0, int ntok, RowsPlan* p) {
   int sms = 0;
   const int rc = sm_count(&sms);
   if (rc) return rc;
   const long long n = (long long)ntok * group;
-  p->rows = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 128;
+  const bool tile = n * nkv * (pos0 + (long long)ntok) >= kTilePairs;
+  p->rows = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 || !tile ? 64 : 128;
   p->tiles = (int)((n + p->rows - 1) / p->rows);
-  const long long ctas = (long long)p->tiles * nkv;
-  const int most = std::max(1, (cap + kQ8Blk - 1) / kQ8Blk / (p->rows == 128 ? kTileLeast : kRowLeast));
-  p->chunks = ctas > kDecTickets ? 1 : (int)std::max(1ll, std::min((long long)most, sms / ctas));
+  p->chunks = rows_chunks(nkv, cap, p->rows, p->tiles, sms);
+  return HV_OK;
+}
+// Floats of scratch that any run of up to ntok rows needs: a shorter run can have more chunks.
+int rows_floats(int nkv, int group, int cap, int ntok, size_t* floats) {
+  int sms = 0;
+  const int rc = sm_count(&sms);
+  if (rc) return rc;
+  const long long n = (long long)ntok * group;
+  *floats = 0;
+  for (int rows = 16; rows <= 128; rows *= 2) {
+    const long long tiles = rows < 64 ? 1 : (n + rows - 1) / rows;
+    for (int t = 1; t <= tiles && 2ll * t * nkv <= sms; ++t) {
+      const int chunks = rows_chunks(nkv, cap, rows, t, sms);
+      if (chunks > 1) *floats = std::max(*floats, (size_t)nkv * t * chunks * rows_part(rows));
+    }
+  }
   return HV_OK;
 }
 
@@ -886,11 +913,10 @@ extern "C" int hv_attn_q8_scratch(int nq, int group, int cap, int ntok, size_t* 
   int nch = 0;
   const int rc = dec_chunks(nq / group, cap, &nch);
   if (rc) return rc;
-  RowsPlan p;
-  const int rc2 = rows_plan(nq / group, group, cap, ntok, &p);
+  size_t rows = 0;
+  const int rc2 = ntok > 1 ? rows_floats(nq / group, group, cap, ntok, &rows) : HV_OK;
   if (rc2) return rc2;
   const size_t dec = (size_t)(nq / group) * nch * kDecPart;
-  const size_t rows = p.chunks > 1 ? (size_t)(nq / group) * p.tiles * p.chunks * rows_part(p.rows) : 0;
   *bytes = kDecTickets * sizeof(unsigned) + std::max(dec, rows) * sizeof(float);
   return HV_OK;
 }
@@ -922,7 +948,7 @@ extern "C" int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const
   if (ntok == 1)
     return dec_launch(q, c, ctx, scale, nullptr, pos0, nq / group, group, cap, scratch, stream);
   RowsPlan p;
-  const int rc2 = rows_plan(nq / group, group, cap, ntok, &p);
+  const int rc2 = rows_plan(nq / group, group, cap, pos0, ntok, &p);
   if (rc2) return rc2;
   RowsArgs a{q, ctx, scale, pos0, ntok, nq, group, p.chunks,
              reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) +

@@ -302,7 +302,8 @@ int hv_kv_read_q8(const void* kv, float* k_out, float* v_out, int pos0, int nkv,
  *   hv_attn_rows_q8    row t over positions 0 .. pos0 + t of the cache as it stands: rows of
  *                      a block that this run completed are read quantised.
  * scratch: hv_attn_q8_scratch bytes, 16-byte aligned, zeroed once by the caller; every call
- * leaves it ready for the next. Calls that may overlap on the GPU (streams, captured graphs)
+ * leaves it ready for the next. Those bytes do for decode and for any run of up to ntok rows
+ * over a cache of cap positions. Calls that may overlap on the GPU (streams, captured graphs)
  * need a scratch each. Nothing is allocated. */
 int hv_attn_q8_scratch(int nq, int group, int cap, int ntok, size_t* bytes);
 int hv_attn_decode_q8(const float* q, const void* kv, float* ctx, const float* scale,

@@ -514,6 +514,32 @@ def test_long_run_sizes_of_q_and_k(hv, size):
         near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
 
 
+def test_scratch_does_for_every_shorter_run(hv):
+    for nq, group, cap in ((8, 1, 500), (40, 5, 20000), (32, 4, 4096), (64, 8, 40960),
+                           (148, 1, 8192), (16, 2, 257), (6, 3, 1 << 20)):
+        sizes = [hv.attn_q8_scratch(nq, group, cap, n) for n in range(1, 300)]
+        assert sizes == sorted(sizes)
+    # one for the longest: short runs of many chunks, long ones of one, single tokens
+    nkv, group, n = 8, 5, 3000
+    nq = nkv * group
+    g, ref, kv = filled(hv, 23, nkv, n, n)
+    q, sc = queries(g, ref, 256, nq), Dev(np.array([SCALE]))
+    need = hv.attn_q8_scratch(nq, group, n, 256)
+    room = np.full(need + 4096, 0x5A, np.uint8)
+    room[:need] = 0
+    s = Dev(room)
+    for ntok in (256, 3, 21, 1, 64, 13, 256, 7):
+        ctx = Dev(np.zeros((ntok, nq, HD), F32))
+        if ntok == 1:
+            hv.attn_decode_q8(Dev(q[:1]), kv, ctx, sc, i32(n - 1), nq, HD, group, n, s)
+        else:
+            hv.attn_rows_q8(Dev(q[:ntok]), kv, ctx, sc, n - ntok, nq, HD, group, n, ntok, s)
+        got = ctx.get(F32, (ntok, nq, HD))
+        for t in {0, ntok - 1}:
+            near(got[t], *R.attention(q[t], ref.val, n - ntok + t, group, float(SCALE)))
+        assert (s.get(np.uint8)[need:] == 0x5A).all(), ntok
+
+
 def test_captured_run_equals_the_direct_one(hv):
     """A write of a run and its attention captured, on a stream that is not the default one."""
     nkv, group, cap, pos0, ntok = 4, 4, 1000, 700, 200
