@@ -6,6 +6,7 @@
 // in one pass with the running maximum and sum of the softmax. k_t and v_t are the values the
 // cache reads back: f32(c s) in complete blocks, the f32 rows of the open one.
 #include <algorithm>
+#include <mutex>
 
 #include "attn_q8.cuh"
 #include "attn_q8_rows.h"
@@ -414,7 +415,6 @@ int dec_chunks(int nkv, int cap, int* out) {
 // the same sums. The open block's f32 rows become two binary16 terms as well, so that it is
 // a block like the others with a third product, hi x lo.
 constexpr int kRowWarps = 8;
-constexpr int kRowLeast = 2;           // blocks of a chunk at the least
 
 template <int kWM>
 struct RowsCfg {
@@ -428,7 +428,7 @@ struct RowsCfg {
   static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kTail + kOpen;
 };
 
-template <int kWM>
+template <int kWM, bool kMeet>
 __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, KvQ8 c) {
   using Cfg = RowsCfg<kWM>;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -438,9 +438,13 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   const int wm = warp % kWM, share = warp / kWM;
   const int kvh = blockIdx.y, tile = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   const int nrows = a.ntok * a.group, row0 = tile * Cfg::kRows;
-  const RowsSpan sp = rows_span(a, c, kvh, row0, Cfg::kRows, kRowLeast);
+  const RowsSpan sp = rows_span(a, c, kvh, row0, Cfg::kRows, Cfg::kShares);
   const int held = sp.held, closed = sp.closed, nb = sp.nb, items = sp.items, nact = sp.nact;
-  if (chunk >= nact) return;
+  const bool meet = kMeet && nact > 1;
+  if (chunk >= nact) {
+    if (meet) { cluster_arrive(); cluster_wait(); cluster_arrive(); cluster_wait(); }
+    return;
+  }
   const int b0 = (int)((long long)items * chunk / nact);
   const int b1 = (int)((long long)items * (chunk + 1) / nact);
   const int c1 = min(b1, nb);                       // blocks b0 .. c1 from codes, then the tail
@@ -730,6 +734,9 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
+  const RowsLand land(smem + Cfg::kSmem - Cfg::kOpen - Cfg::kTail, Cfg::kRows, nact);
+  static_assert(rows_land_bytes(Cfg::kRows) <= Cfg::kOpen + Cfg::kTail, "room for the chunks' sums");
+  if (meet) cluster_arrive();
   {
     float M0 = -INFINITY, M1 = -INFINITY;
 #pragma unroll
@@ -750,6 +757,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   const int ntile = gridDim.x / a.chunks;
   const size_t slot = ((size_t)kvh * ntile + tile) * a.chunks;
   float* mine = a.part + (slot + chunk) * rows_part(Cfg::kRows);
+  if (meet) cluster_wait();
   __syncthreads();
   for (int i = threadIdx.x; i < Cfg::kRows * (kHd / 4); i += blockDim.x) {
     const int r = i / (kHd / 4), d4 = i % (kHd / 4), gr = row0 + r;     // a warp's row
@@ -771,15 +779,23 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       const float inv = a.pos0 + gr / a.group >= held ? __int_as_float(0x7fc00000) : 1.0f / L;
       float* o = a.ctx + ((size_t)(gr / a.group) * a.nq + (size_t)kvh * a.group + gr % a.group) * kHd;
       reinterpret_cast<float4*>(o)[d4] = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+    } else if (meet) {
+      land.send_sums(chunk, r, d4, s);
+      if (d4 == 0) land.send_ml(chunk, r, M, L);
     } else {
       reinterpret_cast<float4*>(mine)[i] = s;
       if (d4 == 0) *reinterpret_cast<float2*>(mine + (size_t)Cfg::kRows * kHd + 2 * r) = make_float2(M, L);
     }
   }
+  if (meet) {
+    cluster_arrive();
+    cluster_wait();
+    land.add_up(a, kvh, row0, Cfg::kRows, chunk, warp, kRowWarps, lane, held);
+  }
 }
 
-// Adds the chunks of every row, in order: a warp per row, a lane per four dims. (The last CTA of
-// a row tile did this behind a ticket before: 8 us for 16 rows of 18 chunks.)
+// Adds the chunks of every row that are no cluster, in order: a warp per row, a lane per four
+// dims. (The last CTA of a row tile, behind a ticket, took 8 us for 16 rows of 18 chunks.)
 __global__ void __launch_bounds__(256) k_rows_join_q8(RowsArgs a, KvQ8 c, int rows, int least) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y;
   const int row = blockIdx.x * 8 + warp, nrows = a.ntok * a.group;
@@ -827,25 +843,63 @@ __global__ void __launch_bounds__(256) k_rows_join_q8(RowsArgs a, KvQ8 c, int ro
 // positions x 4) 16.0 : 19.5, 1.0 M 17.2 : 22.7, 1.9 M 26.7 : 29.0, 1.9 M 22.4 : 21.1,
 // 2.2 M 28.1 : 27.3, 4.2 M 24.7 : 20.9, 8.3 M 44.1 : 22.7, 16 M 71.8 : 32.6.
 // Up to 64 rows fill at most half of the 128 that a product of the tile kernel has.
-// As many chunks as leave no SM without a CTA, of two blocks or more (kRowLeast; eight in the
-// tile kernel, whose step is four blocks).
 struct RowsPlan {
   int rows, tiles, chunks;
+  bool cluster;
 };
 constexpr long long kTilePairs = 1ll << 21;
-int rows_chunks(int nkv, int cap, int rows, int tiles, int sms) {
-  const int most = (cap + kQ8Blk - 1) / kQ8Blk / (rows == 128 ? kTileLeast : kRowLeast);
+// Blocks that a CTA works on at once, and of a chunk at the least: one for each share.
+int rows_step(int rows) { return rows == 128 ? kTileLeast / 2 : 16 * kRowWarps / rows; }
+int rows_least(int rows) { return rows == 128 ? kTileLeast : rows_step(rows); }
+// As many chunks as leave no SM without a CTA.
+int rows_chunks(int nkv, int npos, int rows, int tiles, int sms) {
+  const int most = (npos + kQ8Blk - 1) / kQ8Blk / rows_least(rows);
   return (int)std::max(1ll, std::min((long long)most, sms / ((long long)tiles * nkv)));
 }
-int rows_plan(int nkv, int group, int cap, int pos0, int ntok, RowsPlan* p) {
+// Clusters of n CTAs that the GPU holds at once, a CTA having an SM to itself.
+int cluster_room(int n, int* room) {
+  static std::mutex mu;
+  static int known[64][kRowsCluster + 1];
+  int dev = 0;
+  HV_CUDA(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lk(mu);
+  int (&of)[kRowsCluster + 1] = known[dev & 63];
+  for (int k = 2; k <= kRowsCluster && !of[kRowsCluster]; ++k) {
+    const int rc = attn_tile_q8_room(k, &of[k]);
+    if (rc) return rc;
+  }
+  *room = of[n];
+  return HV_OK;
+}
+int rows_plan(int nkv, int group, int pos0, int ntok, RowsPlan* p) {
   int sms = 0;
   const int rc = sm_count(&sms);
   if (rc) return rc;
   const long long n = (long long)ntok * group;
-  const bool tile = n * nkv * (pos0 + (long long)ntok) >= kTilePairs;
+  const int npos = pos0 + ntok, blocks = (npos + kQ8Blk - 1) / kQ8Blk;
+  const bool tile = n * nkv * npos >= kTilePairs;
   p->rows = n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 || !tile ? 64 : 128;
   p->tiles = (int)((n + p->rows - 1) / p->rows);
-  p->chunks = rows_chunks(nkv, cap, p->rows, p->tiles, sms);
+  p->chunks = rows_chunks(nkv, npos, p->rows, p->tiles, sms);
+  p->cluster = false;
+  // Chunks that are a cluster need no second launch, which costs as much as one step here or two
+  // of the tile kernel's; they are eight at most, and as many as let all clusters run at once. In
+  // microseconds, as a cluster and not: 44 x 2 rows, 300 positions (2 steps, 2) 11.8 : 13.9;
+  // 4 x 4 rows, 4000 positions (2, 1) 15.8 : 17.6; 32 x 4 rows, 1032 positions (3, 2)
+  // 17.3 : 16.7; 8 x 4 rows, 4000 positions (4, 2) 19.5 : 18.6; tile kernel, 32 x 4 rows, 4000
+  // positions (4, 2) 19.3 : 21.4 and 256 x 4, 4096 positions (16, 16) 43.4 : 46.4; 16 clusters
+  // of 8, where 15 run at once, 26.1 : 16.9.
+  const int step = rows_step(p->rows);
+  auto steps = [&](int chunks) { return ((blocks + chunks - 1) / chunks + step - 1) / step; };
+  for (int c = std::min(p->chunks, kRowsCluster); c > 1; --c) {
+    int room = 0;
+    const int rc2 = cluster_room(c, &room);
+    if (rc2) return rc2;
+    if ((long long)p->tiles * nkv > room) continue;
+    p->cluster = steps(c) <= steps(p->chunks) + (p->rows == 128 ? 2 : 1);
+    if (p->cluster) p->chunks = c;
+    break;
+  }
   return HV_OK;
 }
 // Floats of scratch that any run of up to ntok rows needs: a shorter run can have more chunks.
@@ -863,6 +917,16 @@ int rows_floats(int nkv, int group, int cap, int ntok, size_t* floats) {
     }
   }
   return HV_OK;
+}
+
+template <int kWM, bool kMeet>
+int rows_go(const RowsArgs& a, const KvQ8& c, dim3 grid, cudaStream_t st) {
+  const int rc = smem_attr((const void*)k_attn_rows_q8<kWM, kMeet>, RowsCfg<kWM>::kSmem);
+  return rc ? rc : rows_launch(k_attn_rows_q8<kWM, kMeet>, grid, 32 * kRowWarps, RowsCfg<kWM>::kSmem, a, c, st);
+}
+template <int kWM>
+int rows_go(const RowsArgs& a, const KvQ8& c, dim3 grid, cudaStream_t st) {
+  return a.cluster ? rows_go<kWM, true>(a, c, grid, st) : rows_go<kWM, false>(a, c, grid, st);
 }
 
 // One query token at *pos (at pos0 without one).
@@ -948,31 +1012,20 @@ extern "C" int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const
   if (ntok == 1)
     return dec_launch(q, c, ctx, scale, nullptr, pos0, nq / group, group, cap, scratch, stream);
   RowsPlan p;
-  const int rc2 = rows_plan(nq / group, group, cap, pos0, ntok, &p);
+  const int rc2 = rows_plan(nq / group, group, pos0, ntok, &p);
   if (rc2) return rc2;
   RowsArgs a{q, ctx, scale, pos0, ntok, nq, group, p.chunks,
+p.cluster,
              reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) +
                                       kDecTickets * sizeof(unsigned))};
   const dim3 grid((unsigned)(p.tiles * p.chunks), (unsigned)(nq / group));
-#define HV_ROWS(WM)                                                                        \
-  {                                                                                        \
-    const int rc3 = smem_attr((const void*)k_attn_rows_q8<WM>, RowsCfg<WM>::kSmem);        \
-    if (rc3) return rc3;                                                                   \
-    k_attn_rows_q8<WM><<<grid, 32 * kRowWarps, RowsCfg<WM>::kSmem, (cudaStream_t)stream>>>(a, c); \
-  }
-  if (p.rows == 16) HV_ROWS(1)
-  else if (p.rows == 32) HV_ROWS(2)
-  else if (p.rows == 64) HV_ROWS(4)
-  else {
-    const int rc3 = attn_tile_q8_launch(a, c, (unsigned)p.tiles, (unsigned)(nq / group),
-                                        (cudaStream_t)stream);
-    if (rc3) return rc3;
-  }
-#undef HV_ROWS
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail("k_attn_rows_q8", e);
-  if (p.chunks == 1) return HV_OK;
+  const cudaStream_t st = (cudaStream_t)stream;
+  const int rc3 = p.rows == 16 ? rows_go<1>(a, c, grid, st) : p.rows == 32 ? rows_go<2>(a, c, grid, st)
+                : p.rows == 64 ? rows_go<4>(a, c, grid, st)
+                : attn_tile_q8_launch(a, c, (unsigned)p.tiles, (unsigned)(nq / group), st);
+  if (rc3) return rc3;
+  if (p.chunks == 1 || a.cluster) return HV_OK;
   k_rows_join_q8<<<dim3((unsigned)((ntok * group + 7) / 8), (unsigned)(nq / group)), 256, 0,
-                   (cudaStream_t)stream>>>(a, c, p.rows, p.rows == 128 ? kTileLeast : kRowLeast);
+                   st>>>(a, c, p.rows, rows_least(p.rows));
   HV_LAUNCHED("k_rows_join_q8");
 }

@@ -194,6 +194,7 @@ struct TlShared {
 };
 constexpr int kTlSmem = 4 * kTlTile + kTlRows * kTlLine * 4 + (int)sizeof(TlShared);   // K, V twice
 
+template <bool kMeet>
 __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8 c) {
   extern __shared__ __align__(1024) uint8_t smem[];
   TlShared& sh = *reinterpret_cast<TlShared*>(smem + 4 * kTlTile + kTlRows * kTlLine * 4);
@@ -202,7 +203,11 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   const int nrows = a.ntok * a.group, row0 = tile * kTlRows;
   const RowsSpan sp = rows_span(a, c, kvh, row0, kTlRows, kTileLeast);
   const int held = sp.held, closed = sp.closed, nb = sp.nb, items = sp.items, nact = sp.nact;
-  if (chunk >= nact) return;
+  const bool meet = kMeet && nact > 1;
+  if (chunk >= nact) {
+    if (meet) { cluster_arrive(); cluster_wait(); cluster_arrive(); cluster_wait(); }
+    return;
+  }
   const int b0 = (int)((long long)items * chunk / nact);
   const int b1 = (int)((long long)items * (chunk + 1) / nact);
   const int nt = (b1 - b0 + 3) / 4;
@@ -246,15 +251,21 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   const size_t slot = ((size_t)kvh * ntile + tile) * a.chunks;
   float* lines = reinterpret_cast<float*>(smem + 4 * kTlTile);    // [row][kTlLine]
   auto rows_sync = [] { asm volatile("bar.sync 3, 256;" ::: "memory"); };
-  // the rows' sums, once they stand in `lines`: to ctx, or to this chunk's part of the scratch
+  const RowsLand land(smem, kTlRows, nact);       // over the tiles, once they have been multiplied
+  static_assert(rows_land_bytes(kTlRows) <= 4 * kTlTile, "room for the chunks' sums");
+  // the rows' sums, once they stand in `lines`: to ctx, to the cluster's CTA that adds them up, or
+  // to this chunk's part of the scratch
   auto rows_out = [&] {
     asm volatile("bar.sync 2, 384;" ::: "memory");
+    if (meet) cluster_wait();
     float4* part = reinterpret_cast<float4*>(a.part + (slot + chunk) * rows_part(kTlRows));
 #pragma unroll 4
     for (int r = warp; r < kTlRows; r += 12) {
       const float4 x = *reinterpret_cast<const float4*>(lines + (size_t)r * kTlLine + 4 * lane);
       const int gr = row0 + r, tok = gr / a.group;
-      if (nact > 1)
+      if (meet) {
+        if (gr < nrows) land.send_sums(chunk, r, lane, x);
+      } else if (nact > 1)
         part[r * (kHd / 4) + lane] = x;
       else if (gr < nrows)
         reinterpret_cast<float4*>(a.ctx + ((size_t)tok * a.nq + (size_t)kvh * a.group + gr - tok * a.group) * kHd)[lane] = x;
@@ -482,6 +493,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     }
     sh.m[w][row] = m;
     sh.l[w][row] = l;
+    if (meet) cluster_arrive();
     asm volatile("bar.sync 1, 384;" ::: "memory");         // with the warps that have the sums
     rows_out();
   } else if (warp < 12) {
@@ -516,6 +528,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
                                 mul2(pair(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), fo2));
       }
     }
+    if (meet) cluster_arrive();
     asm volatile("bar.sync 1, 384;" ::: "memory");
     const float nan = __int_as_float(0x7fc00000);
     const float l0 = sh.l[0][row], l1 = sh.l[1][row];
@@ -534,9 +547,10 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       *reinterpret_cast<float4*>(line + 2 * d) = make_float4(x.x * f, x.y * f, y.x * f, y.y * f);
     }
     float* part = a.part + (slot + chunk) * rows_part(kTlRows);
-    if (nact > 1)
+    if (nact > 1 && !meet)
       *reinterpret_cast<float2*>(part + kTlRows * kHd + 2 * row) = make_float2(M, L);
     rows_out();
+    if (meet && grow < nrows) land.send_ml(chunk, row, M, L);
   } else if (warp < 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsConv));
     // a warp per block of the tile
@@ -758,6 +772,12 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         bar_arrive(bar(sh.full_v[s]));
       }
     }
+    if (meet) { cluster_arrive(); cluster_wait(); }
+  }
+  if (meet) {
+    cluster_arrive();
+    cluster_wait();
+    land.add_up(a, kvh, row0, kTlRows, chunk, warp, kTlThreads / 32, lane, held);
   }
   __syncwarp();
   fence_before();
@@ -770,18 +790,31 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
 
 }  // namespace
 
-int attn_tile_q8_launch(const RowsArgs& a, const KvQ8& c, unsigned tiles, unsigned nkv,
-                        cudaStream_t st) {
-  const int rc = smem_attr((const void*)k_attn_tile_q8, kTlSmem);
+template <bool kMeet>
+static int tile_launch(const RowsArgs& a, const KvQ8& c, unsigned tiles, unsigned nkv, cudaStream_t st) {
+  const int rc = smem_attr((const void*)k_attn_tile_q8<kMeet>, kTlSmem);
   if (rc) return rc;
   // registers are dealt out of what the kernel starts with: a share too large would wait for good
   static const int regs = [] {
     cudaFuncAttributes f{};
-    return cudaFuncGetAttributes(&f, k_attn_tile_q8) == cudaSuccess ? f.numRegs : 0;
+    return cudaFuncGetAttributes(&f, k_attn_tile_q8<kMeet>) == cudaSuccess ? f.numRegs : 0;
   }();
   HV_REQUIRE(regs == kTlRegs, HV_E_UNSUPPORTED, "k_attn_tile_q8: built with %d registers", regs);
-  k_attn_tile_q8<<<dim3(tiles * a.chunks, nkv), kTlThreads, kTlSmem, st>>>(a, c);
-  HV_LAUNCHED("k_attn_tile_q8");
+  return rows_launch(k_attn_tile_q8<kMeet>, dim3(tiles * a.chunks, nkv), kTlThreads, kTlSmem, a, c, st);
+}
+
+int attn_tile_q8_room(int n, int* room) {
+  const int rc = smem_attr((const void*)k_attn_tile_q8<true>, kTlSmem);
+  if (rc) return rc;
+  cudaLaunchAttribute at{};
+  cudaLaunchConfig_t cfg = rows_config(dim3(n), kTlThreads, kTlSmem, n, &at, nullptr);
+  HV_CUDA(cudaOccupancyMaxActiveClusters(room, k_attn_tile_q8<true>, &cfg));
+  return HV_OK;
+}
+
+int attn_tile_q8_launch(const RowsArgs& a, const KvQ8& c, unsigned tiles, unsigned nkv,
+                        cudaStream_t st) {
+  return a.cluster ? tile_launch<true>(a, c, tiles, nkv, st) : tile_launch<false>(a, c, tiles, nkv, st);
 }
 
 }  // namespace hv

@@ -233,7 +233,8 @@ def test_decode_attention(hv, nkv, group, n):
 
 @pytest.mark.parametrize("nkv,group,pos0,ntok", [
     (1, 1, 0, 1), (2, 4, 0, 33), (8, 2, 256, 44), (2, 5, 31, 70), (4, 8, 100, 129), (1, 3, 5, 200),
-    (8, 4, 992, 64), (2, 1, 0, 256), (1, 8, 3000, 17), (2, 4, 4000, 3), (2, 7, 511, 1)])
+    (8, 4, 992, 64), (2, 1, 0, 256), (1, 8, 3000, 17), (2, 4, 4000, 3), (2, 7, 511, 1),
+    (8, 4, 1000, 32), (8, 2, 0, 256), (5, 3, 700, 40), (1, 1, 9000, 2), (40, 1, 2000, 5)])
 def test_rows_attention(hv, nkv, group, pos0, ntok):
     nq, n = nkv * group, pos0 + ntok
     cap = n + 50
