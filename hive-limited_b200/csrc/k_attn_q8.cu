@@ -24,12 +24,12 @@ namespace {
 // Both products keep the codes as the 16-row operand and the group's queries as the 8
 // columns: S^T = K q^T, then ctx^T += V^T w^T. With up to four heads in the group the columns
 // are the four hi and the four lo terms (kTwo = false); with five to eight, hi and lo are two
-// products. Each warp keeps its own running maximum and sums; they meet in shared memory and,
-// between a head's chunks, in the caller's scratch, where the last CTA to arrive adds them
-// in chunk order.
+// products. Each warp keeps its own running maximum and sums; they meet in shared memory. The
+// chunks of a head meet, added in chunk order, in a cluster's shared memory (kMeet), or, where a
+// head has more than a cluster's eight, in the caller's scratch by the last CTA to arrive.
 constexpr int kDecWarps = 8;
 constexpr int kDecStages = 2;
-constexpr int kDecBlocksMin = 8;       // blocks a chunk holds before a head gets another CTA
+constexpr int kDecBlocksMin = 8;       // of a chunk, one a warp (1000 positions: 4 6.4 us, 8 6.8, 12 7.7, 16 8.0)
 constexpr int kDecStride = 132;        // floats between the columns of a warp's sums
 constexpr int kDecTickets = 1024;      // kv heads with chunks to join: first in the scratch
 constexpr int kDecPart = 8 * (kHd + 2);    // scratch floats of a chunk: sums, then (max, sum)
@@ -41,7 +41,7 @@ HV_DEV void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
 }
 
-template <bool kTwo>
+template <bool kTwo, bool kMeet>
 __global__ void __launch_bounds__(32 * kDecWarps, 1)
     k_attn_dec_q8(const float* __restrict__ q, KvQ8 c, float* __restrict__ ctx,
                   const float* __restrict__ scale, const int32_t* __restrict__ pos_p, int pos0, int group,
@@ -65,7 +65,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   const int ntail = max(0, pos + 1 - closed * kQ8Blk);
   int nact = (nb + kDecBlocksMin - 1) / kDecBlocksMin;
   nact = max(1, min(nact, (int)gridDim.x));
-  if (chunk >= nact) return;
+  const bool meet = kMeet && nact > 1;
+  if (chunk >= nact) {
+    if (meet) { cluster_arrive(); cluster_wait(); cluster_arrive(); cluster_wait(); }
+    return;
+  }
   const int b0 = (int)((long long)nb * chunk / nact), b1 = (int)((long long)nb * (chunk + 1) / nact);
 
   // this lane's units of a block: 16 bytes at 512 u + 16 lane of K, then of V
@@ -306,6 +310,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
+  if (meet) cluster_arrive();                            // the open rows' place is free
   float* red = reinterpret_cast<float*>(smem);           // [warp][column][kDecStride]
   float M0 = -INFINITY, M1 = -INFINITY;
 #pragma unroll
@@ -326,28 +331,46 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     }
   }
   __syncthreads();
-  const int vals = group * kHd;
   const size_t slot = (size_t)kvh * gridDim.x + chunk;
   float* pacc = part + slot * kDecPart;
   float* pml = pacc + 8 * kHd;
-  for (int i = threadIdx.x; i < vals; i += blockDim.x) {
-    const int h = i / kHd, d = i % kHd;
-    float M = -INFINITY, L = 0.0f, A = 0.0f;
+  const RowsLand land(smem + kDecRing, group, nact);
+  static_assert(rows_land_bytes(8) <= kDecSmem - kDecRing, "room for the chunks' sums");
+  if (meet) cluster_wait();
+  const int units = group * (kHd / 4);                   // of four outputs, one a thread
+  static_assert(8 * (kHd / 4) <= 32 * kDecWarps, "a thread for each");
+  if ((int)threadIdx.x < units) {
+    const int i = threadIdx.x, h = i / (kHd / 4), d = 4 * (i % (kHd / 4));
+    float M = -INFINITY, L = 0.0f;
+    float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, s_m[w][h]);
+    auto add = [&](const float* p) {
+      const float4 x = *reinterpret_cast<const float4*>(p);
+      A.x += x.x; A.y += x.y; A.z += x.z; A.w += x.w;
+    };
 #pragma unroll
     for (int w = 0; w < kDecWarps; ++w) {
-      const float a = s_l[w][h] == 0.0f ? 0.0f : ex2(s_m[w][h] - M);
-      L += a * s_l[w][h];
-      A += red[((size_t)w * 8 + h) * kDecStride + d];
-      if (!kTwo) A += red[((size_t)w * 8 + 4 + h) * kDecStride + d];
+      L += s_l[w][h] == 0.0f ? 0.0f : ex2(s_m[w][h] - M) * s_l[w][h];
+      add(red + ((size_t)w * 8 + h) * kDecStride + d);
+      if (!kTwo) add(red + ((size_t)w * 8 + 4 + h) * kDecStride + d);
     }
     if (nact == 1) {
-      out[i] = A / L;
+      reinterpret_cast<float4*>(out)[i] = make_float4(A.x / L, A.y / L, A.z / L, A.w / L);
+    } else if (meet) {
+      land.send_sums(chunk, h, d / 4, A);
+      if (d == 0) land.send_ml(chunk, h, M, L);
     } else {
-      pacc[i] = A;
+      reinterpret_cast<float4*>(pacc)[i] = A;
       if (d == 0) { pml[2 * h] = M; pml[2 * h + 1] = L; }
     }
+  }
+  if (meet) {
+    cluster_arrive();
+    cluster_wait();
+    const RowsArgs a{q, ctx, scale, pos, 1, 0, group, 0, true, nullptr};
+    land.add_up(a, kvh, 0, group, chunk, warp, kDecWarps, lane, held);
+    return;
   }
   if (nact == 1) return;
 
@@ -382,8 +405,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     if (lane == 0) s_l[0][warp] = L;
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < vals / 4; i += blockDim.x) {
-    const int h = i / (kHd / 4);
+  if ((int)threadIdx.x < units) {
+    const int i = threadIdx.x, h = i / (kHd / 4);
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int k = 0; k < nact; ++k) {
@@ -936,18 +959,35 @@ int dec_launch(const float* q, const KvQ8& c, float* ctx, const float* scale, co
   int rc = dec_chunks(nkv, cap, &nch);
   if (rc) return rc;
   const bool two = group > 4;
-  rc = smem_attr(two ? (const void*)k_attn_dec_q8<true> : (const void*)k_attn_dec_q8<false>, kDecSmem);
-  if (rc) return rc;
+  // As a cluster the chunks are joined through shared memory, for which the two trips to the
+  // scratch and the ticket take 2 us. It has eight at most, and as many as let all heads run at
+  // once, so that a full cache takes more steps of a block a warp. In microseconds, as a cluster
+  // and not, 8 heads x 4 queries: 300 positions (steps 1, 1) 6.6 : 8.4, 2000 (1, 1) 7.3 : 9.4,
+  // 4225 (3, 1) 8.4 : 9.3, 8000 (4, 2) 9.6 : 10.9, 16000 (8, 4) 13.5 : 13.6, 39999 (20, 9)
+  // 26.8 : 22.7. Only the cache's size is known here, and a cache is full at its end only.
+  const int blocks = (cap + kQ8Blk - 1) / kQ8Blk;
+  auto steps = [&](int chunks) { return ((blocks + chunks - 1) / chunks + kDecWarps - 1) / kDecWarps; };
+  bool meet = false;
+  for (int k = std::min(nch, kRowsCluster); k > 1 && !meet; --k) {
+    int room = 0;
+    rc = cluster_room(k, &room);
+    if (rc) return rc;
+    if (nkv > room) continue;
+    meet = steps(k) <= steps(nch) + 4;
+    if (!meet) break;
+    nch = k;
+  }
   unsigned* ticket = static_cast<unsigned*>(scratch);
   float* part = reinterpret_cast<float*>(ticket + kDecTickets);
-  const dim3 grid(nch, nkv);
-  if (two)
-    k_attn_dec_q8<true><<<grid, 32 * kDecWarps, kDecSmem, (cudaStream_t)stream>>>(
-        q, c, ctx, scale, pos, pos0, group, part, ticket);
-  else
-    k_attn_dec_q8<false><<<grid, 32 * kDecWarps, kDecSmem, (cudaStream_t)stream>>>(
-        q, c, ctx, scale, pos, pos0, group, part, ticket);
-  HV_LAUNCHED("k_attn_dec_q8");
+  auto* fn = two ? (meet ? k_attn_dec_q8<true, true> : k_attn_dec_q8<true, false>)
+                 : (meet ? k_attn_dec_q8<false, true> : k_attn_dec_q8<false, false>);
+  rc = smem_attr((const void*)fn, kDecSmem);
+  if (rc) return rc;
+  cudaLaunchAttribute at{};
+  const cudaLaunchConfig_t cfg = rows_config(dim3(nch, nkv), 32 * kDecWarps, kDecSmem,
+                                             meet ? nch : 1, &at, (cudaStream_t)stream);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, q, c, ctx, scale, pos, pos0, group, part, ticket);
+  return e == cudaSuccess ? HV_OK : cuda_fail("k_attn_dec_q8", e);
 }
 
 int attn_q8_check(const char* name, const float* q, const void* kv, const float* ctx,
