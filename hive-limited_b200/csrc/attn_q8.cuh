@@ -7,6 +7,7 @@
 // bits, and the products accumulate in f32.
 #pragma once
 
+#include "hv_wait.cuh"
 #include "kv_q8.cuh"
 
 namespace hv {
@@ -65,6 +66,37 @@ HV_DEV float q8_lift(float amax) {
   int e = 13 + 127 - (int)(__float_as_uint(amax) >> 23);        // 13 - floor(log2 amax)
   e = e > 126 ? 126 : (e < -126 ? -126 : e);
   return __uint_as_float((unsigned)(e + 127) << 23);
+}
+
+constexpr unsigned long long kQ8WaitNs = 2000000000ull;     // of a wait on a barrier of a CTA's own
+
+HV_DEV void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count) : "memory");
+}
+// False when the wait ran out here or elsewhere in the CTA.
+HV_DEV bool bar_wait(uint32_t bar, uint32_t parity, volatile int* given_up) {
+  unsigned long long t0 = 0;
+  for (unsigned n = 1;; ++n) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    if (ok) return true;
+    if ((n & 63) == 0) {
+      if (*given_up) return false;
+      const unsigned long long now = global_ns();
+      if (t0 == 0) t0 = now;
+      else if (now - t0 > kQ8WaitNs) { *given_up = 1; return false; }
+    }
+  }
+}
+
+// The same for a whole warp, whose lanes go on or leave together.
+HV_DEV bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* given_up) {
+  const bool ok = bar_wait(bar, parity, given_up);
+  return __all_sync(0xFFFFFFFFu, ok) != 0;
 }
 
 }  // namespace hv

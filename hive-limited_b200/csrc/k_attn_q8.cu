@@ -19,14 +19,16 @@ namespace {
 //
 // Bound by the bytes of the cache for long contexts and by latency for short ones: the
 // positions of a kv head are cut into chunks of whole blocks, one CTA each, and a warp takes
-// blocks in turn. A block's 8 KB of codes comes by asynchronous copies, kDecStages of them
-// ahead; a lane copies exactly the bytes it will multiply, so nothing has to be synchronised.
+// blocks in turn, the 8 KB of codes of kDecStages blocks on their way. For short caches they come
+// by 16-byte asynchronous copies, a lane copying exactly the bytes it will multiply, for long ones
+// (kLong) by one bulk copy a block, with barriers of each warp's own whose waits are bounded (one
+// that runs out leaves NaN): 1000 positions 6.8 us and 7.1, 131072 positions 54.2 and 49.8.
 // Both products keep the codes as the 16-row operand and the group's queries as the 8
 // columns: S^T = K q^T, then ctx^T += V^T w^T. With up to four heads in the group the columns
 // are the four hi and the four lo terms (kTwo = false); with five to eight, hi and lo are two
 // products. Each warp keeps its own running maximum and sums; they meet in shared memory. The
-// chunks of a head meet, added in chunk order, in a cluster's shared memory (kMeet), or, where a
-// head has more than a cluster's eight, in the caller's scratch by the last CTA to arrive.
+// chunks of a head meet, added in chunk order, in a cluster's shared memory, or, where a head has
+// more than a cluster's eight (kLong), in the caller's scratch by the last CTA to arrive.
 constexpr int kDecWarps = 8;
 constexpr int kDecStages = 2;
 constexpr int kDecBlocksMin = 8;       // of a chunk, one a warp (1000 positions: 4 6.4 us, 8 6.8, 12 7.7, 16 8.0)
@@ -41,7 +43,7 @@ HV_DEV void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" :: "r"(dst), "l"(src) : "memory");
 }
 
-template <bool kTwo, bool kMeet>
+template <bool kTwo, bool kLong>
 __global__ void __launch_bounds__(32 * kDecWarps, 1)
     k_attn_dec_q8(const float* __restrict__ q, KvQ8 c, float* __restrict__ ctx,
                   const float* __restrict__ scale, const int32_t* __restrict__ pos_p, int pos0, int group,
@@ -50,6 +52,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   __shared__ float s_m[kDecWarps][8], s_l[kDecWarps][8], s_x[kQ8Blk][8];
   __shared__ __align__(16) float s_q[8][kDecLine];
   __shared__ unsigned s_last;
+  __shared__ unsigned long long s_full[kDecWarps][kDecStages];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, chunk = blockIdx.x;
   const int pos = pos_p ? *pos_p : pos0, held = q8_held(c, kvh);
@@ -65,7 +68,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   const int ntail = max(0, pos + 1 - closed * kQ8Blk);
   int nact = (nb + kDecBlocksMin - 1) / kDecBlocksMin;
   nact = max(1, min(nact, (int)gridDim.x));
-  const bool meet = kMeet && nact > 1;
+  const bool meet = !kLong && nact > 1;
   if (chunk >= nact) {
     if (meet) { cluster_arrive(); cluster_wait(); cluster_arrive(); cluster_wait(); }
     return;
@@ -73,17 +76,34 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   const int b0 = (int)((long long)nb * chunk / nact), b1 = (int)((long long)nb * (chunk + 1) / nact);
 
   // this lane's units of a block: 16 bytes at 512 u + 16 lane of K, then of V
-  const uint8_t* codes = c.codes + (size_t)kvh * c.nblk * 2 * kQ8Codes + 16 * lane;
+  const uint8_t* codes = c.codes + (size_t)kvh * c.nblk * 2 * kQ8Codes;
   const float2* scales = reinterpret_cast<const float2*>(c.scales) + (size_t)kvh * c.nblk;
   const uint8_t* ring = smem + (size_t)warp * kDecStages * 2 * kQ8Codes + 16 * lane;
   const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
-  auto fetch = [&](int b, int stage) {
-    if (b < b1) {
-      const uint8_t* src = codes + (size_t)b * 2 * kQ8Codes;
+  const uint32_t full = (uint32_t)__cvta_generic_to_shared(&s_full[warp][0]);
+  if (kLong && lane == 0) {
 #pragma unroll
-      for (int u = 0; u < 16; ++u) cp_async16(ring_s + stage * 2 * kQ8Codes + 512 * u, src + 512 * u);
+    for (int i = 0; i < kDecStages; ++i) bar_init(full + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  auto fetch = [&](int b, int stage) {
+    const uint8_t* src = codes + (size_t)b * 2 * kQ8Codes;
+    if constexpr (kLong) {
+      if (b < b1 && lane == 0) {
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
+                     :: "r"(full + 8 * stage), "n"(2 * kQ8Codes) : "memory");
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                     :: "r"(ring_s + stage * 2 * kQ8Codes), "l"(src), "n"(2 * kQ8Codes),
+                        "r"(full + 8 * stage) : "memory");
+      }
+    } else {
+      if (b < b1) {
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+          cp_async16(ring_s + stage * 2 * kQ8Codes + 512 * u, src + 16 * lane + 512 * u);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   // the open block's rows go first, to the CTA with the last chunk
   const bool open = chunk == nact - 1 && ntail > 0;
@@ -160,7 +180,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   };
 
   if (open) {                                    // in f32, while the first blocks come in
-    asm volatile("cp.async.wait_group %0;" :: "n"(kDecStages) : "memory");
+    asm volatile("cp.async.wait_group %0;" :: "n"(kLong ? 0 : kDecStages) : "memory");
     __syncthreads();
     const int xr = threadIdx.x >> 3, xh = threadIdx.x & 7;     // a thread per row and head
     if (xr < ntail && xh < group) {
@@ -206,9 +226,11 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     }
   }
 
-  int stage = 0;
+  int stage = 0, phase = 0, given_up = 0;
   for (int b = b0 + warp; b < b1; b += kDecWarps) {
-    asm volatile("cp.async.wait_group %0;" :: "n"(kDecStages - 1) : "memory");
+    // after a wait that ran out nothing is fetched any more; what is under way is waited for
+    if constexpr (kLong) bar_wait_warp(full + 8 * stage, phase, &given_up);
+    else asm volatile("cp.async.wait_group %0;" :: "n"(kDecStages - 1) : "memory");
     const float2 sc = sc_next;
     if (b + kDecWarps < b1) sc_next = __ldg(scales + b + kDecWarps);
     const uint8_t* blk = ring + stage * 2 * kQ8Codes;
@@ -293,9 +315,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
 #pragma unroll
       for (int k = 0; k < 4; ++k) acc[u][k] = fmaf(d[k], sc.y, acc[u][k]);
     }
-    fetch(b + kDecStages * kDecWarps, stage);
+    if (kLong) __syncwarp();
+    if (!given_up) fetch(b + kDecStages * kDecWarps, stage);
     stage = stage + 1 == kDecStages ? 0 : stage + 1;
+    phase ^= stage == 0;
   }
+  if (given_up) l0 = l1 = __int_as_float(0x7fc00000);
 
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
@@ -962,9 +987,9 @@ int dec_launch(const float* q, const KvQ8& c, float* ctx, const float* scale, co
   // As a cluster the chunks are joined through shared memory, for which the two trips to the
   // scratch and the ticket take 2 us. It has eight at most, and as many as let all heads run at
   // once, so that a full cache takes more steps of a block a warp. In microseconds, as a cluster
-  // and not, 8 heads x 4 queries: 300 positions (steps 1, 1) 6.6 : 8.4, 2000 (1, 1) 7.3 : 9.4,
-  // 4225 (3, 1) 8.4 : 9.3, 8000 (4, 2) 9.6 : 10.9, 16000 (8, 4) 13.5 : 13.6, 39999 (20, 9)
-  // 26.8 : 22.7. Only the cache's size is known here, and a cache is full at its end only.
+  // and not, 8 heads x 4 queries: 300 positions (steps 1, 1) 6.6 : 8.2, 2000 (1, 1) 7.1 : 8.6,
+  // 4225 (3, 1) 8.6 : 9.2, 8000 (4, 2) 9.6 : 9.8, 12000 (6, 3) 11.5 : 10.9, 16000 (8, 4)
+  // 13.4 : 11.7. Only the cache's size is known here, and a cache is full at its end only.
   const int blocks = (cap + kQ8Blk - 1) / kQ8Blk;
   auto steps = [&](int chunks) { return ((blocks + chunks - 1) / chunks + kDecWarps - 1) / kDecWarps; };
   bool meet = false;
@@ -973,14 +998,15 @@ int dec_launch(const float* q, const KvQ8& c, float* ctx, const float* scale, co
     rc = cluster_room(k, &room);
     if (rc) return rc;
     if (nkv > room) continue;
-    meet = steps(k) <= steps(nch) + 4;
+    meet = steps(k) <= steps(nch) + 3;
     if (!meet) break;
     nch = k;
   }
+  const bool few = meet || nch == 1;
   unsigned* ticket = static_cast<unsigned*>(scratch);
   float* part = reinterpret_cast<float*>(ticket + kDecTickets);
-  auto* fn = two ? (meet ? k_attn_dec_q8<true, true> : k_attn_dec_q8<true, false>)
-                 : (meet ? k_attn_dec_q8<false, true> : k_attn_dec_q8<false, false>);
+  auto* fn = two ? (few ? k_attn_dec_q8<true, false> : k_attn_dec_q8<true, true>)
+                 : (few ? k_attn_dec_q8<false, false> : k_attn_dec_q8<false, true>);
   rc = smem_attr((const void*)fn, kDecSmem);
   if (rc) return rc;
   cudaLaunchAttribute at{};

@@ -37,7 +37,6 @@
 #include "attn_q8.cuh"
 #include "attn_q8_rows.h"
 #include "hv_internal.h"
-#include "hv_wait.cuh"
 
 namespace hv {
 namespace {
@@ -52,7 +51,6 @@ constexpr uint32_t kTlColO = 256, kTlColQ = 384;   // tensor memory: S twice, O,
 // registers per thread: 128 at launch, then dealt out anew
 constexpr int kTlRegs = 128, kTlRegsRow = 112, kTlRegsSum = 184, kTlRegsConv = 104;
 static_assert(2 * kTlRegsRow + kTlRegsSum + kTlRegsConv <= 4 * kTlRegs, "registers");
-constexpr unsigned long long kTlWaitNs = 2000000000ull;
 
 // kind::f16 with f32 sums, 128 x 128, both operands with the inner dimension contiguous
 constexpr uint32_t kTlDesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
@@ -123,38 +121,9 @@ HV_DEV void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
 }
 HV_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-HV_DEV void bar_init(uint32_t bar, int count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count) : "memory");
-}
 HV_DEV void bar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
 }
-// False when the wait ran out here or elsewhere in the CTA.
-HV_DEV bool bar_wait(uint32_t bar, uint32_t parity, volatile int* given_up) {
-  unsigned long long t0 = 0;
-  for (unsigned n = 1;; ++n) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    if (ok) return true;
-    if ((n & 63) == 0) {
-      if (*given_up) return false;
-      const unsigned long long now = global_ns();
-      if (t0 == 0) t0 = now;
-      else if (now - t0 > kTlWaitNs) { *given_up = 1; return false; }
-    }
-  }
-}
-
-// The same for a whole warp, whose lanes go on or leave together.
-HV_DEV bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* given_up) {
-  const bool ok = bar_wait(bar, parity, given_up);
-  return __all_sync(0xFFFFFFFFu, ok) != 0;
-}
-
 HV_DEV uint64_t pair(float x, float y) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
