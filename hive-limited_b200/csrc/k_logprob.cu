@@ -362,16 +362,21 @@ __global__ void __launch_bounds__(kLpThreads, 2)
 }
 
 // CTAs per row: enough rows fill the SMs with one each; few rows are cut into pieces of whole
-// tiles.
-int lp_pieces(int rows, int n, int* out) {
+// tiles. Without tiles to cut (or tickets) a row is one piece.
+int lp_pieces(int rows, int n, int* out, long long* most = nullptr) {
   int sms = 0;
   const int rc = sm_count(&sms);
   if (rc) return rc;
   const int tiles = (int)(((long long)n + 3 + kLpTile - 1) / kLpTile);
+  const int cut = tiles < kLpPieces ? tiles : kLpPieces;
   int p = 2 * sms / rows;
-  p = p < tiles ? p : tiles;
-  p = p < kLpPieces ? p : kLpPieces;
+  p = p < cut ? p : cut;
   *out = p < 1 || rows > kLpTickets ? 1 : p;
+  // pieces of all rows together, for any number of rows up to `rows`
+  if (most) {
+    const long long all = (long long)rows * cut < 2ll * sms ? (long long)rows * cut : 2ll * sms;
+    *most = all > rows ? all : rows;
+  }
   return HV_OK;
 }
 
@@ -388,11 +393,11 @@ extern "C" int hv_logprob_scratch(int rows, int n, int top, size_t* bytes) {
   HV_REQUIRE(top <= kMaxTop, HV_E_UNSUPPORTED, "hv_logprob_scratch: %d alternatives (at most %d)",
              top, kMaxTop);
   int pieces = 0;
-  const int rc = lp_pieces(rows, n, &pieces);
+  long long most = 0;
+  const int rc = lp_pieces(rows, n, &pieces, &most);
   if (rc) return rc;
-  *bytes = kLpTickets * sizeof(unsigned) +
-           lp_up((size_t)rows * pieces * sizeof(LpSum)) +
-           (size_t)rows * pieces * (top ? kMaxTop : 0) * sizeof(u64);
+  *bytes = kLpTickets * sizeof(unsigned) + lp_up((size_t)most * sizeof(LpSum)) +
+           (size_t)most * (top ? kMaxTop : 0) * sizeof(u64);
   return HV_OK;
 }
 

@@ -368,7 +368,8 @@ int hv_argmax_key_final(uint64_t* keys, int nkeys, int32_t* tok, int32_t* gen,
  * -infinity is a token that cannot occur. A row with a NaN, a +infinity or only -infinity
  * has no distribution: lp, ent and top_lp are NaN, top_id still in np.argmax's order.
  * scratch: hv_logprob_scratch bytes, 16-byte aligned, zeroed once by the caller; every call
- * leaves it ready for the next; calls that may overlap need one each. */
+ * leaves it ready for the next. Those bytes do for any call of up to `rows` rows, n logits and
+ * `top` alternatives. Calls that may overlap need one each. */
 int hv_logprob_scratch(int rows, int n, int top, size_t* bytes);
 int hv_logprob_rows(const float* logits, long long ld, int rows, int n, const int32_t* tok,
                     int top, float* lp, float* ent, int32_t* top_id, float* top_lp,

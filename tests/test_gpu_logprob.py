@@ -184,7 +184,8 @@ def test_engine_score(hv, kv):
         again = e.score(ids)
         assert np.array_equal(bits(again["logprob"]), bits(got["logprob"]))
         assert again["top_ids"].shape == (299, 0)
-        for bad in ([1], [1, -1], [1, cfg.vocab], list(range(322))):
+        for bad in ([1], [1, -1], [1, cfg.vocab], list(range(322)), [1.0, 2.0],
+                    np.array([1, (1 << 32) + 1])):
             with pytest.raises(ValueError):
                 e.score(bad)
         with pytest.raises(ValueError):
@@ -201,6 +202,24 @@ def test_one_scratch_for_calls_of_different_sizes(hv):
         x = g.standard_normal((rows, 30000)).astype(F32)
         tok = g.integers(0, 30000, rows)
         check(call(hv, x, tok, 32, scratch=s), x, tok, 32)
+
+
+def test_scratch_does_for_every_smaller_call(hv):
+    """Fewer rows are cut into more pieces: one scratch, of the largest call, for all."""
+    for n in (1, 4096, 70001, 151936):
+        for top in (0, 5):
+            sizes = [hv.logprob_scratch(r, n, top) for r in range(1, 1400)]
+            assert sizes == sorted(sizes)
+    rows, n, top = 256, 40000, 32
+    need = hv.logprob_scratch(rows, n, top)
+    room = np.full(need + 65536, 0x5A, np.uint8)
+    room[:need] = 0
+    s = Dev(room)
+    x = (np.random.default_rng(31).standard_normal((rows, n)) * 3).astype(F32)
+    for r, t in ((256, 32), (148, 32), (98, 5), (1, 32), (74, 0), (30, 32), (147, 1), (256, 2)):
+        tok = np.arange(r) * 7
+        check(call(hv, x[:r], tok, t, scratch=s), x[:r], tok, t)
+        assert (s.get(np.uint8)[need:] == 0x5A).all(), (r, t)
 
 
 @pytest.mark.parametrize("order", ["up", "down", "saw", "late"])
