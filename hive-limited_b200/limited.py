@@ -601,6 +601,8 @@ class Engine:
                            self.d_pos, ARGMAX_PARTS, s)
 
     def _step_fused(self, flags: int):
+        if self.kv_q8:
+            raise ValueError("the fused step does not run over kv_dtype='q8'")
         hvdrv._call("hv_step_launch", C.byref(self._desc), int(flags),
                     C.c_void_p(self._stream_cur))
 
@@ -618,6 +620,8 @@ class Engine:
         Returns {"total_us", "phases": {name: {"median_us", "max_us"}}, "raw": ns array
         [grid, stride]} where each phase's duration is taken per CTA and summed over the
         layers (median and max over CTAs)."""
+        if self.kv_q8:
+            raise ValueError("the fused step does not run over kv_dtype='q8'")
         c = self.cfg
         stride = 10 + 28 * c.n_layer
         n = self.step_grid * stride
@@ -686,11 +690,13 @@ class Engine:
 
     def step_status(self) -> int:
         """Nonzero if a bounded wait inside the fused step ran out (HV_E_TIMEOUT)."""
-        return self._get_i32(self.d_status)
+        return 0 if self.kv_q8 else self._get_i32(self.d_status)
 
     def reset_step_state(self):
         """Clear the fused step's barrier/ticket/status words after a failed launch."""
         hvdrv.synchronize()
+        if self.kv_q8:
+            return
         hvdrv.memset8(self.d_barrier, 0, 16)
         hvdrv.memset8(self.d_status, 0, 4)
         hvdrv.memset8(self.d_ticket, 0, (2 * self.shard["n_kv"] + 1) * 4)
@@ -1041,14 +1047,15 @@ class Engine:
         goes through the layers and the LM head PREFILL_BATCH tokens at a time, whatever
         `prefill` is; one GPU. Leaves the KV cache holding ids[:-1]."""
         c = self.cfg
-        toks = np.ascontiguousarray(ids, np.int32)
+        toks = np.asarray(ids)
         n = toks.size
         if self.world > 1:
             raise ValueError("score() runs on one GPU (world = 1)")
         if toks.ndim != 1 or n < 2 or n - 1 > c.max_context:
             raise ValueError(f"{n} tokens to score: 2 to {c.max_context + 1}")
-        if toks.min() < 0 or toks.max() >= c.vocab:
+        if toks.dtype.kind not in "iu" or toks.min() < 0 or toks.max() >= c.vocab:
             raise ValueError("a token id outside the vocabulary")
+        toks = np.ascontiguousarray(toks, np.int32)
         if not 0 <= top <= min(32, c.vocab):
             raise ValueError(f"top={top}: 0 to {min(32, c.vocab)} alternatives")
         pf = self._prefill_buffers()

@@ -374,10 +374,11 @@ def test_open_rows_that_are_not_finite_reach_only_who_sees_them(hv):
         assert (not np.isfinite(x[:, 7]).any()) if lost else np.isfinite(x).all(), pos
 
 
-def test_captured_decode_follows_the_device_position(hv):
+@pytest.mark.parametrize("n0,cap", [(30, 200), (1010, 4000), (4000, 20000)])
+def test_captured_decode_follows_the_device_position(hv, n0, cap):
     """Append and attention captured once, replayed while *pos moves over block edges, equal
     to direct calls; two graphs with a scratch each, on two streams."""
-    nkv, group, cap, n0 = 2, 4, 200, 30
+    nkv, group = 2, 4
     nq = nkv * group
     g = np.random.default_rng(14)
     k, v = rows(g, n0 + 40, nkv)
@@ -615,6 +616,10 @@ def test_engine_over_the_8bit_cache(hv, prefill):
         toks, _, _ = a.generate(ids, 40, stop_on_eos=False)
         assert a.generate(ids, 40, stop_on_eos=False, use_graph=True)[0] == toks
         assert a.generate(ids, 40)[0] == toks                  # a shorter cache written over
+        for fused_only in (a.profile_step, lambda: a._step_fused(0)):
+            with pytest.raises(ValueError):
+                fused_only()
+        assert a.step_status() == 0
     finally:
         a.free()
         f.free()
