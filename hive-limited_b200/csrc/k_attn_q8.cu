@@ -29,6 +29,9 @@ namespace {
 // products. Each warp keeps its own running maximum and sums; they meet in shared memory. The
 // chunks of a head meet, added in chunk order, in a cluster's shared memory, or, where a head has
 // more than a cluster's eight (kLong), in the caller's scratch by the last CTA to arrive.
+// 131072 positions of 8 heads x 4 queries (269 MB) take 51 us, 5.3 TB/s, 80% of a plain copy's
+// rate: 60000 and 131072 positions differ by what their bytes take, and 9 us are there whatever
+// the length, the launch, the first blocks' way and the two joins. 4225 take 8.5 us in a graph.
 constexpr int kDecWarps = 8;
 constexpr int kDecStages = 2;
 constexpr int kDecBlocksMin = 8;       // of a chunk, one a warp (1000 positions: 4 6.4 us, 8 6.8, 12 7.7, 16 8.0)
@@ -462,6 +465,8 @@ int dec_chunks(int nkv, int cap, int* out) {
 // Here the rows are the 16-row operand: S = q K^T and ctx += w V, both terms of q (of w) into
 // the same sums. The open block's f32 rows become two binary16 terms as well, so that it is
 // a block like the others with a third product, hi x lo.
+// Bound by latency: 44 tokens of 16 heads (8 kv heads) over 300 positions take 11.8 us in a
+// graph, 8 tokens of 32 heads over 38 positions 10.9.
 constexpr int kRowWarps = 8;
 
 template <int kWM>

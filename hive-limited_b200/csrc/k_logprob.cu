@@ -10,6 +10,11 @@
 // A row with a NaN, a +infinity or nothing above -infinity has no distribution: its log
 // probabilities and entropy are NaN. Tokens order as np.argmax orders them: by value, -0
 // equal to +0, a NaN above all, ties to the lower id.
+//
+// One pass over the logits. 256 rows of 151936 (155 MB) take 42 us, 3.7 TB/s, 56% of a plain
+// copy's rate: bound by instructions (an exponential, four packed operations and two comparisons
+// for each logit) and by 256 CTAs where 296 fit. One row takes 16 us, all of it latency: the first
+// batch's list, two merges of lists and the trip through the scratch between them.
 #include <cfloat>
 
 #include "hv_common.cuh"
