@@ -11,10 +11,15 @@
 // probabilities and entropy are NaN. Tokens order as np.argmax orders them: by value, -0
 // equal to +0, a NaN above all, ties to the lower id.
 //
-// One pass over the logits. 256 rows of 151936 (155 MB) take 42 us, 3.7 TB/s, 56% of a plain
+// One pass over the logits. 256 rows of 151936 (155 MB) take 40 us, 3.9 TB/s, 59% of a plain
 // copy's rate: bound by instructions (an exponential, four packed operations and two comparisons
-// for each logit) and by 256 CTAs where 296 fit. One row takes 16 us, all of it latency: the first
-// batch's list, two merges of lists and the trip through the scratch between them.
+// for each logit) and by 256 CTAs where 296 fit. One row takes 12 us (6 without alternatives), all
+// of it latency: the first batches' list, the trip through the scratch, the merge of 38 lists.
+//
+// Alternatives: a warp keeps its 32 largest, and what is under a bound costs one comparison. The
+// CTA's first logits give the bound (block_first; a list per warp that met afterwards took 14 us
+// for one row and 42 for 256), which the lists' meetings raise while what has been seen grows
+// fourfold.
 #include <cfloat>
 
 #include "hv_common.cuh"
@@ -131,12 +136,18 @@ HV_DEV uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+constexpr int kLpCand = 512;                      // keys that are put in order side by side
+
 struct LpShared {
   u64 lists[kLpWarps][32];
+  u64 cand[kLpCand];
+  u64 best[32];
   LpSum sums[kLpWarps];
   u64 least;
-  unsigned last;
+  unsigned lead[32];             // the first batches' two largest lanes of each warp
+  unsigned count, last;
 };
+static_assert(2 * kLpWarps == 32, "two leading lanes a warp are a warp's lanes");
 
 // The 32 largest of every warp's falling list `v`, falling, in warp 0 (all warps call).
 HV_DEV u64 block_merge(u64 v, LpShared& sh) {
@@ -150,10 +161,74 @@ HV_DEV u64 block_merge(u64 v, LpShared& sh) {
   return v;
 }
 
+// The 32 largest of the `n` keys in sh.cand, falling, in warp 0: a key's place is how many are
+// above it. All warps call, after a barrier.
+HV_DEV u64 block_order(int n, LpShared& sh) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int i = threadIdx.x; i < n; i += kLpThreads) {
+    const u64 k = sh.cand[i];
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) above += sh.cand[j] > k;
+    if (above < 32) sh.best[above] = k;
+  }
+  __syncthreads();
+  return warp == 0 && lane < n ? sh.best[lane] : 0;
+}
+
+// The first batches of all warps, v of ids as in warp_take, those below n. The lanes' two largest
+// of each warp, 32 in all, give a bound that at least `top` logits reach, and
+// few more do: those are put side by side and in order. The list, in warp 0; false where too many
+// reach the bound (equal logits) or there is none.
+HV_DEV bool block_first(const float (&v)[kLpEach], int id, int n, int top, LpShared& sh, u64* list) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float mine = -INFINITY;                               // the lane's largest, if it has any
+  bool any = false;
+#pragma unroll
+  for (int k = 0; k < kLpEach; ++k) {
+    const int i = id + (k & 3) + 128 * (k >> 2);
+    if (i >= 0 && i < n) {
+      mine = any ? max_nan(mine, v[k]) : v[k];
+      any = true;
+    }
+  }
+  const unsigned ord = any ? (unsigned)(lp_key(mine, 0) >> 32) : 0u;
+  const unsigned o0 = __reduce_max_sync(0xFFFFFFFFu, ord);
+  const int l0 = __ffs(__ballot_sync(0xFFFFFFFFu, ord == o0)) - 1;
+  const unsigned o1 = __reduce_max_sync(0xFFFFFFFFu, lane == l0 ? 0u : ord);
+  if (lane < 2) sh.lead[2 * warp + lane] = lane ? o1 : o0;
+  if (threadIdx.x == 0) sh.count = 0;
+  __syncthreads();
+  const unsigned lead = sh.lead[lane];
+  int above = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) above += sh.lead[j] > lead || (sh.lead[j] == lead && j < lane);
+  const unsigned bound =
+      __shfl_sync(0xFFFFFFFFu, lead, __ffs(__ballot_sync(0xFFFFFFFFu, above == top - 1)) - 1);
+  if (bound && o0 >= bound) {
+#pragma unroll
+    for (int k = 0; k < kLpEach; ++k) {
+      const int i = id + (k & 3) + 128 * (k >> 2);
+      const u64 key = i >= 0 && i < n ? lp_key(v[k], i) : 0;
+      const unsigned who = __ballot_sync(0xFFFFFFFFu, (unsigned)(key >> 32) >= bound);
+      if (!who) continue;
+      unsigned at = 0;
+      if (lane == 0) at = atomicAdd(&sh.count, (unsigned)__popc(who));
+      at = __shfl_sync(0xFFFFFFFFu, at, 0) + __popc(who & ((1u << lane) - 1));
+      if ((who >> lane & 1) && at < kLpCand) sh.cand[at] = key;
+    }
+  }
+  __syncthreads();
+  const unsigned count = sh.count;
+  if (!bound || count > kLpCand) return false;
+  *list = block_order(count, sh);
+  return true;
+}
+
 HV_DEV u64 shfl64(u64 v, int src) { return __shfl_sync(0xFFFFFFFFu, v, src); }
 
 // Takes a batch's logits (of ids id + (k & 3) + 128 (k >> 2)) that are above `least` into the
-// warp's falling list of 32; without a bound yet it starts from the lanes' largest.
+// warp's falling list of 32; without a bound it starts from the lanes' largest.
 // Returns the list; the `top`th of it raises `least`.
 HV_DEV u64 warp_take(u64 list, const float (&v)[kLpEach], int id, int n, int top, u64* least) {
   const int lane = threadIdx.x & 31;
@@ -237,8 +312,29 @@ __global__ void __launch_bounds__(kLpThreads, 2)
     }
   };
   const int rounds = (b1 - b0 + kLpWarps - 1) / kLpWarps;
+  const int given = threadIdx.x == 0 ? tok[r] : -1;
+  const float given_x = given >= 0 && given < n ? x[given] : 0.0f;
   int meet = 1;                                          // the round after which lists meet
   if (b0 + warp < b1) load(b0 + warp, next);
+  bool listed = false;                                   // the CTA's list is there already
+  if constexpr (kTop) {
+    const int id = (b0 + warp) * kLpBatch + 4 * lane - off, end = b0 + warp < b1 ? n : 0;
+    if (block_first(next, id, end, top, sh, &list)) {
+      if (rounds == 1) {
+        listed = true;
+        least = ~(u64)0;
+        bar = INFINITY;
+      } else {
+        // the first batches are gone over again, now by a bound that `top` of the CTA's reach
+        if (warp == 0 && lane == top - 1) sh.least = list - 1;
+        __syncthreads();
+        list = 0;
+        least = sh.least;
+        bar = lp_key_value(least);
+        meet = 4;
+      }
+    }
+  }
   for (int i = 0; i < rounds; ++i) {
     const int b = b0 + i * kLpWarps + warp;
     if (b < b1) {
@@ -305,7 +401,7 @@ __global__ void __launch_bounds__(kLpThreads, 2)
     ties += __shfl_xor_sync(0xFFFFFFFFu, ties, o);
   }
   if (lane == 0) sh.sums[warp] = LpSum{m, s + (ties - 1.0f), t};
-  if constexpr (kTop) list = block_merge(list, sh);
+  if (kTop && !listed) list = block_merge(list, sh);
   __syncthreads();
   if (warp > 0 && pieces == 1) return;
   LpSum sum = lane < kLpWarps ? sh.sums[lane] : LpSum{-INFINITY, 0.f, 0.f};
@@ -355,14 +451,12 @@ __global__ void __launch_bounds__(kLpThreads, 2)
   const float nan = __int_as_float(0x7fc00000), ls = log1pf(sum.s);
   const bool fine = fabsf(sum.m) <= FLT_MAX;             // not NaN, +inf, or all -inf
   if (lane == 0) {
-    const int i = tok[r];
-    lp[r] = fine && i >= 0 && i < n ? (x[i] - sum.m) - ls : nan;
+    lp[r] = fine && given >= 0 && given < n ? (given_x - sum.m) - ls : nan;
     ent[r] = fine ? ls + sum.t / (1.0f + sum.s) : nan;
   }
   if (kTop && lane < top) {
-    const int id = (int)~(unsigned)list;
-    top_id[(size_t)r * top + lane] = id;
-    top_lp[(size_t)r * top + lane] = fine ? (x[id] - sum.m) - ls : nan;
+    top_id[(size_t)r * top + lane] = (int)~(unsigned)list;
+    top_lp[(size_t)r * top + lane] = fine ? (lp_key_value(list) - sum.m) - ls : nan;
   }
 }
 

@@ -233,3 +233,30 @@ def test_orders_that_keep_bringing_larger_logits(hv, order):
     if order == "late":
         x[:, :-40] = 0
     check(call(hv, x, [5, n - 1], 32), x, np.array([5, n - 1]), 32)
+
+
+@pytest.mark.parametrize("rows", [2, 300])
+@pytest.mark.parametrize("n", [40, 257, 4096, 4097, 9001, 33000])
+@pytest.mark.parametrize("top", [1, 5, 32])
+def test_alternatives_in_order_whatever_comes_first(hv, n, rows, top):
+    """The order of np.argmax, rows whole and cut: equal logits, few values, NaN and infinities
+    among the first logits or the last, all that counts in one lane."""
+    g = np.random.default_rng(n + top)
+    x = g.standard_normal((rows, n)).astype(F32)
+    x[0] = 1.5
+    x[1] = g.integers(0, 3, n)
+    if rows > 2:
+        x[2, :7] = np.nan
+        x[3, -3:] = np.nan
+        x[4, :4], x[4, -2:] = np.inf, np.nan
+        x[5, 9:] = -np.inf
+        x[6, :-5] = -np.inf
+        x[7, 4:8] += 90
+        x[8, ::512] += 50
+        x[9] = np.linspace(3, -3, n)
+        x[10] = -np.inf
+    ids = call(hv, x, np.zeros(rows, int), top)[2]
+    key = np.where(np.isnan(x), np.inf, np.where(x == 0, 0, x))
+    for r in range(min(rows, 20)):
+        want = np.lexsort((np.arange(n), -key[r], ~np.isnan(x[r])))[:top]
+        assert np.array_equal(ids[r], want), r
