@@ -39,11 +39,13 @@ HV_DEV RowsSpan rows_span(const RowsArgs& a, const KvQ8& c, int kvh, int row0, i
 // row r is added up by CTA r mod nact, and every chunk sends its sums there, 128 floats and
 // (max, sum of weights) of row r to slot [chunk][r / nact] of a buffer that has no other use by
 // then. Two cluster barriers: the first says that the buffers are free (a CTA arrives when it has
-// done with its own), the second that all sums are in them.
+// done with its own), the second that all sums are in them. Every CTA of a cluster takes part in
+// both, whatever it has to do, so that none is gone while another writes to it.
 constexpr int kRowsCluster = 8;
 HV_HD constexpr int rows_land_bytes(int rows) { return (rows + kRowsCluster - 1) * (kHd + 2) * 4; }
 HV_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 HV_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+HV_DEV void cluster_stay() { cluster_arrive(); cluster_wait(); cluster_arrive(); cluster_wait(); }
 
 struct RowsLand {
   uint8_t* at;

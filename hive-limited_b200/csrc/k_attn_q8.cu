@@ -57,6 +57,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   __shared__ unsigned s_last;
   __shared__ unsigned long long s_full[kDecWarps][kDecStages];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
+  constexpr bool kMeet = !kLong;
   const int kvh = blockIdx.y, chunk = blockIdx.x;
   const int pos = pos_p ? *pos_p : pos0, held = q8_held(c, kvh);
   float* out = ctx + (size_t)kvh * group * kHd;
@@ -64,6 +65,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     if (chunk == 0)
       for (int i = threadIdx.x; i < group * kHd; i += blockDim.x)
         out[i] = __int_as_float(0x7fc00000);
+    if (kMeet) cluster_stay();
     return;
   }
   const int closed = held / kQ8Blk;
@@ -71,9 +73,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   const int ntail = max(0, pos + 1 - closed * kQ8Blk);
   int nact = (nb + kDecBlocksMin - 1) / kDecBlocksMin;
   nact = max(1, min(nact, (int)gridDim.x));
-  const bool meet = !kLong && nact > 1;
   if (chunk >= nact) {
-    if (meet) { cluster_arrive(); cluster_wait(); cluster_arrive(); cluster_wait(); }
+    if (kMeet) cluster_stay();
     return;
   }
   const int b0 = (int)((long long)nb * chunk / nact), b1 = (int)((long long)nb * (chunk + 1) / nact);
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  if (meet) cluster_arrive();                            // the open rows' place is free
+  if (kMeet) cluster_arrive();                           // the open rows' place is free
   float* red = reinterpret_cast<float*>(smem);           // [warp][column][kDecStride]
   float M0 = -INFINITY, M1 = -INFINITY;
 #pragma unroll
@@ -364,7 +365,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   float* pml = pacc + 8 * kHd;
   const RowsLand land(smem + kDecRing, group, nact);
   static_assert(rows_land_bytes(8) <= kDecSmem - kDecRing, "room for the chunks' sums");
-  if (meet) cluster_wait();
+  if (kMeet) cluster_wait();
   const int units = group * (kHd / 4);                   // of four outputs, one a thread
   static_assert(8 * (kHd / 4) <= 32 * kDecWarps, "a thread for each");
   if ((int)threadIdx.x < units) {
@@ -385,7 +386,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     }
     if (nact == 1) {
       reinterpret_cast<float4*>(out)[i] = make_float4(A.x / L, A.y / L, A.z / L, A.w / L);
-    } else if (meet) {
+    } else if (kMeet) {
       land.send_sums(chunk, h, d / 4, A);
       if (d == 0) land.send_ml(chunk, h, M, L);
     } else {
@@ -393,9 +394,10 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       if (d == 0) { pml[2 * h] = M; pml[2 * h + 1] = L; }
     }
   }
-  if (meet) {
+  if (kMeet) {
     cluster_arrive();
     cluster_wait();
+    if (nact == 1) return;
     const RowsArgs a{q, ctx, scale, pos, 1, 0, group, 0, true, nullptr};
     land.add_up(a, kvh, 0, group, chunk, warp, kDecWarps, lane, held);
     return;
@@ -493,9 +495,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   const int nrows = a.ntok * a.group, row0 = tile * Cfg::kRows;
   const RowsSpan sp = rows_span(a, c, kvh, row0, Cfg::kRows, Cfg::kShares);
   const int held = sp.held, closed = sp.closed, nb = sp.nb, items = sp.items, nact = sp.nact;
-  const bool meet = kMeet && nact > 1;
   if (chunk >= nact) {
-    if (meet) { cluster_arrive(); cluster_wait(); cluster_arrive(); cluster_wait(); }
+    if (kMeet) cluster_stay();
     return;
   }
   const int b0 = (int)((long long)items * chunk / nact);
@@ -789,7 +790,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   __syncthreads();
   const RowsLand land(smem + Cfg::kSmem - Cfg::kOpen - Cfg::kTail, Cfg::kRows, nact);
   static_assert(rows_land_bytes(Cfg::kRows) <= Cfg::kOpen + Cfg::kTail, "room for the chunks' sums");
-  if (meet) cluster_arrive();
+  if (kMeet) cluster_arrive();
   {
     float M0 = -INFINITY, M1 = -INFINITY;
 #pragma unroll
@@ -810,7 +811,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   const int ntile = gridDim.x / a.chunks;
   const size_t slot = ((size_t)kvh * ntile + tile) * a.chunks;
   float* mine = a.part + (slot + chunk) * rows_part(Cfg::kRows);
-  if (meet) cluster_wait();
+  if (kMeet) cluster_wait();
   __syncthreads();
   for (int i = threadIdx.x; i < Cfg::kRows * (kHd / 4); i += blockDim.x) {
     const int r = i / (kHd / 4), d4 = i % (kHd / 4), gr = row0 + r;     // a warp's row
@@ -832,7 +833,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       const float inv = a.pos0 + gr / a.group >= held ? __int_as_float(0x7fc00000) : 1.0f / L;
       float* o = a.ctx + ((size_t)(gr / a.group) * a.nq + (size_t)kvh * a.group + gr % a.group) * kHd;
       reinterpret_cast<float4*>(o)[d4] = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
-    } else if (meet) {
+    } else if (kMeet) {
       land.send_sums(chunk, r, d4, s);
       if (d4 == 0) land.send_ml(chunk, r, M, L);
     } else {
@@ -840,10 +841,10 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       if (d4 == 0) *reinterpret_cast<float2*>(mine + (size_t)Cfg::kRows * kHd + 2 * r) = make_float2(M, L);
     }
   }
-  if (meet) {
+  if (kMeet) {
     cluster_arrive();
     cluster_wait();
-    land.add_up(a, kvh, row0, Cfg::kRows, chunk, warp, kRowWarps, lane, held);
+    if (nact > 1) land.add_up(a, kvh, row0, Cfg::kRows, chunk, warp, kRowWarps, lane, held);
   }
 }
 

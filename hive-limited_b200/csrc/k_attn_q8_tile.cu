@@ -178,9 +178,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   const int nrows = a.ntok * a.group, row0 = tile * kTlRows;
   const RowsSpan sp = rows_span(a, c, kvh, row0, kTlRows, kTileLeast);
   const int held = sp.held, closed = sp.closed, nb = sp.nb, items = sp.items, nact = sp.nact;
-  const bool meet = kMeet && nact > 1;
   if (chunk >= nact) {
-    if (meet) { cluster_arrive(); cluster_wait(); cluster_arrive(); cluster_wait(); }
+    if (kMeet) cluster_stay();
     return;
   }
   const int b0 = (int)((long long)items * chunk / nact);
@@ -232,13 +231,13 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   // to this chunk's part of the scratch
   auto rows_out = [&] {
     asm volatile("bar.sync 2, 384;" ::: "memory");
-    if (meet) cluster_wait();
+    if (kMeet) cluster_wait();
     float4* part = reinterpret_cast<float4*>(a.part + (slot + chunk) * rows_part(kTlRows));
 #pragma unroll 4
     for (int r = warp; r < kTlRows; r += 12) {
       const float4 x = *reinterpret_cast<const float4*>(lines + (size_t)r * kTlLine + 4 * lane);
       const int gr = row0 + r, tok = gr / a.group;
-      if (meet) {
+      if (kMeet && nact > 1) {
         if (gr < nrows) land.send_sums(chunk, r, lane, x);
       } else if (nact > 1)
         part[r * (kHd / 4) + lane] = x;
@@ -468,7 +467,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     }
     sh.m[w][row] = m;
     sh.l[w][row] = l;
-    if (meet) cluster_arrive();
+    if (kMeet) cluster_arrive();
     asm volatile("bar.sync 1, 384;" ::: "memory");         // with the warps that have the sums
     rows_out();
   } else if (warp < 12) {
@@ -503,7 +502,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
                                 mul2(pair(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), fo2));
       }
     }
-    if (meet) cluster_arrive();
+    if (kMeet) cluster_arrive();
     asm volatile("bar.sync 1, 384;" ::: "memory");
     const float nan = __int_as_float(0x7fc00000);
     const float l0 = sh.l[0][row], l1 = sh.l[1][row];
@@ -522,10 +521,10 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       *reinterpret_cast<float4*>(line + 2 * d) = make_float4(x.x * f, x.y * f, y.x * f, y.y * f);
     }
     float* part = a.part + (slot + chunk) * rows_part(kTlRows);
-    if (nact > 1 && !meet)
+    if (nact > 1 && !kMeet)
       *reinterpret_cast<float2*>(part + kTlRows * kHd + 2 * row) = make_float2(M, L);
     rows_out();
-    if (meet && grow < nrows) land.send_ml(chunk, row, M, L);
+    if (kMeet && nact > 1 && grow < nrows) land.send_ml(chunk, row, M, L);
   } else if (warp < 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsConv));
     // a warp per block of the tile
@@ -747,12 +746,12 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         bar_arrive(bar(sh.full_v[s]));
       }
     }
-    if (meet) { cluster_arrive(); cluster_wait(); }
+    if (kMeet) { cluster_arrive(); cluster_wait(); }
   }
-  if (meet) {
+  if (kMeet) {
     cluster_arrive();
     cluster_wait();
-    land.add_up(a, kvh, row0, kTlRows, chunk, warp, kTlThreads / 32, lane, held);
+    if (nact > 1) land.add_up(a, kvh, row0, kTlRows, chunk, warp, kTlThreads / 32, lane, held);
   }
   __syncwarp();
   fence_before();
