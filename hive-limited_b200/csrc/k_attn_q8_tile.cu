@@ -53,6 +53,8 @@ constexpr int kTlHalf = 128 * 128;              // bytes of 128 rows of 64 halve
 constexpr int kTlTile = 2 * kTlHalf;            // bytes of a 128 x 128 binary16 tile
 constexpr int kTlLine = kHd + 4;               // floats from row to row on their way in and out
 constexpr float kTlLift = 32768.0f;             // 2^15
+constexpr float kTlDrop = 0x1p-20f;             // of sums at the end: the lift, and room for 2^20
+                                                // weights over a scale of 2^-110
 constexpr uint32_t kTlColO = 256, kTlColQ = 384;   // tensor memory: S twice, O, qh, ql
 // registers per thread: 128 at launch, then dealt out anew
 constexpr int kTlRegs = 128, kTlRegsRow = 112, kTlRegsSum = 184, kTlRegsConv = 104;
@@ -518,7 +520,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
 #pragma unroll
     for (int d = 0; d < kHd / 2; d += 2) {
       const float2 x = unpair(acc[d]), y = unpair(acc[d + 1]);
-      *reinterpret_cast<float4*>(line + 2 * d) = make_float4(x.x * f, x.y * f, y.x * f, y.y * f);
+      *reinterpret_cast<float4*>(line + 2 * d) =
+          make_float4(x.x * kTlDrop * f, x.y * kTlDrop * f, y.x * kTlDrop * f, y.y * kTlDrop * f);
     }
     float* part = a.part + (slot + chunk) * rows_part(kTlRows);
     if (nact > 1 && !kMeet)
@@ -641,8 +644,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       asm volatile("bar.sync 4, 128;" ::: "memory");
       lk = q8_lift(sh.open_max[0]);
       // values up to 2^10: their scale is then near that of coded values, which is what a
-      // weight's precision goes by
-      lv = q8_lift(sh.open_max[1]) * 0.0625f;
+      // weight's precision goes by (and never under the least that put_scales lets pass)
+      lv = fminf(q8_lift(sh.open_max[1]) * 0.0625f, 0x1p110f);
     };
     auto none_k = [&](uint8_t* to) {
       const uint32_t y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -681,11 +684,12 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     };
     auto put_scales = [&](int i, float sk, float sv) {
       if (lane == 0) {
-        // a scale under 2^-120 counts as that, so that its reciprocal is a number; a NaN stays
-        sv = sv < 0x1p-120f ? 0x1p-120f : sv;
+        // a scale under 2^-110 counts as that (values up to 10^-31), so that a chunk of such
+        // blocks alone, whose sum of weights goes by its reciprocal, stays in range; a NaN stays
+        sv = sv < 0x1p-110f ? 0x1p-110f : sv;
         sh.sc[i & 3][cw][0] = sk;
         sh.sc[i & 3][cw][1] = log2f(sv);
-        sh.sc[i & 3][cw][2] = sv == sv ? 1.0f / sv : 0.0f;
+        sh.sc[i & 3][cw][2] = sv == sv ? kTlDrop / sv : 0.0f;
       }
     };
     auto scales_of = [&](int i) { return live(i) ? __ldg(scales + b0 + 4 * i + cw) : make_float2(1.f, 1.f); };

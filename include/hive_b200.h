@@ -296,7 +296,9 @@ int hv_kv_read_q8(const void* kv, float* k_out, float* v_out, int pos0, int nkv,
                   int cap, int ntok, void* stream);
 /* Attention over that cache, softmax(scale q k^T) v in f32 precision (not the reference's
  * order of operations: the lane has its own results). Query head h reads kv head h / group,
- * group 1 to 8; q and ctx [ntok][nq][128], 16-byte aligned.
+ * group 1 to 8; q and ctx [ntok][nq][128], 16-byte aligned. The sums run ahead of the quotient
+ * by 2^15 and the number of positions: V to about 10^30 (and from 10^-31 on) keeps f32's
+ * precision.
  *   hv_attn_decode_q8  one query row over positions 0 .. *pos. A *pos that is not held
  *                      leaves NaN in ctx and reads no cache row.            (fda_warp_pos)
  *   hv_attn_rows_q8    row t over positions 0 .. pos0 + t of the cache as it stands: rows of

@@ -516,6 +516,92 @@ def test_long_run_sizes_of_q_and_k(hv, size):
         near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.07, 1e-30, 3.0])
+def test_scales_of_any_sign(hv, scale):
+    """Zero makes all weights equal; below it the smallest products weigh most."""
+    for nkv, group, pos0, ntok in ((2, 4, 70, 1), (2, 4, 70, 5), (8, 8, 30, 220), (1, 1, 500, 40)):
+        nq, n = nkv * group, pos0 + ntok
+        g, ref, kv = filled(hv, 41, nkv, n, n + 9)
+        q = (0.3 * g.standard_normal((ntok, nq, HD))).astype(F32)
+        sc, ctx = Dev(np.array([scale], F32)), Dev(np.zeros((ntok, nq, HD), F32))
+        s = scratch(hv, nq, group, n + 9, ntok)
+        hv.attn_rows_q8(Dev(q), kv, ctx, sc, pos0, nq, HD, group, n + 9, ntok, s)
+        got = ctx.get(F32, (ntok, nq, HD))
+        for t in {0, ntok // 2, ntok - 1}:
+            near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(F32(scale))))
+        hv.attn_decode_q8(Dev(q[-1:]), kv, ctx, sc, i32(n - 1), nq, HD, group, n + 9, s)
+        near(ctx.get(F32, (ntok, nq, HD))[0],
+             *R.attention(q[-1], ref.val, n - 1, group, float(F32(scale))))
+
+
+@pytest.mark.parametrize("ntok", [1, 4, 40])
+@pytest.mark.parametrize("first", [600, 1056])
+@pytest.mark.parametrize("small", [1e-31, 1e-20, 1e20, 1e30])
+def test_values_of_very_different_sizes(hv, ntok, small, first):
+    """The first blocks' V (or all of it) apart from the usual by many orders: their weights
+    count all the same, in whole chunks of them too."""
+    nkv, group, pos0, cap = 8, 8, 1000, 1056
+    nq, n = nkv * group, pos0 + ntok
+    g = np.random.default_rng(43)
+    k, v = rows(g, n, nkv, 0.3)
+    v[:first] *= F32(small)
+    ref = R.Cache(nkv, cap)
+    ref.write(k, v, 0)
+    q = queries(g, ref, ntok, nq)
+    ctx = Dev(np.zeros((ntok, nq, HD), F32))
+    hv.attn_rows_q8(Dev(q), Dev(ref.buffer(0xFF)), ctx, Dev(np.array([SCALE])), pos0, nq, HD,
+                    group, cap, ntok, scratch(hv, nq, group, cap, ntok))
+    got = ctx.get(F32, (ntok, nq, HD))
+    for t in {0, ntok - 1}:
+        near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
+
+
+def test_offsets_past_32_bits(hv):
+    """4.3 GB of codes: the last head's last blocks. What was there before is zeros (K and V
+    values of 0, so weights of exp(0))."""
+    nkv, cap, new = 32, (1 << 19) + 96, 80
+    n0 = cap - new - 7
+    (_, _, at, end), _ = R.parts(nkv, cap)
+    kv = Dev(nbytes=end)
+    nblk = -(-cap // R.BLK)
+    hv.memset8(int(kv), 0x80, nkv * nblk * 2 * 4096)           # codes of 0, scales of 1
+    one = np.ones(nkv * nblk * 2, F32)
+    hv.upload(int(kv) + nkv * nblk * 2 * 4096, one.ctypes.data, one.nbytes)
+    held = np.full(nkv * 2, n0 // 32 * 32, np.int32)           # whole blocks
+    hv.upload(int(kv) + at, held.ctypes.data, held.nbytes)
+    n0 = int(held[0])
+    g = np.random.default_rng(42)
+    k, v = rows(g, new, nkv, 0.1)
+    hv.kv_rows_q8(Dev(k), Dev(v), nkv * HD, kv, n0, nkv, HD, cap, new)
+    ref = R.Cache(nkv, 128)
+    ref.write(k, v, 0)
+    got = read(hv, kv, nkv, cap, n0, new)
+    assert same(got, ref.val[:, :, :new])
+    assert (read(hv, kv, nkv, cap, n0 - 40, 40) == 0).all()
+    val = ref.val[:, :, :new].astype(np.float64)
+    for ntok in (1, 2, 70):                                    # each attention kernel
+        q = (4 * g.standard_normal((ntok, nkv, HD)) * SCALE + k[-1] / 4).astype(F32)
+        ctx = Dev(np.zeros((ntok, nkv, HD), F32))
+        s = scratch(hv, nkv, 1, cap, ntok)
+        pos0 = n0 + new - ntok
+        hv.attn_rows_q8(Dev(q), kv, ctx, Dev(np.array([SCALE])), pos0, nkv, HD, 1, cap, ntok, s)
+        got = ctx.get(F32, (ntok, nkv, HD))
+        for h in (0, 17, nkv - 1):
+            seen = new
+            x = (val[0, h, :seen] @ q[-1, h].astype(np.float64)) * float(SCALE)
+            w = np.exp(x - max(x.max(), 0))
+            total = w.sum() + n0 * np.exp(-max(x.max(), 0))
+            want, size = w @ val[1, h] / total, w @ np.abs(val[1, h]) / total
+            big = (np.abs(val[0, h]) @ np.abs(q[-1, h])).max() * float(SCALE)
+            peak = np.abs(val[1, h]).max()
+            n = n0 + new
+            # the bound of kv_q8_ref.attention; the sum of the weights adds its n terms apart
+            # from the values, whose sum has `new` of them that are not zero
+            tol = (96 * R.U * 2 * big + (n / 8 + 64) * R.U) * size
+            tol += 2.0 ** -32 * n * (w / total).max() * peak
+            near(got[-1, h], want, tol)
+
+
 def test_scratch_does_for_every_shorter_run(hv):
     for nq, group, cap in ((8, 1, 500), (40, 5, 20000), (32, 4, 4096), (64, 8, 40960),
                            (148, 1, 8192), (16, 2, 257), (6, 3, 1 << 20)):
