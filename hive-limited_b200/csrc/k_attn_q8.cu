@@ -477,7 +477,8 @@ struct RowsCfg {
   static constexpr int kRows = 16 * kWM;
   static constexpr int kStages = kShares == 8 ? 2 : 3;
   static constexpr int kRing = kShares * kStages * 2 * kQ8Codes;
-  static constexpr int kMerge = kRowWarps * 16 * (kHd + 4) * 4;
+  static constexpr int kLine = kHd + 8;                    // floats: a fragment's stores meet no bank twice
+  static constexpr int kMerge = kRowWarps * 16 * kLine * 4;
   static constexpr int kTail = 4 * kQ8Codes * 2;          // K hi, K lo, V hi, V lo
   static constexpr int kOpen = 2 * kQ8Codes * 4;          // the open rows in f32
   static constexpr int kSmem = (kRing > kMerge ? kRing : kMerge) + kTail + kOpen;
@@ -493,6 +494,16 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   const int wm = warp % kWM, share = warp / kWM;
   const int kvh = blockIdx.y, tile = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks;
   const int nrows = a.ntok * a.group, row0 = tile * Cfg::kRows;
+  // the queries first, both of a lane's rows: nothing else tells where they are
+  const int r0 = row0 + 16 * wm + gl, r1 = r0 + 8;
+  float4 x[2][8];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = min(half ? r1 : r0, nrows - 1), tok = r / a.group;
+    const float* src = a.q + ((size_t)tok * a.nq + (size_t)kvh * a.group + r - tok * a.group) * kHd;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) x[half][s] = __ldg(reinterpret_cast<const float4*>(src + 4 * t) + 4 * s);
+  }
   const RowsSpan sp = rows_span(a, c, kvh, row0, Cfg::kRows, Cfg::kShares);
   const int held = sp.held, closed = sp.closed, nb = sp.nb, items = sp.items, nact = sp.nact;
   if (chunk >= nact) {
@@ -504,7 +515,6 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   const int c1 = min(b1, nb);                       // blocks b0 .. c1 from codes, then the tail
 
   // this warp's two rows per lane
-  const int r0 = row0 + 16 * wm + gl, r1 = r0 + 8;
   const int lim0 = r0 < nrows ? min(a.pos0 + r0 / a.group, held - 1) : -1;
   const int lim1 = r1 < nrows ? min(a.pos0 + r1 / a.group, held - 1) : -1;
   const int warp_last = min(row0 + 16 * wm + 15, nrows - 1);
@@ -548,17 +558,6 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   float qs0, qs1;
   {
     const float qscale = __ldg(a.scale) * kLog2e;
-    auto row_ptr = [&](int r) {
-      return a.q + (((size_t)(r / a.group)) * a.nq + (size_t)kvh * a.group + r % a.group) * kHd;
-    };
-    float4 x[2][8];                      // both rows' loads under way at once
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int r = half ? r1 : r0;
-      const float4* src = reinterpret_cast<const float4*>(row_ptr(min(r, nrows - 1)) + 4 * t);
-#pragma unroll
-      for (int s = 0; s < 8; ++s) x[half][s] = __ldg(src + 4 * s);
-    }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       float amax = 0.0f;
@@ -799,12 +798,12 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       M1 = fmaxf(M1, s_m[w * kWM + wm][gl + 8]);
     }
     const float a0 = l0 == 0.0f ? 0.0f : ex2(m0 - M0), a1 = l1 == 0.0f ? 0.0f : ex2(m1 - M1);
-    float* red = reinterpret_cast<float*>(smem) + (size_t)warp * 16 * (kHd + 4);
+    float* red = reinterpret_cast<float*>(smem) + (size_t)warp * 16 * Cfg::kLine;
 #pragma unroll
     for (int d = 0; d < 16; ++d) {
-      *reinterpret_cast<float2*>(red + gl * (kHd + 4) + 8 * d + 2 * t) =
+      *reinterpret_cast<float2*>(red + gl * Cfg::kLine + 8 * d + 2 * t) =
           make_float2(acc[d][0] * a0, acc[d][1] * a0);
-      *reinterpret_cast<float2*>(red + (gl + 8) * (kHd + 4) + 8 * d + 2 * t) =
+      *reinterpret_cast<float2*>(red + (gl + 8) * Cfg::kLine + 8 * d + 2 * t) =
           make_float2(acc[d][2] * a1, acc[d][3] * a1);
     }
   }
@@ -813,9 +812,10 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   float* mine = a.part + (slot + chunk) * rows_part(Cfg::kRows);
   if (kMeet) cluster_wait();
   __syncthreads();
-  for (int i = threadIdx.x; i < Cfg::kRows * (kHd / 4); i += blockDim.x) {
-    const int r = i / (kHd / 4), d4 = i % (kHd / 4), gr = row0 + r;     // a warp's row
-    if (gr >= nrows) break;
+#pragma unroll
+  for (int k = 0; k < Cfg::kRows / kRowWarps; ++k) {
+    const int r = warp + kRowWarps * k, d4 = lane, i = r * (kHd / 4) + d4, gr = row0 + r;
+    if (gr >= nrows) continue;
     float M = -INFINITY, L = 0.0f;
 #pragma unroll
     for (int w = 0; w < Cfg::kShares; ++w) M = fmaxf(M, s_m[w * kWM + (r >> 4)][r & 15]);
@@ -824,7 +824,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
     for (int w = 0; w < Cfg::kShares; ++w) {
       const int at = w * kWM + (r >> 4);
       const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem) +
-                                                        ((size_t)at * 16 + (r & 15)) * (kHd + 4) + 4 * d4);
+                                                        ((size_t)at * 16 + (r & 15)) * Cfg::kLine + 4 * d4);
       const float lw = s_l[at][r & 15];
       L += lw == 0.0f ? 0.0f : lw * ex2(s_m[at][r & 15] - M);
       s.x += x.x; s.y += x.y; s.z += x.z; s.w += x.w;
