@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     if (chunk == 0)
       for (int i = threadIdx.x; i < group * kHd; i += blockDim.x)
         out[i] = __int_as_float(0x7fc00000);
-    if (kMeet) cluster_stay();
+    if (kMeet) { cluster_sync(); cluster_sync(); }
     return;
   }
   const int closed = held / kQ8Blk;
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   int nact = (nb + kDecBlocksMin - 1) / kDecBlocksMin;
   nact = max(1, min(nact, (int)gridDim.x));
   if (chunk >= nact) {
-    if (kMeet) cluster_stay();
+    if (kMeet) { cluster_sync(); cluster_sync(); }
     return;
   }
   const int b0 = (int)((long long)nb * chunk / nact), b1 = (int)((long long)nb * (chunk + 1) / nact);
@@ -339,7 +339,6 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  if (kMeet) cluster_arrive();                           // the open rows' place is free
   float* red = reinterpret_cast<float*>(smem);           // [warp][column][kDecStride]
   float M0 = -INFINITY, M1 = -INFINITY;
 #pragma unroll
@@ -363,9 +362,8 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   const size_t slot = (size_t)kvh * gridDim.x + chunk;
   float* pacc = part + slot * kDecPart;
   float* pml = pacc + 8 * kHd;
-  const RowsLand land(smem + kDecRing, group, nact);
-  static_assert(rows_land_bytes(8) <= kDecSmem - kDecRing, "room for the chunks' sums");
-  if (kMeet) cluster_wait();
+  float* sums = reinterpret_cast<float*>(smem + kDecRing);   // where the open rows were
+  float* sums_ml = sums + 8 * kHd;
   const int units = group * (kHd / 4);                   // of four outputs, one a thread
   static_assert(8 * (kHd / 4) <= 32 * kDecWarps, "a thread for each");
   if ((int)threadIdx.x < units) {
@@ -387,19 +385,20 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     if (nact == 1) {
       reinterpret_cast<float4*>(out)[i] = make_float4(A.x / L, A.y / L, A.z / L, A.w / L);
     } else if (kMeet) {
-      land.send_sums(chunk, h, d / 4, A);
-      if (d == 0) land.send_ml(chunk, h, M, L);
+      reinterpret_cast<float4*>(sums)[i] = A;
+      if (d == 0) { sums_ml[2 * h] = M; sums_ml[2 * h + 1] = L; }
     } else {
       reinterpret_cast<float4*>(pacc)[i] = A;
       if (d == 0) { pml[2 * h] = M; pml[2 * h + 1] = L; }
     }
   }
   if (kMeet) {
-    cluster_arrive();
-    cluster_wait();
-    if (nact == 1) return;
-    const RowsArgs a{q, ctx, scale, pos, 1, 0, group, 0, true, nullptr};
-    land.add_up(a, kvh, 0, group, chunk, warp, kDecWarps, lane, held);
+    cluster_sync();
+    if (nact > 1) {
+      const RowsArgs a{q, ctx, scale, pos, 1, 0, group, 0, true, nullptr};
+      cluster_add_up(a, sums, kHd, sums_ml, nact, kvh, 0, group, chunk, warp, kDecWarps, held);
+    }
+    cluster_sync();
     return;
   }
   if (nact == 1) return;
@@ -507,7 +506,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   const RowsSpan sp = rows_span(a, c, kvh, row0, Cfg::kRows, Cfg::kShares);
   const int held = sp.held, closed = sp.closed, nb = sp.nb, items = sp.items, nact = sp.nact;
   if (chunk >= nact) {
-    if (kMeet) cluster_stay();
+    if (kMeet) { cluster_sync(); cluster_sync(); }
     return;
   }
   const int b0 = (int)((long long)items * chunk / nact);
@@ -787,9 +786,9 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
-  const RowsLand land(smem + Cfg::kSmem - Cfg::kOpen - Cfg::kTail, Cfg::kRows, nact);
-  static_assert(rows_land_bytes(Cfg::kRows) <= Cfg::kOpen + Cfg::kTail, "room for the chunks' sums");
-  if (kMeet) cluster_arrive();
+  float* sums = reinterpret_cast<float*>(smem + Cfg::kSmem - Cfg::kOpen - Cfg::kTail);
+  float* sums_ml = sums + Cfg::kRows * kHd;
+  static_assert(Cfg::kRows * (kHd + 2) * 4 <= Cfg::kOpen + Cfg::kTail, "room for the rows' sums");
   {
     float M0 = -INFINITY, M1 = -INFINITY;
 #pragma unroll
@@ -810,7 +809,6 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   const int ntile = gridDim.x / a.chunks;
   const size_t slot = ((size_t)kvh * ntile + tile) * a.chunks;
   float* mine = a.part + (slot + chunk) * rows_part(Cfg::kRows);
-  if (kMeet) cluster_wait();
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < Cfg::kRows / kRowWarps; ++k) {
@@ -834,17 +832,18 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       float* o = a.ctx + ((size_t)(gr / a.group) * a.nq + (size_t)kvh * a.group + gr % a.group) * kHd;
       reinterpret_cast<float4*>(o)[d4] = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
     } else if (kMeet) {
-      land.send_sums(chunk, r, d4, s);
-      if (d4 == 0) land.send_ml(chunk, r, M, L);
+      reinterpret_cast<float4*>(sums)[i] = s;
+      if (d4 == 0) *reinterpret_cast<float2*>(sums_ml + 2 * r) = make_float2(M, L);
     } else {
       reinterpret_cast<float4*>(mine)[i] = s;
       if (d4 == 0) *reinterpret_cast<float2*>(mine + (size_t)Cfg::kRows * kHd + 2 * r) = make_float2(M, L);
     }
   }
   if (kMeet) {
-    cluster_arrive();
-    cluster_wait();
-    if (nact > 1) land.add_up(a, kvh, row0, Cfg::kRows, chunk, warp, kRowWarps, lane, held);
+    cluster_sync();
+    if (nact > 1)
+      cluster_add_up(a, sums, kHd, sums_ml, nact, kvh, row0, Cfg::kRows, chunk, warp, kRowWarps, held);
+    cluster_sync();
   }
 }
 

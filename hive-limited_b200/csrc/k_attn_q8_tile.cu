@@ -164,6 +164,7 @@ struct TlShared {
   float sc[4][4][4];             // of the last four tiles' blocks: s_k, log2 s_v, 1 / s_v
   float top[4][kTlRows];         // of the last four tiles: what their weights are relative to
   float m[2][kTlRows], l[2][kTlRows];
+  float ml[kTlRows][2];          // of the rows' sums, where another CTA of the cluster adds them up
   uint32_t tmem;
   float open_max[2];             // of the open rows: largest |K|, |V|
   int bad;                       // first open row with a value that is not finite
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   const RowsSpan sp = rows_span(a, c, kvh, row0, kTlRows, kTileLeast);
   const int held = sp.held, closed = sp.closed, nb = sp.nb, items = sp.items, nact = sp.nact;
   if (chunk >= nact) {
-    if (kMeet) cluster_stay();
+    if (kMeet) { cluster_sync(); cluster_sync(); }
     return;
   }
   const int b0 = (int)((long long)items * chunk / nact);
@@ -227,21 +228,17 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   const size_t slot = ((size_t)kvh * ntile + tile) * a.chunks;
   float* lines = reinterpret_cast<float*>(smem + 4 * kTlTile);    // [row][kTlLine]
   auto rows_sync = [] { asm volatile("bar.sync 3, 256;" ::: "memory"); };
-  const RowsLand land(smem, kTlRows, nact);       // over the tiles, once they have been multiplied
-  static_assert(rows_land_bytes(kTlRows) <= 4 * kTlTile, "room for the chunks' sums");
-  // the rows' sums, once they stand in `lines`: to ctx, to the cluster's CTA that adds them up, or
-  // to this chunk's part of the scratch
+  // the rows' sums, once they stand in `lines`: to ctx, or to this chunk's part of the scratch (a
+  // cluster's stay where they are)
   auto rows_out = [&] {
+    if (kMeet && nact > 1) return;
     asm volatile("bar.sync 2, 384;" ::: "memory");
-    if (kMeet) cluster_wait();
     float4* part = reinterpret_cast<float4*>(a.part + (slot + chunk) * rows_part(kTlRows));
 #pragma unroll 4
     for (int r = warp; r < kTlRows; r += 12) {
       const float4 x = *reinterpret_cast<const float4*>(lines + (size_t)r * kTlLine + 4 * lane);
       const int gr = row0 + r, tok = gr / a.group;
-      if (kMeet && nact > 1) {
-        if (gr < nrows) land.send_sums(chunk, r, lane, x);
-      } else if (nact > 1)
+      if (nact > 1)
         part[r * (kHd / 4) + lane] = x;
       else if (gr < nrows)
         reinterpret_cast<float4*>(a.ctx + ((size_t)tok * a.nq + (size_t)kvh * a.group + gr - tok * a.group) * kHd)[lane] = x;
@@ -469,9 +466,9 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     }
     sh.m[w][row] = m;
     sh.l[w][row] = l;
-    if (kMeet) cluster_arrive();
     asm volatile("bar.sync 1, 384;" ::: "memory");         // with the warps that have the sums
     rows_out();
+    if (kMeet) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kTlRegs));
   } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kTlRegsSum));
     uint64_t acc[kHd / 2];
@@ -504,7 +501,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
                                 mul2(pair(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), fo2));
       }
     }
-    if (kMeet) cluster_arrive();
     asm volatile("bar.sync 1, 384;" ::: "memory");
     const float nan = __int_as_float(0x7fc00000);
     const float l0 = sh.l[0][row], l1 = sh.l[1][row];
@@ -524,10 +520,10 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
           make_float4(x.x * kTlDrop * f, x.y * kTlDrop * f, y.x * kTlDrop * f, y.y * kTlDrop * f);
     }
     float* part = a.part + (slot + chunk) * rows_part(kTlRows);
-    if (nact > 1 && !kMeet)
-      *reinterpret_cast<float2*>(part + kTlRows * kHd + 2 * row) = make_float2(M, L);
+    if (nact > 1)
+      *reinterpret_cast<float2*>(kMeet ? sh.ml[row] : part + kTlRows * kHd + 2 * row) = make_float2(M, L);
     rows_out();
-    if (kMeet && nact > 1 && grow < nrows) land.send_ml(chunk, row, M, L);
+    if (kMeet) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegs));
   } else if (warp < 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsConv));
     // a warp per block of the tile
@@ -750,12 +746,13 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         bar_arrive(bar(sh.full_v[s]));
       }
     }
-    if (kMeet) { cluster_arrive(); cluster_wait(); }
+    if (kMeet) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kTlRegs));
   }
-  if (kMeet) {
-    cluster_arrive();
-    cluster_wait();
-    if (nact > 1) land.add_up(a, kvh, row0, kTlRows, chunk, warp, kTlThreads / 32, lane, held);
+  if (kMeet) {                                    // all roles have the launch's registers again
+    cluster_sync();
+    if (nact > 1)
+      cluster_add_up(a, lines, kTlLine, sh.ml[0], nact, kvh, row0, kTlRows, chunk, warp, kTlThreads / 32, held);
+    cluster_sync();
   }
   __syncwarp();
   fence_before();
