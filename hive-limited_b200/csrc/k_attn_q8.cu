@@ -31,7 +31,7 @@ namespace {
 // more than a cluster's eight (kLong), in the caller's scratch by the last CTA to arrive.
 // 131072 positions of 8 heads x 4 queries (269 MB) take 51 us, 5.3 TB/s, 80% of a plain copy's
 // rate: 60000 and 131072 positions differ by what their bytes take, and 9 us are there whatever
-// the length, the launch, the first blocks' way and the two joins. 4225 take 8.5 us in a graph.
+// the length, the launch, the first blocks' way and the two joins. 4225 take 8.4 us in a graph.
 constexpr int kDecWarps = 8;
 constexpr int kDecStages = 2;
 constexpr int kDecBlocksMin = 8;       // of a chunk, one a warp (1000 positions: 4 6.4 us, 8 6.8, 12 7.7, 16 8.0)
@@ -466,8 +466,8 @@ int dec_chunks(int nkv, int cap, int* out) {
 // Here the rows are the 16-row operand: S = q K^T and ctx += w V, both terms of q (of w) into
 // the same sums. The open block's f32 rows become two binary16 terms as well, so that it is
 // a block like the others with a third product, hi x lo.
-// Bound by latency: 44 tokens of 16 heads (8 kv heads) over 300 positions take 11.8 us in a
-// graph, 8 tokens of 32 heads over 38 positions 10.9.
+// Bound by latency: 44 tokens of 16 heads (8 kv heads) over 300 positions take 11.6 us in a
+// graph, 8 tokens of 32 heads over 38 positions 10.7.
 constexpr int kRowWarps = 8;
 
 template <int kWM>
@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   }
 
   // the shares meet: all of a row's sums in shared memory, then four outputs a thread
-  static_assert(Cfg::kShares > 1, "more rows are the tile kernel's");
+  static_assert(Cfg::kShares > 1, "a row group has two warps at the least");
   if (t == 0) {
     s_m[warp][gl] = m0; s_m[warp][gl + 8] = m1;
     s_l[warp][gl] = l0; s_l[warp][gl + 8] = l1;
@@ -892,8 +892,8 @@ __global__ void __launch_bounds__(256) k_rows_join_q8(RowsArgs a, KvQ8 c, int ro
 // Rows per CTA and chunks per row tile of a run. The tile kernel (k_attn_q8_tile.cu) pays for
 // filling its tensor memory, its shared memory and a pipeline of five roles, so it takes runs of
 // more than 64 rows a head that have 2^21 (row, position) pairs or more. Tiles of 64 rows here
-// against it, in microseconds, on either side of that: 0.5 M pairs (8 heads x 64 rows, 200
-// positions x 4) 16.0 : 19.5, 1.0 M 17.2 : 22.7, 1.9 M 26.7 : 29.0, 1.9 M 22.4 : 21.1,
+// against it, in microseconds, on either side of that: 0.5 M pairs (8 heads x 256 rows over 264
+// positions) 16.0 : 19.5, 1.0 M 17.2 : 22.7, 1.9 M 26.7 : 29.0, 1.9 M 22.4 : 21.1,
 // 2.2 M 28.1 : 27.3, 4.2 M 24.7 : 20.9, 8.3 M 44.1 : 22.7, 16 M 71.8 : 32.6.
 // Up to 64 rows fill at most half of the 128 that a product of the tile kernel has.
 struct RowsPlan {

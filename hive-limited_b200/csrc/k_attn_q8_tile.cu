@@ -36,8 +36,8 @@
 // Every wait is bounded: one that runs out ends the CTA, whose rows are then NaN.
 //
 // Bound by the tensor cores and by what feeds them: with two terms on one side of each product,
-// 256 tokens of 64 heads over 16384 positions take 265 us and 256 of 32 heads over 4096 45 us,
-// 1.03 and 0.74 PFLOP/s of issued products, 62% and 45% of a large library product's rate. A
+// 256 tokens of 64 heads over 16384 positions take 268 us and 256 of 32 heads over 4096 44 us,
+// 1.01 and 0.76 PFLOP/s of issued products, 61% and 46% of a large library product's rate. A
 // tile's weights (two exponent passes over 128 columns a thread) take about as long as its
 // products; two lanes of work hide the one behind the other, but not the ends of a chunk.
 #include "attn_q8.cuh"
