@@ -895,7 +895,10 @@ __global__ void __launch_bounds__(256) k_rows_join_q8(RowsArgs a, KvQ8 c, int ro
 // against it, in microseconds, on either side of that: 0.5 M pairs (8 heads x 256 rows over 264
 // positions) 16.0 : 19.5, 1.0 M 17.2 : 22.7, 1.9 M 26.7 : 29.0, 1.9 M 22.4 : 21.1,
 // 2.2 M 28.1 : 27.3, 4.2 M 24.7 : 20.9, 8.3 M 44.1 : 22.7, 16 M 71.8 : 32.6.
-// Up to 64 rows fill at most half of the 128 that a product of the tile kernel has.
+// Up to 64 rows fill at most half of the 128 that a product of the tile kernel has; they take the
+// fewest of 16, 32 or 64 that hold them, whose warps then share the positions: 16 rows in tiles of
+// 16, 32 and 64 over 500 positions 12.7, 12.2, 11.9, over 2000 13.1, 14.4, 18.0, over 16000 23.5,
+// 29.1, 41.4; 32 rows in 32 and 64 over 500 13.5, 12.9, over 2000 15.5, 18.6, over 16000 30.8, 42.6.
 struct RowsPlan {
   int rows, tiles, chunks;
   bool cluster;
