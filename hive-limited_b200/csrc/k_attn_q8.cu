@@ -284,14 +284,18 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       y1 = fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, o));
     }
     raise(y0, y1);
-    // weights as 2^15 times what they are to the maximum's, so that the lo terms of small
-    // ones stay above binary16's smallest: a weight is exact to 2^-40 of the largest
+    // Weights as 2^15 times what they are to the block's largest, so that the lo terms of small
+    // ones stay above binary16's smallest: a weight is exact to 2^-40 of its block's largest, and
+    // a block that is hardly attended to counts in full where its values are large.
+    const float g0 = y0 == -INFINITY ? 0.0f : ex2(y0 - m0), g1 = y1 == -INFINITY ? 0.0f : ex2(y1 - m1);
+    if (y0 == -INFINITY) y0 = 0.0f;
+    if (y1 == -INFINITY) y1 = 0.0f;
     uint32_t wh[4], wl[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float p0 = ex2(x0[j] - m0) * 32768.0f, p1 = ex2(x1[j] - m1) * 32768.0f;
-      l0 += p0;
-      l1 += p1;
+      const float p0 = ex2(x0[j] - y0) * 32768.0f, p1 = ex2(x1[j] - y1) * 32768.0f;
+      l0 = fmaf(p0, g0, l0);
+      l1 = fmaf(p1, g1, l1);
       uint32_t hi, lo;
       split_half2(p0, p1, &hi, &lo);
       if (kTwo) {
@@ -301,6 +305,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
         wh[j] = transpose_8x8(t < 2 ? hi : lo);
       }
     }
+    const float v0 = sc.y * g0, v1 = sc.y * g1;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
       const uint4 v = *reinterpret_cast<const uint4*>(blk + kQ8Codes + 512 * u);
@@ -317,7 +322,7 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
         mma_f16(d, e, wl[2], wl[3]);
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k) acc[u][k] = fmaf(d[k], sc.y, acc[u][k]);
+      for (int k = 0; k < 4; ++k) acc[u][k] = fmaf(d[k], k & 1 ? v1 : v0, acc[u][k]);
     }
     if (kLong) __syncwarp();
     if (!given_up) fetch(b + kDecStages * kDecWarps, stage);
@@ -583,8 +588,10 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
 
   // scores of block b in s (position 32 b + 8 j + 2 t + e: s[j][e] of row r0, s[j][2 + e] of
   // r1), already sums of products; f0, f1 make them exponents of 2. Leaves the weights as A
-  // fragments of the second product.
+  // fragments of the second product: 2^15 times what they are to the block's largest, which is
+  // g0 (g1) of the row's.
   uint32_t wh[2][4], wl[2][4];
+  float g0, g1;
   auto weights = [&](int b, float (&s)[4][4], float f0, float f1) {
     const bool cut = 32 * b + 31 > warp_low;
     float y0 = -INFINITY, y1 = -INFINITY;
@@ -605,27 +612,31 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
     }
     y0 = fmaxf(y0, __shfl_xor_sync(0xFFFFFFFFu, y0, 1));
     y1 = fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, 1));
-    y0 = fmaxf(m0, fmaxf(y0, __shfl_xor_sync(0xFFFFFFFFu, y0, 2)));
-    y1 = fmaxf(m1, fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, 2)));
+    y0 = fmaxf(y0, __shfl_xor_sync(0xFFFFFFFFu, y0, 2));
+    y1 = fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, 2));
     if (__any_sync(0xFFFFFFFFu, y0 > m0 || y1 > m1)) {
-      const float a0 = m0 == -INFINITY ? 0.0f : ex2(m0 - y0);
-      const float a1 = m1 == -INFINITY ? 0.0f : ex2(m1 - y1);
-      m0 = y0; m1 = y1;
+      const float n0 = fmaxf(m0, y0), n1 = fmaxf(m1, y1);
+      const float a0 = m0 == -INFINITY ? 0.0f : ex2(m0 - n0);
+      const float a1 = m1 == -INFINITY ? 0.0f : ex2(m1 - n1);
+      m0 = n0; m1 = n1;
       l0 *= a0; l1 *= a1;
 #pragma unroll
       for (int d = 0; d < 16; ++d) { acc[d][0] *= a0; acc[d][1] *= a0; acc[d][2] *= a1; acc[d][3] *= a1; }
     }
-    // a row that sees none of the positions so far keeps m = -inf and weights of 0
-    const float n0 = m0 == -INFINITY ? 0.0f : m0, n1 = m1 == -INFINITY ? 0.0f : m1;
+    // a row that sees none of the block's positions has y = -inf and weights of 0
+    g0 = y0 == -INFINITY ? 0.0f : ex2(y0 - m0);
+    g1 = y1 == -INFINITY ? 0.0f : ex2(y1 - m1);
+    if (y0 == -INFINITY) y0 = 0.0f;
+    if (y1 == -INFINITY) y1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float p[4];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        p[e] = ex2(s[j][e] - n0) * 32768.0f;
-        p[2 + e] = ex2(s[j][2 + e] - n1) * 32768.0f;
-        l0 += p[e];
-        l1 += p[2 + e];
+        p[e] = ex2(s[j][e] - y0) * 32768.0f;
+        p[2 + e] = ex2(s[j][2 + e] - y1) * 32768.0f;
+        l0 = fmaf(p[e], g0, l0);
+        l1 = fmaf(p[2 + e], g1, l1);
       }
       // A fragment: (row g, k 2t), (row g + 8, k 2t), (row g, k 2t + 8), (row g + 8, k 2t + 8)
       split_half2(p[0], p[1], &wh[j >> 1][2 * (j & 1)], &wl[j >> 1][2 * (j & 1)]);
@@ -698,7 +709,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
         }
       }
       weights(closed, s, qs0 / lk, qs1 / lk);
-      const float f = 1.0f / lv;
+      const float f0 = g0 / lv, f1 = g1 / lv;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
 #pragma unroll
@@ -712,7 +723,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
             mma_f16(d, wh[k], vl.x, vl.y);
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[2 * u + h][i] = fmaf(d[i], f, acc[2 * u + h][i]);
+          for (int i = 0; i < 4; ++i)
+            acc[2 * u + h][i] = fmaf(d[i], i < 2 ? f0 : f1, acc[2 * u + h][i]);
         }
       }
       if (lim0 >= closed * kQ8Blk + s_bad) l0 = __int_as_float(0x7fc00000);
@@ -746,7 +758,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       }
       weights(b, s, sc.x * qs0, sc.x * qs1);
       // a row that sees nothing of the block takes nothing from it, whatever its scale
-      const float f0 = 32 * b <= lim0 ? sc.y : 0.0f, f1 = 32 * b <= lim1 ? sc.y : 0.0f;
+      const float f0 = 32 * b <= lim0 ? sc.y * g0 : 0.0f, f1 = 32 * b <= lim1 ? sc.y * g1 : 0.0f;
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const uint4 x = *reinterpret_cast<const uint4*>(blk + kQ8Codes + 512 * u);

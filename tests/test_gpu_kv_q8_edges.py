@@ -1,0 +1,52 @@
+"""Attention over the 8-bit KV cache where blocks, or rows of the open block, differ from their
+neighbours by many orders: each kernel (one token, few rows, long runs) against the 64-bit model
+and bound of kv_q8_ref.py."""
+import numpy as np
+import pytest
+
+import kv_q8_ref as R
+from gpu_util import Dev
+from test_gpu_kv_q8 import SCALE, i32, near, queries, rows, scratch
+
+pytestmark = pytest.mark.gpu
+F32 = np.float32
+HD = 128
+
+# (kv heads, group, pos0, ntok): long runs as one chunk, as a cluster and as chunks of a second
+# launch; few rows whole and cut; one token
+LONG = [(8, 8, 30, 220), (2, 5, 4000, 71), (1, 1, 15001, 200)]
+FEW = [(2, 2, 210, 40), (8, 4, 1000, 8), (1, 4, 246, 4)]
+ONE = [(2, 4, 249, 1), (8, 2, 2000, 1)]
+
+
+def run(hv, ref, q, pos0, group):
+    """The run q [ntok, nq, 128] at pos0 over the model's contents, other bytes 0xFF."""
+    ntok, nq = q.shape[:2]
+    ctx = Dev(np.zeros(q.shape, F32))
+    hv.attn_rows_q8(Dev(q), Dev(ref.buffer(0xFF)), ctx, Dev(np.array([SCALE])), pos0, nq, HD,
+                    group, ref.cap, ntok, scratch(hv, nq, group, ref.cap, ntok))
+    return ctx.get(F32, q.shape)
+
+
+def some(ntok, *more):
+    return sorted({0, 1, ntok // 3, ntok // 2, ntok - 2, ntok - 1, *more} & set(range(ntok)))
+
+
+@pytest.mark.parametrize("nkv,group,pos0,ntok", FEW + ONE)
+def test_blocks_of_values_further_apart_than_an_exponent(hv, nkv, group, pos0, ntok):
+    """V of 1e20 beside V of 1e-20, in one chunk and in different ones: the small values add next
+    to nothing, but their weights count."""
+    n = pos0 + ntok
+    for large in (lambda p: p // 32 % 2 == 0, lambda p: p < n // 2, lambda p: p >= n // 2,
+                  lambda p: p // 32 == 1, lambda p: p >= n // 32 * 32):
+        g = np.random.default_rng(52)
+        k, v = rows(g, n, nkv, 0.3)
+        big = large(np.arange(n))
+        v *= np.where(big, 1e20, 1e-20).astype(F32)[:, None, None]
+        ref = R.Cache(nkv, n + 9)
+        ref.write(k, v, 0)
+        q = queries(g, ref, ntok, nkv * group)
+        q[:, 0] = 0                                            # equal weights
+        got = run(hv, ref, q, pos0, group)
+        for t in some(ntok):
+            near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
