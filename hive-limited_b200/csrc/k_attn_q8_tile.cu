@@ -29,7 +29,11 @@
 // memory: a weight enters as w s_v, that is 2^(x + log2 s_v), and the maximum that the row
 // keeps is that of these products, so that a block with a large scale that the row hardly
 // attends to does not cost the others precision; the sum of the weights adds w s_v / s_v.
-// Weights stand as 2^15 times themselves, exact to 2^-40 of the row's largest.
+// Weights stand as 2^15 times themselves, exact to 2^-40 of the row's largest w s_v. Where a block's
+// largest is under 2^-64 of that, its weights would be lost to the sum too: they are added up apart,
+// without the scale, by a maximum of their own, and leave the tile's scores. Only a chunk whose
+// scales are 2^30 apart looks for them. At its end all goes by one power of two of the sum of the
+// weights.
 // The open block's f32 rows are two binary16 terms: after the tile's products with the first
 // term, the same buffer holds the second one (zero elsewhere) for one product more.
 //
@@ -53,8 +57,11 @@ constexpr int kTlHalf = 128 * 128;              // bytes of 128 rows of 64 halve
 constexpr int kTlTile = 2 * kTlHalf;            // bytes of a 128 x 128 binary16 tile
 constexpr int kTlLine = kHd + 4;               // floats from row to row on their way in and out
 constexpr float kTlLift = 32768.0f;             // 2^15
-constexpr float kTlDrop = 0x1p-20f;             // of sums at the end: the lift, and room for 2^20
-                                                // weights over a scale of 2^-110
+constexpr float kTlDrop = 0x1p-20f;             // of the sum of weights: room for 2^20 of them over
+                                                // a scale of 2^-110
+constexpr float kTlApart = -64.0f;              // log2 of a block's largest w s_v over the row's
+constexpr float kTlFar = 30.0f;                 // exponents between scales: so that without `far` all
+                                                // weights of note are within kTlApart
 constexpr uint32_t kTlColO = 256, kTlColQ = 384;   // tensor memory: S twice, O, qh, ql
 // registers per thread: 128 at launch, then dealt out anew
 constexpr int kTlRegs = 128, kTlRegsRow = 112, kTlRegsSum = 184, kTlRegsConv = 104;
@@ -121,6 +128,17 @@ HV_DEV void tmem_wait(uint32_t (&v)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : HV_P4(v, 0), HV_P4(v, 4), HV_P4(v, 8), HV_P4(v, 12) :: "memory");
 }
+HV_DEV void tmem_ld8(uint32_t at, uint32_t (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : HV_R4(v, 0), HV_R4(v, 4) : "r"(at) : "memory");
+}
+HV_DEV void tmem_wait(uint32_t (&v)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : HV_P4(v, 0), HV_P4(v, 4) :: "memory");
+}
+HV_DEV void tmem_st8(uint32_t at, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               :: "r"(at), HV_W4(v, 0), HV_W4(v, 4) : "memory");
+}
 HV_DEV void tmem_st16(uint32_t at, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -164,11 +182,13 @@ struct TlShared {
   float sc[4][4][4];             // of the last four tiles' blocks: s_k, log2 s_v, 1 / s_v
   float top[4][kTlRows];         // of the last four tiles: what their weights are relative to
   float m[2][kTlRows], l[2][kTlRows];
+  float n[2][kTlRows], k[2][kTlRows];     // of the weights apart: maximum, sum
   float ml[kTlRows][2];          // of the rows' sums, where another CTA of the cluster adds them up
   uint32_t tmem;
   float open_max[2];             // of the open rows: largest |K|, |V|
   int bad;                       // first open row with a value that is not finite
   int given_up;
+  int far;                       // scales of V too far apart for one sum of weights
 };
 constexpr int kTlSmem = 4 * kTlTile + kTlRows * kTlLine * 4 + (int)sizeof(TlShared);   // K, V twice
 
@@ -210,6 +230,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     bar_init(bar(sh.drain[1]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.bad = kQ8Blk;
+    sh.far = 0;
     sh.open_max[0] = sh.open_max[1] = 0.0f;
     sh.given_up = (sm & 1023) != 0;               // the swizzle goes by addresses
   }
@@ -246,6 +267,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
   };
   if (warp < 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegsRow));
+    auto exponent = [](float x) { return (int)(__float_as_uint(x) >> 23) - 127; };
+    int first_e = 0;
     // The queries in two terms, a row per thread (whole lines at a time through shared memory):
     // the first ones from warps 0-3, the second from 4-7. They take the scale's sign, so that
     // the largest sum of products is the largest exponent.
@@ -259,10 +282,17 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
                      :: "r"(to + r * kTlLine * 4), "l"(src) : "memory");
       }
+      // meanwhile: are there scales of V far from the chunk's first?
+      const float2* scales = reinterpret_cast<const float2*>(c.scales) + (size_t)kvh * c.nblk;
+      const int end = min(b1, nb);
+      if (b0 < end) first_e = exponent(__ldg(scales + b0).y);
+      for (int b = b0 + threadIdx.x; b < end; b += 256)
+        if (abs(exponent(__ldg(scales + b).y) - first_e) > (int)kTlFar) sh.far = 1;
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
     const float qscale = __ldg(a.scale) * kLog2e;
     rows_sync();
+    const bool far = sh.far;
     float qs;
     {
       // each of a row's two threads looks over half of it
@@ -300,6 +330,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     rows_sync();
     fence_after();
     float m = -INFINITY, l = 0.0f;                // of this thread's row
+    float n = -INFINITY, apart = 0.0f;            // maximum and sum of the weights apart
     const uint32_t s_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * w;
     const int lim = grow < nrows ? min(min(a.pos0 + grow / a.group, held - 1), 32 * b1 - 1) : -1;
     const uint32_t leader = elect_one();
@@ -352,6 +383,20 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       mma_commit(bar(sh.o_done[s]), leader);
     };
     const bool issues = (warp & 3) == 0;
+    // block b of the tile: its columns by eights, its largest sum of products
+    auto block_at = [&](int b, int h) { return s_at + 64 * (b >> 1) + 16 * h + 8 * (b & 1); };
+    auto block_max = [&](int b) {
+      float big = -INFINITY;
+#pragma unroll 1
+      for (int h = 0; h < 4; ++h) {
+        uint32_t x[8];
+        tmem_ld8(block_at(b, h), x);
+        tmem_wait(x);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) big = fmaxf(big, __uint_as_float(x[k]));
+      }
+      return big;
+    };
 #pragma unroll 1
     for (int i = w;; i += 2) {
       if (issues) {
@@ -384,6 +429,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       // The largest exponent of the row in this tile. Here and below loops stay as rolled as
       // the two buffers allow: the code of all roles has to fit the instruction cache.
       uint32_t v[2][32];
+      // (the open block's scale is known in its tile)
+      const bool look = far || (has_tail && i == nt - 1 && fabsf(sc[(nb - b0) & 3][1] - (float)first_e) > kTlFar);
       float up = m;
       tmem_ld32(s_at, v[0]);
 #pragma unroll 1
@@ -404,10 +451,36 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         if (see >= 0) up = fmaxf(up, fmaf(fmaxf(mx[0], mx[2]), sc[b][0] * qs, sc[b][1]));
         if (see >= 32) up = fmaxf(up, fmaf(fmaxf(mx[1], mx[3]), sc[b + 1][0] * qs, sc[b + 1][1]));
       }
-      l *= m == -INFINITY ? 0.0f : ex2(m - up);
+      const float fl = m == -INFINITY ? 0.0f : ex2(0.5f * (m - up));   // twice: 2^(m - up) may be 0
+      l = l * fl * fl;
       m = up;
       sh.top[i & 3][row] = m;
       const float m0 = m == -INFINITY ? 0.0f : m;
+      if (__builtin_expect(look, 0)) {
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+          const float f = sc[b][0] * qs, x = block_max(b) * f;
+          const bool go = see0 >= 32 * b && x + sc[b][1] - m0 < kTlApart && x > -INFINITY;
+          if (go && x > n) {
+            apart *= n == -INFINITY ? 0.0f : ex2(n - x);
+            n = x;
+          }
+#pragma unroll 1
+          for (int h = 0; h < 4; ++h) {
+            uint32_t y[8];
+            tmem_ld8(block_at(b, h), y);
+            tmem_wait(y);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const bool out = go && y[k] != 0xFF800000u;
+              apart += out ? ex2(fmaf(__uint_as_float(y[k]), f, -n)) : 0.0f;
+              y[k] = out ? 0xFF800000u : y[k];
+            }
+            tmem_st8(block_at(b, h), y);
+          }
+        }
+        tmem_st_wait();
+      }
       uint32_t z[2][16];
       tmem_ld16(s_at, z[0]);
 #pragma unroll 1
@@ -466,6 +539,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     }
     sh.m[w][row] = m;
     sh.l[w][row] = l;
+    sh.n[w][row] = n;
+    sh.k[w][row] = apart;
     asm volatile("bar.sync 1, 384;" ::: "memory");         // with the warps that have the sums
     rows_out();
     if (kMeet) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kTlRegs));
@@ -503,25 +578,40 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     }
     asm volatile("bar.sync 1, 384;" ::: "memory");
     const float nan = __int_as_float(0x7fc00000);
-    const float l0 = sh.l[0][row], l1 = sh.l[1][row];
-    float L = (l0 == 0.0f ? 0.0f : l0 * ex2(sh.m[0][row] - M)) +
-              (l1 == 0.0f ? 0.0f : l1 * ex2(sh.m[1][row] - M));
+    // The sums go by M, and so does l, which lacks 2^-5 of the lift; the weights apart by n. From
+    // here on all goes by N, M and a whole number e that brings the sum of the weights near 1; 2^-e
+    // in two factors, as it may pass the range of one.
+    float l = 0.0f, n = -INFINITY, apart = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float f = ex2(0.5f * (sh.m[k][row] - M)), x = sh.n[k][row], up = fmaxf(n, x);
+      l += sh.l[k][row] == 0.0f ? 0.0f : sh.l[k][row] * f * f;
+      if (up == -INFINITY) continue;
+      apart = apart * ex2(n - up) + sh.k[k][row] * ex2(x - up);
+      n = up;
+    }
+    int e = l == 0.0f ? -250 : (int)(__float_as_uint(l) >> 23 & 255) - 127 + 5;
+    if (apart > 0.0f) e = max(e, (int)fmaxf(fminf(ceilf(n - M), 250.0f), -250.0f));
+    auto two_to = [](int x) { return __int_as_float((127 + x) << 23); };
+    const float p0 = two_to(-(e >> 1)), p1 = two_to((e >> 1) - e);
+    float N = M + (float)e, L = l * p0 * p1 * 32.0f + (apart > 0.0f ? apart * ex2(n - N) : 0.0f);
+    if (M == -INFINITY && l == 0.0f) { N = n; L = apart; }        // no V but zeros
     if (*given_up) L = nan;
     if (nact == 1) {
       L = 1.0f / L;
       if (a.pos0 + grow / a.group >= held) L = nan;
     }
-    const float f = nact > 1 ? 1.0f : L;
+    const float f0 = p0 * (1.0f / kTlLift), f1 = nact > 1 ? p1 : p1 * L;
     float* line = lines + (size_t)row * kTlLine;
 #pragma unroll
     for (int d = 0; d < kHd / 2; d += 2) {
       const float2 x = unpair(acc[d]), y = unpair(acc[d + 1]);
       *reinterpret_cast<float4*>(line + 2 * d) =
-          make_float4(x.x * kTlDrop * f, x.y * kTlDrop * f, y.x * kTlDrop * f, y.y * kTlDrop * f);
+          make_float4(x.x * f0 * f1, x.y * f0 * f1, y.x * f0 * f1, y.y * f0 * f1);
     }
     float* part = a.part + (slot + chunk) * rows_part(kTlRows);
     if (nact > 1)
-      *reinterpret_cast<float2*>(kMeet ? sh.ml[row] : part + kTlRows * kHd + 2 * row) = make_float2(M, L);
+      *reinterpret_cast<float2*>(kMeet ? sh.ml[row] : part + kTlRows * kHd + 2 * row) = make_float2(N, L);
     rows_out();
     if (kMeet) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kTlRegs));
   } else if (warp < 16) {

@@ -32,7 +32,7 @@ def some(ntok, *more):
     return sorted({0, 1, ntok // 3, ntok // 2, ntok - 2, ntok - 1, *more} & set(range(ntok)))
 
 
-@pytest.mark.parametrize("nkv,group,pos0,ntok", FEW + ONE)
+@pytest.mark.parametrize("nkv,group,pos0,ntok", LONG[1:] + FEW + ONE)
 def test_blocks_of_values_further_apart_than_an_exponent(hv, nkv, group, pos0, ntok):
     """V of 1e20 beside V of 1e-20, in one chunk and in different ones: the small values add next
     to nothing, but their weights count."""
