@@ -31,8 +31,9 @@
 // attends to does not cost the others precision; the sum of the weights adds w s_v / s_v.
 // Weights stand as 2^15 times themselves, exact to 2^-40 of the row's largest w s_v. Where a block's
 // largest is under 2^-64 of that, its weights would be lost to the sum too: they are added up apart,
-// without the scale, by a maximum of their own, and leave the tile's scores. Only a chunk whose
-// scales are 2^30 apart looks for them. At its end all goes by one power of two of the sum of the
+// without the scale, by a maximum of their own, and leave the tile's scores. So do those of a block
+// of which the row sees no V but zeros, whose w s_v stands for nothing. Only a chunk whose
+// scales are 2^30 apart, or that may have zeros, looks for them. At its end all goes by one power of two of the sum of the
 // weights.
 // The open block's f32 rows are two binary16 terms: after the tile's products with the first
 // term, the same buffer holds the second one (zero elsewhere) for one product more.
@@ -59,6 +60,7 @@ constexpr int kTlLine = kHd + 4;               // floats from row to row on thei
 constexpr float kTlLift = 32768.0f;             // 2^15
 constexpr float kTlDrop = 0x1p-20f;             // of the sum of weights: room for 2^20 of them over
                                                 // a scale of 2^-110
+constexpr int kTlNone = 1 << 29;
 constexpr float kTlApart = -64.0f;              // log2 of a block's largest w s_v over the row's
 constexpr float kTlFar = 30.0f;                 // exponents between scales: so that without `far` all
                                                 // weights of note are within kTlApart
@@ -180,6 +182,7 @@ struct TlShared {
   unsigned long long full_k[2], full_v[2], s_ready[2], w_ready[2], o_done[2];
   unsigned long long o_free, k_free, v_free, drain[2];
   float sc[4][4][4];             // of the last four tiles' blocks: s_k, log2 s_v, 1 / s_v
+  int first[4][4];               // first position with a V that is not zero, where that is looked for
   float top[4][kTlRows];         // of the last four tiles: what their weights are relative to
   float m[2][kTlRows], l[2][kTlRows];
   float n[2][kTlRows], k[2][kTlRows];     // of the weights apart: maximum, sum
@@ -282,12 +285,14 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
                      :: "r"(to + r * kTlLine * 4), "l"(src) : "memory");
       }
-      // meanwhile: are there scales of V far from the chunk's first?
+      // meanwhile: are there scales of V far from the chunk's first, or one that may be of zeros?
       const float2* scales = reinterpret_cast<const float2*>(c.scales) + (size_t)kvh * c.nblk;
       const int end = min(b1, nb);
       if (b0 < end) first_e = exponent(__ldg(scales + b0).y);
-      for (int b = b0 + threadIdx.x; b < end; b += 256)
-        if (abs(exponent(__ldg(scales + b).y) - first_e) > (int)kTlFar) sh.far = 1;
+      for (int b = b0 + threadIdx.x; b < end; b += 256) {
+        const float s = __ldg(scales + b).y;
+        if (s == 1.0f || abs(exponent(s) - first_e) > (int)kTlFar) sh.far = 1;
+      }
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
     const float qscale = __ldg(a.scale) * kLog2e;
@@ -430,7 +435,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       // the two buffers allow: the code of all roles has to fit the instruction cache.
       uint32_t v[2][32];
       // (the open block's scale is known in its tile)
-      const bool look = far || (has_tail && i == nt - 1 && fabsf(sc[(nb - b0) & 3][1] - (float)first_e) > kTlFar);
+      const bool look = far || (has_tail && i == nt - 1 && (fabsf(sc[(nb - b0) & 3][1] - (float)first_e) > kTlFar || sh.open_max[1] == 0.0f));
       float up = m;
       tmem_ld32(s_at, v[0]);
 #pragma unroll 1
@@ -451,6 +456,15 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         if (see >= 0) up = fmaxf(up, fmaf(fmaxf(mx[0], mx[2]), sc[b][0] * qs, sc[b][1]));
         if (see >= 32) up = fmaxf(up, fmaf(fmaxf(mx[1], mx[3]), sc[b + 1][0] * qs, sc[b + 1][1]));
       }
+      const int (&first)[4] = sh.first[i & 3];
+      if (__builtin_expect(look, 0)) {                      // the largest again, without zeros
+        up = m;
+#pragma unroll 1
+        for (int b = 0; b < 4; ++b) {
+          const float x = block_max(b);
+          if (see0 >= 32 * b + first[b]) up = fmaxf(up, fmaf(x, sc[b][0] * qs, sc[b][1]));
+        }
+      }
       const float fl = m == -INFINITY ? 0.0f : ex2(0.5f * (m - up));   // twice: 2^(m - up) may be 0
       l = l * fl * fl;
       m = up;
@@ -460,7 +474,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
 #pragma unroll 1
         for (int b = 0; b < 4; ++b) {
           const float f = sc[b][0] * qs, x = block_max(b) * f;
-          const bool go = see0 >= 32 * b && x + sc[b][1] - m0 < kTlApart && x > -INFINITY;
+          const int at = see0 - 32 * b;
+          const bool go = at >= 0 && (at < first[b] || x + sc[b][1] - m0 < kTlApart) && x > -INFINITY;
           if (go && x > n) {
             apart *= n == -INFINITY ? 0.0f : ex2(n - x);
             n = x;
@@ -768,7 +783,23 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         }
       }
     };
-    auto put_scales = [&](int i, float sk, float sv) {
+    // the block's first position with a V code that is not 0 (kTlNone without one): a lane's bytes
+    // are those of positions 16 k + 8 j + 2 t + e
+    auto first_of = [&] {
+      constexpr uint32_t kZeros = 0x80808080u;
+      uint32_t any[2] = {0, 0};
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        any[0] |= (vx[u].x ^ kZeros) | (vx[u].z ^ kZeros);
+        any[1] |= (vx[u].y ^ kZeros) | (vx[u].w ^ kZeros);
+      }
+      int at = kTlNone;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (any[k >> 2] >> 8 * (k & 3) & 255) at = min(at, 16 * (k >> 2) + 8 * (k >> 1 & 1) + 2 * t + (k & 1));
+      return __reduce_min_sync(0xFFFFFFFFu, at);
+    };
+    auto put_scales = [&](int i, float sk, float sv, int first) {
       if (lane == 0) {
         // a scale under 2^-110 counts as that (values up to 10^-31), so that a chunk of such
         // blocks alone, whose sum of weights goes by its reciprocal, stays in range; a NaN stays
@@ -776,7 +807,14 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         sh.sc[i & 3][cw][0] = sk;
         sh.sc[i & 3][cw][1] = log2f(sv);
         sh.sc[i & 3][cw][2] = sv == sv ? kTlDrop / sv : 0.0f;
+        sh.first[i & 3][cw] = first;
       }
+    };
+    // only a scale of 1 can be that of a block of zeros, and only a block that some row does not
+    // see whole can have no others to a row
+    auto put_coded = [&](int i, float2 s) {
+      const bool find = live(i) && (s.y == 1.0f || 32 * (b0 + 4 * i + cw) + 31 > a.pos0 + row0 / a.group);
+      put_scales(i, s.x, s.y, find ? first_of() : 0);
     };
     auto scales_of = [&](int i) { return live(i) ? __ldg(scales + b0 + 4 * i + cw) : make_float2(1.f, 1.f); };
     fetch(0, 0, kx);
@@ -790,7 +828,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       ok = i < 2 || bar_wait_warp(bar(sh.s_ready[s]), ((i - 2) >> 1) & 1, given_up);
       if (!ok) break;
       coded_k(i, k_buf + s * kTlTile);
-      put_scales(i, sc.x, sc.y);
+      put_coded(i, sc);
       fence_async();
       bar_arrive(bar(sh.full_k[s]));
       fetch(i + 1, 0, kx);
@@ -812,7 +850,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       ok = i < 2 || bar_wait_warp(bar(sh.s_ready[s]), ((i - 2) >> 1) & 1, given_up);
       if (ok && !mine) coded_k(i, kt);
       if (ok) open_scan();
-      put_scales(i, mine ? 1.0f / lk : sc.x, mine ? 1.0f / lv : sc.y);
+      if (mine) put_scales(i, 1.0f / lk, 1.0f / lv, sh.open_max[1] == 0.0f ? kTlNone : 0);
+      else put_coded(i, sc);
 #pragma unroll 1
       for (int pass = 0; pass < 2 && ok; ++pass) {
         if (pass) {

@@ -32,7 +32,26 @@ def some(ntok, *more):
     return sorted({0, 1, ntok // 3, ntok // 2, ntok - 2, ntok - 1, *more} & set(range(ntok)))
 
 
-@pytest.mark.parametrize("nkv,group,pos0,ntok", LONG[1:] + FEW + ONE)
+@pytest.mark.parametrize("size", [1.0, 1e-6, 1e-12])
+@pytest.mark.parametrize("nkv,group,pos0,ntok", LONG + FEW + ONE)
+def test_blocks_whose_values_are_all_zero(hv, nkv, group, pos0, ntok, size):
+    """They weigh in the sum of the weights and add nothing else, however small the rest is: one
+    block, a whole chunk of them, the open block."""
+    n = pos0 + ntok
+    for zero in (slice(64, 96), slice(0, 32 * (n // 64)), slice(n // 32 * 32, n), slice(0, n)):
+        g = np.random.default_rng(51)
+        k, v = rows(g, n, nkv, 0.3)
+        v *= F32(size)
+        v[zero] = 0
+        ref = R.Cache(nkv, n + 9)
+        ref.write(k, v, 0)
+        q = queries(g, ref, ntok, nkv * group)
+        got = run(hv, ref, q, pos0, group)
+        for t in some(ntok):
+            near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
+
+
+@pytest.mark.parametrize("nkv,group,pos0,ntok", LONG + FEW + ONE)
 def test_blocks_of_values_further_apart_than_an_exponent(hv, nkv, group, pos0, ntok):
     """V of 1e20 beside V of 1e-20, in one chunk and in different ones: the small values add next
     to nothing, but their weights count."""
