@@ -7,6 +7,7 @@
 // cache reads back: f32(c s) in complete blocks, the f32 rows of the open one.
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 
 #include "attn_q8.cuh"
 #include "attn_q8_rows.h"
@@ -470,7 +471,9 @@ int dec_chunks(int nkv, int cap, int* out) {
 // shares of the chunk's blocks: few rows spread over the positions, many share each block.
 // Here the rows are the 16-row operand: S = q K^T and ctx += w V, both terms of q (of w) into
 // the same sums. The open block's f32 rows become two binary16 terms as well, so that it is
-// a block like the others with a third product, hi x lo.
+// a block like the others with a third product, hi x lo. Each of its rows has a power of two of
+// its own, so that no row, least of all one that a query does not see, takes bits from another:
+// a K row's is taken back from its scores, a V row's goes with its weights.
 // Bound by latency: 44 tokens of 16 heads (8 kv heads) over 300 positions take 11.6 us in a
 // graph, 8 tokens of 32 heads over 38 positions 10.7.
 constexpr int kRowWarps = 8;
@@ -492,7 +495,7 @@ template <int kWM, bool kMeet>
 __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, KvQ8 c) {
   using Cfg = RowsCfg<kWM>;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float s_m[kRowWarps][16], s_l[kRowWarps][16], s_amax[2];
+  __shared__ float s_m[kRowWarps][16], s_l[kRowWarps][16], s_amax[2][kQ8Blk];
   __shared__ int s_bad;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
   const int wm = warp % kWM, share = warp / kWM;
@@ -592,7 +595,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   // g0 (g1) of the row's.
   uint32_t wh[2][4], wl[2][4];
   float g0, g1;
-  auto weights = [&](int b, float (&s)[4][4], float f0, float f1) {
+  float v_up = 0.0f;                // of open row `lane`: the exponent that its V lacks, -inf for zeros
+  auto weights = [&](int b, float (&s)[4][4], float f0, float f1, auto is_open) {
     const bool cut = 32 * b + 31 > warp_low;
     float y0 = -INFINITY, y1 = -INFINITY;
 #pragma unroll
@@ -623,6 +627,29 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
 #pragma unroll
       for (int d = 0; d < 16; ++d) { acc[d][0] *= a0; acc[d][1] *= a0; acc[d][2] *= a1; acc[d][3] *= a1; }
     }
+    if constexpr (decltype(is_open)::value) {
+      // the sum of the weights by the scores, the weights by w v
+      const float n0 = m0 == -INFINITY ? 0.0f : m0, n1 = m1 == -INFINITY ? 0.0f : m1;
+      y0 = y1 = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          l0 += ex2(s[j][e] - n0) * 32768.0f;
+          l1 += ex2(s[j][2 + e] - n1) * 32768.0f;
+          const float up = __shfl_sync(0xFFFFFFFFu, v_up, 8 * j + 2 * t + e);
+          s[j][e] += up;
+          s[j][2 + e] += up;
+          y0 = fmaxf(y0, s[j][e]);
+          y1 = fmaxf(y1, s[j][2 + e]);
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        y0 = fmaxf(y0, __shfl_xor_sync(0xFFFFFFFFu, y0, o));
+        y1 = fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, o));
+      }
+    }
     // a row that sees none of the block's positions has y = -inf and weights of 0
     g0 = y0 == -INFINITY ? 0.0f : ex2(y0 - m0);
     g1 = y1 == -INFINITY ? 0.0f : ex2(y1 - m1);
@@ -635,8 +662,10 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       for (int e = 0; e < 2; ++e) {
         p[e] = ex2(s[j][e] - y0) * 32768.0f;
         p[2 + e] = ex2(s[j][2 + e] - y1) * 32768.0f;
-        l0 = fmaf(p[e], g0, l0);
-        l1 = fmaf(p[2 + e], g1, l1);
+        if constexpr (!decltype(is_open)::value) {
+          l0 = fmaf(p[e], g0, l0);
+          l1 = fmaf(p[2 + e], g1, l1);
+        }
       }
       // A fragment: (row g, k 2t), (row g + 8, k 2t), (row g, k 2t + 8), (row g + 8, k 2t + 8)
       split_half2(p[0], p[1], &wh[j >> 1][2 * (j & 1)], &wl[j >> 1][2 * (j & 1)]);
@@ -649,33 +678,31 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
     // are values that are not finite, whose weight of 0 for the rows that do not see them
     // would not be nothing: the rows that see one get a sum of NaN instead
     __half* frag = reinterpret_cast<__half*>(smem + Cfg::kSmem - Cfg::kOpen - Cfg::kTail);
-    if (threadIdx.x < 2) s_amax[threadIdx.x] = 0.0f;
+    if (threadIdx.x < 2 * kQ8Blk) s_amax[threadIdx.x / kQ8Blk][threadIdx.x % kQ8Blk] = 0.0f;
     if (threadIdx.x == 0) s_bad = kQ8Blk;
     asm volatile("cp.async.wait_group %0;" :: "n"(Cfg::kStages) : "memory");
     __syncthreads();
-    for (int which = 0; which < 2; ++which) {
+    for (int r = warp; r < 2 * nopen; r += kRowWarps) {        // a row a warp, K's before V's
+      const int which = r >= nopen, at = which ? r - nopen : r;
+      const float4 x = reinterpret_cast<const float4*>(open + which * kQ8Codes + at * kHd)[lane];
+      const float v[4] = {fabsf(x.x), fabsf(x.y), fabsf(x.z), fabsf(x.w)};
       float amax = 0.0f;
-      for (int i = threadIdx.x; i < nopen * (kHd / 4); i += blockDim.x) {
-        const float4 x = reinterpret_cast<const float4*>(open + which * kQ8Codes)[i];
-        const float v[4] = {fabsf(x.x), fabsf(x.y), fabsf(x.z), fabsf(x.w)};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (v[e] < INFINITY) amax = fmaxf(amax, v[e]);
-          else atomicMin(&s_bad, i / (kHd / 4));
-        }
+      for (int e = 0; e < 4; ++e) {
+        if (v[e] < INFINITY) amax = fmaxf(amax, v[e]);
+        else atomicMin(&s_bad, at);
       }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFu, amax, o));
-      if (lane == 0) atomicMax(reinterpret_cast<int*>(&s_amax[which]), __float_as_int(amax));
+      const unsigned top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(amax));
+      if (lane == 0) s_amax[which][at] = __uint_as_float(top);
     }
     __syncthreads();
-    const float lk = q8_lift(s_amax[0]), lv = q8_lift(s_amax[1]);
     auto term = [&](float x, float lift) { return fabsf(x) < INFINITY ? x * lift : 0.0f; };
     // four dims of a K row are neighbours in a fragment, two rows of a V dim
     for (int i = threadIdx.x; i < kQ8Codes / 4; i += blockDim.x) {
       const int r = i / (kHd / 4), d = 4 * (i % (kHd / 4));
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < nopen) x = *reinterpret_cast<const float4*>(open + r * kHd + d);
+      const float lk = q8_lift(s_amax[0][r]);
       uint2 hi, lo;
       split_half2(term(x.x, lk), term(x.y, lk), &hi.x, &lo.x);
       split_half2(term(x.z, lk), term(x.w, lk), &hi.y, &lo.y);
@@ -686,7 +713,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       const int r = 2 * (i / kHd), d = i % kHd;
       const float* v = open + kQ8Codes + r * kHd + d;
       uint32_t hi, lo;
-      split_half2(r < nopen ? term(v[0], lv) : 0.0f, r + 1 < nopen ? term(v[kHd], lv) : 0.0f, &hi, &lo);
+      split_half2(r < nopen ? term(v[0], q8_lift(s_amax[1][r])) : 0.0f,
+                  r + 1 < nopen ? term(v[kHd], q8_lift(s_amax[1][r + 1])) : 0.0f, &hi, &lo);
       *reinterpret_cast<uint32_t*>(frag + 2 * kQ8Codes + q8_v_at(r, d)) = hi;
       *reinterpret_cast<uint32_t*>(frag + 3 * kQ8Codes + q8_v_at(r, d)) = lo;
     }
@@ -708,8 +736,21 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
           mma_f16(s[j], qh[k], kl.x, kl.y);
         }
       }
-      weights(closed, s, qs0 / lk, qs1 / lk);
-      const float f0 = g0 / lv, f1 = g1 / lv;
+      // the scores by the largest row's power of two: the others' sums fall, and none overflows
+      const float k_max = s_amax[0][lane], v_max = s_amax[1][lane];
+      const float lk = q8_lift(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(k_max))));
+      const float k_down = k_max > 0.0f ? lk / q8_lift(k_max) : 0.0f;
+      if (v_max == 0.0f) v_up = -INFINITY;
+      else v_up = (float)(127 - (int)(__float_as_uint(q8_lift(v_max)) >> 23));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float f = __shfl_sync(0xFFFFFFFFu, k_down, 8 * j + 2 * t + e);
+          s[j][e] *= f;
+          s[j][2 + e] *= f;
+        }
+      weights(closed, s, qs0 / lk, qs1 / lk, std::true_type{});
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
 #pragma unroll
@@ -724,7 +765,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            acc[2 * u + h][i] = fmaf(d[i], i < 2 ? f0 : f1, acc[2 * u + h][i]);
+            acc[2 * u + h][i] = fmaf(d[i], i < 2 ? g0 : g1, acc[2 * u + h][i]);
         }
       }
       if (lim0 >= closed * kQ8Blk + s_bad) l0 = __int_as_float(0x7fc00000);
@@ -756,7 +797,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
           }
         }
       }
-      weights(b, s, sc.x * qs0, sc.x * qs1);
+      weights(b, s, sc.x * qs0, sc.x * qs1, std::false_type{});
       // a row that sees nothing of the block takes nothing from it, whatever its scale
       const float f0 = 32 * b <= lim0 ? sc.y * g0 : 0.0f, f1 = 32 * b <= lim1 ? sc.y * g1 : 0.0f;
 #pragma unroll

@@ -36,7 +36,10 @@
 // scales are 2^30 apart, or that may have zeros, looks for them. At its end all goes by one power of two of the sum of the
 // weights.
 // The open block's f32 rows are two binary16 terms: after the tile's products with the first
-// term, the same buffer holds the second one (zero elsewhere) for one product more.
+// term, the same buffer holds the second one (zero elsewhere) for one product more. Each of its
+// rows has a power of two of its own, so that no row, least of all one that a query does not see,
+// takes bits from another: the scores become exponents of w with a K row's taken back, which are
+// added up with the weights apart, and then those of w v with what a V row's lacks.
 //
 // Every wait is bounded: one that runs out ends the CTA, whose rows are then NaN.
 //
@@ -188,7 +191,8 @@ struct TlShared {
   float n[2][kTlRows], k[2][kTlRows];     // of the weights apart: maximum, sum
   float ml[kTlRows][2];          // of the rows' sums, where another CTA of the cluster adds them up
   uint32_t tmem;
-  float open_max[2];             // of the open rows: largest |K|, |V|
+  float open_max[2][kQ8Blk];     // of the open rows: largest |K|, |V|; what takes K's power of two
+  float open_k[kQ8Blk], open_v[kQ8Blk];   // back but for the block's, the exponent that V lacks
   int bad;                       // first open row with a value that is not finite
   int given_up;
   int far;                       // scales of V too far apart for one sum of weights
@@ -234,7 +238,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.bad = kQ8Blk;
     sh.far = 0;
-    sh.open_max[0] = sh.open_max[1] = 0.0f;
     sh.given_up = (sm & 1023) != 0;               // the swizzle goes by addresses
   }
   if (warp == 15) {
@@ -434,8 +437,41 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       // The largest exponent of the row in this tile. Here and below loops stay as rolled as
       // the two buffers allow: the code of all roles has to fit the instruction cache.
       uint32_t v[2][32];
-      // (the open block's scale is known in its tile)
-      const bool look = far || (has_tail && i == nt - 1 && (fabsf(sc[(nb - b0) & 3][1] - (float)first_e) > kTlFar || sh.open_max[1] == 0.0f));
+      const bool tail = has_tail && i == nt - 1;
+      const int ob = tail ? (nb - b0) & 3 : -1;             // the open block
+      bool look = far;
+      if (tail) {
+        const float f = sc[ob][3] * qs;
+        float most = -INFINITY;
+#pragma unroll 1
+        for (int h = 0; h < 4; ++h) {
+          uint32_t x[8];
+          float big = n;
+          tmem_ld8(block_at(ob, h), x);
+          tmem_wait(x);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int r = 8 * (k >> 1) + 2 * h + (k & 1);
+            const float y = r <= see0 - 32 * ob ? __uint_as_float(x[k]) * sh.open_k[r] * f : -INFINITY;
+            x[k] = __float_as_uint(y);
+            big = fmaxf(big, y);
+          }
+          const float n0 = big == -INFINITY ? 0.0f : big;
+          apart *= n == -INFINITY ? 0.0f : ex2(n - n0);
+          n = big;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const int r = 8 * (k >> 1) + 2 * h + (k & 1);
+            const float y = __uint_as_float(x[k]), v = sh.open_v[r];
+            apart += ex2(y - n0);
+            x[k] = __float_as_uint(y + v);
+            most = fmaxf(most, v);
+          }
+          tmem_st8(block_at(ob, h), x);
+        }
+        tmem_st_wait();
+        look |= most - (float)first_e > kTlFar;
+      }
       float up = m;
       tmem_ld32(s_at, v[0]);
 #pragma unroll 1
@@ -453,8 +489,9 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
             y = fmaxf(y, __uint_as_float(x[k]));
           }
         }
-        if (see >= 0) up = fmaxf(up, fmaf(fmaxf(mx[0], mx[2]), sc[b][0] * qs, sc[b][1]));
-        if (see >= 32) up = fmaxf(up, fmaf(fmaxf(mx[1], mx[3]), sc[b + 1][0] * qs, sc[b + 1][1]));
+        const float qs0 = b == ob ? 1.0f : qs, qs1 = b + 1 == ob ? 1.0f : qs;
+        if (see >= 0) up = fmaxf(up, fmaf(fmaxf(mx[0], mx[2]), sc[b][0] * qs0, sc[b][1]));
+        if (see >= 32) up = fmaxf(up, fmaf(fmaxf(mx[1], mx[3]), sc[b + 1][0] * qs1, sc[b + 1][1]));
       }
       const int (&first)[4] = sh.first[i & 3];
       if (__builtin_expect(look, 0)) {                      // the largest again, without zeros
@@ -462,7 +499,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
 #pragma unroll 1
         for (int b = 0; b < 4; ++b) {
           const float x = block_max(b);
-          if (see0 >= 32 * b + first[b]) up = fmaxf(up, fmaf(x, sc[b][0] * qs, sc[b][1]));
+          if (see0 >= 32 * b + first[b]) up = fmaxf(up, fmaf(x, sc[b][0] * (b == ob ? 1.0f : qs), sc[b][1]));
         }
       }
       const float fl = m == -INFINITY ? 0.0f : ex2(0.5f * (m - up));   // twice: 2^(m - up) may be 0
@@ -475,7 +512,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         for (int b = 0; b < 4; ++b) {
           const float f = sc[b][0] * qs, x = block_max(b) * f;
           const int at = see0 - 32 * b;
-          const bool go = at >= 0 && (at < first[b] || x + sc[b][1] - m0 < kTlApart) && x > -INFINITY;
+          const bool go = b != ob && at >= 0 && (at < first[b] || x + sc[b][1] - m0 < kTlApart) && x > -INFINITY;
           if (go && x > n) {
             apart *= n == -INFINITY ? 0.0f : ex2(n - x);
             n = x;
@@ -506,7 +543,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
           // -inf f has to stay -inf: not with a scale of 0, nor with the scales (which may be
           // NaN) of a block that the row sees nothing of
           const bool seen = see0 >= 32 * (b + e);
-          float f = seen ? sc[b + e][0] * qs : 1.0f;
+          float f = seen ? sc[b + e][0] * (b + e == ob ? 1.0f : qs) : 1.0f;
           f = f == 0.0f ? 1e-38f : f;
           const float add = seen ? sc[b + e][1] - m0 : 0.0f;
           f2[e] = pair(f, f);
@@ -660,11 +697,14 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       *reinterpret_cast<uint4*>(to + (c >> 1) * kTlHalf + (16 * u + 8 * h + g) * 128 +
                                 (((2 * t + (c & 1)) ^ g) << 4)) = make_uint4(x[0], x[1], x[2], x[3]);
     };
-    // the open rows' values in one of their two terms (second: 1)
-    float lk = 1.0f, lv = 1.0f;
-    auto term = [&](float x0, float x1, float lift, int second) {
-      x0 = fabsf(x0) < INFINITY ? x0 * lift : 0.0f;
-      x1 = fabsf(x1) < INFINITY ? x1 * lift : 0.0f;
+    // the open rows' values in one of their two terms (second: 1); V's up to 2^10: a weight's
+    // precision then goes by w v much as with coded values
+    float lk = 1.0f;
+    auto lift_k = [&](int r) { return q8_lift(sh.open_max[0][r]); };
+    auto lift_v = [&](int r) { return q8_lift(sh.open_max[1][r]) * 0.0625f; };
+    auto term = [&](float x0, float x1, float lift0, float lift1, int second) {
+      x0 = fabsf(x0) < INFINITY ? x0 * lift0 : 0.0f;
+      x1 = fabsf(x1) < INFINITY ? x1 * lift1 : 0.0f;
       uint32_t hi, lo;
       split_half2(x0, x1, &hi, &lo);
       return second ? lo : hi;
@@ -673,6 +713,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     // each, several loads under way at a time
     const int oc = (nb - b0) & 3;
     auto open_k = [&](uint8_t* to, int second) {
+      const float lift = lift_k(8 * cw + g);
       float4 x[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -687,8 +728,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         uint32_t y[8];
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          y[2 * s] = term(x[i][s].x, x[i][s].y, lk, second);
-          y[2 * s + 1] = term(x[i][s].z, x[i][s].w, lk, second);
+          y[2 * s] = term(x[i][s].x, x[i][s].y, lift, lift, second);
+          y[2 * s + 1] = term(x[i][s].z, x[i][s].w, lift, lift, second);
         }
         put_k(to, oc, cw, i, y);
       }
@@ -708,14 +749,14 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         for (int i = 0; i < 2; ++i) {
           uint32_t y[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = term(x[i][2 * j], x[i][2 * j + 1], lv, second);
+          for (int j = 0; j < 4; ++j)
+            y[j] = term(x[i][2 * j], x[i][2 * j + 1], lift_v(8 * j + 2 * t), lift_v(8 * j + 2 * t + 1), second);
           put_v(to, oc, 2 * cw + (i0 >> 1), i, y);
         }
       }
     };
-    // the largest of the open rows' values, eight rows a warp
+    // the largest of each open row's values, eight rows a warp
     auto open_scan = [&] {
-      float mk = 0.0f, mv = 0.0f;
 #pragma unroll 1
       for (int i0 = 0; i0 < 8; i0 += 4) {
         float4 x[4][2];
@@ -731,22 +772,24 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float& m = e ? mv : mk;
+            float m = 0.0f;
             const float v[4] = {fabsf(x[i][e].x), fabsf(x[i][e].y), fabsf(x[i][e].z), fabsf(x[i][e].w)};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               if (v[k] < INFINITY) m = fmaxf(m, v[k]);
               else atomicMin(&sh.bad, 8 * cw + i0 + i);
             }
+            const unsigned top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m));
+            if (lane == 0) sh.open_max[e][8 * cw + i0 + i] = __uint_as_float(top);
           }
       }
-      atomicMax(reinterpret_cast<int*>(&sh.open_max[0]), __float_as_int(mk));
-      atomicMax(reinterpret_cast<int*>(&sh.open_max[1]), __float_as_int(mv));
       asm volatile("bar.sync 4, 128;" ::: "memory");
-      lk = q8_lift(sh.open_max[0]);
-      // values up to 2^10: their scale is then near that of coded values, which is what a
-      // weight's precision goes by (and never under the least that put_scales lets pass)
-      lv = fminf(q8_lift(sh.open_max[1]) * 0.0625f, 0x1p110f);
+      const float k_max = sh.open_max[0][lane], v_max = sh.open_max[1][lane];
+      lk = q8_lift(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(k_max))));
+      if (cw == 0) {
+        sh.open_k[lane] = k_max > 0.0f ? lk / q8_lift(k_max) : 0.0f;
+        sh.open_v[lane] = v_max > 0.0f ? (float)(127 - (int)(__float_as_uint(lift_v(lane)) >> 23)) : -INFINITY;
+      }
     };
     auto none_k = [&](uint8_t* to) {
       const uint32_t y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
@@ -850,8 +893,13 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       ok = i < 2 || bar_wait_warp(bar(sh.s_ready[s]), ((i - 2) >> 1) & 1, given_up);
       if (ok && !mine) coded_k(i, kt);
       if (ok) open_scan();
-      if (mine) put_scales(i, 1.0f / lk, 1.0f / lv, sh.open_max[1] == 0.0f ? kTlNone : 0);
-      else put_coded(i, sc);
+      if (!mine) put_coded(i, sc);
+      else if (lane == 0) {            // the scores come as exponents; their weights are added up already
+        sh.sc[i & 3][cw][0] = 1.0f;
+        sh.sc[i & 3][cw][1] = sh.sc[i & 3][cw][2] = 0.0f;
+        sh.sc[i & 3][cw][3] = 1.0f / lk;
+        sh.first[i & 3][cw] = 0;
+      }
 #pragma unroll 1
       for (int pass = 0; pass < 2 && ok; ++pass) {
         if (pass) {

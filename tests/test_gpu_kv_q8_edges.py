@@ -69,3 +69,36 @@ def test_blocks_of_values_further_apart_than_an_exponent(hv, nkv, group, pos0, n
         got = run(hv, ref, q, pos0, group)
         for t in some(ntok):
             near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
+
+
+@pytest.mark.parametrize("which", ["k", "v", "v up", "both"])
+@pytest.mark.parametrize("nkv,group,pos0,ntok", [
+    (8, 8, 30, 220), (2, 5, 4001, 94), (1, 1, 15024, 200), (2, 2, 210, 40), (8, 4, 992, 28),
+    (1, 4, 224, 26), (2, 4, 249, 1)])
+def test_open_rows_of_very_different_sizes(hv, nkv, group, pos0, ntok, which):
+    """The open block's rows are f32: one that a query does not see, however large, takes nothing
+    from those that it sees, and small ones keep their precision beside it."""
+    n = pos0 + ntok
+    first = n // 32 * 32
+    assert n - first >= 24
+    g = np.random.default_rng(53)
+    k, v = rows(g, n, nkv, 0.3)
+    up, down = F32(1e20), F32(1e-20)
+    if which != "k":
+        if which == "v":
+            v *= down                                          # all small, then two large rows
+        v[first + 3] *= down
+        v[first + 4] = 0
+        v[first + 18:first + 20] *= up
+    if which in ("k", "both"):
+        k[first + 3] *= down
+        k[first + 18] *= F32(1e12)
+    ref = R.Cache(nkv, n + 9)
+    ref.write(k, v, 0)
+    q = queries(g, ref, ntok, nkv * group)
+    q[:, 0] = 0
+    if which in ("k", "both"):
+        q = np.clip(q, -8, 8)                                  # look for rows, not the large one
+    got = run(hv, ref, q, pos0, group)
+    for t in some(ntok, *(first + i - pos0 for i in (2, 3, 4, 5, 16, 17, 18, 19, 20))):
+        near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
