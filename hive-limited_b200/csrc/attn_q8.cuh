@@ -62,7 +62,7 @@ HV_DEV float ex2(float x) {
 
 // 2^e that brings a largest value of `amax` to [2^13, 2^14) (1 for zero and non-finite).
 HV_DEV float q8_lift(float amax) {
-  if (!(amax > 0.0f) || amax > 3.4e38f) return 1.0f;
+  if (!(amax > 0.0f && amax < INFINITY)) return 1.0f;
   int e = 13 + 127 - (int)(__float_as_uint(amax) >> 23);        // 13 - floor(log2 amax)
   e = e > 126 ? 126 : (e < -126 ? -126 : e);
   return __uint_as_float((unsigned)(e + 127) << 23);

@@ -102,3 +102,22 @@ def test_open_rows_of_very_different_sizes(hv, nkv, group, pos0, ntok, which):
     got = run(hv, ref, q, pos0, group)
     for t in some(ntok, *(first + i - pos0 for i in (2, 3, 4, 5, 16, 17, 18, 19, 20))):
         near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
+
+
+@pytest.mark.parametrize("nkv,group,pos0,ntok", [(8, 8, 30, 220), (2, 4, 210, 40), (2, 3, 249, 1)])
+def test_queries_and_open_rows_up_to_the_largest_float(hv, nkv, group, pos0, ntok):
+    n, nq = pos0 + ntok, nkv * group
+    g = np.random.default_rng(55)
+    top = np.finfo(F32).max
+    k, v = rows(g, n, nkv, 0.3)
+    k *= F32(3e-38)
+    q = g.standard_normal((ntok, nq, HD)).astype(F32)
+    q[:, ::2] *= F32(5e37)
+    q[:, ::2, 5] = top
+    q[:, 1] = 0
+    q[:, 1, 7] = -top
+    ref = R.Cache(nkv, n + 9)
+    ref.write(k, v, 0)
+    got = run(hv, ref, q, pos0, group)
+    for t in some(ntok):
+        near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
