@@ -208,6 +208,15 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       const int r = warp + kDecWarps * i;
       x0[i] = r < ntail && head0 < group ? s_x[r][head0] : -INFINITY;
       x1[i] = r < ntail && head0 + 1 < group ? s_x[r][head0 + 1] : -INFINITY;
+      if (r >= ntail) continue;
+      // a row with a value that is not finite loses all of the context, as a complete block does
+      const float4 k = *reinterpret_cast<const float4*>(open_k + r * kDecLine + 4 * lane);
+      const float4 v = *reinterpret_cast<const float4*>(open_v + r * kHd + 4 * lane);
+      const float e[8] = {k.x, k.y, k.z, k.w, v.x, v.y, v.z, v.w};
+      bool fine = true;
+#pragma unroll
+      for (int d = 0; d < 8; ++d) fine = fine && fabsf(e[d]) < INFINITY;
+      if (!__all_sync(0xFFFFFFFFu, fine)) x0[i] = x1[i] = __int_as_float(0x7fc00000);
     }
     raise(fmaxf(fmaxf(x0[0], x0[1]), fmaxf(x0[2], x0[3])),
           fmaxf(fmaxf(x1[0], x1[1]), fmaxf(x1[2], x1[3])));

@@ -298,7 +298,8 @@ int hv_kv_read_q8(const void* kv, float* k_out, float* v_out, int pos0, int nkv,
  * order of operations: the lane has its own results). Query head h reads kv head h / group,
  * group 1 to 8; q and ctx [ntok][nq][128], 16-byte aligned. The sums run ahead of the quotient
  * by 2^15 and the number of positions: V to about 10^30 (and from 10^-31 on) keeps f32's
- * precision.
+ * precision. An open row with a NaN or an infinity in its K or V makes the whole context of
+ * every query NaN that sees it, as a complete block that holds one does.
  *   hv_attn_decode_q8  one query row over positions 0 .. *pos. A *pos that is not held
  *                      leaves NaN in ctx and reads no cache row.            (fda_warp_pos)
  *   hv_attn_rows_q8    row t over positions 0 .. pos0 + t of the cache as it stands: rows of

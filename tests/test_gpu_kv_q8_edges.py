@@ -121,3 +121,39 @@ def test_queries_and_open_rows_up_to_the_largest_float(hv, nkv, group, pos0, nto
     got = run(hv, ref, q, pos0, group)
     for t in some(ntok):
         near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
+
+
+@pytest.mark.parametrize("which,bad", [("k", np.nan), ("k", -np.inf), ("k", np.inf),
+                                       ("v", np.nan), ("v", np.inf)])
+@pytest.mark.parametrize("nkv,group,cap", [(8, 8, 288), (1, 4, 288), (8, 3, 288), (1, 8, 40000)])
+def test_open_rows_that_are_not_finite_lose_the_whole_context(hv, nkv, group, cap, which, bad):
+    """As a complete block that holds one reads NaN throughout: every head of that kv head's
+    group, in all its dimensions, from that position on, in each kernel."""
+    n, at = 250, 237
+    g = np.random.default_rng(54)
+    k, v = rows(g, n, nkv, 0.3)
+    (k if which == "k" else v)[at, -1, 77] = bad
+    ref = R.Cache(nkv, cap)
+    ref.write(k, v, 0)
+    nq = nkv * group
+    q = np.abs(g.standard_normal((220, nq, HD))).astype(F32)
+    lost = np.arange(nq) // group == nkv - 1
+    clean = ref.val.copy()
+    clean[:, -1, at] = 0
+    for ntok in (220, 40, 17):
+        got = run(hv, ref, q[:ntok], n - ntok, group)
+        for t in some(ntok, at - 1 - n + ntok, at - n + ntok):
+            pos = n - ntok + t
+            gone = lost & (pos >= at)
+            assert np.isnan(got[t][gone]).all()
+            want, tol = R.attention(q[t], clean, pos, group, float(SCALE))
+            near(got[t][~gone], want[~gone], tol[~gone])
+    kv, s, ctx = Dev(ref.buffer(0xFF)), scratch(hv, nq, group, cap), Dev(nbytes=nq * HD * 4)
+    for pos in (at - 1, at, n - 1):
+        hv.attn_decode_q8(Dev(q[0]), kv, ctx, Dev(np.array([SCALE])), i32(pos), nq, HD, group, cap,
+                          s)
+        got = ctx.get(F32, (nq, HD))
+        gone = lost & (pos >= at)
+        assert np.isnan(got[gone]).all()
+        want, tol = R.attention(q[0], clean, pos, group, float(SCALE))
+        near(got[~gone], want[~gone], tol[~gone])
