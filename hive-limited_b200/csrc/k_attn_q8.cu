@@ -12,6 +12,7 @@
 #include "attn_q8.cuh"
 #include "attn_q8_rows.h"
 #include "hv_internal.h"
+#include "q8_ring.h"
 
 namespace hv {
 namespace {
@@ -23,7 +24,7 @@ namespace {
 // blocks in turn, the 8 KB of codes of kDecStages blocks on their way. For short caches they come
 // by 16-byte asynchronous copies, a lane copying exactly the bytes it will multiply, for long ones
 // (kLong) by one bulk copy a block, with barriers of each warp's own whose waits are bounded (one
-// that runs out leaves NaN): 1000 positions 6.8 us and 7.1, 131072 positions 54.2 and 49.8.
+// that runs out leaves NaN in the head's context, and what is under way is waited for: q8_ring.h): 1000 positions 6.8 us and 7.1, 131072 positions 54.2 and 49.8.
 // Both products keep the codes as the 16-row operand and the group's queries as the 8
 // columns: S^T = K q^T, then ctx^T += V^T w^T. With up to four heads in the group the columns
 // are the four hi and the four lo terms (kTwo = false); with five to eight, hi and lo are two
@@ -240,11 +241,16 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
     }
   }
 
-  int stage = 0, phase = 0, given_up = 0;
-  for (int b = b0 + warp; b < b1; b += kDecWarps) {
-    // after a wait that ran out nothing is fetched any more; what is under way is waited for
-    if constexpr (kLong) bar_wait_warp(full + 8 * stage, phase, &given_up);
-    else asm volatile("cp.async.wait_group %0;" :: "n"(kDecStages - 1) : "memory");
+  auto wait = [&](int stage, int parity) {
+    if constexpr (kLong) {
+      int given_up = 0;                          // each wait has its whole limit
+      return bar_wait_warp(full + 8 * stage, parity, &given_up);
+    } else {
+      asm volatile("cp.async.wait_group %0;" :: "n"(kDecStages - 1) : "memory");
+      return true;
+    }
+  };
+  auto use = [&](int b, int stage) {
     const float2 sc = sc_next;
     if (b + kDecWarps < b1) sc_next = __ldg(scales + b + kDecWarps);
     const uint8_t* blk = ring + stage * 2 * kQ8Codes;
@@ -335,11 +341,9 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       for (int k = 0; k < 4; ++k) acc[u][k] = fmaf(d[k], k & 1 ? v1 : v0, acc[u][k]);
     }
     if (kLong) __syncwarp();
-    if (!given_up) fetch(b + kDecStages * kDecWarps, stage);
-    stage = stage + 1 == kDecStages ? 0 : stage + 1;
-    phase ^= stage == 0;
-  }
-  if (given_up) l0 = l1 = __int_as_float(0x7fc00000);
+  };
+  if (!ring_walk<kDecStages>(b0 + warp, b1, kDecWarps, wait, fetch, use))
+    l0 = l1 = __int_as_float(0x7fc00000);        // in every lane, so in every head
 
 #pragma unroll
   for (int o = 4; o < 32; o <<= 1) {
