@@ -87,10 +87,13 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
   const uint8_t* ring = smem + (size_t)warp * kDecStages * 2 * kQ8Codes + 16 * lane;
   const uint32_t ring_s = (uint32_t)__cvta_generic_to_shared(ring);
   const uint32_t full = (uint32_t)__cvta_generic_to_shared(&s_full[warp][0]);
-  if (kLong && lane == 0) {
+  if constexpr (kLong) {
+    if (lane == 0) {
 #pragma unroll
-    for (int i = 0; i < kDecStages; ++i) bar_init(full + 8 * i, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      for (int i = 0; i < kDecStages; ++i) bar_init(full + 8 * i, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();                                // the other lanes wait on them, too
   }
   auto fetch = [&](int b, int stage) {
     const uint8_t* src = codes + (size_t)b * 2 * kQ8Codes;
