@@ -157,3 +157,58 @@ def test_open_rows_that_are_not_finite_lose_the_whole_context(hv, nkv, group, ca
         assert np.isnan(got[gone]).all()
         want, tol = R.attention(q[0], clean, pos, group, float(SCALE))
         near(got[~gone], want[~gone], tol[~gone])
+
+
+@pytest.mark.parametrize("nkv,group,cap", [(8, 8, 13000), (1, 5, 40000), (2, 6, 20000),
+                                           (3, 7, 12321), (2, 4, 20000)])
+def test_decode_over_caches_too_long_for_a_cluster(hv, nkv, group, cap):
+    """The form with bulk copies, whose chunks meet in the scratch, at any length of the cache."""
+    nq = nkv * group
+    g = np.random.default_rng(56)
+    k, v = rows(g, cap, nkv, 0.3)
+    ref = R.Cache(nkv, cap)
+    s, at = scratch(hv, nq, group, cap), 0
+    for n in (1, 32, 45, 300, 4225, cap):
+        ref.write(k[at:n], v[at:n], at)
+        at = n
+        kv, q, ctx = Dev(ref.buffer(0xFF)), queries(g, ref, 1, nq), Dev(nbytes=nq * HD * 4)
+        for pos in sorted({n - 1, n // 2}):
+            hv.attn_decode_q8(Dev(q), kv, ctx, Dev(np.array([SCALE])), i32(pos), nq, HD, group,
+                              cap, s)
+            near(ctx.get(F32, (nq, HD)), *R.attention(q[0], ref.val, pos, group, float(SCALE)))
+
+
+def test_engine_decodes_past_16384_positions(hv):
+    """A group of 5 query heads over a cache beyond the reference-order attention's reach: the last
+    layer's context against its cache as read back, over the edge of 16384 and of a block."""
+    import limited
+    import synth
+    import w4format
+    cfg = w4format.Config(synth.tiny_arch(hidden=256, n_head=10, n_kv=2))
+    n, cap = 16381, 16500
+    e = limited.Engine(config=cfg, tensors=synth.iter_tensors(cfg, 4), quiet=True, max_context=cap,
+                       kv_dtype="q8", fused=False)
+    try:
+        g = np.random.default_rng(57)
+        for kv in e.KC:
+            k, v = rows(g, n, cfg.n_kv, 0.3)
+            hv.kv_rows_q8(Dev(k), Dev(v), cfg.n_kv * HD, kv, 0, cfg.n_kv, HD, cap, n)
+        e._set_i32(e.d_pos, n)
+        e._set_i32(e.d_tok, 7)
+        e._set_i32(e.d_step, 0)
+        for pos in range(n, n + 8):
+            e._step_eager()
+            hv.synchronize()
+            assert np.isfinite(e.download_logits()).all()
+            if pos in (n, 16383, 16384, n + 7):
+                ko, vo = (Dev(nbytes=(pos + 1) * cfg.n_kv * HD * 4) for _ in range(2))
+                hv.kv_read_q8(e.KC[-1], ko, vo, 0, cfg.n_kv, HD, cap, pos + 1)
+                val = np.stack([x.get(F32, (pos + 1, cfg.n_kv, HD)) for x in (ko, vo)]).swapaxes(1, 2)
+                q = e._download(e.d_qkv, (cfg.n_head, HD), F32)
+                near(e._download(e.d_ctx, (cfg.n_head, HD), F32),
+                     *R.attention(q, val, pos, cfg.group, float(e.attn_scale)))
+            e._argmax_into_next()
+        hv.synchronize()
+        assert e._get_i32(e.d_pos) == n + 8
+    finally:
+        e.free()
