@@ -1024,20 +1024,19 @@ class Engine:
 
     # ---- scoring ------------------------------------------------------------------------
 
-    def _score_buffers(self, rows: int, top: int) -> dict:
-        """Device buffers of one scored run (allocated on first use; the alternatives' part
-        grows when a later call wants more of them)."""
-        sc = self._sc
-        if sc is None:
-            sc = self._sc = {"top": -1, "logits": self._alloc(rows * self.n_head_rows * 4),
-                             "lp": self._alloc(rows * 4), "ent": self._alloc(rows * 4),
-                             "tok": self._alloc(rows * 4)}
-        if top > sc["top"]:
-            nb = hvdrv.logprob_scratch(rows, self.n_head_rows, top)
-            sc.update(top=top, id=self._alloc(rows * top * 4), alt=self._alloc(rows * top * 4),
-                      scratch=self._alloc(nb))
+    def _score_buffers(self, rows: int) -> dict:
+        """Device buffers of one scored run with any number of alternatives (allocated on first
+        use)."""
+        if self._sc is None:
+            n, top = self.n_head_rows, min(32, self.n_head_rows)
+            nb = hvdrv.logprob_scratch(rows, n, top)
+            sc = {"logits": self._alloc(rows * n * 4), "lp": self._alloc(rows * 4),
+                  "ent": self._alloc(rows * 4), "tok": self._alloc(rows * 4),
+                  "id": self._alloc(rows * top * 4), "alt": self._alloc(rows * top * 4),
+                  "scratch": self._alloc(nb)}
             hvdrv.memset8(sc["scratch"], 0, nb)
-        return sc
+            self._sc = sc
+        return self._sc
 
     def score(self, ids, top: int = 0) -> dict:
         """How likely the model finds the text `ids`: for every position i from 1 on, the log
@@ -1059,7 +1058,7 @@ class Engine:
         if not 0 <= top <= min(32, c.vocab):
             raise ValueError(f"top={top}: 0 to {min(32, c.vocab)} alternatives")
         pf = self._prefill_buffers()
-        sc = self._score_buffers(pf["n"], top)
+        sc = self._score_buffers(pf["n"])
         s, v = self._stream_cur, self.n_head_rows
         out = {"logprob": np.empty(n - 1, F32), "entropy": np.empty(n - 1, F32),
                "top_ids": np.empty((n - 1, top), np.int32),
