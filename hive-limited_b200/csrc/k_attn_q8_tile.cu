@@ -29,12 +29,12 @@
 // memory: a weight enters as w s_v, that is 2^(x + log2 s_v), and the maximum that the row
 // keeps is that of these products, so that a block with a large scale that the row hardly
 // attends to does not cost the others precision; the sum of the weights adds w s_v / s_v.
-// Weights stand as 2^15 times themselves, exact to 2^-40 of the row's largest w s_v. Where a block's
-// largest is under 2^-64 of that, its weights would be lost to the sum too: they are added up apart,
-// without the scale, by a maximum of their own, and leave the tile's scores. So do those of a block
-// of which the row sees no V but zeros, whose w s_v stands for nothing. Only a chunk whose
-// scales are 2^30 apart, or that may have zeros, looks for them. At its end all goes by one power of two of the sum of the
-// weights.
+// Weights stand as 2^15 times themselves, exact to 2^-40 of the row's largest w s_v.
+// Where a block's largest is under 2^-64 of that, its weights would be lost to the sum too: they
+// are added up apart, without the scale, by a maximum of their own, and leave the tile's scores. So
+// do those of a block of which the row sees no V but zeros, whose w s_v stands for nothing. Only
+// chunks whose scales are 2^30 apart, or 1 as those of zeros are, and tiles where a row sees part of
+// a block look for them. At a chunk's end all goes by one power of two of the sum of the weights.
 // The open block's f32 rows are two binary16 terms: after the tile's products with the first
 // term, the same buffer holds the second one (zero elsewhere) for one product more. Each of its
 // rows has a power of two of its own, so that no row, least of all one that a query does not see,
@@ -417,6 +417,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       const int see0 = lim - 32 * (b0 + 4 * i);            // positions 0 .. see0 are seen
       const bool all = __all_sync(0xFFFFFFFFu, see0 >= kTlRows - 1);
       const float (&sc)[4][4] = sh.sc[i & 3];
+      const int (&first)[4] = sh.first[i & 3];
+      bool look = far;
       if (!all) {
         // columns of positions that the row does not see become -infinity
 #pragma unroll 1
@@ -433,13 +435,16 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
           tmem_st16(s_at + 16 * h, x);
         }
         tmem_st_wait();
+        bool zeros = false;                                 // are they all that the row sees of a block?
+#pragma unroll
+        for (int b = 0; b < 4; ++b) zeros |= see0 >= 32 * b && see0 < 32 * b + first[b];
+        look |= __any_sync(0xFFFFFFFFu, zeros) != 0;
       }
       // The largest exponent of the row in this tile. Here and below loops stay as rolled as
       // the two buffers allow: the code of all roles has to fit the instruction cache.
       uint32_t v[2][32];
       const bool tail = has_tail && i == nt - 1;
       const int ob = tail ? (nb - b0) & 3 : -1;             // the open block
-      bool look = far;
       if (tail) {
         const float f = sc[ob][3] * qs;
         float most = -INFINITY;
@@ -493,7 +498,6 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         if (see >= 0) up = fmaxf(up, fmaf(fmaxf(mx[0], mx[2]), sc[b][0] * qs0, sc[b][1]));
         if (see >= 32) up = fmaxf(up, fmaf(fmaxf(mx[1], mx[3]), sc[b + 1][0] * qs1, sc[b + 1][1]));
       }
-      const int (&first)[4] = sh.first[i & 3];
       if (__builtin_expect(look, 0)) {                      // the largest again, without zeros
         up = m;
 #pragma unroll 1

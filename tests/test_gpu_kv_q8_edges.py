@@ -212,3 +212,21 @@ def test_engine_decodes_past_16384_positions(hv):
         assert e._get_i32(e.d_pos) == n + 8
     finally:
         e.free()
+
+
+@pytest.mark.parametrize("nkv,group,pos0,ntok", [(8, 5, 11, 231), (8, 8, 30, 220), (2, 4, 60, 40),
+                                                 (2, 3, 81, 1)])
+def test_zeros_that_are_all_a_row_sees_of_a_block(hv, nkv, group, pos0, ntok):
+    """The first rows of a block are zeros that the queries look for; the rest of it, of the usual
+    size, is behind the queries. What little weight the other blocks have is theirs in full."""
+    n = pos0 + ntok
+    g = np.random.default_rng(58)
+    k, v = rows(g, n, nkv, 0.3)
+    v[64:82] = 0
+    ref = R.Cache(nkv, n + 9)
+    ref.write(k, v, 0)
+    q = np.repeat(ref.val[0, :, 75], group, 0)[None].repeat(ntok, 0) * 1.5
+    q = (q + 0.3 * g.standard_normal(q.shape)).astype(F32)
+    got = run(hv, ref, q, pos0, group)
+    for t in some(ntok, *(p - pos0 for p in (75, 76, 80, 81, 82, 95, 96))):
+        near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
