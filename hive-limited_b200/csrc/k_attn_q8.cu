@@ -644,7 +644,9 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       for (int d = 0; d < 16; ++d) { acc[d][0] *= a0; acc[d][1] *= a0; acc[d][2] *= a1; acc[d][3] *= a1; }
     }
     if constexpr (decltype(is_open)::value) {
-      // the sum of the weights by the scores, the weights by w v
+      // The sum of the weights by the scores, the weights by w v. A V row's exponent is a whole
+      // number, of which a whole number near the largest w v is taken before a score is added, so
+      // that the score keeps its bits.
       const float n0 = m0 == -INFINITY ? 0.0f : m0, n1 = m1 == -INFINITY ? 0.0f : m1;
       y0 = y1 = -INFINITY;
 #pragma unroll
@@ -654,10 +656,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
           l0 += ex2(s[j][e] - n0) * 32768.0f;
           l1 += ex2(s[j][2 + e] - n1) * 32768.0f;
           const float up = __shfl_sync(0xFFFFFFFFu, v_up, 8 * j + 2 * t + e);
-          s[j][e] += up;
-          s[j][2 + e] += up;
-          y0 = fmaxf(y0, s[j][e]);
-          y1 = fmaxf(y1, s[j][2 + e]);
+          y0 = fmaxf(y0, s[j][e] + up);
+          y1 = fmaxf(y1, s[j][2 + e] + up);
         }
       }
 #pragma unroll
@@ -665,12 +665,28 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
         y0 = fmaxf(y0, __shfl_xor_sync(0xFFFFFFFFu, y0, o));
         y1 = fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, o));
       }
+      const float e0 = y0 == -INFINITY ? 0.0f : ceilf(y0), e1 = y1 == -INFINITY ? 0.0f : ceilf(y1);
+      const float c0 = ceilf(n0), c1 = ceilf(n1);
+      // 2^16 times what they are, which the sums (up to 2^35) lack
+      g0 = y0 == -INFINITY ? 0.0f : ex2(e0 - c0 + 16.0f) * ex2(c0 - n0);
+      g1 = y1 == -INFINITY ? 0.0f : ex2(e1 - c1 + 16.0f) * ex2(c1 - n1);
+      y0 = y1 = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float up = __shfl_sync(0xFFFFFFFFu, v_up, 8 * j + 2 * t + e);
+          s[j][e] += up - e0;
+          s[j][2 + e] += up - e1;
+        }
+      }
+    } else {
+      // a row that sees none of the block's positions has y = -inf and weights of 0
+      g0 = y0 == -INFINITY ? 0.0f : ex2(y0 - m0);
+      g1 = y1 == -INFINITY ? 0.0f : ex2(y1 - m1);
+      if (y0 == -INFINITY) y0 = 0.0f;
+      if (y1 == -INFINITY) y1 = 0.0f;
     }
-    // a row that sees none of the block's positions has y = -inf and weights of 0
-    g0 = y0 == -INFINITY ? 0.0f : ex2(y0 - m0);
-    g1 = y1 == -INFINITY ? 0.0f : ex2(y1 - m1);
-    if (y0 == -INFINITY) y0 = 0.0f;
-    if (y1 == -INFINITY) y1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float p[4];
@@ -781,7 +797,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            acc[2 * u + h][i] = fmaf(d[i], i < 2 ? g0 : g1, acc[2 * u + h][i]);
+            acc[2 * u + h][i] = fmaf(d[i] * 0x1p-16f, i < 2 ? g0 : g1, acc[2 * u + h][i]);
         }
       }
       if (lim0 >= closed * kQ8Blk + s_bad) l0 = __int_as_float(0x7fc00000);

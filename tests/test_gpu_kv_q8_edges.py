@@ -230,3 +230,28 @@ def test_zeros_that_are_all_a_row_sees_of_a_block(hv, nkv, group, pos0, ntok):
     got = run(hv, ref, q, pos0, group)
     for t in some(ntok, *(p - pos0 for p in (75, 76, 80, 81, 82, 95, 96))):
         near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
+
+
+@pytest.mark.parametrize("nkv,group,pos0,ntok", [(8, 7, 1, 13), (8, 5, 6, 11), (1, 2, 0, 28),
+                                                 (2, 4, 26, 1), (2, 8, 96, 29)])
+def test_few_open_rows_of_every_size(hv, nkv, group, pos0, ntok):
+    """V from 1e-28 to 1e28, row by row, and all of it tiny behind a zero that has the weight."""
+    n = pos0 + ntok
+    for seed in range(8):
+        g = np.random.default_rng(600 + seed)
+        k, v = rows(g, n, nkv, 0.3)
+        if seed < 4:
+            v *= (10.0 ** g.uniform(-28, 28, n)).astype(F32)[:, None, None]
+        else:
+            v *= F32(2e-27)
+            v[0] = 0
+        ref = R.Cache(nkv, n + 9)
+        ref.write(k, v, 0)
+        q = queries(g, ref, ntok, nkv * group)
+        if seed < 4:
+            q[:, ::3] = 0
+        else:
+            q = (np.repeat(ref.val[0, :, 0], group, 0)[None].repeat(ntok, 0) * 1.2 + 0.2 * q).astype(F32)
+        got = run(hv, ref, q, pos0, group)
+        for t in range(ntok):
+            near(got[t], *R.attention(q[t], ref.val, pos0 + t, group, float(SCALE)))
