@@ -1133,6 +1133,8 @@ extern "C" int hv_attn_q8_scratch(int nq, int group, int cap, int ntok, size_t* 
   HV_REQUIRE(nq > 0 && group > 0 && nq % group == 0 && cap > 0 && ntok > 0 && bytes,
              HV_E_INVALID, "hv_attn_q8_scratch: bad arguments");
   HV_REQUIRE(group <= 8, HV_E_UNSUPPORTED, "hv_attn_q8_scratch: group size %d (1 to 8)", group);
+  HV_REQUIRE(nq <= 32768 && cap <= (1 << 30) && ntok <= 65535, HV_E_UNSUPPORTED,
+             "hv_attn_q8_scratch: %d heads, %d positions, %d rows", nq, cap, ntok);
   int nch = 0;
   const int rc = dec_chunks(nq / group, cap, &nch);
   if (rc) return rc;

@@ -493,6 +493,7 @@ extern "C" int hv_logprob_scratch(int rows, int n, int top, size_t* bytes) {
              "hv_logprob_scratch: bad arguments");
   HV_REQUIRE(top <= kMaxTop, HV_E_UNSUPPORTED, "hv_logprob_scratch: %d alternatives (at most %d)",
              top, kMaxTop);
+  HV_REQUIRE(n <= 1 << 30, HV_E_UNSUPPORTED, "hv_logprob_scratch: %d tokens", n);
   int pieces = 0;
   long long most = 0;
   const int rc = lp_pieces(rows, n, &pieces, &most);

@@ -118,3 +118,9 @@ def test_engine_refuses_the_fused_step_over_q8():
         limited.Engine(config=synth.tiny_arch(), tensors={}, kv_dtype="q8")
     with pytest.raises(ValueError, match="kv_dtype"):
         limited.Engine(config=synth.tiny_arch(), tensors={}, kv_dtype="q4")
+
+
+def test_scratch_sizes_refuse_what_their_calls_refuse():
+    for a in ((32769, 1, 64, 1), (8, 4, (1 << 30) + 1, 1), (8, 4, 0x7FFFFFFF, 4), (8, 4, 64, 65536)):
+        refused(UNSUPPORTED, hvdrv.attn_q8_scratch, *a)
+    refused(UNSUPPORTED, hvdrv.logprob_scratch, 1, (1 << 30) + 1, 0)
