@@ -402,7 +402,10 @@ __global__ void k_gather(const __half* __restrict__ emb, const int32_t* __restri
 // ---------------------------------------------------------------------------
 // argmax_p / argmax_f: first maximal index
 // ---------------------------------------------------------------------------
+// As np.argmax: a NaN is above all, so that logits without a number still name a token of the
+// vocabulary (the next step gathers its row).
 HV_DEV bool better(float v, int i, float bv, int bi) {
+  if (v != v || bv != bv) return v != v && (bv == bv || i < bi);
   return v > bv || (v == bv && i < bi);
 }
 
