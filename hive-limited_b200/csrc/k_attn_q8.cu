@@ -34,6 +34,7 @@ namespace {
 // 131072 positions of 8 heads x 4 queries (269 MB) take 51 us, 5.3 TB/s, 80% of a plain copy's
 // rate: 60000 and 131072 positions differ by what their bytes take, and 9 us are there whatever
 // the length, the launch, the first blocks' way and the two joins. 4225 take 8.4 us in a graph.
+constexpr float kLowest = -3e38f;      // finite, so that scores of -infinity are that less it
 constexpr int kDecWarps = 8;
 constexpr int kDecStages = 2;
 constexpr int kDecBlocksMin = 8;       // of a chunk, one a warp (1000 positions: 4 6.4 us, 8 6.8, 12 7.7, 16 8.0)
@@ -212,15 +213,12 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       const int r = warp + kDecWarps * i;
       x0[i] = r < ntail && head0 < group ? s_x[r][head0] : -INFINITY;
       x1[i] = r < ntail && head0 + 1 < group ? s_x[r][head0 + 1] : -INFINITY;
-      if (r >= ntail) continue;
       // a row with a value that is not finite loses all of the context, as a complete block does
       const float4 k = *reinterpret_cast<const float4*>(open_k + r * kDecLine + 4 * lane);
       const float4 v = *reinterpret_cast<const float4*>(open_v + r * kHd + 4 * lane);
-      const float e[8] = {k.x, k.y, k.z, k.w, v.x, v.y, v.z, v.w};
-      bool fine = true;
-#pragma unroll
-      for (int d = 0; d < 8; ++d) fine = fine && fabsf(e[d]) < INFINITY;
-      if (!__all_sync(0xFFFFFFFFu, fine)) x0[i] = x1[i] = __int_as_float(0x7fc00000);
+      const float most = q8_max(q8_max(q8_max(k.x, k.y), q8_max(k.z, k.w)),
+                                q8_max(q8_max(v.x, v.y), q8_max(v.z, v.w)));
+      if (__any_sync(0xFFFFFFFFu, r < ntail && !(most < INFINITY))) x0[i] = x1[i] = __int_as_float(0x7fc00000);
     }
     raise(fmaxf(fmaxf(x0[0], x0[1]), fmaxf(x0[2], x0[3])),
           fmaxf(fmaxf(x1[0], x1[1]), fmaxf(x1[2], x1[3])));
@@ -302,19 +300,19 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
       y0 = fmaxf(y0, __shfl_xor_sync(0xFFFFFFFFu, y0, o));
       y1 = fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, o));
     }
-    raise(y0, y1);
+    // (a block of scores of -infinity has weights of 0)
+    y0 = fmaxf(y0, kLowest);
+    y1 = fmaxf(y1, kLowest);
     // Weights as 2^15 times what they are to the block's largest, so that the lo terms of small
     // ones stay above binary16's smallest: a weight is exact to 2^-40 of its block's largest, and
     // a block that is hardly attended to counts in full where its values are large.
-    const float g0 = y0 == -INFINITY ? 0.0f : ex2(y0 - m0), g1 = y1 == -INFINITY ? 0.0f : ex2(y1 - m1);
-    if (y0 == -INFINITY) y0 = 0.0f;
-    if (y1 == -INFINITY) y1 = 0.0f;
+    float sum0 = 0.0f, sum1 = 0.0f;
     uint32_t wh[4], wl[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float p0 = ex2(x0[j] - y0) * 32768.0f, p1 = ex2(x1[j] - y1) * 32768.0f;
-      l0 = fmaf(p0, g0, l0);
-      l1 = fmaf(p1, g1, l1);
+      sum0 += p0;
+      sum1 += p1;
       uint32_t hi, lo;
       split_half2(p0, p1, &hi, &lo);
       if (kTwo) {
@@ -324,6 +322,10 @@ __global__ void __launch_bounds__(32 * kDecWarps, 1)
         wh[j] = transpose_8x8(t < 2 ? hi : lo);
       }
     }
+    raise(y0, y1);                               // here, so that the weights do not wait for it
+    const float g0 = ex2(y0 - m0), g1 = ex2(y1 - m1);
+    l0 = fmaf(sum0, g0, l0);
+    l1 = fmaf(sum1, g1, l1);
     const float v0 = sc.y * g0, v1 = sc.y * g1;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -511,7 +513,10 @@ template <int kWM, bool kMeet>
 __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, KvQ8 c) {
   using Cfg = RowsCfg<kWM>;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float s_m[kRowWarps][16], s_l[kRowWarps][16], s_amax[2][kQ8Blk];
+  __shared__ float s_m[kRowWarps][16], s_l[kRowWarps][16], s_amax[2][kQ8Blk], s_lift[2][kQ8Blk];
+  // of the open rows: what a score takes after the largest row's power of two, what V lacks
+  __shared__ __align__(8) float s_down[kQ8Blk], s_up[kQ8Blk];
+  __shared__ float s_most;              // that power of two
   __shared__ int s_bad;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
   const int wm = warp % kWM, share = warp / kWM;
@@ -611,7 +616,17 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
   // g0 (g1) of the row's.
   uint32_t wh[2][4], wl[2][4];
   float g0, g1;
-  float v_up = 0.0f;                // of open row `lane`: the exponent that its V lacks, -inf for zeros
+  auto raise = [&](float y0, float y1) {         // a larger maximum: what was summed so far counts less
+    if (__any_sync(0xFFFFFFFFu, y0 > m0 || y1 > m1)) {
+      const float n0 = fmaxf(m0, y0), n1 = fmaxf(m1, y1);
+      const float a0 = m0 == -INFINITY ? 0.0f : ex2(m0 - n0);
+      const float a1 = m1 == -INFINITY ? 0.0f : ex2(m1 - n1);
+      m0 = n0; m1 = n1;
+      l0 *= a0; l1 *= a1;
+#pragma unroll
+      for (int d = 0; d < 16; ++d) { acc[d][0] *= a0; acc[d][1] *= a0; acc[d][2] *= a1; acc[d][3] *= a1; }
+    }
+  };
   auto weights = [&](int b, float (&s)[4][4], float f0, float f1, auto is_open) {
     const bool cut = 32 * b + 31 > warp_low;
     float y0 = -INFINITY, y1 = -INFINITY;
@@ -634,16 +649,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
     y1 = fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, 1));
     y0 = fmaxf(y0, __shfl_xor_sync(0xFFFFFFFFu, y0, 2));
     y1 = fmaxf(y1, __shfl_xor_sync(0xFFFFFFFFu, y1, 2));
-    if (__any_sync(0xFFFFFFFFu, y0 > m0 || y1 > m1)) {
-      const float n0 = fmaxf(m0, y0), n1 = fmaxf(m1, y1);
-      const float a0 = m0 == -INFINITY ? 0.0f : ex2(m0 - n0);
-      const float a1 = m1 == -INFINITY ? 0.0f : ex2(m1 - n1);
-      m0 = n0; m1 = n1;
-      l0 *= a0; l1 *= a1;
-#pragma unroll
-      for (int d = 0; d < 16; ++d) { acc[d][0] *= a0; acc[d][1] *= a0; acc[d][2] *= a1; acc[d][3] *= a1; }
-    }
     if constexpr (decltype(is_open)::value) {
+      raise(y0, y1);
       // The sum of the weights by the scores, the weights by w v. A V row's exponent is a whole
       // number, of which a whole number near the largest w v is taken before a score is added, so
       // that the score keeps its bits.
@@ -655,7 +662,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
         for (int e = 0; e < 2; ++e) {
           l0 += ex2(s[j][e] - n0) * 32768.0f;
           l1 += ex2(s[j][2 + e] - n1) * 32768.0f;
-          const float up = __shfl_sync(0xFFFFFFFFu, v_up, 8 * j + 2 * t + e);
+          const float up = s_up[8 * j + 2 * t + e];
           y0 = fmaxf(y0, s[j][e] + up);
           y1 = fmaxf(y1, s[j][2 + e] + up);
         }
@@ -675,18 +682,16 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float up = __shfl_sync(0xFFFFFFFFu, v_up, 8 * j + 2 * t + e);
+          const float up = s_up[8 * j + 2 * t + e];
           s[j][e] += up - e0;
           s[j][2 + e] += up - e1;
         }
       }
     } else {
-      // a row that sees none of the block's positions has y = -inf and weights of 0
-      g0 = y0 == -INFINITY ? 0.0f : ex2(y0 - m0);
-      g1 = y1 == -INFINITY ? 0.0f : ex2(y1 - m1);
-      if (y0 == -INFINITY) y0 = 0.0f;
-      if (y1 == -INFINITY) y1 = 0.0f;
+      y0 = fmaxf(y0, kLowest);                   // a row that sees nothing of the block has weights of 0
+      y1 = fmaxf(y1, kLowest);
     }
+    float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float p[4];
@@ -694,14 +699,19 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       for (int e = 0; e < 2; ++e) {
         p[e] = ex2(s[j][e] - y0) * 32768.0f;
         p[2 + e] = ex2(s[j][2 + e] - y1) * 32768.0f;
-        if constexpr (!decltype(is_open)::value) {
-          l0 = fmaf(p[e], g0, l0);
-          l1 = fmaf(p[2 + e], g1, l1);
-        }
+        sum0 += p[e];
+        sum1 += p[2 + e];
       }
       // A fragment: (row g, k 2t), (row g + 8, k 2t), (row g, k 2t + 8), (row g + 8, k 2t + 8)
       split_half2(p[0], p[1], &wh[j >> 1][2 * (j & 1)], &wl[j >> 1][2 * (j & 1)]);
       split_half2(p[2], p[3], &wh[j >> 1][2 * (j & 1) + 1], &wl[j >> 1][2 * (j & 1) + 1]);
+    }
+    if constexpr (!decltype(is_open)::value) {
+      raise(y0, y1);
+      g0 = ex2(y0 - m0);
+      g1 = ex2(y1 - m1);
+      l0 = fmaf(sum0, g0, l0);
+      l1 = fmaf(sum1, g1, l1);
     }
   };
 
@@ -725,16 +735,27 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
         else atomicMin(&s_bad, at);
       }
       const unsigned top = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(amax));
-      if (lane == 0) s_amax[which][at] = __uint_as_float(top);
+      if (lane == 0) {
+        s_amax[which][at] = __uint_as_float(top);
+        s_lift[which][at] = q8_lift(__uint_as_float(top));
+      }
     }
     __syncthreads();
+    if (warp == kRowWarps - 1) {
+      // the scores by the largest row's power of two: the others' sums fall, and none overflows
+      const float k = s_amax[0][lane], v = s_amax[1][lane];
+      const float most = q8_lift(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(k))));
+      s_down[lane] = k > 0.0f ? most / q8_lift(k) : 0.0f;
+      s_up[lane] = v > 0.0f ? (float)(127 - (int)(__float_as_uint(q8_lift(v)) >> 23)) : -INFINITY;
+      if (lane == 0) s_most = most;
+    }
     auto term = [&](float x, float lift) { return fabsf(x) < INFINITY ? x * lift : 0.0f; };
     // four dims of a K row are neighbours in a fragment, two rows of a V dim
     for (int i = threadIdx.x; i < kQ8Codes / 4; i += blockDim.x) {
       const int r = i / (kHd / 4), d = 4 * (i % (kHd / 4));
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
       if (r < nopen) x = *reinterpret_cast<const float4*>(open + r * kHd + d);
-      const float lk = q8_lift(s_amax[0][r]);
+      const float lk = r < nopen ? s_lift[0][r] : 0.0f;
       uint2 hi, lo;
       split_half2(term(x.x, lk), term(x.y, lk), &hi.x, &lo.x);
       split_half2(term(x.z, lk), term(x.w, lk), &hi.y, &lo.y);
@@ -745,8 +766,8 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
       const int r = 2 * (i / kHd), d = i % kHd;
       const float* v = open + kQ8Codes + r * kHd + d;
       uint32_t hi, lo;
-      split_half2(r < nopen ? term(v[0], q8_lift(s_amax[1][r])) : 0.0f,
-                  r + 1 < nopen ? term(v[kHd], q8_lift(s_amax[1][r + 1])) : 0.0f, &hi, &lo);
+      split_half2(r < nopen ? term(v[0], s_lift[1][r]) : 0.0f,
+                  r + 1 < nopen ? term(v[kHd], s_lift[1][r + 1]) : 0.0f, &hi, &lo);
       *reinterpret_cast<uint32_t*>(frag + 2 * kQ8Codes + q8_v_at(r, d)) = hi;
       *reinterpret_cast<uint32_t*>(frag + 3 * kQ8Codes + q8_v_at(r, d)) = lo;
     }
@@ -768,21 +789,15 @@ __global__ void __launch_bounds__(32 * kRowWarps, 1) k_attn_rows_q8(RowsArgs a, 
           mma_f16(s[j], qh[k], kl.x, kl.y);
         }
       }
-      // the scores by the largest row's power of two: the others' sums fall, and none overflows
-      const float k_max = s_amax[0][lane], v_max = s_amax[1][lane];
-      const float lk = q8_lift(__uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(k_max))));
-      const float k_down = k_max > 0.0f ? lk / q8_lift(k_max) : 0.0f;
-      if (v_max == 0.0f) v_up = -INFINITY;
-      else v_up = (float)(127 - (int)(__float_as_uint(q8_lift(v_max)) >> 23));
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float f = __shfl_sync(0xFFFFFFFFu, k_down, 8 * j + 2 * t + e);
+          const float f = s_down[8 * j + 2 * t + e];
           s[j][e] *= f;
           s[j][2 + e] *= f;
         }
-      weights(closed, s, qs0 / lk, qs1 / lk, std::true_type{});
+      weights(closed, s, qs0 / s_most, qs1 / s_most, std::true_type{});
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
 #pragma unroll

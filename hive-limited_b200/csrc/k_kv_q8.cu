@@ -35,12 +35,6 @@ struct Q8Src {
 // 4-byte pieces of K and 2-byte pieces of V fall on different banks (two to a bank for V).
 constexpr int kKUnit = 576, kVUnit = 528;
 
-HV_DEV float q8_max(float a, float b) {          // the larger magnitude; NaN if either is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
-  return r;
-}
-
 // Row `t` of the call for head g as a float4 per lane (dims 4 lane ..). One warp.
 template <bool kNorm>
 HV_DEV float4 q8_row(const Q8Src& s, int which, int g, int t, int pos, float* tmp) {

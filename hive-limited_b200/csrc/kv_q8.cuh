@@ -71,6 +71,12 @@ HV_DEV float q8_value(uint32_t biased, float s) {   // 2^23 + code + 128 as a fl
   return __fmul_rn(__fsub_rn(__uint_as_float(0x4B000000u | biased), 8388608.0f + 128.0f), s);
 }
 
+HV_DEV float q8_max(float a, float b) {          // the larger magnitude; NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+  return r;
+}
+
 // Positions the cache holds for kv head g: those both K and V have.
 HV_DEV int q8_held(const KvQ8& c, int g) {
   const int2 h = __ldg(reinterpret_cast<const int2*>(c.held) + g);
