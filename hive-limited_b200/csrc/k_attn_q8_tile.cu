@@ -48,6 +48,8 @@
 // 1.01 and 0.76 PFLOP/s of issued products, 61% and 46% of a large library product's rate. A
 // tile's weights (two exponent passes over 128 columns a thread) take about as long as its
 // products; two lanes of work hide the one behind the other, but not the ends of a chunk.
+#include <type_traits>
+
 #include "attn_q8.cuh"
 #include "attn_q8_rows.h"
 #include "hv_internal.h"
@@ -405,20 +407,16 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       }
       return big;
     };
-#pragma unroll 1
-    for (int i = w;; i += 2) {
-      if (issues) {
-        if (i >= 2) product_o(i - 2);
-        if (i < nt) product_s(i);
-      }
-      if (i >= nt) break;
-      if (!bar_wait_warp(bar(sh.s_ready[w]), (i >> 1) & 1, given_up)) break;
-      fence_after();
+    // The weights of tile i. Most tiles are seen whole by every row and have nothing to look for:
+    // those have a form of their own (`whole`), which the rest would slow by their code alone
+    // (16384 positions 266 us with it, 276 without).
+    auto weights = [&](int i, auto whole_form) {
+      constexpr bool whole = decltype(whole_form)::value;
       const int see0 = lim - 32 * (b0 + 4 * i);            // positions 0 .. see0 are seen
-      const bool all = __all_sync(0xFFFFFFFFu, see0 >= kTlRows - 1);
+      const bool all = whole || __all_sync(0xFFFFFFFFu, see0 >= kTlRows - 1);
       const float (&sc)[4][4] = sh.sc[i & 3];
       const int (&first)[4] = sh.first[i & 3];
-      bool look = far;
+      bool look = !whole && far;
       if (!all) {
         // columns of positions that the row does not see become -infinity
 #pragma unroll 1
@@ -443,7 +441,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       // The largest exponent of the row in this tile. Here and below loops stay as rolled as
       // the two buffers allow: the code of all roles has to fit the instruction cache.
       uint32_t v[2][32];
-      const bool tail = has_tail && i == nt - 1;
+      const bool tail = !whole && has_tail && i == nt - 1;
       const int ob = tail ? (nb - b0) & 3 : -1;             // the open block
       if (tail) {
         const float f = sc[ob][3] * qs;
@@ -495,8 +493,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
           }
         }
         const float qs0 = b == ob ? 1.0f : qs, qs1 = b + 1 == ob ? 1.0f : qs;
-        if (see >= 0) up = fmaxf(up, fmaf(fmaxf(mx[0], mx[2]), sc[b][0] * qs0, sc[b][1]));
-        if (see >= 32) up = fmaxf(up, fmaf(fmaxf(mx[1], mx[3]), sc[b + 1][0] * qs1, sc[b + 1][1]));
+        if (whole || see >= 0) up = fmaxf(up, fmaf(fmaxf(mx[0], mx[2]), sc[b][0] * qs0, sc[b][1]));
+        if (whole || see >= 32) up = fmaxf(up, fmaf(fmaxf(mx[1], mx[3]), sc[b + 1][0] * qs1, sc[b + 1][1]));
       }
       if (__builtin_expect(look, 0)) {                      // the largest again, without zeros
         up = m;
@@ -546,7 +544,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         for (int e = 0; e < 2; ++e) {
           // -inf f has to stay -inf: not with a scale of 0, nor with the scales (which may be
           // NaN) of a block that the row sees nothing of
-          const bool seen = see0 >= 32 * (b + e);
+          const bool seen = whole || see0 >= 32 * (b + e);
           float f = seen ? sc[b + e][0] * (b + e == ob ? 1.0f : qs) : 1.0f;
           f = f == 0.0f ? 1e-38f : f;
           const float add = seen ? sc[b + e][1] - m0 : 0.0f;
@@ -583,10 +581,23 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
         l = fmaf(s0.x + s0.y, sc[b][2], l);
         l = fmaf(s1.x + s1.y, sc[b + 1][2], l);
       }
-      if (has_tail && i == nt - 1 && lim >= 32 * closed + sh.bad) l = __int_as_float(0x7fc00000);
+      if (tail && lim >= 32 * closed + sh.bad) l = __int_as_float(0x7fc00000);
       tmem_st_wait();
       fence_before();
       bar_arrive(bar(sh.w_ready[w]));
+    };
+    const int whole_end = far ? 0 : min((b1 - b0) / 4 - (has_tail ? 1 : 0), (a.pos0 + row0 / a.group + 1 - 32 * b0) / kTlRows);
+#pragma unroll 1
+    for (int i = w;; i += 2) {
+      if (issues) {
+        if (i >= 2) product_o(i - 2);
+        if (i < nt) product_s(i);
+      }
+      if (i >= nt) break;
+      if (!bar_wait_warp(bar(sh.s_ready[w]), (i >> 1) & 1, given_up)) break;
+      fence_after();
+      if (i < whole_end) weights(i, std::true_type{});
+      else weights(i, std::false_type{});
     }
     if (issues && !ok) {                          // what was issued ends before the memory goes
       int no = 0;
@@ -874,8 +885,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       const int s = i & 1;
       ok = i < 2 || bar_wait_warp(bar(sh.s_ready[s]), ((i - 2) >> 1) & 1, given_up);
       if (!ok) break;
+      put_coded(i, sc);                         // before the codes (after them 13 us of 278 more)
       coded_k(i, k_buf + s * kTlTile);
-      put_coded(i, sc);
       fence_async();
       bar_arrive(bar(sh.full_k[s]));
       fetch(i + 1, 0, kx);
