@@ -23,21 +23,25 @@ namespace {
 // positions of a kv head are cut into chunks of whole blocks, one CTA each, and a warp takes
 // blocks in turn, the 8 KB of codes of kDecStages blocks on their way. For short caches they come
 // by 16-byte asynchronous copies, a lane copying exactly the bytes it will multiply, for long ones
-// (kLong) by one bulk copy a block, with barriers of each warp's own whose waits are bounded (one
-// that runs out leaves NaN in the head's context, and what is under way is waited for: q8_ring.h): 1000 positions 6.8 us and 7.1, 131072 positions 54.2 and 49.8.
+// (kLong) by one bulk copy a block, with barriers of each warp's own (1000 positions 6.8 us and 7.1
+// in a graph, 131072 positions 54.2 and 49.8). Their waits are bounded: one that runs out leaves NaN
+// in every head's context, and what is under way is waited for (q8_ring.h).
 // Both products keep the codes as the 16-row operand and the group's queries as the 8
 // columns: S^T = K q^T, then ctx^T += V^T w^T. With up to four heads in the group the columns
 // are the four hi and the four lo terms (kTwo = false); with five to eight, hi and lo are two
 // products. Each warp keeps its own running maximum and sums; they meet in shared memory. The
 // chunks of a head meet, added in chunk order, in a cluster's shared memory, or, where a head has
 // more than a cluster's eight (kLong), in the caller's scratch by the last CTA to arrive.
-// 131072 positions of 8 heads x 4 queries (269 MB) take 51 us, 5.3 TB/s, 80% of a plain copy's
-// rate: 60000 and 131072 positions differ by what their bytes take, and 9 us are there whatever
-// the length, the launch, the first blocks' way and the two joins. 4225 take 8.4 us in a graph.
+// 131072 positions of 8 heads x 4 queries (269 MB) take 51 us among other calls, 5.3 TB/s, 80% of
+// a plain copy's rate, and 47 in a graph: 16000 and 131072 positions differ by what their bytes
+// take, and 7 us are there whatever the length, the launch, the first blocks' way and the two joins.
+// 4225 take 8.6 us in a graph.
 constexpr float kLowest = -3e38f;      // finite, so that scores of -infinity are that less it
 constexpr int kDecWarps = 8;
 constexpr int kDecStages = 2;
-constexpr int kDecBlocksMin = 8;       // of a chunk, one a warp (1000 positions: 4 6.4 us, 8 6.8, 12 7.7, 16 8.0)
+// Of a chunk, one a warp. In a graph, 4, 8, 12, 16: 300 positions 6.4, 6.5, 6.5, 6.5 us, 1000 6.3,
+// 6.7, 7.5, 7.8, 2000 7.1, 7.1, 7.6, 8.2, the same from 4225 on: 4 would gain 0.4 us around 1000.
+constexpr int kDecBlocksMin = 8;
 constexpr int kDecStride = 132;        // floats between the columns of a warp's sums
 constexpr int kDecTickets = 1024;      // kv heads with chunks to join: first in the scratch
 constexpr int kDecPart = 8 * (kHd + 2);    // scratch floats of a chunk: sums, then (max, sum)
@@ -492,8 +496,8 @@ int dec_chunks(int nkv, int cap, int* out) {
 // a block like the others with a third product, hi x lo. Each of its rows has a power of two of
 // its own, so that no row, least of all one that a query does not see, takes bits from another:
 // a K row's is taken back from its scores, a V row's goes with its weights.
-// Bound by latency: 44 tokens of 16 heads (8 kv heads) over 300 positions take 11.6 us in a
-// graph, 8 tokens of 32 heads over 38 positions 10.7.
+// Bound by latency: 44 tokens of 16 heads (8 kv heads) over 300 positions take 11.7 us in a
+// graph, 38 tokens of 32 heads over 38 positions 10.3.
 constexpr int kRowWarps = 8;
 
 template <int kWM>
@@ -992,13 +996,15 @@ __global__ void __launch_bounds__(256) k_rows_join_q8(RowsArgs a, KvQ8 c, int ro
 // Rows per CTA and chunks per row tile of a run. The tile kernel (k_attn_q8_tile.cu) pays for
 // filling its tensor memory, its shared memory and a pipeline of five roles, so it takes runs of
 // more than 64 rows a head that have 2^21 (row, position) pairs or more. Tiles of 64 rows here
-// against it, in microseconds, on either side of that: 0.5 M pairs (8 heads x 256 rows over 264
-// positions) 16.0 : 19.5, 1.0 M 17.2 : 22.7, 1.9 M 26.7 : 29.0, 1.9 M 22.4 : 21.1,
-// 2.2 M 28.1 : 27.3, 4.2 M 24.7 : 20.9, 8.3 M 44.1 : 22.7, 16 M 71.8 : 32.6.
+// against it, in microseconds of a graph, on either side of that: 0.5 M pairs (8 heads x 256 rows
+// over 264 positions) 13.7 : 21.7, 1.0 M 12.4 : 14.1, 1.8 M 18.6 : 18.4, 2.2 M (with an open block)
+// 21.8 : 23.9, 4.2 M 23.6 : 19.8, 6.3 M 32.0 : 19.4, 8.4 M 40.3 : 20.8, 17 M 73.7 : 28.6.
 // Up to 64 rows fill at most half of the 128 that a product of the tile kernel has; they take the
 // fewest of 16, 32 or 64 that hold them, whose warps then share the positions: 16 rows in tiles of
-// 16, 32 and 64 over 500 positions 12.7, 12.2, 11.9, over 2000 13.1, 14.4, 18.0, over 16000 23.5,
-// 29.1, 41.4; 32 rows in 32 and 64 over 500 13.5, 12.9, over 2000 15.5, 18.6, over 16000 30.8, 42.6.
+// 16, 32 and 64 over 104 positions 9.8, 10.2, 11.0, over 500 13.0, 12.4, 12.2, over 2000 13.3, 14.5,
+// 18.0, over 16000 20.2, 26.4, 40.4; 32 rows in 32 and 64 over 108 11.4, 12.1, over 500 13.2, 12.9,
+// over 2000 15.7, 18.5, over 16000 27.0, 40.5. What that loses around 500 positions (up to 0.8) it
+// gains many times over elsewhere.
 struct RowsPlan {
   int rows, tiles, chunks;
   bool cluster;
@@ -1040,11 +1046,11 @@ int rows_plan(int nkv, int group, int pos0, int ntok, RowsPlan* p) {
   p->cluster = false;
   // Chunks that are a cluster need no second launch, which costs as much as one step here or two
   // of the tile kernel's; they are eight at most, and as many as let all clusters run at once. In
-  // microseconds, as a cluster and not: 44 x 2 rows, 300 positions (2 steps, 2) 11.8 : 13.9;
-  // 4 x 4 rows, 4000 positions (2, 1) 15.8 : 17.6; 32 x 4 rows, 1032 positions (3, 2)
-  // 17.3 : 16.7; 8 x 4 rows, 4000 positions (4, 2) 19.5 : 18.6; tile kernel, 32 x 4 rows, 4000
-  // positions (4, 2) 19.3 : 21.4 and 256 x 4, 4096 positions (16, 16) 43.4 : 46.4; 16 clusters
-  // of 8, where 15 run at once, 26.1 : 16.9.
+  // microseconds of a graph, as a cluster and not: 44 x 2 rows, 300 positions (2 steps, 2)
+  // 11.6 : 13.7; 4 x 4 rows, 4000 positions (2, 1) 11.4 : 14.3; 32 x 4 rows, 1032 positions (3, 2)
+  // 17.0 : 16.5, half a microsecond lost; 8 x 4 rows, 4000 positions (4, 2) 16.1 : 15.8; tile
+  // kernel, 32 x 4 rows, 4000 positions (4, 2) 20.8 : 22.0 and 256 x 4, 4096 positions (16, 16)
+  // 43.4 : 47.1; 16 clusters of 8, where 15 run at once, 26.1 : 16.9.
   const int step = rows_step(p->rows);
   auto steps = [&](int chunks) { return ((blocks + chunks - 1) / chunks + step - 1) / step; };
   for (int c = std::min(p->chunks, kRowsCluster); c > 1; --c) {
@@ -1094,10 +1100,11 @@ int dec_launch(const float* q, const KvQ8& c, float* ctx, const float* scale, co
   const bool two = group > 4;
   // As a cluster the chunks are joined through shared memory, for which the two trips to the
   // scratch and the ticket take 2 us. It has eight at most, and as many as let all heads run at
-  // once, so that a full cache takes more steps of a block a warp. In microseconds, as a cluster
-  // and not, 8 heads x 4 queries: 300 positions (steps 1, 1) 6.6 : 8.2, 2000 (1, 1) 7.1 : 8.6,
-  // 4225 (3, 1) 8.6 : 9.2, 8000 (4, 2) 9.6 : 9.8, 12000 (6, 3) 11.5 : 10.9, 16000 (8, 4)
-  // 13.4 : 11.7. Only the cache's size is known here, and a cache is full at its end only.
+  // once, so that a full cache takes more steps of a block a warp. In microseconds of a graph, as a
+  // cluster and not, 8 heads x 4 queries: 300 positions (steps 1, 1) 6.5 : 8.5, 2000 (1, 1)
+  // 7.1 : 9.1, 4225 (3, 1) 8.6 : 9.6, 8000 (4, 2) 8.9 : 10.0, 12000 (6, 3) 11.2 : 11.1, 16000 (8, 4)
+  // 13.1 : 11.8. Only the cache's size is known here: a cache that is too long for clusters when it
+  // is full takes the second figures from its first position on.
   const int blocks = (cap + kQ8Blk - 1) / kQ8Blk;
   auto steps = [&](int chunks) { return ((blocks + chunks - 1) / chunks + kDecWarps - 1) / kDecWarps; };
   bool meet = false;

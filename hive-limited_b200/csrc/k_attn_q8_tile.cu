@@ -44,10 +44,11 @@
 // Every wait is bounded: one that runs out ends the CTA, whose rows are then NaN.
 //
 // Bound by the tensor cores and by what feeds them: with two terms on one side of each product,
-// 256 tokens of 64 heads over 16384 positions take 268 us and 256 of 32 heads over 4096 44 us,
-// 1.01 and 0.76 PFLOP/s of issued products, 61% and 46% of a large library product's rate. A
-// tile's weights (two exponent passes over 128 columns a thread) take about as long as its
-// products; two lanes of work hide the one behind the other, but not the ends of a chunk.
+// 256 tokens of 64 heads over 16384 positions take 265 us and 256 of 32 heads over 4096 45 us (239
+// and 43 in a graph), 1.03 and 0.74 PFLOP/s of issued products, 62% and 45% of a large library
+// product's rate. A tile's weights (a pass for the maximum and one for the exponents over 128
+// columns a thread) stand between two of its lane's products; two lanes of work hide the one behind
+// the other, but not the ends of a chunk.
 #include <type_traits>
 
 #include "attn_q8.cuh"
@@ -409,7 +410,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
     };
     // The weights of tile i. Most tiles are seen whole by every row and have nothing to look for:
     // those have a form of their own (`whole`), which the rest would slow by their code alone
-    // (16384 positions 266 us with it, 276 without).
+    // (256 rows at 16128 in a graph 239 us with it, 250 without).
     auto weights = [&](int i, auto whole_form) {
       constexpr bool whole = decltype(whole_form)::value;
       const int see0 = lim - 32 * (b0 + 4 * i);            // positions 0 .. see0 are seen

@@ -75,7 +75,9 @@ HV_DEV void q8_write_block(const Q8Src& src, const KvQ8& c, int item, int nth, i
   if (first) {
     if (threadIdx.x == 0) s_held = c.held[item];
     __syncthreads();
-    if (pos0 > s_held) return;         // a gap before pos0: nothing is written for this head
+    // a gap before pos0: the head's length and what it holds stay (the codes that the call's other
+    // CTAs write are past the length, where nothing reads them before they are written again)
+    if (pos0 > s_held) return;
     in_tail = old == 0 || (s_held - 1) / kQ8Blk == blk;
   }
 

@@ -463,7 +463,8 @@ __global__ void __launch_bounds__(kLpThreads, 2)
 // CTAs per row: enough rows fill the SMs with one each; few rows are cut into pieces of whole
 // tiles, as many as run at once. Without tiles to cut (or tickets) a row is one piece. Rows of
 // 151936, in microseconds, whole and cut so: 16 rows 23.5 : 14.9, 37 24.6 : 18.3, 64 24.5 : 21.7,
-// 100 25.0 : 27.6, 128 29.2 : 27.7, 148 31.9 : 28.1; 200 whole 35.9, in two pieces 51.5.
+// 100 25.0 : 27.6 (from 75 to about 110 rows the cut loses up to 10%), 128 29.2 : 27.7, 148
+// 31.9 : 28.1; 200 whole 35.9, in two pieces 51.5.
 int lp_pieces(int rows, int n, int* out, long long* most = nullptr) {
   int sms = 0;
   const int rc = sm_count(&sms);

@@ -6,7 +6,8 @@
 //   c = trunc(f32(x / s) + (x < 0 ? -0.5 : 0.5)), clipped to +-127   (quant_a8s's rule)
 // and a value reads back as f32(c s). A block with a NaN or an infinity in it has the scale
 // NaN, so all of it reads NaN. The block that is still open stays in f32 (the tail) and is
-// quantised once, when its 32nd row arrives: no value is ever rounded twice.
+// quantised when its 32nd row arrives: once, unless a write goes back into it later, which reopens
+// it from its codes.
 //
 // One buffer per layer (every part starts on 256 bytes; nblk = ceil(cap / 32)):
 //   codes  u8  [nkv][nblk][2][4096]   a block's K codes, then its V codes, each code + 128

@@ -264,14 +264,15 @@ int hv_attn_decode_f16(const float* q, const uint16_t* kc, const uint16_t* vc, f
  * c = trunc(f32(x / s) + (x < 0 ? -0.5 : 0.5)), clipped to +-127 (quant_a8s's rule,
  * engine/reference.py:44-59); a value reads back as f32(c s). A block that holds a NaN or an
  * infinity reads NaN throughout. The block that is still open (fewer than 32 rows) stays in
- * f32 and is quantised once, when its last row arrives, so no value is rounded twice and the
- * cache does not depend on how the rows were divided into calls.
+ * f32 and is quantised when its last row arrives, so that the cache does not depend on how the
+ * rows were divided into calls, and rows written in order are rounded once.
  *   The buffer: hv_kv_q8_size bytes, 16-byte aligned, zeroed = empty. It knows how many
  * positions it holds (on the device: the calls may be captured). Rows are written in order:
  * a write at pos0 makes the length pos0 + ntok, positions from there on are no longer held,
- * and a write past the length (a gap) writes nothing. Going back into a complete block
- * reopens it from its codes, except the block of the last row written, whose f32 rows are
- * still there. Positions that are not held read NaN and attend to NaN. hd must be 128.
+ * and a write past the length (a gap) leaves the length and all that is held as they are. Going
+ * back into a complete block reopens it from its codes, which are quantised again when it is
+ * complete again, except the block of the last row written, whose f32 rows are still there.
+ * Positions that are not held read NaN and attend to NaN. hd must be 128.
  *   Arrangement (nblk = ceil(cap / 32); every part padded to 256 bytes): codes u8
  * [nkv][nblk][K, V][4096], each code + 128; scales f32 [nkv][nblk][K, V]; the open rows f32
  * [nkv][K, V][32][128]; the length i32 [nkv][K, V]. In a block K's code of position
@@ -298,8 +299,11 @@ int hv_kv_read_q8(const void* kv, float* k_out, float* v_out, int pos0, int nkv,
  * order of operations: the lane has its own results). Query head h reads kv head h / group,
  * group 1 to 8; q and ctx [ntok][nq][128], 16-byte aligned. The sums run ahead of the quotient
  * by 2^15 and the number of positions: V to about 10^30 (and from 10^-31 on) keeps f32's
- * precision. An open row with a NaN or an infinity in its K or V makes the whole context of
- * every query NaN that sees it, as a complete block that holds one does.
+ * precision. A query's values count to 2^-38 of its largest, an open row's to 2^-34 of its own
+ * largest, and a weight to 2^-38 of the largest product of a weight and its block's largest |V|;
+ * weights under 2^-126 of the largest are 0. An open row with a NaN or an infinity in its K or
+ * V makes the whole context of every query NaN that sees it, as a complete block that holds
+ * one does.
  *   hv_attn_decode_q8  one query row over positions 0 .. *pos. A *pos that is not held
  *                      leaves NaN in ctx and reads no cache row.            (fda_warp_pos)
  *   hv_attn_rows_q8    row t over positions 0 .. pos0 + t of the cache as it stands: rows of
