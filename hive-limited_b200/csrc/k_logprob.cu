@@ -12,8 +12,9 @@
 // equal to +0, a NaN above all, ties to the lower id.
 //
 // One pass over the logits. 256 rows of 151936 (155 MB) take 40 us, 3.9 TB/s, 59% of a plain
-// copy's rate: bound by instructions (an exponential, four packed operations and two comparisons
-// for each logit) and by 256 CTAs where 296 fit. One row takes 12 us (6 without alternatives), all
+// copy's rate, with half of the issue slots used: an exponential, four packed operations and two
+// comparisons for each logit in a chain that a warp waits on, and 256 CTAs where 296 fit, so that 40
+// of 148 SMs have one row and the others two. One row takes 12 us (6 without alternatives), all
 // of it latency: the first batches' list, the trip through the scratch, the merge of 38 lists.
 //
 // Alternatives: a warp keeps its 32 largest, and what is under a bound costs one comparison. The
