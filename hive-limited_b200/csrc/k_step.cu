@@ -1760,6 +1760,7 @@ k_step(const hv_step_desc D, int flags, int nslots, int inflight, int evict_firs
         if (cv > v || (cv == v && ci < idx)) { v = cv; idx = ci; }
       }
       if (world > 1 && !exchange_argmax(D, rank, world, &v, &idx)) return;
+      if (idx == 0x7FFFFFFF) idx = 0;                 // no number among the logits: np.argmax's, too
       *D.tok = idx;
       const int s = *D.step;
       if (s >= 0 && s <= D.cap) D.gen[s] = idx;      // gen holds cap + 1 entries

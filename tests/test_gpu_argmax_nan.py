@@ -31,3 +31,25 @@ def test_argmax_of_logits_that_are_not_numbers(hv, case):
     hv.argmax_partial(Dev(x), pv, pi, n, 128)
     hv.argmax_final(pv, pi, tok, gen, step, pos, 128)
     assert tok.get(np.int32)[0] == gen.get(np.int32)[0] == np.argmax(x)
+
+
+@pytest.mark.parametrize("fused,kv", [(True, "f32"), (True, "f16"), (False, "f32"), (False, "q8")])
+def test_engine_whose_logits_are_not_numbers(hv, fused, kv):
+    """Token 0 at every step, and an engine that goes on (the next step reads the token's row)."""
+    import limited
+    import synth
+    import w4format
+    cfg = w4format.Config(synth.tiny_arch())
+
+    def tensors():
+        for name, x in synth.iter_tensors(cfg, 8):
+            yield name, np.full_like(x, np.nan) if name == "model.norm.weight" else x
+    e = limited.Engine(config=cfg, tensors=tensors(), quiet=True, max_context=64, kv_dtype=kv,
+                       fused=fused)
+    try:
+        ids = synth.prompt_ids(cfg, 8, 9)
+        assert np.isnan(e.logits(ids)).all()
+        for graph in (False, True):
+            assert e.generate(ids, 6, stop_on_eos=False, use_graph=graph)[0] == [0] * 6
+    finally:
+        e.free()
