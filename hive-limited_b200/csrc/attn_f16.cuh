@@ -1,0 +1,67 @@
+// What the attention kernels over a binary16 cache in an order of their own share: which
+// positions a query row sees.
+//
+// A row sees a prefix, which every row of the call sees whole, and then part of a tail: the
+// sequence's own positions, up to the row's. hv_attn_shared_f16 has a tail a sequence;
+// hv_attn_rows_mass_f16 is one sequence whose tail is the run itself, behind the positions before
+// it in the same cache; hv_attn_decode_mass_f16 is one row and a prefix.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "attn_q8.cuh"
+#include "hv_internal.h"
+
+namespace hv {
+
+struct SpanArgs {
+  const float* q;                      // [nrow][nq][128]
+  float* ctx;
+  const float* scale;
+  const __half *pk, *pv;               // prefix: head after head, p_head elements apart
+  const __half *tk, *tv;               // tails: sequences t_seq, heads t_head elements apart
+  size_t p_head, t_seq, t_head;
+  const int32_t* plen_p;               // prefix positions: *plen_p + plen, or plen
+  const int32_t *row0, *tlen_p;        // rows row0[s] .. row0[s + 1] - 1 are sequence s's
+  int plen, pmin, pcap, tlen, tcap;    // a prefix of pmin to pcap positions
+  int nq, group, nseq, nrow;
+};
+
+// Positions of the prefix; -1 if it cannot have that many.
+HV_DEV int span_prefix(const SpanArgs& a) {
+  const int n = a.plen + (a.plen_p ? __ldg(a.plen_p) : 0);
+  return n < a.pmin || n > a.pcap ? -1 : n;
+}
+
+// Rows [row, end) of sequence s, whose first row sees `first` positions of its tail and every
+// later one a position more. Without row0 a single sequence has all rows, several one each.
+struct SpanSeq {
+  int s, row, end, len;                // len: the tail's positions, -1 if it cannot hold them
+  HV_DEV int sees(int r) const { return max(0, len - (end - 1 - r)); }
+};
+HV_DEV int span_row0(const SpanArgs& a, int s) {
+  if (a.row0) return min(max(__ldg(a.row0 + s), 0), a.nrow);
+  return a.nseq == 1 ? s * a.nrow : s;
+}
+HV_DEV SpanSeq span_seq(const SpanArgs& a, int s) {
+  SpanSeq x;
+  x.s = s;
+  x.row = span_row0(a, s);
+  x.end = span_row0(a, s + 1);
+  x.len = a.tlen_p ? __ldg(a.tlen_p + s) : a.tlen;
+  if (x.len < 0 || x.len > a.tcap) x.len = -1;
+  return x;
+}
+// The sequence that row r belongs to; false if it lies behind the last one's rows.
+HV_DEV bool span_find(const SpanArgs& a, int r, SpanSeq* x) {
+  int lo = 0, hi = a.nseq - 1;
+  while (lo < hi) {                    // the last sequence that starts at or before r
+    const int mid = (lo + hi + 1) >> 1;
+    if (span_row0(a, mid) <= r) lo = mid;
+    else hi = mid - 1;
+  }
+  *x = span_seq(a, lo);
+  return r >= x->row && r < x->end;
+}
+
+}  // namespace hv

@@ -98,6 +98,17 @@ _SIGS = {
     "hv_attn_q8_scratch": [_I, _I, _I, _I, C.POINTER(_SZ)],
     "hv_attn_decode_q8": [_VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _VP],
     "hv_attn_rows_q8": [_VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP, _VP],
+    "hv_attn_shared_scratch": [_I, _I, _I, _I, _I, _I, C.POINTER(_SZ)],
+    "hv_attn_shared_f16": [_VP, _VP, _VP, _I, _VP, _VP, _VP, _I, _VP, _VP, _VP, _VP, _I, _I, _I, _I,
+                           _I, _VP, _VP],
+    "hv_qk_shared_f16": [_VP, _VP, _VP, _VP, _VP, _I, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I,
+                         _F, _I, _I, _VP],
+    "hv_attn_mass_scratch": [_I, _I, _I, _I, C.POINTER(_SZ)],
+    "hv_attn_decode_mass_f16": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _VP, _VP],
+    "hv_attn_rows_mass_f16": [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _I, _I, _I, _VP, _VP],
+    "hv_kv_evict_scratch": [_I, _I, _I, C.POINTER(_SZ)],
+    "hv_kv_evict_f16": [_VP, _VP, C.c_longlong, _VP, _I, _VP, _I, _VP, _VP, C.c_longlong, _VP, _I,
+                        _VP, _VP, _I, _I, _I, _I, _I, _I, _VP, _VP],
     "hv_logprob_scratch": [_I, _I, _I, C.POINTER(_SZ)],
     "hv_logprob_rows": [_VP, C.c_longlong, _I, _I, _VP, _I, _VP, _VP, _VP, _VP, _VP, _VP],
     "hv_attn_reserve": [_I, _I, _I],
@@ -661,6 +672,68 @@ def attn_rows_q8(q, kv, ctx, scale, pos0, nq, hd, group, cap, ntok, scratch, str
     """Attention of ntok query rows over an 8-bit cache, row t over positions 0 .. pos0 + t."""
     _call("hv_attn_rows_q8", int(q), int(kv), int(ctx), int(scale), int(pos0), nq, hd, group, cap,
           ntok, int(scratch), int(stream))
+
+
+def attn_shared_scratch(nq, group, pcap, tcap, nseq, nrow) -> int:
+    """Bytes of attn_shared's scratch; zero it once."""
+    n = C.c_size_t()
+    _call("hv_attn_shared_scratch", nq, group, pcap, tcap, nseq, nrow, C.byref(n))
+    return n.value
+
+
+def attn_shared(q, pk, pv, pcap, plen, tk, tv, tcap, row0, tlen, ctx, scale, nq, hd, group, nseq,
+                nrow, scratch, stream=0):
+    """Attention of nrow rows of nseq sequences over the binary16 prefix they share and a tail
+    each (hv_attn_shared_f16)."""
+    _call("hv_attn_shared_f16", int(q), int(pk), int(pv), pcap, int(plen), int(tk), int(tv), tcap,
+          int(row0), int(tlen), int(ctx), int(scale), nq, hd, group, nseq, nrow, int(scratch),
+          int(stream))
+
+
+def qk_shared(qkv, qn, kn, cos_t, sin_t, cap, base, row0, tlen, q_out, tk, tv, nq, nkv, hd, tcap,
+              eps, nseq, nrow, stream=0):
+    """Head norms and RoPE of such rows, K and V into the sequences' tails."""
+    _call("hv_qk_shared_f16", int(qkv), int(qn), int(kn), int(cos_t), int(sin_t), cap, int(base),
+          int(row0), int(tlen), int(q_out), int(tk), int(tv), nq, nkv, hd, tcap, C.c_float(eps),
+          nseq, nrow, int(stream))
+
+
+def attn_mass_scratch(nq, group, cap, ntok=1) -> int:
+    """Bytes of the scratch of attn_decode_mass (ntok = 1) and attn_rows_mass; zero it once."""
+    n = C.c_size_t()
+    _call("hv_attn_mass_scratch", nq, group, cap, ntok, C.byref(n))
+    return n.value
+
+
+def attn_decode_mass(q, kc, vc, ctx, mass_in, mass_out, scale, pos, nq, hd, group, cap, scratch,
+                     stream=0):
+    """Decode attention over positions 0 .. *pos of a binary16 cache; mass_out = mass_in + the
+    weights that the positions get."""
+    _call("hv_attn_decode_mass_f16", int(q), int(kc), int(vc), int(ctx), int(mass_in),
+          int(mass_out), int(scale), int(pos), nq, hd, group, cap, int(scratch), int(stream))
+
+
+def attn_rows_mass(q, kc, vc, ctx, mass_in, mass_out, scale, pos0, nq, hd, group, cap, ntok,
+                   scratch, stream=0):
+    """The same for a run of ntok rows, row t over positions 0 .. pos0 + t."""
+    _call("hv_attn_rows_mass_f16", int(q), int(kc), int(vc), int(ctx), int(mass_in), int(mass_out),
+          int(scale), int(pos0), nq, hd, group, cap, ntok, int(scratch), int(stream))
+
+
+def kv_evict_scratch(nkv, cap, nset=1) -> int:
+    """Bytes of kv_evict's scratch; zero it once."""
+    n = C.c_size_t()
+    _call("hv_kv_evict_scratch", nkv, cap, nset, C.byref(n))
+    return n.value
+
+
+def kv_evict(kc, vc, set_, mass, cap, len_, added, kd, vd, set_d, mass_d, dcap, len_out, kept, limit,
+             keep, recent, nkv, hd, nset, scratch, stream=0):
+    """Thins nset binary16 caches that hold *len_ + added positions, if that is over `limit`, to
+    `keep`: the last `recent` and those of most mass (hv_kv_evict_f16)."""
+    _call("hv_kv_evict_f16", int(kc), int(vc), int(set_), int(mass), cap, int(len_), added, int(kd),
+          int(vd), int(set_d), int(mass_d), dcap, int(len_out), int(kept), limit, keep, recent, nkv,
+          hd, nset, int(scratch), int(stream))
 
 
 def logprob_scratch(rows, n, top=0) -> int:

@@ -319,6 +319,73 @@ int hv_attn_decode_q8(const float* q, const void* kv, float* ctx, const float* s
 int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const float* scale, int pos0,
                     int nq, int hd, int group, int cap, int ntok, void* scratch, void* stream);
 
+/* One prompt with many continuations, and caches of bounded size: attention over binary16 caches
+ * in an order of its own (no counterpart in the reference). hd must be 128, query head h reads kv
+ * head h / group, group 1 to 8. q and ctx [rows][nq][128] f32; every pointer to such rows or to
+ * cache rows is 16-byte aligned. Contexts are softmax(scale q k^T) v with f32 sums: queries and
+ * weights count to 2^-22 of themselves and at least to 2^-38 of a row's largest, weights under
+ * 2^-126 of the largest are 0. A position whose K or V holds an infinity or a NaN leaves
+ * infinities or NaN in contexts (and weights) of the queries that see it, and of no others.
+ *
+ *   hv_attn_shared_f16  attention of a batch of sequences that share a prefix, which is read once
+ *     for all of them. The prefix: *plen positions of pk, pv [nkv][pcap][128] (0 to pcap; with
+ *     pcap 0 the three may be NULL). Sequence s has a tail of its own, tlen[s] positions (0 to
+ *     tcap) of tk, tv [nseq][nkv][tcap][128], and the rows row0[s] .. row0[s + 1] - 1 of q: they
+ *     are its last ones, so that row i of R sees the prefix and tail positions
+ *     0 .. tlen[s] - R + i (none where that is negative). row0 is i32 [nseq + 1] on the device, 0
+ *     first and never falling; NULL: one row each (nrow = nseq). A sequence may have no rows. A
+ *     row that sees nothing has a context of 0; rows from row0[nseq] on are left as they are. A
+ *     *plen or tlen[s] out of its range leaves NaN in the rows concerned and reads no row there.
+ *   hv_qk_shared_f16  hv_qk_rows_f16 for such a batch: the rows of qkv [nrow][(nq + 2 nkv) 128]
+ *     get their head norms and are rotated to position *base + slot, row i of R in slot
+ *     tlen[s] - R + i; q to q_out, k and v into the tails at that slot. cos_t and sin_t have `cap`
+ *     positions. A row whose slot or position lies outside writes nothing but NaN in q_out.
+ *   hv_attn_decode_mass_f16, hv_attn_rows_mass_f16  the lane's causal attention over kc, vc
+ *     [nkv][cap][128], one row over positions 0 .. *pos, or row t of ntok over 0 .. pos0 + t, which
+ *     also adds up the weights that positions get: mass_out[g][t] = mass_in[g][t] + the sum over
+ *     the rows that see t and the query heads of kv head g of t's weight. mass_in, mass_out f32
+ *     [nkv][cap], the same one or apart; mass_in NULL counts as 0. Positions that no row sees are
+ *     left as they are in mass_out. A *pos outside [0, cap) leaves NaN in ctx and mass_out as it
+ *     is.                                                                     (fda_warp_pos)
+ *   hv_kv_evict_f16  thins nset caches (the layers of a model): cache i has kc, vc
+ *     [nkv][cap][128] i * set elements on, and mass [nset][nkv][cap]. All hold n = *len + added
+ *     positions. If n is over `limit`, then of every cache and kv head `keep` of them stay: the
+ *     last `recent`, and of the others those with the most mass (ties: the lower position; NaN
+ *     counts as most), in their order, as positions 0 .. keep - 1 of kd, vd [nkv][dcap][128]
+ *     (i * set_d elements on) and of mass_d [nset][nkv][dcap]; *len_out = keep. Otherwise all n stay and
+ *     *len_out = n. kept (NULL or i32 [nset][nkv][dcap]) gets the position each came from. In
+ *     place (kd = kc, vd = vc, mass_d = mass, dcap = cap, set_d = set), where nothing is moved
+ *     and kept is not written unless n is over the limit, or to memory apart from the source.
+ *     recent <= keep <= limit <= dcap. len_out may be len. An n outside [0, cap] changes nothing.
+ * scratch: as many bytes as the _scratch function says, 16-byte aligned, zeroed once by the
+ * caller; every call leaves it ready for the next. Those bytes do for any call of up to the rows,
+ * sequences, positions and caches given there. Calls that may overlap on the GPU (streams, captured
+ * graphs) need one each. Nothing is allocated. */
+int hv_attn_shared_scratch(int nq, int group, int pcap, int tcap, int nseq, int nrow, size_t* bytes);
+int hv_attn_shared_f16(const float* q, const uint16_t* pk, const uint16_t* pv, int pcap,
+                       const int32_t* plen, const uint16_t* tk, const uint16_t* tv, int tcap,
+                       const int32_t* row0, const int32_t* tlen, float* ctx, const float* scale,
+                       int nq, int hd, int group, int nseq, int nrow, void* scratch, void* stream);
+int hv_qk_shared_f16(const float* qkv, const float* qn, const float* kn, const float* cos_t,
+                     const float* sin_t, int cap, const int32_t* base, const int32_t* row0,
+                     const int32_t* tlen, float* q_out, uint16_t* tk, uint16_t* tv, int nq, int nkv,
+                     int hd, int tcap, float eps, int nseq, int nrow, void* stream);
+int hv_attn_mass_scratch(int nq, int group, int cap, int ntok, size_t* bytes);
+int hv_attn_decode_mass_f16(const float* q, const uint16_t* kc, const uint16_t* vc, float* ctx,
+                            const float* mass_in, float* mass_out, const float* scale,
+                            const int32_t* pos, int nq, int hd, int group, int cap, void* scratch,
+                            void* stream);
+int hv_attn_rows_mass_f16(const float* q, const uint16_t* kc, const uint16_t* vc, float* ctx,
+                          const float* mass_in, float* mass_out, const float* scale, int pos0,
+                          int nq, int hd, int group, int cap, int ntok, void* scratch,
+                          void* stream);
+int hv_kv_evict_scratch(int nkv, int cap, int nset, size_t* bytes);
+int hv_kv_evict_f16(const uint16_t* kc, const uint16_t* vc, long long set, const float* mass,
+                    int cap, const int32_t* len, int added, uint16_t* kd, uint16_t* vd,
+                    long long set_d, float* mass_d, int dcap, int32_t* len_out, int32_t* kept,
+                    int limit, int keep, int recent, int nkv, int hd, int nset, void* scratch,
+                    void* stream);
+
 /* Makes sure the attention scratch can serve nkv heads at a cache of `cap` positions. */
 int hv_attn_reserve(int nkv, int group, int cap);
 

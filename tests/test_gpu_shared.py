@@ -1,0 +1,550 @@
+"""Attention over a shared prefix, the write of a batch's rows, attention that adds up its weights
+and eviction on a B200, against the 64-bit plain forms of span_ref.py."""
+import numpy as np
+import pytest
+
+import span_ref as R
+from gpu_util import Dev, bits
+
+pytestmark = pytest.mark.gpu
+F32, F16, HD = np.float32, np.float16, 128
+SCALE = float(F32(1.0 / np.sqrt(HD)))
+
+
+def cache(g, *shape):
+    """K and V in binary16, some dims of K larger than others."""
+    k = g.standard_normal((*shape, HD)) * np.exp(0.5 * g.standard_normal(HD))
+    return k.astype(F16), g.standard_normal((*shape, HD)).astype(F16)
+
+
+def queries(g, rows, nq, scale=1.0):
+    return (scale * g.standard_normal((rows, nq, HD)) * np.exp(0.5 * g.standard_normal(HD))).astype(F32)
+
+
+def i32(x):
+    return Dev(np.atleast_1d(np.array(x, np.int32)))
+
+
+def scratch(n):
+    return Dev(nbytes=n)
+
+
+def near(got, want, tol):
+    off = np.abs(got.astype(np.float64) - want)
+    assert np.isfinite(got).all()
+    assert (off <= tol).all(), float((off / tol).max())
+
+
+# ---- attention over a shared prefix ----------------------------------------------------
+
+def run_shared(hv, q, pk, pv, plen, tk, tv, row0, tlen, scale=SCALE, fill=7.0, s=None, stream=0):
+    nrow, nq, _ = q.shape
+    nseq, nkv, tcap, _ = tk.shape
+    pcap, group = pk.shape[1], nq // nkv
+    s = s or scratch(hv.attn_shared_scratch(nq, group, pcap, tcap, nseq, nrow))
+    ctx = Dev(np.full(q.shape, fill, F32))
+    dev = [Dev(x) for x in (q, tk, tv)] + [Dev(pk) if pcap else 0, Dev(pv) if pcap else 0]
+    dr = 0 if row0 is None else i32(row0)
+    dt, dp, ds = i32(tlen), i32(plen), Dev(np.array([scale], F32))
+    hv.attn_shared(dev[0], dev[3], dev[4], pcap, dp if pcap else 0, dev[1], dev[2], tcap, dr, dt, ctx,
+                   ds, nq, HD, group, nseq, nrow, s, stream)
+    return ctx.get(F32, q.shape)
+
+
+def check_shared(hv, g, nkv, group, plen, pcap, rows, tlen, tcap, extra=0, stale=np.nan, one=False):
+    nseq, nrow = len(rows), sum(rows) + extra
+    pk, pv = cache(g, nkv, pcap)
+    tk, tv = cache(g, nseq, nkv, tcap)
+    pk[:, plen:], pv[:, plen:] = stale, stale            # nothing there may count
+    for s, n in enumerate(tlen):
+        tk[s, :, n:], tv[s, :, n:] = stale, stale
+    q = queries(g, nrow, nkv * group)
+    row0 = None if one else np.concatenate([[0], np.cumsum(rows)])
+    got = run_shared(hv, q, pk, pv, plen, tk, tv, row0, tlen)
+    want, tol = R.shared(q, pk, pv, plen, tk, tv, row0, tlen, SCALE)
+    m = sum(rows)
+    near(got[:m], want[:m], tol[:m])
+    assert (got[m:] == 7).all()
+
+
+@pytest.mark.parametrize("nkv,group,plen,tails", [
+    (1, 1, 0, [1]), (2, 1, 1, [1]), (8, 2, 45, [3, 9]), (2, 4, 31, [0, 1, 2]), (1, 8, 32, [5] * 9),
+    (3, 5, 33, [64, 1, 65, 17]), (2, 3, 127, [2] * 33), (1, 7, 128, [1, 16, 130]),
+    (2, 6, 129, [7] * 20), (8, 4, 300, list(range(1, 17))), (2, 8, 1000, [40] * 16),
+    (1, 4, 4096, [3, 200] * 16), (2, 2, 4225, [9] * 64), (1, 1, 5000, [1, 2, 3])])
+def test_one_row_a_sequence(hv, nkv, group, plen, tails):
+    g = np.random.default_rng(plen + group)
+    check_shared(hv, g, nkv, group, plen, plen + 5, [1] * len(tails), tails, max(tails) + 2, one=True)
+
+
+@pytest.mark.parametrize("nkv,group,plen,rows,tails", [
+    (2, 4, 0, [3], [3]), (1, 2, 10, [1, 0, 5], [4, 9, 5]), (2, 8, 100, [17, 3, 0, 12], [17, 3, 4, 40]),
+    (8, 4, 200, [9, 31, 33, 1], [9, 31, 64, 300]), (1, 5, 700, [40, 2, 65], [41, 2, 65]),
+    (2, 3, 64, [150], [150]), (1, 8, 2000, [3, 17, 8, 8, 9, 2] * 3, [3, 20, 8, 30, 9, 2] * 3),
+    (2, 1, 300, [128, 64], [130, 64]), (1, 4, 20, [0, 0, 2], [5, 0, 2])])
+def test_runs_of_rows(hv, nkv, group, plen, rows, tails):
+    g = np.random.default_rng(plen + len(rows))
+    check_shared(hv, g, nkv, group, plen, plen + 3, rows, tails, max(tails) + 1, extra=2)
+
+
+def test_a_prefix_of_full_capacity_and_none_at_all(hv):
+    g = np.random.default_rng(5)
+    check_shared(hv, g, 2, 4, 256, 256, [1] * 20, [8] * 20, 8, one=True)
+    check_shared(hv, g, 2, 4, 0, 0, [2, 1], [2, 6], 6)
+    check_shared(hv, g, 2, 2, 0, 40, [2, 1], [2, 6], 6)
+
+
+def test_rows_that_see_nothing_are_zero(hv):
+    """A row of a sequence whose tail is shorter than its rows, without a prefix."""
+    g = np.random.default_rng(6)
+    check_shared(hv, g, 2, 4, 0, 8, [3, 1, 2], [1, 0, 2], 4)
+    check_shared(hv, g, 1, 8, 40, 64, [5, 1], [2, 0], 4)
+
+
+@pytest.mark.parametrize("rows,plen", [([1] * 4, 200), ([1] * 40, 600), ([6, 4], 300)])
+def test_lengths_out_of_range_leave_nan(hv, rows, plen):
+    g = np.random.default_rng(7)
+    nseq = len(rows)
+    pk, pv = cache(g, 2, plen)
+    tk, tv = cache(g, nseq, 2, 16)
+    q = queries(g, sum(rows), 8)
+    row0 = np.concatenate([[0], np.cumsum(rows)])
+    tlen = np.full(nseq, 9)
+    tlen[1] = 17
+    got = run_shared(hv, q, pk, pv, plen, tk, tv, row0, tlen)
+    bad = np.arange(row0[1], row0[2])
+    assert np.isnan(got[bad]).all()
+    ok = np.setdiff1d(np.arange(sum(rows)), bad)
+    want, tol = R.shared(q, pk, pv, plen, tk, tv, row0, np.minimum(tlen, 16), SCALE)
+    near(got[ok], want[ok], tol[ok])
+    for n in (-1, plen + 1, 2 ** 31 - 1):
+        assert np.isnan(run_shared(hv, q, pk, pv, n, tk, tv, row0, np.full(nseq, 9))).all()
+    tlen[1] = -1
+    assert np.isnan(run_shared(hv, q, pk, pv, plen, tk, tv, row0, tlen)[bad]).all()
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_what_a_row_does_not_see_does_not_count(hv, which, bad):
+    """An infinity or a NaN in a tail reaches the rows behind it of that sequence only."""
+    g = np.random.default_rng(8)
+    rows, tails = [20, 9, 3], [20, 30, 3]
+    pk, pv = cache(g, 2, 150)
+    tk, tv = cache(g, 3, 2, 32)
+    q = queries(g, 32, 8)
+    row0 = np.concatenate([[0], np.cumsum(rows)])
+    want, tol = R.shared(q, pk, pv, 150, tk, tv, row0, tails, SCALE)
+    (tk if which == "k" else tv)[0, 1, 11, 5] = bad
+    (tk if which == "k" else tv)[1, 1, 26, :] = bad
+    got = run_shared(hv, q, pk, pv, 150, tk, tv, row0, tails)
+    hit = np.zeros((32, 8), bool)
+    hit[11:20, 4:] = True
+    hit[20 + 5:29, 4:] = True
+    near(got[~hit], want[~hit], tol[~hit])
+    assert not np.isfinite(got[25:29, 4:]).all(-1).any()
+    if which == "v" or np.isnan(bad):
+        assert not np.isfinite(got[11:20, 4:]).all(-1).any()
+
+
+@pytest.mark.parametrize("scale,qs,ks", [(SCALE, 1e-20, 1.0), (SCALE, 30.0, 20.0), (-SCALE, 1.0, 1.0),
+                                         (0.0, 1.0, 1.0), (1.0, 2e4, 1e-3), (1e-30, 3e34, 1.0)])
+def test_queries_and_scales_of_any_size(hv, scale, qs, ks):
+    g = np.random.default_rng(9)
+    for nseq, plen in ((3, 300), (40, 300)):
+        pk, pv = cache(g, 1, plen)
+        tk, tv = cache(g, nseq, 1, 40)
+        pk, tk = (pk * F16(ks)).astype(F16), (tk * F16(ks)).astype(F16)
+        pv[:, ::3], tv[:, :, ::3] = F16(6e4), F16(-6e4)
+        q = queries(g, nseq, 4, qs)
+        q[0, 0] = 0
+        q[1, 1, 5:] *= F32(1e-9)
+        tl = [33] * nseq
+        got = run_shared(hv, q, pk, pv, plen, tk, tv, None, tl, scale)
+        want, tol = R.shared(q, pk, pv, plen, tk, tv, None, tl, float(F32(scale)))
+        near(got, want, tol)
+
+
+def test_repeats_are_equal(hv):
+    """The same call gives the same bits."""
+    g = np.random.default_rng(10)
+    pk, pv = cache(g, 2, 500)
+    tk, tv = cache(g, 12, 2, 20)
+    q = queries(g, 12, 8)
+    a = run_shared(hv, q, pk, pv, 500, tk, tv, None, [20] * 12)
+    b = run_shared(hv, q, pk, pv, 500, tk, tv, None, [20] * 12)
+    assert np.array_equal(bits(a), bits(b))
+
+
+def test_one_scratch_serves_calls_of_every_size(hv):
+    """The scratch of the largest call, used by others in turn on a stream of its own."""
+    g = np.random.default_rng(11)
+    s = scratch(hv.attn_shared_scratch(16, 8, 3000, 100, 40, 60))
+    st = hv.stream_create()
+    try:
+        for nseq, plen, tcap in ((40, 3000, 5), (1, 3, 100), (17, 900, 33), (40, 2999, 100), (2, 0, 4)):
+            pk, pv = cache(g, 2, 3000)
+            tk, tv = cache(g, nseq, 2, tcap)
+            q = queries(g, nseq, 16)
+            nq, ctx = 16, Dev(np.zeros(q.shape, F32))
+            dev = [Dev(x) for x in (q, pk, pv, tk, tv)]
+            dp, dt, ds = i32(plen), i32([tcap] * nseq), Dev(np.array([SCALE], F32))
+            hv.synchronize()
+            hv.attn_shared(dev[0], dev[1], dev[2], 3000, dp, dev[3], dev[4], tcap, 0, dt, ctx, ds, nq,
+                           HD, 8, nseq, nseq, s, st)
+            hv.stream_synchronize(st)
+            near(ctx.get(F32, q.shape), *R.shared(q, pk, pv, plen, tk, tv, None, [tcap] * nseq, SCALE))
+    finally:
+        hv.stream_destroy(st)
+
+
+def test_two_captured_graphs_follow_device_lengths(hv):
+    """Write and attention captured twice, each with a scratch of its own, replayed in turn as the
+    lengths on the device grow."""
+    g = np.random.default_rng(12)
+    nkv, group, nseq, tcap, plen, cap = 2, 4, 5, 24, 130, 200
+    nq = nkv * group
+    ang = np.arange(cap)[:, None] * (1e4 ** (-np.arange(64) / 64.0))[None]
+    cos, sin = Dev(np.cos(ang).astype(F32)), Dev(np.sin(ang).astype(F32))
+    gains = [Dev((1 + 0.1 * g.standard_normal(HD)).astype(F32)) for _ in range(2)]
+    lanes = []
+    for _ in range(2):
+        pk, pv = cache(g, nkv, plen)
+        qkv = g.standard_normal((nseq, (nq + 2 * nkv) * HD)).astype(F32)
+        L = dict(pk=pk, pv=pv, qkv=Dev(qkv), dpk=Dev(pk), dpv=Dev(pv),
+                 tk=Dev(nbytes=nseq * nkv * tcap * 256), tv=Dev(nbytes=nseq * nkv * tcap * 256),
+                 q=Dev(nbytes=nseq * nq * 512), ctx=Dev(nbytes=nseq * nq * 512), st=hv.stream_create(),
+                 s=scratch(hv.attn_shared_scratch(nq, group, plen, tcap, nseq, nseq)),
+                 pl=i32(plen), tl=i32([0] * nseq), sc=Dev(np.array([SCALE], F32)))
+        hv.synchronize()
+        hv.capture_begin(L["st"])
+        hv.qk_shared(L["qkv"], *gains, cos, sin, cap, L["pl"], 0, L["tl"], L["q"], L["tk"], L["tv"], nq,
+                     nkv, HD, tcap, 1e-5, nseq, nseq, L["st"])
+        hv.attn_shared(L["q"], L["dpk"], L["dpv"], plen, L["pl"], L["tk"], L["tv"], tcap, 0, L["tl"],
+                       L["ctx"], L["sc"], nq, HD, group, nseq, nseq, L["s"], L["st"])
+        L["graph"] = hv.capture_end(L["st"])
+        L["exec"] = hv.graph_instantiate(L["graph"])
+        lanes.append(L)
+    for step in range(1, 4):
+        tlen = np.array([step, step + 3, step, 2 * step, step + 10], np.int32)
+        for L in lanes:
+            L["tl"].put(tlen)
+            L["qkv"].put(g.standard_normal((nseq, (nq + 2 * nkv) * HD)).astype(F32))
+        hv.synchronize()
+        for L in lanes:
+            hv.graph_launch(L["exec"], L["st"])
+        for L in lanes:
+            hv.stream_synchronize(L["st"])
+            tk, tv = (L[x].get(F16, (nseq, nkv, tcap, HD)) for x in ("tk", "tv"))
+            q = L["q"].get(F32, (nseq, nq, HD))
+            near(L["ctx"].get(F32, q.shape), *R.shared(q, L["pk"], L["pv"], plen, tk, tv, None, tlen, SCALE))
+    for L in lanes:
+        hv.graph_destroy(L["graph"], L["exec"])
+        hv.stream_destroy(L["st"])
+
+
+# ---- the write of a batch's rows -------------------------------------------------------
+
+@pytest.mark.parametrize("nkv,group,rows,tails,base", [
+    (1, 1, [1], [1], 0), (2, 4, [1, 1, 1], [1, 7, 20], 33), (8, 8, [5, 0, 17, 3], [9, 4, 17, 20], 100),
+    (3, 5, [2, 40], [2, 40], 7)])
+def test_rows_are_written_as_runs_are(hv, nkv, group, rows, tails, base):
+    """Bit for bit what qk_rows writes for each sequence's run at its positions."""
+    g = np.random.default_rng(base)
+    nq, nrow, tcap, cap = nkv * group, sum(rows) + 1, 44, 160
+    ang = np.arange(cap)[:, None] * (1e6 ** (-np.arange(64) / 64.0))[None]
+    cos, sin = np.cos(ang).astype(F32), np.sin(ang).astype(F32)
+    dc, dsn = Dev(cos), Dev(sin)
+    qn, kn = (Dev((1 + 0.1 * g.standard_normal(HD)).astype(F32)) for _ in range(2))
+    qkv = g.standard_normal((nrow, (nq + 2 * nkv) * HD)).astype(F32)
+    row0 = np.concatenate([[0], np.cumsum(rows)])
+    old = g.standard_normal((2, len(rows), nkv, tcap, HD)).astype(F16)
+    tk, tv, qo = Dev(old[0]), Dev(old[1]), Dev(np.full((nrow, nq, HD), 7, F32))
+    dq, dbase, dr, dt = Dev(qkv), i32(base), i32(row0), i32(tails)
+    hv.qk_shared(dq, qn, kn, dc, dsn, cap, dbase, dr, dt, qo, tk, tv, nq, nkv, HD, tcap, 1e-5, len(rows),
+                 nrow)
+    want_q = np.full((nrow, nq, HD), 7, F32)
+    want = old.copy()
+    for s, (r, t) in enumerate(zip(rows, tails)):
+        if not r:
+            continue
+        kc, vc, q2 = Dev(nbytes=nkv * cap * 256), Dev(nbytes=nkv * cap * 256), Dev(nbytes=r * nq * 512)
+        run = Dev(qkv[row0[s]:row0[s + 1]])
+        hv.qk_rows(run, qn, kn, dc, dsn, base + t - r, q2, kc, vc, nq, nkv, HD, cap, 1e-5, r, f16=True)
+        want_q[row0[s]:row0[s + 1]] = q2.get(F32, (r, nq, HD))
+        for i, c in enumerate((kc, vc)):
+            want[i, s, :, t - r:t] = c.get(F16, (nkv, cap, HD))[:, base + t - r:base + t]
+    assert np.array_equal(bits(qo.get(F32, want_q.shape)), bits(want_q))
+    for i, c in enumerate((tk, tv)):
+        assert np.array_equal(c.get(np.uint16), want[i].view(np.uint16).ravel())
+
+
+def test_rows_outside_are_not_written(hv):
+    """Slots before 0, tails longer than their room, positions past the tables."""
+    g = np.random.default_rng(3)
+    nq = nkv = 2
+    rows, tails, tcap, cap, base = [3, 1, 2, 1], [2, 9, 6, -3], 8, 40, 35
+    row0 = np.concatenate([[0], np.cumsum(rows)])
+    ones, tab = Dev(np.ones(HD, F32)), Dev(np.ones((cap, 64), F32))
+    old = g.standard_normal((4, nkv, tcap, HD)).astype(F16)
+    tk, tv, qo = Dev(old), Dev(old), Dev(np.full((7, nq, HD), 7, F32))
+    dq = Dev(g.standard_normal((7, 6 * HD)).astype(F32))
+    db, dr, dt = i32(base), i32(row0), i32(tails)
+    hv.qk_shared(dq, ones, ones, tab, tab, cap, db, dr, dt, qo, tk, tv, nq, nkv, HD, tcap, 1e-5, 4, 7)
+    q = qo.get(F32, (7, nq, HD))
+    assert np.isnan(q).all((1, 2)).tolist() == [True, False, False, True, False, True, True]
+    new = tk.get(F16, old.shape)
+    changed = (new != old).any((1, 3))
+    want = np.zeros((4, tcap), bool)
+    want[0, 0] = want[0, 1] = want[2, 4] = True
+    assert np.array_equal(changed, want)
+
+
+# ---- attention that adds up its weights -------------------------------------------------
+
+def run_mass(hv, q, k, v, pos0, mass_in, decode, apart=True, stream=0, s=None, scale=SCALE):
+    """-> context, mass_out (what was in it before: 5)."""
+    ntok, nq, _ = q.shape
+    nkv, cap, _ = k.shape
+    group = nq // nkv
+    dq, dk, dv, ds = Dev(q), Dev(k), Dev(v), Dev(np.array([scale], F32))
+    ctx = Dev(np.full(q.shape, 7, F32))
+    out = Dev(np.full((nkv, cap), 5, F32))
+    src = 0
+    if mass_in is not None:
+        src = Dev(mass_in)
+        out = out if apart else src
+    s = s or scratch(hv.attn_mass_scratch(nq, group, cap, ntok))
+    if decode:
+        dp = i32(pos0)
+        hv.attn_decode_mass(dq, dk, dv, ctx, src, out, ds, dp, nq, HD, group, cap, s, stream)
+    else:
+        hv.attn_rows_mass(dq, dk, dv, ctx, src, out, ds, pos0, nq, HD, group, cap, ntok, s, stream)
+    return ctx.get(F32, q.shape), out.get(F32, (nkv, cap))
+
+
+def check_mass(hv, g, nkv, group, pos0, ntok, cap, decode, form):
+    n = pos0 + ntok
+    k, v = cache(g, nkv, cap)
+    k[:, n:], v[:, n:] = np.nan, np.nan
+    q = queries(g, ntok, nkv * group)
+    mi = None if form == "none" else np.abs(g.standard_normal((nkv, cap))).astype(F32)
+    ctx, m = run_mass(hv, q, k, v, pos0, mi, decode, form == "apart")
+    want, tol, wm, mt = R.mass(q, k, v, pos0, mi, SCALE)
+    near(ctx, want, tol)
+    near(m[:, :n], wm, mt)
+    assert np.array_equal(m[:, n:], mi[:, n:] if form == "same" else np.full((nkv, cap - n), 5, F32))
+
+
+@pytest.mark.parametrize("form", ["same", "apart", "none"])
+@pytest.mark.parametrize("nkv,group,n", [(1, 1, 1), (2, 4, 2), (8, 2, 31), (3, 5, 64), (2, 8, 129),
+                                         (8, 4, 1000), (1, 7, 4225), (2, 3, 9001)])
+def test_decode_with_mass(hv, nkv, group, n, form):
+    check_mass(hv, np.random.default_rng(n), nkv, group, n - 1, 1, n + 3, True, form)
+
+
+@pytest.mark.parametrize("nkv,group,pos0,ntok", [
+    (1, 1, 0, 1), (2, 4, 0, 5), (8, 2, 256, 44), (1, 8, 100, 17), (2, 5, 63, 65), (1, 3, 1000, 31),
+    (2, 4, 128, 128), (1, 8, 700, 256), (2, 1, 0, 300), (1, 2, 2048, 200), (1, 7, 4000, 3)])
+def test_run_with_mass(hv, nkv, group, pos0, ntok):
+    g = np.random.default_rng(pos0 + ntok)
+    check_mass(hv, g, nkv, group, pos0, ntok, pos0 + ntok + 2, False, "apart")
+    check_mass(hv, g, nkv, group, pos0, ntok, pos0 + ntok, False, "same")
+
+
+def test_mass_adds_up_over_calls(hv):
+    """A run, then single rows: every weight once. Each row's weights are 1 in all."""
+    g = np.random.default_rng(20)
+    nkv, group, cap, ntok = 2, 4, 80, 60
+    k, v = cache(g, nkv, cap)
+    q = queries(g, cap, nkv * group)
+    _, m = run_mass(hv, q[:ntok], k, v, 0, np.zeros((nkv, cap), F32), False, False)
+    for t in range(ntok, cap):
+        _, m = run_mass(hv, q[t:t + 1], k, v, t, m, True, False)
+    _, _, want, tol = R.mass(q, k, v, 0, None, SCALE)
+    near(m, want, 4 * tol + 32 * R.U * want)
+    assert np.allclose(m.sum(1), cap * group, rtol=1e-4)
+
+
+def test_decode_with_mass_outside_the_cache(hv):
+    g = np.random.default_rng(21)
+    k, v = cache(g, 2, 40)
+    q = queries(g, 1, 4)
+    for pos in (-1, 40, 2 ** 31 - 1, -2 ** 31):
+        ctx, m = run_mass(hv, q, k, v, pos, np.ones((2, 40), F32), True)
+        assert np.isnan(ctx).all() and (m == 5).all()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_mass_of_rows_before_a_bad_position(hv, bad):
+    g = np.random.default_rng(22)
+    for group, ntok in ((4, 30), (8, 100)):
+        k, v = cache(g, 1, 200)
+        q = queries(g, ntok, group)
+        want, tol, _, _ = R.mass(q, k, v, 60, None, SCALE)
+        v[0, 60 + 11] = bad
+        ctx, m = run_mass(hv, q, k, v, 60, None, False)
+        near(ctx[:11], want[:11], tol[:11])
+        assert not np.isfinite(ctx[11:]).any()
+
+
+def test_captured_decode_with_mass(hv):
+    """Replayed as *pos moves, in place, one scratch."""
+    g = np.random.default_rng(23)
+    nkv, group, cap = 2, 4, 300
+    k, v = cache(g, nkv, cap)
+    q = queries(g, 1, nkv * group)
+    dq, dk, dv, ds = Dev(q), Dev(k), Dev(v), Dev(np.array([SCALE], F32))
+    ctx, m, pos = Dev(nbytes=q.nbytes), Dev(nbytes=nkv * cap * 4), i32(0)
+    s = scratch(hv.attn_mass_scratch(nkv * group, group, cap, 1))
+    st = hv.stream_create()
+    hv.synchronize()
+    hv.capture_begin(st)
+    hv.attn_decode_mass(dq, dk, dv, ctx, m, m, ds, pos, nkv * group, HD, group, cap, s, st)
+    gr = hv.capture_end(st)
+    ex = hv.graph_instantiate(gr)
+    total, tol = np.zeros((nkv, cap)), np.zeros((nkv, cap))
+    for p in (0, 1, 31, 32, 200, 299):
+        pos.put(np.array([p], np.int32))
+        hv.synchronize()
+        hv.graph_launch(ex, st)
+        hv.stream_synchronize(st)
+        want, ct, w, wt = R.mass(q, k, v, p, None, SCALE)
+        near(ctx.get(F32, q.shape), want, ct)
+        total[:, :p + 1] += w
+        tol[:, :p + 1] += wt + 8 * R.U * total[:, :p + 1]
+    near(m.get(F32, (nkv, cap)), total, tol)
+    hv.graph_destroy(gr, ex)
+    hv.stream_destroy(st)
+
+
+# ---- eviction ----------------------------------------------------------------------------
+
+def run_evict(hv, k, v, mass, n, added, limit, keep, recent, dcap=None, stream=0, want_kept=True):
+    """k, v [nset, nkv, cap, 128]; dcap None: in place, the sets' K and V side by side as an engine
+    has them. -> k, v, mass, kept, length."""
+    nset, nkv, cap, _ = k.shape
+    one = nkv * cap * HD
+    both = Dev(np.stack([k, v], 1))                       # [set][K, V]
+    dm, dl, s = Dev(mass), i32(n - added), scratch(hv.kv_evict_scratch(nkv, cap, nset))
+    d = cap if dcap is None else dcap
+    kept = Dev(np.full((nset, nkv, d), -7, np.int32))
+    if dcap is None:
+        out, om, step = both, dm, 2 * one
+    else:
+        out = Dev(np.full((nset, 2, nkv, d, HD), 3, F16))
+        om, step = Dev(np.full((nset, nkv, d), 5, F32)), 2 * nkv * d * HD
+    hv.kv_evict(both.ptr, both.ptr + 2 * one, 2 * one, dm, cap, dl, added, out.ptr,
+                out.ptr + 2 * nkv * d * HD, step, om, d, dl, kept if want_kept else 0, limit, keep, recent,
+                nkv, HD, nset, s, stream)
+    o = out.get(np.uint16, (nset, 2, nkv, d, HD))
+    return o[:, 0], o[:, 1], om.get(F32, (nset, nkv, d)), kept.get(np.int32, (nset, nkv, d)), dl.get(np.int32)[0]
+
+
+def check_evict(hv, k, v, mass, n, added, limit, keep, recent, dcap):
+    nset, nkv, cap, _ = k.shape
+    ko, vo, mo, kept, left = run_evict(hv, k, v, mass, n, added, limit, keep, recent, dcap)
+    moved = n > limit
+    assert left == (keep if moved else n)
+    for i in range(nset):
+        for h in range(nkv):
+            idx = R.evict(mass[i, h], n, limit, keep, recent)
+            m = len(idx)
+            if dcap is not None or moved:
+                assert np.array_equal(kept[i, h, :m], idx)
+                assert (kept[i, h, m:] == -7).all()
+            else:
+                assert (kept[i, h] == -7).all()
+            assert np.array_equal(ko[i, h, :m], k[i, h, idx].view(np.uint16))
+            assert np.array_equal(vo[i, h, :m], v[i, h, idx].view(np.uint16))
+            assert np.array_equal(bits(mo[i, h, :m]), bits(mass[i, h, idx]))
+            if dcap is not None:                           # behind them: untouched
+                assert (mo[i, h, m:] == 5).all()
+                assert (ko[i, h, m:] == F16(3).view(np.uint16)).all()
+
+
+def some_mass(g, *shape):
+    m = np.exp(2 * g.standard_normal(shape)).astype(F32)
+    m[g.random(shape) < 0.2] = 0
+    m[g.random(shape) < 0.1] = F32(1.5)
+    return m
+
+
+@pytest.mark.parametrize("nset,nkv,n,limit,keep,recent", [
+    (1, 1, 1, 1, 1, 0), (1, 1, 2, 1, 1, 0), (1, 1, 2, 1, 1, 1), (2, 3, 40, 32, 32, 8), (1, 2, 300, 256, 256, 32),
+    (3, 2, 300, 299, 1, 0), (1, 8, 1000, 700, 512, 512), (1, 2, 1024, 1023, 1000, 0),
+    (2, 1, 1025, 1024, 1024, 1), (1, 2, 4352, 4351, 4096, 1024), (1, 1, 20000, 9000, 8192, 100),
+    (1, 1, 70000, 60000, 60000, 17), (36, 2, 352, 351, 320, 64), (1, 2, 100, 100, 50, 3), (2, 2, 0, 9, 5, 2)])
+@pytest.mark.parametrize("place", ["in place", "apart"])
+def test_eviction(hv, nset, nkv, n, limit, keep, recent, place):
+    g = np.random.default_rng(n + keep)
+    cap = max(n, limit) + 3
+    k, v = cache(g, nset, nkv, cap)
+    mass = some_mass(g, nset, nkv, cap)
+    mass[..., n:] = np.inf                                 # of no position that is held
+    dcap = None if place == "in place" else max(limit, n if n <= limit else keep) + 2
+    check_evict(hv, k, v, mass, n, min(n, 1), limit, keep, recent, dcap)
+
+
+@pytest.mark.parametrize("fill", ["equal", "nan", "signed", "sorted", "rising", "tiny"])
+def test_eviction_of_unusual_masses(hv, fill):
+    g = np.random.default_rng(31)
+    n = 2500
+    k, v = cache(g, 1, 2, n)
+    mass = {"equal": np.ones((1, 2, n)), "nan": g.standard_normal((1, 2, n)),
+            "signed": g.standard_normal((1, 2, n)).round(1), "sorted": np.arange(n, 0, -1.0) * np.ones((1, 2, 1)),
+            "rising": np.arange(n) * np.ones((1, 2, 1)), "tiny": g.random((1, 2, n)) * 1e-42}[fill].astype(F32)
+    if fill == "nan":
+        mass[:, :, ::7] = np.nan
+        mass[:, :, 3::50] = np.inf
+        mass[:, :, 4::50] = -np.inf
+    if fill == "signed":
+        mass[mass == 0] = F32(-0.0)
+        mass[:, :, ::31] = 0
+    for keep in (200, 400, 2400):
+        for dcap in (None, keep):
+            check_evict(hv, k, v, mass, n, 0, keep, keep, 100, dcap)
+
+
+def test_eviction_leaves_impossible_lengths_alone(hv):
+    g = np.random.default_rng(32)
+    k, v = cache(g, 1, 1, 50)
+    mass = some_mass(g, 1, 1, 50)
+    for n in (51, -1, 2 ** 31 - 1):
+        ko, vo, mo, kept, left = run_evict(hv, k, v, mass, n, 0, 40, 30, 5)
+        assert left == n and (kept == -7).all()
+        assert np.array_equal(ko[0, 0], k[0, 0].view(np.uint16)) and np.array_equal(bits(mo), bits(mass))
+    assert run_evict(hv, k, v, mass, 50, 1, 40, 30, 5, want_kept=False)[4] == 30
+
+
+# ---- a run of them together ---------------------------------------------------------------
+
+def test_a_thinned_prompt_shared_by_a_batch(hv):
+    """A prompt's rows with their weights, its cache thinned into another, and a batch over what is
+    left, on one stream without a wait between them."""
+    g = np.random.default_rng(40)
+    nkv, group, n, keep, nseq, tcap = 2, 4, 500, 160, 6, 9
+    nq = nkv * group
+    k, v = cache(g, nkv, n)
+    q, q2 = queries(g, n, nq), queries(g, nseq, nq)
+    tk, tv = cache(g, nseq, nkv, tcap)
+    st = hv.stream_create()
+    d = {x: Dev(y) for x, y in dict(k=k, v=v, q=q, q2=q2, tk=tk, tv=tv, sc=np.array([SCALE], F32),
+                                    n=np.array([n], np.int32), tl=np.full(nseq, tcap, np.int32)).items()}
+    ctx, ctx2, m = Dev(nbytes=q.nbytes), Dev(nbytes=q2.nbytes), Dev(nbytes=nkv * n * 4)
+    kd, vd, md, kept = (Dev(nbytes=nkv * keep * b) for b in (256, 256, 4, 4))
+    left = i32(0)
+    ss = [scratch(x) for x in (hv.attn_mass_scratch(nq, group, n, n), hv.kv_evict_scratch(nkv, n, 1),
+                               hv.attn_shared_scratch(nq, group, keep, tcap, nseq, nseq))]
+    hv.synchronize()
+    hv.attn_rows_mass(d["q"], d["k"], d["v"], ctx, 0, m, d["sc"], 0, nq, HD, group, n, n, ss[0], st)
+    hv.kv_evict(d["k"], d["v"], 0, m, n, d["n"], 0, kd, vd, 0, md, keep, left, kept, keep, keep, 16, nkv, HD,
+                1, ss[1], st)
+    hv.attn_shared(d["q2"], kd, vd, keep, left, d["tk"], d["tv"], tcap, 0, d["tl"], ctx2, d["sc"], nq, HD,
+                   group, nseq, nseq, ss[2], st)
+    hv.stream_synchronize(st)
+    mass = m.get(F32, (nkv, n))
+    idx = np.stack([R.evict(mass[h], n, keep, keep, 16) for h in range(nkv)])
+    assert np.array_equal(kept.get(np.int32, (nkv, keep)), idx)
+    pk, pv = (np.stack([x[h, idx[h]] for h in range(nkv)]) for x in (k, v))
+    near(ctx2.get(F32, q2.shape), *R.shared(q2, pk, pv, keep, tk, tv, None, [tcap] * nseq, SCALE))
+    hv.stream_destroy(st)
