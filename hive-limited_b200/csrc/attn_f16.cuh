@@ -64,4 +64,51 @@ HV_DEV bool span_find(const SpanArgs& a, int r, SpanSeq* x) {
   return r >= x->row && r < x->end;
 }
 
+// The sequences' rows of a call in items of up to kSpanItem (row, head) pairs each, as blocks of a
+// grid: nseq + F / kSpanItem of them, F = nrow * group. The first nseq have each sequence's first
+// pairs; what a sequence has more starts, kSpanItem further every time, in windows of kSpanItem
+// pairs of all, at most one start a window, and that of the sequence that has the window's first.
+// Pairs [f0, f0 + nf) of sequence x; nf 0: nothing for this block.
+constexpr int kSpanItem = 64;
+struct SpanItem {
+  SpanSeq x;
+  int f0, nf;
+};
+HV_DEV SpanItem span_item(const SpanArgs& a, int b) {
+  SpanItem it;
+  it.nf = 0;
+  if (b < a.nseq) {
+    it.x = span_seq(a, b);
+    it.f0 = it.x.row * a.group;
+  } else {
+    const int w = (b - a.nseq) * kSpanItem;
+    if (!span_find(a, w / a.group, &it.x)) return it;
+    const int start = it.x.row * a.group;
+    const int k = (w - start + kSpanItem - 1) / kSpanItem;
+    it.f0 = start + k * kSpanItem;
+    if (k == 0) return it;
+  }
+  it.nf = min(kSpanItem, it.x.end * a.group - it.f0);
+  it.nf = max(it.nf, 0);
+  return it;
+}
+
+// Positions of a chunk when n are cut into at most `most` chunks of whole stages.
+constexpr int kSpanStage = 64;
+HV_HD int span_chunk(int n, int most) {
+  const int c = (n + most - 1) / most;
+  return (c + kSpanStage - 1) / kSpanStage * kSpanStage;
+}
+
+// Partial results of the chunks, in the caller's scratch: slots 0 .. npc - 1 are the prefix's
+// chunks, npc .. npc + ntc - 1 the tails'. part [slot][nkv][F][128], ml [slot][nkv][F]: sums and
+// the sum of the weights 2^(x - m), relative to m.
+struct SpanParts {
+  float* part;
+  float2* ml;
+  float2* stat;                        // [nkv][F]: m and the sum of all, for the weights' sake
+  float* scores;                       // [nq][pcap], of a single row
+  int npc, ntc;
+};
+
 }  // namespace hv

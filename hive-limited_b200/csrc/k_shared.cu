@@ -5,113 +5,430 @@
 //
 //   ctx_h = sum_t w_t v_t / sum_t w_t,   w_t = exp(scale q_h . k_t - max)
 //   mass[g][t] += sum over rows and the heads of kv head g of w_t / sum w
+#include <algorithm>
+
 #include "attn_decode.cuh"
 #include "attn_f16.cuh"
 
 namespace hv {
 namespace {
 
-constexpr int kShWarps = 8;
+// ---- attention of few rows a head ---------------------------------------------------------
+//
+// A CTA has up to 64 (row, head) pairs of a kv head and a chunk of the prefix or of a sequence's
+// tail. Rows stand by eights as the 16-row operand of the f16 tensor pipe, their first binary16
+// terms above their second ones, so that one product serves both and a thread adds what belongs
+// together (the same for the weights of the second product). Warps share the CTA's rows by eights
+// and then its positions, 32 at a time. K and V come by 16-byte asynchronous copies, 64 positions
+// to a stage, swizzled so that eight rows' 16 bytes meet no bank twice.
+constexpr int kPtWarps = 8;
+constexpr int kPtTile = kSpanStage * kHd * 2;            // bytes of K or of V of a stage
+constexpr int kPtQ = kSpanItem * 2 * kHd * 2;            // bytes of the rows' two terms
+constexpr int kPtLine = kHd + 4;                         // floats between rows that are joined
+constexpr float kPtLift = 14.0f;                         // log2 of what weights are multiplied by
+constexpr int kPtStages = 2;
+constexpr int kPtSmem = kPtQ + kPtStages * 2 * kPtTile;
+static_assert(kPtWarps * 8 * kPtLine * 4 <= kPtStages * 2 * kPtTile, "rows to join");
 
-// A CTA per (row, kv head), its warps taking positions in turn, a lane four dims.
-__global__ void __launch_bounds__(32 * kShWarps) k_span_rows(SpanArgs a, float2* __restrict__ stat) {
-  __shared__ float s_m[kShWarps][8], s_l[kShWarps][8];
-  __shared__ __align__(16) float s_o[kShWarps][8][kHd];
-  const int r = blockIdx.x, kvh = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  SpanSeq x;
-  if (!span_find(a, r, &x)) return;
-  const int np = span_prefix(a);
-  float* out = a.ctx + ((size_t)r * a.nq + (size_t)kvh * a.group) * kHd;
-  float2* st = stat + ((size_t)kvh * a.nrow + r) * a.group;
-  if (np < 0 || x.len < 0) {
-    for (int i = threadIdx.x; i < a.group * kHd; i += blockDim.x) out[i] = __int_as_float(0x7fc00000);
-    if (threadIdx.x < a.group) st[threadIdx.x] = make_float2(0.f, __int_as_float(0x7fc00000));
-    return;
-  }
+HV_DEV uint32_t swz(int row, int unit) { return row * 256 + ((unit ^ (row & 7)) << 4); }
+HV_DEV void ldsm(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+HV_DEV void ldsm_t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+HV_DEV void cp16(uint32_t to, const void* from, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+               :: "r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+
+// The two terms of rows f0 .. f0 + nf - 1 of kv head kvh to shared memory, eight rows of first
+// terms, then their second ones; what takes a row's sums of products to exponents to `fac`.
+HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, float* fac, int warp, int warps) {
+  const int lane = threadIdx.x & 31;
   const float f = __ldg(a.scale) * kLog2e;
-  float4 q[8], o[8];
-  float m[8], l[8];
-#pragma unroll
-  for (int h = 0; h < 8; ++h) {
-    if (h < a.group)
-      q[h] = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + h) * kHd) + lane);
-    o[h] = make_float4(0.f, 0.f, 0.f, 0.f);
-    m[h] = -INFINITY;
-    l[h] = 0.f;
-  }
-  const int n = np + x.sees(r);
-  for (int t = warp; t < n; t += kShWarps) {
-    const bool tail = t >= np;
-    const size_t at = tail ? (size_t)x.s * a.t_seq + kvh * a.t_head + (size_t)(t - np) * kHd
-                           : kvh * a.p_head + (size_t)t * kHd;
-    const uint2 kw = reinterpret_cast<const uint2*>((tail ? a.tk : a.pk) + at)[lane];
-    const uint2 vw = reinterpret_cast<const uint2*>((tail ? a.tv : a.pv) + at)[lane];
-    const float2 k0 = __half22float2(*reinterpret_cast<const __half2*>(&kw.x));
-    const float2 k1 = __half22float2(*reinterpret_cast<const __half2*>(&kw.y));
-    const float2 v0 = __half22float2(*reinterpret_cast<const __half2*>(&vw.x));
-    const float2 v1 = __half22float2(*reinterpret_cast<const __half2*>(&vw.y));
-#pragma unroll
-    for (int h = 0; h < 8; ++h) {
-      if (h >= a.group) break;
-      float s = q[h].x * k0.x + q[h].y * k0.y + q[h].z * k1.x + q[h].w * k1.y;
-#pragma unroll
-      for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-      s *= f;
-      const float up = fmaxf(m[h], s), c = m[h] == -INFINITY ? 0.f : ex2(m[h] - up), w = ex2(s - up);
-      m[h] = up;
-      l[h] = l[h] * c + w;
-      o[h].x = o[h].x * c + w * v0.x;
-      o[h].y = o[h].y * c + w * v0.y;
-      o[h].z = o[h].z * c + w * v1.x;
-      o[h].w = o[h].w * c + w * v1.y;
+  for (int i = warp; i < (nf + 7) / 8 * 8; i += warps) {
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < nf) {
+      const int r = (f0 + i) / a.group, h = f0 + i - r * a.group;
+      x = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + h) * kHd) + lane);
     }
-  }
-#pragma unroll
-  for (int h = 0; h < 8; ++h) {
-    if (h >= a.group) break;
-    if (lane == 0) { s_m[warp][h] = m[h]; s_l[warp][h] = l[h]; }
-    reinterpret_cast<float4*>(s_o[warp][h])[lane] = o[h];
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.group * kHd; i += blockDim.x) {
-    const int h = i / kHd, d = i % kHd;
-    float M = -INFINITY, L = 0.f, s = 0.f;
-    for (int w = 0; w < kShWarps; ++w) M = fmaxf(M, s_m[w][h]);
-    for (int w = 0; w < kShWarps; ++w) {
-      const float c = s_l[w][h] == 0.f ? 0.f : ex2(s_m[w][h] - M);
-      L += c * s_l[w][h];
-      s += c * s_o[w][h][d];
-    }
-    out[i] = n == 0 ? 0.f : s / L;
-    if (d == 0) st[h] = make_float2(M, 1.f / L);
+    float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+    m = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m)));
+    const float lift = q8_lift(m);
+    uint2 hi, lo;
+    split_half2(x.x * lift, x.y * lift, &hi.x, &lo.x);
+    split_half2(x.z * lift, x.w * lift, &hi.y, &lo.y);
+    const int at = (i >> 3) * 16 + (i & 7);
+    *reinterpret_cast<uint2*>(to + swz(at, lane >> 1) + 8 * (lane & 1)) = hi;
+    *reinterpret_cast<uint2*>(to + swz(at + 8, lane >> 1) + 8 * (lane & 1)) = lo;
+    if (lane == 0) fac[i] = f / lift;
   }
 }
 
-// A warp per (position, kv head): the weights that the rows give it.
-__global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, const float2* __restrict__ stat,
-                                                   const float* mass_in, float* mass_out, int cap) {
-  const int t = blockIdx.x * 8 + (threadIdx.x >> 5), kvh = blockIdx.y, lane = threadIdx.x & 31;
-  const int np = span_prefix(a);
-  if (np < 0 || t >= np + max(a.tlen, 0)) return;
-  const bool tail = t >= np;
-  const size_t at = tail ? kvh * a.t_head + (size_t)(t - np) * kHd : kvh * a.p_head + (size_t)t * kHd;
-  const uint2 kw = reinterpret_cast<const uint2*>((tail ? a.tk : a.pk) + at)[lane];
-  const float2 k0 = __half22float2(*reinterpret_cast<const __half2*>(&kw.x));
-  const float2 k1 = __half22float2(*reinterpret_cast<const __half2*>(&kw.y));
-  const float f = __ldg(a.scale) * kLog2e;
-  float sum = 0.f;
-  for (int r = tail ? t - np : 0; r < a.nrow; ++r)
-    for (int h = 0; h < a.group; ++h) {
-      const float4 q = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + h) * kHd) + lane);
-      float s = q.x * k0.x + q.y * k0.y + q.z * k1.x + q.w * k1.y;
+__global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ float s_fac[kSpanItem], s_m[kPtWarps][8], s_l[kPtWarps][8];
+  __shared__ int s_bad[kSpanStage];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
+  const int kvh = blockIdx.y, F = a.nrow * a.group;
+  // what this CTA has
+  const __half *k, *v;
+  int f0, nf, p0, p1, slot, lim_all;     // lim_all: positions that every row sees
+  SpanSeq x;
+  const bool prefix = blockIdx.x < (unsigned)(tiles * p.npc);
+  if (prefix) {
+    const int tile = blockIdx.x / p.npc, chunk = blockIdx.x % p.npc;
+    const int np = span_prefix(a), len = span_chunk(np, p.npc);
+    p0 = chunk * len;
+    p1 = min(np, p0 + len);
+    if (p0 >= p1) return;
+    f0 = tile * kSpanItem;
+    nf = min(kSpanItem, F - f0);
+    slot = chunk;
+    k = a.pk + kvh * a.p_head;
+    v = a.pv + kvh * a.p_head;
+    lim_all = p1;
+  } else {
+    const int b = blockIdx.x - tiles * p.npc, chunk = b % p.ntc;
+    const SpanItem it = span_item(a, b / p.ntc);
+    if (it.nf == 0 || it.x.len <= 0) return;
+    x = it.x;
+    f0 = it.f0;
+    nf = it.nf;
+    const int len = span_chunk(x.len, p.ntc);
+    p0 = chunk * len;
+    p1 = min(x.sees((f0 + nf - 1) / a.group), p0 + len);
+    if (p0 >= p1) return;
+    slot = p.npc + chunk;
+    k = a.tk + (size_t)x.s * a.t_seq + kvh * a.t_head;
+    v = a.tv + (size_t)x.s * a.t_seq + kvh * a.t_head;
+    lim_all = min(p1, x.sees(f0 / a.group));
+  }
+  const int ns = (p1 - p0 + kSpanStage - 1) / kSpanStage;
+  const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem), kv_s = sm + kPtQ;
+  auto fetch = [&](int s) {
+    if (s < ns) {
+      const uint32_t to = kv_s + (s % kPtStages) * 2 * kPtTile;
 #pragma unroll
-      for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-      const float2 st = stat[((size_t)kvh * a.nrow + r) * a.group + h];
-      sum += ex2(s * f - st.x) * st.y;
+      for (int i = 0; i < kSpanStage * 16 / (32 * kPtWarps); ++i) {
+        const int u = threadIdx.x + i * 32 * kPtWarps, r = u >> 4, c = u & 15;
+        const int pos = p0 + s * kSpanStage + r;
+        const bool live = pos < p1;
+        const size_t at = (size_t)(live ? pos : p0) * kHd + 8 * c;
+        cp16(to + swz(r, c), k + at, live);
+        cp16(to + kPtTile + swz(r, c), v + at, live);
+      }
     }
-  if (lane == 0) {
-    const size_t i = (size_t)kvh * cap + t;
-    mass_out[i] = (mass_in ? mass_in[i] : 0.f) + sum;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < kPtStages - 1; ++s) fetch(s);
+  rows_split(a, kvh, f0, nf, smem, s_fac, warp, kPtWarps);
+
+  // warps by eights of rows, then by positions
+  const int oct = (nf + 7) / 8;
+  const int wo = oct > 4 ? 8 : oct > 2 ? 4 : oct, wp = kPtWarps / wo;
+  const int o = warp & (wo - 1), pg = warp / wo;
+  const bool mine = o < oct;
+  const int fr = f0 + 8 * o + gl;                          // this thread's row
+  const bool row_live = mine && fr < f0 + nf;
+  const int lim = !row_live ? 0 : prefix ? p1 : min(p1, x.sees(fr / a.group));
+  float m = -INFINITY, l = 0.0f;
+  float acc[16][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+  __syncthreads();
+  const float fac = row_live ? s_fac[8 * o + gl] : 0.0f;
+  const int qr = 16 * o + (lane & 15);                     // ldmatrix rows of the 16-row operand
+  const uint32_t q_at = sm + qr * 256;
+  for (int s = 0; s < ns; ++s) {
+    fetch(s + kPtStages - 1);
+    asm volatile("cp.async.wait_group %0;" :: "n"(kPtStages - 1) : "memory");
+    __syncthreads();
+    const uint32_t kt = kv_s + (s % kPtStages) * 2 * kPtTile, vt = kt + kPtTile;
+    const int base = p0 + s * kSpanStage;
+    const bool partial = lim_all < min(p1, base + kSpanStage);
+    if (partial) {
+      // V of positions that some row does not see must be finite, as 0 times it is added there:
+      // what is not becomes 0 and takes the rows that see it with it
+      if (threadIdx.x < kSpanStage) s_bad[threadIdx.x] = 0;
+      __syncthreads();
+      for (int u = threadIdx.x; u < kSpanStage * 16; u += 32 * kPtWarps) {
+        uint4* w = reinterpret_cast<uint4*>(smem + kPtQ + (s % kPtStages) * 2 * kPtTile + kPtTile + swz(u >> 4, u & 15));
+        const uint4 y = *w;
+        auto odd = [](uint32_t z) { return (z & 0x7C00u) == 0x7C00u || (z & 0x7C000000u) == 0x7C000000u; };
+        if (odd(y.x) || odd(y.y) || odd(y.z) || odd(y.w)) {
+          *w = make_uint4(0, 0, 0, 0);
+          s_bad[u >> 4] = 1;
+        }
+      }
+      __syncthreads();
+    }
+    if (mine) {
+      for (int u = 0; u < 2; ++u) {
+        const int b = base + 32 * u;                       // 32 positions
+        if ((2 * s + u) % wp != pg || b >= p1) continue;
+        float sc[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[j][i] = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {
+          uint32_t qa[4];
+          ldsm(qa, q_at + (((2 * kk + (lane >> 4)) ^ (qr & 7)) << 4));
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t kb[4];
+            const int r = 32 * u + 16 * j + (lane & 7) + ((lane >> 4) << 3);
+            ldsm(kb, kt + swz(r, 2 * kk + ((lane >> 3) & 1)));
+            mma_f16(sc[2 * j], qa, kb[0], kb[1]);
+            mma_f16(sc[2 * j + 1], qa, kb[2], kb[3]);
+          }
+        }
+        float w[8];
+        float up = m;
+        const bool all = b + 32 <= lim_all;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int pos = b + 8 * (j >> 1) + 2 * t + (j & 1);
+          const float y = (sc[j >> 1][j & 1] + sc[j >> 1][2 + (j & 1)]) * fac;
+          w[j] = all || pos < lim ? y : -INFINITY;
+          up = fmaxf(up, w[j]);
+        }
+        if (p.scores && row_live) {
+          float* to = p.scores + ((size_t)kvh * a.group + fr) * a.pcap;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int pos = b + 8 * (j >> 1) + 2 * t + (j & 1);
+            if (pos < p1) to[pos] = w[j];
+          }
+        }
+        up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, 1));
+        up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, 2));
+        if (__any_sync(0xFFFFFFFFu, up > m)) {
+          const float c = m == -INFINITY ? 0.0f : ex2(m - up);
+          l *= c;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] *= c;
+          m = up;
+        }
+        const float m0 = m == -INFINITY ? 0.0f : m - kPtLift;
+        uint32_t wa[2][4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          w[j] = ex2(w[j] - m0);
+          l += w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_half2(w[2 * j], w[2 * j + 1], &wa[j >> 1][2 * (j & 1)], &wa[j >> 1][2 * (j & 1) + 1]);
+        if (partial) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int pos = b + 8 * (j >> 1) + 2 * t + (j & 1);
+            if (pos < lim && s_bad[pos - base]) l = __int_as_float(0x7fc00000);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            uint32_t vb[4];
+            ldsm_t(vb, vt + swz(32 * u + 16 * j + (lane & 15), 2 * d + (lane >> 4)));
+            mma_f16(acc[2 * d], wa[j], vb[0], vb[1]);
+            mma_f16(acc[2 * d + 1], wa[j], vb[2], vb[3]);
+          }
+      }
+    }
+    __syncthreads();
+  }
+  // the warps that share rows meet
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+  l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+  if (t == 0) { s_m[warp][gl] = m; s_l[warp][gl] = l; }
+  float* line = reinterpret_cast<float*>(smem + kPtQ) + (size_t)warp * 8 * kPtLine;
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    *reinterpret_cast<float2*>(line + gl * kPtLine + 8 * i + 2 * t) =
+        make_float2(acc[i][0] + acc[i][2], acc[i][1] + acc[i][3]);
+  __syncthreads();
+  const size_t row = ((size_t)slot * gridDim.y + kvh) * F + f0;
+  for (int i = warp; i < nf; i += kPtWarps) {
+    const int oo = i >> 3, g = i & 7;
+    float M = -INFINITY, L = 0.0f;
+    for (int j = 0; j < wp; ++j) M = fmaxf(M, s_m[oo + j * wo][g]);
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < wp; ++j) {
+      const int w = oo + j * wo;
+      const float c = s_l[w][g] == 0.0f ? 0.0f : ex2(s_m[w][g] - M);
+      const float4 z = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + kPtQ) + (size_t)w * 8 * kPtLine + g * kPtLine + 4 * lane);
+      L += c * s_l[w][g];
+      y.x += c * z.x; y.y += c * z.y; y.z += c * z.z; y.w += c * z.w;
+    }
+    reinterpret_cast<float4*>(p.part + (row + i) * kHd)[lane] = y;
+    if (lane == 0) p.ml[row + i] = make_float2(M - kPtLift, L);
+  }
+}
+
+// A warp per (row, head): its chunks added up.
+__global__ void __launch_bounds__(256) k_span_join(SpanArgs a, SpanParts p) {
+  const int kvh = blockIdx.y, F = a.nrow * a.group, f = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (f >= F) return;
+  const int r = f / a.group;
+  SpanSeq x;
+  if (!span_find(a, r, &x)) return;
+  const int np = span_prefix(a);
+  float4* out = reinterpret_cast<float4*>(a.ctx + ((size_t)r * a.nq + (size_t)kvh * a.group + f - r * a.group) * kHd) + lane;
+  const size_t at = (size_t)kvh * F + f, step = (size_t)gridDim.y * F;
+  const float nan = __int_as_float(0x7fc00000);
+  if (np < 0 || x.len < 0) {
+    *out = make_float4(nan, nan, nan, nan);
+    if (p.stat && lane == 0) p.stat[at] = make_float2(0.f, nan);
+    return;
+  }
+  const int see = x.sees(r);
+  const int n0 = np ? (np + span_chunk(np, p.npc) - 1) / span_chunk(np, p.npc) : 0;
+  const int n1 = see ? (see + span_chunk(x.len, p.ntc) - 1) / span_chunk(x.len, p.ntc) : 0;
+  auto slot = [&](int i) { return i < n0 ? i : p.npc + i - n0; };
+  float M = -INFINITY;
+  for (int i = lane; i < n0 + n1; i += 32) M = fmaxf(M, p.ml[at + slot(i) * step].x);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
+  float L = 0.0f;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = 0; i < n0 + n1; ++i) {
+    const float2 ml = p.ml[at + slot(i) * step];
+    const float4 y = reinterpret_cast<const float4*>(p.part + (at + slot(i) * step) * kHd)[lane];
+    const float c = ml.y == 0.0f ? 0.0f : ex2(ml.x - M);
+    L += c * ml.y;
+    s.x += c * y.x; s.y += c * y.y; s.z += c * y.z; s.w += c * y.w;
+  }
+  const float inv = n0 + n1 ? 1.0f / L : 0.0f;
+  *out = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+  if (p.stat && lane == 0) p.stat[at] = make_float2(M, L);
+}
+
+// The weights of a single row's scores, which k_span_part has left in the scratch.
+__global__ void __launch_bounds__(256) k_mass_dec(SpanArgs a, SpanParts p, const float* mass_in, float* mass_out) {
+  __shared__ float2 s_ml[8];
+  const int kvh = blockIdx.y, np = span_prefix(a), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (np < 0 || (int)blockIdx.x * 256 >= np) return;
+  const int len = span_chunk(np, p.npc), n0 = (np + len - 1) / len;
+  if (warp < a.group) {
+    const size_t at = (size_t)kvh * a.group + warp, step = (size_t)gridDim.y * a.group;
+    float M = -INFINITY, L = 0.0f;
+    for (int i = lane; i < n0; i += 32) M = fmaxf(M, p.ml[at + i * step].x);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
+    for (int i = lane; i < n0; i += 32) {
+      const float2 ml = p.ml[at + i * step];
+      L += ml.y == 0.0f ? 0.0f : ex2(ml.x - M) * ml.y;
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, d);
+    if (lane == 0) s_ml[warp] = make_float2(M, 1.0f / L);
+  }
+  __syncthreads();
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= np) return;
+  float sum = 0.0f;
+  for (int h = 0; h < a.group; ++h)
+    sum += ex2(p.scores[((size_t)kvh * a.group + h) * a.pcap + t] - s_ml[h].x) * s_ml[h].y;
+  const size_t i = (size_t)kvh * a.pcap + t;
+  mass_out[i] = (mass_in ? mass_in[i] : 0.0f) + sum;
+}
+
+// ---- the weights that a run's rows give ------------------------------------------------------
+//
+// w = 2^(x - m) / l once every row's m and l are known, so the scores are formed again, this time
+// with the positions as the 16-row operand: a thread then has two positions and adds up over
+// the columns, the rows. wpos of a CTA's warps have 16 positions each, and wpos warps at a time
+// take the rows in turn, 64 to a stage, split as k_span_part splits them.
+template <int kPos>                                        // warps with positions of their own
+__global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, const float* mass_in, float* mass_out, int cap) {
+  extern __shared__ __align__(1024) uint8_t smem[];         // 64 rows' two terms, then K
+  __shared__ float s_fac[kSpanItem], s_part[8][16];
+  __shared__ float2 s_stat[kSpanItem];
+  constexpr int kN = 16 * kPos;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
+  const int kvh = blockIdx.y, F = a.nrow * a.group, p0 = blockIdx.x * kN;
+  const int n = a.plen + a.tlen;                            // a run's positions, in one cache
+  if (p0 >= n) return;
+  uint8_t* ks = smem + kPtQ;
+  for (int u = threadIdx.x; u < kN * 16; u += 256) {
+    const int r = u >> 4, pos = p0 + r;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (pos < n) x = __ldg(reinterpret_cast<const uint4*>(a.pk + kvh * a.p_head + (size_t)pos * kHd) + (u & 15));
+    *reinterpret_cast<uint4*>(ks + swz(r, u & 15)) = x;
+  }
+  __syncthreads();
+  const int wpos = warp % kPos, wrow = warp / kPos;
+  uint32_t ka[8][4];
+  {
+    const int r = 16 * wpos + (lane & 15);
+    const uint32_t at = (uint32_t)__cvta_generic_to_shared(ks);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) ldsm(ka[k], at + swz(r, 2 * k + (lane >> 4)));
+  }
+  // the first (row, head) pair that sees each of the thread's two positions
+  const int pos_a = p0 + 16 * wpos + gl, pos_b = pos_a + 8;
+  const int see_a = max(0, pos_a - a.plen) * a.group, see_b = max(0, pos_b - a.plen) * a.group;
+  const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(smem);
+  float sum_a = 0.0f, sum_b = 0.0f;
+  const int first = max(0, p0 - a.plen) * a.group / kSpanItem * kSpanItem;   // rows before see none of it
+  for (int f0 = first; f0 < F; f0 += kSpanItem) {
+    const int nf = min(kSpanItem, F - f0);
+    __syncthreads();
+    rows_split(a, kvh, f0, nf, smem, s_fac, warp, 8);
+    if (threadIdx.x < nf) {
+      const float2 s = p.stat[(size_t)kvh * F + f0 + threadIdx.x];
+      s_stat[threadIdx.x] = make_float2(s.x, 1.0f / s.y);
+    }
+    __syncthreads();
+    for (int o = wrow; o < (nf + 7) / 8; o += 8 / kPos) {
+      float c[4] = {0.f, 0.f, 0.f, 0.f}, d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        uint32_t b[4];
+        ldsm(b, q_at + swz(16 * o + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+        mma_f16(d, ka[k], b[2], b[3]);
+        mma_f16(c, ka[k], b[0], b[1]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = 8 * o + 2 * t + i;
+        if (j < nf) {
+          const float fac = s_fac[j];
+          const float2 s = s_stat[j];
+          const float wa = ex2(fmaf(c[i] + d[i], fac, -s.x)), wb = ex2(fmaf(c[2 + i] + d[2 + i], fac, -s.x));
+          if (f0 + j >= see_a) sum_a = fmaf(wa, s.y, sum_a);
+          if (f0 + j >= see_b) sum_b = fmaf(wb, s.y, sum_b);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 1; i < 4; i <<= 1) {
+    sum_a += __shfl_xor_sync(0xFFFFFFFFu, sum_a, i);
+    sum_b += __shfl_xor_sync(0xFFFFFFFFu, sum_b, i);
+  }
+  if (t == 0) { s_part[warp][gl] = sum_a; s_part[warp][gl + 8] = sum_b; }
+  __syncthreads();
+  if (threadIdx.x < kN && p0 + threadIdx.x < n) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 8 / kPos; ++w) s += s_part[(threadIdx.x >> 4) + w * kPos][threadIdx.x & 15];
+    const size_t i = (size_t)kvh * cap + p0 + threadIdx.x;
+    mass_out[i] = (mass_in ? mass_in[i] : 0.0f) + s;
   }
 }
 
@@ -170,17 +487,94 @@ int span_check(const char* name, int nq, int hd, int group, int nseq, int nrow) 
 }
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// How a call's positions are cut, by its capacities (the lengths are on the device): as many
+// chunks as give every SM two CTAs, of a stage at the least.
+constexpr int kPtCtas = 2 * 148;
+struct SpanPlan {
+  int tiles, items, npc, ntc;          // tiles of the prefix's rows, items of the tails'
+  size_t part, ml, stat, scores, bytes;
+};
+SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool mass) {
+  SpanPlan p{};
+  auto stages = [](int n) { return (n + kSpanStage - 1) / kSpanStage; };
+  p.tiles = (F + kSpanItem - 1) / kSpanItem;
+  p.items = nseq + p.tiles;
+  p.npc = std::min(stages(pcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * p.tiles)));
+  p.ntc = std::min(stages(tcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * std::max(nseq, p.tiles))));
+  // room for this call and any smaller one, which may have more chunks of fewer rows: chunks times
+  // tiles (or sequences) are at most kPtCtas / nkv, or one each
+  auto room = [&](int n) {
+    const size_t all = (size_t)nkv * F;
+    return std::min((size_t)stages(n) * all, (size_t)kPtCtas * std::min(F, kSpanItem) + all);
+  };
+  const size_t rows = room(pcap) + room(tcap);
+  auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+  p.part = up(rows * kHd * 4);
+  p.ml = up(rows * 8);
+  p.stat = up(mass ? (size_t)nkv * F * 8 : 0);
+  p.scores = up(mass ? (size_t)nkv * 8 * pcap * 4 : 0);
+  p.bytes = p.part + p.ml + p.stat + p.scores + 256;
+  return p;
+}
+SpanParts span_parts(const SpanPlan& p, void* scratch, bool mass, bool scores) {
+  uint8_t* at = reinterpret_cast<uint8_t*>(scratch);
+  SpanParts s{};
+  s.part = reinterpret_cast<float*>(at);
+  s.ml = reinterpret_cast<float2*>(at + p.part);
+  s.stat = mass ? reinterpret_cast<float2*>(at + p.part + p.ml) : nullptr;
+  s.scores = scores ? reinterpret_cast<float*>(at + p.part + p.ml + p.stat) : nullptr;
+  s.npc = p.npc;
+  s.ntc = p.ntc;
+  return s;
+}
+
+int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const SpanParts& s, cudaStream_t st) {
+  const int rc = smem_attr((const void*)k_span_part, kPtSmem);
+  if (rc) return rc;
+  const unsigned nkv = (unsigned)(a.nq / a.group), F = (unsigned)(a.nrow * a.group);
+  const long long ctas = (long long)p.tiles * p.npc + (long long)p.items * p.ntc;
+  HV_REQUIRE(ctas < (1ll << 31), HV_E_UNSUPPORTED, "%s: too many rows", name);
+  k_span_part<<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, kPtSmem, st>>>(a, s, p.tiles);
+  HV_CUDA(cudaGetLastError());
+  k_span_join<<<dim3((F + 7) / 8, nkv), 256, 0, st>>>(a, s);
+  HV_LAUNCHED(name);
+}
+
+template <int kPos>
+int mass_rows_launch(const char* name, const SpanArgs& a, const SpanParts& s, const float* mass_in, float* mass_out,
+                     int cap, cudaStream_t st) {
+  constexpr int smem = kPtQ + 16 * kPos * kHd * 2;
+  const int rc = smem_attr((const void*)k_mass_rows<kPos>, smem);
+  if (rc) return rc;
+  const unsigned n = (unsigned)(a.plen + a.tlen);
+  k_mass_rows<kPos><<<dim3((n + 16 * kPos - 1) / (16 * kPos), (unsigned)(a.nq / a.group)), 256, smem, st>>>(
+      a, s, mass_in, mass_out, cap);
+  HV_LAUNCHED(name);
+}
+
 int mass_any(const char* name, const SpanArgs& a, const float* mass_in, float* mass_out, int cap,
              void* scratch, cudaStream_t st) {
   HV_REQUIRE(a.q && a.pk && a.pv && a.ctx && a.scale && mass_out && scratch && cap > 0, HV_E_INVALID, "%s: bad arguments", name);
   HV_REQUIRE(cap <= kShMaxCap, HV_E_UNSUPPORTED, "%s: a cache of %d positions", name, cap);
   HV_REQUIRE(aligned16(a.q) && aligned16(a.pk) && aligned16(a.pv) && aligned16(a.ctx) && aligned16(scratch),
              HV_E_INVALID, "%s: unaligned pointer", name);
-  const unsigned nkv = (unsigned)(a.nq / a.group);
-  float2* stat = reinterpret_cast<float2*>(scratch);
-  k_span_rows<<<dim3((unsigned)a.nrow, nkv), 32 * kShWarps, 0, st>>>(a, stat);
-  k_mass_rows<<<dim3((unsigned)((cap + 7) / 8), nkv), 256, 0, st>>>(a, stat, mass_in, mass_out, cap);
-  HV_LAUNCHED(name);
+  const int nkv = a.nq / a.group;
+  const bool one = a.plen_p != nullptr;                     // a single row at a device position
+  const SpanPlan p = span_plan(nkv, a.nrow * a.group, 1, cap, a.tcap, true);
+  SpanParts s = span_parts(p, scratch, true, one);
+  int rc = span_launch(name, a, p, s, st);
+  if (rc) return rc;
+  if (one) {
+    k_mass_dec<<<dim3((unsigned)((cap + 255) / 256), (unsigned)nkv), 256, 0, st>>>(a, s, mass_in, mass_out);
+    HV_LAUNCHED(name);
+  }
+  // a CTA an SM, as far as the positions go
+  const int n = a.plen + a.tlen;
+  auto ctas = [&](int pos) { return (long long)nkv * ((n + 16 * pos - 1) / (16 * pos)); };
+  if (ctas(8) >= 148) return mass_rows_launch<8>(name, a, s, mass_in, mass_out, cap, st);
+  if (ctas(4) >= 148) return mass_rows_launch<4>(name, a, s, mass_in, mass_out, cap, st);
+  if (ctas(2) >= 148) return mass_rows_launch<2>(name, a, s, mass_in, mass_out, cap, st);
+  return mass_rows_launch<1>(name, a, s, mass_in, mass_out, cap, st);
 }
 
 }  // namespace
@@ -195,7 +589,7 @@ extern "C" int hv_attn_shared_scratch(int nq, int group, int pcap, int tcap, int
   HV_REQUIRE(pcap >= 0 && tcap > 0 && bytes, HV_E_INVALID, "hv_attn_shared_scratch: bad arguments");
   HV_REQUIRE(pcap <= kShMaxCap && tcap <= kShMaxCap, HV_E_UNSUPPORTED,
              "hv_attn_shared_scratch: a prefix of %d, tails of %d positions", pcap, tcap);
-  *bytes = (size_t)nq * nrow * sizeof(float2);
+  *bytes = span_plan(nq / group, nrow * group, nseq, pcap, tcap, false).bytes;
   return HV_OK;
 }
 
@@ -224,9 +618,8 @@ extern "C" int hv_attn_shared_f16(const float* q, const uint16_t* pk, const uint
   a.plen_p = pcap ? plen : nullptr; a.row0 = row0; a.tlen_p = tlen;
   a.pcap = pcap; a.tcap = tcap;
   a.nq = nq; a.group = group; a.nseq = nseq; a.nrow = nrow;
-  k_span_rows<<<dim3((unsigned)nrow, (unsigned)nkv), 32 * kShWarps, 0, (cudaStream_t)stream>>>(
-      a, reinterpret_cast<float2*>(scratch));
-  HV_LAUNCHED(name);
+  const SpanPlan p = span_plan((int)nkv, nrow * group, nseq, pcap, tcap, false);
+  return span_launch(name, a, p, span_parts(p, scratch, false, false), (cudaStream_t)stream);
 }
 
 extern "C" int hv_attn_mass_scratch(int nq, int group, int cap, int ntok, size_t* bytes) {
@@ -234,7 +627,7 @@ extern "C" int hv_attn_mass_scratch(int nq, int group, int cap, int ntok, size_t
   if (rc) return rc;
   HV_REQUIRE(cap > 0 && bytes, HV_E_INVALID, "hv_attn_mass_scratch: bad arguments");
   HV_REQUIRE(cap <= kShMaxCap, HV_E_UNSUPPORTED, "hv_attn_mass_scratch: a cache of %d positions", cap);
-  *bytes = (size_t)nq * ntok * sizeof(float2);
+  *bytes = span_plan(nq / group, ntok * group, 1, cap, ntok, true).bytes;
   return HV_OK;
 }
 
