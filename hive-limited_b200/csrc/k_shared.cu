@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(256) k_mass_dec(SpanArgs a, SpanParts p, const
   for (int h = 0; h < a.group; ++h)
     sum += ex2(p.scores[((size_t)kvh * a.group + h) * a.pcap + t] - s_ml[h].x) * s_ml[h].y;
   const size_t i = (size_t)kvh * a.pcap + t;
-  mass_out[i] = (mass_in ? mass_in[i] : 0.0f) + sum;
+  mass_out[i] = (mass_in && t < np - 1 ? mass_in[i] : 0.0f) + sum;
 }
 
 // ---- the weights that a run's rows give ------------------------------------------------------
@@ -428,7 +428,7 @@ __global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, cons
 #pragma unroll
     for (int w = 0; w < 8 / kPos; ++w) s += s_part[(threadIdx.x >> 4) + w * kPos][threadIdx.x & 15];
     const size_t i = (size_t)kvh * cap + p0 + threadIdx.x;
-    mass_out[i] = (mass_in ? mass_in[i] : 0.0f) + s;
+    mass_out[i] = (mass_in && p0 + (int)threadIdx.x < a.plen ? mass_in[i] : 0.0f) + s;
   }
 }
 

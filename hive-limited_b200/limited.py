@@ -155,15 +155,24 @@ class Engine:
                            reference-order attention. Its batched prefill reads the rows of
                            a block that the same run completed quantised, where the
                            token-by-token prefill still read them in f32.
+      kv_keep / kv_recent -- a binary16 cache of bounded size (kv_dtype="f16", fused=False, one
+                           GPU): room for kv_keep + PREFILL_BATCH positions a layer, whatever
+                           max_context is. When it is full, every kv head keeps kv_keep of them,
+                           the last kv_recent (default: a quarter) and those that attention has
+                           given the most weight so far (hv_kv_evict_f16). Attention is the lane's
+                           own (hv_attn_*_mass_f16), with f32 precision, not the reference's order
+                           of operations; when the cache is thinned depends on `prefill`.
     """
 
     kv_q8 = False
-    _sc = None
+    kv_keep = None
+    _sc = _many = None
 
     def __init__(self, model_dir=None, kernels_dir=None, verify_kernels=True, quiet=False, *,
                  config=None, tensors=None, max_context=None, device=0, fused=True,
                  quantize_on="device", world=1, rank=0, exchange=None, weight_cache=None,
-                 cache_tag=None, prefill="steps", kv_dtype="f32", gemv_layout="pp"):
+                 cache_tag=None, prefill="steps", kv_dtype="f32", gemv_layout="pp",
+                 kv_keep=None, kv_recent=None):
         if config is None:
             self.cfg = Config.load(model_dir)
         else:
@@ -187,6 +196,17 @@ class Engine:
         self.kv_dtype = kv_dtype
         self.kv_f16 = kv_dtype == "f16"
         self.kv_q8 = kv_dtype == "q8"
+        if kv_keep is not None:
+            if kv_dtype != "f16" or self.fused or self.world > 1:
+                raise ValueError("kv_keep bounds a binary16 cache of one GPU: pass kv_dtype='f16', "
+                                 "fused=False")
+            kv_recent = kv_keep // 4 if kv_recent is None else kv_recent
+            if not 1 <= kv_keep or not 0 <= kv_recent <= kv_keep:
+                raise ValueError(f"kv_keep={kv_keep}, kv_recent={kv_recent}: at least 1 and 0 to "
+                                 "kv_keep")
+            self.kv_keep, self.kv_recent = int(kv_keep), int(kv_recent)
+        elif kv_recent is not None:
+            raise ValueError("kv_recent goes with kv_keep")
         if gemv_layout not in ("pp", "dq"):
             raise ValueError(f"gemv_layout={gemv_layout!r}: 'pp' or 'dq'")
         self.gemv_layout = gemv_layout
@@ -244,6 +264,15 @@ class Engine:
         p = hvdrv.alloc(max(int(nbytes), 16))
         self._buffers.append(p)
         return p
+
+    def _zeroed(self, nbytes: int) -> int:
+        p = self._alloc(nbytes)
+        hvdrv.memset8(p, 0, max(int(nbytes), 16))
+        return p
+
+    def _release(self, p: int):
+        self._buffers.remove(p)
+        hvdrv.free(p)
 
     def _up(self, arr: np.ndarray) -> int:
         arr = np.ascontiguousarray(arr)
@@ -434,11 +463,11 @@ class Engine:
             self.d_kv = self._alloc(self.kv_bytes)
             self.KC = self.VC = [self.d_kv + l * per for l in range(c.n_layer)]
         else:
-            # KV cache: f32 (or binary16), one allocation, [layer][k|v][n_kv][cap][hd]
+            # KV cache: f32 (or binary16), one allocation, [layer][k|v][n_kv][kv_cap][hd]
             esz = 2 if self.kv_f16 else 4
-            self.kv_bytes = 2 * c.n_layer * nkv * cap * qd * esz
+            self.kv_bytes = 2 * c.n_layer * nkv * self.kv_cap * qd * esz
             self.d_kv = self._alloc(self.kv_bytes)
-            per = nkv * cap * qd * esz
+            per = nkv * self.kv_cap * qd * esz
             self.KC = [self.d_kv + (2 * l) * per for l in range(c.n_layer)]
             self.VC = [self.d_kv + (2 * l + 1) * per for l in range(c.n_layer)]
         hvdrv.memset8(self.d_kv, 0, self.kv_bytes)
@@ -460,6 +489,16 @@ class Engine:
             n = hvdrv.attn_q8_scratch(nq, c.group, cap)
             self.d_q8scr = self._alloc(n)
             hvdrv.memset8(self.d_q8scr, 0, n)
+            return                         # no fused step over this cache
+        if self.kv_keep is not None:
+            # what every position has been given, how many a layer holds, and scratch
+            self.d_mass = self._alloc(c.n_layer * nkv * self.kv_cap * 4)
+            self.d_held = self._alloc(4)
+            self._held = 0                 # the same, as far as the host has followed it
+            hvdrv.memset8(self.d_mass, 0, c.n_layer * nkv * self.kv_cap * 4)
+            self._set_i32(self.d_held, 0)
+            self.d_mass_scr = self._zeroed(hvdrv.attn_mass_scratch(nq, c.group, self.kv_cap, 1))
+            self.d_evict_scr = self._zeroed(hvdrv.kv_evict_scratch(nkv, self.kv_cap, c.n_layer))
             return                         # no fused step over this cache
         hvdrv.attn_reserve(nkv, c.group, cap)
         self._build_desc()
@@ -577,6 +616,13 @@ class Engine:
                 hvdrv.kv_append_q8(dk, dv, self.KC[l], self.d_pos, nkv, qd, cap, s)
                 hvdrv.attn_decode_q8(dq, self.KC[l], self.d_ctx, self.d_scale, self.d_pos, nq,
                                      qd, c.group, cap, self.d_q8scr, s)
+            elif self.kv_keep is not None:
+                # rotated at its position in the text, kept in the next place of the cache
+                hvdrv.kv_append(dk, dv, self.KC[l], self.VC[l], self.d_held, nkv, qd, self.kv_cap,
+                                s, f16=True)
+                hvdrv.attn_decode_mass(dq, self.KC[l], self.VC[l], self.d_ctx, self._mass(l),
+                                       self._mass(l), self.d_scale, self.d_held, nq, qd, c.group,
+                                       self.kv_cap, self.d_mass_scr, s)
             else:
                 hvdrv.kv_append(dk, dv, self.KC[l], self.VC[l], self.d_pos, nkv, qd, cap, s,
                                 f16=self.kv_f16)
@@ -589,8 +635,37 @@ class Engine:
             hvdrv.silu_mul(self.d_gu, self.d_gu + ffn * 4, self.d_act, ffn, s)
             self._gemv(self.d_act, w["down"], self.d_o)
             hvdrv.vadd(self.d_h, self.d_o, self.d_h, hid, s)
+        if self.kv_keep is not None:
+            self._evict(1, self.kv_cap - 1)
         hvdrv.rmsnorm(self.d_h, self.d_hn, self.d_onorm, 1, hid, RMS_EPS, s)
         self._gemv(self.d_hn, self.head, self.d_logits)
+
+    # ---- the bounded cache --------------------------------------------------------------
+
+    @property
+    def kv_cap(self) -> int:
+        """Positions that a layer's cache has room for."""
+        cap = self.cfg.max_context
+        return cap if self.kv_keep is None else min(cap, self.kv_keep + self.PREFILL_BATCH)
+
+    def _mass(self, l: int) -> int:
+        return self.d_mass + l * self.shard["n_kv"] * self.kv_cap * 4
+
+    def _evict(self, added: int, limit: int):
+        """Counts `added` rows written since; thins every layer's cache to kv_keep positions if it
+        then holds more than `limit`."""
+        c, nkv = self.cfg, self.shard["n_kv"]
+        one, keep = nkv * self.kv_cap * c.head_dim, min(self.kv_keep, limit)
+        hvdrv.kv_evict(self.d_kv, self.d_kv + 2 * one, 2 * one, self.d_mass, self.kv_cap, self.d_held,
+                       added, self.d_kv, self.d_kv + 2 * one, 2 * one, self.d_mass, self.kv_cap,
+                       self.d_held, 0, limit, keep, min(self.kv_recent, keep), nkv, c.head_dim,
+                       c.n_layer, self.d_evict_scr, self._stream_cur)
+
+    def _empty_cache(self):
+        """A new text: the bounded cache holds nothing."""
+        if self.kv_keep is not None:
+            self._held = 0
+            self._set_i32(self.d_held, 0)
 
     def _argmax_into_next(self):
         """Pick the next token and advance tok/pos/step on device (limited.py:421-428)."""
@@ -600,9 +675,14 @@ class Engine:
         hvdrv.argmax_final(self.d_pv, self.d_pi, self.d_tok, self.d_gen, self.d_step,
                            self.d_pos, ARGMAX_PARTS, s)
 
-    def _step_fused(self, flags: int):
+    def _no_fused(self):
         if self.kv_q8:
             raise ValueError("the fused step does not run over kv_dtype='q8'")
+        if self.kv_keep is not None:
+            raise ValueError("the fused step does not run over a bounded cache (kv_keep)")
+
+    def _step_fused(self, flags: int):
+        self._no_fused()
         hvdrv._call("hv_step_launch", C.byref(self._desc), int(flags),
                     C.c_void_p(self._stream_cur))
 
@@ -620,8 +700,7 @@ class Engine:
         Returns {"total_us", "phases": {name: {"median_us", "max_us"}}, "raw": ns array
         [grid, stride]} where each phase's duration is taken per CTA and summed over the
         layers (median and max over CTAs)."""
-        if self.kv_q8:
-            raise ValueError("the fused step does not run over kv_dtype='q8'")
+        self._no_fused()
         c = self.cfg
         stride = 10 + 28 * c.n_layer
         n = self.step_grid * stride
@@ -690,12 +769,12 @@ class Engine:
 
     def step_status(self) -> int:
         """Nonzero if a bounded wait inside the fused step ran out (HV_E_TIMEOUT)."""
-        return 0 if self.kv_q8 else self._get_i32(self.d_status)
+        return 0 if self.kv_q8 or self.kv_keep is not None else self._get_i32(self.d_status)
 
     def reset_step_state(self):
         """Clear the fused step's barrier/ticket/status words after a failed launch."""
         hvdrv.synchronize()
-        if self.kv_q8:
+        if self.kv_q8 or self.kv_keep is not None:
             return
         hvdrv.memset8(self.d_barrier, 0, 16)
         hvdrv.memset8(self.d_status, 0, 4)
@@ -752,6 +831,7 @@ class Engine:
         if self.prefill_mode == "batched":
             self._prefill_batched(prompt_ids, argmax=bool(last_flags & STEP_ARGMAX))
             return
+        self._empty_cache()
         self._set_i32(self.d_step, 0)
         hvdrv.memset8(self.d_gen, 0, (self.cfg.max_context + 1) * 4)
         n = len(prompt_ids)
@@ -772,6 +852,8 @@ class Engine:
         wide = max(hid, ffn, nq * qd)
         if self.kv_q8:
             part_b, ticket_b = hvdrv.attn_q8_scratch(nq, c.group, c.max_context, b), 4
+        elif self.kv_keep is not None:
+            part_b, ticket_b = hvdrv.attn_mass_scratch(nq, c.group, self.kv_cap, b), 4
         else:
             part_b, ticket_b = hvdrv.attn_rows_scratch(nq, c.group, c.max_context, b)
         pf = {"n": b, "tok": self._alloc(b * 4), "h": self._alloc(b * hid * 4),
@@ -782,7 +864,7 @@ class Engine:
               "gu": self._alloc(b * 2 * ffn * 4), "act": self._alloc(b * ffn * 4),
               "part": self._alloc(part_b), "ticket": self._alloc(ticket_b)}
         hvdrv.memset8(pf["ticket"], 0, ticket_b)
-        if self.kv_q8:
+        if self.kv_q8 or self.kv_keep is not None:
             hvdrv.memset8(pf["part"], 0, part_b)
         self._pf = pf
         return pf
@@ -800,28 +882,54 @@ class Engine:
         rows into the cache, their final hidden rows (before the last norm) into the
         buffers' "h"."""
         c = self.cfg
-        hid, ffn, qd, nq, nkv, cap = (c.hidden, c.ffn, c.head_dim, c.n_head, c.n_kv,
-                                      c.max_context)
+        qd, nq, nkv, cap = c.head_dim, c.n_head, c.n_kv, self.kv_cap
         pf, m = self._pf, toks.size
         s = self._stream_cur
         hvdrv.synchronize()                 # the host copy below reuses pf["tok"]
         hvdrv.upload(pf["tok"], toks.ctypes.data, 4 * m)
-        hvdrv.gather_rows(self.d_emb16, pf["tok"], pf["h"], hid, m, s)
-        for l, w in enumerate(self.layers):
-            hvdrv.rmsnorm(pf["h"], pf["hn"], w["an"], m, hid, RMS_EPS, s)
-            self._gemm(pf["hn"], w["qkv"], pf["qkv"], m)
+        at = b0                             # where the run's rows go
+        if self.kv_keep is not None:
+            if self._held + m > cap:
+                self._evict(0, cap - m)
+                self._held = min(self.kv_keep, cap - m)
+            at = self._held
+
+        def attend(l, w):
             if self.kv_q8:
                 hvdrv.qk_rows_q8(pf["qkv"], w["qn"], w["kn"], self.d_cos, self.d_sin, b0,
                                  pf["q"], self.KC[l], nq, nkv, qd, cap, RMS_EPS, m, s)
                 hvdrv.attn_rows_q8(pf["q"], self.KC[l], pf["ctx"], self.d_scale, b0, nq, qd,
                                    c.group, cap, m, pf["part"], s)
+                return
+            turn = (b0 - at) * (qd // 2) * 4           # rotation goes by the position in the text
+            hvdrv.qk_rows(pf["qkv"], w["qn"], w["kn"], self.d_cos + turn, self.d_sin + turn, at,
+                          pf["q"], self.KC[l], self.VC[l], nq, nkv, qd, cap, RMS_EPS, m, s,
+                          f16=self.kv_f16)
+            if self.kv_keep is not None:
+                hvdrv.attn_rows_mass(pf["q"], self.KC[l], self.VC[l], pf["ctx"], self._mass(l),
+                                     self._mass(l), self.d_scale, at, nq, qd, c.group, cap, m,
+                                     pf["part"], s)
             else:
-                hvdrv.qk_rows(pf["qkv"], w["qn"], w["kn"], self.d_cos, self.d_sin, b0, pf["q"],
-                              self.KC[l], self.VC[l], nq, nkv, qd, cap, RMS_EPS, m, s,
-                              f16=self.kv_f16)
                 hvdrv.attn_rows(pf["q"], self.KC[l], self.VC[l], pf["ctx"], self.d_scale, b0,
                                 nq, qd, c.group, cap * qd, m, pf["part"], pf["ticket"], s,
                                 f16=self.kv_f16)
+
+        self._run_layers(m, attend)
+        if self.kv_keep is not None:
+            self._held += m
+            self._evict(m, cap)             # counts the rows
+
+    def _run_layers(self, m: int, attend):
+        """The buffers' "tok" (m rows) through every layer; attend(l, w) takes the rows' "qkv" to
+        their "ctx"."""
+        c = self.cfg
+        hid, ffn = c.hidden, c.ffn
+        pf, s = self._pf, self._stream_cur
+        hvdrv.gather_rows(self.d_emb16, pf["tok"], pf["h"], hid, m, s)
+        for l, w in enumerate(self.layers):
+            hvdrv.rmsnorm(pf["h"], pf["hn"], w["an"], m, hid, RMS_EPS, s)
+            self._gemm(pf["hn"], w["qkv"], pf["qkv"], m)
+            attend(l, w)
             self._gemm(pf["ctx"], w["o"], pf["o"], m)
             hvdrv.vadd(pf["h"], pf["o"], pf["h"], m * hid, s)
             hvdrv.rmsnorm(pf["h"], pf["hn"], w["fn"], m, hid, RMS_EPS, s)
@@ -845,6 +953,7 @@ class Engine:
             raise ValueError(f"{n} prompt tokens for a {cap}-token context")
         pf = self._prefill_buffers()
         s = self._stream_cur
+        self._empty_cache()
         self._set_i32(self.d_step, 0)
         hvdrv.memset8(self.d_gen, 0, (cap + 1) * 4)
         m = 0
@@ -1010,6 +1119,7 @@ class Engine:
         if self.prefill_mode == "batched":
             self._prefill_batched(prompt_ids, argmax=False)
         else:
+            self._empty_cache()
             for i, tok in enumerate(prompt_ids):
                 self._prefill_token(tok, i, STEP_HEAD if i == n - 1 else None)
         hvdrv.synchronize()
@@ -1060,6 +1170,7 @@ class Engine:
         pf = self._prefill_buffers()
         sc = self._score_buffers(pf["n"])
         s, v = self._stream_cur, self.n_head_rows
+        self._empty_cache()
         out = {"logprob": np.empty(n - 1, F32), "entropy": np.empty(n - 1, F32),
                "top_ids": np.empty((n - 1, top), np.int32),
                "top_logprobs": np.empty((n - 1, top), F32)}
@@ -1077,6 +1188,200 @@ class Engine:
                 part = out[key][b0:b0 + m]
                 if part.size:
                     hvdrv.download(part.ctypes.data, sc[ptr], part.nbytes)
+        return out
+
+    # ---- many continuations of one prompt ------------------------------------------------
+
+    def _check_many(self, prompt_ids, branches, more: int):
+        """-> the prompt and the branches as arrays of tokens."""
+        c = self.cfg
+        if self.world > 1 or not self.kv_f16:
+            raise ValueError("many continuations run over the binary16 cache of one GPU: "
+                             "kv_dtype='f16'")
+        toks = [np.asarray(x) for x in [prompt_ids, *branches]]
+        for x in toks:
+            if x.ndim != 1 or (x.size and (x.dtype.kind not in "iu" or x.min() < 0
+                                           or x.max() >= c.vocab)):
+                raise ValueError("a token id outside the vocabulary")
+        if not toks[0].size:
+            raise ValueError("prompt_ids is empty")
+        if not 1 <= len(branches) <= self.PREFILL_BATCH:
+            raise ValueError(f"{len(branches)} branches: 1 to {self.PREFILL_BATCH}")
+        most = max(x.size for x in toks[1:])
+        if toks[0].size + most + more > c.max_context:
+            raise ValueError(f"{toks[0].size} prompt + {most} branch + {more} new exceeds the "
+                             f"{c.max_context}-token context of this engine")
+        toks = [np.ascontiguousarray(x, np.int32) for x in toks]
+        return toks[0], toks[1:]
+
+    def _many_buffers(self, nseq: int, tcap: int) -> dict:
+        """Tails of tcap positions for nseq sequences, and what their rows need (allocated on first
+        use, again when more is wanted)."""
+        c = self.cfg
+        mb = self._many
+        if mb is not None and mb["nseq"] >= nseq and mb["tcap"] >= tcap:
+            return mb
+        if mb is not None:
+            hvdrv.synchronize()
+            for k in ("tails", "scr", "hl", "row0", "tlen", "plen", "base"):
+                self._release(mb[k])
+            self._many = None
+        rows, per = self.PREFILL_BATCH, 2 * c.n_kv * c.head_dim * 2
+        n = hvdrv.attn_shared_scratch(c.n_head, c.group, self.kv_cap, tcap, nseq, rows)
+        mb = {"nseq": nseq, "tcap": tcap,
+              "tails": self._alloc(c.n_layer * nseq * tcap * per),
+              "scr": self._zeroed(n), "hl": self._alloc(nseq * c.hidden * 4),
+              "row0": self._alloc((nseq + 1) * 4), "tlen": self._alloc(nseq * 4),
+              "plen": self._alloc(4), "base": self._alloc(4)}
+        self._many = mb
+        return mb
+
+    def _shared_prefix(self, prompt: np.ndarray, mb: dict):
+        """All of the prompt but its last token into the cache: the prefix. Its last token begins
+        every tail."""
+        pf = self._prefill_buffers()
+        self._empty_cache()
+        n = prompt.size - 1
+        for b0 in range(0, n, pf["n"]):
+            self._prefill_run(prompt[b0:min(b0 + pf["n"], n)], b0)
+        self._set_i32(mb["plen"], n if self.kv_keep is None else self._held)
+        self._set_i32(mb["base"], n)
+
+    def _many_run(self, mb: dict, rows: list, tlen: list, toks=None):
+        """The next rows[s] tokens of every sequence (toks, sequence after sequence; None: the
+        buffers' "tok" has them) through every layer; tails then hold tlen[s] positions. Final
+        hidden rows into the buffers' "h"."""
+        c = self.cfg
+        qd, nq, nkv = c.head_dim, c.n_head, c.n_kv
+        pf, s, m = self._pf, self._stream_cur, int(sum(rows))
+        nseq, tcap = len(rows), mb["tcap"]
+        hvdrv.synchronize()                 # the host copies below reuse the buffers
+        if toks is not None:
+            hvdrv.upload(pf["tok"], toks.ctypes.data, 4 * m)
+        row0 = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+        ends = np.ascontiguousarray(tlen, np.int32)
+        hvdrv.upload(mb["row0"], row0.ctypes.data, row0.nbytes)
+        hvdrv.upload(mb["tlen"], ends.ctypes.data, ends.nbytes)
+        one = nseq * nkv * tcap * qd * 2    # bytes of a layer's K tails
+
+        def attend(l, w):
+            tk = mb["tails"] + 2 * l * one
+            hvdrv.qk_shared(pf["qkv"], w["qn"], w["kn"], self.d_cos, self.d_sin, c.max_context,
+                            mb["base"], mb["row0"], mb["tlen"], pf["q"], tk, tk + one, nq, nkv, qd,
+                            tcap, RMS_EPS, nseq, m, s)
+            hvdrv.attn_shared(pf["q"], self.KC[l], self.VC[l], self.kv_cap, mb["plen"], tk, tk + one,
+                              tcap, mb["row0"], mb["tlen"], pf["ctx"], self.d_scale, nq, qd,
+                              c.group, nseq, m, mb["scr"], s)
+
+        self._run_layers(m, attend)
+
+    def _many_prompts(self, mb: dict, texts: list, done):
+        """The tails' first tokens, PREFILL_BATCH rows at a time, sequence after sequence;
+        done(parts): after each run, parts [(sequence, first token, tokens, row)]."""
+        nseq, most = len(texts), self.PREFILL_BATCH
+        have = [0] * nseq
+        s = 0
+        while s < nseq:
+            parts, left, rows = [], most, [0] * nseq
+            while s < nseq and left:
+                n = min(left, texts[s].size - have[s])
+                parts.append((s, have[s], n, most - left))
+                rows[s] = n
+                have[s] += n
+                left -= n
+                if have[s] == texts[s].size:
+                    s += 1
+            toks = np.concatenate([texts[i][lo:lo + n] for i, lo, n, _ in parts])
+            self._many_run(mb, rows, have, np.ascontiguousarray(toks, np.int32))
+            done(parts)
+
+    def generate_many(self, prompt_ids, branches, max_new=64, stop_on_eos=True) -> list:
+        """Greedy continuations of prompt_ids + b for every b of `branches` (which may be empty
+        ones), together: the prompt goes through the model once and its cache is read once a
+        step for all of them (hv_attn_shared_f16), and so are the weights. -> a list of tokens
+        a branch, up to and with the end-of-text token. kv_dtype="f16", one GPU; attention is the
+        lane's own, with f32 precision, so that near ties may fall otherwise than in
+        generate()."""
+        if max_new < 0:
+            raise ValueError(f"max_new={max_new}")
+        prompt, tails = self._check_many(prompt_ids, branches, max_new)
+        c, nseq = self.cfg, len(tails)
+        out = [[] for _ in tails]
+        if max_new == 0:
+            return out
+        texts = [np.concatenate([prompt[-1:], b]) for b in tails]
+        mb = self._many_buffers(nseq, max(x.size for x in texts) + max_new - 1)
+        pf = self._prefill_buffers()
+        sc = self._score_buffers(pf["n"])
+        s, v, hid = self._stream_cur, self.n_head_rows, c.hidden
+        self._shared_prefix(prompt, mb)
+
+        def last_rows(parts):
+            for i, lo, n, row in parts:
+                if lo + n == texts[i].size:
+                    hvdrv.copy_async(mb["hl"] + i * hid * 4, pf["h"] + (row + n - 1) * hid * 4,
+                                     hid * 4, s)
+
+        self._many_prompts(mb, texts, last_rows)
+        live, lens = list(range(nseq)), [x.size for x in texts]
+        src = mb["hl"]
+        for step in range(max_new):
+            m = len(live)
+            hvdrv.rmsnorm(src, pf["hn"], self.d_onorm, m, hid, RMS_EPS, s)
+            self._gemm(pf["hn"], self.head, sc["logits"], m)
+            hvdrv.logprob_rows(sc["logits"], v, m, v, pf["tok"], 1, sc["lp"], sc["ent"], sc["id"],
+                               sc["alt"], sc["scratch"], s)
+            ids = np.empty(m, np.int32)
+            hvdrv.synchronize()
+            hvdrv.download(ids.ctypes.data, sc["id"], ids.nbytes)
+            for i, tok in zip(live, ids):
+                out[i].append(int(tok))
+            stay = [j for j, tok in enumerate(ids) if not (stop_on_eos and tok == c.eos)]
+            live = [live[j] for j in stay]
+            if not live or step == max_new - 1:
+                break
+            for i in live:
+                lens[i] += 1
+            rows = [0] * nseq
+            for i in live:
+                rows[i] = 1
+            self._many_run(mb, rows, lens, np.ascontiguousarray(ids[stay]))
+            src = pf["h"]
+        return out
+
+    def score_many(self, prompt_ids, branches) -> list:
+        """How likely the model finds each text b of `branches` (one token or more) after the
+        prompt: a dict a branch with the log probability of every token of it given all before it
+        ("logprob", f32 [len(b)]) and the entropy of those distributions ("entropy"). The prompt
+        goes through the model once, the branches together, PREFILL_BATCH tokens at a time.
+        kv_dtype="f16", one GPU."""
+        prompt, tails = self._check_many(prompt_ids, branches, 0)
+        if min(x.size for x in tails) == 0:
+            raise ValueError("a branch without a token to score")
+        texts = [np.concatenate([prompt[-1:], b[:-1]]) for b in tails]
+        mb = self._many_buffers(len(tails), max(x.size for x in texts))
+        pf = self._prefill_buffers()
+        sc = self._score_buffers(pf["n"])
+        s, v = self._stream_cur, self.n_head_rows
+        out = [{"logprob": np.empty(b.size, F32), "entropy": np.empty(b.size, F32)} for b in tails]
+        self._shared_prefix(prompt, mb)
+
+        def scored(parts):
+            m = sum(n for _, _, n, _ in parts)
+            want = np.concatenate([tails[i][lo:lo + n] for i, lo, n, _ in parts])
+            want = np.ascontiguousarray(want, np.int32)
+            hvdrv.upload(sc["tok"], want.ctypes.data, want.nbytes)
+            hvdrv.rmsnorm(pf["h"], pf["hn"], self.d_onorm, m, self.cfg.hidden, RMS_EPS, s)
+            self._gemm(pf["hn"], self.head, sc["logits"], m)
+            hvdrv.logprob_rows(sc["logits"], v, m, v, sc["tok"], 0, sc["lp"], sc["ent"], 0, 0,
+                               sc["scratch"], s)
+            hvdrv.synchronize()
+            for key, name in (("logprob", "lp"), ("entropy", "ent")):
+                got = self._download(sc[name], (m,), F32)
+                for i, lo, n, row in parts:
+                    out[i][key][lo:lo + n] = got[row:row + n]
+
+        self._many_prompts(mb, texts, scored)
         return out
 
     def _weight_bits(self) -> tuple[int, int]:

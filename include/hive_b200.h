@@ -344,7 +344,8 @@ int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const float* sca
  *     [nkv][cap][128], one row over positions 0 .. *pos, or row t of ntok over 0 .. pos0 + t, which
  *     also adds up the weights that positions get: mass_out[g][t] = mass_in[g][t] + the sum over
  *     the rows that see t and the query heads of kv head g of t's weight. mass_in, mass_out f32
- *     [nkv][cap], the same one or apart; mass_in NULL counts as 0. Positions that no row sees are
+ *     [nkv][cap], the same one or apart. The rows' own positions (*pos; pos0 on) start at 0,
+ *     whatever mass_in has there, and mass_in NULL is 0 throughout. Positions that no row sees are
  *     left as they are in mass_out. A *pos outside [0, cap) leaves NaN in ctx and mass_out as it
  *     is.                                                                     (fda_warp_pos)
  *   hv_kv_evict_f16  thins nset caches (the layers of a model): cache i has kc, vc

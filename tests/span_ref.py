@@ -61,12 +61,14 @@ def shared(q, pk, pv, plen, tk, tv, row0, tlen, scale):
 def mass(q, k, v, pos0, mass_in, scale):
     """Causal: row t of q [ntok, nq, 128] over positions 0 .. pos0 + t of k, v [nkv, cap, 128] ->
     context, bound, mass [nkv, pos0 + ntok], bound. A mass is a sum of rows * heads weights, each
-    added once (in any order: one u a weight), to mass_in."""
+    added once (in any order: one u a weight), to mass_in, which counts before pos0."""
     ntok, nq, _ = q.shape
     nkv = k.shape[0]
     group, n = nq // nkv, pos0 + ntok
     out, tol = np.empty(q.shape), np.empty(q.shape)
-    m = np.zeros((nkv, n)) if mass_in is None else mass_in[:, :n].astype(np.float64)
+    m = np.zeros((nkv, n))
+    if mass_in is not None:
+        m[:, :pos0] = mass_in[:, :pos0]
     mt = 4 * U * np.abs(m)
     for t in range(ntok):
         for h in range(nq):

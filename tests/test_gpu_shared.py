@@ -548,3 +548,177 @@ def test_a_thinned_prompt_shared_by_a_batch(hv):
     pk, pv = (np.stack([x[h, idx[h]] for h in range(nkv)]) for x in (k, v))
     near(ctx2.get(F32, q2.shape), *R.shared(q2, pk, pv, keep, tk, tv, None, [tcap] * nseq, SCALE))
     hv.stream_destroy(st)
+
+
+# ---- the engine -----------------------------------------------------------------------------
+
+def engine(arch, seed, cap, **kw):
+    import limited
+    import synth
+    import w4format
+    cfg = w4format.Config(arch)
+    return limited.Engine(config=cfg, tensors=synth.iter_tensors(cfg, seed), quiet=True, max_context=cap,
+                          kv_dtype="f16", **kw)
+
+
+def prompt(e, seed, n):
+    import synth
+    return synth.prompt_ids(e.cfg, seed, n)
+
+
+def layer(e, l, cap):
+    c = e.cfg
+    return [e._download(p, (c.n_kv, cap, HD), F16) for p in (e.KC[l], e.VC[l])]
+
+
+@pytest.mark.parametrize("prefill", ["steps", "batched"])
+def test_engine_with_a_bounded_cache(hv, prefill):
+    """The first layer's K and V do not depend on attention: what the bounded cache holds are rows
+    of the whole one, in order, the latest at the end. The last layer's context is attention over
+    what its cache holds. The graph-replayed decode gives the direct one's tokens."""
+    import synth
+    arch = synth.tiny_arch(hidden=512, n_head=8, n_kv=2)
+    n, keep, recent, cap = 500, 96, 24, 600
+    a = engine(arch, 3, cap, fused=False, prefill=prefill, kv_keep=keep, kv_recent=recent)
+    f = engine(arch, 3, cap, fused=False, prefill="batched")
+    try:
+        c, slots = a.cfg, keep + a.PREFILL_BATCH
+        assert a.kv_cap == slots
+        assert a.kv_bytes == c.n_layer * 2 * c.n_kv * slots * HD * 2
+        ids = prompt(a, 3, n)
+        la = a.logits(ids)
+        f.logits(ids)
+        assert np.isfinite(la).all()
+        held = a._get_i32(a.d_held)
+        assert keep <= held < slots
+        whole = layer(f, 0, cap)
+        for h in range(c.n_kv):
+            k, v = (x[h].view(np.uint16) for x in layer(a, 0, slots))
+            kw, vw = (x[h].view(np.uint16) for x in whole)
+            where = {kw[i].tobytes() + vw[i].tobytes(): i for i in range(n)}
+            at = [where[k[i].tobytes() + v[i].tobytes()] for i in range(held)]
+            assert at == sorted(at) and len(set(at)) == held
+            late = recent + held - keep
+            assert at[-late:] == list(range(n - late, n))
+        m = a._download(a._mass(c.n_layer - 1), (c.n_kv, slots), F32)[:, :held]
+        assert np.isfinite(m).all() and (m >= 0).all() and (m > 0).any(1).all()
+        if prefill == "steps":
+            q, ctx = (a._download(x, (c.n_head, HD), F32) for x in (a.d_qkv, a.d_ctx))
+            end = held
+        else:
+            r = (n - 1) % a.PREFILL_BATCH
+            q, ctx = (a._download(a._pf[x] + r * c.n_head * HD * 4, (c.n_head, HD), F32) for x in ("q", "ctx"))
+            end = held
+        k, v = layer(a, c.n_layer - 1, slots)
+        for h in range(c.n_head):
+            want, tol = R.attend(q[h], k[h // c.group, :end], v[h // c.group, :end], float(a.attn_scale))[:2]
+            near(ctx[h], want, tol)
+        toks, _, _ = a.generate(ids[:300], 90, stop_on_eos=False)
+        assert a.generate(ids[:300], 90, stop_on_eos=False, use_graph=True)[0] == toks
+        assert a.generate(ids[:300], 90)[0] == toks
+        for no in (a.profile_step, lambda: a._step_fused(0)):
+            with pytest.raises(ValueError, match="kv_keep"):
+                no()
+        assert a.step_status() == 0
+        s = a.score(ids)
+        assert np.isfinite(s["logprob"]).all()
+    finally:
+        a.free()
+        f.free()
+
+
+def test_bounded_engine_past_the_reference_orders_16384(hv):
+    """Room for 64 + 256 positions while the text goes on past what the reference-order attention
+    can hold."""
+    import synth
+    a = engine(synth.tiny_arch(hidden=256, n_head=10, n_kv=2), 4, 17000, fused=False, prefill="batched",
+               kv_keep=64, kv_recent=64)
+    try:
+        ids = prompt(a, 4, 16500)
+        toks, _, _ = a.generate(ids, 8, stop_on_eos=False)
+        assert len(toks) == 8 and a.kv_cap == 320
+    finally:
+        a.free()
+
+
+def check_many_state(hv, e, ids, branches, plen):
+    """The first layer's tails are the rows that the whole text's cache has there; the last layer's
+    contexts are attention over prefix and tails as they stand."""
+    c, mb, nseq = e.cfg, e._many, len(branches)
+    tcap = mb["tcap"]
+    got = lambda l, which: e._download(  # noqa: E731
+        mb["tails"] + (2 * l + which) * nseq * c.n_kv * tcap * HD * 2, (nseq, c.n_kv, tcap, HD), F16)
+    row0, tlen = (e._download(mb[x], (k,), np.int32) for x, k in (("row0", nseq + 1), ("tlen", nseq)))
+    m = row0[-1]
+    q, ctx = (e._download(e._pf[x], (m, c.n_head, HD), F32) for x in ("q", "ctx"))
+    pk, pv = layer(e, c.n_layer - 1, e.kv_cap)
+    near(ctx, *R.shared(q, pk, pv, plen, got(c.n_layer - 1, 0), got(c.n_layer - 1, 1), row0, tlen,
+                        float(e.attn_scale)))
+    return got(0, 0), got(0, 1), tlen
+
+
+@pytest.mark.parametrize("keep", [None, 120])
+def test_many_continuations(hv, keep):
+    import synth
+    arch = synth.tiny_arch(hidden=512, n_head=8, n_kv=2)
+    cap = 512
+    kw = dict(fused=False, kv_keep=keep) if keep else {}
+    e = engine(arch, 5, cap, **kw)
+    f = engine(arch, 5, cap, fused=False, prefill="batched")
+    try:
+        ids = prompt(e, 5, 400)
+        g = np.random.default_rng(5)
+        branches = [g.integers(0, e.cfg.vocab, n).tolist() for n in (0, 3, 17, 1, 40, 0)]
+        max_new = 6
+        got = e.generate_many(ids, branches, max_new, stop_on_eos=False)
+        assert [len(x) for x in got] == [max_new] * 6 and got[0] == got[5]
+        held = e._held if keep else len(ids) - 1
+        tk, tv, tlen = check_many_state(hv, e, ids, branches, held)
+        assert tlen.tolist() == [1 + len(b) + max_new - 1 for b in branches]
+        for s, b in enumerate(branches):
+            text = ids + b + got[s]
+            f.logits(text)
+            k, v = layer(f, 0, cap)
+            at = slice(len(ids) - 1, len(ids) - 1 + tlen[s])
+            assert np.array_equal(tk[s, :, :tlen[s]].view(np.uint16), k[:, at].view(np.uint16))
+            assert np.array_equal(tv[s, :, :tlen[s]].view(np.uint16), v[:, at].view(np.uint16))
+        assert e.generate_many(ids, branches, max_new, stop_on_eos=False) == got
+        # other sizes after it, and one prompt token (no prefix at all)
+        assert len(e.generate_many(ids[:1], [[5, 6]] * 9, 3, stop_on_eos=False)) == 9
+        e.cfg.eos = got[1][2]
+        stopped = e.generate_many(ids, branches, max_new)
+        for a, b in zip(stopped, got):
+            n = b.index(e.cfg.eos) + 1 if e.cfg.eos in b else max_new
+            assert a == b[:n]
+    finally:
+        e.free()
+        f.free()
+
+
+def test_many_texts_scored(hv):
+    """Over 256 rows in all, so several runs; the log probabilities are those of the logits, and a
+    branch scored twice has the same ones."""
+    import synth
+    e = engine(synth.tiny_arch(hidden=512, n_head=8, n_kv=2), 6, 512)
+    try:
+        ids = prompt(e, 6, 100)
+        g = np.random.default_rng(6)
+        branches = [g.integers(0, e.cfg.vocab, n).tolist() for n in (5, 130, 1, 140, 9)] + [[7, 8, 9, 3, 2]]
+        out = e.score_many(ids, branches)
+        for b, o in zip(branches, out):
+            assert o["logprob"].shape == o["entropy"].shape == (len(b),)
+            assert np.isfinite(o["logprob"]).all() and (o["logprob"] < 0).all()
+        rows = sum(len(b) for b in branches) - 256                   # of the second run
+        x = e._download(e._sc["logits"], (rows, e.n_head_rows), F32).astype(np.float64)
+        lp = x - x.max(1, keepdims=True)
+        lp -= np.log(np.exp(lp).sum(1, keepdims=True))
+        last = branches[-1]
+        want = [lp[rows - len(last) + i, t] for i, t in enumerate(last)]
+        # logits of size |x| are in f32: a log probability is off by a few steps of the largest
+        assert np.abs(out[-1]["logprob"] - want).max() <= 16 * R.U * (np.abs(x).max() + 12)
+        check_many_state(hv, e, ids, branches, len(ids) - 1)
+        again = e.score_many(ids, branches)
+        for a, b in zip(out, again):
+            assert np.array_equal(bits(a["logprob"]), bits(b["logprob"]))
+    finally:
+        e.free()

@@ -125,3 +125,81 @@ def test_plain_eviction():
     assert R.evict(m, 8, 7, 4, 1).tolist() == [1, 2, 5, 7]
     assert R.evict(m, 8, 7, 5, 2).tolist() == [1, 2, 5, 6, 7]
     assert R.evict(m, 7, 5, 3, 3).tolist() == [4, 5, 6]
+
+
+# ---- the engine's arguments -----------------------------------------------------------------
+
+def test_engine_refusals():
+    import limited
+    import synth
+    make = lambda **kw: limited.Engine(config=synth.tiny_arch(), tensors={}, **kw)  # noqa: E731
+    for kw in (dict(kv_keep=64), dict(kv_keep=64, kv_dtype="f16"), dict(kv_keep=64, fused=False),
+               dict(kv_keep=64, kv_dtype="q8", fused=False),
+               dict(kv_keep=0, kv_dtype="f16", fused=False),
+               dict(kv_keep=64, kv_recent=65, kv_dtype="f16", fused=False),
+               dict(kv_keep=64, kv_recent=-1, kv_dtype="f16", fused=False),
+               dict(kv_recent=8, kv_dtype="f16", fused=False)):
+        with pytest.raises(ValueError, match="kv_keep"):
+            make(**kw)
+
+
+def test_many_refusals():
+    """Checked before any device work: an engine without a device will do."""
+    import limited
+    import synth
+    import w4format
+    e = object.__new__(limited.Engine)
+    e.cfg, e.world, e.kv_f16 = w4format.Config(synth.tiny_arch()), 1, True
+    e.cfg.max_context = 64
+    v = e.cfg.vocab
+    for prompt, branches in (([], [[1]]), ([1], []), ([1, v], [[1]]), ([1], [[-1]]), ([1.5], [[1]]),
+                             ([1], [[1]] * 257), ([1] * 60, [[1] * 5]), ([[1]], [[1]])):
+        with pytest.raises(ValueError):
+            e.score_many(prompt, branches)
+        with pytest.raises(ValueError):
+            e.generate_many(prompt, branches, 1)
+    with pytest.raises(ValueError, match="without a token"):
+        e.score_many([1, 2], [[3], []])
+    with pytest.raises(ValueError):
+        e.generate_many([1] * 30, [[1] * 5, []], 30)
+    with pytest.raises(ValueError):
+        e.generate_many([1], [[1]], -1)
+    assert e.generate_many([1], [[1], []], 0) == [[], []]
+    for kw in (dict(kv_f16=False), dict(world=2)):
+        for k, x in kw.items():
+            setattr(e, k, x)
+        with pytest.raises(ValueError, match="f16"):
+            e.score_many([1], [[1]])
+        e.kv_f16 = True
+
+
+def rows_seen(texts, most):
+    """What Engine._many_prompts runs, on a stand-in for the device part."""
+    import limited
+    e = object.__new__(limited.Engine)
+    e.PREFILL_BATCH = most
+    log, parts = [], []
+    e._many_run = lambda mb, rows, tlen, toks: log.append((list(rows), list(tlen), toks.tolist()))
+    e._many_prompts({}, [np.array(t, np.int32) for t in texts], parts.append)
+    return log, parts
+
+
+@pytest.mark.parametrize("sizes,most", [([1], 4), ([3, 1, 4, 2], 4), ([9, 1], 4), ([4, 4], 4),
+                                        ([1] * 9, 4), ([13], 5), ([2, 300, 7], 256)])
+def test_ragged_prompts_go_through_in_order(sizes, most):
+    texts = [[100 * s + i for i in range(n)] for s, n in enumerate(sizes)]
+    log, parts = rows_seen(texts, most)
+    got = [[] for _ in texts]
+    for (rows, tlen, toks), part in zip(log, parts):
+        assert sum(rows) == len(toks) <= most
+        at = 0
+        for s, n in enumerate(rows):                       # rows stand sequence after sequence
+            got[s] += toks[at:at + n]
+            at += n
+            assert tlen[s] == len(got[s])
+        assert [(s, tlen[s] - rows[s], rows[s]) for s in range(len(texts)) if rows[s]] == [
+            p[:3] for p in part]
+        for s, lo, n, row in part:
+            assert toks[row:row + n] == texts[s][lo:lo + n]
+    assert got == texts
+    assert len(log) == -(-sum(sizes) // most)
