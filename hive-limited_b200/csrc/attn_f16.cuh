@@ -3,8 +3,8 @@
 //
 // A row sees a prefix, which every row of the call sees whole, and then part of a tail: the
 // sequence's own positions, up to the row's. hv_attn_shared_f16 has a tail a sequence;
-// hv_attn_rows_mass_f16 is one sequence whose tail is the run itself, behind the positions before
-// it in the same cache; hv_attn_decode_mass_f16 is one row and a prefix.
+// hv_attn_decode_mass_f16 is one row and a prefix; hv_attn_rows_mass_f16 (`run`) is one cache
+// without tails, of which row t sees plen + t + 1 positions.
 #pragma once
 
 #include <cuda_fp16.h>
@@ -25,6 +25,7 @@ struct SpanArgs {
   const int32_t *row0, *tlen_p;        // rows row0[s] .. row0[s + 1] - 1 are sequence s's
   int plen, pmin, pcap, tlen, tcap;    // a prefix of pmin to pcap positions
   int nq, group, nseq, nrow;
+  bool run;
 };
 
 // Positions of the prefix; -1 if it cannot have that many.
@@ -100,15 +101,44 @@ HV_HD int span_chunk(int n, int most) {
   return (c + kSpanStage - 1) / kSpanStage * kSpanStage;
 }
 
-// Partial results of the chunks, in the caller's scratch: slots 0 .. npc - 1 are the prefix's
-// chunks, npc .. npc + ntc - 1 the tails'. part [slot][nkv][F][128], ml [slot][nkv][F]: sums and
-// the sum of the weights 2^(x - m), relative to m.
+// The whole tiles of the prefix that k_span_tile takes: for each tile of kStRows (row, head) pairs
+// the positions that all its rows see, in tiles of kStRows positions. Units of work are (kv head,
+// tile of rows, tile of positions), `tiles` of the last for every tile of rows (a run's first ones
+// have fewer), cut evenly among `ctas` CTAs.
+constexpr int kStRows = 128;
+struct SpanWhole {
+  long long units;
+  int tiles, rows, ctas;
+};
+HV_DEV int span_whole_of(const SpanArgs& a, int np, int tile) {
+  if (np < 0) return 0;
+  return (a.run ? np + tile * kStRows / a.group + 1 : np) / kStRows;
+}
+HV_DEV SpanWhole span_whole(const SpanArgs& a, int np, int grid) {
+  SpanWhole w;
+  w.rows = (a.nrow * a.group + kStRows - 1) / kStRows;
+  w.tiles = span_whole_of(a, np, w.rows - 1);
+  w.units = (long long)(a.nq / a.group) * w.rows * w.tiles;
+  w.ctas = (int)min((long long)grid, w.units);
+  return w;
+}
+// The first CTA with unit u or one behind it: CTA c has units * c / ctas and on.
+HV_DEV int span_cta(const SpanWhole& w, long long u) {
+  return (int)(((u + 1) * w.ctas - 1) / w.units);
+}
+
+// Partial results in the caller's scratch, in slots: nwt for the stretches of k_span_tile (at most
+// that many a tile of rows), npc for the prefix's chunks (or what is left of it), ntc for the
+// tails'. part [slot][nkv][F][128], ml [slot][nkv][F]: sums and the sum of the weights 2^(x - m),
+// relative to m.
 struct SpanParts {
   float* part;
   float2* ml;
   float2* stat;                        // [nkv][F]: m and the sum of all, for the weights' sake
   float* scores;                       // [nq][pcap], of a single row
-  int npc, ntc;
+  int nwt, npc, ntc, grid;             // grid: CTAs of k_span_tile
 };
+
+int span_tile_launch(const SpanArgs& a, const SpanParts& p, cudaStream_t st);
 
 }  // namespace hv

@@ -68,6 +68,19 @@ HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, 
   }
 }
 
+// What k_span_part has of the prefix for the rows of a tile of kSpanItem: all, or what k_span_tile
+// leaves. A run's end goes by the tile's last row.
+struct SpanRest {
+  int start, end;
+};
+HV_DEV SpanRest span_rest(const SpanArgs& a, const SpanParts& p, int tile) {
+  const int np = span_prefix(a);
+  SpanRest r;
+  r.start = p.nwt ? span_whole_of(a, np, tile * kSpanItem / kStRows) * kStRows : 0;
+  r.end = a.run ? np + (min(a.nrow * a.group, (tile + 1) * kSpanItem) - 1) / a.group + 1 : np;
+  return r;
+}
+
 __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles) {
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ float s_fac[kSpanItem], s_m[kPtWarps][8], s_l[kPtWarps][8];
@@ -81,16 +94,17 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
   const bool prefix = blockIdx.x < (unsigned)(tiles * p.npc);
   if (prefix) {
     const int tile = blockIdx.x / p.npc, chunk = blockIdx.x % p.npc;
-    const int np = span_prefix(a), len = span_chunk(np, p.npc);
-    p0 = chunk * len;
-    p1 = min(np, p0 + len);
+    const SpanRest rest = span_rest(a, p, tile);
+    const int len = span_chunk(rest.end - rest.start, p.npc);
+    p0 = rest.start + chunk * len;
+    p1 = min(rest.end, p0 + len);
     if (p0 >= p1) return;
     f0 = tile * kSpanItem;
     nf = min(kSpanItem, F - f0);
-    slot = chunk;
+    slot = p.nwt + chunk;
     k = a.pk + kvh * a.p_head;
     v = a.pv + kvh * a.p_head;
-    lim_all = p1;
+    lim_all = a.run ? min(p1, a.plen + f0 / a.group + 1) : p1;
   } else {
     const int b = blockIdx.x - tiles * p.npc, chunk = b % p.ntc;
     const SpanItem it = span_item(a, b / p.ntc);
@@ -102,7 +116,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
     p0 = chunk * len;
     p1 = min(x.sees((f0 + nf - 1) / a.group), p0 + len);
     if (p0 >= p1) return;
-    slot = p.npc + chunk;
+    slot = p.nwt + p.npc + chunk;
     k = a.tk + (size_t)x.s * a.t_seq + kvh * a.t_head;
     v = a.tv + (size_t)x.s * a.t_seq + kvh * a.t_head;
     lim_all = min(p1, x.sees(f0 / a.group));
@@ -135,7 +149,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
   const bool mine = o < oct;
   const int fr = f0 + 8 * o + gl;                          // this thread's row
   const bool row_live = mine && fr < f0 + nf;
-  const int lim = !row_live ? 0 : prefix ? p1 : min(p1, x.sees(fr / a.group));
+  const int lim = !row_live ? 0 : a.run ? min(p1, a.plen + fr / a.group + 1) : prefix ? p1 : min(p1, x.sees(fr / a.group));
   float m = -INFINITY, l = 0.0f;
   float acc[16][4];
 #pragma unroll
@@ -294,25 +308,42 @@ __global__ void __launch_bounds__(256) k_span_join(SpanArgs a, SpanParts p) {
     if (p.stat && lane == 0) p.stat[at] = make_float2(0.f, nan);
     return;
   }
-  const int see = x.sees(r);
-  const int n0 = np ? (np + span_chunk(np, p.npc) - 1) / span_chunk(np, p.npc) : 0;
-  const int n1 = see ? (see + span_chunk(x.len, p.ntc) - 1) / span_chunk(x.len, p.ntc) : 0;
-  auto slot = [&](int i) { return i < n0 ? i : p.npc + i - n0; };
+  // its stretches of whole tiles, its chunks of the rest, its chunks of the tail
+  int nw = 0, n0 = 0, n1 = 0;
+  if (p.nwt) {
+    const SpanWhole wh = span_whole(a, np, p.grid);
+    const int tile = f / kStRows, whole = span_whole_of(a, np, tile);
+    if (whole) {
+      const long long u = ((long long)kvh * wh.rows + tile) * wh.tiles;
+      nw = span_cta(wh, u + whole - 1) - span_cta(wh, u) + 1;
+    }
+  }
+  if (p.npc) {
+    const SpanRest rest = span_rest(a, p, f / kSpanItem);
+    const int end = a.run ? a.plen + r + 1 : rest.end, len = span_chunk(rest.end - rest.start, p.npc);
+    if (end > rest.start) n0 = (end - rest.start + len - 1) / len;
+  }
+  if (p.ntc) {
+    const int see = x.sees(r);
+    if (see) n1 = (see + span_chunk(x.len, p.ntc) - 1) / span_chunk(x.len, p.ntc);
+  }
+  auto slot = [&](int i) { return i < nw ? i : i < nw + n0 ? p.nwt + i - nw : p.nwt + p.npc + i - nw - n0; };
+  const int all = nw + n0 + n1;
   float M = -INFINITY;
-  for (int i = lane; i < n0 + n1; i += 32) M = fmaxf(M, p.ml[at + slot(i) * step].x);
+  for (int i = lane; i < all; i += 32) M = fmaxf(M, p.ml[at + slot(i) * step].x);
 #pragma unroll
   for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
   float L = 0.0f;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int i = 0; i < n0 + n1; ++i) {
+  for (int i = 0; i < all; ++i) {
     const float2 ml = p.ml[at + slot(i) * step];
     const float4 y = reinterpret_cast<const float4*>(p.part + (at + slot(i) * step) * kHd)[lane];
     const float c = ml.y == 0.0f ? 0.0f : ex2(ml.x - M);
     L += c * ml.y;
     s.x += c * y.x; s.y += c * y.y; s.z += c * y.z; s.w += c * y.w;
   }
-  const float inv = n0 + n1 ? 1.0f / L : 0.0f;
+  const float inv = all ? 1.0f / L : 0.0f;
   *out = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
   if (p.stat && lane == 0) p.stat[at] = make_float2(M, L);
 }
@@ -361,7 +392,7 @@ __global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, cons
   constexpr int kN = 16 * kPos;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, F = a.nrow * a.group, p0 = blockIdx.x * kN;
-  const int n = a.plen + a.tlen;                            // a run's positions, in one cache
+  const int n = a.plen + a.nrow;
   if (p0 >= n) return;
   uint8_t* ks = smem + kPtQ;
   for (int u = threadIdx.x; u < kN * 16; u += 256) {
@@ -489,25 +520,31 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // How a call's positions are cut, by its capacities (the lengths are on the device): as many
 // chunks as give every SM two CTAs, of a stage at the least.
-constexpr int kPtCtas = 2 * 148;
+constexpr int kSms = 148, kPtCtas = 2 * kSms;
 struct SpanPlan {
-  int tiles, items, npc, ntc;          // tiles of the prefix's rows, items of the tails'
+  int tiles, items, nwt, npc, ntc;     // tiles of the prefix's rows, items of the tails'
   size_t part, ml, stat, scores, bytes;
 };
-SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool mass) {
+SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool mass) {
   SpanPlan p{};
   auto stages = [](int n) { return (n + kSpanStage - 1) / kSpanStage; };
   p.tiles = (F + kSpanItem - 1) / kSpanItem;
   p.items = nseq + p.tiles;
-  p.npc = std::min(stages(pcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * p.tiles)));
-  p.ntc = std::min(stages(tcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * std::max(nseq, p.tiles))));
+  // many rows over many positions go by whole tiles
+  if (F > 64 && (long long)F * pcap >= 1 << 18) {
+    const long long rows = (long long)nkv * ((F + kStRows - 1) / kStRows);
+    p.nwt = (int)std::min((long long)(pcap / kStRows), kSms / rows + 2);
+  }
+  p.npc = std::min(stages(p.nwt ? 2 * kStRows : pcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * p.tiles)));
+  if (!run) p.ntc = std::min(stages(tcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * std::max(nseq, p.tiles))));
   // room for this call and any smaller one, which may have more chunks of fewer rows: chunks times
   // tiles (or sequences) are at most kPtCtas / nkv, or one each
+  const size_t all = (size_t)nkv * F;
   auto room = [&](int n) {
-    const size_t all = (size_t)nkv * F;
     return std::min((size_t)stages(n) * all, (size_t)kPtCtas * std::min(F, kSpanItem) + all);
   };
-  const size_t rows = room(pcap) + room(tcap);
+  const size_t whole = std::min((size_t)(pcap / kStRows) * all, (size_t)kSms * std::min(F, kStRows) + 2 * all);
+  const size_t rows = whole + room(pcap) + (run ? 0 : room(tcap));
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   p.part = up(rows * kHd * 4);
   p.ml = up(rows * 8);
@@ -523,13 +560,16 @@ SpanParts span_parts(const SpanPlan& p, void* scratch, bool mass, bool scores) {
   s.ml = reinterpret_cast<float2*>(at + p.part);
   s.stat = mass ? reinterpret_cast<float2*>(at + p.part + p.ml) : nullptr;
   s.scores = scores ? reinterpret_cast<float*>(at + p.part + p.ml + p.stat) : nullptr;
+  s.nwt = p.nwt;
   s.npc = p.npc;
   s.ntc = p.ntc;
+  s.grid = kSms;
   return s;
 }
 
 int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const SpanParts& s, cudaStream_t st) {
-  const int rc = smem_attr((const void*)k_span_part, kPtSmem);
+  int rc = smem_attr((const void*)k_span_part, kPtSmem);
+  if (!rc && s.nwt) rc = span_tile_launch(a, s, st);
   if (rc) return rc;
   const unsigned nkv = (unsigned)(a.nq / a.group), F = (unsigned)(a.nrow * a.group);
   const long long ctas = (long long)p.tiles * p.npc + (long long)p.items * p.ntc;
@@ -546,7 +586,7 @@ int mass_rows_launch(const char* name, const SpanArgs& a, const SpanParts& s, co
   constexpr int smem = kPtQ + 16 * kPos * kHd * 2;
   const int rc = smem_attr((const void*)k_mass_rows<kPos>, smem);
   if (rc) return rc;
-  const unsigned n = (unsigned)(a.plen + a.tlen);
+  const unsigned n = (unsigned)(a.plen + a.nrow);
   k_mass_rows<kPos><<<dim3((n + 16 * kPos - 1) / (16 * kPos), (unsigned)(a.nq / a.group)), 256, smem, st>>>(
       a, s, mass_in, mass_out, cap);
   HV_LAUNCHED(name);
@@ -560,7 +600,7 @@ int mass_any(const char* name, const SpanArgs& a, const float* mass_in, float* m
              HV_E_INVALID, "%s: unaligned pointer", name);
   const int nkv = a.nq / a.group;
   const bool one = a.plen_p != nullptr;                     // a single row at a device position
-  const SpanPlan p = span_plan(nkv, a.nrow * a.group, 1, cap, a.tcap, true);
+  const SpanPlan p = span_plan(nkv, a.nrow * a.group, 1, cap, 0, true, true);
   SpanParts s = span_parts(p, scratch, true, one);
   int rc = span_launch(name, a, p, s, st);
   if (rc) return rc;
@@ -569,7 +609,7 @@ int mass_any(const char* name, const SpanArgs& a, const float* mass_in, float* m
     HV_LAUNCHED(name);
   }
   // a CTA an SM, as far as the positions go
-  const int n = a.plen + a.tlen;
+  const int n = a.plen + a.nrow;
   auto ctas = [&](int pos) { return (long long)nkv * ((n + 16 * pos - 1) / (16 * pos)); };
   if (ctas(8) >= 148) return mass_rows_launch<8>(name, a, s, mass_in, mass_out, cap, st);
   if (ctas(4) >= 148) return mass_rows_launch<4>(name, a, s, mass_in, mass_out, cap, st);
@@ -589,7 +629,7 @@ extern "C" int hv_attn_shared_scratch(int nq, int group, int pcap, int tcap, int
   HV_REQUIRE(pcap >= 0 && tcap > 0 && bytes, HV_E_INVALID, "hv_attn_shared_scratch: bad arguments");
   HV_REQUIRE(pcap <= kShMaxCap && tcap <= kShMaxCap, HV_E_UNSUPPORTED,
              "hv_attn_shared_scratch: a prefix of %d, tails of %d positions", pcap, tcap);
-  *bytes = span_plan(nq / group, nrow * group, nseq, pcap, tcap, false).bytes;
+  *bytes = span_plan(nq / group, nrow * group, nseq, pcap, tcap, false, false).bytes;
   return HV_OK;
 }
 
@@ -618,7 +658,7 @@ extern "C" int hv_attn_shared_f16(const float* q, const uint16_t* pk, const uint
   a.plen_p = pcap ? plen : nullptr; a.row0 = row0; a.tlen_p = tlen;
   a.pcap = pcap; a.tcap = tcap;
   a.nq = nq; a.group = group; a.nseq = nseq; a.nrow = nrow;
-  const SpanPlan p = span_plan((int)nkv, nrow * group, nseq, pcap, tcap, false);
+  const SpanPlan p = span_plan((int)nkv, nrow * group, nseq, pcap, tcap, false, false);
   return span_launch(name, a, p, span_parts(p, scratch, false, false), (cudaStream_t)stream);
 }
 
@@ -627,7 +667,7 @@ extern "C" int hv_attn_mass_scratch(int nq, int group, int cap, int ntok, size_t
   if (rc) return rc;
   HV_REQUIRE(cap > 0 && bytes, HV_E_INVALID, "hv_attn_mass_scratch: bad arguments");
   HV_REQUIRE(cap <= kShMaxCap, HV_E_UNSUPPORTED, "hv_attn_mass_scratch: a cache of %d positions", cap);
-  *bytes = span_plan(nq / group, ntok * group, 1, cap, ntok, true).bytes;
+  *bytes = span_plan(nq / group, ntok * group, 1, cap, 0, true, true).bytes;
   return HV_OK;
 }
 
@@ -660,10 +700,9 @@ extern "C" int hv_attn_rows_mass_f16(const float* q, const uint16_t* kc, const u
   SpanArgs a{};
   a.q = q; a.ctx = ctx; a.scale = scale;
   a.pk = reinterpret_cast<const __half*>(kc); a.pv = reinterpret_cast<const __half*>(vc);
-  a.p_head = a.t_head = (size_t)cap * kHd;
-  if (kc && vc) { a.tk = a.pk + (size_t)pos0 * kHd; a.tv = a.pv + (size_t)pos0 * kHd; }
+  a.p_head = (size_t)cap * kHd;
   a.plen = pos0; a.pcap = cap;
-  a.tlen = a.tcap = ntok;
+  a.run = true;
   a.nq = nq; a.group = group; a.nseq = 1; a.nrow = ntok;
   return mass_any(name, a, mass_in, mass_out, cap, scratch, (cudaStream_t)stream);
 }

@@ -323,9 +323,10 @@ int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const float* sca
  * in an order of its own (no counterpart in the reference). hd must be 128, query head h reads kv
  * head h / group, group 1 to 8. q and ctx [rows][nq][128] f32; every pointer to such rows or to
  * cache rows is 16-byte aligned. Contexts are softmax(scale q k^T) v with f32 sums: queries and
- * weights count to 2^-22 of themselves and at least to 2^-38 of a row's largest, weights under
- * 2^-126 of the largest are 0. A position whose K or V holds an infinity or a NaN leaves
- * infinities or NaN in contexts (and weights) of the queries that see it, and of no others.
+ * weights count to 2^-22 of themselves, a query's values at least to 2^-38 of its largest and a
+ * row's weights to 2^-31 of theirs; weights under 2^-126 of the largest are 0. Contexts (and
+ * weights) of queries that see a position whose K or V holds an infinity or a NaN are not
+ * defined; those of others do not depend on it.
  *
  *   hv_attn_shared_f16  attention of a batch of sequences that share a prefix, which is read once
  *     for all of them. The prefix: *plen positions of pk, pv [nkv][pcap][128] (0 to pcap; with

@@ -20,7 +20,10 @@ def attend(q, k, v, scale):
     2^x and the quotient themselves. The weighted sum adds each of the n positions once in tiles
     of at least 16: (n / 8 + 64) u of sum w |v| covers it with the sum of the weights.
     A weight enters the second product as two binary16 terms and is then exact to 2^-22 (in the
-    64 u) or to 2^-36 of the largest weight: 2^-36 n max w max|v|."""
+    64 u) or to half of binary16's smallest step, 2^-25. At the least it stands as 2^8 times itself
+    over 2^m, m a whole number at most 1 over the largest exponent so far, which is 2^-32 of the
+    largest weight, and where m rose meanwhile what stood was scaled down, another 2^-32:
+    2^-31 n max w max|v|."""
     n = len(k)
     if n == 0:
         return np.zeros(HD), np.full(HD, 1e-37), np.zeros(0), np.zeros(0)
@@ -30,7 +33,7 @@ def attend(q, k, v, scale):
     w = np.exp(x - x.max())
     w /= w.sum()
     off = 96 * U * big + 4 * U
-    tol = (off + (n / 8 + 64) * U) * (w @ np.abs(v)) + 2.0 ** -36 * n * w.max() * np.abs(v).max(0)
+    tol = (off + (n / 8 + 64) * U) * (w @ np.abs(v)) + 2.0 ** -31 * n * w.max() * np.abs(v).max(0)
     return w @ v, tol + 1e-37, w, off * w + (n / 8 + 64) * U * w + 2.0 ** -124
 
 

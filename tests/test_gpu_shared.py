@@ -87,6 +87,34 @@ def test_runs_of_rows(hv, nkv, group, plen, rows, tails):
     check_shared(hv, g, nkv, group, plen, plen + 3, rows, tails, max(tails) + 1, extra=2)
 
 
+@pytest.mark.parametrize("nkv,group,nseq,plen", [
+    (1, 1, 129, 2100), (2, 3, 50, 2500), (1, 5, 70, 1024), (8, 4, 64, 1100), (3, 7, 40, 1500),
+    (1, 8, 64, 4097), (1, 2, 65, 2176), (1, 4, 40, 12800)])
+def test_many_rows_over_a_long_prefix(hv, nkv, group, nseq, plen):
+    g = np.random.default_rng(plen)
+    check_shared(hv, g, nkv, group, plen, plen + 130, [1] * nseq, [1 + i % 7 for i in range(nseq)], 9, one=True)
+
+
+@pytest.mark.parametrize("nseq", [3, 70])
+@pytest.mark.parametrize("way", ["rising", "falling", "steps", "peaks", "far"])
+def test_scores_that_change_along_the_prefix(hv, nseq, way):
+    """The largest score so far is passed often, seldom, by a little and by far."""
+    g = np.random.default_rng(13)
+    plen, nkv, group = 2300, 1, 4
+    pk, pv = cache(g, nkv, plen)
+    tk, tv = cache(g, nseq, nkv, 4)
+    q = queries(g, nseq, nkv * group)
+    u = g.standard_normal(HD)
+    u /= np.sqrt(HD)
+    t = np.arange(plen)
+    size = {"rising": 0.05 * t, "falling": -0.05 * t, "steps": 12.0 * (t // 100), "peaks": 150.0 * (t % 331 == 330) * (t / plen),
+            "far": np.where(t == 1777, 4000.0, -0.02 * t)}[way]
+    pk = (pk * 0.2 + size[None, :, None] * u).astype(F16)
+    q += (u * np.sqrt(HD) * 0.9).astype(F32)
+    got = run_shared(hv, q, pk, pv, plen, tk, tv, None, [4] * nseq)
+    near(got, *R.shared(q, pk, pv, plen, tk, tv, None, [4] * nseq, SCALE))
+
+
 def test_a_prefix_of_full_capacity_and_none_at_all(hv):
     g = np.random.default_rng(5)
     check_shared(hv, g, 2, 4, 256, 256, [1] * 20, [8] * 20, 8, one=True)
@@ -101,7 +129,7 @@ def test_rows_that_see_nothing_are_zero(hv):
     check_shared(hv, g, 1, 8, 40, 64, [5, 1], [2, 0], 4)
 
 
-@pytest.mark.parametrize("rows,plen", [([1] * 4, 200), ([1] * 40, 600), ([6, 4], 300)])
+@pytest.mark.parametrize("rows,plen", [([1] * 4, 200), ([1] * 40, 600), ([6, 4], 300), ([1] * 40, 2000)])
 def test_lengths_out_of_range_leave_nan(hv, rows, plen):
     g = np.random.default_rng(7)
     nseq = len(rows)
@@ -150,7 +178,7 @@ def test_what_a_row_does_not_see_does_not_count(hv, which, bad):
                                          (0.0, 1.0, 1.0), (1.0, 2e4, 1e-3), (1e-30, 3e34, 1.0)])
 def test_queries_and_scales_of_any_size(hv, scale, qs, ks):
     g = np.random.default_rng(9)
-    for nseq, plen in ((3, 300), (40, 300)):
+    for nseq, plen in ((3, 300), (40, 300), (40, 2000)):
         pk, pv = cache(g, 1, plen)
         tk, tv = cache(g, nseq, 1, 40)
         pk, tk = (pk * F16(ks)).astype(F16), (tk * F16(ks)).astype(F16)
@@ -344,7 +372,8 @@ def test_decode_with_mass(hv, nkv, group, n, form):
 
 @pytest.mark.parametrize("nkv,group,pos0,ntok", [
     (1, 1, 0, 1), (2, 4, 0, 5), (8, 2, 256, 44), (1, 8, 100, 17), (2, 5, 63, 65), (1, 3, 1000, 31),
-    (2, 4, 128, 128), (1, 8, 700, 256), (2, 1, 0, 300), (1, 2, 2048, 200), (1, 7, 4000, 3)])
+    (2, 4, 128, 128), (1, 8, 700, 256), (2, 1, 0, 300), (1, 2, 2048, 200), (1, 7, 4000, 3),
+    (1, 1, 900, 290), (2, 5, 500, 120), (1, 3, 0, 700)])
 def test_run_with_mass(hv, nkv, group, pos0, ntok):
     g = np.random.default_rng(pos0 + ntok)
     check_mass(hv, g, nkv, group, pos0, ntok, pos0 + ntok + 2, False, "apart")
@@ -377,8 +406,8 @@ def test_decode_with_mass_outside_the_cache(hv):
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
 def test_mass_of_rows_before_a_bad_position(hv, bad):
     g = np.random.default_rng(22)
-    for group, ntok in ((4, 30), (8, 100)):
-        k, v = cache(g, 1, 200)
+    for group, ntok, cap in ((4, 30, 200), (8, 100, 200), (8, 100, 2000)):
+        k, v = cache(g, 1, cap)
         q = queries(g, ntok, group)
         want, tol, _, _ = R.mass(q, k, v, 60, None, SCALE)
         v[0, 60 + 11] = bad
