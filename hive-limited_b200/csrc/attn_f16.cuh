@@ -7,6 +7,7 @@
 // without tails, of which row t sees plen + t + 1 positions.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_fp16.h>
 
 #include "attn_q8.cuh"
@@ -136,9 +137,28 @@ struct SpanParts {
   float2* ml;
   float2* stat;                        // [nkv][F]: m and the sum of all, for the weights' sake
   float* scores;                       // [nq][pcap], of a single row
+  // what k_mass_tile reads of the rows: their two binary16 terms [2][nkv][F][128]; and, F rounded
+  // up to whole tiles, what takes their sums of products to exponents, -m and 1 / l, 0 behind F
+  __half* terms;
+  float* facs;
   int nwt, npc, ntc, grid;             // grid: CTAs of k_span_tile
 };
 
+// Tensor copies of boxes of kStRows rows by 64 values of [outer][rows][128], rows of 128 bytes in
+// shared memory, swizzled; rows past the end are zeros.
+int f16_rows_map(const __half* base, int rows, int outer, CUtensorMap* out);
+HV_DEV void tile_copy(uint32_t to, const CUtensorMap* map, int dim, int pos, int head, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+      "[%0], [%1, {%2, %3, %4}], [%5];"
+      :: "r"(to), "l"(map), "r"(dim), "r"(pos), "r"(head), "r"(bar) : "memory");
+}
+HV_DEV void bar_expect(uint32_t bar, int bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+
 int span_tile_launch(const SpanArgs& a, const SpanParts& p, cudaStream_t st);
+int mass_tile_launch(const SpanArgs& a, const SpanParts& p, const float* mass_in, float* mass_out, int cap,
+                     cudaStream_t st);
 
 }  // namespace hv

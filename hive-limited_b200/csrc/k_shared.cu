@@ -44,6 +44,17 @@ HV_DEV void cp16(uint32_t to, const void* from, bool live) {
                :: "r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
 }
 
+// A row of 128 values, four a lane, as two binary16 terms of itself times a power of two, which is
+// returned.
+HV_DEV float row_terms(const float4& x, uint2* hi, uint2* lo) {
+  float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+  m = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m)));
+  const float lift = q8_lift(m);
+  split_half2(x.x * lift, x.y * lift, &hi->x, &lo->x);
+  split_half2(x.z * lift, x.w * lift, &hi->y, &lo->y);
+  return lift;
+}
+
 // The two terms of rows f0 .. f0 + nf - 1 of kv head kvh to shared memory, eight rows of first
 // terms, then their second ones; what takes a row's sums of products to exponents to `fac`.
 HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, float* fac, int warp, int warps) {
@@ -55,12 +66,8 @@ HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, 
       const int r = (f0 + i) / a.group, h = f0 + i - r * a.group;
       x = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + h) * kHd) + lane);
     }
-    float m = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-    m = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(m)));
-    const float lift = q8_lift(m);
     uint2 hi, lo;
-    split_half2(x.x * lift, x.y * lift, &hi.x, &lo.x);
-    split_half2(x.z * lift, x.w * lift, &hi.y, &lo.y);
+    const float lift = row_terms(x, &hi, &lo);
     const int at = (i >> 3) * 16 + (i & 7);
     *reinterpret_cast<uint2*>(to + swz(at, lane >> 1) + 8 * (lane & 1)) = hi;
     *reinterpret_cast<uint2*>(to + swz(at + 8, lane >> 1) + 8 * (lane & 1)) = lo;
@@ -295,7 +302,12 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
 // A warp per (row, head): its chunks added up.
 __global__ void __launch_bounds__(256) k_span_join(SpanArgs a, SpanParts p) {
   const int kvh = blockIdx.y, F = a.nrow * a.group, f = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (f >= F) return;
+  const int Fp = (F + kStRows - 1) / kStRows * kStRows;
+  auto facs = [&](int i) -> float& { return p.facs[((size_t)i * gridDim.y + kvh) * Fp + f]; };
+  if (f >= F) {
+    if (p.terms && f < Fp && lane < 3) facs(lane) = 0.0f;
+    return;
+  }
   const int r = f / a.group;
   SpanSeq x;
   if (!span_find(a, r, &x)) return;
@@ -346,6 +358,18 @@ __global__ void __launch_bounds__(256) k_span_join(SpanArgs a, SpanParts p) {
   const float inv = all ? 1.0f / L : 0.0f;
   *out = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
   if (p.stat && lane == 0) p.stat[at] = make_float2(M, L);
+  if (p.terms) {
+    const float4 q = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + f - r * a.group) * kHd) + lane);
+    uint2 hi, lo;
+    const float lift = row_terms(q, &hi, &lo);
+    reinterpret_cast<uint2*>(p.terms + at * kHd)[lane] = hi;
+    reinterpret_cast<uint2*>(p.terms + (at + step) * kHd)[lane] = lo;
+    if (lane == 0) {
+      facs(0) = __ldg(a.scale) * kLog2e / lift;
+      facs(1) = -M;
+      facs(2) = 1.0f / L;
+    }
+  }
 }
 
 // The weights of a single row's scores, which k_span_part has left in the scratch.
@@ -523,7 +547,8 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int kSms = 148, kPtCtas = 2 * kSms;
 struct SpanPlan {
   int tiles, items, nwt, npc, ntc;     // tiles of the prefix's rows, items of the tails'
-  size_t part, ml, stat, scores, bytes;
+  size_t part, ml, stat, scores, terms, facs, bytes;
+  bool mass_tiles;
 };
 SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool mass) {
   SpanPlan p{};
@@ -550,7 +575,9 @@ SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool 
   p.ml = up(rows * 8);
   p.stat = up(mass ? (size_t)nkv * F * 8 : 0);
   p.scores = up(mass ? (size_t)nkv * 8 * pcap * 4 : 0);
-  p.bytes = p.part + p.ml + p.stat + p.scores + 256;
+  p.terms = up(mass ? 2 * all * kHd * 2 : 0);
+  p.facs = up(mass ? 3 * (size_t)nkv * (F + kStRows) * 4 : 0);
+  p.bytes = p.part + p.ml + p.stat + p.scores + p.terms + p.facs + 256;
   return p;
 }
 SpanParts span_parts(const SpanPlan& p, void* scratch, bool mass, bool scores) {
@@ -560,6 +587,9 @@ SpanParts span_parts(const SpanPlan& p, void* scratch, bool mass, bool scores) {
   s.ml = reinterpret_cast<float2*>(at + p.part);
   s.stat = mass ? reinterpret_cast<float2*>(at + p.part + p.ml) : nullptr;
   s.scores = scores ? reinterpret_cast<float*>(at + p.part + p.ml + p.stat) : nullptr;
+  uint8_t* rows = at + p.part + p.ml + p.stat + p.scores;
+  s.terms = p.mass_tiles ? reinterpret_cast<__half*>(rows) : nullptr;
+  s.facs = reinterpret_cast<float*>(rows + p.terms);
   s.nwt = p.nwt;
   s.npc = p.npc;
   s.ntc = p.ntc;
@@ -576,7 +606,8 @@ int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const Sp
   HV_REQUIRE(ctas < (1ll << 31), HV_E_UNSUPPORTED, "%s: too many rows", name);
   k_span_part<<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, kPtSmem, st>>>(a, s, p.tiles);
   HV_CUDA(cudaGetLastError());
-  k_span_join<<<dim3((F + 7) / 8, nkv), 256, 0, st>>>(a, s);
+  const unsigned rows = s.terms ? (F + kStRows - 1) / kStRows * kStRows : F;
+  k_span_join<<<dim3((rows + 7) / 8, nkv), 256, 0, st>>>(a, s);
   HV_LAUNCHED(name);
 }
 
@@ -600,7 +631,9 @@ int mass_any(const char* name, const SpanArgs& a, const float* mass_in, float* m
              HV_E_INVALID, "%s: unaligned pointer", name);
   const int nkv = a.nq / a.group;
   const bool one = a.plen_p != nullptr;                     // a single row at a device position
-  const SpanPlan p = span_plan(nkv, a.nrow * a.group, 1, cap, 0, true, true);
+  SpanPlan p = span_plan(nkv, a.nrow * a.group, 1, cap, 0, true, true);
+  const int n = a.plen + a.nrow;
+  p.mass_tiles = !one && (long long)a.nrow * a.group * n >= 1 << 18;
   SpanParts s = span_parts(p, scratch, true, one);
   int rc = span_launch(name, a, p, s, st);
   if (rc) return rc;
@@ -608,8 +641,8 @@ int mass_any(const char* name, const SpanArgs& a, const float* mass_in, float* m
     k_mass_dec<<<dim3((unsigned)((cap + 255) / 256), (unsigned)nkv), 256, 0, st>>>(a, s, mass_in, mass_out);
     HV_LAUNCHED(name);
   }
+  if (p.mass_tiles) return mass_tile_launch(a, s, mass_in, mass_out, cap, st);
   // a CTA an SM, as far as the positions go
-  const int n = a.plen + a.nrow;
   auto ctas = [&](int pos) { return (long long)nkv * ((n + 16 * pos - 1) / (16 * pos)); };
   if (ctas(8) >= 148) return mass_rows_launch<8>(name, a, s, mass_in, mass_out, cap, st);
   if (ctas(4) >= 148) return mass_rows_launch<4>(name, a, s, mass_in, mass_out, cap, st);

@@ -25,8 +25,6 @@
 // to the scratch.
 //
 // Every wait is bounded: one that runs out ends the CTA's work, whose rows are then NaN.
-#include <cuda.h>
-
 #include "attn_f16.cuh"
 #include "hv_internal.h"
 #include "tcgen05.cuh"
@@ -63,16 +61,6 @@ struct StShared {
   int given_up;
 };
 constexpr int kStSmem = 4 * kStTile + kStRows * kStLine * 4 + (int)sizeof(StShared);   // K, V twice
-
-HV_DEV void tile_copy(uint32_t to, const CUtensorMap* map, int dim, int pos, int head, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%2, %3, %4}], [%5];"
-      :: "r"(to), "l"(map), "r"(dim), "r"(pos), "r"(head), "r"(bar) : "memory");
-}
-HV_DEV void bar_expect(uint32_t bar, int bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
-}
 
 __global__ void __launch_bounds__(kStThreads, 1)
     k_span_tile(SpanArgs a, SpanParts p, const __grid_constant__ CUtensorMap map_k,
@@ -448,8 +436,9 @@ __global__ void __launch_bounds__(kStThreads, 1)
 typedef CUresult (*MapFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                           const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                           CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-// A cache [nkv][cap][128] in boxes of 128 positions by 64 dims.
-int cache_map(const __half* base, int nkv, int cap, CUtensorMap* out) {
+}  // namespace
+
+int f16_rows_map(const __half* base, int rows, int outer, CUtensorMap* out) {
   static MapFn fn = [] {
     void* f = nullptr;
     cudaDriverEntryPointQueryResult r;
@@ -458,18 +447,17 @@ int cache_map(const __half* base, int nkv, int cap, CUtensorMap* out) {
                ? (MapFn)f
                : (MapFn) nullptr;
   }();
-  HV_REQUIRE(fn != nullptr, HV_E_UNSUPPORTED, "k_span_tile: the driver has no cuTensorMapEncodeTiled");
-  const cuuint64_t dims[3] = {(cuuint64_t)kHd, (cuuint64_t)cap, (cuuint64_t)nkv};
-  const cuuint64_t strides[2] = {(cuuint64_t)kHd * 2, (cuuint64_t)cap * kHd * 2};
+  HV_REQUIRE(fn != nullptr, HV_E_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
+  const cuuint64_t dims[3] = {(cuuint64_t)kHd, (cuuint64_t)rows, (cuuint64_t)outer};
+  const cuuint64_t strides[2] = {(cuuint64_t)kHd * 2, (cuuint64_t)rows * kHd * 2};
   const cuuint32_t box[3] = {64u, (cuuint32_t)kStRows, 1u}, step[3] = {1u, 1u, 1u};
   const CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(base), dims, strides, box, step,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  HV_REQUIRE(r == CUDA_SUCCESS, HV_E_INVALID, "k_span_tile: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  HV_REQUIRE(r == CUDA_SUCCESS, HV_E_INVALID, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return HV_OK;
 }
 
-}  // namespace
 
 int span_tile_launch(const SpanArgs& a, const SpanParts& p, cudaStream_t st) {
   int rc = smem_attr((const void*)k_span_tile, kStSmem);
@@ -481,8 +469,8 @@ int span_tile_launch(const SpanArgs& a, const SpanParts& p, cudaStream_t st) {
   }();
   HV_REQUIRE(regs == kStRegs, HV_E_UNSUPPORTED, "k_span_tile: built with %d registers", regs);
   CUtensorMap mk, mv;
-  rc = cache_map(a.pk, a.nq / a.group, a.pcap, &mk);
-  if (!rc) rc = cache_map(a.pv, a.nq / a.group, a.pcap, &mv);
+  rc = f16_rows_map(a.pk, a.pcap, a.nq / a.group, &mk);
+  if (!rc) rc = f16_rows_map(a.pv, a.pcap, a.nq / a.group, &mv);
   if (rc) return rc;
   k_span_tile<<<(unsigned)p.grid, kStThreads, kStSmem, st>>>(a, p, mk, mv);
   HV_LAUNCHED("k_span_tile");
