@@ -138,7 +138,8 @@ struct SpanParts {
   float2* stat;                        // [nkv][F]: m and the sum of all, for the weights' sake
   float* scores;                       // [nq][pcap], of a single row
   // what k_mass_tile reads of the rows: their two binary16 terms [2][nkv][F][128]; and, F rounded
-  // up to whole tiles, what takes their sums of products to exponents, -m and 1 / l, 0 behind F
+  // up to whole tiles, the factor and the term [2][nkv][..] that take their sums of products to
+  // exponents of weights (-m - log2 l; -infinity behind F)
   __half* terms;
   float* facs;
   int nwt, npc, ntc, grid;             // grid: CTAs of k_span_tile

@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(256) k_span_join(SpanArgs a, SpanParts p) {
   const int Fp = (F + kStRows - 1) / kStRows * kStRows;
   auto facs = [&](int i) -> float& { return p.facs[((size_t)i * gridDim.y + kvh) * Fp + f]; };
   if (f >= F) {
-    if (p.terms && f < Fp && lane < 3) facs(lane) = 0.0f;
+    if (p.terms && f < Fp && lane < 2) facs(lane) = lane ? -INFINITY : 0.0f;
     return;
   }
   const int r = f / a.group;
@@ -366,8 +366,7 @@ __global__ void __launch_bounds__(256) k_span_join(SpanArgs a, SpanParts p) {
     reinterpret_cast<uint2*>(p.terms + (at + step) * kHd)[lane] = lo;
     if (lane == 0) {
       facs(0) = __ldg(a.scale) * kLog2e / lift;
-      facs(1) = -M;
-      facs(2) = 1.0f / L;
+      facs(1) = -(M + log2f(L));
     }
   }
 }
@@ -576,7 +575,7 @@ SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool 
   p.stat = up(mass ? (size_t)nkv * F * 8 : 0);
   p.scores = up(mass ? (size_t)nkv * 8 * pcap * 4 : 0);
   p.terms = up(mass ? 2 * all * kHd * 2 : 0);
-  p.facs = up(mass ? 3 * (size_t)nkv * (F + kStRows) * 4 : 0);
+  p.facs = up(mass ? 2 * (size_t)nkv * (F + kStRows) * 4 : 0);
   p.bytes = p.part + p.ml + p.stat + p.scores + p.terms + p.facs + 256;
   return p;
 }
