@@ -102,10 +102,10 @@ HV_HD int span_chunk(int n, int most) {
   return (c + kSpanStage - 1) / kSpanStage * kSpanStage;
 }
 
-// The whole tiles of the prefix that k_span_tile takes: for each tile of kStRows (row, head) pairs
-// the positions that all its rows see, in tiles of kStRows positions. Units of work are (kv head,
-// tile of rows, tile of positions), `tiles` of the last for every tile of rows (a run's first ones
-// have fewer), cut evenly among `ctas` CTAs.
+// What k_span_tile takes: of a shared prefix everything, in tiles of kStRows positions, of a run's
+// cache the whole tiles that every row of a tile of kStRows (row, head) pairs sees. Units of work are
+// (kv head, tile of rows, tile of positions), `tiles` of the last for every tile of rows (a run's
+// first ones have fewer), cut evenly among `ctas` CTAs.
 constexpr int kStRows = 128;
 struct SpanWhole {
   long long units;
@@ -113,19 +113,29 @@ struct SpanWhole {
 };
 HV_DEV int span_whole_of(const SpanArgs& a, int np, int tile) {
   if (np < 0) return 0;
-  return (a.run ? np + tile * kStRows / a.group + 1 : np) / kStRows;
+  return a.run ? (np + tile * kStRows / a.group + 1) / kStRows : (np + kStRows - 1) / kStRows;
 }
+// Where the tiles of rows are few enough, as many CTAs take each as there are SMs for: a CTA that
+// ends one tile of rows and begins another pays for it about what three tiles of positions take.
 HV_DEV SpanWhole span_whole(const SpanArgs& a, int np, int grid) {
   SpanWhole w;
   w.rows = (a.nrow * a.group + kStRows - 1) / kStRows;
   w.tiles = span_whole_of(a, np, w.rows - 1);
-  w.units = (long long)(a.nq / a.group) * w.rows * w.tiles;
+  const long long all = (long long)(a.nq / a.group) * w.rows;
+  w.units = all * w.tiles;
   w.ctas = (int)min((long long)grid, w.units);
+  const int each = all > grid ? 0 : min(grid / (int)all, w.tiles);
+  if (each > 0 && (w.tiles + each - 1) / each <= w.units / grid + 3) w.ctas = (int)all * each;
   return w;
 }
-// The first CTA with unit u or one behind it: CTA c has units * c / ctas and on.
+// The CTA that has unit u: CTA c has units * c / ctas and on. By an estimate: a 64-bit division
+// takes longer.
 HV_DEV int span_cta(const SpanWhole& w, long long u) {
-  return (int)(((u + 1) * w.ctas - 1) / w.units);
+  const long long n = (u + 1) * w.ctas - 1;
+  int c = (int)((float)n / (float)w.units);
+  while (w.units * c > n) --c;
+  while (w.units * (c + 1) <= n) ++c;
+  return c;
 }
 
 // Partial results in the caller's scratch, in slots: nwt for the stretches of k_span_tile (at most

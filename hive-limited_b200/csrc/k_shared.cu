@@ -6,6 +6,7 @@
 //   ctx_h = sum_t w_t v_t / sum_t w_t,   w_t = exp(scale q_h . k_t - max)
 //   mass[g][t] += sum over rows and the heads of kv head g of w_t / sum w
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_decode.cuh"
 #include "attn_f16.cuh"
@@ -23,12 +24,15 @@ namespace {
 // to a stage, swizzled so that eight rows' 16 bytes meet no bank twice.
 constexpr int kPtWarps = 8;
 constexpr int kPtTile = kSpanStage * kHd * 2;            // bytes of K or of V of a stage
-constexpr int kPtQ = kSpanItem * 2 * kHd * 2;            // bytes of the rows' two terms
+constexpr int kPtQ = kSpanItem * 2 * kHd * 2;            // bytes of 64 rows' two terms
 constexpr int kPtLine = kHd + 4;                         // floats between rows that are joined
 constexpr float kPtLift = 14.0f;                         // log2 of what weights are multiplied by
-constexpr int kPtStages = 2;
-constexpr int kPtSmem = kPtQ + kPtStages * 2 * kPtTile;
-static_assert(kPtWarps * 8 * kPtLine * 4 <= kPtStages * 2 * kPtTile, "rows to join");
+// Up to kOct eights of rows; two CTAs an SM, and what their rows leave of it for stages
+template <int kOct>
+constexpr int kPtStages = kOct == 1 ? 3 : 2;
+template <int kOct>
+constexpr int kPtSmem = kOct * (kPtQ / 8) + kPtStages<kOct> * 2 * kPtTile;
+static_assert(kPtWarps * 8 * kPtLine * 4 <= 2 * 2 * kPtTile, "rows to join");
 
 HV_DEV uint32_t swz(int row, int unit) { return row * 256 + ((unit ^ (row & 7)) << 4); }
 HV_DEV void ldsm(uint32_t (&r)[4], uint32_t at) {
@@ -88,8 +92,10 @@ HV_DEV SpanRest span_rest(const SpanArgs& a, const SpanParts& p, int tile) {
   return r;
 }
 
+template <int kOct>
 __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles) {
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];         // the rows, then stages of K and V
+  constexpr int kStages = kPtStages<kOct>, kQ = kOct * (kPtQ / 8);
   __shared__ float s_fac[kSpanItem], s_m[kPtWarps][8], s_l[kPtWarps][8];
   __shared__ int s_bad[kSpanStage];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
@@ -129,10 +135,10 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
     lim_all = min(p1, x.sees(f0 / a.group));
   }
   const int ns = (p1 - p0 + kSpanStage - 1) / kSpanStage;
-  const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem), kv_s = sm + kPtQ;
+  const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem), kv_s = sm + kQ;
   auto fetch = [&](int s) {
     if (s < ns) {
-      const uint32_t to = kv_s + (s % kPtStages) * 2 * kPtTile;
+      const uint32_t to = kv_s + (s % kStages) * 2 * kPtTile;
 #pragma unroll
       for (int i = 0; i < kSpanStage * 16 / (32 * kPtWarps); ++i) {
         const int u = threadIdx.x + i * 32 * kPtWarps, r = u >> 4, c = u & 15;
@@ -146,7 +152,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int s = 0; s < kPtStages - 1; ++s) fetch(s);
+  for (int s = 0; s < kStages; ++s) fetch(s);
   rows_split(a, kvh, f0, nf, smem, s_fac, warp, kPtWarps);
 
   // warps by eights of rows, then by positions
@@ -168,10 +174,9 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
   const int qr = 16 * o + (lane & 15);                     // ldmatrix rows of the 16-row operand
   const uint32_t q_at = sm + qr * 256;
   for (int s = 0; s < ns; ++s) {
-    fetch(s + kPtStages - 1);
-    asm volatile("cp.async.wait_group %0;" :: "n"(kPtStages - 1) : "memory");
+    asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 1) : "memory");
     __syncthreads();
-    const uint32_t kt = kv_s + (s % kPtStages) * 2 * kPtTile, vt = kt + kPtTile;
+    const uint32_t kt = kv_s + (s % kStages) * 2 * kPtTile, vt = kt + kPtTile;
     const int base = p0 + s * kSpanStage;
     const bool partial = lim_all < min(p1, base + kSpanStage);
     if (partial) {
@@ -180,7 +185,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
       if (threadIdx.x < kSpanStage) s_bad[threadIdx.x] = 0;
       __syncthreads();
       for (int u = threadIdx.x; u < kSpanStage * 16; u += 32 * kPtWarps) {
-        uint4* w = reinterpret_cast<uint4*>(smem + kPtQ + (s % kPtStages) * 2 * kPtTile + kPtTile + swz(u >> 4, u & 15));
+        uint4* w = reinterpret_cast<uint4*>(smem + kQ + (s % kStages) * 2 * kPtTile + kPtTile + swz(u >> 4, u & 15));
         const uint4 y = *w;
         auto odd = [](uint32_t z) { return (z & 0x7C00u) == 0x7C00u || (z & 0x7C000000u) == 0x7C000000u; };
         if (odd(y.x) || odd(y.y) || odd(y.z) || odd(y.w)) {
@@ -190,92 +195,103 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
       }
       __syncthreads();
     }
-    if (mine) {
-      for (int u = 0; u < 2; ++u) {
-        const int b = base + 32 * u;                       // 32 positions
-        if ((2 * s + u) % wp != pg || b >= p1) continue;
-        float sc[4][4];
+    // kN times 16 positions at a time, the warps that share rows in turn
+    auto unit = [&](int at, auto n_form) {
+      constexpr int kN = decltype(n_form)::value;
+      const int b = base + at;
+      float sc[2 * kN][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 2 * kN; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[j][i] = 0.0f;
+        for (int i = 0; i < 4; ++i) sc[j][i] = 0.0f;
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          uint32_t qa[4];
-          ldsm(qa, q_at + (((2 * kk + (lane >> 4)) ^ (qr & 7)) << 4));
+      for (int kk = 0; kk < 8; ++kk) {
+        uint32_t qa[4];
+        ldsm(qa, q_at + (((2 * kk + (lane >> 4)) ^ (qr & 7)) << 4));
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t kb[4];
-            const int r = 32 * u + 16 * j + (lane & 7) + ((lane >> 4) << 3);
-            ldsm(kb, kt + swz(r, 2 * kk + ((lane >> 3) & 1)));
-            mma_f16(sc[2 * j], qa, kb[0], kb[1]);
-            mma_f16(sc[2 * j + 1], qa, kb[2], kb[3]);
-          }
+        for (int j = 0; j < kN; ++j) {
+          uint32_t kb[4];
+          ldsm(kb, kt + swz(at + 16 * j + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
+          mma_f16(sc[2 * j], qa, kb[0], kb[1]);
+          mma_f16(sc[2 * j + 1], qa, kb[2], kb[3]);
         }
-        float w[8];
-        float up = m;
-        const bool all = b + 32 <= lim_all;
+      }
+      float w[4 * kN];
+      float up = m;
+      const bool all = b + 16 * kN <= lim_all;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < 4 * kN; ++j) {
+        const int pos = b + 8 * (j >> 1) + 2 * t + (j & 1);
+        const float y = (sc[j >> 1][j & 1] + sc[j >> 1][2 + (j & 1)]) * fac;
+        w[j] = all || pos < lim ? y : -INFINITY;
+        up = fmaxf(up, w[j]);
+      }
+      if (kOct == 1 && p.scores && row_live) {
+        float* to = p.scores + ((size_t)kvh * a.group + fr) * a.pcap;
+#pragma unroll
+        for (int j = 0; j < 4 * kN; ++j) {
           const int pos = b + 8 * (j >> 1) + 2 * t + (j & 1);
-          const float y = (sc[j >> 1][j & 1] + sc[j >> 1][2 + (j & 1)]) * fac;
-          w[j] = all || pos < lim ? y : -INFINITY;
-          up = fmaxf(up, w[j]);
+          if (pos < p1) to[pos] = w[j];
         }
-        if (p.scores && row_live) {
-          float* to = p.scores + ((size_t)kvh * a.group + fr) * a.pcap;
+      }
+      up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, 1));
+      up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, 2));
+      if (__any_sync(0xFFFFFFFFu, up > m)) {
+        const float c = m == -INFINITY ? 0.0f : ex2(m - up);
+        l *= c;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int pos = b + 8 * (j >> 1) + 2 * t + (j & 1);
-            if (pos < p1) to[pos] = w[j];
-          }
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] *= c;
+        m = up;
+      }
+      const float m0 = m == -INFINITY ? 0.0f : m - kPtLift;
+      uint32_t wa[kN][4];
+#pragma unroll
+      for (int j = 0; j < 4 * kN; ++j) {
+        w[j] = ex2(w[j] - m0);
+        l += w[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 2 * kN; ++j)
+        split_half2(w[2 * j], w[2 * j + 1], &wa[j >> 1][2 * (j & 1)], &wa[j >> 1][2 * (j & 1) + 1]);
+      if (partial) {
+#pragma unroll
+        for (int j = 0; j < 4 * kN; ++j) {
+          const int pos = b + 8 * (j >> 1) + 2 * t + (j & 1);
+          if (pos < lim && s_bad[pos - base]) l = __int_as_float(0x7fc00000);
         }
-        up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, 1));
-        up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, 2));
-        if (__any_sync(0xFFFFFFFFu, up > m)) {
-          const float c = m == -INFINITY ? 0.0f : ex2(m - up);
-          l *= c;
+      }
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
+      for (int j = 0; j < kN; ++j)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] *= c;
-          m = up;
+        for (int d = 0; d < 8; ++d) {
+          uint32_t vb[4];
+          ldsm_t(vb, vt + swz(at + 16 * j + (lane & 15), 2 * d + (lane >> 4)));
+          mma_f16(acc[2 * d], wa[j], vb[0], vb[1]);
+          mma_f16(acc[2 * d + 1], wa[j], vb[2], vb[3]);
         }
-        const float m0 = m == -INFINITY ? 0.0f : m - kPtLift;
-        uint32_t wa[2][4];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          w[j] = ex2(w[j] - m0);
-          l += w[j];
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) split_half2(w[2 * j], w[2 * j + 1], &wa[j >> 1][2 * (j & 1)], &wa[j >> 1][2 * (j & 1) + 1]);
-        if (partial) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int pos = b + 8 * (j >> 1) + 2 * t + (j & 1);
-            if (pos < lim && s_bad[pos - base]) l = __int_as_float(0x7fc00000);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            uint32_t vb[4];
-            ldsm_t(vb, vt + swz(32 * u + 16 * j + (lane & 15), 2 * d + (lane >> 4)));
-            mma_f16(acc[2 * d], wa[j], vb[0], vb[1]);
-            mma_f16(acc[2 * d + 1], wa[j], vb[2], vb[3]);
-          }
+    };
+    if (mine) {
+      if (wp > 4) {
+        // eight warps with the same rows: every second stage's 16 positions are this warp's
+        const int at = 16 * (pg & 3);
+        if ((s & 1) == pg >> 2 && base + at < p1) unit(at, std::integral_constant<int, 1>{});
+      } else {
+#pragma unroll 1
+        for (int u = 0; u < 2; ++u)
+          if ((2 * s + u) % wp == pg && base + 32 * u < p1) unit(32 * u, std::integral_constant<int, 2>{});
       }
     }
     __syncthreads();
+    fetch(s + kStages);
   }
   // the warps that share rows meet
   asm volatile("cp.async.wait_all;" ::: "memory");
   l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
   l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
   if (t == 0) { s_m[warp][gl] = m; s_l[warp][gl] = l; }
-  float* line = reinterpret_cast<float*>(smem + kPtQ) + (size_t)warp * 8 * kPtLine;
+  float* line = reinterpret_cast<float*>(smem + kQ) + (size_t)warp * 8 * kPtLine;
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     *reinterpret_cast<float2*>(line + gl * kPtLine + 8 * i + 2 * t) =
@@ -290,7 +306,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
     for (int j = 0; j < wp; ++j) {
       const int w = oo + j * wo;
       const float c = s_l[w][g] == 0.0f ? 0.0f : ex2(s_m[w][g] - M);
-      const float4 z = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + kPtQ) + (size_t)w * 8 * kPtLine + g * kPtLine + 4 * lane);
+      const float4 z = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + kQ) + (size_t)w * 8 * kPtLine + g * kPtLine + 4 * lane);
       L += c * s_l[w][g];
       y.x += c * z.x; y.y += c * z.y; y.z += c * z.z; y.w += c * z.w;
     }
@@ -341,19 +357,35 @@ __global__ void __launch_bounds__(256) k_span_join(SpanArgs a, SpanParts p) {
   }
   auto slot = [&](int i) { return i < nw ? i : i < nw + n0 ? p.nwt + i - nw : p.nwt + p.npc + i - nw - n0; };
   const int all = nw + n0 + n1;
-  float M = -INFINITY;
-  for (int i = lane; i < all; i += 32) M = fmaxf(M, p.ml[at + slot(i) * step].x);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
-  float L = 0.0f;
+  // a lane has a chunk's maximum and sum (32 chunks at a time), then all lanes its row's sums
+  float M = -INFINITY, L = 0.0f;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = 0; i < all; ++i) {
-    const float2 ml = p.ml[at + slot(i) * step];
-    const float4 y = reinterpret_cast<const float4*>(p.part + (at + slot(i) * step) * kHd)[lane];
-    const float c = ml.y == 0.0f ? 0.0f : ex2(ml.x - M);
-    L += c * ml.y;
-    s.x += c * y.x; s.y += c * y.y; s.z += c * y.z; s.w += c * y.w;
+  for (int i0 = 0; i0 < all; i0 += 32) {
+    const int n = min(32, all - i0);
+    const float2 ml = lane < n ? p.ml[at + slot(i0 + lane) * step] : make_float2(-INFINITY, 0.0f);
+    float up = fmaxf(M, ml.x);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, d));
+    const float c = ml.y == 0.0f ? 0.0f : ex2(ml.x - up), old = M == -INFINITY ? 0.0f : ex2(M - up);
+    float sum = c * ml.y;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+    M = up;
+    L = L * old + sum;
+    s.x *= old; s.y *= old; s.z *= old; s.w *= old;
+#pragma unroll 1
+    for (int j0 = 0; j0 < n; j0 += 8) {
+      float4 y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j0 + j < n) y[j] = __ldg(reinterpret_cast<const float4*>(p.part + (at + slot(i0 + j0 + j) * step) * kHd) + lane);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j0 + j >= n) continue;
+        const float f = __shfl_sync(0xFFFFFFFFu, c, j0 + j);
+        s.x += f * y[j].x; s.y += f * y[j].y; s.z += f * y[j].z; s.w += f * y[j].w;
+      }
+    }
   }
   const float inv = all ? 1.0f / L : 0.0f;
   *out = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
@@ -555,11 +587,12 @@ SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool 
   p.tiles = (F + kSpanItem - 1) / kSpanItem;
   p.items = nseq + p.tiles;
   // many rows over many positions go by whole tiles
-  if (F > 64 && (long long)F * pcap >= 1 << 18) {
+  if (F > 32 && (long long)F * pcap >= 1 << 17) {
     const long long rows = (long long)nkv * ((F + kStRows - 1) / kStRows);
-    p.nwt = (int)std::min((long long)(pcap / kStRows), kSms / rows + 2);
+    p.nwt = (int)std::min((long long)((pcap + kStRows - 1) / kStRows), kSms / rows + 2);
   }
-  p.npc = std::min(stages(p.nwt ? 2 * kStRows : pcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * p.tiles)));
+  // ... of a shared prefix all of it, of a run's cache what every row of a tile sees
+  p.npc = std::min(stages(p.nwt ? (run ? 2 * kStRows : 0) : pcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * p.tiles)));
   if (!run) p.ntc = std::min(stages(tcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * std::max(nseq, p.tiles))));
   // room for this call and any smaller one, which may have more chunks of fewer rows: chunks times
   // tiles (or sequences) are at most kPtCtas / nkv, or one each
@@ -567,7 +600,7 @@ SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool 
   auto room = [&](int n) {
     return std::min((size_t)stages(n) * all, (size_t)kPtCtas * std::min(F, kSpanItem) + all);
   };
-  const size_t whole = std::min((size_t)(pcap / kStRows) * all, (size_t)kSms * std::min(F, kStRows) + 2 * all);
+  const size_t whole = std::min((size_t)((pcap + kStRows - 1) / kStRows) * all, (size_t)kSms * std::min(F, kStRows) + 2 * all);
   const size_t rows = whole + room(pcap) + (run ? 0 : room(tcap));
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   p.part = up(rows * kHd * 4);
@@ -597,13 +630,21 @@ SpanParts span_parts(const SpanPlan& p, void* scratch, bool mass, bool scores) {
 }
 
 int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const SpanParts& s, cudaStream_t st) {
-  int rc = smem_attr((const void*)k_span_part, kPtSmem);
-  if (!rc && s.nwt) rc = span_tile_launch(a, s, st);
-  if (rc) return rc;
+  if (s.nwt) {
+    const int rc = span_tile_launch(a, s, st);
+    if (rc) return rc;
+  }
   const unsigned nkv = (unsigned)(a.nq / a.group), F = (unsigned)(a.nrow * a.group);
   const long long ctas = (long long)p.tiles * p.npc + (long long)p.items * p.ntc;
   HV_REQUIRE(ctas < (1ll << 31), HV_E_UNSUPPORTED, "%s: too many rows", name);
-  k_span_part<<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, kPtSmem, st>>>(a, s, p.tiles);
+  // eight rows at the most where every row of a sequence has its own and the prefix has no more
+  const bool few = F <= 8 || (!a.run && !a.row0 && s.npc == 0);
+  const void* fn = few ? (const void*)k_span_part<1> : (const void*)k_span_part<8>;
+  const int smem = few ? kPtSmem<1> : kPtSmem<8>;
+  const int rc = smem_attr(fn, smem);
+  if (rc) return rc;
+  if (few) k_span_part<1><<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, smem, st>>>(a, s, p.tiles);
+  else k_span_part<8><<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, smem, st>>>(a, s, p.tiles);
   HV_CUDA(cudaGetLastError());
   const unsigned rows = s.terms ? (F + kStRows - 1) / kStRows * kStRows : F;
   k_span_join<<<dim3((rows + 7) / 8, nkv), 256, 0, st>>>(a, s);

@@ -1,7 +1,7 @@
-// Attention of many rows a head over whole tiles of a binary16 cache, on the fifth-generation
-// tensor cores: the part of a prefix that every row of a tile of 128 (row, head) pairs sees, 128
-// positions to a tile. What is left (a prefix's last positions, a run's own, tails) is k_span_part's,
-// and k_span_join adds up.
+// Attention of many rows a head over a binary16 cache, on the fifth-generation tensor cores: what
+// every row of a tile of 128 (row, head) pairs sees, 128 positions to a tile, the last one of a
+// shared prefix maybe less. What is left (a run's own positions, tails) is k_span_part's, and
+// k_span_join adds up.
 //
 // The rows' first and second binary16 terms are the operand in tensor memory, K and V tiles come
 // by tensor copies into swizzled shared memory as they stand in the cache: K with the dims
@@ -14,6 +14,7 @@
 //   warps 8-11   a thread adds its row of O to 128 sums in registers (tensor memory's sums are cut,
 //                not rounded, so O is of one tile, and the small terms go first)
 //   warps 12, 13 one thread each: the copies of K and of V
+//   warps 14, 15 make zeros of what a last tile's V has behind the prefix
 // A row's weights are 2^(x - m + 8) with m a whole number that a tile's largest exponent may pass:
 // as long as no 16 of them add up to more than 2^15 they fit binary16 and are exact to 2^-33 of
 // the largest, so that the scores are read once, without a pass for their maximum. The first tile
@@ -54,7 +55,7 @@ HV_DEV uint64_t smem_desc_mn(uint32_t addr) {   // 128-byte swizzle, 64 halves o
 
 struct StShared {
   unsigned long long full_k[2], full_v[2], s_ready[2], w_ready[2], o_done[2];
-  unsigned long long o_free, drain[2];
+  unsigned long long o_free, v_clean, drain[2];
   float top[4][kStRows];         // of the last four tiles: what their weights are relative to
   float m[2][kStRows], l[2][kStRows];
   uint32_t tmem;
@@ -87,6 +88,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
       bar_init(bar(sh.drain[i]), 1);
     }
     bar_init(bar(sh.o_free), 128);
+    bar_init(bar(sh.v_clean), 64);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.given_up = (sm & 1023) != 0;               // the swizzle goes by addresses
   }
@@ -107,6 +109,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
   struct Stretch {
     long long u;
     int kvh, row0, j0, nt;
+    int cut;                                      // positions of its last tile, 0: all
     size_t part_row;
   };
   auto next = [&](Stretch& s) {
@@ -119,6 +122,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
       s.nt = min(span_whole_of(a, np, tile) - s.j0, some);
       if (s.nt <= 0) continue;
       s.row0 = tile * kStRows;
+      s.cut = !a.run && s.j0 + s.nt == wh.tiles ? np % kStRows : 0;
       const int slot = blockIdx.x - span_cta(wh, (long long)R * wh.tiles);
       s.part_row = ((size_t)slot * nkv + s.kvh) * F + s.row0;
       return true;
@@ -133,7 +137,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
   };
   Stretch st;
   st.u = u0;
-  int g0 = 0;                                     // tiles before this stretch's
+  int g0 = 0, cuts = 0;                           // tiles and cut ones before this stretch's
   auto rows_out = [&] {
     asm volatile("bar.sync 2, 384;" ::: "memory");
     float4* to = reinterpret_cast<float4*>(p.part + st.part_row * kHd);
@@ -146,7 +150,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kStRegsRow));
     int drains = 0;
 #pragma unroll 1
-    for (; next(st); g0 += st.nt, stretch_end()) {
+    for (; next(st); g0 += st.nt, cuts += st.cut > 0, stretch_end()) {
       // The queries in two terms, a row per thread (whole lines at a time through shared memory):
       // the first ones from warps 0-3, the second from 4-7. They take the scale's sign.
       {
@@ -176,6 +180,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
         amax = fmaxf(amax, sh.m[1 - w][row]);
         const float lift = copysignf(q8_lift(amax), qscale);
         qs = qscale / lift;
+        qs = qs == 0.0f ? 2e-38f : qs;             // -infinity times it is to stay that
         const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kStColQ + 64 * w;
 #pragma unroll 1
         for (int d = 0; d < kHd / 4; d += 8) {
@@ -225,6 +230,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
         ok = ok && bar_wait_warp(bar(sh.full_v[s]), (i >> 1) & 1, given_up);
         ok = ok && bar_wait_warp(bar(sh.w_ready[s]), (i >> 1) & 1, given_up);
         if (i > 0) ok = ok && bar_wait_warp(bar(sh.o_free), (i - 1) & 1, given_up);
+        if (st.cut && i == g0 + st.nt - 1) ok = ok && bar_wait_warp(bar(sh.v_clean), cuts & 1, given_up);
         fence_after();
 #pragma unroll 1
         for (int pass = 0; pass < 2 && ok; ++pass) {
@@ -252,6 +258,18 @@ __global__ void __launch_bounds__(kStThreads, 1)
         return ceilf(big * qs);
       };
       auto weights = [&](int i, bool first) {
+        if (st.cut && i == g0 + st.nt - 1) {      // what the tile has behind the prefix
+#pragma unroll 1
+          for (int c = st.cut & ~15; c < kStRows; c += 16) {
+            uint32_t x[16];
+            tmem_ld16(s_at + c, x);
+            tmem_wait(x);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[k] = c + k < st.cut ? x[k] : 0xFF800000u;
+            tmem_st16(s_at + c, x);
+          }
+          tmem_st_wait();
+        }
         if (first) m = largest(0);
         uint64_t f2 = pair(qs, qs), off, sum = 0;
         auto base = [&] {
@@ -358,7 +376,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
   } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kStRegsSum));
 #pragma unroll 1
-    for (; next(st); g0 += st.nt, stretch_end()) {
+    for (; next(st); g0 += st.nt, cuts += st.cut > 0, stretch_end()) {
       uint64_t acc[kHd / 2];
 #pragma unroll
       for (int d = 0; d < kHd / 2; ++d) acc[d] = 0;
@@ -407,8 +425,21 @@ __global__ void __launch_bounds__(kStThreads, 1)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kStRegsCopy));
 #pragma unroll 1
-    for (; next(st); g0 += st.nt, stretch_end()) {
-      if (warp >= 14 || lane != 0) continue;
+    for (; next(st); g0 += st.nt, cuts += st.cut > 0, stretch_end()) {
+      if (warp >= 14) {
+        if (!st.cut) continue;
+        const int i = g0 + st.nt - 1;
+        if (bar_wait_warp(bar(sh.full_v[i & 1]), (i >> 1) & 1, given_up)) {
+          uint8_t* v = smem + (2 + (i & 1)) * kStTile + 16 * (lane & 7);
+          for (int r = st.cut + (lane >> 3) + 4 * (warp - 14); r < kStRows; r += 8)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) *reinterpret_cast<uint4*>(v + h * kStHalf + r * 128) = make_uint4(0, 0, 0, 0);
+        }
+        fence_async();
+        bar_arrive(bar(sh.v_clean));
+        continue;
+      }
+      if (lane != 0) continue;
       // the copies of K (warp 12) and V (13): a buffer is free once its last product is done
       const bool kk = warp == 12;
       const CUtensorMap* map = kk ? &map_k : &map_v;
