@@ -54,15 +54,25 @@ HV_DEV SpanSeq span_seq(const SpanArgs& a, int s) {
   if (x.len < 0 || x.len > a.tcap) x.len = -1;
   return x;
 }
-// The sequence that row r belongs to; false if it lies behind the last one's rows.
+// The sequence that row r belongs to; false if it lies behind the last one's rows. By a whole warp
+// with the same r, 32 sequences looked at together: one after the other their loads would take
+// longer than most of what follows.
 HV_DEV bool span_find(const SpanArgs& a, int r, SpanSeq* x) {
-  int lo = 0, hi = a.nseq - 1;
-  while (lo < hi) {                    // the last sequence that starts at or before r
-    const int mid = (lo + hi + 1) >> 1;
-    if (span_row0(a, mid) <= r) lo = mid;
-    else hi = mid - 1;
+  int s = a.nseq == 1 ? 0 : r;
+  if (a.row0) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = a.nseq;            // the last sequence that starts at or before r is in [lo, lo + n)
+    while (n > 1) {
+      const int step = (n + 31) / 32, at = lo + lane * step;
+      const bool before = lane * step < n && (lane == 0 || span_row0(a, at) <= r);
+      const int k = 31 - __clz(__ballot_sync(0xFFFFFFFFu, before));
+      lo += k * step;
+      n = min(step, n - k * step);
+    }
+    s = lo;
   }
-  *x = span_seq(a, lo);
+  if (s >= a.nseq) return false;
+  *x = span_seq(a, s);
   return r >= x->row && r < x->end;
 }
 

@@ -151,50 +151,38 @@ __global__ void __launch_bounds__(kStThreads, 1)
     int drains = 0;
 #pragma unroll 1
     for (; next(st); g0 += st.nt, cuts += st.cut > 0, stretch_end()) {
-      // The queries in two terms, a row per thread (whole lines at a time through shared memory):
-      // the first ones from warps 0-3, the second from 4-7. They take the scale's sign.
-      {
-        const uint32_t to = sm + 4 * kStTile + 16 * lane;
-#pragma unroll 4
-        for (int r = warp; r < kStRows; r += 8) {
-          const int gr = min(st.row0 + r, F - 1), tok = gr / a.group;
-          const float* src = a.q + ((size_t)tok * a.nq + (size_t)st.kvh * a.group + gr - tok * a.group) * kHd + 4 * lane;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                       :: "r"(to + r * kStLine * 4), "l"(src) : "memory");
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-      }
-      const float qscale = __ldg(a.scale) * kLog2e;
-      rows_sync();
+      // The queries in two terms: a row's two threads have half of its dims each. They take the
+      // scale's sign.
       float qs;
       {
-        const float4* q = reinterpret_cast<const float4*>(lines + (size_t)row * kStLine);
+        const int gr = min(st.row0 + row, F - 1), tok = gr / a.group;
+        const float4* src = reinterpret_cast<const float4*>(
+            a.q + ((size_t)tok * a.nq + (size_t)st.kvh * a.group + gr - tok * a.group) * kHd) + (kHd / 8) * w;
+        float4 x[kHd / 8];
+#pragma unroll
+        for (int d = 0; d < kHd / 8; ++d) x[d] = __ldg(src + d);
+        const float qscale = __ldg(a.scale) * kLog2e;
         float amax = 0.0f;
-#pragma unroll 4
-        for (int d = 0; d < kHd / 8; ++d) {       // each of a row's two threads looks over half of it
-          const float4 x = q[(kHd / 8) * w + d];
-          amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x.x), fabsf(x.y))), fmaxf(fabsf(x.z), fabsf(x.w)));
-        }
+#pragma unroll
+        for (int d = 0; d < kHd / 8; ++d)
+          amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[d].x), fabsf(x[d].y))), fmaxf(fabsf(x[d].z), fabsf(x[d].w)));
         sh.m[w][row] = amax;
         rows_sync();
         amax = fmaxf(amax, sh.m[1 - w][row]);
         const float lift = copysignf(q8_lift(amax), qscale);
         qs = qscale / lift;
         qs = qs == 0.0f ? 2e-38f : qs;             // -infinity times it is to stay that
-        const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kStColQ + 64 * w;
-#pragma unroll 1
-        for (int d = 0; d < kHd / 4; d += 8) {
-          uint32_t v[16];
+        const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kStColQ + 32 * w;
+#pragma unroll
+        for (int d = 0; d < kHd / 8; d += 8) {
+          uint32_t hi[16], lo[16];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float4 x = q[d + k];
-            uint32_t h0, h1, l0, l1;
-            split_half2(x.x * lift, x.y * lift, &h0, &l0);
-            split_half2(x.z * lift, x.w * lift, &h1, &l1);
-            v[2 * k] = w ? l0 : h0;
-            v[2 * k + 1] = w ? l1 : h1;
+            split_half2(x[d + k].x * lift, x[d + k].y * lift, &hi[2 * k], &lo[2 * k]);
+            split_half2(x[d + k].z * lift, x[d + k].w * lift, &hi[2 * k + 1], &lo[2 * k + 1]);
           }
-          tmem_st16(to + 2 * d, v);
+          tmem_st16(to + 2 * d, hi);
+          tmem_st16(to + 64 + 2 * d, lo);
         }
         tmem_st_wait();
       }
