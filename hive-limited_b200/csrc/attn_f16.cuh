@@ -76,31 +76,31 @@ HV_DEV bool span_find(const SpanArgs& a, int r, SpanSeq* x) {
   return r >= x->row && r < x->end;
 }
 
-// The sequences' rows of a call in items of up to kSpanItem (row, head) pairs each, as blocks of a
-// grid: nseq + F / kSpanItem of them, F = nrow * group. The first nseq have each sequence's first
-// pairs; what a sequence has more starts, kSpanItem further every time, in windows of kSpanItem
-// pairs of all, at most one start a window, and that of the sequence that has the window's first.
-// Pairs [f0, f0 + nf) of sequence x; nf 0: nothing for this block.
-constexpr int kSpanItem = 64;
+// The sequences' rows of a call in items of up to `size` (row, head) pairs each, as blocks of a grid:
+// nseq + F / size of them, F = nrow * group. The first nseq have each sequence's first pairs; what a
+// sequence has more starts, `size` further every time, in windows of `size` pairs of all, at most
+// one start a window, and that of the sequence that has the window's first. Pairs [f0, f0 + nf) of
+// sequence x; nf 0: nothing for this block.
+constexpr int kSpanItem = 64, kFewRows = 8;
 struct SpanItem {
   SpanSeq x;
   int f0, nf;
 };
-HV_DEV SpanItem span_item(const SpanArgs& a, int b) {
+HV_DEV SpanItem span_item(const SpanArgs& a, int b, int size) {
   SpanItem it;
   it.nf = 0;
   if (b < a.nseq) {
     it.x = span_seq(a, b);
     it.f0 = it.x.row * a.group;
   } else {
-    const int w = (b - a.nseq) * kSpanItem;
+    const int w = (b - a.nseq) * size;
     if (!span_find(a, w / a.group, &it.x)) return it;
     const int start = it.x.row * a.group;
-    const int k = (w - start + kSpanItem - 1) / kSpanItem;
-    it.f0 = start + k * kSpanItem;
+    const int k = (w - start + size - 1) / size;
+    it.f0 = start + k * size;
     if (k == 0) return it;
   }
-  it.nf = min(kSpanItem, it.x.end * a.group - it.f0);
+  it.nf = min(size, it.x.end * a.group - it.f0);
   it.nf = max(it.nf, 0);
   return it;
 }
@@ -118,7 +118,7 @@ HV_HD int span_chunk(int n, int most) {
 // first ones have fewer), cut evenly among `ctas` CTAs.
 constexpr int kStRows = 128;
 struct SpanWhole {
-  long long units;
+  unsigned units;
   int tiles, rows, ctas;
 };
 HV_DEV int span_whole_of(const SpanArgs& a, int np, int tile) {
@@ -131,20 +131,22 @@ HV_DEV SpanWhole span_whole(const SpanArgs& a, int np, int grid) {
   SpanWhole w;
   w.rows = (a.nrow * a.group + kStRows - 1) / kStRows;
   w.tiles = span_whole_of(a, np, w.rows - 1);
-  const long long all = (long long)(a.nq / a.group) * w.rows;
-  w.units = all * w.tiles;
-  w.ctas = (int)min((long long)grid, w.units);
-  const int each = all > grid ? 0 : min(grid / (int)all, w.tiles);
-  if (each > 0 && (w.tiles + each - 1) / each <= w.units / grid + 3) w.ctas = (int)all * each;
+  const unsigned all = (unsigned)(a.nq / a.group) * w.rows;
+  w.units = all * w.tiles;                       // under 2^31: see span_plan
+  w.ctas = (int)min((unsigned)grid, w.units);
+  const unsigned each = min((unsigned)grid / all, (unsigned)w.tiles);
+  if (each > 0 && (w.tiles + each - 1) / each <= w.units / grid + 3) w.ctas = (int)(all * each);
   return w;
 }
-// The CTA that has unit u: CTA c has units * c / ctas and on. By an estimate: a 64-bit division
-// takes longer.
-HV_DEV int span_cta(const SpanWhole& w, long long u) {
-  const long long n = (u + 1) * w.ctas - 1;
-  int c = (int)((float)n / (float)w.units);
-  while (w.units * c > n) --c;
-  while (w.units * (c + 1) <= n) ++c;
+// CTA c's first unit, units * c / ctas, and the CTA that has unit u.
+HV_DEV unsigned span_first(const SpanWhole& w, unsigned c) {
+  const unsigned q = w.units / w.ctas, r = w.units - q * w.ctas;
+  return q * c + r * c / w.ctas;
+}
+HV_DEV int span_cta(const SpanWhole& w, unsigned u) {
+  int c = (int)((float)u * ((float)w.ctas / (float)w.units));      // one off at the most
+  if (span_first(w, c) > u) --c;
+  if (span_first(w, c + 1) <= u) ++c;
   return c;
 }
 

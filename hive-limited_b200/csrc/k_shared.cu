@@ -27,12 +27,9 @@ constexpr int kPtTile = kSpanStage * kHd * 2;            // bytes of K or of V o
 constexpr int kPtQ = kSpanItem * 2 * kHd * 2;            // bytes of 64 rows' two terms
 constexpr int kPtLine = kHd + 4;                         // floats between rows that are joined
 constexpr float kPtLift = 14.0f;                         // log2 of what weights are multiplied by
-// Up to kOct eights of rows; two CTAs an SM, and what their rows leave of it for stages
-template <int kOct>
-constexpr int kPtStages = kOct == 1 ? 3 : 2;
-template <int kOct>
-constexpr int kPtSmem = kOct * (kPtQ / 8) + kPtStages<kOct> * 2 * kPtTile;
-static_assert(kPtWarps * 8 * kPtLine * 4 <= 2 * 2 * kPtTile, "rows to join");
+constexpr int kPtStages = 2;
+constexpr int kPtSmem = kPtQ + kPtStages * 2 * kPtTile;
+static_assert(kPtWarps * 8 * kPtLine * 4 <= kPtStages * 2 * kPtTile, "rows to join");
 
 HV_DEV uint32_t swz(int row, int unit) { return row * 256 + ((unit ^ (row & 7)) << 4); }
 HV_DEV void ldsm(uint32_t (&r)[4], uint32_t at) {
@@ -79,6 +76,12 @@ HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, 
   }
 }
 
+// Is one of eight halves an infinity or a NaN?
+HV_DEV bool not_finite(const uint4& y) {
+  auto odd = [](uint32_t z) { return (z & 0x7C00u) == 0x7C00u || (z & 0x7C000000u) == 0x7C000000u; };
+  return odd(y.x) || odd(y.y) || odd(y.z) || odd(y.w);
+}
+
 // What k_span_part has of the prefix for the rows of a tile of kSpanItem: all, or what k_span_tile
 // leaves. A run's end goes by the tile's last row.
 struct SpanRest {
@@ -92,10 +95,8 @@ HV_DEV SpanRest span_rest(const SpanArgs& a, const SpanParts& p, int tile) {
   return r;
 }
 
-template <int kOct>
 __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles) {
   extern __shared__ __align__(1024) uint8_t smem[];         // the rows, then stages of K and V
-  constexpr int kStages = kPtStages<kOct>, kQ = kOct * (kPtQ / 8);
   __shared__ float s_fac[kSpanItem], s_m[kPtWarps][8], s_l[kPtWarps][8];
   __shared__ int s_bad[kSpanStage];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
     lim_all = a.run ? min(p1, a.plen + f0 / a.group + 1) : p1;
   } else {
     const int b = blockIdx.x - tiles * p.npc, chunk = b % p.ntc;
-    const SpanItem it = span_item(a, b / p.ntc);
+    const SpanItem it = span_item(a, b / p.ntc, kSpanItem);
     if (it.nf == 0 || it.x.len <= 0) return;
     x = it.x;
     f0 = it.f0;
@@ -135,10 +136,10 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
     lim_all = min(p1, x.sees(f0 / a.group));
   }
   const int ns = (p1 - p0 + kSpanStage - 1) / kSpanStage;
-  const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem), kv_s = sm + kQ;
+  const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem), kv_s = sm + kPtQ;
   auto fetch = [&](int s) {
     if (s < ns) {
-      const uint32_t to = kv_s + (s % kStages) * 2 * kPtTile;
+      const uint32_t to = kv_s + (s % kPtStages) * 2 * kPtTile;
 #pragma unroll
       for (int i = 0; i < kSpanStage * 16 / (32 * kPtWarps); ++i) {
         const int u = threadIdx.x + i * 32 * kPtWarps, r = u >> 4, c = u & 15;
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) fetch(s);
+  for (int s = 0; s < kPtStages; ++s) fetch(s);
   rows_split(a, kvh, f0, nf, smem, s_fac, warp, kPtWarps);
 
   // warps by eights of rows, then by positions
@@ -174,9 +175,9 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
   const int qr = 16 * o + (lane & 15);                     // ldmatrix rows of the 16-row operand
   const uint32_t q_at = sm + qr * 256;
   for (int s = 0; s < ns; ++s) {
-    asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 1) : "memory");
+    asm volatile("cp.async.wait_group %0;" :: "n"(kPtStages - 1) : "memory");
     __syncthreads();
-    const uint32_t kt = kv_s + (s % kStages) * 2 * kPtTile, vt = kt + kPtTile;
+    const uint32_t kt = kv_s + (s % kPtStages) * 2 * kPtTile, vt = kt + kPtTile;
     const int base = p0 + s * kSpanStage;
     const bool partial = lim_all < min(p1, base + kSpanStage);
     if (partial) {
@@ -185,10 +186,9 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
       if (threadIdx.x < kSpanStage) s_bad[threadIdx.x] = 0;
       __syncthreads();
       for (int u = threadIdx.x; u < kSpanStage * 16; u += 32 * kPtWarps) {
-        uint4* w = reinterpret_cast<uint4*>(smem + kQ + (s % kStages) * 2 * kPtTile + kPtTile + swz(u >> 4, u & 15));
+        uint4* w = reinterpret_cast<uint4*>(smem + kPtQ + (s % kPtStages) * 2 * kPtTile + kPtTile + swz(u >> 4, u & 15));
         const uint4 y = *w;
-        auto odd = [](uint32_t z) { return (z & 0x7C00u) == 0x7C00u || (z & 0x7C000000u) == 0x7C000000u; };
-        if (odd(y.x) || odd(y.y) || odd(y.z) || odd(y.w)) {
+        if (not_finite(y)) {
           *w = make_uint4(0, 0, 0, 0);
           s_bad[u >> 4] = 1;
         }
@@ -225,14 +225,6 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
         const float y = (sc[j >> 1][j & 1] + sc[j >> 1][2 + (j & 1)]) * fac;
         w[j] = all || pos < lim ? y : -INFINITY;
         up = fmaxf(up, w[j]);
-      }
-      if (kOct == 1 && p.scores && row_live) {
-        float* to = p.scores + ((size_t)kvh * a.group + fr) * a.pcap;
-#pragma unroll
-        for (int j = 0; j < 4 * kN; ++j) {
-          const int pos = b + 8 * (j >> 1) + 2 * t + (j & 1);
-          if (pos < p1) to[pos] = w[j];
-        }
       }
       up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, 1));
       up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, 2));
@@ -284,14 +276,14 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
       }
     }
     __syncthreads();
-    fetch(s + kStages);
+    fetch(s + kPtStages);
   }
   // the warps that share rows meet
   asm volatile("cp.async.wait_all;" ::: "memory");
   l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
   l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
   if (t == 0) { s_m[warp][gl] = m; s_l[warp][gl] = l; }
-  float* line = reinterpret_cast<float*>(smem + kQ) + (size_t)warp * 8 * kPtLine;
+  float* line = reinterpret_cast<float*>(smem + kPtQ) + (size_t)warp * 8 * kPtLine;
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     *reinterpret_cast<float2*>(line + gl * kPtLine + 8 * i + 2 * t) =
@@ -306,7 +298,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
     for (int j = 0; j < wp; ++j) {
       const int w = oo + j * wo;
       const float c = s_l[w][g] == 0.0f ? 0.0f : ex2(s_m[w][g] - M);
-      const float4 z = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + kQ) + (size_t)w * 8 * kPtLine + g * kPtLine + 4 * lane);
+      const float4 z = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(smem + kPtQ) + (size_t)w * 8 * kPtLine + g * kPtLine + 4 * lane);
       L += c * s_l[w][g];
       y.x += c * z.x; y.y += c * z.y; y.z += c * z.z; y.w += c * z.w;
     }
@@ -315,90 +307,332 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
   }
 }
 
-// A warp per (row, head): its chunks added up.
-__global__ void __launch_bounds__(256) k_span_join(SpanArgs a, SpanParts p) {
-  const int kvh = blockIdx.y, F = a.nrow * a.group, f = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int Fp = (F + kStRows - 1) / kStRows * kStRows;
-  auto facs = [&](int i) -> float& { return p.facs[((size_t)i * gridDim.y + kvh) * Fp + f]; };
-  if (f >= F) {
-    if (p.terms && f < Fp && lane < 2) facs(lane) = lane ? -INFINITY : 0.0f;
-    return;
-  }
-  const int r = f / a.group;
+// ---- attention of up to eight rows ---------------------------------------------------------
+//
+// One item of eight (row, head) pairs and a chunk of positions a CTA, as for k_span_part, but every
+// warp has all rows, takes 16 positions in turn with the others and has a ring of its own for them,
+// so that no warp waits for another before the end. Bound by the bytes of the cache.
+constexpr int kFwWarps = 4, kFwStages = 3, kFwBlock = 16;
+constexpr int kFwTile = kFwBlock * kHd * 2;              // bytes of K or of V of 16 positions
+constexpr int kFwQ = 2 * kFewRows * kHd * 2;
+constexpr int kFwSmem = kFwQ + kFwWarps * kFwStages * 2 * kFwTile;
+
+__global__ void __launch_bounds__(32 * kFwWarps, 2) k_span_few(SpanArgs a, SpanParts p, int tiles) {
+  extern __shared__ __align__(1024) uint8_t smem[];         // the rows, then the warps' rings
+  __shared__ float s_fac[kFewRows], s_m[kFwWarps][8], s_l[kFwWarps][8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
+  const int kvh = blockIdx.y, F = a.nrow * a.group;
+  const __half *k, *v;
+  int f0, nf, p0, p1, slot, lim_all;
   SpanSeq x;
-  if (!span_find(a, r, &x)) return;
-  const int np = span_prefix(a);
-  float4* out = reinterpret_cast<float4*>(a.ctx + ((size_t)r * a.nq + (size_t)kvh * a.group + f - r * a.group) * kHd) + lane;
-  const size_t at = (size_t)kvh * F + f, step = (size_t)gridDim.y * F;
-  const float nan = __int_as_float(0x7fc00000);
-  if (np < 0 || x.len < 0) {
-    *out = make_float4(nan, nan, nan, nan);
-    if (p.stat && lane == 0) p.stat[at] = make_float2(0.f, nan);
-    return;
+  const bool prefix = blockIdx.x < (unsigned)(tiles * p.npc);   // (then F is 8 or less)
+  if (prefix) {
+    const SpanRest rest = span_rest(a, p, 0);
+    const int len = span_chunk(rest.end - rest.start, p.npc);
+    p0 = rest.start + blockIdx.x * len;
+    p1 = min(rest.end, p0 + len);
+    f0 = 0;
+    nf = F;
+    slot = p.nwt + blockIdx.x;
+    k = a.pk + kvh * a.p_head;
+    v = a.pv + kvh * a.p_head;
+    lim_all = a.run ? min(p1, a.plen + 1) : p1;
+  } else {
+    const int b = blockIdx.x - tiles * p.npc, chunk = b % p.ntc;
+    const SpanItem it = span_item(a, b / p.ntc, kFewRows);
+    if (it.nf == 0 || it.x.len <= 0) return;
+    x = it.x;
+    f0 = it.f0;
+    nf = it.nf;
+    const int len = span_chunk(x.len, p.ntc);
+    p0 = chunk * len;
+    p1 = min(x.sees((f0 + nf - 1) / a.group), p0 + len);
+    slot = p.nwt + p.npc + chunk;
+    k = a.tk + (size_t)x.s * a.t_seq + kvh * a.t_head;
+    v = a.tv + (size_t)x.s * a.t_seq + kvh * a.t_head;
+    lim_all = min(p1, x.sees(f0 / a.group));
   }
-  // its stretches of whole tiles, its chunks of the rest, its chunks of the tail
-  int nw = 0, n0 = 0, n1 = 0;
-  if (p.nwt) {
+  if (p0 >= p1) return;
+  const int nb = (p1 - p0 + kFwBlock - 1) / kFwBlock;
+  const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem);
+  uint8_t* ring = smem + kFwQ + warp * kFwStages * 2 * kFwTile;
+  const uint32_t ring_s = sm + kFwQ + warp * kFwStages * 2 * kFwTile;
+  auto fetch = [&](int b, int stage) {
+    if (b < nb) {
+      const uint32_t to = ring_s + stage * 2 * kFwTile;
+#pragma unroll
+      for (int i = 0; i < kFwBlock * 16 / 32; ++i) {
+        const int u = lane + 32 * i, r = u >> 4, c = u & 15, pos = p0 + b * kFwBlock + r;
+        const bool live = pos < p1;
+        const size_t at = (size_t)(live ? pos : p0) * kHd + 8 * c;
+        cp16(to + swz(r, c), k + at, live);
+        cp16(to + kFwTile + swz(r, c), v + at, live);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < kFwStages; ++s) fetch(warp + s * kFwWarps, s);
+  rows_split(a, kvh, f0, nf, smem, s_fac, warp, kFwWarps);
+  __syncthreads();
+  const int fr = f0 + gl;
+  const bool row_live = gl < nf;
+  const int lim = !row_live ? 0 : a.run ? min(p1, a.plen + fr / a.group + 1) : prefix ? p1 : min(p1, x.sees(fr / a.group));
+  const float fac = row_live ? s_fac[gl] : 0.0f;
+  uint32_t qa[8][4];
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) ldsm(qa[kk], sm + swz(lane & 15, 2 * kk + (lane >> 4)));
+  float m = -INFINITY, l = 0.0f;
+  float acc[16][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0f;
+  int stage = 0;
+#pragma unroll 1
+  for (int b = warp; b < nb; b += kFwWarps) {
+    asm volatile("cp.async.wait_group %0;" :: "n"(kFwStages - 1) : "memory");
+    __syncwarp();
+    const uint32_t kt = ring_s + stage * 2 * kFwTile, vt = kt + kFwTile;
+    const int base = p0 + b * kFwBlock;
+    const bool all = base + kFwBlock <= lim_all;
+    unsigned bad = 0;
+    if (lim_all < min(p1, base + kFwBlock)) {
+      // V of positions that some row does not see: as in k_span_part
+      uint8_t* vs = ring + stage * 2 * kFwTile + kFwTile;
+#pragma unroll
+      for (int i = 0; i < kFwBlock * 16 / 32; ++i) {
+        const int u = lane + 32 * i;
+        uint4* w = reinterpret_cast<uint4*>(vs + swz(u >> 4, u & 15));
+        if (not_finite(*w)) {
+          *w = make_uint4(0, 0, 0, 0);
+          bad |= 1u << (u >> 4);
+        }
+      }
+      bad = __reduce_or_sync(0xFFFFFFFFu, bad);
+      __syncwarp();
+    }
+    float sc[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sc[j][i] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < 8; ++kk) {
+      uint32_t kb[4];
+      ldsm(kb, kt + swz((lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)));
+      mma_f16(sc[0], qa[kk], kb[0], kb[1]);
+      mma_f16(sc[1], qa[kk], kb[2], kb[3]);
+    }
+    float w[4];
+    float up = m;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int pos = base + 8 * (j >> 1) + 2 * t + (j & 1);
+      const float y = (sc[j >> 1][j & 1] + sc[j >> 1][2 + (j & 1)]) * fac;
+      w[j] = all || pos < lim ? y : -INFINITY;
+      up = fmaxf(up, w[j]);
+    }
+    if (p.scores && row_live) {
+      float* to = p.scores + ((size_t)kvh * a.group + fr) * a.pcap;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int pos = base + 8 * (j >> 1) + 2 * t + (j & 1);
+        if (pos < p1) to[pos] = w[j];
+      }
+    }
+    up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, 1));
+    up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, 2));
+    if (__any_sync(0xFFFFFFFFu, up > m)) {
+      const float c = m == -INFINITY ? 0.0f : ex2(m - up);
+      l *= c;
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] *= c;
+      m = up;
+    }
+    const float m0 = m == -INFINITY ? 0.0f : m - kPtLift;
+    uint32_t wa[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      w[j] = ex2(w[j] - m0);
+      l += w[j];
+    }
+    if (bad) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = 8 * (j >> 1) + 2 * t + (j & 1);
+        if (base + at < lim && (bad >> at & 1)) l = __int_as_float(0x7fc00000);
+      }
+    }
+    split_half2(w[0], w[1], &wa[0], &wa[1]);
+    split_half2(w[2], w[3], &wa[2], &wa[3]);
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      uint32_t vb[4];
+      ldsm_t(vb, vt + swz(lane & 15, 2 * d + (lane >> 4)));
+      mma_f16(acc[2 * d], wa, vb[0], vb[1]);
+      mma_f16(acc[2 * d + 1], wa, vb[2], vb[3]);
+    }
+    __syncwarp();
+    fetch(b + kFwStages * kFwWarps, stage);
+    stage = stage + 1 == kFwStages ? 0 : stage + 1;
+  }
+  // the warps meet
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+  l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+  if (t == 0) { s_m[warp][gl] = m; s_l[warp][gl] = l; }
+  __syncthreads();                                         // the rings are free
+  float* lines = reinterpret_cast<float*>(smem + kFwQ);
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    *reinterpret_cast<float2*>(lines + (warp * 8 + gl) * kPtLine + 8 * i + 2 * t) =
+        make_float2(acc[i][0] + acc[i][2], acc[i][1] + acc[i][3]);
+  __syncthreads();
+  const size_t row = ((size_t)slot * gridDim.y + kvh) * F + f0;
+  for (int g = warp; g < nf; g += kFwWarps) {
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kFwWarps; ++j) M = fmaxf(M, s_m[j][g]);
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < kFwWarps; ++j) {
+      const float c = s_l[j][g] == 0.0f ? 0.0f : ex2(s_m[j][g] - M);
+      const float4 z = *reinterpret_cast<const float4*>(lines + (j * 8 + g) * kPtLine + 4 * lane);
+      L += c * s_l[j][g];
+      y.x += c * z.x; y.y += c * z.y; y.z += c * z.z; y.w += c * z.w;
+    }
+    reinterpret_cast<float4*>(p.part + (row + g) * kHd)[lane] = y;
+    if (lane == 0) p.ml[row + g] = make_float2(M - kPtLift, L);
+  }
+}
+
+// ---- a row's chunks added up -----------------------------------------------------------------
+//
+// kWarps warps share a row's slots, kPer rows a CTA (all of one tile of kStRows): one warp a row
+// where slots are few, with several rows after each other where rows are many, so that the fixed
+// part (which slots there are) is spread over them; four where a row's loads would follow each other.
+template <int kWarps, int kPer>
+__global__ void __launch_bounds__(256, kWarps == 1 ? 5 : 3) k_span_join(SpanArgs a, SpanParts p) {
+  constexpr int kAt = kWarps == 1 ? 4 : 8;                 // slots' rows under way
+  __shared__ float4 s_sum[8][32];
+  __shared__ float2 s_ml[8];
+  const int kvh = blockIdx.y, F = a.nrow * a.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int fb = blockIdx.x * kPer;             // the CTA's first row
+  const int np = span_prefix(a);
+  const size_t step = (size_t)gridDim.y * F;
+  const float nan = __int_as_float(0x7fc00000);
+  // its stretches of whole tiles
+  int nw = 0;
+  if (p.nwt && fb < F) {
     const SpanWhole wh = span_whole(a, np, p.grid);
-    const int tile = f / kStRows, whole = span_whole_of(a, np, tile);
+    const int tile = fb / kStRows, whole = span_whole_of(a, np, tile);
     if (whole) {
-      const long long u = ((long long)kvh * wh.rows + tile) * wh.tiles;
+      const unsigned u = ((unsigned)kvh * wh.rows + tile) * wh.tiles;
       nw = span_cta(wh, u + whole - 1) - span_cta(wh, u) + 1;
     }
   }
-  if (p.npc) {
-    const SpanRest rest = span_rest(a, p, f / kSpanItem);
-    const int end = a.run ? a.plen + r + 1 : rest.end, len = span_chunk(rest.end - rest.start, p.npc);
-    if (end > rest.start) n0 = (end - rest.start + len - 1) / len;
-  }
-  if (p.ntc) {
-    const int see = x.sees(r);
-    if (see) n1 = (see + span_chunk(x.len, p.ntc) - 1) / span_chunk(x.len, p.ntc);
-  }
-  auto slot = [&](int i) { return i < nw ? i : i < nw + n0 ? p.nwt + i - nw : p.nwt + p.npc + i - nw - n0; };
-  const int all = nw + n0 + n1;
-  // a lane has a chunk's maximum and sum (32 chunks at a time), then all lanes its row's sums
-  float M = -INFINITY, L = 0.0f;
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < all; i0 += 32) {
-    const int n = min(32, all - i0);
-    const float2 ml = lane < n ? p.ml[at + slot(i0 + lane) * step] : make_float2(-INFINITY, 0.0f);
-    float up = fmaxf(M, ml.x);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, d));
-    const float c = ml.y == 0.0f ? 0.0f : ex2(ml.x - up), old = M == -INFINITY ? 0.0f : ex2(M - up);
-    float sum = c * ml.y;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    M = up;
-    L = L * old + sum;
-    s.x *= old; s.y *= old; s.z *= old; s.w *= old;
 #pragma unroll 1
-    for (int j0 = 0; j0 < n; j0 += 8) {
-      float4 y[8];
+  for (int i = warp / kWarps; i < kPer; i += 8 / kWarps) {
+    const int f = fb + i;
+    if (f >= F) {
+      const int Fp = (F + kStRows - 1) / kStRows * kStRows;
+      if (p.terms && f < Fp && lane < 2) p.facs[((size_t)lane * gridDim.y + kvh) * Fp + f] = lane ? -INFINITY : 0.0f;
+      if (kWarps == 1) continue;
+    }
+    const int r = f / a.group;
+    SpanSeq x;
+    const bool here = f < F && span_find(a, r, &x);        // the same for the row's warps
+    if (kWarps == 1 && !here) continue;
+    const size_t at = (size_t)kvh * F + f;
+    const bool no = here && (np < 0 || x.len < 0);
+    // its chunks of the rest, its chunks of the tail
+    int n0 = 0, n1 = 0;
+    if (here && !no && p.npc) {
+      const SpanRest rest = span_rest(a, p, f / kSpanItem);
+      const int end = a.run ? a.plen + r + 1 : rest.end, len = span_chunk(rest.end - rest.start, p.npc);
+      if (end > rest.start) n0 = (end - rest.start + len - 1) / len;
+    }
+    if (here && !no && p.ntc) {
+      const int see = x.sees(r);
+      if (see) n1 = (see + span_chunk(x.len, p.ntc) - 1) / span_chunk(x.len, p.ntc);
+    }
+    const int all = here && !no ? nw + n0 + n1 : 0;
+    auto slot = [&](int k) {
+      const int j = k * kWarps + warp % kWarps;            // this warp's k-th
+      return at + (j < nw ? j : j < nw + n0 ? p.nwt + j - nw : p.nwt + p.npc + j - nw - n0) * step;
+    };
+    const int mine = (all - warp % kWarps + kWarps - 1) / kWarps;
+    // a lane has a chunk's maximum and sum, 32 chunks at a time; the rows' sums are loaded before
+    // those are known, kAt at a time
+    float M = -INFINITY, L = 0.0f;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int i0 = 0; i0 < mine; i0 += 32) {
+      const int n = min(32, mine - i0);
+      float4 y[kAt];
+      auto load = [&](int j0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j0 + j < n) y[j] = __ldg(reinterpret_cast<const float4*>(p.part + (at + slot(i0 + j0 + j) * step) * kHd) + lane);
+        for (int j = 0; j < kAt; ++j)
+          if (j0 + j < n) y[j] = __ldg(reinterpret_cast<const float4*>(p.part + slot(i0 + j0 + j) * kHd) + lane);
+      };
+      const float2 ml = lane < n ? p.ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.0f);
+      load(0);
+      float up = fmaxf(M, ml.x);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (j0 + j >= n) continue;
-        const float f = __shfl_sync(0xFFFFFFFFu, c, j0 + j);
-        s.x += f * y[j].x; s.y += f * y[j].y; s.z += f * y[j].z; s.w += f * y[j].w;
+      for (int d = 16; d; d >>= 1) up = fmaxf(up, __shfl_xor_sync(0xFFFFFFFFu, up, d));
+      const float c = ml.y == 0.0f ? 0.0f : ex2(ml.x - up), old = M == -INFINITY ? 0.0f : ex2(M - up);
+      float sum = c * ml.y;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
+      M = up;
+      L = L * old + sum;
+      s.x *= old; s.y *= old; s.z *= old; s.w *= old;
+#pragma unroll 1
+      for (int j0 = 0; j0 < n; j0 += kAt) {
+        if (j0) load(j0);
+#pragma unroll
+        for (int j = 0; j < kAt; ++j) {
+          if (j0 + j >= n) continue;
+          const float g = __shfl_sync(0xFFFFFFFFu, c, j0 + j);
+          s.x += g * y[j].x; s.y += g * y[j].y; s.z += g * y[j].z; s.w += g * y[j].w;
+        }
       }
     }
-  }
-  const float inv = all ? 1.0f / L : 0.0f;
-  *out = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
-  if (p.stat && lane == 0) p.stat[at] = make_float2(M, L);
-  if (p.terms) {
-    const float4 q = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + f - r * a.group) * kHd) + lane);
-    uint2 hi, lo;
-    const float lift = row_terms(q, &hi, &lo);
-    reinterpret_cast<uint2*>(p.terms + at * kHd)[lane] = hi;
-    reinterpret_cast<uint2*>(p.terms + (at + step) * kHd)[lane] = lo;
-    if (lane == 0) {
-      facs(0) = __ldg(a.scale) * kLog2e / lift;
-      facs(1) = -(M + log2f(L));
+    if constexpr (kWarps > 1) {
+      s_sum[warp][lane] = s;
+      if (lane == 0) s_ml[warp] = make_float2(M, L);
+      __syncthreads();                                     // (one round: kPer is 8 / kWarps)
+      if (warp % kWarps != 0) continue;
+      for (int j = 1; j < kWarps; ++j) M = fmaxf(M, s_ml[warp + j].x);
+      L = 0.0f;
+      s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int j = 0; j < kWarps; ++j) {
+        const float2 ml = s_ml[warp + j];
+        const float g = ml.y == 0.0f ? 0.0f : ex2(ml.x - M);
+        const float4 z = s_sum[warp + j][lane];
+        L += g * ml.y;
+        s.x += g * z.x; s.y += g * z.y; s.z += g * z.z; s.w += g * z.w;
+      }
+      if (!here) continue;
+    }
+    const float inv = no ? nan : all ? 1.0f / L : 0.0f;
+    if (no) L = nan;
+    const size_t out = ((size_t)r * a.nq + (size_t)kvh * a.group + f - r * a.group) * kHd;
+    reinterpret_cast<float4*>(a.ctx + out)[lane] = make_float4(s.x * inv, s.y * inv, s.z * inv, s.w * inv);
+    if (p.stat && lane == 0) p.stat[at] = make_float2(M, L);
+    if (p.terms) {
+      const float4 q = __ldg(reinterpret_cast<const float4*>(a.q + out) + lane);
+      uint2 hi, lo;
+      const float lift = row_terms(q, &hi, &lo);
+      reinterpret_cast<uint2*>(p.terms + at * kHd)[lane] = hi;
+      reinterpret_cast<uint2*>(p.terms + (at + step) * kHd)[lane] = lo;
+      const int Fp = (F + kStRows - 1) / kStRows * kStRows;
+      if (lane < 2)
+        p.facs[((size_t)lane * gridDim.y + kvh) * Fp + f] = lane ? -(M + log2f(L)) : __ldg(a.scale) * kLog2e / lift;
     }
   }
 }
@@ -579,21 +813,25 @@ constexpr int kSms = 148, kPtCtas = 2 * kSms;
 struct SpanPlan {
   int tiles, items, nwt, npc, ntc;     // tiles of the prefix's rows, items of the tails'
   size_t part, ml, stat, scores, terms, facs, bytes;
-  bool mass_tiles;
+  bool mass_tiles, few;
 };
 SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool mass) {
   SpanPlan p{};
   auto stages = [](int n) { return (n + kSpanStage - 1) / kSpanStage; };
   p.tiles = (F + kSpanItem - 1) / kSpanItem;
-  p.items = nseq + p.tiles;
   // many rows over many positions go by whole tiles
   if (F > 32 && (long long)F * pcap >= 1 << 17) {
     const long long rows = (long long)nkv * ((F + kStRows - 1) / kStRows);
-    p.nwt = (int)std::min((long long)((pcap + kStRows - 1) / kStRows), kSms / rows + 2);
+    if (rows * ((pcap + kStRows - 1) / kStRows) < 1ll << 31)
+      p.nwt = (int)std::min((long long)((pcap + kStRows - 1) / kStRows), kSms / rows + 2);
   }
   // ... of a shared prefix all of it, of a run's cache what every row of a tile sees
   p.npc = std::min(stages(p.nwt ? (run ? 2 * kStRows : 0) : pcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * p.tiles)));
   if (!run) p.ntc = std::min(stages(tcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * std::max(nseq, p.tiles))));
+  // eights of rows where the prefix has no more, or is k_span_tile's and the tails' rows are few
+  p.few = F <= kFewRows || (!run && p.nwt && F / nseq <= 2 * kFewRows);
+  const int size = p.few ? kFewRows : kSpanItem;
+  p.items = run ? 0 : nseq + (F + size - 1) / size;
   // room for this call and any smaller one, which may have more chunks of fewer rows: chunks times
   // tiles (or sequences) are at most kPtCtas / nkv, or one each
   const size_t all = (size_t)nkv * F;
@@ -637,17 +875,18 @@ int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const Sp
   const unsigned nkv = (unsigned)(a.nq / a.group), F = (unsigned)(a.nrow * a.group);
   const long long ctas = (long long)p.tiles * p.npc + (long long)p.items * p.ntc;
   HV_REQUIRE(ctas < (1ll << 31), HV_E_UNSUPPORTED, "%s: too many rows", name);
-  // eight rows at the most where every row of a sequence has its own and the prefix has no more
-  const bool few = F <= 8 || (!a.run && !a.row0 && s.npc == 0);
-  const void* fn = few ? (const void*)k_span_part<1> : (const void*)k_span_part<8>;
-  const int smem = few ? kPtSmem<1> : kPtSmem<8>;
+  const void* fn = p.few ? (const void*)k_span_few : (const void*)k_span_part;
+  const int smem = p.few ? kFwSmem : kPtSmem;
   const int rc = smem_attr(fn, smem);
   if (rc) return rc;
-  if (few) k_span_part<1><<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, smem, st>>>(a, s, p.tiles);
-  else k_span_part<8><<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, smem, st>>>(a, s, p.tiles);
+  if (p.few) k_span_few<<<dim3((unsigned)ctas, nkv), 32 * kFwWarps, smem, st>>>(a, s, p.tiles);
+  else k_span_part<<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, smem, st>>>(a, s, p.tiles);
   HV_CUDA(cudaGetLastError());
   const unsigned rows = s.terms ? (F + kStRows - 1) / kStRows * kStRows : F;
-  k_span_join<<<dim3((rows + 7) / 8, nkv), 256, 0, st>>>(a, s);
+  const size_t all = (size_t)rows * nkv;
+  if (s.nwt + s.npc + s.ntc > 8 && all <= 1024) k_span_join<4, 2><<<dim3((rows + 1) / 2, nkv), 256, 0, st>>>(a, s);
+  else if (all <= 8192) k_span_join<1, 8><<<dim3((rows + 7) / 8, nkv), 256, 0, st>>>(a, s);
+  else k_span_join<1, 32><<<dim3((rows + 31) / 32, nkv), 256, 0, st>>>(a, s);
   HV_LAUNCHED(name);
 }
 

@@ -73,8 +73,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
   const int np = span_prefix(a);
   const SpanWhole wh = span_whole(a, np, gridDim.x);
   if ((int)blockIdx.x >= wh.ctas) return;
-  const long long u1 = wh.units * (blockIdx.x + 1) / wh.ctas;
-  const long long u0 = wh.units * blockIdx.x / wh.ctas;
+  const unsigned u0 = span_first(wh, blockIdx.x), u1 = span_first(wh, blockIdx.x + 1);
 
   const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem);
   auto bar = [](const unsigned long long& b) { return (uint32_t)__cvta_generic_to_shared(&b); };
@@ -107,23 +106,24 @@ __global__ void __launch_bounds__(kStThreads, 1)
   auto rows_sync = [] { asm volatile("bar.sync 3, 256;" ::: "memory"); };
   // the next stretch with work: its place, tiles j0 .. j0 + nt - 1 of positions, and its rows' slot
   struct Stretch {
-    long long u;
+    unsigned u;
     int kvh, row0, j0, nt;
     int cut;                                      // positions of its last tile, 0: all
     size_t part_row;
   };
   auto next = [&](Stretch& s) {
     while (s.u < u1) {
-      const int R = (int)(s.u / wh.tiles), tile = R % wh.rows;
-      s.kvh = R / wh.rows;
-      s.j0 = (int)(s.u - (long long)R * wh.tiles);
-      const int some = (int)min((long long)wh.tiles - s.j0, u1 - s.u);
+      const unsigned R = s.u / wh.tiles;
+      s.kvh = (int)(R / wh.rows);
+      const int tile = (int)(R - s.kvh * wh.rows);
+      s.j0 = (int)(s.u - R * wh.tiles);
+      const int some = min(wh.tiles - s.j0, (int)(u1 - s.u));
       s.u += some;
       s.nt = min(span_whole_of(a, np, tile) - s.j0, some);
       if (s.nt <= 0) continue;
       s.row0 = tile * kStRows;
       s.cut = !a.run && s.j0 + s.nt == wh.tiles ? np % kStRows : 0;
-      const int slot = blockIdx.x - span_cta(wh, (long long)R * wh.tiles);
+      const int slot = blockIdx.x - span_cta(wh, R * wh.tiles);
       s.part_row = ((size_t)slot * nkv + s.kvh) * F + s.row0;
       return true;
     }
