@@ -158,7 +158,8 @@ struct SpanParts {
   float* part;
   float2* ml;
   float2* stat;                        // [nkv][F]: m and the sum of all, for the weights' sake
-  float* scores;                       // [nq][pcap], of a single row
+  float* scores;                       // [nq][scores_ld], of a single row
+  size_t scores_ld;
   // what k_mass_tile reads of the rows: their two binary16 terms [2][nkv][F][128]; and, F rounded
   // up to whole tiles, the factor and the term [2][nkv][..] that take their sums of products to
   // exponents of weights (-m - log2 l; -infinity behind F)

@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(32 * kFwWarps, 2) k_span_few(SpanArgs a, SpanP
       up = fmaxf(up, w[j]);
     }
     if (p.scores && row_live) {
-      float* to = p.scores + ((size_t)kvh * a.group + fr) * a.pcap;
+      float* to = p.scores + ((size_t)kvh * a.group + fr) * p.scores_ld;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int pos = base + 8 * (j >> 1) + 2 * t + (j & 1);
@@ -515,7 +515,7 @@ __global__ void __launch_bounds__(32 * kFwWarps, 2) k_span_few(SpanArgs a, SpanP
 // where slots are few, with several rows after each other where rows are many, so that the fixed
 // part (which slots there are) is spread over them; four where a row's loads would follow each other.
 template <int kWarps, int kPer>
-__global__ void __launch_bounds__(256, kWarps == 1 ? 5 : 3) k_span_join(SpanArgs a, SpanParts p) {
+HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
   constexpr int kAt = kWarps == 1 ? 4 : 8;                 // slots' rows under way
   __shared__ float4 s_sum[8][32];
   __shared__ float2 s_ml[8];
@@ -637,34 +637,61 @@ __global__ void __launch_bounds__(256, kWarps == 1 ? 5 : 3) k_span_join(SpanArgs
   }
 }
 
-// The weights of a single row's scores, which k_span_part has left in the scratch.
-__global__ void __launch_bounds__(256) k_mass_dec(SpanArgs a, SpanParts p, const float* mass_in, float* mass_out) {
-  __shared__ float2 s_ml[8];
+template <int kWarps, int kPer>
+__global__ void __launch_bounds__(256, kWarps == 1 ? 5 : 3) k_span_join(SpanArgs a, SpanParts p) {
+  span_join<kWarps, kPer>(a, p);
+}
+
+// A single row's end: its chunks added up by the first CTAs of a kv head, and by the others the
+// weights of the scores that k_span_few has left, 1024 positions each.
+constexpr int kOnePos = 1024;
+__global__ void __launch_bounds__(256) k_span_one(SpanArgs a, SpanParts p, const float* mass_in, float* mass_out, int joins) {
+  if ((int)blockIdx.x < joins) return span_join<4, 2>(a, p);
+  __shared__ float2 s_one[8];
   const int kvh = blockIdx.y, np = span_prefix(a), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (np < 0 || (int)blockIdx.x * 256 >= np) return;
+  const int t0 = (blockIdx.x - joins) * kOnePos + 4 * threadIdx.x;
+  if (np < 0 || t0 - 4 * (int)threadIdx.x >= np) return;
+  const float* scores = p.scores + (size_t)kvh * a.group * p.scores_ld + t0;
+  float4 x[8];
+#pragma unroll
+  for (int h = 0; h < 8; ++h)
+    if (h < a.group && t0 < np) x[h] = __ldg(reinterpret_cast<const float4*>(scores + (size_t)h * p.scores_ld));
+  const size_t i = (size_t)kvh * a.pcap + t0;
+  float in[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) in[k] = mass_in && t0 + k < np - 1 ? mass_in[i + k] : 0.0f;
   const int len = span_chunk(np, p.npc), n0 = (np + len - 1) / len;
   if (warp < a.group) {
     const size_t at = (size_t)kvh * a.group + warp, step = (size_t)gridDim.y * a.group;
     float M = -INFINITY, L = 0.0f;
-    for (int i = lane; i < n0; i += 32) M = fmaxf(M, p.ml[at + i * step].x);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xFFFFFFFFu, M, d));
-    for (int i = lane; i < n0; i += 32) {
-      const float2 ml = p.ml[at + i * step];
-      L += ml.y == 0.0f ? 0.0f : ex2(ml.x - M) * ml.y;
+    for (int c = lane; c < n0; c += 32) {
+      const float2 ml = p.ml[at + c * step];
+      const float up = fmaxf(M, ml.x);
+      L = (M == -INFINITY ? 0.0f : L * ex2(M - up)) + (ml.y == 0.0f ? 0.0f : ex2(ml.x - up) * ml.y);
+      M = up;
     }
 #pragma unroll
-    for (int d = 16; d; d >>= 1) L += __shfl_xor_sync(0xFFFFFFFFu, L, d);
-    if (lane == 0) s_ml[warp] = make_float2(M, 1.0f / L);
+    for (int d = 16; d; d >>= 1) {
+      const float m2 = __shfl_xor_sync(0xFFFFFFFFu, M, d), l2 = __shfl_xor_sync(0xFFFFFFFFu, L, d), up = fmaxf(M, m2);
+      L = (L == 0.0f ? 0.0f : L * ex2(M - up)) + (l2 == 0.0f ? 0.0f : l2 * ex2(m2 - up));
+      M = up;
+    }
+    if (lane == 0) s_one[warp] = make_float2(M, 1.0f / L);
   }
   __syncthreads();
-  const int t = blockIdx.x * 256 + threadIdx.x;
-  if (t >= np) return;
-  float sum = 0.0f;
-  for (int h = 0; h < a.group; ++h)
-    sum += ex2(p.scores[((size_t)kvh * a.group + h) * a.pcap + t] - s_ml[h].x) * s_ml[h].y;
-  const size_t i = (size_t)kvh * a.pcap + t;
-  mass_out[i] = (mass_in && t < np - 1 ? mass_in[i] : 0.0f) + sum;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int h = 0; h < 8; ++h) {
+    if (h >= a.group) break;
+    const float2 s = s_one[h];
+    sum[0] += ex2(x[h].x - s.x) * s.y;
+    sum[1] += ex2(x[h].y - s.x) * s.y;
+    sum[2] += ex2(x[h].z - s.x) * s.y;
+    sum[3] += ex2(x[h].w - s.x) * s.y;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (t0 + k < np) mass_out[i + k] = in[k] + sum[k];
 }
 
 // ---- the weights that a run's rows give ------------------------------------------------------
@@ -844,13 +871,13 @@ SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool 
   p.part = up(rows * kHd * 4);
   p.ml = up(rows * 8);
   p.stat = up(mass ? (size_t)nkv * F * 8 : 0);
-  p.scores = up(mass ? (size_t)nkv * 8 * pcap * 4 : 0);
+  p.scores = up(mass ? (size_t)nkv * 8 * (pcap + 4) * 4 : 0);
   p.terms = up(mass ? 2 * all * kHd * 2 : 0);
   p.facs = up(mass ? 2 * (size_t)nkv * (F + kStRows) * 4 : 0);
   p.bytes = p.part + p.ml + p.stat + p.scores + p.terms + p.facs + 256;
   return p;
 }
-SpanParts span_parts(const SpanPlan& p, void* scratch, bool mass, bool scores) {
+SpanParts span_parts(const SpanPlan& p, void* scratch, int pcap, bool mass, bool scores) {
   uint8_t* at = reinterpret_cast<uint8_t*>(scratch);
   SpanParts s{};
   s.part = reinterpret_cast<float*>(at);
@@ -864,6 +891,7 @@ SpanParts span_parts(const SpanPlan& p, void* scratch, bool mass, bool scores) {
   s.npc = p.npc;
   s.ntc = p.ntc;
   s.grid = kSms;
+  s.scores_ld = (size_t)(pcap + 3) / 4 * 4;
   return s;
 }
 
@@ -882,6 +910,10 @@ int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const Sp
   if (p.few) k_span_few<<<dim3((unsigned)ctas, nkv), 32 * kFwWarps, smem, st>>>(a, s, p.tiles);
   else k_span_part<<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, smem, st>>>(a, s, p.tiles);
   HV_CUDA(cudaGetLastError());
+  return HV_OK;
+}
+int join_launch(const char* name, const SpanArgs& a, const SpanParts& s, cudaStream_t st) {
+  const unsigned nkv = (unsigned)(a.nq / a.group), F = (unsigned)(a.nrow * a.group);
   const unsigned rows = s.terms ? (F + kStRows - 1) / kStRows * kStRows : F;
   const size_t all = (size_t)rows * nkv;
   if (s.nwt + s.npc + s.ntc > 8 && all <= 1024) k_span_join<4, 2><<<dim3((rows + 1) / 2, nkv), 256, 0, st>>>(a, s);
@@ -913,13 +945,17 @@ int mass_any(const char* name, const SpanArgs& a, const float* mass_in, float* m
   SpanPlan p = span_plan(nkv, a.nrow * a.group, 1, cap, 0, true, true);
   const int n = a.plen + a.nrow;
   p.mass_tiles = !one && (long long)a.nrow * a.group * n >= 1 << 18;
-  SpanParts s = span_parts(p, scratch, true, one);
+  SpanParts s = span_parts(p, scratch, cap, true, one);
   int rc = span_launch(name, a, p, s, st);
   if (rc) return rc;
   if (one) {
-    k_mass_dec<<<dim3((unsigned)((cap + 255) / 256), (unsigned)nkv), 256, 0, st>>>(a, s, mass_in, mass_out);
+    const int joins = (a.group + 1) / 2;
+    k_span_one<<<dim3((unsigned)(joins + (cap + kOnePos - 1) / kOnePos), (unsigned)nkv), 256, 0, st>>>(
+        a, s, mass_in, mass_out, joins);
     HV_LAUNCHED(name);
   }
+  rc = join_launch(name, a, s, st);
+  if (rc) return rc;
   if (p.mass_tiles) return mass_tile_launch(a, s, mass_in, mass_out, cap, st);
   // a CTA an SM, as far as the positions go
   auto ctas = [&](int pos) { return (long long)nkv * ((n + 16 * pos - 1) / (16 * pos)); };
@@ -971,7 +1007,9 @@ extern "C" int hv_attn_shared_f16(const float* q, const uint16_t* pk, const uint
   a.pcap = pcap; a.tcap = tcap;
   a.nq = nq; a.group = group; a.nseq = nseq; a.nrow = nrow;
   const SpanPlan p = span_plan((int)nkv, nrow * group, nseq, pcap, tcap, false, false);
-  return span_launch(name, a, p, span_parts(p, scratch, false, false), (cudaStream_t)stream);
+  const SpanParts s = span_parts(p, scratch, pcap, false, false);
+  const int rc2 = span_launch(name, a, p, s, (cudaStream_t)stream);
+  return rc2 ? rc2 : join_launch(name, a, s, (cudaStream_t)stream);
 }
 
 extern "C" int hv_attn_mass_scratch(int nq, int group, int cap, int ntok, size_t* bytes) {
