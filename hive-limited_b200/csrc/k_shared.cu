@@ -58,17 +58,27 @@ HV_DEV float row_terms(const float4& x, uint2* hi, uint2* lo) {
 
 // The two terms of rows f0 .. f0 + nf - 1 of kv head kvh to shared memory, eight rows of first
 // terms, then their second ones; what takes a row's sums of products to exponents to `fac`.
-HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, float* fac, int warp, int warps) {
+// A warp's rows are all loaded before the first is worked on.
+template <int kRows, int kWarps>
+HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, float* fac, int warp) {
   const int lane = threadIdx.x & 31;
   const float f = __ldg(a.scale) * kLog2e;
-  for (int i = warp; i < (nf + 7) / 8 * 8; i += warps) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 x[kRows / kWarps];
+#pragma unroll
+  for (int j = 0; j < kRows / kWarps; ++j) {
+    const int i = warp + j * kWarps;
+    x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (i < nf) {
       const int r = (f0 + i) / a.group, h = f0 + i - r * a.group;
-      x = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + h) * kHd) + lane);
+      x[j] = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + h) * kHd) + lane);
     }
+  }
+#pragma unroll
+  for (int j = 0; j < kRows / kWarps; ++j) {
+    const int i = warp + j * kWarps;
+    if (i >= (nf + 7) / 8 * 8) break;
     uint2 hi, lo;
-    const float lift = row_terms(x, &hi, &lo);
+    const float lift = row_terms(x[j], &hi, &lo);
     const int at = (i >> 3) * 16 + (i & 7);
     *reinterpret_cast<uint2*>(to + swz(at, lane >> 1) + 8 * (lane & 1)) = hi;
     *reinterpret_cast<uint2*>(to + swz(at + 8, lane >> 1) + 8 * (lane & 1)) = lo;
@@ -154,7 +164,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
   };
 #pragma unroll
   for (int s = 0; s < kPtStages; ++s) fetch(s);
-  rows_split(a, kvh, f0, nf, smem, s_fac, warp, kPtWarps);
+  rows_split<kSpanItem, kPtWarps>(a, kvh, f0, nf, smem, s_fac, warp);
 
   // warps by eights of rows, then by positions
   const int oct = (nf + 7) / 8;
@@ -373,7 +383,7 @@ __global__ void __launch_bounds__(32 * kFwWarps, 2) k_span_few(SpanArgs a, SpanP
   };
 #pragma unroll
   for (int s = 0; s < kFwStages; ++s) fetch(warp + s * kFwWarps, s);
-  rows_split(a, kvh, f0, nf, smem, s_fac, warp, kFwWarps);
+  rows_split<kFewRows, kFwWarps>(a, kvh, f0, nf, smem, s_fac, warp);
   __syncthreads();
   const int fr = f0 + gl;
   const bool row_live = gl < nf;
@@ -735,7 +745,7 @@ __global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, cons
   for (int f0 = first; f0 < F; f0 += kSpanItem) {
     const int nf = min(kSpanItem, F - f0);
     __syncthreads();
-    rows_split(a, kvh, f0, nf, smem, s_fac, warp, 8);
+    rows_split<kSpanItem, 8>(a, kvh, f0, nf, smem, s_fac, warp);
     if (threadIdx.x < nf) {
       const float2 s = p.stat[(size_t)kvh * F + f0 + threadIdx.x];
       s_stat[threadIdx.x] = make_float2(s.x, 1.0f / s.y);
