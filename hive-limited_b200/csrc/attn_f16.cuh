@@ -112,25 +112,29 @@ HV_HD int span_chunk(int n, int most) {
   return (c + kSpanStage - 1) / kSpanStage * kSpanStage;
 }
 
-// What k_span_tile takes: of a shared prefix everything, in tiles of kStRows positions, of a run's
-// cache the whole tiles that every row of a tile of kStRows (row, head) pairs sees. Units of work are
-// (kv head, tile of rows, tile of positions), `tiles` of the last for every tile of rows (a run's
-// first ones have fewer), cut evenly among `ctas` CTAs.
+// What k_span_tile takes: a shared prefix, or all that a run's rows see, in tiles of kStRows
+// positions. Units of work are (kv head, tile of kStRows (row, head) pairs, tile of positions),
+// `tiles` of the last for every tile of rows (a run's first ones have fewer), cut evenly among `ctas`
+// CTAs.
 constexpr int kStRows = 128;
 struct SpanWhole {
   unsigned units;
   int tiles, rows, ctas;
 };
-HV_DEV int span_whole_of(const SpanArgs& a, int np, int tile) {
-  if (np < 0) return 0;
-  return a.run ? (np + tile * kStRows / a.group + 1) / kStRows : (np + kStRows - 1) / kStRows;
+// Positions of the prefix (or cache) that pair f sees.
+HV_DEV int span_sees(const SpanArgs& a, int np, int f) {
+  return np < 0 ? 0 : a.run ? np + f / a.group + 1 : np;
+}
+HV_DEV int span_tiles_of(const SpanArgs& a, int np, int tile) {
+  const int last = min(a.nrow * a.group, (tile + 1) * kStRows) - 1;
+  return (span_sees(a, np, last) + kStRows - 1) / kStRows;
 }
 // Where the tiles of rows are few enough, as many CTAs take each as there are SMs for: a CTA that
 // ends one tile of rows and begins another pays for it about what three tiles of positions take.
 HV_DEV SpanWhole span_whole(const SpanArgs& a, int np, int grid) {
   SpanWhole w;
   w.rows = (a.nrow * a.group + kStRows - 1) / kStRows;
-  w.tiles = span_whole_of(a, np, w.rows - 1);
+  w.tiles = span_tiles_of(a, np, w.rows - 1);
   const unsigned all = (unsigned)(a.nq / a.group) * w.rows;
   w.units = all * w.tiles;                       // under 2^31: see span_plan
   w.ctas = (int)min((unsigned)grid, w.units);
@@ -150,9 +154,14 @@ HV_DEV int span_cta(const SpanWhole& w, unsigned u) {
   return c;
 }
 
+// Is one of eight halves an infinity or a NaN?
+HV_DEV bool not_finite(const uint4& y) {
+  auto odd = [](uint32_t z) { return (z & 0x7C00u) == 0x7C00u || (z & 0x7C000000u) == 0x7C000000u; };
+  return odd(y.x) || odd(y.y) || odd(y.z) || odd(y.w);
+}
+
 // Partial results in the caller's scratch, in slots: nwt for the stretches of k_span_tile (at most
-// that many a tile of rows), npc for the prefix's chunks (or what is left of it), ntc for the
-// tails'. part [slot][nkv][F][128], ml [slot][nkv][F]: sums and the sum of the weights 2^(x - m),
+// that many a tile of rows) or npc for the prefix's chunks, ntc for the tails'. part [slot][nkv][F][128], ml [slot][nkv][F]: sums and the sum of the weights 2^(x - m),
 // relative to m.
 struct SpanParts {
   float* part;
@@ -166,6 +175,7 @@ struct SpanParts {
   __half* terms;
   float* facs;
   int nwt, npc, ntc, grid;             // grid: CTAs of k_span_tile
+  int size;                            // pairs of a tile of the prefix's chunks and of an item
 };
 
 // Tensor copies of boxes of kStRows rows by 64 values of [outer][rows][128], rows of 128 bytes in

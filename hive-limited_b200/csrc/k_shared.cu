@@ -86,26 +86,7 @@ HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, 
   }
 }
 
-// Is one of eight halves an infinity or a NaN?
-HV_DEV bool not_finite(const uint4& y) {
-  auto odd = [](uint32_t z) { return (z & 0x7C00u) == 0x7C00u || (z & 0x7C000000u) == 0x7C000000u; };
-  return odd(y.x) || odd(y.y) || odd(y.z) || odd(y.w);
-}
-
-// What k_span_part has of the prefix for the rows of a tile of kSpanItem: all, or what k_span_tile
-// leaves. A run's end goes by the tile's last row.
-struct SpanRest {
-  int start, end;
-};
-HV_DEV SpanRest span_rest(const SpanArgs& a, const SpanParts& p, int tile) {
-  const int np = span_prefix(a);
-  SpanRest r;
-  r.start = p.nwt ? span_whole_of(a, np, tile * kSpanItem / kStRows) * kStRows : 0;
-  r.end = a.run ? np + (min(a.nrow * a.group, (tile + 1) * kSpanItem) - 1) / a.group + 1 : np;
-  return r;
-}
-
-__global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles) {
+__global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles, int size) {
   extern __shared__ __align__(1024) uint8_t smem[];         // the rows, then stages of K and V
   __shared__ float s_fac[kSpanItem], s_m[kPtWarps][8], s_l[kPtWarps][8];
   __shared__ int s_bad[kSpanStage];
@@ -118,20 +99,19 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
   const bool prefix = blockIdx.x < (unsigned)(tiles * p.npc);
   if (prefix) {
     const int tile = blockIdx.x / p.npc, chunk = blockIdx.x % p.npc;
-    const SpanRest rest = span_rest(a, p, tile);
-    const int len = span_chunk(rest.end - rest.start, p.npc);
-    p0 = rest.start + chunk * len;
-    p1 = min(rest.end, p0 + len);
+    f0 = tile * size;
+    nf = min(size, F - f0);
+    const int n = span_sees(a, span_prefix(a), f0 + nf - 1), len = span_chunk(n, p.npc);
+    p0 = chunk * len;
+    p1 = min(n, p0 + len);
     if (p0 >= p1) return;
-    f0 = tile * kSpanItem;
-    nf = min(kSpanItem, F - f0);
     slot = p.nwt + chunk;
     k = a.pk + kvh * a.p_head;
     v = a.pv + kvh * a.p_head;
     lim_all = a.run ? min(p1, a.plen + f0 / a.group + 1) : p1;
   } else {
     const int b = blockIdx.x - tiles * p.npc, chunk = b % p.ntc;
-    const SpanItem it = span_item(a, b / p.ntc, kSpanItem);
+    const SpanItem it = span_item(a, b / p.ntc, size);
     if (it.nf == 0 || it.x.len <= 0) return;
     x = it.x;
     f0 = it.f0;
@@ -275,10 +255,10 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
         }
     };
     if (mine) {
-      if (wp > 4) {
-        // eight warps with the same rows: every second stage's 16 positions are this warp's
+      if (wp >= 4) {
+        // four warps with the same rows have 16 positions each, eight those of every second stage
         const int at = 16 * (pg & 3);
-        if ((s & 1) == pg >> 2 && base + at < p1) unit(at, std::integral_constant<int, 1>{});
+        if ((wp == 4 || (s & 1) == pg >> 2) && base + at < p1) unit(at, std::integral_constant<int, 1>{});
       } else {
 #pragma unroll 1
         for (int u = 0; u < 2; ++u)
@@ -300,6 +280,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
         make_float2(acc[i][0] + acc[i][2], acc[i][1] + acc[i][3]);
   __syncthreads();
   const size_t row = ((size_t)slot * gridDim.y + kvh) * F + f0;
+#pragma unroll 2
   for (int i = warp; i < nf; i += kPtWarps) {
     const int oo = i >> 3, g = i & 7;
     float M = -INFINITY, L = 0.0f;
@@ -337,10 +318,9 @@ __global__ void __launch_bounds__(32 * kFwWarps, 2) k_span_few(SpanArgs a, SpanP
   SpanSeq x;
   const bool prefix = blockIdx.x < (unsigned)(tiles * p.npc);   // (then F is 8 or less)
   if (prefix) {
-    const SpanRest rest = span_rest(a, p, 0);
-    const int len = span_chunk(rest.end - rest.start, p.npc);
-    p0 = rest.start + blockIdx.x * len;
-    p1 = min(rest.end, p0 + len);
+    const int n = span_sees(a, span_prefix(a), F - 1), len = span_chunk(n, p.npc);
+    p0 = blockIdx.x * len;
+    p1 = min(n, p0 + len);
     f0 = 0;
     nf = F;
     slot = p.nwt + blockIdx.x;
@@ -538,7 +518,7 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
   int nw = 0;
   if (p.nwt && fb < F) {
     const SpanWhole wh = span_whole(a, np, p.grid);
-    const int tile = fb / kStRows, whole = span_whole_of(a, np, tile);
+    const int tile = fb / kStRows, whole = span_tiles_of(a, np, tile);
     if (whole) {
       const unsigned u = ((unsigned)kvh * wh.rows + tile) * wh.tiles;
       nw = span_cta(wh, u + whole - 1) - span_cta(wh, u) + 1;
@@ -558,12 +538,11 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
     if (kWarps == 1 && !here) continue;
     const size_t at = (size_t)kvh * F + f;
     const bool no = here && (np < 0 || x.len < 0);
-    // its chunks of the rest, its chunks of the tail
+    // its chunks of the prefix, its chunks of the tail
     int n0 = 0, n1 = 0;
     if (here && !no && p.npc) {
-      const SpanRest rest = span_rest(a, p, f / kSpanItem);
-      const int end = a.run ? a.plen + r + 1 : rest.end, len = span_chunk(rest.end - rest.start, p.npc);
-      if (end > rest.start) n0 = (end - rest.start + len - 1) / len;
+      const int n = span_sees(a, np, min(F, (f / p.size + 1) * p.size) - 1), len = span_chunk(n, p.npc);
+      if (n > 0) n0 = (span_sees(a, np, f) + len - 1) / len;
     }
     if (here && !no && p.ntc) {
       const int see = x.sees(r);
@@ -848,27 +827,33 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // chunks as give every SM two CTAs, of a stage at the least.
 constexpr int kSms = 148, kPtCtas = 2 * kSms;
 struct SpanPlan {
-  int tiles, items, nwt, npc, ntc;     // tiles of the prefix's rows, items of the tails'
+  int size, tiles, items, nwt, npc, ntc;   // tiles of the prefix's rows, items of the tails'
   size_t part, ml, stat, scores, terms, facs, bytes;
   bool mass_tiles, few;
 };
 SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool mass) {
   SpanPlan p{};
   auto stages = [](int n) { return (n + kSpanStage - 1) / kSpanStage; };
-  p.tiles = (F + kSpanItem - 1) / kSpanItem;
   // many rows over many positions go by whole tiles
   if (F > 32 && (long long)F * pcap >= 1 << 17) {
     const long long rows = (long long)nkv * ((F + kStRows - 1) / kStRows);
     if (rows * ((pcap + kStRows - 1) / kStRows) < 1ll << 31)
       p.nwt = (int)std::min((long long)((pcap + kStRows - 1) / kStRows), kSms / rows + 2);
   }
-  // ... of a shared prefix all of it, of a run's cache what every row of a tile sees
-  p.npc = std::min(stages(p.nwt ? (run ? 2 * kStRows : 0) : pcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * p.tiles)));
-  if (!run) p.ntc = std::min(stages(tcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * std::max(nseq, p.tiles))));
-  // eights of rows where the prefix has no more, or is k_span_tile's and the tails' rows are few
+  // eights of rows where the prefix has no more, or is k_span_tile's and the tails' rows are few;
+  // else as many of them a CTA as leave one for every SM: a product of the f16 pipe takes 16 cycles
+  // of a quarter of an SM, so that 64 rows by 64 positions are 2.5 us of one CTA's time
   p.few = F <= kFewRows || (!run && p.nwt && F / nseq <= 2 * kFewRows);
-  const int size = p.few ? kFewRows : kSpanItem;
-  p.items = run ? 0 : nseq + (F + size - 1) / size;
+  p.size = kFewRows;
+  if (!p.few) {
+    p.size = kSpanItem;
+    const int most = p.nwt ? stages(tcap) : stages(pcap) + (run ? 0 : stages(tcap));
+    while (p.size > 16 && (long long)nkv * ((F + p.size - 1) / p.size) * most < kSms) p.size /= 2;
+  }
+  p.tiles = (F + p.size - 1) / p.size;
+  p.items = run ? 0 : nseq + p.tiles;
+  if (!p.nwt) p.npc = std::min(stages(pcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * p.tiles)));
+  if (!run) p.ntc = std::min(stages(tcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * std::max(nseq, p.tiles))));
   // room for this call and any smaller one, which may have more chunks of fewer rows: chunks times
   // tiles (or sequences) are at most kPtCtas / nkv, or one each
   const size_t all = (size_t)nkv * F;
@@ -900,6 +885,7 @@ SpanParts span_parts(const SpanPlan& p, void* scratch, int pcap, bool mass, bool
   s.nwt = p.nwt;
   s.npc = p.npc;
   s.ntc = p.ntc;
+  s.size = p.size;
   s.grid = kSms;
   s.scores_ld = (size_t)(pcap + 3) / 4 * 4;
   return s;
@@ -912,13 +898,14 @@ int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const Sp
   }
   const unsigned nkv = (unsigned)(a.nq / a.group), F = (unsigned)(a.nrow * a.group);
   const long long ctas = (long long)p.tiles * p.npc + (long long)p.items * p.ntc;
+  if (ctas == 0) return HV_OK;                              // a run that k_span_tile has all of
   HV_REQUIRE(ctas < (1ll << 31), HV_E_UNSUPPORTED, "%s: too many rows", name);
   const void* fn = p.few ? (const void*)k_span_few : (const void*)k_span_part;
   const int smem = p.few ? kFwSmem : kPtSmem;
   const int rc = smem_attr(fn, smem);
   if (rc) return rc;
   if (p.few) k_span_few<<<dim3((unsigned)ctas, nkv), 32 * kFwWarps, smem, st>>>(a, s, p.tiles);
-  else k_span_part<<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, smem, st>>>(a, s, p.tiles);
+  else k_span_part<<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, smem, st>>>(a, s, p.tiles, p.size);
   HV_CUDA(cudaGetLastError());
   return HV_OK;
 }

@@ -1,7 +1,6 @@
-// Attention of many rows a head over a binary16 cache, on the fifth-generation tensor cores: what
-// every row of a tile of 128 (row, head) pairs sees, 128 positions to a tile, the last one of a
-// shared prefix maybe less. What is left (a run's own positions, tails) is k_span_part's, and
-// k_span_join adds up.
+// Attention of many rows a head over a binary16 cache, on the fifth-generation tensor cores: a shared
+// prefix, or all that a run's rows see, for tiles of 128 (row, head) pairs by 128 positions. Tails
+// are k_span_few's or k_span_part's, and k_span_join adds up.
 //
 // The rows' first and second binary16 terms are the operand in tensor memory, K and V tiles come
 // by tensor copies into swizzled shared memory as they stand in the cache: K with the dims
@@ -14,7 +13,9 @@
 //   warps 8-11   a thread adds its row of O to 128 sums in registers (tensor memory's sums are cut,
 //                not rounded, so O is of one tile, and the small terms go first)
 //   warps 12, 13 one thread each: the copies of K and of V
-//   warps 14, 15 make zeros of what a last tile's V has behind the prefix
+//   warps 14, 15 look over V of tiles that some row does not see whole: what lies behind the rows'
+//                positions becomes zeros, and so does a position that is not finite, as 0 times it
+//                would be added to rows that do not see it; those that do end as NaN
 // A row's weights are 2^(x - m + 8) with m a whole number that a tile's largest exponent may pass:
 // as long as no 16 of them add up to more than 2^15 they fit binary16 and are exact to 2^-33 of
 // the largest, so that the scores are read once, without a pass for their maximum. The first tile
@@ -55,10 +56,11 @@ HV_DEV uint64_t smem_desc_mn(uint32_t addr) {   // 128-byte swizzle, 64 halves o
 
 struct StShared {
   unsigned long long full_k[2], full_v[2], s_ready[2], w_ready[2], o_done[2];
-  unsigned long long o_free, v_clean, drain[2];
+  unsigned long long o_free, v_clean[2], drain[2];
   float top[4][kStRows];         // of the last four tiles: what their weights are relative to
   float m[2][kStRows], l[2][kStRows];
   uint32_t tmem;
+  int bad;                       // first position of the stretch that is not finite
   int given_up;
 };
 constexpr int kStSmem = 4 * kStTile + kStRows * kStLine * 4 + (int)sizeof(StShared);   // K, V twice
@@ -85,9 +87,9 @@ __global__ void __launch_bounds__(kStThreads, 1)
       bar_init(bar(sh.w_ready[i]), 128);
       bar_init(bar(sh.o_done[i]), 1);
       bar_init(bar(sh.drain[i]), 1);
+      bar_init(bar(sh.v_clean[i]), 64);
     }
     bar_init(bar(sh.o_free), 128);
-    bar_init(bar(sh.v_clean), 64);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.given_up = (sm & 1023) != 0;               // the swizzle goes by addresses
   }
@@ -108,7 +110,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
   struct Stretch {
     unsigned u;
     int kvh, row0, j0, nt;
-    int cut;                                      // positions of its last tile, 0: all
+    int full, end;                                // its tiles that all rows see whole, positions
     size_t part_row;
   };
   auto next = [&](Stretch& s) {
@@ -119,10 +121,11 @@ __global__ void __launch_bounds__(kStThreads, 1)
       s.j0 = (int)(s.u - R * wh.tiles);
       const int some = min(wh.tiles - s.j0, (int)(u1 - s.u));
       s.u += some;
-      s.nt = min(span_whole_of(a, np, tile) - s.j0, some);
+      s.nt = min(span_tiles_of(a, np, tile) - s.j0, some);
       if (s.nt <= 0) continue;
       s.row0 = tile * kStRows;
-      s.cut = !a.run && s.j0 + s.nt == wh.tiles ? np % kStRows : 0;
+      s.full = min(max(span_sees(a, np, s.row0) / kStRows - s.j0, 0), s.nt);
+      s.end = span_sees(a, np, min(F, s.row0 + kStRows) - 1) - s.j0 * kStRows;
       const int slot = blockIdx.x - span_cta(wh, R * wh.tiles);
       s.part_row = ((size_t)slot * nkv + s.kvh) * F + s.row0;
       return true;
@@ -137,7 +140,12 @@ __global__ void __launch_bounds__(kStThreads, 1)
   };
   Stretch st;
   st.u = u0;
-  int g0 = 0, cuts = 0;                           // tiles and cut ones before this stretch's
+  int g0 = 0, parts = 0;                          // tiles before this stretch's; bit i mod 2: was the
+                                                  // number of those with a part odd?
+  auto step_on = [&] {                            // (at most two tiles of a stretch are parts)
+    for (int i = g0 + st.full; i < g0 + st.nt; ++i) parts ^= 1 << (i & 1);
+    g0 += st.nt;
+  };
   auto rows_out = [&] {
     asm volatile("bar.sync 2, 384;" ::: "memory");
     float4* to = reinterpret_cast<float4*>(p.part + st.part_row * kHd);
@@ -150,7 +158,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kStRegsRow));
     int drains = 0;
 #pragma unroll 1
-    for (; next(st); g0 += st.nt, cuts += st.cut > 0, stretch_end()) {
+    for (; next(st); step_on(), stretch_end()) {
       // The queries in two terms: a row's two threads have half of its dims each. They take the
       // scale's sign.
       float qs;
@@ -190,6 +198,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
       rows_sync();
       fence_after();
       float m = -INFINITY, l = 0.0f;              // of this thread's row
+      const int sees = span_sees(a, np, min(st.row0 + row, F - 1)) - st.j0 * kStRows;
       const uint32_t s_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * w;
       const uint32_t leader = elect_one();
       const uint32_t qh = tmem + kStColQ, ql = qh + 64;
@@ -218,7 +227,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
         ok = ok && bar_wait_warp(bar(sh.full_v[s]), (i >> 1) & 1, given_up);
         ok = ok && bar_wait_warp(bar(sh.w_ready[s]), (i >> 1) & 1, given_up);
         if (i > 0) ok = ok && bar_wait_warp(bar(sh.o_free), (i - 1) & 1, given_up);
-        if (st.cut && i == g0 + st.nt - 1) ok = ok && bar_wait_warp(bar(sh.v_clean), cuts & 1, given_up);
+        if (i - g0 >= st.full) ok = ok && bar_wait_warp(bar(sh.v_clean[s]), parts >> s & 1, given_up);
         fence_after();
 #pragma unroll 1
         for (int pass = 0; pass < 2 && ok; ++pass) {
@@ -246,14 +255,15 @@ __global__ void __launch_bounds__(kStThreads, 1)
         return ceilf(big * qs);
       };
       auto weights = [&](int i, bool first) {
-        if (st.cut && i == g0 + st.nt - 1) {      // what the tile has behind the prefix
+        if (i - g0 >= st.full) {                  // what the row does not see of the tile
+          const int see = sees - (i - g0) * kStRows;
 #pragma unroll 1
-          for (int c = st.cut & ~15; c < kStRows; c += 16) {
+          for (int c = 0; c < kStRows; c += 16) {
             uint32_t x[16];
             tmem_ld16(s_at + c, x);
             tmem_wait(x);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) x[k] = c + k < st.cut ? x[k] : 0xFF800000u;
+            for (int k = 0; k < 16; ++k) x[k] = c + k < see ? x[k] : 0xFF800000u;
             tmem_st16(s_at + c, x);
           }
           tmem_st_wait();
@@ -364,7 +374,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
   } else if (warp < 12) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kStRegsSum));
 #pragma unroll 1
-    for (; next(st); g0 += st.nt, cuts += st.cut > 0, stretch_end()) {
+    for (; next(st); step_on(), stretch_end()) {
       uint64_t acc[kHd / 2];
 #pragma unroll
       for (int d = 0; d < kHd / 2; ++d) acc[d] = 0;
@@ -400,7 +410,9 @@ __global__ void __launch_bounds__(kStThreads, 1)
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         L += sh.l[k][row] == 0.0f ? 0.0f : sh.l[k][row] * ex2(sh.m[k][row] - M);
-      if (*given_up) L = __int_as_float(0x7fc00000);
+      // (warps 14 and 15 are done with V once the last sums are there)
+      if (*given_up || span_sees(a, np, min(st.row0 + row, F - 1)) - st.j0 * kStRows > sh.bad)
+        L = __int_as_float(0x7fc00000);
       float* line = lines + (size_t)row * kStLine;
 #pragma unroll
       for (int d = 0; d < kHd / 2; d += 2) {
@@ -413,18 +425,30 @@ __global__ void __launch_bounds__(kStThreads, 1)
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kStRegsCopy));
 #pragma unroll 1
-    for (; next(st); g0 += st.nt, cuts += st.cut > 0, stretch_end()) {
+    for (; next(st); step_on(), stretch_end()) {
       if (warp >= 14) {
-        if (!st.cut) continue;
-        const int i = g0 + st.nt - 1;
-        if (bar_wait_warp(bar(sh.full_v[i & 1]), (i >> 1) & 1, given_up)) {
-          uint8_t* v = smem + (2 + (i & 1)) * kStTile + 16 * (lane & 7);
-          for (int r = st.cut + (lane >> 3) + 4 * (warp - 14); r < kStRows; r += 8)
+        if (warp == 14 && lane == 0) sh.bad = 1 << 30;
+        asm volatile("bar.sync 4, 64;" ::: "memory");
+#pragma unroll 1
+        for (int i = g0 + st.full; i < g0 + st.nt; ++i) {
+          if (bar_wait_warp(bar(sh.full_v[i & 1]), (i >> 1) & 1, given_up)) {
+            // a thread has 16 bytes of every eighth row
+            uint8_t* v = smem + (2 + (i & 1)) * kStTile + 16 * (lane & 7);
+            const int at = (i - g0) * kStRows;
+            for (int r = (lane >> 3) + 4 * (warp - 14); r < kStRows; r += 8)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) *reinterpret_cast<uint4*>(v + h * kStHalf + r * 128) = make_uint4(0, 0, 0, 0);
+              for (int h = 0; h < 2; ++h) {
+                uint4* y = reinterpret_cast<uint4*>(v + h * kStHalf + r * 128);
+                const bool behind = at + r >= st.end;
+                if (behind || not_finite(*y)) {
+                  *y = make_uint4(0, 0, 0, 0);
+                  if (!behind) atomicMin(&sh.bad, at + r);
+                }
+              }
+          }
+          fence_async();
+          bar_arrive(bar(sh.v_clean[i & 1]));
         }
-        fence_async();
-        bar_arrive(bar(sh.v_clean));
         continue;
       }
       if (lane != 0) continue;
