@@ -12,8 +12,8 @@
 //                the next S_w = ql K^T + qh K^T
 //   warps 8-11   a thread adds its row of O to 128 sums in registers (tensor memory's sums are cut,
 //                not rounded, so O is of one tile, and the small terms go first)
-//   warps 12, 13 one thread each: the copies of K and of V
-//   warps 14, 15 look over V of tiles that some row does not see whole: what lies behind the rows'
+//   warps 12, 13 the copies of K and of V, issued by one thread
+//   warps 13-15  look over V of tiles that some row does not see whole: what lies behind the rows'
 //                positions becomes zeros, and so does a position that is not finite, as 0 times it
 //                would be added to rows that do not see it; those that do end as NaN
 // A row's weights are 2^(x - m + 8) with m a whole number that a tile's largest exponent may pass:
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
       bar_init(bar(sh.w_ready[i]), 128);
       bar_init(bar(sh.o_done[i]), 1);
       bar_init(bar(sh.drain[i]), 1);
-      bar_init(bar(sh.v_clean[i]), 64);
+      bar_init(bar(sh.v_clean[i]), 96);
     }
     bar_init(bar(sh.o_free), 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
 #pragma unroll
       for (int k = 0; k < 2; ++k)
         L += sh.l[k][row] == 0.0f ? 0.0f : sh.l[k][row] * ex2(sh.m[k][row] - M);
-      // (warps 14 and 15 are done with V once the last sums are there)
+      // (V has been looked over once the last sums are there)
       if (*given_up || span_sees(a, np, min(st.row0 + row, F - 1)) - st.j0 * kStRows > sh.bad)
         L = __int_as_float(0x7fc00000);
       float* line = lines + (size_t)row * kStLine;
@@ -424,52 +424,76 @@ __global__ void __launch_bounds__(kStThreads, 1)
     }
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kStRegsCopy));
+    // a tile of K or V; a buffer is free once its last product is done
+    auto tile_load = [&](int to, const CUtensorMap* map, int pos, int head, uint32_t full) {
+      if (lane != 0) return;
+      bar_expect(full, kStTile);
+      tile_copy(sm + to, map, 0, pos, head, full);
+      tile_copy(sm + to + kStHalf, map, 64, pos, head, full);
+    };
 #pragma unroll 1
     for (; next(st); step_on(), stretch_end()) {
-      if (warp >= 14) {
-        if (warp == 14 && lane == 0) sh.bad = 1 << 30;
-        asm volatile("bar.sync 4, 64;" ::: "memory");
-#pragma unroll 1
-        for (int i = g0 + st.full; i < g0 + st.nt; ++i) {
-          if (bar_wait_warp(bar(sh.full_v[i & 1]), (i >> 1) & 1, given_up)) {
-            // a thread has 16 bytes of every eighth row
-            uint8_t* v = smem + (2 + (i & 1)) * kStTile + 16 * (lane & 7);
-            const int at = (i - g0) * kStRows;
-            for (int r = (lane >> 3) + 4 * (warp - 14); r < kStRows; r += 8)
+      if (warp == 13 && lane == 0) sh.bad = 1 << 30;
+      // Warps 13 to 15 meet at every part once its V has come, which warp 13 has seen: a barrier's
+      // phases can only be told apart by who follows each of them.
+      auto clean = [&](int i, bool live) {
+        asm volatile("bar.sync 4, 96;" ::: "memory");
+        if (live) {
+          // a thread has 16 bytes of every twelfth row
+          uint8_t* v = smem + (2 + (i & 1)) * kStTile + 16 * (lane & 7);
+          const int at = (i - g0) * kStRows;
+          for (int r = (lane >> 3) + 4 * (warp - 13); r < kStRows; r += 12)
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                uint4* y = reinterpret_cast<uint4*>(v + h * kStHalf + r * 128);
-                const bool behind = at + r >= st.end;
-                if (behind || not_finite(*y)) {
-                  *y = make_uint4(0, 0, 0, 0);
-                  if (!behind) atomicMin(&sh.bad, at + r);
-                }
+            for (int h = 0; h < 2; ++h) {
+              uint4* y = reinterpret_cast<uint4*>(v + h * kStHalf + r * 128);
+              const bool behind = at + r >= st.end;
+              if (behind || not_finite(*y)) {
+                *y = make_uint4(0, 0, 0, 0);
+                if (!behind) atomicMin(&sh.bad, at + r);
               }
-          }
-          fence_async();
-          bar_arrive(bar(sh.v_clean[i & 1]));
+            }
         }
+        fence_async();
+        bar_arrive(bar(sh.v_clean[i & 1]));
+      };
+      if (warp >= 14) {
+#pragma unroll 1
+        for (int i = g0 + st.full; i < g0 + st.nt; ++i) clean(i, true);
+        continue;
+      }
+      if (warp == 13) {
+        bool live = true;
+        int issued = g0;
+#pragma unroll 1
+        for (int i = g0; i < g0 + st.nt; ++i) {
+          const int s = i & 1;
+          live = live && (i < 2 || bar_wait_warp(bar(sh.o_done[s]), ((i - 2) >> 1) & 1, given_up));
+          live = live && !__any_sync(0xFFFFFFFFu, *given_up);
+          if (live) {
+            tile_load(2 * kStTile + s * kStTile, &map_v, (st.j0 + i - g0) * kStRows, st.kvh, bar(sh.full_v[s]));
+            issued = i + 1;
+          }
+          if (i - g0 >= st.full) {
+            if (live) bar_wait_warp(bar(sh.full_v[s]), (i >> 1) & 1, given_up);
+            clean(i, live);
+          }
+        }
+        int no = 0;                               // no copy outlives the CTA
+        for (int i = max(g0, issued - 2); i < issued; ++i)
+          bar_wait_warp(bar(sh.full_v[i & 1]), (i >> 1) & 1, &no);
         continue;
       }
       if (lane != 0) continue;
-      // the copies of K (warp 12) and V (13): a buffer is free once its last product is done
-      const bool kk = warp == 12;
-      const CUtensorMap* map = kk ? &map_k : &map_v;
-      const uint32_t to = sm + (kk ? 0 : 2 * kStTile);
       int issued = g0;
       for (int i = g0; i < g0 + st.nt; ++i, ++issued) {
         const int s = i & 1;
-        const uint32_t full = bar(kk ? sh.full_k[s] : sh.full_v[s]);
-        if (i >= 2 && !bar_wait(bar(kk ? sh.s_ready[s] : sh.o_done[s]), ((i - 2) >> 1) & 1, given_up)) break;
+        if (i >= 2 && !bar_wait(bar(sh.s_ready[s]), ((i - 2) >> 1) & 1, given_up)) break;
         if (*given_up) break;
-        bar_expect(full, kStTile);
-        const int pos = (st.j0 + i - g0) * kStRows;
-        tile_copy(to + s * kStTile, map, 0, pos, st.kvh, full);
-        tile_copy(to + s * kStTile + kStHalf, map, 64, pos, st.kvh, full);
+        tile_load(s * kStTile, &map_k, (st.j0 + i - g0) * kStRows, st.kvh, bar(sh.full_k[s]));
       }
-      int no = 0;                                 // no copy outlives the CTA
+      int no = 0;
       for (int i = max(g0, issued - 2); i < issued; ++i)
-        bar_wait(bar(kk ? sh.full_k[i & 1] : sh.full_v[i & 1]), (i >> 1) & 1, &no);
+        bar_wait(bar(sh.full_k[i & 1]), (i >> 1) & 1, &no);
     }
   }
   if (warp == 15)

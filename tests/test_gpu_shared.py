@@ -89,7 +89,7 @@ def test_runs_of_rows(hv, nkv, group, plen, rows, tails):
 
 @pytest.mark.parametrize("nkv,group,nseq,plen", [
     (1, 1, 129, 2100), (2, 3, 50, 2500), (1, 5, 70, 1024), (8, 4, 64, 1100), (3, 7, 40, 1500),
-    (1, 8, 64, 4097), (1, 2, 65, 2176), (1, 4, 40, 12800)])
+    (1, 8, 64, 4097), (1, 2, 65, 2176), (1, 4, 40, 12800), (8, 8, 64, 2100), (8, 4, 33, 8190)])
 def test_many_rows_over_a_long_prefix(hv, nkv, group, nseq, plen):
     g = np.random.default_rng(plen)
     check_shared(hv, g, nkv, group, plen, plen + 130, [1] * nseq, [1 + i % 7 for i in range(nseq)], 9, one=True)
@@ -373,7 +373,7 @@ def test_decode_with_mass(hv, nkv, group, n, form):
 @pytest.mark.parametrize("nkv,group,pos0,ntok", [
     (1, 1, 0, 1), (2, 4, 0, 5), (8, 2, 256, 44), (1, 8, 100, 17), (2, 5, 63, 65), (1, 3, 1000, 31),
     (2, 4, 128, 128), (1, 8, 700, 256), (2, 1, 0, 300), (1, 2, 2048, 200), (1, 7, 4000, 3),
-    (1, 1, 900, 290), (2, 5, 500, 120), (1, 3, 0, 700)])
+    (1, 1, 900, 290), (2, 5, 500, 120), (1, 3, 0, 700), (8, 8, 2100, 64), (8, 4, 1000, 200)])
 def test_run_with_mass(hv, nkv, group, pos0, ntok):
     g = np.random.default_rng(pos0 + ntok)
     check_mass(hv, g, nkv, group, pos0, ntok, pos0 + ntok + 2, False, "apart")
