@@ -14,6 +14,12 @@
 namespace hv {
 namespace {
 
+// The kernel that this one may have started beside ends before this one does, and so before whatever
+// comes next: its first CTA waits for that.
+HV_DEV void end_after_prior() {
+  if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 // ---- attention of few rows a head ---------------------------------------------------------
 //
 // A CTA has up to 64 (row, head) pairs of a kv head and a chunk of the prefix or of a sequence's
@@ -86,7 +92,7 @@ HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, 
   }
 }
 
-__global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles, int size) {
+HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles, int size) {
   extern __shared__ __align__(1024) uint8_t smem[];         // the rows, then stages of K and V
   __shared__ float s_fac[kSpanItem], s_m[kPtWarps][8], s_l[kPtWarps][8];
   __shared__ int s_bad[kSpanStage];
@@ -298,6 +304,11 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
   }
 }
 
+__global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles, int size) {
+  span_part(a, p, tiles, size);
+  end_after_prior();
+}
+
 // ---- attention of up to eight rows ---------------------------------------------------------
 //
 // One item of eight (row, head) pairs and a chunk of positions a CTA, as for k_span_part, but every
@@ -308,7 +319,7 @@ constexpr int kFwTile = kFwBlock * kHd * 2;              // bytes of K or of V o
 constexpr int kFwQ = 2 * kFewRows * kHd * 2;
 constexpr int kFwSmem = kFwQ + kFwWarps * kFwStages * 2 * kFwTile;
 
-__global__ void __launch_bounds__(32 * kFwWarps, 2) k_span_few(SpanArgs a, SpanParts p, int tiles) {
+HV_DEV void span_few(const SpanArgs& a, const SpanParts& p, int tiles) {
   extern __shared__ __align__(1024) uint8_t smem[];         // the rows, then the warps' rings
   __shared__ float s_fac[kFewRows], s_m[kFwWarps][8], s_l[kFwWarps][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
@@ -497,6 +508,11 @@ __global__ void __launch_bounds__(32 * kFwWarps, 2) k_span_few(SpanArgs a, SpanP
     reinterpret_cast<float4*>(p.part + (row + g) * kHd)[lane] = y;
     if (lane == 0) p.ml[row + g] = make_float2(M - kPtLift, L);
   }
+}
+
+__global__ void __launch_bounds__(32 * kFwWarps, 2) k_span_few(SpanArgs a, SpanParts p, int tiles) {
+  span_few(a, p, tiles);
+  end_after_prior();
 }
 
 // ---- a row's chunks added up -----------------------------------------------------------------
@@ -768,46 +784,72 @@ __global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, cons
   }
 }
 
-// hv_qk_rows's arithmetic for the rows of a batch: a warp per (row, head).
-__global__ void __launch_bounds__(256) k_qk_shared(const float* __restrict__ qkv, const float* __restrict__ qn,
+// hv_qk_rows's arithmetic for the rows of a batch. Eight lanes have a head, lane j its dims j, j + 8,
+// ..: those are numpy's accumulator j of the sum of squares, and a dim's partner in the rotation is
+// the same lane's, so that a head takes three shuffles and no shared memory (a warp a head, as
+// k_qk_rows has it: 228 rows of 64 + 8 heads 10.5 us).
+constexpr int kQkWarps = 2;             // of a CTA: few rows are to be spread over the SMs
+__global__ void __launch_bounds__(32 * kQkWarps) k_qk_shared(const float* __restrict__ qkv, const float* __restrict__ qn,
                                                    const float* __restrict__ kn, const float* __restrict__ cos_t,
                                                    const float* __restrict__ sin_t, int cap,
                                                    const int32_t* __restrict__ base, SpanArgs a,
                                                    float* __restrict__ q_out, __half* tk, __half* tv,
                                                    int nkv, float eps) {
-  __shared__ __align__(16) float tmp[8][kHd], row_s[8][kHd];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, heads = a.nq + nkv;
-  const long long wi = (long long)blockIdx.x * 8 + warp;
-  if (wi >= (long long)a.nrow * heads) return;            // whole warps
-  const int r = (int)(wi / heads), h = (int)(wi % heads);
-  SpanSeq x;
-  if (!span_find(a, r, &x)) return;
-  const int slot = x.len - (x.end - r);
-  const long long pos = (long long)__ldg(base) + slot;
-  const bool ok = x.len >= 0 && slot >= 0 && pos >= 0 && pos < cap;
-  const float* row = qkv + (size_t)r * (a.nq + 2 * nkv) * kHd;
+  const int heads = a.nq + nkv, per = (heads + 3) / 4;     // warps a row
+  const long long wi = (long long)blockIdx.x * kQkWarps + (threadIdx.x >> 5);
+  const int r = (int)(wi / per), h = 4 * (int)(wi - (long long)r * per) + ((threadIdx.x & 31) >> 3), j = threadIdx.x & 7;
+  if (r >= a.nrow) return;                                 // whole warps
+  const float* row = qkv + (size_t)r * (a.nq + 2 * nkv) * kHd + j;
+  const bool here = h < heads, is_q = h < a.nq;
+  float x[16], v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    x[i] = here ? __ldg(row + (size_t)h * kHd + 8 * i) : 0.0f;
+    v[i] = here && !is_q ? __ldg(row + (size_t)(h + nkv) * kHd + 8 * i) : 0.0f;
+  }
+  const int first = __ldg(base);
+  SpanSeq s;
+  if (!span_find(a, r, &s)) return;
+  const int slot = s.len - (s.end - r);
+  const long long pos = (long long)first + slot;
+  const bool ok = s.len >= 0 && slot >= 0 && pos >= 0 && pos < cap;
+  float* q = q_out + ((size_t)r * a.nq + h) * kHd + j;
   if (!ok) {
-    if (h < a.nq) {
-      const float nan = __int_as_float(0x7fc00000);
-      reinterpret_cast<float4*>(q_out + ((size_t)r * a.nq + h) * kHd)[lane] = make_float4(nan, nan, nan, nan);
-    }
+    if (is_q)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) q[8 * i] = __int_as_float(0x7fc00000);
     return;
   }
-  const float* cs = cos_t + (size_t)pos * (kHd / 2);
-  const float* sn = sin_t + (size_t)pos * (kHd / 2);
-  if (h < a.nq) {
-    warp_norm_rope(row + (size_t)h * kHd, qn, cs, sn, eps, tmp[warp], q_out + ((size_t)r * a.nq + h) * kHd);
+  // the norm, as warp_norm_rope forms it
+  float ss = __fmul_rn(x[0], x[0]);
+#pragma unroll
+  for (int i = 1; i < 16; ++i) ss = __fadd_rn(ss, __fmul_rn(x[i], x[i]));
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xFFFFFFFFu, ss, d));
+  if (!here) return;
+  const float d = __fsqrt_rn(__fadd_rn(__fdiv_rn(__fadd_rn(0.0f, ss), (float)kHd), eps));
+  const float* gain = (is_q ? qn : kn) + j;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = __fmul_rn(__ldg(gain + 8 * i), __fdiv_rn(x[i], d));
+  const float* cs = cos_t + (size_t)pos * (kHd / 2) + j;
+  const float* sn = sin_t + (size_t)pos * (kHd / 2) + j;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float c = __ldg(cs + 8 * i), t = __ldg(sn + 8 * i), lo = x[i], hi = x[i + 8];
+    x[i] = __fsub_rn(__fmul_rn(lo, c), __fmul_rn(hi, t));
+    x[i + 8] = __fadd_rn(__fmul_rn(hi, c), __fmul_rn(lo, t));
+  }
+  if (is_q) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) q[8 * i] = x[i];
     return;
   }
-  const int g = h - a.nq;
-  warp_norm_rope(row + (size_t)h * kHd, kn, cs, sn, eps, tmp[warp], row_s[warp]);
-  const float4 k4 = reinterpret_cast<const float4*>(row_s[warp])[lane];
-  const float4 v4 = reinterpret_cast<const float4*>(row + (size_t)(h + nkv) * kHd)[lane];
-  const size_t at = (size_t)x.s * a.t_seq + g * a.t_head + (size_t)slot * kHd + 4 * lane;
-  reinterpret_cast<__half2*>(tk + at)[0] = __floats2half2_rn(k4.x, k4.y);
-  reinterpret_cast<__half2*>(tk + at)[1] = __floats2half2_rn(k4.z, k4.w);
-  reinterpret_cast<__half2*>(tv + at)[0] = __floats2half2_rn(v4.x, v4.y);
-  reinterpret_cast<__half2*>(tv + at)[1] = __floats2half2_rn(v4.z, v4.w);
+  const size_t at = (size_t)s.s * a.t_seq + (h - a.nq) * a.t_head + (size_t)slot * kHd + j;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    tk[at + 8 * i] = __float2half_rn(x[i]);
+    tv[at + 8 * i] = __float2half_rn(v[i]);
+  }
 }
 
 constexpr int kShMaxRows = 65535;      // rows and sequences of a call
@@ -904,9 +946,19 @@ int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const Sp
   const int smem = p.few ? kFwSmem : kPtSmem;
   const int rc = smem_attr(fn, smem);
   if (rc) return rc;
-  if (p.few) k_span_few<<<dim3((unsigned)ctas, nkv), 32 * kFwWarps, smem, st>>>(a, s, p.tiles);
-  else k_span_part<<<dim3((unsigned)ctas, nkv), 32 * kPtWarps, smem, st>>>(a, s, p.tiles, p.size);
-  HV_CUDA(cudaGetLastError());
+  // the tails need nothing of k_span_tile's: they may start once all its CTAs have
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)ctas, nkv);
+  cfg.blockDim = dim3(p.few ? 32 * kFwWarps : 32 * kPtWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = s.nwt ? 1 : 0;
+  if (p.few) HV_CUDA(cudaLaunchKernelEx(&cfg, k_span_few, a, s, p.tiles));
+  else HV_CUDA(cudaLaunchKernelEx(&cfg, k_span_part, a, s, p.tiles, p.size));
   return HV_OK;
 }
 int join_launch(const char* name, const SpanArgs& a, const SpanParts& s, cudaStream_t st) {
@@ -1072,8 +1124,9 @@ extern "C" int hv_qk_shared_f16(const float* qkv, const float* qn, const float* 
   a.row0 = row0; a.tlen_p = tlen; a.tcap = tcap;
   a.t_head = (size_t)tcap * kHd; a.t_seq = (size_t)nkv * a.t_head;
   a.nq = nq; a.group = 1; a.nseq = nseq; a.nrow = nrow;
-  const long long warps = (long long)(nq + nkv) * nrow;
-  k_qk_shared<<<(unsigned)((warps + 7) / 8), 256, 0, (cudaStream_t)stream>>>(
+  const long long warps = (long long)((nq + nkv + 3) / 4) * nrow;
+  HV_REQUIRE(warps < (1ll << 31), HV_E_UNSUPPORTED, "%s: %d rows of %d heads", name, nrow, nq);
+  k_qk_shared<<<(unsigned)((warps + kQkWarps - 1) / kQkWarps), 32 * kQkWarps, 0, (cudaStream_t)stream>>>(
       qkv, qn, kn, cos_t, sin_t, cap, base, a, q_out, reinterpret_cast<__half*>(tk),
       reinterpret_cast<__half*>(tv), nkv, eps);
   HV_LAUNCHED(name);

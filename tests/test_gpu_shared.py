@@ -270,6 +270,37 @@ def test_two_captured_graphs_follow_device_lengths(hv):
         hv.stream_destroy(L["st"])
 
 
+@pytest.mark.parametrize("nseq,plen", [(40, 1500), (70, 5000)])
+def test_captured_call_over_a_long_prefix(hv, nseq, plen):
+    """Several kernels in a call: replayed back to back over changing inputs."""
+    g = np.random.default_rng(plen)
+    nkv, group, tcap = 2, 4, 40
+    nq = nkv * group
+    pk, pv = cache(g, nkv, plen)
+    tk, tv = cache(g, nseq, nkv, tcap)
+    d = [Dev(x) for x in (pk, pv, tk, tv)]
+    tlen = g.integers(0, tcap + 1, nseq)
+    pl, tl, sc = i32(plen), i32(tlen), Dev(np.array([SCALE], F32))
+    q, ctx = Dev(nbytes=nseq * nq * 512), Dev(nbytes=nseq * nq * 512)
+    s = scratch(hv.attn_shared_scratch(nq, group, plen, tcap, nseq, nseq))
+    st = hv.stream_create()
+    hv.synchronize()
+    hv.capture_begin(st)
+    hv.attn_shared(q, d[0], d[1], plen, pl, d[2], d[3], tcap, 0, tl, ctx, sc, nq, HD, group, nseq, nseq, s, st)
+    gr = hv.capture_end(st)
+    ex = hv.graph_instantiate(gr)
+    for rep in range(3):
+        rows = queries(g, nseq, nq)
+        q.put(rows)
+        hv.synchronize()
+        for _ in range(1 + 5 * rep):
+            hv.graph_launch(ex, st)
+        hv.stream_synchronize(st)
+        near(ctx.get(F32, rows.shape), *R.shared(rows, pk, pv, plen, tk, tv, None, tlen, SCALE))
+    hv.graph_destroy(gr, ex)
+    hv.stream_destroy(st)
+
+
 # ---- the write of a batch's rows -------------------------------------------------------
 
 @pytest.mark.parametrize("nkv,group,rows,tails,base", [
