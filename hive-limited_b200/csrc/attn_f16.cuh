@@ -160,6 +160,26 @@ HV_DEV bool not_finite(const uint4& y) {
   return odd(y.x) || odd(y.y) || odd(y.z) || odd(y.w);
 }
 
+// Kernels of a call may start before the one before them has ended: what they read of it, or write
+// over, comes after prior_done. Each of them calls it, at its end at the latest, so that the end of
+// one is the end of all before it.
+HV_DEV void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+HV_DEV void prior_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <class... P, class... A>
+cudaError_t launch_beside(void (*fn)(P...), dim3 grid, int threads, int smem, cudaStream_t st, bool beside, A... args) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &at;
+  cfg.numAttrs = beside ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, fn, (P)args...);
+}
+
 // Partial results in the caller's scratch, in slots: nwt for the stretches of k_span_tile (at most
 // that many a tile of rows) or npc for the prefix's chunks, ntc for the tails'. part [slot][nkv][F][128], ml [slot][nkv][F]: sums and the sum of the weights 2^(x - m),
 // relative to m.

@@ -215,6 +215,7 @@ __global__ void __launch_bounds__(kMtThreads, 1)
   } else if (lane == 0) {
     int issued = 0;
     bool ok = true;
+    prior_done();                                 // the rows' terms
     while (next(x))
       for (int r = x.r0; r < rtiles && ok; ++r, ++qi) {
         const int stage = qi % kMtStages;
@@ -258,8 +259,8 @@ int mass_tile_launch(const SpanArgs& a, const SpanParts& p, const float* mass_in
   CUtensorMap mq;
   rc = f16_rows_map(p.terms, a.nrow * a.group, 2 * (a.nq / a.group), &mq);
   if (rc) return rc;
-  k_mass_tile<<<(unsigned)p.grid, kMtThreads, kMtSmem, st>>>(a, p, mass_in, mass_out, cap, mq);
-  HV_LAUNCHED("k_mass_tile");
+  HV_CUDA(launch_beside(k_mass_tile, dim3((unsigned)p.grid), kMtThreads, kMtSmem, st, true, a, p, mass_in, mass_out, cap, mq));
+  return HV_OK;
 }
 
 }  // namespace hv

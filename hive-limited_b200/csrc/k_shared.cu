@@ -14,12 +14,6 @@
 namespace hv {
 namespace {
 
-// The kernel that this one may have started beside ends before this one does, and so before whatever
-// comes next: its first CTA waits for that.
-HV_DEV void end_after_prior() {
-  if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-}
-
 // ---- attention of few rows a head ---------------------------------------------------------
 //
 // A CTA has up to 64 (row, head) pairs of a kv head and a chunk of the prefix or of a sequence's
@@ -305,8 +299,9 @@ HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles, int size
 }
 
 __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles, int size) {
+  next_may_start();
   span_part(a, p, tiles, size);
-  end_after_prior();
+  if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) prior_done();
 }
 
 // ---- attention of up to eight rows ---------------------------------------------------------
@@ -511,8 +506,9 @@ HV_DEV void span_few(const SpanArgs& a, const SpanParts& p, int tiles) {
 }
 
 __global__ void __launch_bounds__(32 * kFwWarps, 2) k_span_few(SpanArgs a, SpanParts p, int tiles) {
+  next_may_start();
   span_few(a, p, tiles);
-  end_after_prior();
+  if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) prior_done();
 }
 
 // ---- a row's chunks added up -----------------------------------------------------------------
@@ -540,6 +536,7 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
       nw = span_cta(wh, u + whole - 1) - span_cta(wh, u) + 1;
     }
   }
+  prior_done();
 #pragma unroll 1
   for (int i = warp / kWarps; i < kPer; i += 8 / kWarps) {
     const int f = fb + i;
@@ -644,6 +641,7 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
 
 template <int kWarps, int kPer>
 __global__ void __launch_bounds__(256, kWarps == 1 ? 5 : 3) k_span_join(SpanArgs a, SpanParts p) {
+  next_may_start();
   span_join<kWarps, kPer>(a, p);
 }
 
@@ -655,6 +653,7 @@ __global__ void __launch_bounds__(256) k_span_one(SpanArgs a, SpanParts p, const
   __shared__ float2 s_one[8];
   const int kvh = blockIdx.y, np = span_prefix(a), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t0 = (blockIdx.x - joins) * kOnePos + 4 * threadIdx.x;
+  prior_done();
   if (np < 0 || t0 - 4 * (int)threadIdx.x >= np) return;
   const float* scores = p.scores + (size_t)kvh * a.group * p.scores_ld + t0;
   float4 x[8];
@@ -714,7 +713,7 @@ __global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, cons
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
   const int kvh = blockIdx.y, F = a.nrow * a.group, p0 = blockIdx.x * kN;
   const int n = a.plen + a.nrow;
-  if (p0 >= n) return;
+  if (p0 >= n) return;                                      // (the others wait)
   uint8_t* ks = smem + kPtQ;
   for (int u = threadIdx.x; u < kN * 16; u += 256) {
     const int r = u >> 4, pos = p0 + r;
@@ -735,6 +734,7 @@ __global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, cons
   const int pos_a = p0 + 16 * wpos + gl, pos_b = pos_a + 8;
   const int see_a = max(0, pos_a - a.plen) * a.group, see_b = max(0, pos_b - a.plen) * a.group;
   const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(smem);
+  prior_done();
   float sum_a = 0.0f, sum_b = 0.0f;
   const int first = max(0, p0 - a.plen) * a.group / kSpanItem * kSpanItem;   // rows before see none of it
   for (int f0 = first; f0 < F; f0 += kSpanItem) {
@@ -946,41 +946,35 @@ int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const Sp
   const int smem = p.few ? kFwSmem : kPtSmem;
   const int rc = smem_attr(fn, smem);
   if (rc) return rc;
-  // the tails need nothing of k_span_tile's: they may start once all its CTAs have
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)ctas, nkv);
-  cfg.blockDim = dim3(p.few ? 32 * kFwWarps : 32 * kPtWarps);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = &at;
-  cfg.numAttrs = s.nwt ? 1 : 0;
-  if (p.few) HV_CUDA(cudaLaunchKernelEx(&cfg, k_span_few, a, s, p.tiles));
-  else HV_CUDA(cudaLaunchKernelEx(&cfg, k_span_part, a, s, p.tiles, p.size));
+  // the tails need nothing of k_span_tile's
+  const dim3 grid((unsigned)ctas, nkv);
+  if (p.few) HV_CUDA(launch_beside(k_span_few, grid, 32 * kFwWarps, smem, st, s.nwt > 0, a, s, p.tiles));
+  else HV_CUDA(launch_beside(k_span_part, grid, 32 * kPtWarps, smem, st, s.nwt > 0, a, s, p.tiles, p.size));
   return HV_OK;
 }
-int join_launch(const char* name, const SpanArgs& a, const SpanParts& s, cudaStream_t st) {
+int join_launch(const SpanArgs& a, const SpanParts& s, cudaStream_t st) {
   const unsigned nkv = (unsigned)(a.nq / a.group), F = (unsigned)(a.nrow * a.group);
   const unsigned rows = s.terms ? (F + kStRows - 1) / kStRows * kStRows : F;
   const size_t all = (size_t)rows * nkv;
-  if (s.nwt + s.npc + s.ntc > 8 && all <= 1024) k_span_join<4, 2><<<dim3((rows + 1) / 2, nkv), 256, 0, st>>>(a, s);
-  else if (all <= 8192) k_span_join<1, 8><<<dim3((rows + 7) / 8, nkv), 256, 0, st>>>(a, s);
-  else k_span_join<1, 32><<<dim3((rows + 31) / 32, nkv), 256, 0, st>>>(a, s);
-  HV_LAUNCHED(name);
+  if (s.nwt + s.npc + s.ntc > 8 && all <= 1024)
+    HV_CUDA(launch_beside(k_span_join<4, 2>, dim3((rows + 1) / 2, nkv), 256, 0, st, true, a, s));
+  else if (all <= 8192)
+    HV_CUDA(launch_beside(k_span_join<1, 8>, dim3((rows + 7) / 8, nkv), 256, 0, st, true, a, s));
+  else
+    HV_CUDA(launch_beside(k_span_join<1, 32>, dim3((rows + 31) / 32, nkv), 256, 0, st, true, a, s));
+  return HV_OK;
 }
 
 template <int kPos>
-int mass_rows_launch(const char* name, const SpanArgs& a, const SpanParts& s, const float* mass_in, float* mass_out,
+int mass_rows_launch(const SpanArgs& a, const SpanParts& s, const float* mass_in, float* mass_out,
                      int cap, cudaStream_t st) {
   constexpr int smem = kPtQ + 16 * kPos * kHd * 2;
   const int rc = smem_attr((const void*)k_mass_rows<kPos>, smem);
   if (rc) return rc;
   const unsigned n = (unsigned)(a.plen + a.nrow);
-  k_mass_rows<kPos><<<dim3((n + 16 * kPos - 1) / (16 * kPos), (unsigned)(a.nq / a.group)), 256, smem, st>>>(
-      a, s, mass_in, mass_out, cap);
-  HV_LAUNCHED(name);
+  HV_CUDA(launch_beside(k_mass_rows<kPos>, dim3((n + 16 * kPos - 1) / (16 * kPos), (unsigned)(a.nq / a.group)), 256, smem,
+                        st, true, a, s, mass_in, mass_out, cap));
+  return HV_OK;
 }
 
 int mass_any(const char* name, const SpanArgs& a, const float* mass_in, float* mass_out, int cap,
@@ -999,19 +993,19 @@ int mass_any(const char* name, const SpanArgs& a, const float* mass_in, float* m
   if (rc) return rc;
   if (one) {
     const int joins = (a.group + 1) / 2;
-    k_span_one<<<dim3((unsigned)(joins + (cap + kOnePos - 1) / kOnePos), (unsigned)nkv), 256, 0, st>>>(
-        a, s, mass_in, mass_out, joins);
-    HV_LAUNCHED(name);
+    HV_CUDA(launch_beside(k_span_one, dim3((unsigned)(joins + (cap + kOnePos - 1) / kOnePos), (unsigned)nkv), 256, 0, st,
+                          true, a, s, mass_in, mass_out, joins));
+    return HV_OK;
   }
-  rc = join_launch(name, a, s, st);
+  rc = join_launch(a, s, st);
   if (rc) return rc;
   if (p.mass_tiles) return mass_tile_launch(a, s, mass_in, mass_out, cap, st);
   // a CTA an SM, as far as the positions go
   auto ctas = [&](int pos) { return (long long)nkv * ((n + 16 * pos - 1) / (16 * pos)); };
-  if (ctas(8) >= 148) return mass_rows_launch<8>(name, a, s, mass_in, mass_out, cap, st);
-  if (ctas(4) >= 148) return mass_rows_launch<4>(name, a, s, mass_in, mass_out, cap, st);
-  if (ctas(2) >= 148) return mass_rows_launch<2>(name, a, s, mass_in, mass_out, cap, st);
-  return mass_rows_launch<1>(name, a, s, mass_in, mass_out, cap, st);
+  if (ctas(8) >= 148) return mass_rows_launch<8>(a, s, mass_in, mass_out, cap, st);
+  if (ctas(4) >= 148) return mass_rows_launch<4>(a, s, mass_in, mass_out, cap, st);
+  if (ctas(2) >= 148) return mass_rows_launch<2>(a, s, mass_in, mass_out, cap, st);
+  return mass_rows_launch<1>(a, s, mass_in, mass_out, cap, st);
 }
 
 }  // namespace
@@ -1058,7 +1052,7 @@ extern "C" int hv_attn_shared_f16(const float* q, const uint16_t* pk, const uint
   const SpanPlan p = span_plan((int)nkv, nrow * group, nseq, pcap, tcap, false, false);
   const SpanParts s = span_parts(p, scratch, pcap, false, false);
   const int rc2 = span_launch(name, a, p, s, (cudaStream_t)stream);
-  return rc2 ? rc2 : join_launch(name, a, s, (cudaStream_t)stream);
+  return rc2 ? rc2 : join_launch(a, s, (cudaStream_t)stream);
 }
 
 extern "C" int hv_attn_mass_scratch(int nq, int group, int cap, int ntok, size_t* bytes) {

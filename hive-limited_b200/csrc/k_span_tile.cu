@@ -72,7 +72,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
   StShared& sh = *reinterpret_cast<StShared*>(smem + 4 * kStTile + kStRows * kStLine * 4);
   const int warp = __shfl_sync(0xFFFFFFFFu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int F = a.nrow * a.group, nkv = a.nq / a.group;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the tails may start beside it
+  next_may_start();
   const int np = span_prefix(a);
   const SpanWhole wh = span_whole(a, np, gridDim.x);
   if ((int)blockIdx.x >= wh.ctas) return;
