@@ -60,19 +60,20 @@ HV_DEV float row_terms(const float4& x, uint2* hi, uint2* lo) {
 // terms, then their second ones; what takes a row's sums of products to exponents to `fac`.
 // A warp's rows are all loaded before the first is worked on.
 template <int kRows, int kWarps>
-HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, float* fac, int warp) {
-  const int lane = threadIdx.x & 31;
-  const float f = __ldg(a.scale) * kLog2e;
-  float4 x[kRows / kWarps];
+HV_DEV void rows_load(const SpanArgs& a, int kvh, int f0, int nf, int warp, float4 (&x)[kRows / kWarps]) {
 #pragma unroll
   for (int j = 0; j < kRows / kWarps; ++j) {
     const int i = warp + j * kWarps;
     x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (i < nf) {
       const int r = (f0 + i) / a.group, h = f0 + i - r * a.group;
-      x[j] = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + h) * kHd) + lane);
+      x[j] = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + h) * kHd) + (threadIdx.x & 31));
     }
   }
+}
+template <int kRows, int kWarps>
+HV_DEV void rows_put(const float4 (&x)[kRows / kWarps], float f, int nf, uint8_t* to, float* fac, int warp) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int j = 0; j < kRows / kWarps; ++j) {
     const int i = warp + j * kWarps;
@@ -84,6 +85,13 @@ HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, 
     *reinterpret_cast<uint2*>(to + swz(at + 8, lane >> 1) + 8 * (lane & 1)) = lo;
     if (lane == 0) fac[i] = f / lift;
   }
+}
+template <int kRows, int kWarps>
+HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, float* fac, int warp) {
+  float4 x[kRows / kWarps];
+  const float f = __ldg(a.scale) * kLog2e;
+  rows_load<kRows, kWarps>(a, kvh, f0, nf, warp, x);
+  rows_put<kRows, kWarps>(x, f, nf, to, fac, warp);
 }
 
 HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles, int size) {
@@ -734,13 +742,17 @@ __global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, cons
   const int pos_a = p0 + 16 * wpos + gl, pos_b = pos_a + 8;
   const int see_a = max(0, pos_a - a.plen) * a.group, see_b = max(0, pos_b - a.plen) * a.group;
   const uint32_t q_at = (uint32_t)__cvta_generic_to_shared(smem);
-  prior_done();
   float sum_a = 0.0f, sum_b = 0.0f;
   const int first = max(0, p0 - a.plen) * a.group / kSpanItem * kSpanItem;   // rows before see none of it
+  const float scale = __ldg(a.scale) * kLog2e;
+  float4 x[kSpanItem / 8];                                  // the next stage's rows
+  rows_load<kSpanItem, 8>(a, kvh, first, min(kSpanItem, F - first), warp, x);
+  prior_done();
   for (int f0 = first; f0 < F; f0 += kSpanItem) {
     const int nf = min(kSpanItem, F - f0);
     __syncthreads();
-    rows_split<kSpanItem, 8>(a, kvh, f0, nf, smem, s_fac, warp);
+    rows_put<kSpanItem, 8>(x, scale, nf, smem, s_fac, warp);
+    if (f0 + kSpanItem < F) rows_load<kSpanItem, 8>(a, kvh, f0 + kSpanItem, min(kSpanItem, F - f0 - kSpanItem), warp, x);
     if (threadIdx.x < nf) {
       const float2 s = p.stat[(size_t)kvh * F + f0 + threadIdx.x];
       s_stat[threadIdx.x] = make_float2(s.x, 1.0f / s.y);
