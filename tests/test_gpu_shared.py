@@ -81,7 +81,8 @@ def test_one_row_a_sequence(hv, nkv, group, plen, tails):
     (2, 4, 0, [3], [3]), (1, 2, 10, [1, 0, 5], [4, 9, 5]), (2, 8, 100, [17, 3, 0, 12], [17, 3, 4, 40]),
     (8, 4, 200, [9, 31, 33, 1], [9, 31, 64, 300]), (1, 5, 700, [40, 2, 65], [41, 2, 65]),
     (2, 3, 64, [150], [150]), (1, 8, 2000, [3, 17, 8, 8, 9, 2] * 3, [3, 20, 8, 30, 9, 2] * 3),
-    (2, 1, 300, [128, 64], [130, 64]), (1, 4, 20, [0, 0, 2], [5, 0, 2])])
+    (2, 1, 300, [128, 64], [130, 64]), (1, 4, 20, [0, 0, 2], [5, 0, 2]),
+    (2, 4, 2000, [1, 2, 3] * 10, [1, 2, 9] * 10), (1, 8, 1111, [0, 4, 1] * 9, [7, 30, 1] * 9)])
 def test_runs_of_rows(hv, nkv, group, plen, rows, tails):
     g = np.random.default_rng(plen + len(rows))
     check_shared(hv, g, nkv, group, plen, plen + 3, rows, tails, max(tails) + 1, extra=2)
@@ -120,6 +121,8 @@ def test_a_prefix_of_full_capacity_and_none_at_all(hv):
     check_shared(hv, g, 2, 4, 256, 256, [1] * 20, [8] * 20, 8, one=True)
     check_shared(hv, g, 2, 4, 0, 0, [2, 1], [2, 6], 6)
     check_shared(hv, g, 2, 2, 0, 40, [2, 1], [2, 6], 6)
+    check_shared(hv, g, 2, 4, 0, 5000, [1] * 40, [i % 5 for i in range(40)], 5, one=True)
+    check_shared(hv, g, 1, 4, 1024, 1024, [1] * 40, [5] * 40, 5, one=True)
 
 
 def test_rows_that_see_nothing_are_zero(hv):
@@ -398,13 +401,14 @@ def check_mass(hv, g, nkv, group, pos0, ntok, cap, decode, form):
 @pytest.mark.parametrize("nkv,group,n", [(1, 1, 1), (2, 4, 2), (8, 2, 31), (3, 5, 64), (2, 8, 129),
                                          (8, 4, 1000), (1, 7, 4225), (2, 3, 9001)])
 def test_decode_with_mass(hv, nkv, group, n, form):
-    check_mass(hv, np.random.default_rng(n), nkv, group, n - 1, 1, n + 3, True, form)
+    check_mass(hv, np.random.default_rng(n), nkv, group, n - 1, 1, n + 3 * (form != "apart"), True, form)
 
 
 @pytest.mark.parametrize("nkv,group,pos0,ntok", [
     (1, 1, 0, 1), (2, 4, 0, 5), (8, 2, 256, 44), (1, 8, 100, 17), (2, 5, 63, 65), (1, 3, 1000, 31),
     (2, 4, 128, 128), (1, 8, 700, 256), (2, 1, 0, 300), (1, 2, 2048, 200), (1, 7, 4000, 3),
-    (1, 1, 900, 290), (2, 5, 500, 120), (1, 3, 0, 700), (8, 8, 2100, 64), (8, 4, 1000, 200)])
+    (1, 1, 900, 290), (2, 5, 500, 120), (1, 3, 0, 700), (8, 8, 2100, 64), (8, 4, 1000, 200),
+    (8, 4, 2400, 2), (8, 4, 1200, 4), (8, 4, 600, 4), (1, 2, 0, 2500)])
 def test_run_with_mass(hv, nkv, group, pos0, ntok):
     g = np.random.default_rng(pos0 + ntok)
     check_mass(hv, g, nkv, group, pos0, ntok, pos0 + ntok + 2, False, "apart")
@@ -574,6 +578,46 @@ def test_eviction_leaves_impossible_lengths_alone(hv):
         assert left == n and (kept == -7).all()
         assert np.array_equal(ko[0, 0], k[0, 0].view(np.uint16)) and np.array_equal(bits(mo), bits(mass))
     assert run_evict(hv, k, v, mass, 50, 1, 40, 30, 5, want_kept=False)[4] == 30
+
+
+def test_offsets_past_32_bits(hv):
+    """Heads and caches more than 2^32 bytes apart: a few rows at the front of each."""
+    g = np.random.default_rng(33)
+    nkv, group, n, cap = 9, 4, 700, 1 << 21
+    head = cap * HD * 2                                     # bytes
+    big = [Dev(nbytes=nkv * head) for _ in range(2)]
+    k, v = cache(g, nkv, n)
+    for d, x in zip(big, (k, v)):
+        for h in range(nkv):
+            hv.upload(d.ptr + h * head, np.ascontiguousarray(x[h]).ctypes.data, n * HD * 2)
+    sc = Dev(np.array([SCALE], F32))
+    # one row, and a batch over it as a prefix, by tiles and without
+    q = queries(g, 1, nkv * group)
+    dq, ctx, m, pos = Dev(q), Dev(nbytes=q.nbytes), Dev(nbytes=nkv * cap * 4), i32(n - 1)
+    s = scratch(hv.attn_mass_scratch(nkv * group, group, cap, 1))
+    hv.attn_decode_mass(dq, big[0], big[1], ctx, 0, m, sc, pos, nkv * group, HD, group, cap, s)
+    want, tol, wm, mt = R.mass(q, k, v, n - 1, None, SCALE)
+    near(ctx.get(F32, q.shape), want, tol)
+    near(m.get(F32, (nkv, cap))[:, :n], wm, mt)
+    del s
+    for nseq in (2, 20):
+        tk, tv = cache(g, nseq, nkv, 3)
+        q = queries(g, nseq, nkv * group)
+        dq, ctx, dt = Dev(q), Dev(nbytes=q.nbytes), [Dev(tk), Dev(tv)]
+        s = scratch(hv.attn_shared_scratch(nkv * group, group, cap, 3, nseq, nseq))
+        pl, tl = i32(n), i32([3] * nseq)
+        hv.attn_shared(dq, big[0], big[1], cap, pl, dt[0], dt[1], 3, 0, tl, ctx, sc, nkv * group, HD, group,
+                       nseq, nseq, s)
+        near(ctx.get(F32, q.shape), *R.shared(q, k, v, n, tk, tv, None, [3] * nseq, SCALE))
+    # thinned in place
+    mass = some_mass(g, nkv, cap)
+    dm, ln, s = Dev(mass), i32(n), scratch(hv.kv_evict_scratch(nkv, cap, 1))
+    hv.kv_evict(big[0], big[1], 0, dm, cap, ln, 0, big[0], big[1], 0, dm, cap, ln, 0, 500, 300, 50, nkv, HD, 1, s)
+    hv.synchronize()
+    for h in range(nkv):
+        got = np.empty((300, HD), np.uint16)
+        hv.download(got.ctypes.data, big[1].ptr + h * head, got.nbytes)
+        assert np.array_equal(got, v[h, R.evict(mass[h], n, 500, 300, 50)].view(np.uint16))
 
 
 # ---- a run of them together ---------------------------------------------------------------
