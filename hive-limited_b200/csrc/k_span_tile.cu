@@ -56,7 +56,7 @@ HV_DEV uint64_t smem_desc_mn(uint32_t addr) {   // 128-byte swizzle, 64 halves o
 
 struct StShared {
   unsigned long long full_k[2], full_v[2], s_ready[2], w_ready[2], o_done[2];
-  unsigned long long o_free, v_clean[2], drain[2];
+  unsigned long long o_free[2], v_clean[2], drain[2];
   float top[4][kStRows];         // of the last four tiles: what their weights are relative to
   float m[2][kStRows], l[2][kStRows];
   uint32_t tmem;
@@ -89,8 +89,8 @@ __global__ void __launch_bounds__(kStThreads, 1)
       bar_init(bar(sh.o_done[i]), 1);
       bar_init(bar(sh.drain[i]), 1);
       bar_init(bar(sh.v_clean[i]), 96);
+      bar_init(bar(sh.o_free[i]), 128);
     }
-    bar_init(bar(sh.o_free), 128);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.given_up = (sm & 1023) != 0;               // the swizzle goes by addresses
   }
@@ -227,7 +227,8 @@ __global__ void __launch_bounds__(kStThreads, 1)
         const uint32_t d = tmem + kStColO;
         ok = ok && bar_wait_warp(bar(sh.full_v[s]), (i >> 1) & 1, given_up);
         ok = ok && bar_wait_warp(bar(sh.w_ready[s]), (i >> 1) & 1, given_up);
-        if (i > 0) ok = ok && bar_wait_warp(bar(sh.o_free), (i - 1) & 1, given_up);
+        // (O of the tile before, on a barrier of which this lane follows every phase)
+        if (i > 0) ok = ok && bar_wait_warp(bar(sh.o_free[1 - s]), ((i - 1) >> 1) & 1, given_up);
         if (i - g0 >= st.full) ok = ok && bar_wait_warp(bar(sh.v_clean[s]), parts >> s & 1, given_up);
         fence_after();
 #pragma unroll 1
@@ -398,7 +399,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
             tmem_ld16(o_at + 16 * (h + 1), v[(h + 1) & 1]);
           } else {
             fence_before();
-            bar_arrive(bar(sh.o_free));
+            bar_arrive(bar(sh.o_free[i & 1]));
           }
 #pragma unroll
           for (int k = 0; k < 8; ++k)
