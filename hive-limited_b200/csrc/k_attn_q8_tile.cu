@@ -81,7 +81,7 @@ constexpr uint32_t kTlDesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 2
 
 struct TlShared {
   unsigned long long full_k[2], full_v[2], s_ready[2], w_ready[2], o_done[2];
-  unsigned long long o_free, k_free, v_free, drain[2];
+  unsigned long long o_free[2], k_free, v_free, drain[2];
   float sc[4][4][4];             // of the last four tiles' blocks: s_k, log2 s_v, 1 / s_v
   int first[4][4];               // first position with a V that is not zero, where that is looked for
   float top[4][kTlRows];         // of the last four tiles: what their weights are relative to
@@ -127,8 +127,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       bar_init(bar(sh.s_ready[i]), 1);
       bar_init(bar(sh.w_ready[i]), 128);
       bar_init(bar(sh.o_done[i]), 1);
+      bar_init(bar(sh.o_free[i]), 128);
     }
-    bar_init(bar(sh.o_free), 128);
     bar_init(bar(sh.k_free), 1);
     bar_init(bar(sh.v_free), 1);
     bar_init(bar(sh.drain[0]), 1);
@@ -271,7 +271,8 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
       const uint32_t d = tmem + kTlColO;
       ok = ok && bar_wait_warp(bar(sh.full_v[s]), (i >> 1) & 1, given_up);
       ok = ok && bar_wait_warp(bar(sh.w_ready[s]), (i >> 1) & 1, given_up);
-      if (i > 0) ok = ok && bar_wait_warp(bar(sh.o_free), (i - 1) & 1, given_up);
+      // (O of the tile before, on a barrier of which this lane follows every phase)
+      if (i > 0) ok = ok && bar_wait_warp(bar(sh.o_free[1 - s]), ((i - 1) >> 1) & 1, given_up);
       fence_after();
 #pragma unroll 1
       for (int pass = 0; pass < passes && ok; ++pass) {
@@ -531,7 +532,7 @@ __global__ void __launch_bounds__(kTlThreads, 1) k_attn_tile_q8(RowsArgs a, KvQ8
           tmem_ld16(o_at + 16 * (h + 1), v[(h + 1) & 1]);
         } else {
           fence_before();
-          bar_arrive(bar(sh.o_free));
+          bar_arrive(bar(sh.o_free[i & 1]));
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k)
