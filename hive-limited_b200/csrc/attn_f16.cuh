@@ -26,8 +26,12 @@ struct SpanArgs {
   const int32_t *row0, *tlen_p;        // rows row0[s] .. row0[s + 1] - 1 are sequence s's
   int plen, pmin, pcap, tlen, tcap;    // a prefix of pmin to pcap positions
   int nq, group, nseq, nrow;
+  unsigned long long inv;              // 2^32 / group, rounded up: see span_row
   bool run;
 };
+// The row of pair f: f / group, exact for f under 2^29 (a division takes some thirty instructions,
+// several of them in every kernel before its first load).
+HV_DEV int span_row(const SpanArgs& a, int f) { return (int)(((unsigned long long)(unsigned)f * a.inv) >> 32); }
 
 // Positions of the prefix; -1 if it cannot have that many.
 HV_DEV int span_prefix(const SpanArgs& a) {
@@ -94,7 +98,7 @@ HV_DEV SpanItem span_item(const SpanArgs& a, int b, int size) {
     it.f0 = it.x.row * a.group;
   } else {
     const int w = (b - a.nseq) * size;
-    if (!span_find(a, w / a.group, &it.x)) return it;
+    if (!span_find(a, span_row(a, w), &it.x)) return it;
     const int start = it.x.row * a.group;
     const int k = (w - start + size - 1) / size;
     it.f0 = start + k * size;
@@ -108,7 +112,7 @@ HV_DEV SpanItem span_item(const SpanArgs& a, int b, int size) {
 // Positions of a chunk when n are cut into at most `most` chunks of whole stages.
 constexpr int kSpanStage = 64;
 HV_HD int span_chunk(int n, int most) {
-  const int c = (n + most - 1) / most;
+  const int c = most == 1 ? n : (n + most - 1) / most;
   return (c + kSpanStage - 1) / kSpanStage * kSpanStage;
 }
 
@@ -123,7 +127,7 @@ struct SpanWhole {
 };
 // Positions of the prefix (or cache) that pair f sees.
 HV_DEV int span_sees(const SpanArgs& a, int np, int f) {
-  return np < 0 ? 0 : a.run ? np + f / a.group + 1 : np;
+  return np < 0 ? 0 : a.run ? np + span_row(a, f) + 1 : np;
 }
 HV_DEV int span_tiles_of(const SpanArgs& a, int np, int tile) {
   const int last = min(a.nrow * a.group, (tile + 1) * kStRows) - 1;
@@ -186,6 +190,7 @@ cudaError_t launch_beside(void (*fn)(P...), dim3 grid, int threads, int smem, cu
 struct SpanParts {
   float* part;
   float2* ml;
+  int32_t* stretches;                  // [nkv][tiles of rows]: the slots that k_span_tile has used
   float2* stat;                        // [nkv][F]: m and the sum of all, for the weights' sake
   float* scores;                       // [nq][scores_ld], of a single row
   size_t scores_ld;

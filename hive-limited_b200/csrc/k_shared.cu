@@ -66,7 +66,7 @@ HV_DEV void rows_load(const SpanArgs& a, int kvh, int f0, int nf, int warp, floa
     const int i = warp + j * kWarps;
     x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (i < nf) {
-      const int r = (f0 + i) / a.group, h = f0 + i - r * a.group;
+      const int r = span_row(a, f0 + i), h = f0 + i - r * a.group;
       x[j] = __ldg(reinterpret_cast<const float4*>(a.q + ((size_t)r * a.nq + (size_t)kvh * a.group + h) * kHd) + (threadIdx.x & 31));
     }
   }
@@ -116,7 +116,7 @@ HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles, int size
     slot = p.nwt + chunk;
     k = a.pk + kvh * a.p_head;
     v = a.pv + kvh * a.p_head;
-    lim_all = a.run ? min(p1, a.plen + f0 / a.group + 1) : p1;
+    lim_all = a.run ? min(p1, a.plen + span_row(a, f0) + 1) : p1;
   } else {
     const int b = blockIdx.x - tiles * p.npc, chunk = b % p.ntc;
     const SpanItem it = span_item(a, b / p.ntc, size);
@@ -126,12 +126,12 @@ HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles, int size
     nf = it.nf;
     const int len = span_chunk(x.len, p.ntc);
     p0 = chunk * len;
-    p1 = min(x.sees((f0 + nf - 1) / a.group), p0 + len);
+    p1 = min(x.sees(span_row(a, f0 + nf - 1)), p0 + len);
     if (p0 >= p1) return;
     slot = p.nwt + p.npc + chunk;
     k = a.tk + (size_t)x.s * a.t_seq + kvh * a.t_head;
     v = a.tv + (size_t)x.s * a.t_seq + kvh * a.t_head;
-    lim_all = min(p1, x.sees(f0 / a.group));
+    lim_all = min(p1, x.sees(span_row(a, f0)));
   }
   const int ns = (p1 - p0 + kSpanStage - 1) / kSpanStage;
   const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem), kv_s = sm + kPtQ;
@@ -161,7 +161,7 @@ HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles, int size
   const bool mine = o < oct;
   const int fr = f0 + 8 * o + gl;                          // this thread's row
   const bool row_live = mine && fr < f0 + nf;
-  const int lim = !row_live ? 0 : a.run ? min(p1, a.plen + fr / a.group + 1) : prefix ? p1 : min(p1, x.sees(fr / a.group));
+  const int lim = !row_live ? 0 : a.run ? min(p1, a.plen + span_row(a, fr) + 1) : prefix ? p1 : min(p1, x.sees(span_row(a, fr)));
   float m = -INFINITY, l = 0.0f;
   float acc[16][4];
 #pragma unroll
@@ -350,11 +350,11 @@ HV_DEV void span_few(const SpanArgs& a, const SpanParts& p, int tiles) {
     nf = it.nf;
     const int len = span_chunk(x.len, p.ntc);
     p0 = chunk * len;
-    p1 = min(x.sees((f0 + nf - 1) / a.group), p0 + len);
+    p1 = min(x.sees(span_row(a, f0 + nf - 1)), p0 + len);
     slot = p.nwt + p.npc + chunk;
     k = a.tk + (size_t)x.s * a.t_seq + kvh * a.t_head;
     v = a.tv + (size_t)x.s * a.t_seq + kvh * a.t_head;
-    lim_all = min(p1, x.sees(f0 / a.group));
+    lim_all = min(p1, x.sees(span_row(a, f0)));
   }
   if (p0 >= p1) return;
   const int nb = (p1 - p0 + kFwBlock - 1) / kFwBlock;
@@ -381,7 +381,7 @@ HV_DEV void span_few(const SpanArgs& a, const SpanParts& p, int tiles) {
   __syncthreads();
   const int fr = f0 + gl;
   const bool row_live = gl < nf;
-  const int lim = !row_live ? 0 : a.run ? min(p1, a.plen + fr / a.group + 1) : prefix ? p1 : min(p1, x.sees(fr / a.group));
+  const int lim = !row_live ? 0 : a.run ? min(p1, a.plen + span_row(a, fr) + 1) : prefix ? p1 : min(p1, x.sees(span_row(a, fr)));
   const float fac = row_live ? s_fac[gl] : 0.0f;
   uint32_t qa[8][4];
 #pragma unroll
@@ -534,17 +534,11 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
   const int np = span_prefix(a);
   const size_t step = (size_t)gridDim.y * F;
   const float nan = __int_as_float(0x7fc00000);
-  // its stretches of whole tiles
-  int nw = 0;
-  if (p.nwt && fb < F) {
-    const SpanWhole wh = span_whole(a, np, p.grid);
-    const int tile = fb / kStRows, whole = span_tiles_of(a, np, tile);
-    if (whole) {
-      const unsigned u = ((unsigned)kvh * wh.rows + tile) * wh.tiles;
-      nw = span_cta(wh, u + whole - 1) - span_cta(wh, u) + 1;
-    }
-  }
   prior_done();
+  // its stretches of tiles
+  int nw = 0;
+  if (p.nwt && fb < F && span_tiles_of(a, np, fb / kStRows))
+    nw = p.stretches[kvh * ((F + kStRows - 1) / kStRows) + fb / kStRows];
 #pragma unroll 1
   for (int i = warp / kWarps; i < kPer; i += 8 / kWarps) {
     const int f = fb + i;
@@ -553,7 +547,7 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
       if (p.terms && f < Fp && lane < 2) p.facs[((size_t)lane * gridDim.y + kvh) * Fp + f] = lane ? -INFINITY : 0.0f;
       if (kWarps == 1) continue;
     }
-    const int r = f / a.group;
+    const int r = span_row(a, f);
     SpanSeq x;
     const bool here = f < F && span_find(a, r, &x);        // the same for the row's warps
     if (kWarps == 1 && !here) continue;
@@ -567,7 +561,7 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
     }
     if (here && !no && p.ntc) {
       const int see = x.sees(r);
-      if (see) n1 = (see + span_chunk(x.len, p.ntc) - 1) / span_chunk(x.len, p.ntc);
+      if (see) n1 = p.ntc == 1 ? 1 : (see + span_chunk(x.len, p.ntc) - 1) / span_chunk(x.len, p.ntc);
     }
     const int all = here && !no ? nw + n0 + n1 : 0;
     auto slot = [&](int k) {
@@ -875,6 +869,10 @@ int span_check(const char* name, int nq, int hd, int group, int nseq, int nrow) 
              "%s: %d rows of %d sequences at once", name, nrow, nseq);
   return HV_OK;
 }
+void span_group(SpanArgs* a, int group) {
+  a->group = group;
+  a->inv = ((1ull << 32) + group - 1) / group;
+}
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // How a call's positions are cut, by its capacities (the lengths are on the device): as many
@@ -882,7 +880,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int kSms = 148, kPtCtas = 2 * kSms;
 struct SpanPlan {
   int size, tiles, items, nwt, npc, ntc;   // tiles of the prefix's rows, items of the tails'
-  size_t part, ml, stat, scores, terms, facs, bytes;
+  size_t part, ml, stretches, stat, scores, terms, facs, bytes;
   bool mass_tiles, few;
 };
 SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool mass) {
@@ -919,11 +917,12 @@ SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool 
   auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
   p.part = up(rows * kHd * 4);
   p.ml = up(rows * 8);
+  p.stretches = up((size_t)nkv * ((F + kStRows - 1) / kStRows) * 4);
   p.stat = up(mass ? (size_t)nkv * F * 8 : 0);
   p.scores = up(mass ? (size_t)nkv * 8 * (pcap + 4) * 4 : 0);
   p.terms = up(mass ? 2 * all * kHd * 2 : 0);
   p.facs = up(mass ? 2 * (size_t)nkv * (F + kStRows) * 4 : 0);
-  p.bytes = p.part + p.ml + p.stat + p.scores + p.terms + p.facs + 256;
+  p.bytes = p.part + p.ml + p.stretches + p.stat + p.scores + p.terms + p.facs + 256;
   return p;
 }
 SpanParts span_parts(const SpanPlan& p, void* scratch, int pcap, bool mass, bool scores) {
@@ -931,11 +930,15 @@ SpanParts span_parts(const SpanPlan& p, void* scratch, int pcap, bool mass, bool
   SpanParts s{};
   s.part = reinterpret_cast<float*>(at);
   s.ml = reinterpret_cast<float2*>(at + p.part);
-  s.stat = mass ? reinterpret_cast<float2*>(at + p.part + p.ml) : nullptr;
-  s.scores = scores ? reinterpret_cast<float*>(at + p.part + p.ml + p.stat) : nullptr;
-  uint8_t* rows = at + p.part + p.ml + p.stat + p.scores;
-  s.terms = p.mass_tiles ? reinterpret_cast<__half*>(rows) : nullptr;
-  s.facs = reinterpret_cast<float*>(rows + p.terms);
+  at += p.part + p.ml;
+  s.stretches = reinterpret_cast<int32_t*>(at);
+  at += p.stretches;
+  s.stat = mass ? reinterpret_cast<float2*>(at) : nullptr;
+  at += p.stat;
+  s.scores = scores ? reinterpret_cast<float*>(at) : nullptr;
+  at += p.scores;
+  s.terms = p.mass_tiles ? reinterpret_cast<__half*>(at) : nullptr;
+  s.facs = reinterpret_cast<float*>(at + p.terms);
   s.nwt = p.nwt;
   s.npc = p.npc;
   s.ntc = p.ntc;
@@ -1060,7 +1063,8 @@ extern "C" int hv_attn_shared_f16(const float* q, const uint16_t* pk, const uint
   a.p_head = (size_t)pcap * kHd; a.t_head = (size_t)tcap * kHd; a.t_seq = nkv * a.t_head;
   a.plen_p = pcap ? plen : nullptr; a.row0 = row0; a.tlen_p = tlen;
   a.pcap = pcap; a.tcap = tcap;
-  a.nq = nq; a.group = group; a.nseq = nseq; a.nrow = nrow;
+  a.nq = nq; a.nseq = nseq; a.nrow = nrow;
+  span_group(&a, group);
   const SpanPlan p = span_plan((int)nkv, nrow * group, nseq, pcap, tcap, false, false);
   const SpanParts s = span_parts(p, scratch, pcap, false, false);
   const int rc2 = span_launch(name, a, p, s, (cudaStream_t)stream);
@@ -1089,7 +1093,8 @@ extern "C" int hv_attn_decode_mass_f16(const float* q, const uint16_t* kc, const
   a.pk = reinterpret_cast<const __half*>(kc); a.pv = reinterpret_cast<const __half*>(vc);
   a.p_head = (size_t)cap * kHd;
   a.plen_p = pos; a.plen = a.pmin = 1; a.pcap = cap;
-  a.nq = nq; a.group = group; a.nseq = a.nrow = 1;
+  a.nq = nq; a.nseq = a.nrow = 1;
+  span_group(&a, group);
   return mass_any(name, a, mass_in, mass_out, cap, scratch, (cudaStream_t)stream);
 }
 
@@ -1108,7 +1113,8 @@ extern "C" int hv_attn_rows_mass_f16(const float* q, const uint16_t* kc, const u
   a.p_head = (size_t)cap * kHd;
   a.plen = pos0; a.pcap = cap;
   a.run = true;
-  a.nq = nq; a.group = group; a.nseq = 1; a.nrow = ntok;
+  a.nq = nq; a.nseq = 1; a.nrow = ntok;
+  span_group(&a, group);
   return mass_any(name, a, mass_in, mass_out, cap, scratch, (cudaStream_t)stream);
 }
 
@@ -1129,7 +1135,8 @@ extern "C" int hv_qk_shared_f16(const float* qkv, const float* qn, const float* 
   SpanArgs a{};
   a.row0 = row0; a.tlen_p = tlen; a.tcap = tcap;
   a.t_head = (size_t)tcap * kHd; a.t_seq = (size_t)nkv * a.t_head;
-  a.nq = nq; a.group = 1; a.nseq = nseq; a.nrow = nrow;
+  a.nq = nq; a.nseq = nseq; a.nrow = nrow;
+  span_group(&a, 1);
   const long long warps = (long long)((nq + nkv + 3) / 4) * nrow;
   HV_REQUIRE(warps < (1ll << 31), HV_E_UNSUPPORTED, "%s: %d rows of %d heads", name, nrow, nq);
   k_qk_shared<<<(unsigned)((warps + kQkWarps - 1) / kQkWarps), 32 * kQkWarps, 0, (cudaStream_t)stream>>>(

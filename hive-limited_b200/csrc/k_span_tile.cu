@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
     unsigned u;
     int kvh, row0, j0, nt;
     int full, end;                                // its tiles that all rows see whole, positions
+    int last;                                     // with the last of its rows' tiles: their slots
     size_t part_row;
   };
   auto next = [&](Stretch& s) {
@@ -122,12 +123,14 @@ __global__ void __launch_bounds__(kStThreads, 1)
       s.j0 = (int)(s.u - R * wh.tiles);
       const int some = min(wh.tiles - s.j0, (int)(u1 - s.u));
       s.u += some;
-      s.nt = min(span_tiles_of(a, np, tile) - s.j0, some);
+      const int tiles = span_tiles_of(a, np, tile);
+      s.nt = min(tiles - s.j0, some);
       if (s.nt <= 0) continue;
       s.row0 = tile * kStRows;
       s.full = min(max(span_sees(a, np, s.row0) / kStRows - s.j0, 0), s.nt);
       s.end = span_sees(a, np, min(F, s.row0 + kStRows) - 1) - s.j0 * kStRows;
       const int slot = blockIdx.x - span_cta(wh, R * wh.tiles);
+      s.last = s.j0 + s.nt == tiles ? slot + 1 : 0;
       s.part_row = ((size_t)slot * nkv + s.kvh) * F + s.row0;
       return true;
     }
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
       // scale's sign.
       float qs;
       {
-        const int gr = min(st.row0 + row, F - 1), tok = gr / a.group;
+        const int gr = min(st.row0 + row, F - 1), tok = span_row(a, gr);
         const float4* src = reinterpret_cast<const float4*>(
             a.q + ((size_t)tok * a.nq + (size_t)st.kvh * a.group + gr - tok * a.group) * kHd) + (kHd / 8) * w;
         float4 x[kHd / 8];
@@ -421,6 +424,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
         const float2 x = unpair(acc[d]), y = unpair(acc[d + 1]);
         *reinterpret_cast<float4*>(line + 2 * d) = make_float4(x.x, x.y, y.x, y.y);
       }
+      if (st.last && row == 0) p.stretches[st.kvh * wh.rows + st.row0 / kStRows] = st.last;
       if (st.row0 + row < F) p.ml[st.part_row + row] = make_float2(M - (float)kStLift, L);
       rows_out();
     }
