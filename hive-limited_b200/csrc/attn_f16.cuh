@@ -142,7 +142,11 @@ HV_DEV SpanWhole span_whole(const SpanArgs& a, int np, int grid) {
   const unsigned all = (unsigned)(a.nq / a.group) * w.rows;
   w.units = all * w.tiles;                       // under 2^31: see span_plan
   w.ctas = (int)min((unsigned)grid, w.units);
-  const unsigned each = min((unsigned)grid / all, (unsigned)w.tiles);
+  unsigned each = min((unsigned)grid / all, (unsigned)w.tiles);
+  if (each > 0) {                                // no more than make the longest share shorter
+    const unsigned most = (w.tiles + each - 1) / each;
+    each = (w.tiles + most - 1) / most;
+  }
   if (each > 0 && (w.tiles + each - 1) / each <= w.units / grid + 3) w.ctas = (int)(all * each);
   return w;
 }

@@ -316,13 +316,18 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
 //
 // One item of eight (row, head) pairs and a chunk of positions a CTA, as for k_span_part, but every
 // warp has all rows, takes 16 positions in turn with the others and has a ring of its own for them,
-// so that no warp waits for another before the end. Bound by the bytes of the cache.
-constexpr int kFwWarps = 4, kFwStages = 3, kFwBlock = 16;
+// so that no warp waits for another before the end. Bound by the bytes of the cache. Short tails of
+// many rows have one warp a CTA: an item is then over in a few steps of 16 positions, and eleven
+// of them fit an SM.
+constexpr int kFwBlock = 16;
 constexpr int kFwTile = kFwBlock * kHd * 2;              // bytes of K or of V of 16 positions
 constexpr int kFwQ = 2 * kFewRows * kHd * 2;
-constexpr int kFwSmem = kFwQ + kFwWarps * kFwStages * 2 * kFwTile;
+constexpr int few_stages(int warps) { return warps == 4 ? 3 : 2; }
+constexpr int few_smem(int warps) { return kFwQ + warps * few_stages(warps) * 2 * kFwTile; }
 
+template <int kFwWarps>
 HV_DEV void span_few(const SpanArgs& a, const SpanParts& p, int tiles) {
+  constexpr int kFwStages = few_stages(kFwWarps);
   extern __shared__ __align__(1024) uint8_t smem[];         // the rows, then the warps' rings
   __shared__ float s_fac[kFewRows], s_m[kFwWarps][8], s_l[kFwWarps][8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane >> 2, t = lane & 3;
@@ -513,9 +518,10 @@ HV_DEV void span_few(const SpanArgs& a, const SpanParts& p, int tiles) {
   }
 }
 
-__global__ void __launch_bounds__(32 * kFwWarps, 2) k_span_few(SpanArgs a, SpanParts p, int tiles) {
+template <int kFwWarps>
+__global__ void __launch_bounds__(32 * kFwWarps, kFwWarps == 1 ? 11 : kFwWarps == 2 ? 6 : 2) k_span_few(SpanArgs a, SpanParts p, int tiles) {
   next_may_start();
-  span_few(a, p, tiles);
+  span_few<kFwWarps>(a, p, tiles);
   if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) prior_done();
 }
 
@@ -534,13 +540,16 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
   const int np = span_prefix(a);
   const size_t step = (size_t)gridDim.y * F;
   const float nan = __int_as_float(0x7fc00000);
+  SpanSeq x;
+  auto find = [&](int i) { return fb + i < F && span_find(a, span_row(a, fb + i), &x); };
+  bool here = find(warp / kWarps);                         // the same for the row's warps
   prior_done();
   // its stretches of tiles
   int nw = 0;
   if (p.nwt && fb < F && span_tiles_of(a, np, fb / kStRows))
     nw = p.stretches[kvh * ((F + kStRows - 1) / kStRows) + fb / kStRows];
 #pragma unroll 1
-  for (int i = warp / kWarps; i < kPer; i += 8 / kWarps) {
+  for (int i = warp / kWarps; i < kPer; i += 8 / kWarps, here = kPer > 8 / kWarps && i < kPer && find(i)) {
     const int f = fb + i;
     if (f >= F) {
       const int Fp = (F + kStRows - 1) / kStRows * kStRows;
@@ -548,8 +557,6 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
       if (kWarps == 1) continue;
     }
     const int r = span_row(a, f);
-    SpanSeq x;
-    const bool here = f < F && span_find(a, r, &x);        // the same for the row's warps
     if (kWarps == 1 && !here) continue;
     const size_t at = (size_t)kvh * F + f;
     const bool no = here && (np < 0 || x.len < 0);
@@ -642,7 +649,7 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
 }
 
 template <int kWarps, int kPer>
-__global__ void __launch_bounds__(256, kWarps == 1 ? 5 : 3) k_span_join(SpanArgs a, SpanParts p) {
+__global__ void __launch_bounds__(256, kWarps == 1 ? 4 : 3) k_span_join(SpanArgs a, SpanParts p) {
   next_may_start();
   span_join<kWarps, kPer>(a, p);
 }
@@ -881,7 +888,8 @@ constexpr int kSms = 148, kPtCtas = 2 * kSms;
 struct SpanPlan {
   int size, tiles, items, nwt, npc, ntc;   // tiles of the prefix's rows, items of the tails'
   size_t part, ml, stretches, stat, scores, terms, facs, bytes;
-  bool mass_tiles, few;
+  bool mass_tiles;
+  int few;                                 // warps of k_span_few, or 0: k_span_part
 };
 SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool mass) {
   SpanPlan p{};
@@ -892,10 +900,20 @@ SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool 
     if (rows * ((pcap + kStRows - 1) / kStRows) < 1ll << 31)
       p.nwt = (int)std::min((long long)((pcap + kStRows - 1) / kStRows), kSms / rows + 2);
   }
-  // eights of rows where the prefix has no more, or is k_span_tile's and the tails' rows are few;
-  // else as many of them a CTA as leave one for every SM: a product of the f16 pipe takes 16 cycles
-  // of a quarter of an SM, so that 64 rows by 64 positions are 2.5 us of one CTA's time
-  p.few = F <= kFewRows || (!run && p.nwt && F / nseq <= 2 * kFewRows);
+  // Eights of rows where there are no more, or where only tails are left. Four warps share an item's
+  // positions as long as all items find room at once: an item is over sooner then. Else short tails
+  // have as many warps an item as there is work for (256 sequences of one row, tails up to 250,
+  // group 4: 97 us with four, 84 with two; tails up to 20: 65 and, with one warp, 50; ragged runs of 24
+  // after 2000: 39 by k_span_part, 36.7), and long ones as long as rows are few (24 runs of 3 to 17
+  // rows, tails of 1000, group 4: 109 by k_span_part, 90 by fours; group 8: 145 and 153).
+  const bool tails = !run && p.nwt;
+  const bool many = (long long)nkv * std::max(nseq, F / kFewRows) > kPtCtas;
+  if (F <= kFewRows || (tails && !many)) p.few = 4;
+  else if (tails && tcap <= 256) p.few = tcap <= 32 ? 1 : 2;
+  else if (tails && (F / nseq <= 2 * kFewRows ||
+                     (F / nseq <= 64 && (long long)nkv * (F / kFewRows + nseq) <= 8 * kSms))) p.few = 4;
+  // All others as many rows a CTA as leave one for every SM: a product of the f16 pipe takes 16
+  // cycles of a quarter of an SM, so that 64 rows by 64 positions are 2.5 us of one CTA's time
   p.size = kFewRows;
   if (!p.few) {
     p.size = kSpanItem;
@@ -957,13 +975,18 @@ int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const Sp
   const long long ctas = (long long)p.tiles * p.npc + (long long)p.items * p.ntc;
   if (ctas == 0) return HV_OK;                              // a run that k_span_tile has all of
   HV_REQUIRE(ctas < (1ll << 31), HV_E_UNSUPPORTED, "%s: too many rows", name);
-  const void* fn = p.few ? (const void*)k_span_few : (const void*)k_span_part;
-  const int smem = p.few ? kFwSmem : kPtSmem;
+  const void* fn = p.few == 4   ? (const void*)k_span_few<4>
+                   : p.few == 2 ? (const void*)k_span_few<2>
+                   : p.few == 1 ? (const void*)k_span_few<1>
+                                : (const void*)k_span_part;
+  const int smem = p.few ? few_smem(p.few) : kPtSmem;
   const int rc = smem_attr(fn, smem);
   if (rc) return rc;
   // the tails need nothing of k_span_tile's
   const dim3 grid((unsigned)ctas, nkv);
-  if (p.few) HV_CUDA(launch_beside(k_span_few, grid, 32 * kFwWarps, smem, st, s.nwt > 0, a, s, p.tiles));
+  if (p.few == 4) HV_CUDA(launch_beside(k_span_few<4>, grid, 128, smem, st, s.nwt > 0, a, s, p.tiles));
+  else if (p.few == 2) HV_CUDA(launch_beside(k_span_few<2>, grid, 64, smem, st, s.nwt > 0, a, s, p.tiles));
+  else if (p.few == 1) HV_CUDA(launch_beside(k_span_few<1>, grid, 32, smem, st, s.nwt > 0, a, s, p.tiles));
   else HV_CUDA(launch_beside(k_span_part, grid, 32 * kPtWarps, smem, st, s.nwt > 0, a, s, p.tiles, p.size));
   return HV_OK;
 }

@@ -74,10 +74,6 @@ __global__ void __launch_bounds__(kStThreads, 1)
   const int F = a.nrow * a.group, nkv = a.nq / a.group;
   next_may_start();
   const int np = span_prefix(a);
-  const SpanWhole wh = span_whole(a, np, gridDim.x);
-  if ((int)blockIdx.x >= wh.ctas) return;
-  const unsigned u0 = span_first(wh, blockIdx.x), u1 = span_first(wh, blockIdx.x + 1);
-
   const uint32_t sm = (uint32_t)__cvta_generic_to_shared(smem);
   auto bar = [](const unsigned long long& b) { return (uint32_t)__cvta_generic_to_shared(&b); };
   if (threadIdx.x == 0) {
@@ -99,6 +95,9 @@ __global__ void __launch_bounds__(kStThreads, 1)
                  :: "r"((uint32_t)__cvta_generic_to_shared(&sh.tmem)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
+  const SpanWhole wh = span_whole(a, np, gridDim.x);         // (its loads take as long as what is above)
+  const bool some = (int)blockIdx.x < wh.ctas;
+  const unsigned u0 = some ? span_first(wh, blockIdx.x) : 0, u1 = some ? span_first(wh, blockIdx.x + 1) : 0;
   fence_before();
   __syncthreads();
   fence_after();
@@ -163,25 +162,32 @@ __global__ void __launch_bounds__(kStThreads, 1)
     int drains = 0;
 #pragma unroll 1
     for (; next(st); step_on(), stretch_end()) {
-      // The queries in two terms: a row's two threads have half of its dims each. They take the
-      // scale's sign.
+      // The queries in two terms. A warp loads whole rows (a thread its own row's half: 32 rows an
+      // instruction, 4 us), and through shared memory a row's two threads get half of its dims
+      // each. They take the scale's sign.
       float qs;
       {
-        const int gr = min(st.row0 + row, F - 1), tok = span_row(a, gr);
-        const float4* src = reinterpret_cast<const float4*>(
-            a.q + ((size_t)tok * a.nq + (size_t)st.kvh * a.group + gr - tok * a.group) * kHd) + (kHd / 8) * w;
-        float4 x[kHd / 8];
+        float4 x[kStRows / 8];
 #pragma unroll
-        for (int d = 0; d < kHd / 8; ++d) x[d] = __ldg(src + d);
+        for (int j = 0; j < kStRows / 8; ++j) {
+          const int gr = min(st.row0 + warp + 8 * j, F - 1), tok = span_row(a, gr);
+          x[j] = __ldg(reinterpret_cast<const float4*>(
+              a.q + ((size_t)tok * a.nq + (size_t)st.kvh * a.group + gr - tok * a.group) * kHd) + lane);
+        }
         const float qscale = __ldg(a.scale) * kLog2e;
-        float amax = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kStRows / 8; ++j) {
+          const float big = fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w)));
+          const unsigned u = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(big));
+          if (lane == 0) sh.m[0][warp + 8 * j] = __uint_as_float(u);
+          *reinterpret_cast<float4*>(lines + (size_t)(warp + 8 * j) * kStLine + 4 * lane) = x[j];
+        }
+        asm volatile("bar.sync 5, 288;" ::: "memory");     // with the warp that copies V
+        static_assert(kStRows == kHd, "x");
 #pragma unroll
         for (int d = 0; d < kHd / 8; ++d)
-          amax = fmaxf(fmaxf(amax, fmaxf(fabsf(x[d].x), fabsf(x[d].y))), fmaxf(fabsf(x[d].z), fabsf(x[d].w)));
-        sh.m[w][row] = amax;
-        rows_sync();
-        amax = fmaxf(amax, sh.m[1 - w][row]);
-        const float lift = copysignf(q8_lift(amax), qscale);
+          x[d] = *reinterpret_cast<const float4*>(lines + (size_t)row * kStLine + 64 * w + 4 * d);
+        const float lift = copysignf(q8_lift(sh.m[0][row]), qscale);
         qs = qscale / lift;
         qs = qs == 0.0f ? 2e-38f : qs;             // -infinity times it is to stay that
         const uint32_t to = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kStColQ + 32 * w;
@@ -468,6 +474,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
         continue;
       }
       if (warp == 13) {
+        asm volatile("bar.sync 5, 288;" ::: "memory");     // the queries come before V
         bool live = true;
         int issued = g0;
 #pragma unroll 1

@@ -116,6 +116,42 @@ def test_scores_that_change_along_the_prefix(hv, nseq, way):
     near(got, *R.shared(q, pk, pv, plen, tk, tv, None, [4] * nseq, SCALE))
 
 
+@pytest.mark.parametrize("nkv,group,rows,longest", [
+    (8, 1, [1] * 40, 31), (8, 4, [2, 9, 17] * 6, 30), (8, 8, [16, 0, 3, 5] * 5, 30), (2, 4, [40, 33, 65] * 3, 66),
+    (8, 3, [5, 6, 1] * 12, 120), (8, 8, [7, 2] * 20, 250), (4, 2, [1] * 100, 257), (8, 4, [3, 12] * 9, 400),
+    (8, 8, [30, 2] * 12, 300), (1, 7, [8] * 5, 1100)])
+def test_tails_of_many_rows_after_a_long_prefix(hv, nkv, group, rows, longest):
+    """Tails from the shortest to the longest in one call, their chunks ending inside a block."""
+    g = np.random.default_rng(longest + group)
+    tails = [max(r, min(longest, 1 + (i * 37) % longest)) for i, r in enumerate(rows)]
+    tails[-1] = longest
+    plen = -(-2 ** 17 // (group * (sum(rows) + 3)))       # just enough for tiles
+    check_shared(hv, g, nkv, group, plen, plen, rows, tails, longest + 1, extra=3)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("bad", [np.nan, -np.inf])
+@pytest.mark.parametrize("longest", [30, 200, 300])
+def test_tails_of_many_rows_and_what_is_not_finite(hv, which, bad, longest):
+    """As below, for sequences of many rows after a prefix of whole tiles."""
+    g = np.random.default_rng(longest)
+    nseq, n = 24, 20
+    plen = -(-2 ** 17 // (2 * nseq * n))
+    pk, pv = cache(g, 8, plen)
+    tk, tv = cache(g, nseq, 8, longest)
+    q = queries(g, nseq * n, 16)
+    row0, tails = np.arange(nseq + 1) * n, [longest - s % 3 for s in range(nseq)]
+    want, tol = R.shared(q, pk, pv, plen, tk, tv, row0, tails, SCALE)
+    at = tails[5] - n + 11                                # row 11 of sequence 5 is the first to see it
+    (tk if which == "k" else tv)[5, 3, at, :] = bad
+    got = run_shared(hv, q, pk, pv, plen, tk, tv, row0, tails)
+    hit = np.zeros((nseq * n, 16), bool)
+    hit[5 * n + 11:6 * n, 6:8] = True
+    near(got[~hit], want[~hit], tol[~hit])
+    if which == "v" or np.isnan(bad):
+        assert not np.isfinite(got[hit]).all(-1).any()
+
+
 def test_a_prefix_of_full_capacity_and_none_at_all(hv):
     g = np.random.default_rng(5)
     check_shared(hv, g, 2, 4, 256, 256, [1] * 20, [8] * 20, 8, one=True)
