@@ -94,7 +94,7 @@ HV_DEV void rows_split(const SpanArgs& a, int kvh, int f0, int nf, uint8_t* to, 
   rows_put<kRows, kWarps>(x, f, nf, to, fac, warp);
 }
 
-HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles, int size) {
+HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles) {
   extern __shared__ __align__(1024) uint8_t smem[];         // the rows, then stages of K and V
   __shared__ float s_fac[kSpanItem], s_m[kPtWarps][8], s_l[kPtWarps][8];
   __shared__ int s_bad[kSpanStage];
@@ -107,19 +107,19 @@ HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles, int size
   const bool prefix = blockIdx.x < (unsigned)(tiles * p.npc);
   if (prefix) {
     const int tile = blockIdx.x / p.npc, chunk = blockIdx.x % p.npc;
-    f0 = tile * size;
-    nf = min(size, F - f0);
-    const int n = span_sees(a, span_prefix(a), f0 + nf - 1), len = span_chunk(n, p.npc);
+    f0 = tile * kSpanItem;
+    nf = min(kSpanItem, F - f0);
+    const int n = max(span_prefix(a), 0), len = span_chunk(n, p.npc);
     p0 = chunk * len;
     p1 = min(n, p0 + len);
     if (p0 >= p1) return;
     slot = p.nwt + chunk;
     k = a.pk + kvh * a.p_head;
     v = a.pv + kvh * a.p_head;
-    lim_all = a.run ? min(p1, a.plen + span_row(a, f0) + 1) : p1;
+    lim_all = p1;
   } else {
     const int b = blockIdx.x - tiles * p.npc, chunk = b % p.ntc;
-    const SpanItem it = span_item(a, b / p.ntc, size);
+    const SpanItem it = span_item(a, b / p.ntc, kSpanItem);
     if (it.nf == 0 || it.x.len <= 0) return;
     x = it.x;
     f0 = it.f0;
@@ -161,7 +161,7 @@ HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles, int size
   const bool mine = o < oct;
   const int fr = f0 + 8 * o + gl;                          // this thread's row
   const bool row_live = mine && fr < f0 + nf;
-  const int lim = !row_live ? 0 : a.run ? min(p1, a.plen + span_row(a, fr) + 1) : prefix ? p1 : min(p1, x.sees(span_row(a, fr)));
+  const int lim = !row_live ? 0 : prefix ? p1 : min(p1, x.sees(span_row(a, fr)));
   float m = -INFINITY, l = 0.0f;
   float acc[16][4];
 #pragma unroll
@@ -306,9 +306,9 @@ HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles, int size
   }
 }
 
-__global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles, int size) {
+__global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, SpanParts p, int tiles) {
   next_may_start();
-  span_part(a, p, tiles, size);
+  span_part(a, p, tiles);
   if ((blockIdx.x | blockIdx.y | threadIdx.x) == 0) prior_done();
 }
 
@@ -335,17 +335,18 @@ HV_DEV void span_few(const SpanArgs& a, const SpanParts& p, int tiles) {
   const __half *k, *v;
   int f0, nf, p0, p1, slot, lim_all;
   SpanSeq x;
-  const bool prefix = blockIdx.x < (unsigned)(tiles * p.npc);   // (then F is 8 or less)
+  const bool prefix = blockIdx.x < (unsigned)(tiles * p.npc);
   if (prefix) {
-    const int n = span_sees(a, span_prefix(a), F - 1), len = span_chunk(n, p.npc);
-    p0 = blockIdx.x * len;
+    const int tile = blockIdx.x / p.npc, chunk = blockIdx.x % p.npc;
+    f0 = tile * kFewRows;
+    nf = min(kFewRows, F - f0);
+    const int n = span_sees(a, span_prefix(a), f0 + nf - 1), len = span_chunk(n, p.npc);
+    p0 = chunk * len;
     p1 = min(n, p0 + len);
-    f0 = 0;
-    nf = F;
-    slot = p.nwt + blockIdx.x;
+    slot = p.nwt + chunk;
     k = a.pk + kvh * a.p_head;
     v = a.pv + kvh * a.p_head;
-    lim_all = a.run ? min(p1, a.plen + 1) : p1;
+    lim_all = a.run ? min(p1, a.plen + span_row(a, f0) + 1) : p1;
   } else {
     const int b = blockIdx.x - tiles * p.npc, chunk = b % p.ntc;
     const SpanItem it = span_item(a, b / p.ntc, kFewRows);
@@ -884,7 +885,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 // How a call's positions are cut, by its capacities (the lengths are on the device): as many
 // chunks as give every SM two CTAs, of a stage at the least.
-constexpr int kSms = 148, kPtCtas = 2 * kSms;
+constexpr int kSms = 148, kPtCtas = 2 * kSms, kFwCtas2 = 6 * kSms;   // that run at once; k_span_few<2>
 struct SpanPlan {
   int size, tiles, items, nwt, npc, ntc;   // tiles of the prefix's rows, items of the tails'
   size_t part, ml, stretches, stat, scores, terms, facs, bytes;
@@ -900,35 +901,31 @@ SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool 
     if (rows * ((pcap + kStRows - 1) / kStRows) < 1ll << 31)
       p.nwt = (int)std::min((long long)((pcap + kStRows - 1) / kStRows), kSms / rows + 2);
   }
-  // Eights of rows where there are no more, or where only tails are left. Four warps share an item's
-  // positions as long as all items find room at once: an item is over sooner then. Else short tails
-  // have as many warps an item as there is work for (256 sequences of one row, tails up to 250,
-  // group 4: 97 us with four, 84 with two; tails up to 20: 65 and, with one warp, 50; ragged runs of 24
-  // after 2000: 39 by k_span_part, 36.7), and long ones as long as rows are few (24 runs of 3 to 17
-  // rows, tails of 1000, group 4: 109 by k_span_part, 90 by fours; group 8: 145 and 153).
+  // Eights of rows, four warps to an item, as long as all items find room at once: an item is over
+  // sooner then. Else two, or one where only short tails are left (256 sequences of one row, tails
+  // up to 250, group 4: 97 us with four, 84 with two; tails up to 20: 65 and, with one, 50; a run of
+  // 64 at 0, 64 q over 8 kv heads: 33, 28; of 16 at 1000: 21, 23, and 27 by k_span_part). k_span_part
+  // has long tails of many rows (24 runs of 3 to 17 rows, tails of 1000: group 4 109 us, and 90 by
+  // fours; group 8 145 and 153).
+  const int eights = (F + kFewRows - 1) / kFewRows;
   const bool tails = !run && p.nwt;
-  const bool many = (long long)nkv * std::max(nseq, F / kFewRows) > kPtCtas;
-  if (F <= kFewRows || (tails && !many)) p.few = 4;
-  else if (tails && tcap <= 256) p.few = tcap <= 32 ? 1 : 2;
-  else if (tails && (F / nseq <= 2 * kFewRows ||
-                     (F / nseq <= 64 && (long long)nkv * (F / kFewRows + nseq) <= 8 * kSms))) p.few = 4;
-  // All others as many rows a CTA as leave one for every SM: a product of the f16 pipe takes 16
-  // cycles of a quarter of an SM, so that 64 rows by 64 positions are 2.5 us of one CTA's time
-  p.size = kFewRows;
-  if (!p.few) {
-    p.size = kSpanItem;
-    const int most = p.nwt ? stages(tcap) : stages(pcap) + (run ? 0 : stages(tcap));
-    while (p.size > 16 && (long long)nkv * ((F + p.size - 1) / p.size) * most < kSms) p.size /= 2;
-  }
+  const long long items = (long long)nkv * (run ? eights : std::max(nseq, eights) + (p.nwt ? 0 : eights));
+  if (F <= kFewRows || items <= kPtCtas) p.few = 4;
+  else if (run || tcap <= 256) p.few = tails && tcap <= 32 ? 1 : 2;
+  else if (F / nseq <= 2 * kFewRows || (F / nseq <= 64 && (long long)nkv * (eights + nseq) <= 8 * kSms)) p.few = !tails && F / nseq <= kFewRows ? 2 : 4;
+  p.size = p.few ? kFewRows : kSpanItem;
   p.tiles = (F + p.size - 1) / p.size;
   p.items = run ? 0 : nseq + p.tiles;
-  if (!p.nwt) p.npc = std::min(stages(pcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * p.tiles)));
-  if (!run) p.ntc = std::min(stages(tcap), (int)std::max(1ll, kPtCtas / ((long long)nkv * std::max(nseq, p.tiles))));
+  // Chunks: as many as run at once, the prefix's and the tails' by their shares of the work
+  const int fit = p.few == 2 && !tails ? kFwCtas2 : kPtCtas, lines = std::max(nseq, p.tiles);
+  const long long work_t = (long long)lines * stages(tcap), work_p = tails ? 0 : (long long)p.tiles * stages(pcap);
+  if (!run) p.ntc = std::min(stages(tcap), (int)std::max(1ll, fit * work_t / (work_t + work_p) / ((long long)nkv * lines)));
+  if (!p.nwt) p.npc = std::min(stages(pcap), std::max(1, (fit / nkv - (run ? 0 : lines * p.ntc)) / p.tiles));
   // room for this call and any smaller one, which may have more chunks of fewer rows: chunks times
-  // tiles (or sequences) are at most kPtCtas / nkv, or one each
+  // tiles (or sequences) are at most what fits / nkv, or one each
   const size_t all = (size_t)nkv * F;
   auto room = [&](int n) {
-    return std::min((size_t)stages(n) * all, (size_t)kPtCtas * std::min(F, kSpanItem) + all);
+    return std::min((size_t)stages(n) * all, (size_t)std::max(kPtCtas * std::min(F, kSpanItem), kFwCtas2 * std::min(F, kFewRows)) + all);
   };
   const size_t whole = std::min((size_t)((pcap + kStRows - 1) / kStRows) * all, (size_t)kSms * std::min(F, kStRows) + 2 * all);
   const size_t rows = whole + room(pcap) + (run ? 0 : room(tcap));
@@ -987,7 +984,7 @@ int span_launch(const char* name, const SpanArgs& a, const SpanPlan& p, const Sp
   if (p.few == 4) HV_CUDA(launch_beside(k_span_few<4>, grid, 128, smem, st, s.nwt > 0, a, s, p.tiles));
   else if (p.few == 2) HV_CUDA(launch_beside(k_span_few<2>, grid, 64, smem, st, s.nwt > 0, a, s, p.tiles));
   else if (p.few == 1) HV_CUDA(launch_beside(k_span_few<1>, grid, 32, smem, st, s.nwt > 0, a, s, p.tiles));
-  else HV_CUDA(launch_beside(k_span_part, grid, 32 * kPtWarps, smem, st, s.nwt > 0, a, s, p.tiles, p.size));
+  else HV_CUDA(launch_beside(k_span_part, grid, 32 * kPtWarps, smem, st, s.nwt > 0, a, s, p.tiles));
   return HV_OK;
 }
 int join_launch(const SpanArgs& a, const SpanParts& s, cudaStream_t st) {

@@ -129,6 +129,15 @@ def test_tails_of_many_rows_after_a_long_prefix(hv, nkv, group, rows, longest):
     check_shared(hv, g, nkv, group, plen, plen, rows, tails, longest + 1, extra=3)
 
 
+@pytest.mark.parametrize("nkv,group,plen,rows,tails", [
+    (8, 8, 50, [40] * 4, [40, 300, 129, 64]), (8, 4, 0, [30, 50, 80, 1], [400, 300, 80, 270]),
+    (8, 4, 45, [1] * 64, [1 + 37 * s % 290 for s in range(64)]), (8, 8, 3, [2] * 40, [2 + 7 * s for s in range(40)]),
+    (8, 2, 200, [9] * 8, [60 - s for s in range(8)]), (2, 8, 90, [70, 3, 90], [70, 600, 95])])
+def test_tails_of_many_rows_after_a_short_prefix(hv, nkv, group, plen, rows, tails):
+    g = np.random.default_rng(plen + group)
+    check_shared(hv, g, nkv, group, plen, plen + 2, rows, tails, max(tails) + 1, extra=1)
+
+
 @pytest.mark.parametrize("which", ["k", "v"])
 @pytest.mark.parametrize("bad", [np.nan, -np.inf])
 @pytest.mark.parametrize("longest", [30, 200, 300])
