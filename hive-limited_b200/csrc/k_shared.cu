@@ -895,8 +895,11 @@ struct SpanPlan {
 SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool mass) {
   SpanPlan p{};
   auto stages = [](int n) { return (n + kSpanStage - 1) / kSpanStage; };
-  // many rows over many positions go by whole tiles
-  if (F > 32 && (long long)F * pcap >= 1 << 17) {
+  // Many rows over many positions go by whole tiles, whose kernel takes 10 us for the first of them
+  // (256 pairs a head, 8 heads: over 512 positions 18 us, and 25 by eights; over 256 14 and 11; a
+  // run's 128 over 1280 26.5 and 24.6, over 2048 24.6 and 26.6)
+  const long long work = (long long)nkv * F * pcap;
+  if (F > 32 && work >= (run ? 3 : 2) << 19) {
     const long long rows = (long long)nkv * ((F + kStRows - 1) / kStRows);
     if (rows * ((pcap + kStRows - 1) / kStRows) < 1ll << 31)
       p.nwt = (int)std::min((long long)((pcap + kStRows - 1) / kStRows), kSms / rows + 2);
@@ -1022,7 +1025,10 @@ int mass_any(const char* name, const SpanArgs& a, const float* mass_in, float* m
   const bool one = a.plen_p != nullptr;                     // a single row at a device position
   SpanPlan p = span_plan(nkv, a.nrow * a.group, 1, cap, 0, true, true);
   const int n = a.plen + a.nrow;
-  p.mass_tiles = !one && (long long)a.nrow * a.group * n >= 1 << 18;
+  // k_mass_rows goes through the rows one stage after the other (8 heads: 128 pairs over 768
+  // positions 19.7 us, and 18.0 by tiles; 512 over 128 32.7 and 20.4; 40 over 5000 28.5 and 31.8)
+  const long long F = (long long)a.nrow * a.group, work = nkv * F * n;
+  p.mass_tiles = !one && work * F >= 1ll << (F >= kStRows ? 26 : 27);
   SpanParts s = span_parts(p, scratch, cap, true, one);
   int rc = span_launch(name, a, p, s, st);
   if (rc) return rc;

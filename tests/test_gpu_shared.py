@@ -90,13 +90,14 @@ def test_runs_of_rows(hv, nkv, group, plen, rows, tails):
 
 @pytest.mark.parametrize("nkv,group,nseq,plen", [
     (1, 1, 129, 2100), (2, 3, 50, 2500), (1, 5, 70, 1024), (8, 4, 64, 1100), (3, 7, 40, 1500),
-    (1, 8, 64, 4097), (1, 2, 65, 2176), (1, 4, 40, 12800), (8, 8, 64, 2100), (8, 4, 33, 8190)])
+    (1, 8, 64, 4097), (1, 2, 65, 2176), (1, 4, 40, 12800), (8, 8, 64, 2100), (8, 4, 33, 8190),
+    (1, 1, 600, 2100), (2, 3, 100, 2500), (1, 2, 300, 2176), (1, 5, 250, 1024)])
 def test_many_rows_over_a_long_prefix(hv, nkv, group, nseq, plen):
     g = np.random.default_rng(plen)
     check_shared(hv, g, nkv, group, plen, plen + 130, [1] * nseq, [1 + i % 7 for i in range(nseq)], 9, one=True)
 
 
-@pytest.mark.parametrize("nseq", [3, 70])
+@pytest.mark.parametrize("nseq", [3, 70, 160])
 @pytest.mark.parametrize("way", ["rising", "falling", "steps", "peaks", "far"])
 def test_scores_that_change_along_the_prefix(hv, nseq, way):
     """The largest score so far is passed often, seldom, by a little and by far."""
@@ -125,7 +126,7 @@ def test_tails_of_many_rows_after_a_long_prefix(hv, nkv, group, rows, longest):
     g = np.random.default_rng(longest + group)
     tails = [max(r, min(longest, 1 + (i * 37) % longest)) for i, r in enumerate(rows)]
     tails[-1] = longest
-    plen = -(-2 ** 17 // (group * (sum(rows) + 3)))       # just enough for tiles
+    plen = -(-2 ** 20 // (nkv * group * (sum(rows) + 3)))  # just enough for tiles
     check_shared(hv, g, nkv, group, plen, plen, rows, tails, longest + 1, extra=3)
 
 
@@ -168,6 +169,7 @@ def test_a_prefix_of_full_capacity_and_none_at_all(hv):
     check_shared(hv, g, 2, 2, 0, 40, [2, 1], [2, 6], 6)
     check_shared(hv, g, 2, 4, 0, 5000, [1] * 40, [i % 5 for i in range(40)], 5, one=True)
     check_shared(hv, g, 1, 4, 1024, 1024, [1] * 40, [5] * 40, 5, one=True)
+    check_shared(hv, g, 2, 8, 1024, 1024, [1] * 70, [5] * 70, 5, one=True)
 
 
 def test_rows_that_see_nothing_are_zero(hv):
@@ -177,7 +179,7 @@ def test_rows_that_see_nothing_are_zero(hv):
     check_shared(hv, g, 1, 8, 40, 64, [5, 1], [2, 0], 4)
 
 
-@pytest.mark.parametrize("rows,plen", [([1] * 4, 200), ([1] * 40, 600), ([6, 4], 300), ([1] * 40, 2000)])
+@pytest.mark.parametrize("rows,plen", [([1] * 4, 200), ([1] * 40, 600), ([6, 4], 300), ([1] * 40, 2000), ([1] * 100, 2000)])
 def test_lengths_out_of_range_leave_nan(hv, rows, plen):
     g = np.random.default_rng(7)
     nseq = len(rows)
@@ -226,7 +228,7 @@ def test_what_a_row_does_not_see_does_not_count(hv, which, bad):
                                          (0.0, 1.0, 1.0), (1.0, 2e4, 1e-3), (1e-30, 3e34, 1.0)])
 def test_queries_and_scales_of_any_size(hv, scale, qs, ks):
     g = np.random.default_rng(9)
-    for nseq, plen in ((3, 300), (40, 300), (40, 2000)):
+    for nseq, plen in ((3, 300), (40, 300), (40, 2000), (150, 2000)):
         pk, pv = cache(g, 1, plen)
         tk, tv = cache(g, nseq, 1, 40)
         pk, tk = (pk * F16(ks)).astype(F16), (tk * F16(ks)).astype(F16)
