@@ -12,7 +12,8 @@
 // move the masses before all have read them; apart they have some of the rows each.
 //
 // Bound by HBM when caches are many (36 caches of 8 heads, 4352 positions to 4096: 1.21 GB read and
-// written), by latency when they are few.
+// written in 228 us, 82% of a copy's rate; 271 with rows through registers and one bit of the border a
+// pass), by latency when they are few (300 positions of 2 heads to 256: 8.4 us for 19).
 #include <cuda_fp16.h>
 
 #include <algorithm>

@@ -14,14 +14,16 @@
 namespace hv {
 namespace {
 
-// ---- attention of few rows a head ---------------------------------------------------------
+// ---- long tails of many rows --------------------------------------------------------------
 //
 // A CTA has up to 64 (row, head) pairs of a kv head and a chunk of the prefix or of a sequence's
-// tail. Rows stand by eights as the 16-row operand of the f16 tensor pipe, their first binary16
+// tail, so that K and V come from the L2 cache once for 64 pairs. Rows stand by eights as the 16-row operand of the f16 tensor pipe, their first binary16
 // terms above their second ones, so that one product serves both and a thread adds what belongs
 // together (the same for the weights of the second product). Warps share the CTA's rows by eights
 // and then its positions, 32 at a time. K and V come by 16-byte asynchronous copies, 64 positions
-// to a stage, swizzled so that eight rows' 16 bytes meet no bank twice.
+// to a stage, swizzled so that eight rows' 16 bytes meet no bank twice. Bound by the f16 pipe, of
+// which a product takes 16 cycles of a quarter of an SM: 64 rows by 64 positions are 2.5 us of a
+// CTA's time (16 runs of 100 to 120 rows with tails to 600, 32 q over 8 kv heads: 177 us).
 constexpr int kPtWarps = 8;
 constexpr int kPtTile = kSpanStage * kHd * 2;            // bytes of K or of V of a stage
 constexpr int kPtQ = kSpanItem * 2 * kHd * 2;            // bytes of 64 rows' two terms
@@ -316,9 +318,11 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
 //
 // One item of eight (row, head) pairs and a chunk of positions a CTA, as for k_span_part, but every
 // warp has all rows, takes 16 positions in turn with the others and has a ring of its own for them,
-// so that no warp waits for another before the end. Bound by the bytes of the cache. Short tails of
-// many rows have one warp a CTA: an item is then over in a few steps of 16 positions, and eleven
-// of them fit an SM.
+// so that no warp waits for another before the end. With four warps two CTAs fit an SM, with two
+// six and with one eleven: short items want few warps, as they are over in a few steps, and few
+// items many. One row over a long cache is bound by HBM (39999 positions of 8 heads: 164 MB in 33 us),
+// most calls by the chain of an item: lengths, rows and first blocks, steps, the warps' meeting
+// (4 us).
 constexpr int kFwBlock = 16;
 constexpr int kFwTile = kFwBlock * kHd * 2;              // bytes of K or of V of 16 positions
 constexpr int kFwQ = 2 * kFewRows * kHd * 2;
@@ -530,7 +534,9 @@ __global__ void __launch_bounds__(32 * kFwWarps, kFwWarps == 1 ? 11 : kFwWarps =
 //
 // kWarps warps share a row's slots, kPer rows a CTA (all of one tile of kStRows): one warp a row
 // where slots are few, with several rows after each other where rows are many, so that the fixed
-// part (which slots there are) is spread over them; four where a row's loads would follow each other.
+// part (which slots there are) is spread over them; four where a row's loads would follow each other
+// (16 sequences over 4096 positions, 512 rows of up to 20 slots: 21.1 us for the call, 23.2 by one). A row's sequence is looked up
+// before the wait for the parts: 1 us of the 3 that the join adds to a call.
 template <int kWarps, int kPer>
 HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
   constexpr int kAt = kWarps == 1 ? 4 : 8;                 // slots' rows under way
@@ -656,7 +662,8 @@ __global__ void __launch_bounds__(256, kWarps == 1 ? 4 : 3) k_span_join(SpanArgs
 }
 
 // A single row's end: its chunks added up by the first CTAs of a kv head, and by the others the
-// weights of the scores that k_span_few has left, 1024 positions each.
+// weights of the scores that k_span_few has left, 1024 positions each (39999 positions, 64 q over 8
+// kv heads: 51 us for the call with two launches in place of this one, 39 with it).
 constexpr int kOnePos = 1024;
 __global__ void __launch_bounds__(256) k_span_one(SpanArgs a, SpanParts p, const float* mass_in, float* mass_out, int joins) {
   if ((int)blockIdx.x < joins) return span_join<4, 2>(a, p);
@@ -713,7 +720,9 @@ __global__ void __launch_bounds__(256) k_span_one(SpanArgs a, SpanParts p, const
 // w = 2^(x - m) / l once every row's m and l are known, so the scores are formed again, this time
 // with the positions as the 16-row operand: a thread then has two positions and adds up over
 // the columns, the rows. wpos of a CTA's warps have 16 positions each, and wpos warps at a time
-// take the rows in turn, 64 to a stage, split as k_span_part splits them.
+// take the rows in turn, 64 to a stage, split as k_span_part splits them. Bound by the f16 pipe where
+// rows or positions are many, else by its chain of row stages (16 rows at 8176, 8 q over 8 kv heads:
+// 22.7 us for the call, 30 by tiles; 256 at 704, 32 over 8: 30.6 and 22.6).
 template <int kPos>                                        // warps with positions of their own
 __global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, const float* mass_in, float* mass_out, int cap) {
   extern __shared__ __align__(1024) uint8_t smem[];         // 64 rows' two terms, then K
