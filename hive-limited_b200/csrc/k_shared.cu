@@ -897,6 +897,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 constexpr int kSms = 148, kPtCtas = 2 * kSms, kFwCtas2 = 6 * kSms;   // that run at once; k_span_few<2>
 struct SpanPlan {
   int size, tiles, items, nwt, npc, ntc;   // tiles of the prefix's rows, items of the tails'
+  int grid;                                // CTAs of k_span_tile
   size_t part, ml, stretches, stat, scores, terms, facs, bytes;
   bool mass_tiles;
   int few;                                 // warps of k_span_few, or 0: k_span_part
@@ -933,6 +934,35 @@ SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool 
   const long long work_t = (long long)lines * stages(tcap), work_p = tails ? 0 : (long long)p.tiles * stages(pcap);
   if (!run) p.ntc = std::min(stages(tcap), (int)std::max(1ll, fit * work_t / (work_t + work_p) / ((long long)nkv * lines)));
   if (!p.nwt) p.npc = std::min(stages(pcap), std::max(1, (fit / nkv - (run ? 0 : lines * p.ntc)) / p.tiles));
+  // Where few tiles are a CTA's, they go to fewer CTAs, so that the tails run on the SMs that leaves
+  // (times in us: a CTA's first tile and every further one, an item). 16 sequences over 4096
+  // positions, tails up to 250, 32 q over 8 kv heads: 21.3 us with 128 CTAs for the tiles, 18.8 with 88;
+  // 64 over 2000, 16 q: 29.5 and 21.8.
+  p.grid = kSms;
+  if (tails) {
+    const int rows = nkv * ((F + kStRows - 1) / kStRows), whole = (pcap + kStRows - 1) / kStRows;
+    const int warps = p.few ? p.few : 8, at_once = p.few == 1 ? 11 : p.few == 2 ? 6 : 2;
+    const int steps = (span_chunk(tcap, p.ntc) + 16 * warps - 1) / (16 * warps);
+    const float item = 3.5f + 0.4f * steps, first = 9.0f, tile = 1.8f;
+    const long long all_items = (long long)nkv * lines * p.ntc;
+    auto behind = [&](long long n) { return item * ((n + at_once * kSms - 1) / (at_once * kSms)); };
+    // evenly cut among all SMs, where most CTAs go from one tile of rows to the next
+    float best = first + tile * ((float)rows * whole / kSms + 2) + behind(all_items);
+    for (int each = std::min(kSms / rows, whole), last = 0; each > 0; --each) {
+      const int share = (whole + each - 1) / each;
+      if (share == last) continue;
+      last = share;
+      const int ctas = rows * ((whole + share - 1) / share);
+      const float time = first + tile * (share - 1);
+      const long long beside = (long long)(at_once * (kSms - ctas) * (time / item));
+      const float all_time = time + behind(std::max(0ll, all_items - beside));
+      if (all_time < best) {
+        best = all_time;
+        p.grid = ctas;
+      }
+      if (time > best) break;
+    }
+  }
   // room for this call and any smaller one, which may have more chunks of fewer rows: chunks times
   // tiles (or sequences) are at most what fits / nkv, or one each
   const size_t all = (size_t)nkv * F;
@@ -970,7 +1000,7 @@ SpanParts span_parts(const SpanPlan& p, void* scratch, int pcap, bool mass, bool
   s.npc = p.npc;
   s.ntc = p.ntc;
   s.size = p.size;
-  s.grid = kSms;
+  s.grid = p.grid;
   s.scores_ld = (size_t)(pcap + 3) / 4 * 4;
   return s;
 }
@@ -1037,7 +1067,7 @@ int mass_any(const char* name, const SpanArgs& a, const float* mass_in, float* m
   // k_mass_rows goes through the rows one stage after the other (8 heads: 128 pairs over 768
   // positions 19.7 us, and 18.0 by tiles; 512 over 128 32.7 and 20.4; 40 over 5000 28.5 and 31.8)
   const long long F = (long long)a.nrow * a.group, work = nkv * F * n;
-  p.mass_tiles = !one && work * F >= 1ll << (F >= kStRows ? 26 : 27);
+  p.mass_tiles = !one && work >= (1ll << (F >= kStRows ? 26 : 27)) / F;
   SpanParts s = span_parts(p, scratch, cap, true, one);
   int rc = span_launch(name, a, p, s, st);
   if (rc) return rc;
