@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(32 * kPtWarps, 2) k_span_part(SpanArgs a, Span
 // One item of eight (row, head) pairs and a chunk of positions a CTA, as for k_span_part, but every
 // warp has all rows, takes 16 positions in turn with the others and has a ring of its own for them,
 // so that no warp waits for another before the end. With four warps two CTAs fit an SM, with two
-// six and with one eleven: short items want few warps, as they are over in a few steps, and few
+// six and with one ten: short items want few warps, as they are over in a few steps, and few
 // items many. One row over a long cache is bound by HBM (39999 positions of 8 heads: 164 MB in 33 us),
 // most calls by the chain of an item: lengths, rows and first blocks, steps, the warps' meeting
 // (4 us).
@@ -935,25 +935,26 @@ SpanPlan span_plan(int nkv, int F, int nseq, int pcap, int tcap, bool run, bool 
   if (!run) p.ntc = std::min(stages(tcap), (int)std::max(1ll, fit * work_t / (work_t + work_p) / ((long long)nkv * lines)));
   if (!p.nwt) p.npc = std::min(stages(pcap), std::max(1, (fit / nkv - (run ? 0 : lines * p.ntc)) / p.tiles));
   // Where few tiles are a CTA's, they go to fewer CTAs, so that the tails run on the SMs that leaves
-  // (times in us: a CTA's first tile and every further one, an item). 16 sequences over 4096
+  // (times in us: of a CTA's n tiles and of an item, as measured). 16 sequences over 4096
   // positions, tails up to 250, 32 q over 8 kv heads: 21.3 us with 128 CTAs for the tiles, 18.8 with 88;
   // 64 over 2000, 16 q: 29.5 and 21.8.
   p.grid = kSms;
   if (tails) {
     const int rows = nkv * ((F + kStRows - 1) / kStRows), whole = (pcap + kStRows - 1) / kStRows;
-    const int warps = p.few ? p.few : 8, at_once = p.few == 1 ? 11 : p.few == 2 ? 6 : 2;
-    const int steps = (span_chunk(tcap, p.ntc) + 16 * warps - 1) / (16 * warps);
-    const float item = 3.5f + 0.4f * steps, first = 9.0f, tile = 1.8f;
+    const int warps = p.few ? p.few : 8, at_once = p.few == 1 ? 10 : p.few == 2 ? 6 : 2;
+    const int chunk = span_chunk(tcap, p.ntc), steps = (chunk + 16 * warps - 1) / (16 * warps);
+    const float item = p.few ? 2.3f + std::max(2, steps) : 4.0f + 2.5f * (chunk / kSpanStage);
+    auto tiles_take = [](float n) { return 9.0f + 1.4f * std::min(n - 1, 6.0f) + 1.8f * std::max(n - 7, 0.0f); };
     const long long all_items = (long long)nkv * lines * p.ntc;
     auto behind = [&](long long n) { return item * ((n + at_once * kSms - 1) / (at_once * kSms)); };
     // evenly cut among all SMs, where most CTAs go from one tile of rows to the next
-    float best = first + tile * ((float)rows * whole / kSms + 2) + behind(all_items);
+    float best = tiles_take((float)rows * whole / kSms + 3) + behind(all_items);
     for (int each = std::min(kSms / rows, whole), last = 0; each > 0; --each) {
       const int share = (whole + each - 1) / each;
       if (share == last) continue;
       last = share;
       const int ctas = rows * ((whole + share - 1) / share);
-      const float time = first + tile * (share - 1);
+      const float time = tiles_take(share);
       const long long beside = (long long)(at_once * (kSms - ctas) * (time / item));
       const float all_time = time + behind(std::max(0ll, all_items - beside));
       if (all_time < best) {
