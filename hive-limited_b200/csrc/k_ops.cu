@@ -361,6 +361,7 @@ __global__ void k_kvapp(const float* __restrict__ k, const float* __restrict__ v
                         float* __restrict__ kc, float* __restrict__ vc,
                         const int32_t* __restrict__ pos, int hd, int cap) {
   const int p = *pos;
+  if (p < 0 || p >= cap) return;
   const int h = blockIdx.x;
   for (int d = threadIdx.x; d < hd; d += blockDim.x) {
     kc[((size_t)h * cap + p) * hd + d] = k[h * hd + d];
@@ -374,6 +375,7 @@ __global__ void k_kvapp16(const float* __restrict__ k, const float* __restrict__
                           __half* __restrict__ kc, __half* __restrict__ vc,
                           const int32_t* __restrict__ pos, int hd, int cap) {
   const int p = *pos;
+  if (p < 0 || p >= cap) return;
   const int h = blockIdx.x;
   for (int d = threadIdx.x; d < hd; d += blockDim.x) {
     kc[((size_t)h * cap + p) * hd + d] = __float2half_rn(k[h * hd + d]);

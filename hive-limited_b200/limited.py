@@ -960,6 +960,10 @@ class Engine:
         for b0 in range(0, n, pf["n"]):
             m = min(pf["n"], n - b0)
             self._prefill_run(toks[b0:b0 + m], b0)
+        if self.kv_keep is not None and self._held == self.kv_cap:
+            # a decode step counts on room for its row: it thins the cache after it, not before
+            self._evict(0, self.kv_cap - 1)
+            self._held = min(self.kv_keep, self.kv_cap - 1)
         # the last prompt token: final norm and LM head, as the eager step ends
         hvdrv.copy_async(self.d_h, pf["h"] + (m - 1) * hid * 4, hid * 4, s)
         hvdrv.rmsnorm(self.d_h, self.d_hn, self.d_onorm, 1, hid, RMS_EPS, s)

@@ -229,7 +229,7 @@ int hv_rope(float* vec, const float* cos_t, const float* sin_t, const int32_t* p
             int half, void* stream);
 
 /* kvapp_pos (k_devgen.ptx; engine/limited.py:398-400): KC/VC [nkv][cap][hd] <- k, v at
- * the device position *pos. */
+ * the device position *pos (nothing outside [0, cap)). */
 int hv_kv_append(const float* k, const float* v, float* kc, float* vc, const int32_t* pos,
                  int nkv, int hd, int cap, void* stream);
 
@@ -249,7 +249,8 @@ int hv_attn_decode(const float* q, const float* kc, const float* vc, float* ctx,
 /* The compressed-KV lane (no counterpart in the reference, which keeps an f32 cache;
  * engine/limited.py:323-325 names the fp32 KV as the engine's sharpest limitation): the
  * cache holds IEEE binary16 values [nkv][cap][hd] (half the bytes). hv_kv_append_f16
- * stores f16(k), f16(v) rounded to nearest-even (numpy's astype(float16)); then
+ * stores f16(k), f16(v) rounded to nearest-even (numpy's astype(float16); nothing where *pos is
+ * outside [0, cap)); then
  * hv_attn_decode_f16 computes exactly what hv_attn_decode computes over an f32 cache that
  * holds those f16 values widened (same chunking, same arithmetic). */
 int hv_kv_append_f16(const float* k, const float* v, uint16_t* kc, uint16_t* vc,
