@@ -39,7 +39,7 @@ constexpr uint32_t kMtColK = 128 * kMtSums;     // tensor memory: D, then K of t
 constexpr uint32_t kMtDesc = (1u << 4) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
 
 struct MtShared {
-  unsigned long long q_full[kMtStages], q_free[kMtStages], d_full[kMtSums], d_free[kMtSums], drain;
+  unsigned long long q_full[kMtStages], q_free[kMtStages], d_full[2][2], d_free[kMtSums], drain;
   float sum[4][kStRows];
   uint32_t tmem;
   int given_up;
@@ -64,10 +64,8 @@ __global__ void __launch_bounds__(kMtThreads, 1)
       bar_init(bar(sh.q_full[i]), 1);
       bar_init(bar(sh.q_free[i]), 1 + kMtSumThreads);
     }
-    for (int i = 0; i < kMtSums; ++i) {
-      bar_init(bar(sh.d_full[i]), 1);
-      bar_init(bar(sh.d_free[i]), 256);
-    }
+    for (int i = 0; i < kMtSums; ++i) bar_init(bar(sh.d_free[i]), 256);
+    for (int i = 0; i < 4; ++i) bar_init(bar(sh.d_full[i >> 1][i & 1]), 1);
     bar_init(bar(sh.drain), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.given_up = (sm & 1023) != 0;               // the swizzle goes by addresses
@@ -100,9 +98,14 @@ __global__ void __launch_bounds__(kMtThreads, 1)
   Unit x;
   x.u = u0;
   int qi = 0, di = 0;                             // tiles of rows, sums, so far
+  // Sum di goes to group `two ? k : di & 1` of the warps that add up, which has d_full barriers of
+  // its own, two in turn: a barrier's phases can only be told apart by who follows each of them. Two
+  // are enough: no three sums in a row are one group's, so that before the next but one of it is
+  // issued, the present one has been left (there are kMtSums places).
   if (warp < 16) {
     const int g = (warp >> 2) & 1, half = warp >> 3, row = threadIdx.x & 127;
     const uint32_t to_lane = (uint32_t)(32 * (warp & 3)) << 16;
+    int di_own = 0;                               // the group's sums so far
     while (next(x)) {
       const int pos = x.p0 + (x.two ? g * kStRows : 0) + row;
       if (g <= x.two) {                           // half of this position's K: 32 of a lane's 64 columns
@@ -166,7 +169,8 @@ __global__ void __launch_bounds__(kMtThreads, 1)
         for (int k = 0; k <= x.two; ++k, ++di) {
           if (x.two ? k != g : (di & 1) != g) continue;
           const int b = di % kMtSums;
-          ok = ok && bar_wait_warp(bar(sh.d_full[b]), (di / kMtSums) & 1, given_up);
+          ok = ok && bar_wait_warp(bar(sh.d_full[g][di_own & 1]), (di_own >> 1) & 1, given_up);
+          ++di_own;
           if (!ok) continue;
           fence_after();
           const int see = first - r * kStRows - 64 * half;
@@ -189,6 +193,7 @@ __global__ void __launch_bounds__(kMtThreads, 1)
   } else if (warp == 16) {
     const uint32_t leader = elect_one();
     bool ok = true;
+    int di_of[2] = {0, 0};                        // each group's sums so far
     while (next(x)) {
       asm volatile("bar.sync 1, 544;" ::: "memory");
       fence_after();
@@ -208,7 +213,10 @@ __global__ void __launch_bounds__(kMtThreads, 1)
               mma_ts(tmem + 128 * b, tmem + kMtColK + 64 * k + 8 * s,
                      qd + (uint64_t)((pass * kMtTerm + (s >> 2) * kMtHalf + (s & 3) * 32) >> 4), kMtDesc,
                      pass == 0 || s > 0, leader);
-          mma_commit(bar(sh.d_full[b]), leader);
+          const int g = x.two ? k : di & 1;
+          mma_commit(bar(sh.d_full[g][(g ? di_of[1] : di_of[0]) & 1]), leader);
+          di_of[0] += g == 0;
+          di_of[1] += g;
         }
         mma_commit(bar(sh.q_free[stage]), leader);
       }
