@@ -170,7 +170,8 @@ HV_DEV bool not_finite(const uint4& y) {
 
 // Kernels of a call may start before the one before them has ended: what they read of it, or write
 // over, comes after prior_done. Each of them calls it, at its end at the latest, so that the end of
-// one is the end of all before it.
+// one is the end of all before it. What an earlier kernel of the call writes is read by __ldcg, never
+// by __ldg: that one is for what nobody writes as long as the kernel lives, and it began before.
 HV_DEV void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 HV_DEV void prior_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 template <class... P, class... A>

@@ -554,7 +554,7 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
   // its stretches of tiles
   int nw = 0;
   if (p.nwt && fb < F && span_tiles_of(a, np, fb / kStRows))
-    nw = p.stretches[kvh * ((F + kStRows - 1) / kStRows) + fb / kStRows];
+    nw = __ldcg(p.stretches + kvh * ((F + kStRows - 1) / kStRows) + fb / kStRows);
 #pragma unroll 1
   for (int i = warp / kWarps; i < kPer; i += 8 / kWarps, here = kPer > 8 / kWarps && i < kPer && find(i)) {
     const int f = fb + i;
@@ -594,9 +594,9 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
       auto load = [&](int j0) {
 #pragma unroll
         for (int j = 0; j < kAt; ++j)
-          if (j0 + j < n) y[j] = __ldg(reinterpret_cast<const float4*>(p.part + slot(i0 + j0 + j) * kHd) + lane);
+          if (j0 + j < n) y[j] = __ldcg(reinterpret_cast<const float4*>(p.part + slot(i0 + j0 + j) * kHd) + lane);
       };
-      const float2 ml = lane < n ? p.ml[slot(i0 + lane)] : make_float2(-INFINITY, 0.0f);
+      const float2 ml = lane < n ? __ldcg(p.ml + slot(i0 + lane)) : make_float2(-INFINITY, 0.0f);
       load(0);
       float up = fmaxf(M, ml.x);
 #pragma unroll
@@ -676,7 +676,7 @@ __global__ void __launch_bounds__(256) k_span_one(SpanArgs a, SpanParts p, const
   float4 x[8];
 #pragma unroll
   for (int h = 0; h < 8; ++h)
-    if (h < a.group && t0 < np) x[h] = __ldg(reinterpret_cast<const float4*>(scores + (size_t)h * p.scores_ld));
+    if (h < a.group && t0 < np) x[h] = __ldcg(reinterpret_cast<const float4*>(scores + (size_t)h * p.scores_ld));
   const size_t i = (size_t)kvh * a.pcap + t0;
   float in[4];
 #pragma unroll
@@ -686,7 +686,7 @@ __global__ void __launch_bounds__(256) k_span_one(SpanArgs a, SpanParts p, const
     const size_t at = (size_t)kvh * a.group + warp, step = (size_t)gridDim.y * a.group;
     float M = -INFINITY, L = 0.0f;
     for (int c = lane; c < n0; c += 32) {
-      const float2 ml = p.ml[at + c * step];
+      const float2 ml = __ldcg(p.ml + at + c * step);
       const float up = fmaxf(M, ml.x);
       L = (M == -INFINITY ? 0.0f : L * ex2(M - up)) + (ml.y == 0.0f ? 0.0f : ex2(ml.x - up) * ml.y);
       M = up;
@@ -765,7 +765,7 @@ __global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, cons
     rows_put<kSpanItem, 8>(x, scale, nf, smem, s_fac, warp);
     if (f0 + kSpanItem < F) rows_load<kSpanItem, 8>(a, kvh, f0 + kSpanItem, min(kSpanItem, F - f0 - kSpanItem), warp, x);
     if (threadIdx.x < nf) {
-      const float2 s = p.stat[(size_t)kvh * F + f0 + threadIdx.x];
+      const float2 s = __ldcg(p.stat + (size_t)kvh * F + f0 + threadIdx.x);
       s_stat[threadIdx.x] = make_float2(s.x, 1.0f / s.y);
     }
     __syncthreads();

@@ -1,0 +1,26 @@
+"""What the sources of kernels that start beside the one before them may not do, as no run can show it."""
+import re
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parent.parent / "hive-limited_b200" / "csrc"
+CALL_WRITES = r"\b(part|ml|stretches|stat|scores|terms|facs)\b"     # in a call's scratch
+
+
+def arguments(text, name):
+    """Of every call of `name` in the text, what stands between its parentheses."""
+    for m in re.finditer(rf"\b{name}\(", text):
+        depth, i = 1, m.end()
+        while depth:
+            depth += {"(": 1, ")": -1}.get(text[i], 0)
+            i += 1
+        yield text[m.end():i - 1]
+
+
+@pytest.mark.parametrize("name", ["k_shared.cu", "k_span_tile.cu", "k_mass_tile.cu"])
+def test_results_of_the_kernel_before_are_not_read_as_constants(name):
+    found = list(arguments((CSRC / name).read_text(), "__ldg"))
+    assert found
+    for arg in found:
+        assert not re.search(CALL_WRITES, arg), arg
