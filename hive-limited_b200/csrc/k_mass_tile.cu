@@ -19,7 +19,8 @@
 // the rate of a library's product; tensor pipe and exponentials are both active 54% of the time, and
 // every score's factor and offset come from shared memory. Eight warps in place of sixteen: 152 us.
 //
-// Every wait is bounded: one that runs out leaves NaN in the positions' mass.
+// Every wait is bounded, from the end of the kernel before on, beside which this one starts: one
+// that runs out leaves NaN in the positions' mass.
 #include <type_traits>
 
 #include "attn_f16.cuh"
@@ -123,6 +124,7 @@ __global__ void __launch_bounds__(kMtThreads, 1)
         tmem_st_wait();
       }
       fence_before();
+      prior_done();                                        // waits are for this kernel's work alone
       asm volatile("bar.sync 1, 544;" ::: "memory");       // with the warp that issues
       uint64_t acc[2] = {0, 0};
       const int first = max(0, pos - a.plen) * a.group;    // the first row that sees the position
@@ -194,6 +196,7 @@ __global__ void __launch_bounds__(kMtThreads, 1)
     const uint32_t leader = elect_one();
     bool ok = true;
     int di_of[2] = {0, 0};                        // each group's sums so far
+    prior_done();
     while (next(x)) {
       asm volatile("bar.sync 1, 544;" ::: "memory");
       fence_after();

@@ -24,3 +24,13 @@ def test_results_of_the_kernel_before_are_not_read_as_constants(name):
     assert found
     for arg in found:
         assert not re.search(CALL_WRITES, arg), arg
+
+
+def test_bounded_waits_begin_after_the_kernel_before():
+    """The limit of a wait on a barrier is for this kernel's work: no role counts the time that the
+    kernel before it still takes."""
+    text = (CSRC / "k_mass_tile.cu").read_text()
+    starts = [text.index(x) for x in ("if (warp < 16) {", "} else if (warp == 16) {", "} else if (lane == 0) {")]
+    for lo, hi in zip(starts, starts[1:] + [text.index("tcgen05.dealloc")]):
+        role = text[lo:hi]
+        assert "bar_wait" in role and 0 < role.find("prior_done();") < role.index("bar_wait")
