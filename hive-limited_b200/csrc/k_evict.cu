@@ -17,6 +17,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "attn_decode.cuh"
 #include "hv_internal.h"
@@ -284,6 +285,17 @@ int evict_launch(const EvictArgs& a, int parts, int nkv, int nset, cudaStream_t 
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+// Do n pieces of `bytes` from x on and n from y on, each `step` after the one before it, share
+// nothing? Pieces i and j are |y - x + (j - i) step| apart, the least at one of two j - i.
+bool pieces_apart(const void* x, const void* y, long long bytes, long long step, int n) {
+  const long long d = (long long)((uintptr_t)y - (uintptr_t)x);
+  if (n == 1) return std::llabs(d) >= bytes;
+  const long long near = std::max<long long>(1 - n, std::min<long long>(n - 1, -(d / step)));
+  for (long long m = std::max<long long>(1 - n, near - 1); m <= std::min<long long>(n - 1, near + 1); ++m)
+    if (std::llabs(d + m * step) < bytes) return false;
+  return true;
+}
+
 }  // namespace
 }  // namespace hv
 
@@ -328,10 +340,11 @@ extern "C" int hv_kv_evict_f16(const uint16_t* kc, const uint16_t* vc, long long
     };
     const long long from = 2 * ((nset - 1) * set * (nset > 1) + one), to = 2 * ((nset - 1) * set_d * (nset > 1) + one_d);
     HV_REQUIRE(apart(kc, from, kd, to) && apart(kc, from, vd, to) && apart(vc, from, kd, to) &&
-                   apart(vc, from, vd, to) && apart(kd, one_d * 2, vd, one_d * 2) &&
+                   apart(vc, from, vd, to) &&
                    apart(mass, 4ll * nset * nkv * cap, mass_d, 4ll * nset * nkv * dcap),
                HV_E_INVALID, "%s: source and destination overlap", name);
   }
+  HV_REQUIRE(pieces_apart(kd, vd, 2 * one_d, 2 * set_d, nset), HV_E_INVALID, "%s: K and V of the destination overlap", name);
   EvictArgs a{};
   a.kc = reinterpret_cast<const __half*>(kc); a.vc = reinterpret_cast<const __half*>(vc);
   a.kd = reinterpret_cast<__half*>(kd); a.vd = reinterpret_cast<__half*>(vd);

@@ -358,7 +358,8 @@ int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const float* sca
  *     (i * set_d elements on) and of mass_d [nset][nkv][dcap]; *len_out = keep. Otherwise all n stay and
  *     *len_out = n. kept (NULL or i32 [nset][nkv][dcap]) gets the position each came from. In
  *     place (kd = kc, vd = vc, mass_d = mass, dcap = cap, set_d = set), where nothing is moved
- *     and kept is not written unless n is over the limit, or to memory apart from the source.
+ *     and kept is not written unless n is over the limit, or to memory apart from the source. No
+ *     cache's K may lie where any one's V does, in the destination.
  *     recent <= keep <= limit <= dcap. len_out may be len. An n outside [0, cap] changes nothing.
  * scratch: as many bytes as the _scratch function says, 16-byte aligned, zeroed once by the
  * caller; every call leaves it ready for the next. Those bytes do for any call of up to the rows,

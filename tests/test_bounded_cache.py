@@ -81,3 +81,32 @@ def test_a_prompt_of_the_whole_context(monkeypatch):
         e, dev = engine(monkeypatch, keep, 100)
         e._prefill_batched([1] * 100, argmax=False)
         assert 0 < dev.held == e._held <= e.kv_cap
+
+
+# ---- K and V of an eviction's destination -------------------------------------------------
+
+P = 1 << 30
+ONE = 2 * 64 * 128                   # values of a cache of 2 heads, 64 positions
+
+
+def evict(kd, vd, set_d, nset, in_place=False):
+    import hvdrv
+    kc, vc = (kd, vd) if in_place else (P << 8, P << 9)
+    mass = P << 10
+    hvdrv.kv_evict(kc, vc, set_d if in_place else ONE, mass, 64, P << 11, 0, kd, vd, set_d,
+                   mass if in_place else P << 12, 64, P << 11, 0, 60, 40, 8, 2, 128, nset, P << 13)
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("nset,set_d,off", [
+    (1, 0, 0), (1, 0, ONE - 8), (1, 0, 8 - ONE),
+    (2, ONE, ONE), (2, ONE, -ONE), (2, 2 * ONE, 2 * ONE), (2, 2 * ONE, 3 * ONE - 8),
+    (3, 2 * ONE, ONE + 8), (3, 2 * ONE, ONE - 8), (3, 2 * ONE, 2 * ONE), (3, 2 * ONE, -4 * ONE), (3, 2 * ONE, 5 * ONE - 8),
+    (36, 2 * ONE, 70 * ONE), (36, 2 * ONE, -70 * ONE), (36, 3 * ONE, 2 * ONE + 8), (36, 3 * ONE, ONE - 8),
+    (4, 1 << 38, (1 << 38) + 64), (4, 1 << 38, -3 * (1 << 38))])
+def test_eviction_refuses_v_on_k(in_place, nset, set_d, off):
+    import hvdrv
+    kd = P << 20
+    with pytest.raises(hvdrv.CudaError, match="K and V of the destination") as e:
+        evict(kd, kd + 2 * off, set_d, nset, in_place)
+    assert e.value.code == 1001
