@@ -1219,25 +1219,25 @@ class Engine:
         return toks[0], toks[1:]
 
     def _many_buffers(self, nseq: int, tcap: int) -> dict:
-        """Tails of tcap positions for nseq sequences, and what their rows need (allocated on first
-        use, again when more is wanted)."""
+        """Tails of tcap positions for nseq sequences, and what their rows need. The memory stays from
+        call to call, each piece as large as any call wanted it; how it is laid out, and with it the
+        order of every sum, is this call's alone."""
         c = self.cfg
+        per = 2 * c.n_kv * c.head_dim * 2
+        scr = hvdrv.attn_shared_scratch(c.n_head, c.group, self.kv_cap, tcap, nseq, self.PREFILL_BATCH)
+        if self._many is None:
+            self._many = {"room": {}}
         mb = self._many
-        if mb is not None and mb["nseq"] >= nseq and mb["tcap"] >= tcap:
-            return mb
-        if mb is not None:
-            hvdrv.synchronize()
-            for k in ("tails", "scr", "hl", "row0", "tlen", "plen", "base"):
-                self._release(mb[k])
-            self._many = None
-        rows, per = self.PREFILL_BATCH, 2 * c.n_kv * c.head_dim * 2
-        n = hvdrv.attn_shared_scratch(c.n_head, c.group, self.kv_cap, tcap, nseq, rows)
-        mb = {"nseq": nseq, "tcap": tcap,
-              "tails": self._alloc(c.n_layer * nseq * tcap * per),
-              "scr": self._zeroed(n), "hl": self._alloc(nseq * c.hidden * 4),
-              "row0": self._alloc((nseq + 1) * 4), "tlen": self._alloc(nseq * 4),
-              "plen": self._alloc(4), "base": self._alloc(4)}
-        self._many = mb
+        for key, nbytes in (("tails", c.n_layer * nseq * tcap * per), ("scr", scr),
+                            ("hl", nseq * c.hidden * 4), ("row0", (nseq + 1) * 4), ("tlen", nseq * 4),
+                            ("plen", 4), ("base", 4)):
+            if mb["room"].get(key, 0) < nbytes:
+                if mb["room"].pop(key, 0):
+                    hvdrv.synchronize()
+                    self._release(mb.pop(key))
+                mb[key] = self._zeroed(nbytes) if key == "scr" else self._alloc(nbytes)
+                mb["room"][key] = nbytes
+        mb["tcap"] = tcap
         return mb
 
     def _shared_prefix(self, prompt: np.ndarray, mb: dict):

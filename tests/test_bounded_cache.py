@@ -110,3 +110,40 @@ def test_eviction_refuses_v_on_k(in_place, nset, set_d, off):
     with pytest.raises(hvdrv.CudaError, match="K and V of the destination") as e:
         evict(kd, kd + 2 * off, set_d, nset, in_place)
     assert e.value.code == 1001
+
+
+# ---- the buffers of many continuations ------------------------------------------------------
+
+def test_buffers_of_many_continuations_are_kept_but_laid_out_by_the_call(monkeypatch):
+    e, dev = engine(monkeypatch, 5, 100)
+    held, n = {}, [0]
+
+    def alloc(nbytes):
+        n[0] += 1
+        held[n[0] << 12] = nbytes
+        return n[0] << 12
+    e._buffers, e._many = [], None
+    dev.alloc, dev.free = alloc, held.pop
+    dev.attn_shared_scratch = lambda nq, group, pcap, tcap, nseq, nrow: 8 * tcap * nseq + 100
+    per = e.cfg.n_layer * 2 * e.cfg.n_kv * e.cfg.head_dim * 2
+    most, calls = {}, [(2, 10), (40, 10), (3, 90), (2, 10), (40, 10), (1, 400), (2, 10)]
+    for nseq, tcap in calls + calls:
+        before = dict(held)
+        mb = e._many_buffers(nseq, tcap)
+        assert mb["tcap"] == tcap
+        assert held[mb["tails"]] >= nseq * tcap * per and held[mb["scr"]] >= 8 * tcap * nseq + 100
+        assert held[mb["hl"]] >= nseq * e.cfg.hidden * 4 and held[mb["tlen"]] >= 4 * nseq
+        assert held[mb["row0"]] >= 4 * (nseq + 1)
+        assert len(held) == len(e._buffers) == 7
+        if (nseq, tcap) in most:
+            assert held == before                            # a call of a size that was there allocates nothing
+        most[nseq, tcap] = True
+
+    def fails(nbytes):
+        raise MemoryError
+    dev.alloc = fails
+    with pytest.raises(MemoryError):
+        e._many_buffers(41, 500)
+    dev.alloc = alloc
+    mb = e._many_buffers(41, 500)                            # what could not be had is asked for again
+    assert held[mb["tails"]] >= 41 * 500 * per and len(held) == len(e._buffers) == 7
