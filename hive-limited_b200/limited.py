@@ -1120,6 +1120,8 @@ class Engine:
     def logits(self, prompt_ids) -> np.ndarray:
         """Run the prompt and return the final f32 logits."""
         n = len(prompt_ids)
+        if not 1 <= n <= self.cfg.max_context:
+            raise ValueError(f"{n} prompt tokens for a {self.cfg.max_context}-token context")
         if self.prefill_mode == "batched":
             self._prefill_batched(prompt_ids, argmax=False)
         else:
