@@ -162,6 +162,11 @@ HV_DEV int span_cta(const SpanWhole& w, unsigned u) {
   return c;
 }
 
+// What the exponents of a row's weights are taken relative to where its scores are formed a second
+// time, for a first time's m. From 2^26 on the two times differ by enough to be seen in any weight;
+// what is added there keeps weights from passing 1, so that sums of them stay finite.
+HV_DEV float span_top(float m) { return fabsf(m) > 67108864.0f ? m + fabsf(m) * 0x1p-20f : m; }
+
 // Is one of eight halves an infinity or a NaN?
 HV_DEV bool not_finite(const uint4& y) {
   auto odd = [](uint32_t z) { return (z & 0x7C00u) == 0x7C00u || (z & 0x7C000000u) == 0x7C000000u; };

@@ -29,6 +29,7 @@ constexpr int kPtTile = kSpanStage * kHd * 2;            // bytes of K or of V o
 constexpr int kPtQ = kSpanItem * 2 * kHd * 2;            // bytes of 64 rows' two terms
 constexpr int kPtLine = kHd + 4;                         // floats between rows that are joined
 constexpr float kPtLift = 14.0f;                         // log2 of what weights are multiplied by
+constexpr float kPtDrop = 0x1p-14f;
 constexpr int kPtStages = 2;
 constexpr int kPtSmem = kPtQ + kPtStages * 2 * kPtTile;
 static_assert(kPtWarps * 8 * kPtLine * 4 <= kPtStages * 2 * kPtTile, "rows to join");
@@ -48,6 +49,7 @@ HV_DEV void add_up(float (&sum)[2], const float (&c)[4]) {
   sum[0] += c[0] + c[2];
   sum[1] += c[1] + c[3];
 }
+HV_DEV float4 dropped(const float4& x) { return make_float4(x.x * kPtDrop, x.y * kPtDrop, x.z * kPtDrop, x.w * kPtDrop); }
 HV_DEV void cp16(uint32_t to, const void* from, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
                :: "r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
@@ -242,11 +244,11 @@ HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles) {
         }
         m = up;
       }
-      const float m0 = m == -INFINITY ? 0.0f : m - kPtLift;
+      const float m0 = m == -INFINITY ? 0.0f : m;
       uint32_t wa[kN][4];
 #pragma unroll
       for (int j = 0; j < 4 * kN; ++j) {
-        w[j] = ex2(w[j] - m0);
+        w[j] = ex2((w[j] - m0) + kPtLift);       // (m - kPtLift may be m)
         l += w[j];
       }
 #pragma unroll
@@ -312,8 +314,8 @@ HV_DEV void span_part(const SpanArgs& a, const SpanParts& p, int tiles) {
       L += c * s_l[w][g];
       y.x += c * z.x; y.y += c * z.y; y.z += c * z.z; y.w += c * z.w;
     }
-    reinterpret_cast<float4*>(p.part + (row + i) * kHd)[lane] = y;
-    if (lane == 0) p.ml[row + i] = make_float2(M - kPtLift, L);
+    reinterpret_cast<float4*>(p.part + (row + i) * kHd)[lane] = dropped(y);
+    if (lane == 0) p.ml[row + i] = make_float2(M, L * kPtDrop);
   }
 }
 
@@ -474,11 +476,11 @@ HV_DEV void span_few(const SpanArgs& a, const SpanParts& p, int tiles) {
       }
       m = up;
     }
-    const float m0 = m == -INFINITY ? 0.0f : m - kPtLift;
+    const float m0 = m == -INFINITY ? 0.0f : m;
     uint32_t wa[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      w[j] = ex2(w[j] - m0);
+      w[j] = ex2((w[j] - m0) + kPtLift);       // (m - kPtLift may be m)
       l += w[j];
     }
     if (bad) {
@@ -529,8 +531,8 @@ HV_DEV void span_few(const SpanArgs& a, const SpanParts& p, int tiles) {
       L += c * s_l[j][g];
       y.x += c * z.x; y.y += c * z.y; y.z += c * z.z; y.w += c * z.w;
     }
-    reinterpret_cast<float4*>(p.part + (row + g) * kHd)[lane] = y;
-    if (lane == 0) p.ml[row + g] = make_float2(M - kPtLift, L);
+    reinterpret_cast<float4*>(p.part + (row + g) * kHd)[lane] = dropped(y);
+    if (lane == 0) p.ml[row + g] = make_float2(M, L * kPtDrop);
   }
 }
 
@@ -661,7 +663,7 @@ HV_DEV void span_join(const SpanArgs& a, const SpanParts& p) {
       reinterpret_cast<uint2*>(p.terms + (at + step) * kHd)[lane] = lo;
       const int Fp = (F + kStRows - 1) / kStRows * kStRows;
       if (lane < 2)
-        p.facs[((size_t)lane * gridDim.y + kvh) * Fp + f] = lane ? -(M + log2f(L)) : __ldg(a.scale) * kLog2e / lift;
+        p.facs[((size_t)lane * gridDim.y + kvh) * Fp + f] = lane ? -(span_top(M) + log2f(L)) : __ldg(a.scale) * kLog2e / lift;
     }
   }
 }
@@ -777,7 +779,7 @@ __global__ void __launch_bounds__(256) k_mass_rows(SpanArgs a, SpanParts p, cons
     if (f0 + kSpanItem < F) rows_load<kSpanItem, 8>(a, kvh, f0 + kSpanItem, min(kSpanItem, F - f0 - kSpanItem), warp, x);
     if (threadIdx.x < nf) {
       const float2 s = __ldcg(p.stat + (size_t)kvh * F + f0 + threadIdx.x);
-      s_stat[threadIdx.x] = make_float2(s.x, 1.0f / s.y);
+      s_stat[threadIdx.x] = make_float2(span_top(s.x), 1.0f / s.y);
     }
     __syncthreads();
     for (int o = wrow; o < (nf + 7) / 8; o += 8 / kPos) {

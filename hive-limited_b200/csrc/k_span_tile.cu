@@ -43,6 +43,7 @@ constexpr int kStHalf = kStRows * 128;          // bytes of 128 positions of 64 
 constexpr int kStTile = 2 * kStHalf;
 constexpr int kStLine = kHd + 4;                // floats from row to row on their way in and out
 constexpr int kStLift = 8;                      // log2 of what weights are multiplied by
+constexpr float kStDrop = 1.0f / (1 << kStLift);
 constexpr uint32_t kStColO = 256, kStColQ = 384;   // tensor memory: S twice, O, qh, ql
 // registers per thread: 128 at launch, then dealt out anew
 constexpr int kStRegs = 128, kStRegsRow = 144, kStRegsSum = 184, kStRegsCopy = 40;
@@ -211,7 +212,8 @@ __global__ void __launch_bounds__(kStThreads, 1)
       fence_before();
       rows_sync();
       fence_after();
-      float m = -INFINITY, l = 0.0f;              // of this thread's row
+      float m = -INFINITY, l = 0.0f;              // of this thread's row, m in units of `unit`
+      float unit = 1.0f;
       const int sees = span_sees(a, np, min(st.row0 + row, F - 1)) - st.j0 * kStRows;
       const uint32_t s_at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 128 * w;
       const uint32_t leader = elect_one();
@@ -283,13 +285,24 @@ __global__ void __launch_bounds__(kStThreads, 1)
           }
           tmem_st_wait();
         }
-        if (first) m = largest(0);
-        uint64_t f2 = pair(qs, qs), off, sum = 0;
-        auto base = [&] {
+        // An exponent is a product's, rounded once with m taken off, so it may pass m by half of what
+        // m is rounded by: beyond 2^26 too much for a weight. Exponents of such rows count in units
+        // of a power of two that keeps them under it. Weights are then not 0 within 150 such units, which
+        // is 2^-17.8 of the score: no more than what errors of 44 u on two scores come to.
+        uint64_t f2, off, sum = 0;
+        auto base = [&](float top) {
+          if (fabsf(top) > 67108864.0f && fabsf(top) < INFINITY) {
+            const float s = __uint_as_float((127u + 25u + 127u) * 0x800000u - (__float_as_uint(top) & 0x7F800000u));
+            top = ceilf(top * s);
+            qs *= s;
+            unit /= s;
+          }
+          m = top;
+          f2 = pair(qs, qs);
           const float o = m == -INFINITY ? 0.0f : (float)kStLift - m;
           off = pair(o, o);
         };
-        base();
+        base(first ? largest(0) : m);
         uint32_t z[2][16];
         tmem_ld16(s_at, z[0]);
 #pragma unroll 1
@@ -320,10 +333,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
               sum = pair(s2.x * f0, s2.y * f0);
               const float fa = ex2(floorf(0.5f * fall)), fb = ex2(fall - floorf(0.5f * fall));
               const __half2 ha = __floats2half2_rn(fa, fa), hb = __floats2half2_rn(fb, fb);
-              if (m != up) {
-                m = up;
-                base();
-              }
+              if (m != up) base(up);
               tmem_st_wait();
 #pragma unroll 1
               for (int c = 0; c < h + g; ++c) {             // what has been written of the tile
@@ -356,7 +366,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
         }
         const float2 s2 = unpair(sum);
         l += s2.x + s2.y;
-        sh.top[i & 3][row] = m;
+        sh.top[i & 3][row] = m * unit;
         tmem_st_wait();
         fence_before();
         bar_arrive(bar(sh.w_ready[w]));
@@ -381,7 +391,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
         mma_commit(bar(sh.drain[w]), leader);
         bar_wait_warp(bar(sh.drain[w]), drains++ & 1, &no);
       }
-      sh.m[w][row] = m;
+      sh.m[w][row] = m * unit;
       sh.l[w][row] = l;
       asm volatile("bar.sync 1, 384;" ::: "memory");       // with the warps that have the sums
       rows_out();
@@ -431,11 +441,11 @@ __global__ void __launch_bounds__(kStThreads, 1)
       float* line = lines + (size_t)row * kStLine;
 #pragma unroll
       for (int d = 0; d < kHd / 2; d += 2) {
-        const float2 x = unpair(acc[d]), y = unpair(acc[d + 1]);
+        const float2 x = unpair(mul2(acc[d], pair(kStDrop, kStDrop))), y = unpair(mul2(acc[d + 1], pair(kStDrop, kStDrop)));
         *reinterpret_cast<float4*>(line + 2 * d) = make_float4(x.x, x.y, y.x, y.y);
       }
       if (st.last && row == 0) p.stretches[st.kvh * wh.rows + st.row0 / kStRows] = st.last;
-      if (st.row0 + row < F) p.ml[st.part_row + row] = make_float2(M - (float)kStLift, L);
+      if (st.row0 + row < F) p.ml[st.part_row + row] = make_float2(M, L * kStDrop);
       rows_out();
     }
   } else {

@@ -327,7 +327,9 @@ int hv_attn_rows_q8(const float* q, const void* kv, float* ctx, const float* sca
  * weights count to 2^-22 of themselves, a query's values at least to 2^-38 of its largest and a
  * row's weights to 2^-31 of theirs; weights under 2^-126 of the largest are 0. Contexts (and
  * weights) of queries that see a position whose K or V holds an infinity or a NaN are not
- * defined; those of others do not depend on it.
+ * defined; those of others do not depend on it. Scores are f32: past its range nothing is defined,
+ * and of a run's rows whose scores pass 2^26 the weights added up are only known to be between
+ * 0 and 1 (their contexts, and one token's weights, have the scores as they are).
  *
  *   hv_attn_shared_f16  attention of a batch of sequences that share a prefix, which is read once
  *     for all of them. The prefix: *plen positions of pk, pv [nkv][pcap][128] (0 to pcap; with
