@@ -325,6 +325,9 @@ __global__ void __launch_bounds__(kStThreads, 1)
             exps();
             const float2 both = unpair(cs);
             if (__builtin_expect(__any_sync(0xFFFFFFFFu, !(both.x + both.y <= 32768.0f)), 0)) {
+              m *= unit;                           // (units are chosen anew)
+              qs *= unit;
+              unit = 1.0f;
               const float up = fmaxf(m, largest(16 * (h + g)));
               const float fall = m == -INFINITY ? 0.0f : fmaxf(m - up, -60.0f);   // 2^-60 of it is as good as 0
               const float f0 = ex2(fall);
@@ -333,7 +336,7 @@ __global__ void __launch_bounds__(kStThreads, 1)
               sum = pair(s2.x * f0, s2.y * f0);
               const float fa = ex2(floorf(0.5f * fall)), fb = ex2(fall - floorf(0.5f * fall));
               const __half2 ha = __floats2half2_rn(fa, fa), hb = __floats2half2_rn(fb, fb);
-              if (m != up) base(up);
+              base(up);
               tmem_st_wait();
 #pragma unroll 1
               for (int c = 0; c < h + g; ++c) {             // what has been written of the tile

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import span_ref as R
-from test_gpu_shared import run_mass, run_shared, SCALE
+from test_gpu_shared import near, run_mass, run_shared, SCALE
 
 pytestmark = pytest.mark.gpu
 F32, F16, HD = np.float32, np.float16, 128
@@ -37,6 +37,28 @@ def test_shared(hv, size, sign, nkv, group, nseq, plen):
         want = pv[:, tops].astype(np.float64).mean(1).repeat(group, 0)
         assert np.abs(got - want).max() <= 64 * R.U
     assert (got >= 1 - 64 * R.U).all() and (got <= 2 + 64 * R.U).all()
+
+
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e7])
+@pytest.mark.parametrize("where", ["first", "middle", "every third"])
+@pytest.mark.parametrize("nkv,group,nseq,plen", [(2, 4, 3, 700), (8, 4, 40, 1500), (4, 8, 200, 3001)])
+def test_scores_far_below_the_others(hv, size, where, nkv, group, nseq, plen):
+    """Positions whose scores lie 2^18 to 2^31 below take nothing from what the others are told
+    apart by: contexts are those of the others alone, at their own bound."""
+    g = np.random.default_rng(plen)
+    t = np.arange(plen)
+    far = {"first": t < 300, "middle": (t > 250) & (t < 600), "every third": t % 3 == 0}[where]
+    step = F16(2.0 ** np.round(np.log2(1 / size)))           # scores of the others are a few units
+    pk = (g.integers(-8, 9, (nkv, plen, HD)) * step).astype(F16)
+    pk[:, far] = -2
+    tk = (g.integers(-8, 9, (nseq, nkv, 20, HD)) * step).astype(F16)
+    pv, tv = (g.standard_normal(x.shape).astype(F16) for x in (pk, tk))
+    q = np.full((nseq, nkv * group, HD), size, F32)
+    tails = [20 - s % 20 for s in range(nseq)]
+    got = run_shared(hv, q, pk, pv, plen, tk, tv, None, tails)
+    some = [0, nseq // 2, nseq - 1]
+    near(got[some], *R.shared(q[some], pk[:, ~far], pv[:, ~far], int((~far).sum()), tk[some], tv[some], None,
+                              [tails[s] for s in some], SCALE))
 
 
 @pytest.mark.parametrize("size", [1e4, 3e6, 3e7, 1e9, 1e12, 1e30])
